@@ -72,6 +72,9 @@ extern "C" {
 #define KNJ_DT_F32 0
 #define KNJ_DT_BF16 1
 #define KNJ_DT_F16 2
+/* 8-bit codes with f32 scales beside them: rows one scale for each 128 values ([rows][ceil(K/128)]), matrices one for each
+ * block of 128 x 128 ([ceil(N/128)][ceil(K/128)]). Where an entry point does not name it, the three above are taken. */
+#define KNJ_DT_E4M3 3
 
 typedef void *knj_stream_t; /* a cudaStream_t */
 typedef void *knj_event_t;  /* a cudaEvent_t */
@@ -464,6 +467,89 @@ int knj_moe_stack_set_wait(knj_moe_stack *st, long long wait_cycles, int stall_f
  * (the scalar kernel waits for no such copy). */
 int knj_moe_stack_test_stall_copy(knj_moe_stack *st, int warp);
 void knj_moe_stack_destroy(knj_moe_stack *st);
+
+/* ======================================================================== */
+/* Experts in bf16, fp16 and e4m3, and what stands between two blocks        */
+/* ======================================================================== */
+/* The reference decodes GGUF's unquantised types on its CPU path only (src/loader/dequant.cpp:1032 fp16_to_fp32, :1068
+ * bf16_to_fp32) and has no device kernel for such experts; e4m3 experts and the gate of a block have no counterpart there. */
+
+/* Rows as e4m3 codes. Per group of 128 values of a row (the last may be shorter), in f32: scale = most * f32(1/448) with
+ * `most` the largest magnitude, code = e4m3(v * (1 / scale)), to nearest, ties to even. A group with most < 2^-100 is
+ * stored as zeros under scale 0; a NaN or an infinity in a group becomes its scale, and products of the row are NaN.
+ * x [rows][K] f32 / bf16 / f16 with row stride ldx; q dense [rows][K]; scale [rows][ceil(K/128)]. */
+int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K, void *q, float *scale, knj_stream_t s);
+
+/* What stands between two blocks of a residual stream, in one launch (rmsnorm_rows and the residual add of
+ * src/model/model.cpp:258-271, :652 are its simplest cases). Per row, in f32:
+ *   n = y * rsqrt(mean(y^2) + eps) * post_w   (post_w NULL: n = y)
+ *   s = beta * x + alpha * g * n              (y NULL: s = beta * x)
+ *   h = s * rsqrt(mean(s^2) + eps) * pre_w    (pre_w and h NULL: not formed)
+ * stream_out receives s (NULL: not stored), h the rows of the next block; h is formed from s before s is rounded to
+ * stream_dtype. The gate g: one value per channel (gate [hidden]), per row (gate[t * ldg]) or per element (row stride
+ * ldg); gate_sigmoid = 1 applies 1 / (1 + exp(-g)) first. h_dtype KNJ_DT_E4M3: codes as knj_fp8_rows_launch forms them,
+ * scales in h_scale. stream_out may be x or y itself (same type and stride), h must not overlap an input. Rows whose
+ * strides and bases are whole 16-byte units, with hidden a multiple of 8, take 16-byte loads and stores. */
+#define KNJ_GATE_NONE 0
+#define KNJ_GATE_CHANNEL 1
+#define KNJ_GATE_ROW 2
+#define KNJ_GATE_FULL 3
+#define KNJ_BLOCK_NORM_MAX_HIDDEN 32768
+typedef struct knj_block_norm_args {
+  int32_t n_tokens, hidden;
+  const void *x; /* [n_tokens][hidden] the residual stream */
+  int64_t ldx;
+  const void *y; /* the block's output, or NULL */
+  int64_t ldy;
+  const void *post_w, *pre_w; /* [hidden] norm weights, or NULL */
+  const void *gate;
+  int64_t ldg;
+  void *stream_out;
+  int64_t ld_stream;
+  void *h;
+  int64_t ldh;
+  float *h_scale;
+  int32_t x_dtype, y_dtype, w_dtype, gate_dtype, stream_dtype, h_dtype;
+  int32_t gate_kind, gate_sigmoid;
+  float alpha, beta, eps;
+} knj_block_norm_args;
+int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s);
+
+/* Products of routed rows with expert matrices, grouped by expert, from one pair per expert to all pairs at one
+ * (tables as knj_moe_permute_launch makes them; an expert without pairs is not read, rows of out that no table entry
+ * names are left as they were):
+ *   knj_expert_gateup_launch: out[p][n] = out_scale * silu(x[row(p)] . w0[e][n]) * (x[row(p)] . w1[e][n])
+ *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
+ * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
+ * p / row_div. e4m3: x_scale [n_rows][ceil(K/128)], w*_scale [n_experts][ceil(N/128)][ceil(K/128)]; the sum over each 128
+ * values of K is scaled and added in f32. N is any number, K and ldx are whole 16-byte units, bases are 16-byte aligned.
+ * out f32, bf16 or f16 [n_pairs][N], row stride ldo. Table entries outside [0, n_pairs) are skipped, rows outside
+ * [0, n_rows) read as zeros. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
+ * the outputs it concerns are then NaN. */
+typedef struct knj_expert_gemm_args {
+  const void *x;
+  const float *x_scale;
+  int64_t ldx;
+  const void *w0, *w1;
+  const float *w0_scale, *w1_scale;
+  const int32_t *pair_idx, *pair_cnt, *row_map;
+  int64_t idx_stride;
+  void *out;
+  int64_t ldo;
+  int32_t *status;
+  int32_t n_rows, n_pairs, N, K, n_experts, row_div;
+  int32_t x_dtype, w_dtype, out_dtype;
+  float out_scale;
+} knj_expert_gemm_args;
+int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
+int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
+
+/* Dense product with an e4m3 matrix: y[m][n_out] = x[m][n_in] . W^T, W e4m3 [n_out][n_in] with W_scale
+ * [ceil(n_out/128)][ceil(n_in/128)]; the rows of x (f32, bf16 or f16) are turned into e4m3 codes first, as
+ * knj_fp8_rows_launch does, in the workspace (256-byte aligned). n_in a multiple of 16. y f32, bf16 or f16. */
+size_t knj_fp8_matmul_workspace_bytes(int m, int n_in);
+int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, int64_t ldx, int m, void *y,
+                          int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);
 
 /* ======================================================================== */
 /* Device-clock spans for a host profiler                                   */

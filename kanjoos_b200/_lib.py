@@ -13,7 +13,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 # KNJ_DEVICE_LIB points at another build of the same library (e.g. a measurement build); default: the in-tree one
 LIB_PATH = os.environ.get("KNJ_DEVICE_LIB") or os.path.join(PKG, "libknj_device.so")
 
-DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16, DT_E4M3 = 0, 1, 2, 3
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3  # KNJ_GATE_*
 EP_FLAG_WORDS, EP_MAX_CHUNKS = 4096, 8  # KNJ_EP_FLAG_WORDS, KNJ_EP_MAX_CHUNKS
 
 
@@ -41,6 +42,23 @@ class MoeFfnArgs(C.Structure):
                 ("workspace_bytes", C.c_size_t), ("tap_pair_exp", C.c_void_p), ("tap_pair_w", C.c_void_p),
                 ("down_format", C.c_int32), ("fused_combine", C.c_int32)]
 
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("n_tokens", C.c_int32), ("hidden", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("post_w", C.c_void_p), ("pre_w", C.c_void_p), ("gate", C.c_void_p), ("ldg", C.c_int64),
+                ("stream_out", C.c_void_p), ("ld_stream", C.c_int64), ("h", C.c_void_p), ("ldh", C.c_int64),
+                ("h_scale", C.c_void_p), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("w_dtype", C.c_int32),
+                ("gate_dtype", C.c_int32), ("stream_dtype", C.c_int32), ("h_dtype", C.c_int32), ("gate_kind", C.c_int32),
+                ("gate_sigmoid", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float)]
+
+
+class ExpertGemmArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scale", C.c_void_p), ("ldx", C.c_int64), ("w0", C.c_void_p), ("w1", C.c_void_p),
+                ("w0_scale", C.c_void_p), ("w1_scale", C.c_void_p), ("pair_idx", C.c_void_p), ("pair_cnt", C.c_void_p),
+                ("row_map", C.c_void_p), ("idx_stride", C.c_int64), ("out", C.c_void_p), ("ldo", C.c_int64),
+                ("status", C.c_void_p), ("n_rows", C.c_int32), ("n_pairs", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("n_experts", C.c_int32), ("row_div", C.c_int32), ("x_dtype", C.c_int32), ("w_dtype", C.c_int32),
+                ("out_dtype", C.c_int32), ("out_scale", C.c_float)]
 
 
 class EpDescC(C.Structure):
@@ -176,6 +194,12 @@ SIGNATURES = {
     "knj_q4k_matmul_launch": (_i, [_vp, _i, _i, _vp, _i, _i64, _i, _vp, _i64, _vp, _sz, _vp]),
     "knj_q4k_matmul_noalloc_max_scratch": (_sz, []),
     "knj_q4k_matmul_noalloc_launch": (_i, [_vp, _i, _i, _vp, _i, _i64, _i, _vp, _i64, _vp]),
+    "knj_fp8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
+    "knj_block_norm_launch": (_i, [C.POINTER(BlockNormArgs), _vp]),
+    "knj_expert_gateup_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
+    "knj_expert_proj_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
+    "knj_fp8_matmul_workspace_bytes": (_sz, [_i, _i]),
+    "knj_fp8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),
     "knj_moe_ffn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "knj_moe_ffn_decode_launch": (_i, [C.POINTER(MoeFfnArgs), _vp]),
     "knj_moe_ffn_prefill_launch": (_i, [C.POINTER(MoeFfnArgs), _vp]),

@@ -9,9 +9,12 @@ import functools
 import torch
 
 from . import _lib
-from ._lib import DT_BF16, DT_F16, DT_F32, check, lib
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, check,
+                   lib)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+_E4M3 = torch.float8_e4m3fn
+_DT_ALL = {**_DT, _E4M3: DT_E4M3}
 
 
 def _p(t: torch.Tensor | None):
@@ -261,3 +264,168 @@ def q4k_down_tc(ah, Wd, pair_idx, pair_cnt, P: int, pair_row=None, poison: bool 
     check(lib().knj_q4k_down_tc_launch(_p(ah), _p(Wd), _p(pair_idx), _p(pair_cnt), _p(pair_row), _p(Y), N, nsb * 256,
                                        nsb * 144, pair_idx.shape[1], E, P, _p(status), _stream()))
     return Y, status
+
+
+# ---- experts in bf16, fp16 and e4m3, and what stands between two blocks -------------------------------------------
+
+def _rows(t: torch.Tensor, what: str, dtypes, shape=None) -> int:
+    """Checks a matrix of rows (dense inside a row, any row stride) on the current device; its row stride in elements."""
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{what} lives on {t.device}, not on the current CUDA device")
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}" + (f", expected {tuple(shape)}" if shape is not None else ", expected rows"))
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} is {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
+    n, k = t.shape
+    if k > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what} has rows that are not dense")
+    ld = t.stride(0) if n > 1 else k
+    if ld < k:
+        raise ValueError(f"{what} has overlapping rows (stride {ld} for {k} values)")
+    return ld
+
+
+def _dense(t: torch.Tensor, what: str, dtypes, shape) -> int:
+    """Checks a contiguous tensor of this shape on the current device; its address."""
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{what} lives on {t.device}, not on the current CUDA device")
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.dtype not in dtypes:
+        raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)}, expected contiguous {' / '.join(str(d) for d in dtypes)} {tuple(shape)}")
+    return t.data_ptr()
+
+
+def fp8_rows(x: torch.Tensor):
+    """x [rows][K] (f32 / bf16 / f16) -> (codes float8_e4m3fn [rows][K], scale f32 [rows][ceil(K/128)])."""
+    ld = _rows(x, "x", _DT)
+    n, k = x.shape
+    q = torch.empty((n, k), dtype=_E4M3, device=x.device)
+    scale = torch.empty((n, -(-k // 128)), dtype=torch.float32, device=x.device)
+    check(lib().knj_fp8_rows_launch(x.data_ptr(), _DT[x.dtype], ld, n, k, q.data_ptr(), scale.data_ptr(), _raw_stream()))
+    return q, scale
+
+
+def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
+    """W float8_e4m3fn [n_out][n_in] with W_scale f32 [ceil(n_out/128)][ceil(n_in/128)], x [m][n_in] (f32 / bf16 / f16, turned
+    into e4m3 rows as fp8_rows does) -> [m][n_out] in out_dtype."""
+    ld = _rows(x, "x", _DT)
+    m, k = x.shape
+    if W.dim() != 2 or out_dtype not in _DT:
+        raise ValueError(f"W has shape {tuple(W.shape)}, out_dtype is {out_dtype}")
+    n = W.shape[0]
+    w = _dense(W, "W", (_E4M3,), (n, k))
+    ws = _dense(W_scale, "W_scale", (torch.float32,), (-(-n // 128), -(-k // 128)))
+    y = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    L = lib()
+    nbytes = L.knj_fp8_matmul_workspace_bytes(m, k)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    check(L.knj_fp8_matmul_launch(w, ws, k, n, x.data_ptr(), _DT[x.dtype], ld, m, y.data_ptr(), _DT[out_dtype], n, work.data_ptr(), nbytes, None,
+                                  _raw_stream()))
+    return y
+
+
+def _expert_args(x, x_scale, mats, scales, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale):
+    w = mats[0]
+    if w.dim() != 3 or w.dtype not in (torch.bfloat16, torch.float16, _E4M3):
+        raise ValueError(f"expert matrices are bf16, f16 or float8_e4m3fn [E][N][K], got {w.dtype} {tuple(w.shape)}")
+    E, N, K = w.shape
+    ptrs = [_dense(m, "an expert matrix", (w.dtype,), (E, N, K)) for m in mats] + [None]
+    sc = [None, None]
+    if w.dtype == _E4M3:
+        if any(s is None for s in scales):
+            raise ValueError("e4m3 expert matrices need their scales")
+        sc = [_dense(s, "a matrix's scales", (torch.float32,), (E, -(-N // 128), -(-K // 128))) for s in scales] + [None]
+        if x.dtype != _E4M3:
+            x, x_scale = fp8_rows(x)
+        elif x_scale is None:
+            raise ValueError("e4m3 rows need x_scale")
+    elif any(s is not None for s in scales) or x_scale is not None:
+        raise ValueError("scales belong to e4m3 matrices and rows")
+    ld = _rows(x, "x", (w.dtype,))
+    n_rows = x.shape[0]
+    if x.shape[1] != K:
+        raise ValueError(f"x has rows of {x.shape[1]} values, the matrices of {K}")
+    xs = None if x_scale is None else _dense(x_scale, "x_scale", (torch.float32,), (n_rows, -(-K // 128)))
+    stride = pair_idx.shape[1] if pair_idx.dim() == 2 else -1
+    idx = _dense(pair_idx, "pair_idx", (torch.int32,), (E, stride))
+    cnt = _dense(pair_cnt, "pair_cnt", (torch.int32,), (E,))
+    rmap = None if row_map is None else _dense(row_map, "the row map", (torch.int32,), (P,))
+    if out is None:
+        out = torch.empty((P, N), dtype=out_dtype, device=x.device)
+    ldo = _rows(out, "out", _DT, (P, N))
+    a = ExpertGemmArgs(x.data_ptr(), xs, ld, ptrs[0], ptrs[1], sc[0], sc[1], idx, cnt, rmap, stride, out.data_ptr(), ldo, None, n_rows, P, N, K, E,
+                       row_div, _DT_ALL[x.dtype], _DT_ALL[w.dtype], _DT[out.dtype], out_scale)
+    return a, out, x, x_scale
+
+
+def expert_gateup(x, Wg, Wu, pair_idx, pair_cnt, P: int, top_k: int, pair_tok=None, gate_scale=None, up_scale=None, x_scale=None,
+                  out_dtype=None, out=None, out_scale: float = 1.0):
+    """silu(x . Wg[e]) * (x . Wu[e]) * out_scale for every routed pair: [P][N] in out_dtype (default: the matrices' type, bf16
+    for e4m3 ones). Wg, Wu [E][N][K] bf16 / f16 (x in the same type) or float8_e4m3fn with gate_scale and up_scale f32
+    [E][ceil(N/128)][ceil(K/128)] (x e4m3 with x_scale, or f32 / bf16 / f16, which fp8_rows turns into e4m3 rows). x [T][K];
+    pair p reads row pair_tok[p], or p // top_k. Rows of pairs that no table entry names are left as they were."""
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if Wg.dtype == _E4M3 else Wg.dtype
+    a, out, *keep = _expert_args(x, x_scale, (Wg, Wu), (gate_scale, up_scale), pair_idx, pair_cnt, P, pair_tok, top_k, out, out_dtype, out_scale)
+    check(lib().knj_expert_gateup_launch(C.byref(a), _raw_stream()))
+    return out
+
+
+def expert_proj(a, W, pair_idx, pair_cnt, P: int, pair_row=None, scale=None, a_scale=None, out_dtype=torch.float32, out=None,
+                out_scale: float = 1.0):
+    """a . W[e] * out_scale for every routed pair: [P][N] in out_dtype. a holds one row per pair (row pair_row[p] when given,
+    else p); types, scales and unnamed rows as for expert_gateup."""
+    args, out, *keep = _expert_args(a, a_scale, (W,), (scale,), pair_idx, pair_cnt, P, pair_row, 1, out, out_dtype, out_scale)
+    check(lib().knj_expert_proj_launch(C.byref(args), _raw_stream()))
+    return out
+
+
+def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False, alpha: float = 1.0, beta: float = 1.0, pre_w=None,
+               eps: float = 1e-6, stream_dtype=None, norm_dtype=torch.bfloat16, stream_out=None):
+    """What stands between two blocks: s = beta * x + alpha * gate * norm(y; post_w), h = norm(s; pre_w).
+    x [T][H] the residual stream, y [T][H] the block's output or None, post_w / pre_w [H] norm weights or None (one type),
+    gate [H], [T][1] or [T][H] (through a sigmoid with gate_sigmoid). Returns (s, h): s in stream_dtype (default: x's type;
+    None without y unless stream_out or stream_dtype asks for it), h in norm_dtype (None without pre_w), for
+    torch.float8_e4m3fn as (codes, scale). stream_out may be x or y."""
+    ldx = _rows(x, "x", _DT)
+    T, H = x.shape
+    a = BlockNormArgs(n_tokens=T, hidden=H, x=x.data_ptr(), ldx=ldx, x_dtype=_DT[x.dtype], alpha=alpha, beta=beta, eps=eps,
+                      gate_sigmoid=1 if gate_sigmoid else 0)
+    if y is not None:
+        a.ldy, a.y, a.y_dtype = _rows(y, "y", _DT, (T, H)), y.data_ptr(), _DT[y.dtype]
+    for w in (post_w, pre_w):
+        if w is not None:
+            ptr = _dense(w, "a norm weight", _DT, (H,))
+            if post_w is not None and pre_w is not None and post_w.dtype != pre_w.dtype:
+                raise ValueError("post_w and pre_w are of one type")
+            a.w_dtype = _DT[w.dtype]
+            if w is post_w:
+                a.post_w = ptr
+            if w is pre_w:
+                a.pre_w = ptr
+    if gate is not None:
+        if gate.dim() == 1:
+            _dense(gate, "gate", _DT, (H,))
+            a.gate_kind = GATE_CHANNEL
+        elif gate.dim() == 2 and gate.shape[1] == 1 and H > 1:
+            a.ldg = max(1, _rows(gate, "gate", _DT, (T, 1)))
+            a.gate_kind = GATE_ROW
+        else:
+            a.ldg = _rows(gate, "gate", _DT, (T, H))
+            a.gate_kind = GATE_FULL
+        a.gate, a.gate_dtype = gate.data_ptr(), _DT[gate.dtype]
+    s = stream_out
+    if s is None and (y is not None or stream_dtype is not None):
+        s = torch.empty((T, H), dtype=stream_dtype or x.dtype, device=x.device)
+    if s is not None:
+        a.ld_stream, a.stream_out, a.stream_dtype = _rows(s, "the stream", _DT, (T, H)), s.data_ptr(), _DT[s.dtype]
+    h = scale = None
+    if pre_w is not None:
+        if norm_dtype not in _DT_ALL:
+            raise ValueError(f"norm_dtype is {norm_dtype}")
+        h = torch.empty((T, H), dtype=norm_dtype, device=x.device)
+        a.h, a.ldh, a.h_dtype = h.data_ptr(), H, _DT_ALL[norm_dtype]
+        if norm_dtype == _E4M3:
+            scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
+            a.h_scale = scale.data_ptr()
+    check(lib().knj_block_norm_launch(C.byref(a), _raw_stream()))
+    return s, (h if scale is None else (h, scale))

@@ -1,0 +1,315 @@
+"""The operators around an MoE block -- fp8 rows, block norm, expert products in 16 and 8 bits, the dense e4m3 product --
+against their definitions in 64 bits, value by value, under bounds derived from the roundings and the f32 sums."""
+import pytest
+import torch
+
+import block_ops_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def gen(*key):
+    g = torch.Generator()
+    g.manual_seed(sum((i + 1) * 7919 * ord(c) for i, c in enumerate(str(key))))
+    return g
+
+
+def strided(t, pad):
+    """The same rows inside a wider tensor."""
+    wide = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), dtype=t.dtype, device=t.device)
+    wide[:, :t.shape[1]] = t
+    return wide[:, :t.shape[1]]
+
+
+# ------------------------------------------------------------------------------------------------------- fp8 rows
+
+@pytest.mark.parametrize("rows,K,dtype,pad", [(1, 1, F32, 0), (1, 128, BF16, 0), (3, 2048, BF16, 0), (5, 130, F16, 0), (7, 127, F32, 3),
+                                              (301, 1000, BF16, 8), (2, 4096, F32, 4), (33, 264, F16, 1)])
+def test_fp8_rows_are_the_definitions_bits(rows, K, dtype, pad):
+    from kanjoos_b200 import ops
+    x = (torch.randn((rows, K), generator=gen(rows, K)) * torch.exp(torch.randn((rows, 1), generator=gen(K)) * 3)).to(dtype)
+    want, want_s = ref.fp8_rows(x)
+    xd = x.cuda()
+    q, s = ops.fp8_rows(strided(xd, pad) if pad else xd)
+    assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8)) and torch.equal(s.cpu(), want_s)
+
+
+def test_fp8_rows_special_groups():
+    from kanjoos_b200 import ops
+    x = torch.randn((6, 384), generator=gen("special"))
+    x[0] = 0.0
+    x[1, :128] = 2.0 ** -101           # below the smallest group that keeps a scale
+    x[1, 128:256] = 2.0 ** -100
+    x[2, 5] = float("inf")
+    x[3, 200] = float("nan")
+    x[4, 383] = 3e38
+    x[5] *= 1e-30
+    q, s = ops.fp8_rows(x.cuda())
+    q, s = q.cpu(), s.cpu()
+    want, want_s = ref.fp8_rows(x)
+    fine = torch.isfinite(want_s)
+    assert torch.equal(s[fine], want_s[fine])
+    keep = fine.repeat_interleave(128, 1)
+    assert torch.equal(q.view(torch.uint8)[keep], want.view(torch.uint8)[keep])
+    assert (q[0].float() == 0).all() and (s[0] == 0).all() and s[1, 0] == 0 and s[1, 1] > 0
+    assert torch.isinf(s[2, 0]) and torch.isnan(s[3, 1])
+    assert torch.isnan(q[3, 128:256].float()).all()
+
+
+# ------------------------------------------------------------------------------------------------------ block norm
+
+NORMS = [
+    # T, H, stream, y, weights, gate, sigmoid, post, pre, h
+    (1, 2048, BF16, F32, BF16, None, False, True, True, BF16),
+    (3, 2048, F32, BF16, BF16, "channel", True, True, True, E4M3),
+    (5, 1000, F32, BF16, F32, "row", True, True, True, F16),
+    (2, 1001, BF16, F16, F16, "full", False, True, True, F32),       # odd width: no 16-byte rows
+    (4, 136, F16, F32, BF16, "full", True, False, True, E4M3),       # a last group of eight values
+    (7, 257, F32, F32, F32, "row", False, False, False, None),
+    (2, 8, BF16, None, BF16, None, False, False, True, BF16),
+    (1, 1, F32, BF16, BF16, "channel", False, True, True, F32),
+    (67, 4096, BF16, BF16, BF16, "row", False, True, True, E4M3),
+    (2, 16384, BF16, BF16, BF16, "channel", True, True, True, BF16),
+    (2, 32768, F32, F32, BF16, None, False, True, True, E4M3),
+    (1, 32001, BF16, F32, BF16, None, False, True, True, F16),
+    (600, 512, BF16, F32, BF16, None, False, False, False, None),
+]
+
+
+@pytest.mark.parametrize("T,H,st,yt,wt,gate,sig,post,pre,ht", NORMS)
+@pytest.mark.parametrize("pad", [0, 8])
+def test_block_norm(T, H, st, yt, wt, gate, sig, post, pre, ht, pad):
+    from kanjoos_b200 import ops
+    g = gen(T, H, gate)
+    x = torch.randn((T, H), generator=g).to(st)
+    y = None if yt is None else (2 * torch.randn((T, H), generator=g)).to(yt)
+    pw, nw = ((1 + 0.3 * torch.randn(H, generator=g)).to(wt) if on else None for on in (post, pre))
+    gt = None if gate is None else torch.randn({"channel": (H,), "row": (T, 1), "full": (T, H)}[gate], generator=g).to(BF16)
+    alpha, beta, eps = 0.7, 1.25, 1e-6
+    s, es, h, eh = ref.block_norm(x, y, pw, gt, sig, alpha, beta, nw, eps)
+
+    def dev(t):
+        return None if t is None else strided(t.cuda(), pad) if pad and t.dim() == 2 and t.shape[1] == H else t.cuda()
+    got_s, got_h = ops.block_norm(dev(x), dev(y), post_w=dev(pw), gate=dev(gt), gate_sigmoid=sig, alpha=alpha, beta=beta, pre_w=dev(nw), eps=eps,
+                                  norm_dtype=ht or BF16)
+    if y is None:
+        assert got_s is None
+    else:
+        assert got_s.dtype == st
+        ref.check(got_s, s, es + ref.held(s, st), "stream")
+    if not pre:
+        assert got_h is None
+    elif ht == E4M3:
+        codes, scale = got_h
+        most = torch.nn.functional.pad(h.abs(), (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
+        slack = torch.nn.functional.pad(eh, (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
+        ref.check(scale, most / 448, slack / 448 + 3 * 2.0 ** -24 * most / 448, "scales")
+        sc = scale.double().cpu().repeat_interleave(128, 1)[:, :H]
+        # half a step of e4m3: 2^-4 relative, 2^-10 of the scale below the normal range
+        ref.check(ref.rows_value(codes.cpu(), scale.cpu()), h, eh + 2.0 ** -4 * (h.abs() + eh) * (1 + 2.0 ** -20) + 2.0 ** -10 * sc, "codes")
+    else:
+        assert got_h.dtype == ht
+        ref.check(got_h, h, eh + ref.held(h, ht), "normalised rows")
+
+
+def test_block_norm_in_place_and_plain_stream():
+    from kanjoos_b200 import ops
+    g = gen("inplace")
+    for H in (1024, 1001):
+        x, y = torch.randn((9, H), generator=g).to(BF16).cuda(), torch.randn((9, H), generator=g).to(BF16).cuda()
+        w = torch.ones(H, dtype=BF16, device="cuda")
+        want_s, want_h = ops.block_norm(x, y, pre_w=w)
+        a, b = x.clone(), y.clone()
+        s, h = ops.block_norm(a, b, pre_w=w, stream_out=a)
+        assert s.data_ptr() == a.data_ptr() and torch.equal(a, want_s) and torch.equal(h, want_h) and torch.equal(b, y)
+        b2 = y.clone()
+        ops.block_norm(x, b2, pre_w=w, stream_out=b2)
+        assert torch.equal(b2, want_s)
+        scaled, none = ops.block_norm(x, beta=0.5, stream_dtype=F32)
+        assert none is None and torch.equal(scaled, x.float() * 0.5)
+
+
+def test_block_norm_special_rows():
+    """Rows of zeros, a NaN in one row and a huge row: each row stands for itself."""
+    from kanjoos_b200 import ops
+    H = 512
+    x = torch.randn((5, H), generator=gen("rows"))
+    x[0] = 0
+    x[1, 7] = float("nan")
+    x[2] *= 1e18
+    w = torch.ones(H)
+    s, h = ops.block_norm(x.cuda(), torch.zeros((5, H)).cuda(), pre_w=w.cuda(), norm_dtype=F32)
+    h = h.cpu()
+    assert (h[0] == 0).all() and torch.isnan(h[1]).all()
+    rs, es, rh, eh = ref.block_norm(x[2:], None, None, None, False, 1.0, 1.0, w, 1e-6)
+    ref.check(h[2:], rh, eh + ref.held(rh, F32), "rows beside a NaN")
+
+
+# --------------------------------------------------------------------------------------------------- expert products
+
+EXPERTS = [
+    # E, N, K (16 bits: multiples of 8; 8 bits: of 16), counts
+    (1, 128, 64, [1]),
+    (4, 256, 256, [5, 0, 1, 40]),
+    (3, 256, 512, [16, 300, 0]),
+    (2, 768, 2048, [33, 7]),
+    (2, 100, 144, [130, 9]),          # rows behind the last whole tile, a last K step that is not full
+    (2, 257, 400, [256, 255]),
+    (3, 72, 1040, [0, 0, 2]),
+    (5, 384, 640, [1, 1, 1, 1, 1]),
+    (8, 512, 1024, [3, 70, 129, 64, 65, 17, 16, 15]),
+    (256, 32, 32, [1] * 100 + [0] * 100 + [2] * 56),
+    (2, 128, 16, [600, 1]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, E4M3])
+@pytest.mark.parametrize("E,N,K,counts", EXPERTS)
+@pytest.mark.parametrize("kind", ["gateup", "proj"])
+def test_expert_products(kind, E, N, K, counts, dtype):
+    run_expert(kind, E, N, K, counts, dtype, {"gateup": BF16, "proj": F32}[kind])
+
+
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+@pytest.mark.parametrize("kind,dtype", [("gateup", F16), ("gateup", E4M3), ("proj", BF16), ("proj", E4M3)])
+def test_expert_output_types(kind, dtype, out):
+    run_expert(kind, 3, 264, 288, [70, 0, 9], dtype, out)
+
+
+def run_expert(kind, E, N, K, counts, dtype, out_t):
+    from kanjoos_b200 import ops
+    g = gen(kind, E, N, K, dtype)
+    P = sum(counts)
+    idx, cnt = ref.tables(counts, g, stride=max(counts) + 3)
+    mats = [ref.matrix((E, N, K), g, dtype) for _ in range(2 if kind == "gateup" else 1)]
+    top_k = 3
+    rows = -(-P // top_k) if kind == "gateup" else P
+    x = torch.randn((rows, K), generator=g).to(dtype if dtype != E4M3 else BF16)
+    xv = ref.rows_value(*ref.fp8_rows(x)) if dtype == E4M3 else x.double()
+    mv = [ref.matrix_value(*m) for m in mats]
+    sc = [None if m[1] is None else m[1].cuda() for m in mats]
+    md = [m[0].cuda() for m in mats]
+    out = torch.full((P + 2, N + 5), -12345.0, dtype=out_t, device="cuda")
+    part = out[:P, :N]
+    if kind == "gateup":
+        want, err, wrote = ref.gateup(xv, mv[0], mv[1], idx, cnt, lambda p: p // top_k, P)
+        got = ops.expert_gateup(x.cuda(), md[0], md[1], idx.cuda(), cnt.cuda(), P, top_k, gate_scale=sc[0], up_scale=sc[1], out=part)
+    else:
+        want, err, wrote = ref.proj(xv, mv[0], idx, cnt, lambda p: p, P)
+        got = ops.expert_proj(x.cuda(), md[0], idx.cuda(), cnt.cuda(), P, scale=sc[0], out=part)
+    assert got is part and wrote.all()
+    ref.check(part, want, err + ref.held(want.abs() + err, out_t), kind)
+    out = out.cpu()
+    assert (out[P:] == -12345.0).all() and (out[:, N:] == -12345.0).all(), "something outside the output was written"
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_unnamed_rows_bad_entries_and_row_maps(dtype):
+    """Rows that no table entry names stay as they were, entries outside the pairs are skipped, a row outside x reads as
+    zeros, a count above the table's stride is the stride; strided rows with NaN between them."""
+    from kanjoos_b200 import ops
+    g = gen("unnamed", dtype)
+    E, N, K, P = 3, 136, 272, 40
+    w, sc = ref.matrix((E, N, K), g, dtype)
+    x = torch.randn((12, K), generator=g).to(BF16)
+    xv = ref.rows_value(*ref.fp8_rows(x)) if dtype == E4M3 else x.double()
+    idx = torch.tensor([[0, 7, 7, -1], [3, P, 1 << 30, -5], [11, 12, 13, 39]], dtype=torch.int32)
+    cnt = torch.tensor([3, 4, 9], dtype=torch.int32)
+    row_map = torch.randint(0, 12, (P,), generator=g, dtype=torch.int32)
+    row_map[12], row_map[13] = 12, -1                      # outside x
+    out = torch.full((P, N), 7.0, dtype=F32, device="cuda")
+    if dtype == E4M3:
+        q, s = ops.fp8_rows(x.cuda())
+        q8 = torch.full((12, K + 16), 0x7F, dtype=torch.uint8, device="cuda")
+        q8[:, :K] = q.view(torch.uint8)
+        ops.expert_proj(q8.view(E4M3)[:, :K], w.cuda(), idx.cuda(), cnt.cuda(), P, pair_row=row_map.cuda(), scale=sc.cuda(), a_scale=s, out=out)
+    else:
+        ops.expert_proj(strided(x.cuda(), 8), w.cuda(), idx.cuda(), cnt.cuda(), P, pair_row=row_map.cuda(), out=out)
+    out = out.cpu()
+    wv = ref.matrix_value(w, sc)
+    named = {0: 0, 7: 0, 3: 1, 11: 2, 12: 2, 13: 2, 39: 2}
+    for p in range(P):
+        if p not in named:
+            assert (out[p] == 7.0).all(), p
+        elif p in (12, 13):
+            assert (out[p] == 0).all(), p
+        else:
+            want, err = ref.product(xv[row_map[p]][None], wv[named[p]])
+            ref.check(out[p][None], want, err + ref.held(want.abs() + err, F32), f"pair {p}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_no_pairs_at_all(dtype):
+    from kanjoos_b200 import ops
+    g = gen("empty")
+    w, sc = ref.matrix((4, 128, 128), g, dtype)
+    w = w.cuda()
+    sc = None if sc is None else sc.cuda()
+    idx, cnt = torch.full((4, 6), -1, dtype=torch.int32).cuda(), torch.zeros(4, dtype=torch.int32).cuda()
+    out = torch.full((6, 128), 3.0, dtype=F32, device="cuda")
+    x = torch.randn((6, 128), generator=g).to(BF16).cuda()
+    ops.expert_proj(x, w, idx, cnt, 6, scale=sc, out=out)
+    assert (out == 3.0).all()
+    assert ops.expert_proj(x[:0], w, idx, cnt, 0, scale=sc).shape == (0, 128)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_non_finite_values_stay_in_their_rows(dtype):
+    from kanjoos_b200 import ops
+    g = gen("nan", dtype)
+    E, N, K = 2, 256, 384
+    w, sc = ref.matrix((E, N, K), g, dtype)
+    w2 = w.clone()
+    w2[1, 5, 300] = float("nan")
+    x = torch.randn((20, K), generator=g).to(BF16)
+    x[3, 17] = float("nan")
+    x[4, 383] = float("inf")
+    idx, cnt = ref.tables([9, 11], g)
+    s = None if sc is None else sc.cuda()
+    got = ops.expert_proj(x.cuda(), w2.cuda(), idx.cuda(), cnt.cuda(), 20, scale=s).cpu()
+    clean = x.clone()
+    clean[3], clean[4] = 0, 0
+    base = ops.expert_proj(clean.cuda(), w.cuda(), idx.cuda(), cnt.cuda(), 20, scale=s).cpu()
+    of = {int(p): e for e in range(2) for p in idx[e] if p >= 0}
+    for p in range(20):
+        row = got[p].clone()
+        if p == 3:
+            assert torch.isnan(row).all()
+            continue
+        if p == 4:
+            assert not torch.isfinite(row).any()
+            continue
+        if of[p] == 1:
+            assert torch.isnan(row[5])
+            row[5] = base[p, 5]
+        assert torch.equal(row, base[p]), p
+
+
+# ------------------------------------------------------------------------------------------------- dense e4m3 product
+
+@pytest.mark.parametrize("m,n,k,dtype,out,pad", [(1, 2048, 2048, BF16, F32, 0), (1, 1, 16, F32, F32, 0), (2, 100, 144, F16, BF16, 0),
+                                                 (17, 128, 128, BF16, F16, 8), (64, 1000, 2064, F32, F32, 4), (65, 257, 400, BF16, BF16, 0),
+                                                 (301, 1000, 2048, BF16, BF16, 0), (513, 384, 256, F16, F32, 0), (3, 4096, 4096, BF16, F32, 0)])
+def test_fp8_matmul(m, n, k, dtype, out, pad):
+    from kanjoos_b200 import ops
+    g = gen(m, n, k)
+    w, sc = ref.matrix((n, k), g, E4M3)
+    x = torch.randn((m, k), generator=g).to(dtype)
+    want, err = ref.product(ref.rows_value(*ref.fp8_rows(x)), ref.matrix_value(w, sc))
+    xd = x.cuda()
+    got = ops.fp8_matmul(w.cuda(), sc.cuda(), strided(xd, pad) if pad else xd, out_dtype=out)
+    assert got.dtype == out
+    ref.check(got, want, err + ref.held(want.abs() + err, out), "product")
+
+
+def test_results_do_not_depend_on_the_run():
+    from kanjoos_b200 import ops
+    g = gen("again")
+    w, sc = ref.matrix((300, 2048), g, E4M3)
+    w, sc = w.cuda(), sc.cuda()
+    x = torch.randn((7, 2048), generator=g).to(BF16).cuda()
+    first = ops.fp8_matmul(w, sc, x)
+    for _ in range(20):
+        assert torch.equal(first, ops.fp8_matmul(w, sc, x))
