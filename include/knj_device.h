@@ -522,7 +522,7 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s);
  *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
  * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
  * p / row_div. e4m3: x_scale [n_rows][ceil(K/128)], w*_scale [n_experts][ceil(N/128)][ceil(K/128)]; the sum over each 128
- * values of K is scaled and added in f32. N is any number, K and ldx are whole 16-byte units, bases are 16-byte aligned.
+ * values of K is scaled and added in f32. N is any number, n_rows >= 1, K and ldx are whole 16-byte units, bases are 16-byte aligned.
  * out f32, bf16 or f16 [n_pairs][N], row stride ldo. Table entries outside [0, n_pairs) are skipped, rows outside
  * [0, n_rows) read as zeros. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
  * the outputs it concerns are then NaN. */
@@ -543,6 +543,9 @@ typedef struct knj_expert_gemm_args {
 } knj_expert_gemm_args;
 int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
+/* 1 = these products (and the dense e4m3 one) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
+ * always on CTA pairs (buckets of up to 256), 0 (default) = by the number of pairs per expert. Process-wide. */
+void knj_expert_tc_form(int form);
 
 /* Dense product with an e4m3 matrix: y[m][n_out] = x[m][n_in] . W^T, W e4m3 [n_out][n_in] with W_scale
  * [ceil(n_out/128)][ceil(n_in/128)]; the rows of x (f32, bf16 or f16) are turned into e4m3 codes first, as

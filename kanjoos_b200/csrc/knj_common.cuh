@@ -93,6 +93,11 @@ int make_row_tensor_map(CUtensorMap *map, const void *base, uint64_t rows, uint3
 // base 16-byte aligned): one copy moves four rows of 64 elements into 512 bytes of a 128-byte-swizzled tile.
 int make_gather_tensor_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t row_bytes);
 
+// TMA descriptor over rows of `cols` one- or two-byte elements (row stride `ld` elements, 16-byte units, base 16-byte
+// aligned): one copy moves a box of box_rows rows x 128 bytes into a 128-byte-swizzled tile; what lies outside reads as
+// zero. With box_rows = 1 the map serves tile::gather4 copies.
+int make_operand_tensor_map(CUtensorMap *map, const void *base, int elem_bytes, uint64_t cols, uint64_t ld, uint64_t rows, uint32_t box_rows);
+
 // Limit (SM clock cycles) of the bounded waits of the decode-class kernels, as set by knj_decode_wait_limit.
 long long decode_wait_cycles();
 

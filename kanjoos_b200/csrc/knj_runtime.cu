@@ -75,6 +75,25 @@ int make_gather_tensor_map(CUtensorMap *map, const void *base, uint64_t rows, ui
   return KNJ_OK;
 }
 
+int make_operand_tensor_map(CUtensorMap *map, const void *base, int elem_bytes, uint64_t cols, uint64_t ld, uint64_t rows, uint32_t box_rows) {
+  const EncodeFn encode = tensor_map_encoder();
+  if (!encode) return KNJ_E_RUNTIME;
+  KNJ_REQUIRE(ld * elem_bytes % 16 == 0 && ld >= cols && rows >= 1 && box_rows >= 1 && box_rows <= 256 && aligned16(base),
+              "tensor map: rows of %llu values with stride %llu are not TMA-addressable", (unsigned long long)cols, (unsigned long long)ld);
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {ld * elem_bytes};
+  const cuuint32_t box[2] = {128u / elem_bytes, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims,
+                      strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with driver status %d", (int)r);
+    return KNJ_E_RUNTIME;
+  }
+  return KNJ_OK;
+}
+
 int make_row_tensor_map(CUtensorMap *map, const void *base, uint64_t rows, uint32_t row_bytes, uint32_t box_bytes,
                         uint32_t box_rows) {
   const EncodeFn encode = tensor_map_encoder();

@@ -76,7 +76,7 @@ E8 = dict(x_dtype=3, w_dtype=3, x_scale=A, w0_scale=A, w1_scale=A)
 
 @pytest.mark.parametrize("change,word", [
     (dict(N=0), "sizes"), (dict(K=0), "sizes"), (dict(n_experts=0), "sizes"), (dict(n_experts=257), "sizes"), (dict(n_pairs=-1), "sizes"),
-    (dict(n_rows=-1), "sizes"), (dict(w_dtype=0, x_dtype=0), "bf16, f16 or e4m3"), (dict(w_dtype=4, x_dtype=4), "bf16, f16 or e4m3"),
+    (dict(n_rows=-1), "sizes"), (dict(n_rows=0), "without a row"), (dict(w_dtype=0, x_dtype=0), "bf16, f16 or e4m3"), (dict(w_dtype=4, x_dtype=4), "bf16, f16 or e4m3"),
     (dict(x_dtype=2), "one type"), (dict(x=None), "null"), (dict(w0=None), "null"), (dict(pair_idx=None), "null"), (dict(pair_cnt=None), "null"),
     (dict(out=None), "null"), (dict(w_dtype=3, x_dtype=3), "scales"), ({**E8, "x_scale": None}, "scales"), ({**E8, "w0_scale": None}, "scales"),
     (dict(K=60, ldx=64), "16-byte"), (dict(ldx=68), "16-byte"), ({**E8, "K": 40}, "16-byte"), ({**E8, "ldx": 72}, "16-byte"),

@@ -16,6 +16,15 @@ def gen(*key):
     return g
 
 
+@pytest.fixture(params=[1, 2], ids=["single", "pair"])
+def form(request):
+    """Both forms of the products: single SMs with buckets of 64 rows, CTA pairs with buckets of 256."""
+    from kanjoos_b200 import _lib
+    _lib.lib().knj_expert_tc_form(request.param)
+    yield request.param
+    _lib.lib().knj_expert_tc_form(0)
+
+
 def strided(t, pad):
     """The same rows inside a wider tensor."""
     wide = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), dtype=t.dtype, device=t.device)
@@ -168,13 +177,13 @@ EXPERTS = [
 @pytest.mark.parametrize("dtype", [BF16, F16, E4M3])
 @pytest.mark.parametrize("E,N,K,counts", EXPERTS)
 @pytest.mark.parametrize("kind", ["gateup", "proj"])
-def test_expert_products(kind, E, N, K, counts, dtype):
+def test_expert_products(kind, E, N, K, counts, dtype, form):
     run_expert(kind, E, N, K, counts, dtype, {"gateup": BF16, "proj": F32}[kind])
 
 
 @pytest.mark.parametrize("out", [F32, BF16, F16])
 @pytest.mark.parametrize("kind,dtype", [("gateup", F16), ("gateup", E4M3), ("proj", BF16), ("proj", E4M3)])
-def test_expert_output_types(kind, dtype, out):
+def test_expert_output_types(kind, dtype, out, form):
     run_expert(kind, 3, 264, 288, [70, 0, 9], dtype, out)
 
 
@@ -206,7 +215,7 @@ def run_expert(kind, E, N, K, counts, dtype, out_t):
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_unnamed_rows_bad_entries_and_row_maps(dtype):
+def test_unnamed_rows_bad_entries_and_row_maps(dtype, form):
     """Rows that no table entry names stay as they were, entries outside the pairs are skipped, a row outside x reads as
     zeros, a count above the table's stride is the stride; strided rows with NaN between them."""
     from kanjoos_b200 import ops
@@ -241,7 +250,7 @@ def test_unnamed_rows_bad_entries_and_row_maps(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_no_pairs_at_all(dtype):
+def test_no_pairs_at_all(dtype, form):
     from kanjoos_b200 import ops
     g = gen("empty")
     w, sc = ref.matrix((4, 128, 128), g, dtype)
@@ -256,7 +265,7 @@ def test_no_pairs_at_all(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_non_finite_values_stay_in_their_rows(dtype):
+def test_non_finite_values_stay_in_their_rows(dtype, form):
     from kanjoos_b200 import ops
     g = gen("nan", dtype)
     E, N, K = 2, 256, 384
@@ -292,7 +301,7 @@ def test_non_finite_values_stay_in_their_rows(dtype):
 @pytest.mark.parametrize("m,n,k,dtype,out,pad", [(1, 2048, 2048, BF16, F32, 0), (1, 1, 16, F32, F32, 0), (2, 100, 144, F16, BF16, 0),
                                                  (17, 128, 128, BF16, F16, 8), (64, 1000, 2064, F32, F32, 4), (65, 257, 400, BF16, BF16, 0),
                                                  (301, 1000, 2048, BF16, BF16, 0), (513, 384, 256, F16, F32, 0), (3, 4096, 4096, BF16, F32, 0)])
-def test_fp8_matmul(m, n, k, dtype, out, pad):
+def test_fp8_matmul(m, n, k, dtype, out, pad, form):
     from kanjoos_b200 import ops
     g = gen(m, n, k)
     w, sc = ref.matrix((n, k), g, E4M3)
@@ -304,7 +313,7 @@ def test_fp8_matmul(m, n, k, dtype, out, pad):
     ref.check(got, want, err + ref.held(want.abs() + err, out), "product")
 
 
-def test_results_do_not_depend_on_the_run():
+def test_results_do_not_depend_on_the_run(form):
     from kanjoos_b200 import ops
     g = gen("again")
     w, sc = ref.matrix((300, 2048), g, E4M3)
