@@ -22,6 +22,8 @@
 #include "knj_fp8.cuh"
 #include "knj_tc.cuh"
 
+#include <type_traits>
+
 using namespace knj;
 
 namespace {
@@ -36,6 +38,7 @@ struct GemmParams {
   int64_t ldo, idx_stride;
   int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles;
   uint32_t idesc_format;
+  int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
   float out_scale;
   CUtensorMap map0, map1, mapx;
 };
@@ -46,6 +49,7 @@ struct Shape {
   static constexpr int kTokStep = 16 * CG;               // bucket sizes are multiples of this
   static constexpr int kEpiWarps = CG == 2 ? 8 : 4;
   static constexpr int kMmaWarp = kEpiWarps, kMatWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
+  static constexpr int kScaleWarps = CG == 2 ? 2 : 1;
   static constexpr int kRowWarps = CG == 2 ? 4 : 1, kRowWarp = CG == 2 ? 12 : 7;
   static constexpr int kThreads = 32 * (kRowWarp + kRowWarps);
   static constexpr int kBlocksPerSm = CG == 2 ? 1 : 2;
@@ -55,15 +59,17 @@ struct Shape {
   static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per stage
   static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile
   static constexpr int kVecs = GATEUP ? 2 : 1;
-  static constexpr int kScaleSlots = FP8 ? 4 : 0;
-  static constexpr int kScaleSlot = kVecs * kTok * 4 + (GATEUP ? 64 : 0);   // the second vector starts 16 banks on
+  static constexpr int kAccs = CG == 2 ? 2 : 4;          // accumulator buffers of kTok columns
+  static constexpr int kScaleGroups = FP8 ? 2 : 0;       // ring of scale vectors, four blocks of K to a group
+  static constexpr int kScaleVec = kVecs * kTok * 4;
+  static constexpr int kScaleGroup = 4 * kScaleVec;
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kATile;
   static constexpr int kOffScale = kOffB + kStages * kBTile;
-  static constexpr int kOffPairs = kOffScale + kScaleSlots * kScaleSlot;    // [2][kTok] pair of each column
+  static constexpr int kOffPairs = kOffScale + kScaleGroups * kScaleGroup;    // [2][kTok] pair of each column
   static constexpr int kOffPref = kOffPairs + 2 * kTok * 4;                 // [E + 1] buckets before expert e, [E] pairs of it
   static constexpr int kOffBars = kOffPref + (2 * kMaxExperts + 4) * 4;
-  static constexpr int kBytes = kOffBars + 256 + 1024;
+  static constexpr int kBytes = kOffBars + 320 + 1024;
 };
 
 struct Tile {
@@ -77,14 +83,14 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   else tc_mma_f16<CG>(d, a, b, idesc, acc);
 }
 
-__device__ __forceinline__ void fma2(float &a0, float &a1, uint32_t x0, uint32_t x1, float s0, float s1) {
-  asm("{\n\t.reg .b64 x, s, a;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\tmov.b64 a, {%0, %1};\n\t"
-      "fma.rn.f32x2 a, x, s, a;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(a0), "+f"(a1)
-      : "r"(x0), "r"(x1), "f"(s0), "f"(s1));
+// (a0, a1) += (x0 * s0, x1 * s1): the pairs stay in 64-bit registers, packed and unpacked they would cost more than the product
+__device__ __forceinline__ void fma2(unsigned long long &a, uint32_t x0, uint32_t x1, unsigned long long s) {
+  asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}" : "+l"(a) : "r"(x0), "r"(x1), "l"(s));
 }
+
+__device__ __forceinline__ void put_as(float *at, float v) { *at = v; }
+__device__ __forceinline__ void put_as(__nv_bfloat16 *at, float v) { *at = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put_as(__half *at, float v) { *at = __float2half_rn(v); }
 
 template <bool FP8, bool GATEUP, int CG>
 __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, GATEUP, CG>::kBlocksPerSm)
@@ -99,11 +105,11 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kOffBars);
   uint64_t *full = bars;                        // [kStages] operands of both CTAs landed (the even CTA's are used)
   uint64_t *empty = full + S::kStages;          // [kStages] the stage's products are done
-  uint64_t *acc_full = empty + S::kStages;      // [2] accumulator buffer complete
-  uint64_t *acc_empty = acc_full + 2;           // [2] accumulator buffer read (the even CTA's are used)
-  uint64_t *sc_full = acc_empty + 2;            // [kScaleSlots]
-  uint64_t *sc_empty = sc_full + 4;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sc_empty + 4);
+  uint64_t *acc_full = empty + S::kStages;      // [kAccs] accumulator buffer complete
+  uint64_t *acc_empty = acc_full + S::kAccs;    // [kAccs] accumulator buffer read (the even CTA's are used)
+  uint64_t *sc_full = acc_empty + S::kAccs;     // [kScaleGroups]
+  uint64_t *sc_empty = sc_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sc_empty + 2);
   volatile int *s_fail = reinterpret_cast<volatile int *>(tmem_slot + 1);  // raised by the first wait that gives up
   int32_t *s_pair = reinterpret_cast<int32_t *>(smem + S::kOffPairs);
   int32_t *s_pref = reinterpret_cast<int32_t *>(smem + S::kOffPref), *s_cnt = s_pref + kMaxExperts + 1;
@@ -113,18 +119,18 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kAccs; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], CG * S::kEpiWarps);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&sc_full[i], 1);
+    for (int i = 0; i < S::kScaleGroups; ++i) {
+      mbar_init(&sc_full[i], S::kScaleWarps);
       mbar_init(&sc_empty[i], S::kEpiWarps);
     }
     *s_fail = 0;
     mbar_init_fence();
   }
-  constexpr uint32_t kTmemCols = 2 * S::kTok;
+  constexpr uint32_t kTmemCols = S::kAccs * S::kTok;
   if (warp == S::kMmaWarp) {
     tmem_alloc<CG>(tmem_slot, kTmemCols);
     tmem_relinquish<CG>();
@@ -164,7 +170,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
 
   const int nslab = (p.K + S::kSlab - 1) / S::kSlab;
   const int n_tiles = s_pref[kMaxExperts] * p.m_tiles;   // < 2^31: checked on the host
-  const int step = gridDim.x / CG;
+  // As many CTAs (pairs) as take part in whole rounds: of 1536 tiles on 296 CTAs, 256 take six each instead of 56 a sixth; the matrices
+  // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
+  const int avail = gridDim.x / CG, rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
+  const int first = (int)(blockIdx.x / CG) < step ? blockIdx.x / CG : n_tiles;
   auto tile_at = [&](int t) {
     Tile r;
     const int b = t / p.m_tiles;
@@ -205,167 +214,211 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   }
 
+  // A warp waits, and goes on or gives up, as a whole. The loops of the issuing warps stay warp-uniform around the elected thread's
+  // instructions: with the loop inside the elected branch a stage took ~480 cycles to issue, so ~60 and the wait.
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (ok && !mbar_wait(bar, parity, s_fail)) ok = false;
+    ok = __all_sync(0xffffffffu, ok);
+    return ok;
+  };
+
   if (warp < S::kEpiWarps) {
     // =========================== epilogue ===========================
-    const int group = warp >> 2, quad = warp & 3;     // chunks of 32 columns are dealt to the warp groups in turn
+    // Chunks of 32 columns are dealt to the warp groups in turn. A thread holds, of each 8 columns, two columns of the rows t/4,
+    // t/4 + 8 and (half 1) 16 further of its warp's 32 rows: for gate and up, half 0 is gate and half 1 up of the same outputs.
+    const int group = warp >> 2, quad = warp & 3;
     constexpr int kGroups = S::kEpiWarps / 4, kChunks = S::kTok / 32 / kGroups;
     const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16);
-    auto wait_all = [&](uint64_t *bar, uint32_t parity) {
-      if (ok && !mbar_wait(bar, parity, s_fail)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-    };
-    int buf = 0, slot = 0, pb = 0;
-    uint32_t par = 0, sc_par = 0;
-    for (int t = blockIdx.x / CG; t < n_tiles; t += step, pb ^= 1) {
+    int buf = 0, sg = 0, pb = 0;
+    uint32_t par = 0, sg_par = 0;
+    int next_pr = -1, unused;
+    if (first < n_tiles && tid < S::kTok) resolve(tile_at(first), tid, next_pr, unused);
+    for (int t = first; t < n_tiles; t += step, pb ^= 1) {
       const Tile tl = tile_at(t);
       const int ncol = columns(tl);
-      if (tid < S::kTok) {
-        int pr, row;
-        resolve(tl, tid, pr, row);
-        s_pair[pb * S::kTok + tid] = pr;
-      }
+      if (tid < S::kTok) s_pair[pb * S::kTok + tid] = next_pr;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kEpiWarps) : "memory");
-      const int32_t *pairs = s_pair + pb * S::kTok;
-      const int n0 = tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
-      const int n = n0 + (GATEUP ? quad * 16 + (lane & 15) : quad * 32 + lane);
-      auto put = [&](int pr, float v) {
-        if (pr == -1 || n >= p.N) return;
-        if (!ok) v = __int_as_float(0x7fffffff);
-        else v *= p.out_scale;
-        if (pr < 0) {
-          pr = -2 - pr;
-          if (ok) v = 0.f;
-        }
-        store_from_f32(p.out, p.out_dtype, pr * p.ldo + n, v);
-      };
-      // 32 columns from c0 on: one output per lane and column, or for gate and up one per lane and pair of columns
-      auto finish = [&](const float (&v)[32], int c0) {
-        if constexpr (GATEUP) {
+      // the next tile's pairs travel during this one: behind a full memory queue a load of the tables takes microseconds
+      if (t + step < n_tiles && tid < S::kTok) resolve(tile_at(t + step), tid, next_pr, unused);
+      const int32_t *pairs = s_pair + pb * S::kTok + 2 * (lane & 3);
+      const int n = tl.mt * S::kOuts * CG + (int)rank * S::kOuts + quad * (GATEUP ? 16 : 32) + (lane >> 2);
+      // 16 columns from c0 on
+      auto finish_as = [&](auto *out, const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c0) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float got = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[j + 1] : v[j], 16);
-            const float g = lane < 16 ? v[j] : got, u = lane < 16 ? got : v[j + 1];
-            put(pairs[c0 + j + (lane >> 4)], __fdividef(g, 1.0f + __expf(-g)) * u);
+        for (int i = 0; i < 2; ++i) {
+          const int2 pp = *reinterpret_cast<const int2 *>(pairs + c0 + 8 * i);
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int pr = cc ? pp.y : pp.x;
+            if (pr == -1) continue;
+            auto *row = out + (pr < 0 ? -2 - pr : pr) * p.ldo + n;
+            auto put = [&](int off, float v) {
+              v = ok ? (pr < 0 ? 0.f : v * p.out_scale) : __int_as_float(0x7fffffff);
+              if (n + off < p.N) put_as(row + off, v);
+            };
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              const float a = __uint_as_float(lo[4 * i + 2 * rr + cc]), b = __uint_as_float(hi[4 * i + 2 * rr + cc]);
+              if constexpr (GATEUP) {
+                put(8 * rr, __fdividef(a, 1.0f + __expf(-a)) * b);
+              } else {
+                put(8 * rr, a);
+                put(8 * rr + 16, b);
+              }
+            }
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) put(pairs[c0 + j], v[j]);
         }
       };
-      if constexpr (!FP8) {
-        wait_all(&acc_full[buf], par);
-        tc_fence_after();
-#pragma unroll 1
-        for (int ch = group; ch * 32 < ncol; ch += kGroups) {
-          uint32_t r[32] = {};
-          if (ok) {
-            tmem_ld32(lanes + buf * S::kTok + ch * 32, r);
-            tmem_ld_wait();
-          }
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          finish(v, ch * 32);
-        }
+      auto finish = [&](const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c0) {
+        if (p.out_dtype == KNJ_DT_F32) finish_as(static_cast<float *>(p.out), lo, hi, c0);
+        else if (p.out_dtype == KNJ_DT_BF16) finish_as(static_cast<__nv_bfloat16 *>(p.out), lo, hi, c0);
+        else finish_as(static_cast<__half *>(p.out), lo, hi, c0);
+      };
+      auto load = [&](uint32_t (&lo)[8], uint32_t (&hi)[8], int col) {
+        tmem_ld_16x16(lanes + buf * S::kTok + col, lo);
+        tmem_ld_16x16(lanes + (16u << 16) + buf * S::kTok + col, hi);
+      };
+      auto release = [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
           if (CG == 2) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
           else mbar_arrive(&acc_empty[buf]);
         }
-        buf ^= 1;
-        if (buf == 0) par ^= 1u;
+        if (++buf == S::kAccs) {
+          buf = 0;
+          par ^= 1u;
+        }
+      };
+      if constexpr (!FP8) {
+        wait(&acc_full[buf], par);
+        tc_fence_after();
+#pragma unroll 1
+        for (int ch = group; ch * 32 < ncol; ch += kGroups) {
+          uint32_t r[4][8] = {};
+          if (ok) {
+            load(r[0], r[1], ch * 32);
+            load(r[2], r[3], ch * 32 + 16);
+            tmem_ld_wait(r[0], r[1]);
+            tmem_ld_wait(r[2], r[3]);
+          }
+          finish(r[0], r[1], ch * 32);
+          finish(r[2], r[3], ch * 32 + 16);
+        }
+        release();
       } else {
-        float acc[kChunks][32];
+        // One straight run of code for each number of chunks: with a branch around every chunk their loads could not be started in
+        // front of each other's sums.
+        auto blocks = [&](auto chunks) {
+          constexpr int kSteps = 2 * decltype(chunks)::value;   // of 16 columns
+          auto col_of = [&](int c) { return ((c >> 1) * kGroups + group) * 32 + (c & 1) * 16; };
+          unsigned long long acc[kSteps > 0 ? kSteps : 1][2][4];   // pairs of f32 sums: steps, halves, (8 columns, rows)
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
+          for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c][j] = 0.f;
-        for (int ks = 0; ks < nslab; ++ks) {
-          wait_all(&sc_full[slot], sc_par);
-          wait_all(&acc_full[buf], par);
-          if (!ok) break;
-          tc_fence_after();
-          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + slot * S::kScaleSlot) +
-                            (GATEUP && lane >= 16 ? S::kTok + 16 : 0);
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const int c0 = (c * kGroups + group) * 32;
-            if (c0 < ncol) {
-              uint32_t r[32];
-              tmem_ld32(lanes + buf * S::kTok + c0, r);
-              tmem_ld_wait();
+              for (int j = 0; j < 4; ++j) acc[c][h][j] = 0ull;
+          for (int ks = 0; ks < nslab && ok; ++ks) {
+            if ((ks & 3) == 0) wait(&sc_full[sg], sg_par);
+            if (!wait(&acc_full[buf], par)) break;
+            tc_fence_after();
+            const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + 2 * (lane & 3);
+            uint32_t r[2][2][8];
+            if constexpr (kSteps > 0) load(r[0][0], r[0][1], col_of(0));
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(sc + c0 + j);
-                fma2(acc[c][j], acc[c][j + 1], r[j], r[j + 1], f.x, f.y);
-                fma2(acc[c][j + 2], acc[c][j + 3], r[j + 2], r[j + 3], f.z, f.w);
+            for (int c = 0; c < kSteps; ++c) {
+              tmem_ld_wait(r[c & 1][0], r[c & 1][1]);
+              if (c + 1 < kSteps) load(r[(c + 1) & 1][0], r[(c + 1) & 1][1], col_of(c + 1));
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const unsigned long long s0 = *reinterpret_cast<const unsigned long long *>(sc + col_of(c) + 8 * i);
+                const unsigned long long s1 = GATEUP ? *reinterpret_cast<const unsigned long long *>(sc + S::kTok + col_of(c) + 8 * i) : s0;
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr) {
+                  fma2(acc[c][0][2 * i + rr], r[c & 1][0][4 * i + 2 * rr], r[c & 1][0][4 * i + 2 * rr + 1], s0);
+                  fma2(acc[c][1][2 * i + rr], r[c & 1][1][4 * i + 2 * rr], r[c & 1][1][4 * i + 2 * rr + 1], s1);
+                }
+              }
+            }
+            release();
+            if ((ks & 3) == 3 || ks + 1 == nslab) {
+              if (lane == 0) mbar_arrive(&sc_empty[sg]);   // behind release()'s __syncwarp
+              if (++sg == S::kScaleGroups) {
+                sg = 0;
+                sg_par ^= 1u;
               }
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (CG == 2) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
-            else mbar_arrive(&acc_empty[buf]);
-            mbar_arrive(&sc_empty[slot]);
-          }
-          buf ^= 1;
-          if (buf == 0) par ^= 1u;
-          if (++slot == S::kScaleSlots) {
-            slot = 0;
-            sc_par ^= 1u;
-          }
-        }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int c0 = (c * kGroups + group) * 32;
-          if (c0 < ncol) finish(acc[c], c0);
+          for (int c = 0; c < kSteps; ++c) {
+            uint32_t lo[8], hi[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              lo[2 * j] = (uint32_t)acc[c][0][j];
+              lo[2 * j + 1] = (uint32_t)(acc[c][0][j] >> 32);
+              hi[2 * j] = (uint32_t)acc[c][1][j];
+              hi[2 * j + 1] = (uint32_t)(acc[c][1][j] >> 32);
+            }
+            finish(lo, hi, col_of(c));
+          }
+        };
+        const int nc = ((ncol + 31) / 32 - group + kGroups - 1) / kGroups;   // chunks of this group
+        if (nc <= 0) blocks(std::integral_constant<int, 0>{});
+        else if (nc == 1) blocks(std::integral_constant<int, 1>{});
+        else if (nc == 2) blocks(std::integral_constant<int, 2>{});
+        else if constexpr (kChunks > 2) {
+          if (nc == 3) blocks(std::integral_constant<int, 3>{});
+          else blocks(std::integral_constant<int, 4>{});
         }
       }
     }
   } else if (warp == S::kMmaWarp) {
     // =========================== MMA issue ===========================
-    if (rank == 0 && elect_one()) {
+    if (rank == 0) {
       const uint64_t a_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffA)), b_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffB));
       int st = 0, buf = 0;
       uint32_t par = 0, acc_par = 1;  // a fresh barrier passes a wait for parity 1
-      for (int t = blockIdx.x / CG; t < n_tiles && ok; t += step) {
+      for (int t = first; t < n_tiles && ok; t += step) {
         const uint32_t idesc = instr_desc_f16(128 * CG, columns(tile_at(t))) | p.idesc_format;
-        if (!FP8 && !mbar_spin(&acc_empty[buf], acc_par, s_fail)) { ok = false; break; }
         for (int ks = 0; ks < nslab; ++ks) {
-          if (FP8 && !mbar_spin(&acc_empty[buf], acc_par, s_fail)) { ok = false; break; }
-          if (!mbar_spin(&full[st], par, s_fail)) { ok = false; break; }
+          if ((FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
+          if (!wait(&full[st], par)) break;
           tc_fence_after();
           const uint64_t a = a_desc0 + (uint32_t)(st * S::kATile) / 16, b = b_desc0 + (uint32_t)(st * S::kBTile) / 16;
+          const bool last = FP8 || ks + 1 == nslab;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma<FP8, CG>(tmem_base + buf * S::kTok, a + 2 * k, b + 2 * k, idesc, (k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
-          if (CG == 2) tc_commit_pair(smem_u32(&empty[st]));
-          else tc_commit_addr<CG>(smem_u32(&empty[st]));
-          if (FP8 || ks + 1 == nslab) {
-            if (CG == 2) tc_commit_pair(smem_u32(&acc_full[buf]));
-            else tc_commit_addr<CG>(smem_u32(&acc_full[buf]));
-            buf ^= 1;
-            if (buf == 0) acc_par ^= 1u;
+            for (int k = 0; k < 4; ++k)
+              mma<FP8, CG>(tmem_base + buf * S::kTok, a + 2 * k, b + 2 * k, idesc, (k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+            if (CG == 2) tc_commit_pair(smem_u32(&empty[st]));
+            else tc_commit_addr<CG>(smem_u32(&empty[st]));
+            if (last) {
+              if (CG == 2) tc_commit_pair(smem_u32(&acc_full[buf]));
+              else tc_commit_addr<CG>(smem_u32(&acc_full[buf]));
+            }
           }
+          __syncwarp();
+          if (last && ++buf == S::kAccs) { buf = 0; acc_par ^= 1u; }
           if (++st == S::kStages) { st = 0; par ^= 1u; }
         }
       }
     }
   } else if (warp == S::kMatWarp) {
     // =========================== matrix rows ===========================
-    if (elect_one()) {
-      int st = 0;
-      uint32_t par = 1;
-      for (int t = blockIdx.x / CG; t < n_tiles && ok; t += step) {
-        const Tile tl = tile_at(t);
-        const int y = tl.e * p.N + tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
-        const uint32_t bytes = (uint32_t)(CG * S::kATile + columns(tl) * 128);  // of both CTAs, matrix and rows
-        for (int ks = 0; ks < nslab; ++ks) {
-          if (!mbar_spin(&empty[st], par, s_fail)) { ok = false; break; }
+    int st = 0;
+    uint32_t par = 1;
+    for (int t = first; t < n_tiles && ok; t += step) {
+      const Tile tl = tile_at(t);
+      const int y = tl.e * p.N + tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
+      // of both CTAs, matrix and rows
+      const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : columns(tl) * 128));
+      for (int ks = 0; ks < nslab; ++ks) {
+        if (!wait(&empty[st], par)) break;
+        const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
+        const uint32_t dst = smem_u32(smem + S::kOffA + st * S::kATile);
+        if (elect_one()) {
           if (rank == 0) mbar_expect_tx(&full[st], bytes);
-          const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
-          const uint32_t dst = smem_u32(smem + S::kOffA + st * S::kATile);
           if (GATEUP) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -375,104 +428,122 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           } else {
             tma_load_box<CG>(dst, &p.map0, ks * S::kSlab, y, bar);
           }
-          if (++st == S::kStages) { st = 0; par ^= 1u; }
         }
+        __syncwarp();
+        if (++st == S::kStages) { st = 0; par ^= 1u; }
       }
     }
-  } else if (FP8 && warp == S::kScaleWarp) {
+  } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
     // =========================== scales ===========================
-    constexpr int kPer = S::kTok / 32, kAhead = 4;   // columns per lane, blocks of K read at once
-    const int nb_n = (p.N + 127) / 128;
-    int slot = 0;
+    // Four blocks of K are read at once, as one 16-byte load a column where the rows of scales allow it, and the next four before
+    // the ring is waited for; the rows of the next tile are found a tile ahead.
+    constexpr int kPer = S::kTok / 32 / S::kScaleWarps;   // columns per lane
+    const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
+    const bool quads = nslab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.xs) & 15) == 0;
+    int sg = 0, unused, next_row[kPer];
     uint32_t par = 1;
-    for (int t = blockIdx.x / CG; t < n_tiles && ok; t += step) {
+    auto rows_of = [&](int t) {
+      const Tile tl = tile_at(t);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) resolve(tl, c0 + 32 * j, unused, next_row[j]);
+    };
+    if (first < n_tiles) rows_of(first);
+    for (int t = first; t < n_tiles && ok; t += step) {
       const Tile tl = tile_at(t);
       const int n0 = tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
       // a CTA behind the last output of a pair's tile has no block of its own: any block's scales do
       const int64_t blk = ((int64_t)tl.e * nb_n + min(n0 / 128, nb_n - 1)) * nslab;
       const float *xs[kPer];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        int pr, row;
-        resolve(tl, lane + 32 * j, pr, row);
-        xs[j] = p.xs + (int64_t)row * nslab;
-      }
-      for (int k0 = 0; k0 < nslab && ok; k0 += kAhead) {
-        float v[kAhead][kPer], w0[kAhead], w1[kAhead];
+      for (int j = 0; j < kPer; ++j) xs[j] = p.xs + (int64_t)next_row[j] * nslab;
+      if (t + step < n_tiles) rows_of(t + step);
+      float v[4][kPer], w0[4], w1[4];
+      auto fetch = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int kb = min(k0 + i, nslab - 1);
           w0[i] = p.ws0[blk + kb];
           if (GATEUP) w1[i] = p.ws1[blk + kb];
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) v[i][j] = xs[j][kb];
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (k0 + i < nslab && ok) {
-            if (!mbar_wait(&sc_empty[slot], par, s_fail)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-              float *dst = reinterpret_cast<float *>(smem + S::kOffScale + slot * S::kScaleSlot);
+        for (int j = 0; j < kPer; ++j) {
+          if (quads) {
+            const float4 f = *reinterpret_cast<const float4 *>(xs[j] + k0);
+            v[0][j] = f.x; v[1][j] = f.y; v[2][j] = f.z; v[3][j] = f.w;
+          } else {
 #pragma unroll
-              for (int j = 0; j < kPer; ++j) {
-                dst[lane + 32 * j] = v[i][j] * w0[i];
-                if (GATEUP) dst[S::kTok + 16 + lane + 32 * j] = v[i][j] * w1[i];
-              }
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sc_full[slot]);
-              if (++slot == S::kScaleSlots) {
-                slot = 0;
-                par ^= 1u;
-              }
-            }
+            for (int i = 0; i < 4; ++i) v[i][j] = xs[j][min(k0 + i, nslab - 1)];
           }
+        }
+      };
+      fetch(0);
+      for (int k0 = 0; k0 < nslab; k0 += 4) {
+        if (!wait(&sc_empty[sg], par)) break;
+        float *dst = reinterpret_cast<float *>(smem + S::kOffScale + sg * S::kScaleGroup) + c0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            dst[i * S::kVecs * S::kTok + 32 * j] = v[i][j] * w0[i];
+            if (GATEUP) dst[(2 * i + 1) * S::kTok + 32 * j] = v[i][j] * w1[i];
+          }
+        if (k0 + 4 < nslab) fetch(k0 + 4);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_full[sg]);
+        if (++sg == S::kScaleGroups) {
+          sg = 0;
+          par ^= 1u;
         }
       }
     }
   } else if (warp >= S::kRowWarp && warp < S::kRowWarp + S::kRowWarps) {
     // =========================== routed rows ===========================
     const int w = warp - S::kRowWarp;
-    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps);   // copies of four rows per warp and stage
-    int st = 0;
+    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps), kSets = kQuads / 8;   // copies of four rows per warp and stage
+    int st = 0, next_row[kSets], unused;
     uint32_t par = 1;
-    for (int t = blockIdx.x / CG; t < n_tiles; t += step) {
+    auto rows_of = [&](int t) {
+      const Tile tl = tile_at(t);
+      const int n_cta = columns(tl) / CG;
+#pragma unroll
+      for (int g = 0; g < kSets; ++g) {
+        // lane 4q + i finds row i of the warp's quad 8g + q
+        const int r = 4 * (w + S::kRowWarps * (8 * g + (lane >> 2))) + (lane & 3);
+        next_row[g] = 0;
+        if (r < n_cta) resolve(tl, (int)rank * n_cta + r, unused, next_row[g]);
+      }
+    };
+    if (first < n_tiles) rows_of(first);
+    for (int t = first; t < n_tiles && ok; t += step) {
       const Tile tl = tile_at(t);
       const int n_cta = columns(tl) / CG;
       int4 rows[kQuads];
 #pragma unroll
-      for (int g = 0; g < kQuads / 8; ++g) {
-        // lane 4q + i finds row i of the warp's quad 8g + q
-        const int r = 4 * (w + S::kRowWarps * (8 * g + (lane >> 2))) + (lane & 3);
-        int pr, row = 0;
-        if (r < n_cta) resolve(tl, (int)rank * n_cta + r, pr, row);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          rows[8 * g + q].x = __shfl_sync(0xffffffffu, row, 4 * q);
-          rows[8 * g + q].y = __shfl_sync(0xffffffffu, row, 4 * q + 1);
-          rows[8 * g + q].z = __shfl_sync(0xffffffffu, row, 4 * q + 2);
-          rows[8 * g + q].w = __shfl_sync(0xffffffffu, row, 4 * q + 3);
-        }
+      for (int q = 0; q < kQuads; ++q) {
+        rows[q].x = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8));
+        rows[q].y = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 1);
+        rows[q].z = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 2);
+        rows[q].w = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 3);
       }
-      if (elect_one()) {
-        int s = st;
-        uint32_t sp = par;
-        for (int ks = 0; ks < nslab; ++ks) {
-          if (!mbar_spin(&empty[s], sp, s_fail)) { ok = false; break; }
-          const uint32_t bar = CG == 2 ? cluster_addr(&full[s], 0) : smem_u32(&full[s]);
-          const uint32_t dst = smem_u32(smem + S::kOffB + s * S::kBTile);
+      if (t + step < n_tiles) rows_of(t + step);
+      for (int ks = 0; ks < nslab; ++ks) {
+        if (!wait(&empty[st], par)) break;
+        const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
+        const uint32_t dst = smem_u32(smem + S::kOffB + st * S::kBTile);
+        if (elect_one()) {
+          if (p.dense) {
+            if (w == 0) tma_load_box<CG>(dst, &p.mapx, ks * S::kSlab, tl.tok0 + (int)rank * n_cta, bar);
+          } else {
 #pragma unroll
-          for (int q = 0; q < kQuads; ++q) {
-            const int r = 4 * (w + S::kRowWarps * q);
-            if (r < n_cta) tma_gather4<CG>(dst + r * 128, &p.mapx, ks * S::kSlab, rows[q], bar);
+            for (int q = 0; q < kQuads; ++q) {
+              const int r = 4 * (w + S::kRowWarps * q);
+              if (r < n_cta) tma_gather4<CG>(dst + r * 128, &p.mapx, ks * S::kSlab, rows[q], bar);
+            }
           }
-          if (++s == S::kStages) { s = 0; sp ^= 1u; }
         }
+        __syncwarp();
+        if (++st == S::kStages) { st = 0; par ^= 1u; }
       }
-      par ^= (uint32_t)((st + nslab) / S::kStages) & 1u;
-      st = (st + nslab) % S::kStages;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
     }
   }
 
@@ -513,7 +584,7 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   const uint64_t w_rows = (uint64_t)p.E * p.N;
   int rc = make_operand_tensor_map(&p.map0, o.w0, esz, p.K, p.K, w_rows, GATEUP ? 16 : 128);
   if (!rc && GATEUP) rc = make_operand_tensor_map(&p.map1, o.w1, esz, p.K, p.K, w_rows, 16);
-  if (!rc) rc = make_operand_tensor_map(&p.mapx, o.x, esz, p.K, o.ldx, p.n_rows, 1);
+  if (!rc) rc = make_operand_tensor_map(&p.mapx, o.x, esz, p.K, o.ldx, p.n_rows, p.dense ? S::kTok / CG : 1);
   if (rc) return rc;
   p.m_tiles = (p.N + S::kOuts * CG - 1) / (S::kOuts * CG);
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
@@ -618,7 +689,7 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
   if (rc) return rc;
   GemmParams p{};
   p.xs = qs; p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
-  p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f;
+  p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f; p.dense = 1;
   return launch_gemm<false>(p, Operands{q, W, nullptr, n_in, true}, as_stream(s));
 }
 
