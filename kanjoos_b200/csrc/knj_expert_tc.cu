@@ -38,6 +38,7 @@ struct GemmParams {
   int64_t ldo, idx_stride;
   int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles;
   uint32_t idesc_format;
+  int vec_out;                // 16-byte stores of 16-bit outputs
   int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
   float out_scale;
   CUtensorMap map0, map1, mapx;
@@ -66,7 +67,9 @@ struct Shape {
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kATile;
   static constexpr int kOffScale = kOffB + kStages * kBTile;
-  static constexpr int kOffPairs = kOffScale + kScaleGroups * kScaleGroup;    // [2][kTok] pair of each column
+  static constexpr int kStage = 16 * 48;                 // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16
+  static constexpr int kOffStage = kOffScale + kScaleGroups * kScaleGroup;
+  static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [2][kTok] pair of each column
   static constexpr int kOffPref = kOffPairs + 2 * kTok * 4;                 // [E + 1] buckets before expert e, [E] pairs of it
   static constexpr int kOffBars = kOffPref + (2 * kMaxExperts + 4) * 4;
   static constexpr int kBytes = kOffBars + 320 + 1024;
@@ -87,10 +90,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 __device__ __forceinline__ void fma2(unsigned long long &a, uint32_t x0, uint32_t x1, unsigned long long s) {
   asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}" : "+l"(a) : "r"(x0), "r"(x1), "l"(s));
 }
-
-__device__ __forceinline__ void put_as(float *at, float v) { *at = v; }
-__device__ __forceinline__ void put_as(__nv_bfloat16 *at, float v) { *at = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put_as(__half *at, float v) { *at = __float2half_rn(v); }
 
 template <bool FP8, bool GATEUP, int CG>
 __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, GATEUP, CG>::kBlocksPerSm)
@@ -240,39 +239,89 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kEpiWarps) : "memory");
       // the next tile's pairs travel during this one: behind a full memory queue a load of the tables takes microseconds
       if (t + step < n_tiles && tid < S::kTok) resolve(tile_at(t + step), tid, next_pr, unused);
-      const int32_t *pairs = s_pair + pb * S::kTok + 2 * (lane & 3);
-      const int n = tl.mt * S::kOuts * CG + (int)rank * S::kOuts + quad * (GATEUP ? 16 : 32) + (lane >> 2);
-      // 16 columns from c0 on
-      auto finish_as = [&](auto *out, const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c0) {
+      const int32_t *pairs = s_pair + pb * S::kTok;
+      const int n0 = tl.mt * S::kOuts * CG + (int)rank * S::kOuts + quad * (GATEUP ? 16 : 32);   // the warp's first output
+      // 16 columns from c0 on, f32: the eight lanes of a column write one 32-byte sector of its row
+      auto finish_f32 = [&](float *out, const float (&v)[2][8], int c0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int2 pp = *reinterpret_cast<const int2 *>(pairs + c0 + 8 * i);
+          const int2 pp = *reinterpret_cast<const int2 *>(pairs + c0 + 8 * i + 2 * (lane & 3));
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
             const int pr = cc ? pp.y : pp.x;
             if (pr == -1) continue;
-            auto *row = out + (pr < 0 ? -2 - pr : pr) * p.ldo + n;
-            auto put = [&](int off, float v) {
-              v = ok ? (pr < 0 ? 0.f : v * p.out_scale) : __int_as_float(0x7fffffff);
-              if (n + off < p.N) put_as(row + off, v);
-            };
+            float *row = out + (pr < 0 ? -2 - pr : pr) * p.ldo + n0 + (lane >> 2);
 #pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-              const float a = __uint_as_float(lo[4 * i + 2 * rr + cc]), b = __uint_as_float(hi[4 * i + 2 * rr + cc]);
-              if constexpr (GATEUP) {
-                put(8 * rr, __fdividef(a, 1.0f + __expf(-a)) * b);
-              } else {
-                put(8 * rr, a);
-                put(8 * rr + 16, b);
+            for (int h = 0; h < (GATEUP ? 1 : 2); ++h)
+#pragma unroll
+              for (int rr = 0; rr < 2; ++rr) {
+                float f = v[h][4 * i + 2 * rr + cc];
+                f = ok ? (pr < 0 ? 0.f : f) : __int_as_float(0x7fffffff);
+                if (n0 + (lane >> 2) + 8 * rr + 16 * h < p.N) row[8 * rr + 16 * h] = f;
               }
+          }
+        }
+      };
+      // 16 bits: transposed through shared memory (stmatrix), so that whole sectors are written -- 16-byte pieces of a row from
+      // two instructions made the stores of a tile of 256 columns take 28,000 cycles
+      auto finish_16 = [&](const float (&v)[2][8], int c0) {
+        const bool bf16 = p.out_dtype == KNJ_DT_BF16;
+        auto pack = [&](float a, float b) {
+          if (bf16) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const uint32_t *>(&x);
+          }
+          const __half2 x = __floats2half2_rn(a, b);
+          return *reinterpret_cast<const uint32_t *>(&x);
+        };
+        constexpr int kRow = GATEUP ? 32 : 64, kPitch = kRow + 16;          // bytes of a column's outputs
+        constexpr int kCols = GATEUP ? 16 : 8;                              // columns per store of the warp
+        uint8_t *stg = smem + S::kOffStage + warp * S::kStage;
+#pragma unroll
+        for (int i = 0; i < 16 / kCols; ++i) {
+          uint32_t m[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            // matrix q: 8 outputs x 8 columns
+            const int g = GATEUP ? q >> 1 : i, h = GATEUP ? 0 : q >> 1, rr = q & 1;
+            m[q] = pack(v[h][4 * g + 2 * rr], v[h][4 * g + 2 * rr + 1]);
+          }
+          const int q = lane >> 3, c = (GATEUP ? 8 * (q >> 1) : 0) + (lane & 7);
+          __syncwarp();
+          asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                           smem_u32(stg + c * kPitch + (GATEUP ? q & 1 : q) * 16)),
+                       "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+                       : "memory");
+          __syncwarp();
+          const int col = lane / (kRow / 16), part = lane % (kRow / 16);
+          uint4 u = *reinterpret_cast<const uint4 *>(stg + col * kPitch + part * 16);
+          int pr = pairs[c0 + i * kCols + col];
+          if (pr != -1) {
+            if (!ok) u = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            else if (pr < 0) u = make_uint4(0, 0, 0, 0);
+            const int n = n0 + 8 * part;
+            uint16_t *at = static_cast<uint16_t *>(p.out) + (pr < 0 ? -2 - pr : pr) * p.ldo + n;
+            if (p.vec_out && n + 8 <= p.N) {
+              *reinterpret_cast<uint4 *>(at) = u;
+            } else {
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < p.N) at[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
             }
           }
         }
       };
       auto finish = [&](const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c0) {
-        if (p.out_dtype == KNJ_DT_F32) finish_as(static_cast<float *>(p.out), lo, hi, c0);
-        else if (p.out_dtype == KNJ_DT_BF16) finish_as(static_cast<__nv_bfloat16 *>(p.out), lo, hi, c0);
-        else finish_as(static_cast<__half *>(p.out), lo, hi, c0);
+        float v[2][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float a = __uint_as_float(lo[j]), b = __uint_as_float(hi[j]);
+          v[0][j] = (GATEUP ? __fdividef(a, 1.0f + __expf(-a)) * b : a) * p.out_scale;
+          v[1][j] = b * p.out_scale;
+        }
+        if (p.out_dtype == KNJ_DT_F32) finish_f32(static_cast<float *>(p.out), v, c0);
+        else finish_16(v, c0);
       };
       auto load = [&](uint32_t (&lo)[8], uint32_t (&hi)[8], int col) {
         tmem_ld_16x16(lanes + buf * S::kTok + col, lo);
@@ -587,6 +636,7 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   if (!rc) rc = make_operand_tensor_map(&p.mapx, o.x, esz, p.K, o.ldx, p.n_rows, p.dense ? S::kTok / CG : 1);
   if (rc) return rc;
   p.m_tiles = (p.N + S::kOuts * CG - 1) / (S::kOuts * CG);
+  p.vec_out = aligned16(p.out) && p.ldo % 8 == 0;
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
   KNJ_REQUIRE(most * p.m_tiles < (1ll << 31) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
