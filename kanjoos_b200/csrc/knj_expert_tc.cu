@@ -51,7 +51,7 @@ struct Shape {
   static constexpr int kEpiWarps = CG == 2 ? 8 : 4;
   static constexpr int kMmaWarp = kEpiWarps, kMatWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
   static constexpr int kScaleWarps = CG == 2 ? 2 : 1;
-  static constexpr int kRowWarps = CG == 2 ? 4 : 1, kRowWarp = CG == 2 ? 12 : 7;
+  static constexpr int kRowWarps = CG == 2 ? (FP8 ? 4 : 8) : 1, kRowWarp = CG == 2 ? 12 : 7;
   static constexpr int kThreads = 32 * (kRowWarp + kRowWarps);
   static constexpr int kBlocksPerSm = CG == 2 ? 1 : 2;
   static constexpr int kStages = CG == 2 ? 6 : 4;
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   } else if (warp >= S::kRowWarp && warp < S::kRowWarp + S::kRowWarps) {
     // =========================== routed rows ===========================
     const int w = warp - S::kRowWarp;
-    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps), kSets = kQuads / 8;   // copies of four rows per warp and stage
+    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps), kSets = (kQuads + 7) / 8;   // copies of four rows per warp and stage
     int st = 0, next_row[kSets], unused;
     uint32_t par = 1;
     auto rows_of = [&](int t) {
@@ -557,9 +557,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
 #pragma unroll
       for (int g = 0; g < kSets; ++g) {
         // lane 4q + i finds row i of the warp's quad 8g + q
-        const int r = 4 * (w + S::kRowWarps * (8 * g + (lane >> 2))) + (lane & 3);
+        const int q = 8 * g + (lane >> 2), r = 4 * (w + S::kRowWarps * q) + (lane & 3);
         next_row[g] = 0;
-        if (r < n_cta) resolve(tl, (int)rank * n_cta + r, unused, next_row[g]);
+        if (q < kQuads && r < n_cta) resolve(tl, (int)rank * n_cta + r, unused, next_row[g]);
       }
     };
     if (first < n_tiles) rows_of(first);
