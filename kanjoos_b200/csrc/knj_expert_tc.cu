@@ -54,10 +54,11 @@ struct Shape {
   static constexpr int kRowWarps = CG == 2 ? (FP8 ? 4 : 8) : 1, kRowWarp = CG == 2 ? 12 : 7;
   static constexpr int kThreads = 32 * (kRowWarp + kRowWarps);
   static constexpr int kBlocksPerSm = CG == 2 ? 1 : 2;
-  static constexpr int kStages = CG == 2 ? 6 : 4;
+  static constexpr int kSub = CG == 2 && !FP8 ? 2 : 1;   // slabs of 128 bytes of K per stage
+  static constexpr int kStages = CG == 2 ? 6 / kSub : 4;
   static constexpr int kATile = 128 * 128;               // bytes: 128 matrix rows x 128 bytes of K
   static constexpr int kBTile = kTok / CG * 128;
-  static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per stage
+  static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per slab
   static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile
   static constexpr int kVecs = GATEUP ? 2 : 1;
   static constexpr int kAccs = CG == 2 ? 2 : 4;          // accumulator buffers of kTok columns
@@ -65,18 +66,21 @@ struct Shape {
   static constexpr int kScaleVec = kVecs * kTok * 4;
   static constexpr int kScaleGroup = 4 * kScaleVec;
   static constexpr int kOffA = 0;
-  static constexpr int kOffB = kOffA + kStages * kATile;
-  static constexpr int kOffScale = kOffB + kStages * kBTile;
+  static constexpr int kOffB = kOffA + kStages * kSub * kATile;
+  static constexpr int kOffScale = kOffB + kStages * kSub * kBTile;
   static constexpr int kStage = 16 * 48;                 // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16
   static constexpr int kOffStage = kOffScale + kScaleGroups * kScaleGroup;
-  static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [2][kTok] pair of each column
-  static constexpr int kOffPref = kOffPairs + 2 * kTok * 4;                 // [E + 1] buckets before expert e, [E] pairs of it
+  static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [kTiles][kTok] pair of each column
+  static constexpr int kTiles = 3;                       // ring of tile descriptions
+  static constexpr int kOffRows = kOffPairs + kTiles * kTok * 4;            // [kTiles][kTok] row of each column
+  static constexpr int kOffTile = kOffRows + kTiles * kTok * 4;             // [kTiles] Tile
+  static constexpr int kOffPref = kOffTile + kTiles * 16;                   // [E + 1] buckets before expert e, [E] pairs of it
   static constexpr int kOffBars = kOffPref + (2 * kMaxExperts + 4) * 4;
   static constexpr int kBytes = kOffBars + 320 + 1024;
 };
 
 struct Tile {
-  int e, tok0, ntok, mt;
+  int e, n0, ncol, tok0;   // expert, first output of the CTA, columns (routed rows, rounded up), first pair of the bucket
 };
 
 // one MMA's K step is 32 bytes of every operand row in both element sizes
@@ -108,9 +112,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   uint64_t *acc_empty = acc_full + S::kAccs;    // [kAccs] accumulator buffer read (the even CTA's are used)
   uint64_t *sc_full = acc_empty + S::kAccs;     // [kScaleGroups]
   uint64_t *sc_empty = sc_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sc_empty + 2);
+  uint64_t *tile_full = sc_empty + 2;           // [kTiles] the tile's description is there
+  uint64_t *tile_empty = tile_full + S::kTiles; // [kTiles] every warp is done with it
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tile_empty + S::kTiles);
   volatile int *s_fail = reinterpret_cast<volatile int *>(tmem_slot + 1);  // raised by the first wait that gives up
   int32_t *s_pair = reinterpret_cast<int32_t *>(smem + S::kOffPairs);
+  int32_t *s_row = reinterpret_cast<int32_t *>(smem + S::kOffRows);
+  int4 *s_tile = reinterpret_cast<int4 *>(smem + S::kOffTile);
   int32_t *s_pref = reinterpret_cast<int32_t *>(smem + S::kOffPref), *s_cnt = s_pref + kMaxExperts + 1;
 
   if (tid == 0) {
@@ -125,6 +133,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     for (int i = 0; i < S::kScaleGroups; ++i) {
       mbar_init(&sc_full[i], S::kScaleWarps);
       mbar_init(&sc_empty[i], S::kEpiWarps);
+    }
+    for (int i = 0; i < S::kTiles; ++i) {
+      mbar_init(&tile_full[i], 1);
+      mbar_init(&tile_empty[i], S::kEpiWarps + S::kRowWarps + (FP8 ? S::kScaleWarps : 0) + (rank == 0 ? 1 : 0));
     }
     *s_fail = 0;
     mbar_init_fence();
@@ -173,38 +185,26 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
   const int avail = gridDim.x / CG, rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
   const int first = (int)(blockIdx.x / CG) < step ? blockIdx.x / CG : n_tiles;
-  auto tile_at = [&](int t) {
-    Tile r;
-    const int b = t / p.m_tiles;
-    r.mt = t - b * p.m_tiles;
-    int lo = 0;  // the last expert whose first bucket is not behind b
-#pragma unroll
-    for (int h = kMaxExperts / 2; h > 0; h >>= 1)
-      if (s_pref[lo + h] <= b) lo += h;
-    r.e = lo;
-    const int nb = s_pref[lo + 1] - s_pref[lo], cnt = s_cnt[lo];
-    // an expert's pairs are spread evenly over its buckets: 256 + 14 pairs would stream the matrix twice for 14
-    const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
-    r.tok0 = (b - s_pref[lo]) * per;
-    r.ntok = min(per, cnt - r.tok0);
-    return r;
-  };
-  auto columns = [&](const Tile &t) { return (t.ntok + S::kTokStep - 1) / S::kTokStep * S::kTokStep; };
-  // pair of column c (-1: none) and its row of x; pair -2 - p: p's row lies outside x, its output is zero
-  auto resolve = [&](const Tile &t, int c, int &pr, int &row) {
-    pr = -1;
-    row = 0;
-    if (c >= t.ntok) return;
-    pr = p.pair_idx ? p.pair_idx[t.e * p.idx_stride + t.tok0 + c] : t.tok0 + c;
-    if (pr < 0 || pr >= p.n_pairs) {
-      pr = -1;
-      return;
-    }
-    row = p.row_map ? p.row_map[pr] : pr / p.row_div;
-    if (row < 0 || row >= p.n_rows) {
-      pr = -2 - pr;
-      row = 0;
-    }
+      auto tile_at = [&](int t, int &ntok) {
+        const int b = t / p.m_tiles, mt = t - b * p.m_tiles;
+        int lo = 0;  // the last expert whose first bucket is not behind b
+  #pragma unroll
+        for (int h = kMaxExperts / 2; h > 0; h >>= 1)
+          if (s_pref[lo + h] <= b) lo += h;
+        const int nb = s_pref[lo + 1] - s_pref[lo], cnt = s_cnt[lo];
+        // an expert's pairs are spread evenly over its buckets: 256 + 14 pairs would stream the matrix twice for 14
+        const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
+        Tile r;
+        r.e = lo;
+        r.n0 = (mt * CG + (int)rank) * S::kOuts;
+        r.tok0 = (b - s_pref[lo]) * per;
+        ntok = min(per, cnt - r.tok0);
+        r.ncol = (ntok + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
+        return r;
+      };
+  // pair and row of column c of a tile: pair -1: none; pair -2 - p: p's row lies outside x, its output is zero
+  auto pair_at = [&](const Tile &tl, int ntok, int c) {
+    return c < ntok ? (p.pair_idx ? p.pair_idx[tl.e * p.idx_stride + tl.tok0 + c] : tl.tok0 + c) : -1;
   };
   bool ok = true;  // once false this thread skips all work and waits but still meets every barrier
   // e4m3 in pairs: the epilogue's sums take 128 registers a thread. 512 threads x 128 registers at launch = 2 x 128 x 192 + 2 x 128 x 64
@@ -221,6 +221,24 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     return ok;
   };
 
+  // What a tile is, is found once per CTA, by the matrix warp, and handed on through a ring.
+  int tslot = 0;
+  uint32_t tpar = 0;
+  auto tile_take = [&](Tile &tl) {
+    if (!wait(&tile_full[tslot], tpar)) return false;
+    const int4 v = s_tile[tslot];
+    tl = Tile{v.x, v.y, v.z, v.w};
+    return true;
+  };
+  auto tile_done = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tile_empty[tslot]);
+    if (++tslot == S::kTiles) {
+      tslot = 0;
+      tpar ^= 1u;
+    }
+  };
+
   if (warp < S::kEpiWarps) {
     // =========================== epilogue ===========================
     // Chunks of 32 columns are dealt to the warp groups in turn. A thread holds, of each 8 columns, two columns of the rows t/4,
@@ -228,19 +246,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     const int group = warp >> 2, quad = warp & 3;
     constexpr int kGroups = S::kEpiWarps / 4, kChunks = S::kTok / 32 / kGroups;
     const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16);
-    int buf = 0, sg = 0, pb = 0;
+    int buf = 0, sg = 0;
     uint32_t par = 0, sg_par = 0;
-    int next_pr = -1, unused;
-    if (first < n_tiles && tid < S::kTok) resolve(tile_at(first), tid, next_pr, unused);
-    for (int t = first; t < n_tiles; t += step, pb ^= 1) {
-      const Tile tl = tile_at(t);
-      const int ncol = columns(tl);
-      if (tid < S::kTok) s_pair[pb * S::kTok + tid] = next_pr;
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kEpiWarps) : "memory");
-      // the next tile's pairs travel during this one: behind a full memory queue a load of the tables takes microseconds
-      if (t + step < n_tiles && tid < S::kTok) resolve(tile_at(t + step), tid, next_pr, unused);
-      const int32_t *pairs = s_pair + pb * S::kTok;
-      const int n0 = tl.mt * S::kOuts * CG + (int)rank * S::kOuts + quad * (GATEUP ? 16 : 32);   // the warp's first output
+    int t = first;
+    for (; t < n_tiles; t += step, tile_done()) {
+      Tile tl;
+      if (!tile_take(tl)) break;
+      const int ncol = tl.ncol;
+      const int32_t *pairs = s_pair + tslot * S::kTok;
+      const int n0 = tl.n0 + quad * (GATEUP ? 16 : 32);   // the warp's first output
       // 16 columns from c0 on, f32: the eight lanes of a column write one 32-byte sector of its row
       auto finish_f32 = [&](float *out, const float (&v)[2][8], int c0) {
 #pragma unroll
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
 #pragma unroll
               for (int rr = 0; rr < 2; ++rr) {
                 float f = v[h][4 * i + 2 * rr + cc];
-                f = ok ? (pr < 0 ? 0.f : f) : __int_as_float(0x7fffffff);
+                if (pr < 0) f = 0.f;
                 if (n0 + (lane >> 2) + 8 * rr + 16 * h < p.N) row[8 * rr + 16 * h] = f;
               }
           }
@@ -297,8 +311,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           uint4 u = *reinterpret_cast<const uint4 *>(stg + col * kPitch + part * 16);
           int pr = pairs[c0 + i * kCols + col];
           if (pr != -1) {
-            if (!ok) u = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-            else if (pr < 0) u = make_uint4(0, 0, 0, 0);
+            if (pr < 0) u = make_uint4(0, 0, 0, 0);
             const int n = n0 + 8 * part;
             uint16_t *at = static_cast<uint16_t *>(p.out) + (pr < 0 ? -2 - pr : pr) * p.ldo + n;
             if (p.vec_out && n + 8 <= p.N) {
@@ -340,17 +353,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         }
       };
       if constexpr (!FP8) {
-        wait(&acc_full[buf], par);
+        if (!wait(&acc_full[buf], par)) break;
         tc_fence_after();
 #pragma unroll 1
         for (int ch = group; ch * 32 < ncol; ch += kGroups) {
-          uint32_t r[4][8] = {};
-          if (ok) {
-            load(r[0], r[1], ch * 32);
-            load(r[2], r[3], ch * 32 + 16);
-            tmem_ld_wait(r[0], r[1]);
-            tmem_ld_wait(r[2], r[3]);
-          }
+          uint32_t r[4][8];
+          load(r[0], r[1], ch * 32);
+          load(r[2], r[3], ch * 32 + 16);
+          tmem_ld_wait(r[0], r[1]);
+          tmem_ld_wait(r[2], r[3]);
           finish(r[0], r[1], ch * 32);
           finish(r[2], r[3], ch * 32 + 16);
         }
@@ -368,9 +379,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int j = 0; j < 4; ++j) acc[c][h][j] = 0ull;
-          for (int ks = 0; ks < nslab && ok; ++ks) {
+          for (int ks = 0; ks < nslab; ++ks) {
             if ((ks & 3) == 0) wait(&sc_full[sg], sg_par);
-            if (!wait(&acc_full[buf], par)) break;
+            if (!wait(&acc_full[buf], par)) return;
             tc_fence_after();
             const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + 2 * (lane & 3);
             uint32_t r[2][2][8];
@@ -420,6 +431,18 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           if (nc == 3) blocks(std::integral_constant<int, 3>{});
           else blocks(std::integral_constant<int, 4>{});
         }
+        if (!ok) break;
+      }
+    }
+    // a wait gave up: NaN for what this warp has not stored, its tile at that moment and those behind it
+    for (; !ok && t < n_tiles; t += step) {
+      int ntok;
+      const Tile tl = tile_at(t, ntok);
+      const int n = tl.n0 + quad * (GATEUP ? 16 : 32) + lane;
+      for (int c = 0; c < ntok; ++c) {
+        if ((c / 32) % kGroups != group || n >= p.N || lane >= (GATEUP ? 16 : 32)) continue;
+        const int pr = pair_at(tl, ntok, c);
+        if (pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n, __int_as_float(0x7fffffff));
       }
     }
   } else if (warp == S::kMmaWarp) {
@@ -428,18 +451,25 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       const uint64_t a_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffA)), b_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffB));
       int st = 0, buf = 0;
       uint32_t par = 0, acc_par = 1;  // a fresh barrier passes a wait for parity 1
-      for (int t = first; t < n_tiles && ok; t += step) {
-        const uint32_t idesc = instr_desc_f16(128 * CG, columns(tile_at(t))) | p.idesc_format;
-        for (int ks = 0; ks < nslab; ++ks) {
+      for (int t = first; t < n_tiles; t += step, tile_done()) {
+        Tile tl;
+        if (!tile_take(tl)) break;
+        const uint32_t idesc = instr_desc_f16(128 * CG, tl.ncol) | p.idesc_format;
+        for (int ks = 0; ks < nslab; ks += S::kSub) {
           if ((FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
           if (!wait(&full[st], par)) break;
           tc_fence_after();
-          const uint64_t a = a_desc0 + (uint32_t)(st * S::kATile) / 16, b = b_desc0 + (uint32_t)(st * S::kBTile) / 16;
-          const bool last = FP8 || ks + 1 == nslab;
+          const uint64_t a = a_desc0 + (uint32_t)(st * S::kSub * S::kATile) / 16, b = b_desc0 + (uint32_t)(st * S::kSub * S::kBTile) / 16;
+          const bool last = FP8 || ks + S::kSub >= nslab;
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma<FP8, CG>(tmem_base + buf * S::kTok, a + 2 * k, b + 2 * k, idesc, (k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+            for (int u = 0; u < S::kSub; ++u) {
+              if (u > 0 && ks + u >= nslab) break;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma<FP8, CG>(tmem_base + buf * S::kTok, a + u * (S::kATile / 16) + 2 * k, b + u * (S::kBTile / 16) + 2 * k, idesc,
+                             (u > 0 || k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+            }
             if (CG == 2) tc_commit_pair(smem_u32(&empty[st]));
             else tc_commit_addr<CG>(smem_u32(&empty[st]));
             if (last) {
@@ -451,61 +481,110 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           if (last && ++buf == S::kAccs) { buf = 0; acc_par ^= 1u; }
           if (++st == S::kStages) { st = 0; par ^= 1u; }
         }
+        if (!ok) break;
       }
     }
   } else if (warp == S::kMatWarp) {
-    // =========================== matrix rows ===========================
+    // =========================== tiles and matrix rows ===========================
+    constexpr int kPer = S::kTok / 32;
+    // the tables of the next tile are read during this one: behind a full memory queue such a load takes microseconds
+    Tile next{};
+    int pr[kPer], row[kPer];
+    auto look = [&](int t) {
+      int ntok;
+      next = tile_at(t, ntok);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int c = lane + 32 * j;
+        pr[j] = pair_at(next, ntok, c);
+        row[j] = 0;
+      }
+    };
+    auto resolve = [&] {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (pr[j] < 0 || pr[j] >= p.n_pairs) {
+          pr[j] = -1;
+        } else {
+          row[j] = p.row_map ? p.row_map[pr[j]] : p.row_div == 1 ? pr[j] : pr[j] / p.row_div;
+          if (row[j] < 0 || row[j] >= p.n_rows) {
+            pr[j] = -2 - pr[j];
+            row[j] = 0;
+          }
+        }
+      }
+    };
+    if (first < n_tiles) {
+      look(first);
+      resolve();
+    }
     int st = 0;
     uint32_t par = 1;
-    for (int t = first; t < n_tiles && ok; t += step) {
-      const Tile tl = tile_at(t);
-      const int y = tl.e * p.N + tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
-      // of both CTAs, matrix and rows
-      const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : columns(tl) * 128));
-      for (int ks = 0; ks < nslab; ++ks) {
+    tpar = 1;
+    for (int t = first; t < n_tiles; t += step) {
+      const Tile tl = next;
+      if (!wait(&tile_empty[tslot], tpar)) break;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        s_pair[tslot * S::kTok + lane + 32 * j] = pr[j];
+        s_row[tslot * S::kTok + lane + 32 * j] = row[j];
+      }
+      if (lane == 0) s_tile[tslot] = make_int4(tl.e, tl.n0, tl.ncol, tl.tok0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tile_full[tslot]);
+      if (++tslot == S::kTiles) {
+        tslot = 0;
+        tpar ^= 1u;
+      }
+      const int y = tl.e * p.N + tl.n0;
+      // of both CTAs, matrix and rows, per slab
+      const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : tl.ncol * 128));
+      const bool more = t + step < n_tiles;
+      for (int ks = 0; ks < nslab; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
         const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
-        const uint32_t dst = smem_u32(smem + S::kOffA + st * S::kATile);
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&full[st], bytes);
-          if (GATEUP) {
+          if (rank == 0) mbar_expect_tx(&full[st], bytes * min(S::kSub, nslab - ks));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              tma_load_box<CG>(dst + j * 4096, &p.map0, ks * S::kSlab, y + 16 * j, bar);
-              tma_load_box<CG>(dst + j * 4096 + 2048, &p.map1, ks * S::kSlab, y + 16 * j, bar);
+          for (int u = 0; u < S::kSub; ++u) {
+            if (u > 0 && ks + u >= nslab) break;
+            const uint32_t dst = smem_u32(smem + S::kOffA + (st * S::kSub + u) * S::kATile);
+            const int x = (ks + u) * S::kSlab;
+            if (GATEUP) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                tma_load_box<CG>(dst + j * 4096, &p.map0, x, y + 16 * j, bar);
+                tma_load_box<CG>(dst + j * 4096 + 2048, &p.map1, x, y + 16 * j, bar);
+              }
+            } else {
+              tma_load_box<CG>(dst, &p.map0, x, y, bar);
             }
-          } else {
-            tma_load_box<CG>(dst, &p.map0, ks * S::kSlab, y, bar);
           }
         }
         __syncwarp();
         if (++st == S::kStages) { st = 0; par ^= 1u; }
+        if (ks == 0 && more) look(t + step);
       }
+      if (!ok) break;
+      if (more) resolve();
     }
   } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
     // =========================== scales ===========================
     // Four blocks of K are read at once, as one 16-byte load a column where the rows of scales allow it, and the next four before
-    // the ring is waited for; the rows of the next tile are found a tile ahead.
+    // the ring is waited for.
     constexpr int kPer = S::kTok / 32 / S::kScaleWarps;   // columns per lane
     const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
     const bool quads = nslab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.xs) & 15) == 0;
-    int sg = 0, unused, next_row[kPer];
+    int sg = 0;
     uint32_t par = 1;
-    auto rows_of = [&](int t) {
-      const Tile tl = tile_at(t);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) resolve(tl, c0 + 32 * j, unused, next_row[j]);
-    };
-    if (first < n_tiles) rows_of(first);
-    for (int t = first; t < n_tiles && ok; t += step) {
-      const Tile tl = tile_at(t);
-      const int n0 = tl.mt * S::kOuts * CG + (int)rank * S::kOuts;
+    for (int t = first; t < n_tiles; t += step, tile_done()) {
+      Tile tl;
+      if (!tile_take(tl)) break;
       // a CTA behind the last output of a pair's tile has no block of its own: any block's scales do
-      const int64_t blk = ((int64_t)tl.e * nb_n + min(n0 / 128, nb_n - 1)) * nslab;
+      const int64_t blk = ((int64_t)tl.e * nb_n + min(tl.n0 / 128, nb_n - 1)) * nslab;
       const float *xs[kPer];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) xs[j] = p.xs + (int64_t)next_row[j] * nslab;
-      if (t + step < n_tiles) rows_of(t + step);
+      for (int j = 0; j < kPer; ++j) xs[j] = p.xs + (int64_t)s_row[tslot * S::kTok + c0 + 32 * j] * nslab;
       float v[4][kPer], w0[4], w1[4];
       auto fetch = [&](int k0) {
 #pragma unroll
@@ -544,55 +623,48 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           par ^= 1u;
         }
       }
+      if (!ok) break;
     }
   } else if (warp >= S::kRowWarp && warp < S::kRowWarp + S::kRowWarps) {
     // =========================== routed rows ===========================
     const int w = warp - S::kRowWarp;
-    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps), kSets = (kQuads + 7) / 8;   // copies of four rows per warp and stage
-    int st = 0, next_row[kSets], unused;
+    constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps);   // copies of four rows per warp and slab
+    int st = 0;
     uint32_t par = 1;
-    auto rows_of = [&](int t) {
-      const Tile tl = tile_at(t);
-      const int n_cta = columns(tl) / CG;
-#pragma unroll
-      for (int g = 0; g < kSets; ++g) {
-        // lane 4q + i finds row i of the warp's quad 8g + q
-        const int q = 8 * g + (lane >> 2), r = 4 * (w + S::kRowWarps * q) + (lane & 3);
-        next_row[g] = 0;
-        if (q < kQuads && r < n_cta) resolve(tl, (int)rank * n_cta + r, unused, next_row[g]);
-      }
-    };
-    if (first < n_tiles) rows_of(first);
-    for (int t = first; t < n_tiles && ok; t += step) {
-      const Tile tl = tile_at(t);
-      const int n_cta = columns(tl) / CG;
+    for (int t = first; t < n_tiles; t += step, tile_done()) {
+      Tile tl;
+      if (!tile_take(tl)) break;
+      const int n_cta = tl.ncol / CG;
       int4 rows[kQuads];
 #pragma unroll
       for (int q = 0; q < kQuads; ++q) {
-        rows[q].x = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8));
-        rows[q].y = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 1);
-        rows[q].z = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 2);
-        rows[q].w = __shfl_sync(0xffffffffu, next_row[q / 8], 4 * (q % 8) + 3);
+        const int r = 4 * (w + S::kRowWarps * q);
+        rows[q] = *reinterpret_cast<const int4 *>(s_row + tslot * S::kTok + (r < n_cta ? (int)rank * n_cta + r : 0));
       }
-      if (t + step < n_tiles) rows_of(t + step);
-      for (int ks = 0; ks < nslab; ++ks) {
+      for (int ks = 0; ks < nslab; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
         const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
-        const uint32_t dst = smem_u32(smem + S::kOffB + st * S::kBTile);
         if (elect_one()) {
-          if (p.dense) {
-            if (w == 0) tma_load_box<CG>(dst, &p.mapx, ks * S::kSlab, tl.tok0 + (int)rank * n_cta, bar);
-          } else {
 #pragma unroll
-            for (int q = 0; q < kQuads; ++q) {
-              const int r = 4 * (w + S::kRowWarps * q);
-              if (r < n_cta) tma_gather4<CG>(dst + r * 128, &p.mapx, ks * S::kSlab, rows[q], bar);
+          for (int u = 0; u < S::kSub; ++u) {
+            if (u > 0 && ks + u >= nslab) break;
+            const uint32_t dst = smem_u32(smem + S::kOffB + (st * S::kSub + u) * S::kBTile);
+            const int x = (ks + u) * S::kSlab;
+            if (p.dense) {
+              if (w == 0) tma_load_box<CG>(dst, &p.mapx, x, tl.tok0 + (int)rank * n_cta, bar);
+            } else {
+#pragma unroll
+              for (int q = 0; q < kQuads; ++q) {
+                const int r = 4 * (w + S::kRowWarps * q);
+                if (r < n_cta) tma_gather4<CG>(dst + r * 128, &p.mapx, x, rows[q], bar);
+              }
             }
           }
         }
         __syncwarp();
         if (++st == S::kStages) { st = 0; par ^= 1u; }
       }
+      if (!ok) break;
     }
   }
 
