@@ -38,7 +38,7 @@ struct GemmParams {
   int64_t ldo, idx_stride;
   int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles;
   uint32_t idesc_format;
-  int vec_out;                // 16-byte stores of 16-bit outputs
+  int vec_out;                // bases and strides of the outputs allow 16-byte (lane = row form: 32-byte) stores
   int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
   float out_scale;
   CUtensorMap map0, map1, mapx;
@@ -46,8 +46,10 @@ struct GemmParams {
 
 template <bool FP8, bool GATEUP, int CG>
 struct Shape {
-  static constexpr int kTok = CG == 2 ? 256 : 64;        // routed rows of a bucket (MMA N upper bound)
-  static constexpr int kTokStep = 16 * CG;               // bucket sizes are multiples of this
+  // e4m3 in pairs: the MMA's M side is the routed rows and its N side 256 matrix rows (of them 128 of gate and 128 of up)
+  static constexpr bool kRowsM = FP8 && CG == 2;
+  static constexpr int kTok = CG == 2 ? 256 : 64;        // routed rows of a bucket
+  static constexpr int kTokStep = kRowsM ? 8 : 16 * CG;  // bucket sizes are multiples of this
   static constexpr int kEpiWarps = CG == 2 ? 8 : 4;
   static constexpr int kMmaWarp = kEpiWarps, kMatWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
   static constexpr int kScaleWarps = CG == 2 ? 2 : 1;
@@ -59,16 +61,18 @@ struct Shape {
   static constexpr int kATile = 128 * 128;               // bytes: 128 matrix rows x 128 bytes of K
   static constexpr int kBTile = kTok / CG * 128;
   static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per slab
-  static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile
-  static constexpr int kVecs = GATEUP ? 2 : 1;
+  static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile (of a pair: kOuts * CG)
+  static constexpr int kBoxRows = GATEUP && !kRowsM ? 16 : 128;
+  static constexpr int kVecs = GATEUP || kRowsM ? 2 : 1; // scale vectors per block of K: gate and up, or two blocks of 128 outputs
+  static constexpr int kVecRows = kRowsM ? 128 : kTok;   // of this length: the routed rows that this CTA's epilogue sees
   static constexpr int kAccs = CG == 2 ? 2 : 4;          // accumulator buffers of kTok columns
   static constexpr int kScaleGroups = FP8 ? 2 : 0;       // ring of scale vectors, four blocks of K to a group
-  static constexpr int kScaleVec = kVecs * kTok * 4;
+  static constexpr int kScaleVec = kVecs * kVecRows * 4;
   static constexpr int kScaleGroup = 4 * kScaleVec;
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kSub * kATile;
   static constexpr int kOffScale = kOffB + kStages * kSub * kBTile;
-  static constexpr int kStage = 16 * 48;                 // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16
+  static constexpr int kStage = kRowsM ? 0 : 16 * 48;    // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16
   static constexpr int kOffStage = kOffScale + kScaleGroups * kScaleGroup;
   static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [kTiles][kTok] pair of each column
   static constexpr int kTiles = 3;                       // ring of tile descriptions
@@ -93,6 +97,22 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 // (a0, a1) += (x0 * s0, x1 * s1): the pairs stay in 64-bit registers, packed and unpacked they would cost more than the product
 __device__ __forceinline__ void fma2(unsigned long long &a, uint32_t x0, uint32_t x1, unsigned long long s) {
   asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}" : "+l"(a) : "r"(x0), "r"(x1), "l"(s));
+}
+
+// 32 bytes, one whole sector
+__device__ __forceinline__ void store_sector(float *at, const float *v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+// two values in the 16-bit type `dtype`
+__device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {
+  if (dtype == KNJ_DT_BF16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  }
+  const __half2 x = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&x);
 }
 
 template <bool FP8, bool GATEUP, int CG>
@@ -196,7 +216,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
         Tile r;
         r.e = lo;
-        r.n0 = (mt * CG + (int)rank) * S::kOuts;
+        r.n0 = (mt * CG + (S::kRowsM ? 0 : (int)rank)) * S::kOuts;
         r.tok0 = (b - s_pref[lo]) * per;
         ntok = min(per, cnt - r.tok0);
         r.ncol = (ntok + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
@@ -279,15 +299,6 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       // 16 bits: transposed through shared memory (stmatrix), so that whole sectors are written -- 16-byte pieces of a row from
       // two instructions made the stores of a tile of 256 columns take 28,000 cycles
       auto finish_16 = [&](const float (&v)[2][8], int c0) {
-        const bool bf16 = p.out_dtype == KNJ_DT_BF16;
-        auto pack = [&](float a, float b) {
-          if (bf16) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
-            return *reinterpret_cast<const uint32_t *>(&x);
-          }
-          const __half2 x = __floats2half2_rn(a, b);
-          return *reinterpret_cast<const uint32_t *>(&x);
-        };
         constexpr int kRow = GATEUP ? 32 : 64, kPitch = kRow + 16;          // bytes of a column's outputs
         constexpr int kCols = GATEUP ? 16 : 8;                              // columns per store of the warp
         uint8_t *stg = smem + S::kOffStage + warp * S::kStage;
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           for (int q = 0; q < 4; ++q) {
             // matrix q: 8 outputs x 8 columns
             const int g = GATEUP ? q >> 1 : i, h = GATEUP ? 0 : q >> 1, rr = q & 1;
-            m[q] = pack(v[h][4 * g + 2 * rr], v[h][4 * g + 2 * rr + 1]);
+            m[q] = pack16(p.out_dtype, v[h][4 * g + 2 * rr], v[h][4 * g + 2 * rr + 1]);
           }
           const int q = lane >> 3, c = (GATEUP ? 8 * (q >> 1) : 0) + (lane & 7);
           __syncwarp();
@@ -366,6 +377,100 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           finish(r[2], r[3], ch * 32 + 16);
         }
         release();
+      } else if constexpr (S::kRowsM) {
+        // Lane = routed row, so that a block's scale is one register (two for gate and up) and the loads take the 32-lane form, 935
+        // bytes a cycle; with lane = matrix row every thread has to fetch a scale for each of its columns, 1024 cycles of shared
+        // memory a block, or load in the 16-lane form, 524 cycles of tensor memory (the products take 512). Group g holds outputs
+        // 128 g .. + 127, or for gate and up the 64 outputs 64 g .. of both. The loads run one step of 16 columns ahead of the
+        // sums, across blocks of K too.
+        constexpr int kSteps = 8;
+        auto col_of = [&](int c) { return GATEUP ? (c >> 2) * 128 + group * 64 + (c & 3) * 16 : group * 128 + c * 16; };
+        const int local = quad * 32 + lane;
+        unsigned long long acc[kSteps][8];   // pairs of f32 sums
+        uint32_t r[2][16];
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[c][j] = 0ull;
+        if (!wait(&acc_full[buf], par)) break;
+        tc_fence_after();
+        tmem_ld_32x16(lanes + buf * S::kTok + col_of(0), r[0]);
+        for (int ks = 0; ks < nslab; ++ks) {
+          if ((ks & 3) == 0 && !wait(&sc_full[sg], sg_par)) break;
+          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + local;
+          unsigned long long s0, s1;
+          {
+            const uint32_t f0 = __float_as_uint(sc[GATEUP ? 0 : group * S::kVecRows]), f1 = GATEUP ? __float_as_uint(sc[S::kVecRows]) : f0;
+            asm("mov.b64 %0, {%1, %1};" : "=l"(s0) : "r"(f0));
+            asm("mov.b64 %0, {%1, %1};" : "=l"(s1) : "r"(f1));
+          }
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c) {
+            tmem_ld_wait(r[c & 1]);
+            if (c + 1 < kSteps) {
+              tmem_ld_32x16(lanes + buf * S::kTok + col_of(c + 1), r[(c + 1) & 1]);
+            } else {
+              release();
+              if (ks + 1 < nslab) {
+                if (!wait(&acc_full[buf], par)) break;
+                tc_fence_after();
+                tmem_ld_32x16(lanes + buf * S::kTok + col_of(0), r[0]);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fma2(acc[c][j], r[c & 1][2 * j], r[c & 1][2 * j + 1], GATEUP && c >= 4 ? s1 : s0);
+          }
+          if (!ok) break;
+          if ((ks & 3) == 3 || ks + 1 == nslab) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_empty[sg]);
+            if (++sg == S::kScaleGroups) {
+              sg = 0;
+              sg_par ^= 1u;
+            }
+          }
+        }
+        if (!ok) break;
+        const int n_cta = ncol / CG;
+        int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
+        if (pr != -1) {
+          const float scale = pr < 0 ? 0.f : p.out_scale;
+          if (pr < 0) pr = -2 - pr;
+          auto value = [&](int c, int j) {   // output 16 c + j of this thread's row
+            const unsigned long long w = acc[c][j >> 1];
+            return __uint_as_float((uint32_t)((j & 1) ? w >> 32 : w));
+          };
+          constexpr int kOut16 = GATEUP ? 4 : 8;   // runs of 16 outputs
+          const int nb = tl.n0 + group * (GATEUP ? 64 : 128);
+#pragma unroll
+          for (int c = 0; c < kOut16; ++c) {
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              f[j] = value(c, j);
+              if constexpr (GATEUP) f[j] = __fdividef(f[j], 1.0f + __expf(-f[j])) * value(c + 4, j);
+              f[j] = scale == 0.f ? 0.f : f[j] * scale;
+            }
+            const int n = nb + 16 * c;
+            if (n >= p.N) continue;
+            const int64_t at = pr * p.ldo + n;
+            if (p.vec_out && n + 16 <= p.N) {
+              if (p.out_dtype == KNJ_DT_F32) {
+                store_sector(static_cast<float *>(p.out) + at, f);
+                store_sector(static_cast<float *>(p.out) + at + 8, f + 8);
+              } else {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __uint_as_float(pack16(p.out_dtype, f[2 * j], f[2 * j + 1]));
+                store_sector(reinterpret_cast<float *>(static_cast<uint16_t *>(p.out) + at), w);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (n + j < p.N) store_from_f32(p.out, p.out_dtype, at + j, f[j]);
+            }
+          }
+        }
       } else {
         // One straight run of code for each number of chunks: with a branch around every chunk their loads could not be started in
         // front of each other's sums.
@@ -393,7 +498,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
                 const unsigned long long s0 = *reinterpret_cast<const unsigned long long *>(sc + col_of(c) + 8 * i);
-                const unsigned long long s1 = GATEUP ? *reinterpret_cast<const unsigned long long *>(sc + S::kTok + col_of(c) + 8 * i) : s0;
+                const unsigned long long s1 = GATEUP ? *reinterpret_cast<const unsigned long long *>(sc + S::kVecRows + col_of(c) + 8 * i) : s0;
 #pragma unroll
                 for (int rr = 0; rr < 2; ++rr) {
                   fma2(acc[c][0][2 * i + rr], r[c & 1][0][4 * i + 2 * rr], r[c & 1][0][4 * i + 2 * rr + 1], s0);
@@ -438,11 +543,18 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     for (; !ok && t < n_tiles; t += step) {
       int ntok;
       const Tile tl = tile_at(t, ntok);
-      const int n = tl.n0 + quad * (GATEUP ? 16 : 32) + lane;
-      for (int c = 0; c < ntok; ++c) {
-        if ((c / 32) % kGroups != group || n >= p.N || lane >= (GATEUP ? 16 : 32)) continue;
-        const int pr = pair_at(tl, ntok, c);
-        if (pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n, __int_as_float(0x7fffffff));
+      if constexpr (S::kRowsM) {
+        const int n_cta = tl.ncol / CG, local = quad * 32 + lane, pr = local < n_cta ? pair_at(tl, ntok, (int)rank * n_cta + local) : -1;
+        const int n = tl.n0 + group * S::kOuts;
+        for (int j = 0; j < S::kOuts && n + j < p.N; ++j)
+          if (pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n + j, __int_as_float(0x7fffffff));
+      } else {
+        const int n = tl.n0 + quad * (GATEUP ? 16 : 32) + lane;
+        for (int c = 0; c < ntok; ++c) {
+          if ((c / 32) % kGroups != group || n >= p.N || lane >= (GATEUP ? 16 : 32)) continue;
+          const int pr = pair_at(tl, ntok, c);
+          if (pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n, __int_as_float(0x7fffffff));
+        }
       }
     }
   } else if (warp == S::kMmaWarp) {
@@ -454,12 +566,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       for (int t = first; t < n_tiles; t += step, tile_done()) {
         Tile tl;
         if (!tile_take(tl)) break;
-        const uint32_t idesc = instr_desc_f16(128 * CG, tl.ncol) | p.idesc_format;
+        const uint32_t idesc = instr_desc_f16(128 * CG, S::kRowsM ? 256 : tl.ncol) | p.idesc_format;
         for (int ks = 0; ks < nslab; ks += S::kSub) {
           if ((FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
           if (!wait(&full[st], par)) break;
           tc_fence_after();
-          const uint64_t a = a_desc0 + (uint32_t)(st * S::kSub * S::kATile) / 16, b = b_desc0 + (uint32_t)(st * S::kSub * S::kBTile) / 16;
+          const uint64_t mat = a_desc0 + (uint32_t)(st * S::kSub * S::kATile) / 16, rows = b_desc0 + (uint32_t)(st * S::kSub * S::kBTile) / 16;
+          const uint64_t a = S::kRowsM ? rows : mat, b = S::kRowsM ? mat : rows;
           const bool last = FP8 || ks + S::kSub >= nslab;
           if (elect_one()) {
 #pragma unroll
@@ -536,7 +649,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         tslot = 0;
         tpar ^= 1u;
       }
-      const int y = tl.e * p.N + tl.n0;
+      const int y = tl.e * p.N + tl.n0 + (S::kRowsM && !GATEUP ? 128 * (int)rank : 0);
       // of both CTAs, matrix and rows, per slab
       const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : tl.ncol * 128));
       const bool more = t + step < n_tiles;
@@ -550,7 +663,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             if (u > 0 && ks + u >= nslab) break;
             const uint32_t dst = smem_u32(smem + S::kOffA + (st * S::kSub + u) * S::kATile);
             const int x = (ks + u) * S::kSlab;
-            if (GATEUP) {
+            if (S::kRowsM) {
+              tma_load_box<CG>(dst, GATEUP && rank ? &p.map1 : &p.map0, x, y, bar);
+            } else if (GATEUP) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 tma_load_box<CG>(dst + j * 4096, &p.map0, x, y + 16 * j, bar);
@@ -572,7 +687,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     // =========================== scales ===========================
     // Four blocks of K are read at once, as one 16-byte load a column where the rows of scales allow it, and the next four before
     // the ring is waited for.
-    constexpr int kPer = S::kTok / 32 / S::kScaleWarps;   // columns per lane
+    constexpr int kPer = S::kVecRows / 32 / S::kScaleWarps;   // rows per lane
     const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
     const bool quads = nslab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.xs) & 15) == 0;
     int sg = 0;
@@ -580,18 +695,26 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     for (int t = first; t < n_tiles; t += step, tile_done()) {
       Tile tl;
       if (!tile_take(tl)) break;
-      // a CTA behind the last output of a pair's tile has no block of its own: any block's scales do
-      const int64_t blk = ((int64_t)tl.e * nb_n + min(tl.n0 / 128, nb_n - 1)) * nslab;
+      // scales of block `blk` of matrix 0 and, for two vectors, of matrix 1 or of the next block; behind the last output there is no
+      // block: any one's scales do
+      const int blk = min(tl.n0 / 128, nb_n - 1);
+      const float *ws0 = p.ws0 + ((int64_t)tl.e * nb_n + blk) * nslab;
+      const float *ws1 = GATEUP ? p.ws1 + ((int64_t)tl.e * nb_n + blk) * nslab : p.ws0 + ((int64_t)tl.e * nb_n + min(blk + 1, nb_n - 1)) * nslab;
+      const int n_cta = tl.ncol / CG;
       const float *xs[kPer];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) xs[j] = p.xs + (int64_t)s_row[tslot * S::kTok + c0 + 32 * j] * nslab;
+      for (int j = 0; j < kPer; ++j) {
+        const int c = c0 + 32 * j;   // of the bucket, or in lane = row form of this CTA's part of it
+        const int at = S::kRowsM ? (c < n_cta ? (int)rank * n_cta + c : 0) : c;
+        xs[j] = p.xs + (int64_t)s_row[tslot * S::kTok + at] * nslab;
+      }
       float v[4][kPer], w0[4], w1[4];
       auto fetch = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int kb = min(k0 + i, nslab - 1);
-          w0[i] = p.ws0[blk + kb];
-          if (GATEUP) w1[i] = p.ws1[blk + kb];
+          w0[i] = ws0[kb];
+          if (S::kVecs == 2) w1[i] = ws1[kb];
         }
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -612,8 +735,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
-            dst[i * S::kVecs * S::kTok + 32 * j] = v[i][j] * w0[i];
-            if (GATEUP) dst[(2 * i + 1) * S::kTok + 32 * j] = v[i][j] * w1[i];
+            dst[i * S::kVecs * S::kVecRows + 32 * j] = v[i][j] * w0[i];
+            if (S::kVecs == 2) dst[(2 * i + 1) * S::kVecRows + 32 * j] = v[i][j] * w1[i];
           }
         if (k0 + 4 < nslab) fetch(k0 + 4);
         __syncwarp();
@@ -703,12 +826,13 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   }
   constexpr int esz = FP8 ? 1 : 2;
   const uint64_t w_rows = (uint64_t)p.E * p.N;
-  int rc = make_operand_tensor_map(&p.map0, o.w0, esz, p.K, p.K, w_rows, GATEUP ? 16 : 128);
-  if (!rc && GATEUP) rc = make_operand_tensor_map(&p.map1, o.w1, esz, p.K, p.K, w_rows, 16);
+  int rc = make_operand_tensor_map(&p.map0, o.w0, esz, p.K, p.K, w_rows, S::kBoxRows);
+  if (!rc && GATEUP) rc = make_operand_tensor_map(&p.map1, o.w1, esz, p.K, p.K, w_rows, S::kBoxRows);
   if (!rc) rc = make_operand_tensor_map(&p.mapx, o.x, esz, p.K, o.ldx, p.n_rows, p.dense ? S::kTok / CG : 1);
   if (rc) return rc;
   p.m_tiles = (p.N + S::kOuts * CG - 1) / (S::kOuts * CG);
-  p.vec_out = aligned16(p.out) && p.ldo % 8 == 0;
+  const int out_esz = p.out_dtype == KNJ_DT_F32 ? 4 : 2, unit = S::kRowsM ? 32 : 16;
+  p.vec_out = reinterpret_cast<uintptr_t>(p.out) % unit == 0 && p.ldo * out_esz % unit == 0;
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
   KNJ_REQUIRE(most * p.m_tiles < (1ll << 31) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
