@@ -65,7 +65,8 @@ struct Shape {
   static constexpr int kBoxRows = GATEUP && !kRowsM ? 16 : 128;
   static constexpr int kVecs = GATEUP || kRowsM ? 2 : 1; // scale vectors per block of K: gate and up, or two blocks of 128 outputs
   static constexpr int kVecRows = kRowsM ? 128 : kTok;   // of this length: the routed rows that this CTA's epilogue sees
-  static constexpr int kAccs = CG == 2 ? 2 : 4;          // accumulator buffers of kTok columns
+  static constexpr int kAccCols = kRowsM ? 128 : kTok;   // columns of an accumulator buffer
+  static constexpr int kAccs = CG == 2 && !kRowsM ? 2 : 4;
   static constexpr int kScaleGroups = FP8 ? 2 : 0;       // ring of scale vectors, four blocks of K to a group
   static constexpr int kScaleVec = kVecs * kVecRows * 4;
   static constexpr int kScaleGroup = 4 * kScaleVec;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     }
     for (int i = 0; i < S::kAccs; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], CG * S::kEpiWarps);
+      mbar_init(&acc_empty[i], CG * (S::kRowsM ? S::kEpiWarps / 2 : S::kEpiWarps));
     }
     for (int i = 0; i < S::kScaleGroups; ++i) {
       mbar_init(&sc_full[i], S::kScaleWarps);
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     *s_fail = 0;
     mbar_init_fence();
   }
-  constexpr uint32_t kTmemCols = S::kAccs * S::kTok;
+  constexpr uint32_t kTmemCols = S::kAccs * S::kAccCols;
   if (warp == S::kMmaWarp) {
     tmem_alloc<CG>(tmem_slot, kTmemCols);
     tmem_relinquish<CG>();
@@ -227,10 +228,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     return c < ntok ? (p.pair_idx ? p.pair_idx[tl.e * p.idx_stride + tl.tok0 + c] : tl.tok0 + c) : -1;
   };
   bool ok = true;  // once false this thread skips all work and waits but still meets every barrier
-  // e4m3 in pairs: the epilogue's sums take 128 registers a thread. 512 threads x 128 registers at launch = 2 x 128 x 192 + 2 x 128 x 64
+  // e4m3 in pairs: the epilogue's sums take 128 registers a thread. 512 threads x 128 registers at launch = 2 x 128 x 208 + 2 x 128 x 48
   if constexpr (FP8 && CG == 2) {
-    if (warp < S::kEpiWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < S::kEpiWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
   }
 
   // A warp waits, and goes on or gives up, as a whole. The loops of the issuing warps stay warp-uniform around the elected thread's
@@ -266,7 +267,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     const int group = warp >> 2, quad = warp & 3;
     constexpr int kGroups = S::kEpiWarps / 4, kChunks = S::kTok / 32 / kGroups;
     const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16);
-    int buf = 0, sg = 0;
+    constexpr int kBufStep = S::kRowsM ? 2 : 1;   // lane = routed row: each group has two of the four buffers
+    int buf = S::kRowsM ? group : 0, sg = 0;
     uint32_t par = 0, sg_par = 0;
     int t = first;
     for (; t < n_tiles; t += step, tile_done()) {
@@ -348,8 +350,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         else finish_16(v, c0);
       };
       auto load = [&](uint32_t (&lo)[8], uint32_t (&hi)[8], int col) {
-        tmem_ld_16x16(lanes + buf * S::kTok + col, lo);
-        tmem_ld_16x16(lanes + (16u << 16) + buf * S::kTok + col, hi);
+        tmem_ld_16x16(lanes + buf * S::kAccCols + col, lo);
+        tmem_ld_16x16(lanes + (16u << 16) + buf * S::kAccCols + col, hi);
       };
       auto release = [&] {
         tc_fence_before();
@@ -358,8 +360,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           if (CG == 2) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
           else mbar_arrive(&acc_empty[buf]);
         }
-        if (++buf == S::kAccs) {
-          buf = 0;
+        buf += kBufStep;
+        if (buf >= S::kAccs) {
+          buf -= S::kAccs;
           par ^= 1u;
         }
       };
@@ -378,13 +381,14 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         }
         release();
       } else if constexpr (S::kRowsM) {
-        // Lane = routed row, so that a block's scale is one register (two for gate and up) and the loads take the 32-lane form, 935
-        // bytes a cycle; with lane = matrix row every thread has to fetch a scale for each of its columns, 1024 cycles of shared
-        // memory a block, or load in the 16-lane form, 524 cycles of tensor memory (the products take 512). Group g holds outputs
-        // 128 g .. + 127, or for gate and up the 64 outputs 64 g .. of both. The loads run one step of 16 columns ahead of the
-        // sums, across blocks of K too.
+        // Lane = routed row, so that a block's scale is one register and the loads take the 32-lane form, 935 bytes a cycle; with lane
+        // = matrix row every thread has to fetch a scale for each of its columns, 1024 cycles of shared memory a block, or load in
+        // the 16-lane form, 524 cycles of tensor memory (the products take 512). A product is issued as two of 128 columns, 64 rows
+        // of each CTA's matrix tile, into buffers of their own: group g reads the buffers of half g, outputs 64 g .. + 63 of gate and
+        // of up, or of both blocks of 128 outputs. Whole products in two buffers left the tensor core waiting for the hand-offs
+        // (8192 x 4096 x 4096: 193 us). The loads run one step of 16 columns ahead of the sums, across blocks of K too.
         constexpr int kSteps = 8;
-        auto col_of = [&](int c) { return GATEUP ? (c >> 2) * 128 + group * 64 + (c & 3) * 16 : group * 128 + c * 16; };
+        auto col_of = [&](int c) { return c * 16; };
         const int local = quad * 32 + lane;
         unsigned long long acc[kSteps][8];   // pairs of f32 sums
         uint32_t r[2][16];
@@ -394,13 +398,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           for (int j = 0; j < 8; ++j) acc[c][j] = 0ull;
         if (!wait(&acc_full[buf], par)) break;
         tc_fence_after();
-        tmem_ld_32x16(lanes + buf * S::kTok + col_of(0), r[0]);
+        tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
         for (int ks = 0; ks < nslab; ++ks) {
           if ((ks & 3) == 0 && !wait(&sc_full[sg], sg_par)) break;
           const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + local;
           unsigned long long s0, s1;
           {
-            const uint32_t f0 = __float_as_uint(sc[GATEUP ? 0 : group * S::kVecRows]), f1 = GATEUP ? __float_as_uint(sc[S::kVecRows]) : f0;
+            const uint32_t f0 = __float_as_uint(sc[0]), f1 = __float_as_uint(sc[S::kVecRows]);
             asm("mov.b64 %0, {%1, %1};" : "=l"(s0) : "r"(f0));
             asm("mov.b64 %0, {%1, %1};" : "=l"(s1) : "r"(f1));
           }
@@ -408,17 +412,17 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           for (int c = 0; c < kSteps; ++c) {
             tmem_ld_wait(r[c & 1]);
             if (c + 1 < kSteps) {
-              tmem_ld_32x16(lanes + buf * S::kTok + col_of(c + 1), r[(c + 1) & 1]);
+              tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(c + 1), r[(c + 1) & 1]);
             } else {
               release();
               if (ks + 1 < nslab) {
                 if (!wait(&acc_full[buf], par)) break;
                 tc_fence_after();
-                tmem_ld_32x16(lanes + buf * S::kTok + col_of(0), r[0]);
+                tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
               }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fma2(acc[c][j], r[c & 1][2 * j], r[c & 1][2 * j + 1], GATEUP && c >= 4 ? s1 : s0);
+            for (int j = 0; j < 8; ++j) fma2(acc[c][j], r[c & 1][2 * j], r[c & 1][2 * j + 1], c >= 4 ? s1 : s0);
           }
           if (!ok) break;
           if ((ks & 3) == 3 || ks + 1 == nslab) {
@@ -441,7 +445,6 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             return __uint_as_float((uint32_t)((j & 1) ? w >> 32 : w));
           };
           constexpr int kOut16 = GATEUP ? 4 : 8;   // runs of 16 outputs
-          const int nb = tl.n0 + group * (GATEUP ? 64 : 128);
 #pragma unroll
           for (int c = 0; c < kOut16; ++c) {
             float f[16];
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
               if constexpr (GATEUP) f[j] = __fdividef(f[j], 1.0f + __expf(-f[j])) * value(c + 4, j);
               f[j] = scale == 0.f ? 0.f : f[j] * scale;
             }
-            const int n = nb + 16 * c;
+            const int n = tl.n0 + group * 64 + (c & 3) * 16 + (c >> 2) * 128;
             if (n >= p.N) continue;
             const int64_t at = pr * p.ldo + n;
             if (p.vec_out && n + 16 <= p.N) {
@@ -545,9 +548,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       const Tile tl = tile_at(t, ntok);
       if constexpr (S::kRowsM) {
         const int n_cta = tl.ncol / CG, local = quad * 32 + lane, pr = local < n_cta ? pair_at(tl, ntok, (int)rank * n_cta + local) : -1;
-        const int n = tl.n0 + group * S::kOuts;
-        for (int j = 0; j < S::kOuts && n + j < p.N; ++j)
-          if (pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n + j, __int_as_float(0x7fffffff));
+        for (int j = 0; j < S::kOuts; ++j) {
+          const int n = tl.n0 + group * 64 + (j & 63) + (j >> 6) * 128;
+          if (n < p.N && pr >= 0 && pr < p.n_pairs) store_from_f32(p.out, p.out_dtype, pr * p.ldo + n, __int_as_float(0x7fffffff));
+        }
       } else {
         const int n = tl.n0 + quad * (GATEUP ? 16 : 32) + lane;
         for (int c = 0; c < ntok; ++c) {
@@ -566,32 +570,51 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       for (int t = first; t < n_tiles; t += step, tile_done()) {
         Tile tl;
         if (!tile_take(tl)) break;
-        const uint32_t idesc = instr_desc_f16(128 * CG, S::kRowsM ? 256 : tl.ncol) | p.idesc_format;
+        const uint32_t idesc = instr_desc_f16(128 * CG, S::kRowsM ? 128 : tl.ncol) | p.idesc_format;
         for (int ks = 0; ks < nslab; ks += S::kSub) {
-          if ((FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
+          if (!S::kRowsM && (FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
           if (!wait(&full[st], par)) break;
           tc_fence_after();
           const uint64_t mat = a_desc0 + (uint32_t)(st * S::kSub * S::kATile) / 16, rows = b_desc0 + (uint32_t)(st * S::kSub * S::kBTile) / 16;
-          const uint64_t a = S::kRowsM ? rows : mat, b = S::kRowsM ? mat : rows;
-          const bool last = FP8 || ks + S::kSub >= nslab;
-          if (elect_one()) {
+          auto commit = [&](uint64_t *bar) {
+            if (CG == 2) tc_commit_pair(smem_u32(bar));
+            else tc_commit_addr<CG>(smem_u32(bar));
+          };
+          auto next_buf = [&] {
+            if (++buf == S::kAccs) { buf = 0; acc_par ^= 1u; }
+          };
+          if constexpr (S::kRowsM) {
 #pragma unroll
-            for (int u = 0; u < S::kSub; ++u) {
-              if (u > 0 && ks + u >= nslab) break;
+            for (int h = 0; h < 2; ++h) {
+              if (!wait(&acc_empty[buf], acc_par)) break;
+              tc_fence_after();
+              if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma<FP8, CG>(tmem_base + buf * S::kTok, a + u * (S::kATile / 16) + 2 * k, b + u * (S::kBTile / 16) + 2 * k, idesc,
-                             (u > 0 || k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) mma<FP8, CG>(tmem_base + buf * S::kAccCols, rows + 2 * k, mat + h * 512 + 2 * k, idesc, k > 0 ? 1u : 0u);
+                commit(&acc_full[buf]);
+                if (h == 1) commit(&empty[st]);
+              }
+              __syncwarp();
+              next_buf();
             }
-            if (CG == 2) tc_commit_pair(smem_u32(&empty[st]));
-            else tc_commit_addr<CG>(smem_u32(&empty[st]));
-            if (last) {
-              if (CG == 2) tc_commit_pair(smem_u32(&acc_full[buf]));
-              else tc_commit_addr<CG>(smem_u32(&acc_full[buf]));
+            if (!ok) break;
+          } else {
+            const bool last = FP8 || ks + S::kSub >= nslab;
+            if (elect_one()) {
+#pragma unroll
+              for (int u = 0; u < S::kSub; ++u) {
+                if (u > 0 && ks + u >= nslab) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma<FP8, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
+                               (u > 0 || k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+              }
+              commit(&empty[st]);
+              if (last) commit(&acc_full[buf]);
             }
+            __syncwarp();
+            if (last) next_buf();
           }
-          __syncwarp();
-          if (last && ++buf == S::kAccs) { buf = 0; acc_par ^= 1u; }
           if (++st == S::kStages) { st = 0; par ^= 1u; }
         }
         if (!ok) break;
