@@ -63,13 +63,12 @@ struct Shape {
   static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per slab
   static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile (of a pair: kOuts * CG)
   static constexpr int kBoxRows = GATEUP && !kRowsM ? 16 : 128;
-  static constexpr int kVecs = GATEUP || kRowsM ? 2 : 1; // scale vectors per block of K: gate and up, or two blocks of 128 outputs
-  static constexpr int kVecRows = kRowsM ? 128 : kTok;   // of this length: the routed rows that this CTA's epilogue sees
+  static constexpr int kVecs = GATEUP || kRowsM ? 2 : 1; // matrix scales per block of K: gate and up, or two blocks of 128 outputs
+  static constexpr int kVecRows = kRowsM ? 128 : kTok;   // the routed rows that this CTA's epilogue sees
   static constexpr int kAccCols = kRowsM ? 128 : kTok;   // columns of an accumulator buffer
   static constexpr int kAccs = CG == 2 && !kRowsM ? 2 : 4;
-  static constexpr int kScaleGroups = FP8 ? 2 : 0;       // ring of scale vectors, four blocks of K to a group
-  static constexpr int kScaleVec = kVecs * kVecRows * 4;
-  static constexpr int kScaleGroup = 4 * kScaleVec;
+  static constexpr int kScaleGroups = FP8 ? 4 : 0;       // ring of scales, four blocks of K to a group
+  static constexpr int kScaleGroup = 4 * kVecRows * 4 + 32;   // [4][kVecRows] of the rows, [4][2] of the matrix blocks
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kSub * kATile;
   static constexpr int kOffScale = kOffB + kStages * kSub * kBTile;
@@ -88,18 +87,39 @@ struct Tile {
   int e, n0, ncol, tok0;   // expert, first output of the CTA, columns (routed rows, rounded up), first pair of the bucket
 };
 
-// one MMA's K step is 32 bytes of every operand row in both element sizes
-template <bool FP8, int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  if constexpr (FP8) tc_mma_f8<CG>(d, a, b, idesc, acc);
-  else tc_mma_f16<CG>(d, a, b, idesc, acc);
-}
-
 // (a0, a1) += (x0 * s0, x1 * s1): the pairs stay in 64-bit registers, packed and unpacked they would cost more than the product
 __device__ __forceinline__ void fma2(unsigned long long &a, uint32_t x0, uint32_t x1, unsigned long long s) {
   asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tfma.rn.f32x2 %0, x, %3, %0;\n\t}" : "+l"(a) : "r"(x0), "r"(x1), "l"(s));
 }
 
+// whether the phase is complete, without waiting and without ordering: who acts on it fences or waits
+__device__ __forceinline__ bool mbar_ask(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity));
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long twice(float f) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(f)));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// four bytes to shared memory by an asynchronous copy; cp_async_arrive: an arrival at the barrier once this thread's copies are there
+__device__ __forceinline__ void cp_async4(const void *dst_smem, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // 32 bytes, one whole sector
 __device__ __forceinline__ void store_sector(float *at, const float *v) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
@@ -132,8 +152,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   uint64_t *acc_full = empty + S::kStages;      // [kAccs] accumulator buffer complete
   uint64_t *acc_empty = acc_full + S::kAccs;    // [kAccs] accumulator buffer read (the even CTA's are used)
   uint64_t *sc_full = acc_empty + S::kAccs;     // [kScaleGroups]
-  uint64_t *sc_empty = sc_full + 2;
-  uint64_t *tile_full = sc_empty + 2;           // [kTiles] the tile's description is there
+  uint64_t *sc_empty = sc_full + 4;
+  uint64_t *tile_full = sc_empty + 4;           // [kTiles] the tile's description is there
   uint64_t *tile_empty = tile_full + S::kTiles; // [kTiles] every warp is done with it
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tile_empty + S::kTiles);
   volatile int *s_fail = reinterpret_cast<volatile int *>(tmem_slot + 1);  // raised by the first wait that gives up
@@ -152,7 +172,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       mbar_init(&acc_empty[i], CG * (S::kRowsM ? S::kEpiWarps / 2 : S::kEpiWarps));
     }
     for (int i = 0; i < S::kScaleGroups; ++i) {
-      mbar_init(&sc_full[i], S::kScaleWarps);
+      mbar_init(&sc_full[i], 32 * S::kScaleWarps);
       mbar_init(&sc_empty[i], S::kEpiWarps);
     }
     for (int i = 0; i < S::kTiles; ++i) {
@@ -386,7 +406,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         // the 16-lane form, 524 cycles of tensor memory (the products take 512). A product is issued as two of 128 columns, 64 rows
         // of each CTA's matrix tile, into buffers of their own: group g reads the buffers of half g, outputs 64 g .. + 63 of gate and
         // of up, or of both blocks of 128 outputs. Whole products in two buffers left the tensor core waiting for the hand-offs
-        // (8192 x 4096 x 4096: 193 us). The loads run one step of 16 columns ahead of the sums, across blocks of K too.
+        // (8192 x 4096 x 4096: 193 us). The loads run one step of 16 columns ahead of the sums, across blocks of K too,
+        // and whether the next buffer is complete is asked two steps before it is needed.
         constexpr int kSteps = 8;
         auto col_of = [&](int c) { return c * 16; };
         const int local = quad * 32 + lane;
@@ -401,22 +422,24 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
         for (int ks = 0; ks < nslab; ++ks) {
           if ((ks & 3) == 0 && !wait(&sc_full[sg], sg_par)) break;
-          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + local;
-          unsigned long long s0, s1;
-          {
-            const uint32_t f0 = __float_as_uint(sc[0]), f1 = __float_as_uint(sc[S::kVecRows]);
-            asm("mov.b64 %0, {%1, %1};" : "=l"(s0) : "r"(f0));
-            asm("mov.b64 %0, {%1, %1};" : "=l"(s1) : "r"(f1));
-          }
+          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup);
+          const float sx = sc[(ks & 3) * S::kVecRows + local];
+          const float2 sw = *reinterpret_cast<const float2 *>(sc + 4 * S::kVecRows + 2 * (ks & 3));
+          const unsigned long long s0 = twice(sx * sw.x), s1 = twice(sx * sw.y);
+          bool ready = false;
 #pragma unroll
           for (int c = 0; c < kSteps; ++c) {
             tmem_ld_wait(r[c & 1]);
+            if (c + 2 == kSteps) {
+              const int nb = buf + kBufStep < S::kAccs ? buf + kBufStep : buf + kBufStep - S::kAccs;
+              ready = mbar_ask(&acc_full[nb], nb < buf ? par ^ 1u : par);
+            }
             if (c + 1 < kSteps) {
               tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(c + 1), r[(c + 1) & 1]);
             } else {
               release();
               if (ks + 1 < nslab) {
-                if (!wait(&acc_full[buf], par)) break;
+                if (!__all_sync(0xffffffffu, ready) && !wait(&acc_full[buf], par)) break;
                 tc_fence_after();
                 tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
               }
@@ -491,7 +514,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             if ((ks & 3) == 0) wait(&sc_full[sg], sg_par);
             if (!wait(&acc_full[buf], par)) return;
             tc_fence_after();
-            const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup + (ks & 3) * S::kScaleVec) + 2 * (lane & 3);
+            const float *sg_at = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup);
+            const float *sc = sg_at + (ks & 3) * S::kVecRows + 2 * (lane & 3);
+            const float2 sw = *reinterpret_cast<const float2 *>(sg_at + 4 * S::kVecRows + 2 * (ks & 3));
+            const unsigned long long w0 = twice(sw.x), w1 = twice(sw.y);
             uint32_t r[2][2][8];
             if constexpr (kSteps > 0) load(r[0][0], r[0][1], col_of(0));
 #pragma unroll
@@ -500,8 +526,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
               if (c + 1 < kSteps) load(r[(c + 1) & 1][0], r[(c + 1) & 1][1], col_of(c + 1));
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const unsigned long long s0 = *reinterpret_cast<const unsigned long long *>(sc + col_of(c) + 8 * i);
-                const unsigned long long s1 = GATEUP ? *reinterpret_cast<const unsigned long long *>(sc + S::kVecRows + col_of(c) + 8 * i) : s0;
+                const unsigned long long sx = *reinterpret_cast<const unsigned long long *>(sc + col_of(c) + 8 * i);
+                const unsigned long long s0 = mul2(sx, w0), s1 = GATEUP ? mul2(sx, w1) : s0;
 #pragma unroll
                 for (int rr = 0; rr < 2; ++rr) {
                   fma2(acc[c][0][2 * i + rr], r[c & 1][0][4 * i + 2 * rr], r[c & 1][0][4 * i + 2 * rr + 1], s0);
@@ -590,7 +616,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
               tc_fence_after();
               if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma<FP8, CG>(tmem_base + buf * S::kAccCols, rows + 2 * k, mat + h * 512 + 2 * k, idesc, k > 0 ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) tc_mma<FP8, CG>(tmem_base + buf * S::kAccCols, rows + 2 * k, mat + h * 512 + 2 * k, idesc, k > 0 ? 1u : 0u);
                 commit(&acc_full[buf]);
                 if (h == 1) commit(&empty[st]);
               }
@@ -606,7 +632,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
                 if (u > 0 && ks + u >= nslab) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma<FP8, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
+                  tc_mma<FP8, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
                                (u > 0 || k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
               }
               commit(&empty[st]);
@@ -708,21 +734,19 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     }
   } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
     // =========================== scales ===========================
-    // Four blocks of K are read at once, as one 16-byte load a column where the rows of scales allow it, and the next four before
-    // the ring is waited for.
+    // Asynchronous copies of four bytes, four blocks of K to a group: read into registers, a group had to wait for its loads, and an
+    // L2 or HBM latency for four blocks set the pace (8192 x 4096 x 4096: 166 us beside SCALES_NOW).
     constexpr int kPer = S::kVecRows / 32 / S::kScaleWarps;   // rows per lane
     const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
-    const bool quads = nslab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.xs) & 15) == 0;
     int sg = 0;
     uint32_t par = 1;
     for (int t = first; t < n_tiles; t += step, tile_done()) {
       Tile tl;
       if (!tile_take(tl)) break;
-      // scales of block `blk` of matrix 0 and, for two vectors, of matrix 1 or of the next block; behind the last output there is no
-      // block: any one's scales do
-      const int blk = min(tl.n0 / 128, nb_n - 1);
-      const float *ws0 = p.ws0 + ((int64_t)tl.e * nb_n + blk) * nslab;
-      const float *ws1 = GATEUP ? p.ws1 + ((int64_t)tl.e * nb_n + blk) * nslab : p.ws0 + ((int64_t)tl.e * nb_n + min(blk + 1, nb_n - 1)) * nslab;
+      // scales of block `blk` of matrix 0 and, for two, of matrix 1 or of the next block; behind the last output there is no block:
+      // any one's scales do. Lanes 0..3: the first, lanes 4..7 the second, block of K lane % 4.
+      const int blk = min(tl.n0 / 128, nb_n - 1), second = lane >> 2 & 1;
+      const float *ws = (GATEUP && second ? p.ws1 : p.ws0) + ((int64_t)tl.e * nb_n + (GATEUP || !second ? blk : min(blk + 1, nb_n - 1))) * nslab + (lane & 3);
       const int n_cta = tl.ncol / CG;
       const float *xs[kPer];
 #pragma unroll
@@ -731,39 +755,17 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         const int at = S::kRowsM ? (c < n_cta ? (int)rank * n_cta + c : 0) : c;
         xs[j] = p.xs + (int64_t)s_row[tslot * S::kTok + at] * nslab;
       }
-      float v[4][kPer], w0[4], w1[4];
-      auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kb = min(k0 + i, nslab - 1);
-          w0[i] = ws0[kb];
-          if (S::kVecs == 2) w1[i] = ws1[kb];
-        }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          if (quads) {
-            const float4 f = *reinterpret_cast<const float4 *>(xs[j] + k0);
-            v[0][j] = f.x; v[1][j] = f.y; v[2][j] = f.z; v[3][j] = f.w;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i][j] = xs[j][min(k0 + i, nslab - 1)];
-          }
-        }
-      };
-      fetch(0);
       for (int k0 = 0; k0 < nslab; k0 += 4) {
         if (!wait(&sc_empty[sg], par)) break;
-        float *dst = reinterpret_cast<float *>(smem + S::kOffScale + sg * S::kScaleGroup) + c0;
+        float *dst = reinterpret_cast<float *>(smem + S::kOffScale + sg * S::kScaleGroup);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
+          if (k0 + i < nslab) {
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            dst[i * S::kVecs * S::kVecRows + 32 * j] = v[i][j] * w0[i];
-            if (S::kVecs == 2) dst[(2 * i + 1) * S::kVecRows + 32 * j] = v[i][j] * w1[i];
+            for (int j = 0; j < kPer; ++j) cp_async4(dst + i * S::kVecRows + c0 + 32 * j, xs[j] + k0 + i);
           }
-        if (k0 + 4 < nslab) fetch(k0 + 4);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_full[sg]);
+        if (warp == S::kScaleWarp && lane < 4 * S::kVecs && k0 + (lane & 3) < nslab) cp_async4(dst + 4 * S::kVecRows + 2 * (lane & 3) + second, ws + k0);
+        cp_async_arrive(&sc_full[sg]);
         if (++sg == S::kScaleGroups) {
           sg = 0;
           par ^= 1u;
@@ -771,6 +773,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       }
       if (!ok) break;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= S::kRowWarp && warp < S::kRowWarp + S::kRowWarps) {
     // =========================== routed rows ===========================
     const int w = warp - S::kRowWarp;

@@ -174,25 +174,19 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :);
 }
-// D(tmem) (+)= A(smem desc) * B(smem desc), e4m3 operands, f32 accumulate
-template <int CG>
-__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t zero = 0;
-  if (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(zero), "r"(zero), "r"(zero), "r"(zero)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(zero), "r"(zero), "r"(zero), "r"(zero), "r"(zero),
-          "r"(zero), "r"(zero), "r"(zero)
-        : "memory");
+// D(tmem) (+)= A(smem desc) * B(smem desc), f16 / bf16 (by the instruction descriptor) or e4m3 operands, f32 accumulate, every
+// lane of D written: without the operands of the lane mask, which the issuing thread would have to bring into place each time
+template <bool FP8, int CG>
+__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+#define KNJ_TC_MMA(GROUP, KIND)                                                                                                       \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
+               ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                                       \
+               : "memory")
+  if constexpr (FP8 && CG == 1) KNJ_TC_MMA("1", "f8f6f4");
+  else if constexpr (FP8) KNJ_TC_MMA("2", "f8f6f4");
+  else if constexpr (CG == 1) KNJ_TC_MMA("1", "f16");
+  else KNJ_TC_MMA("2", "f16");
+#undef KNJ_TC_MMA
 }
 // one box of rows out of a matrix (x = first element, y = first row) into this CTA's swizzled tile; the bytes count on the
 // barrier at `bar_addr`, which in a pair may be the peer's
