@@ -6,7 +6,6 @@
 // The reference's rows (src/model/model.cpp:258-271 rmsnorm_rows, :652 residual add) are the case y = NULL and the case
 // without weights and gate.
 #include "knj_fp8.cuh"
-#include <stdlib.h>
 
 using namespace knj;
 
@@ -18,7 +17,7 @@ struct NormParams {
   float *h_scale;
   int64_t ldx, ldy, ldg, ld_stream, ldh;
   int T, H, x_dtype, y_dtype, w_dtype, gate_dtype, gate_kind, gate_sigmoid, stream_dtype, h_dtype;
-  float alpha, beta, eps;
+  float alpha, beta, eps, inv_h;
 };
 
 __device__ __forceinline__ float gate_value(const NormParams &p, int64_t i) {
@@ -39,10 +38,11 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 // 1 / sqrt(mean square + eps) of a row whose sum of squares is `tot`. Where the squares of a large row leave the f32 range
 // they are summed once more from values * 2^-64 (`again`); eps does not count there.
 constexpr float kDown = 0x1p-64f;
+// rsqrtf is off by 2 units in the last place; an IEEE root and two divisions are a hundred instructions of every thread and row.
 template <class Again>
-__device__ __forceinline__ float rms_inverse(float tot, int H, float eps, Again again) {
-  if (tot <= 3.402823466e38f || tot != tot) return 1.0f / sqrtf(tot / (float)H + eps);
-  return kDown / sqrtf(again() / (float)H);
+__device__ __forceinline__ float rms_inverse(float tot, float inv_h, float eps, Again again) {
+  if (tot <= 3.402823466e38f || tot != tot) return rsqrtf(fmaf(tot, inv_h, eps));
+  return kDown * rsqrtf(again() * inv_h);
 }
 
 // ---- rows whose strides and bases are whole 16-byte units, H a multiple of 8 ----------------------------------------
@@ -126,120 +126,234 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float &scale) {
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
-// TPR threads per row (a warp, or the CTA's 256), thread i holds the elements 8 (i + TPR c) .. + 7, c < NC, of the row in
-// registers: one pass over memory, the loads of all chunks under way before the first sum. Bound by HBM from a few hundred rows on
-// and by two dependent sums and the launch below that.
-template <int TPR, int NC, bool XW, int Y>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) block_norm_vec_kernel(const NormParams p) {
-  __shared__ float red[8];
+// sum over the CTA; `red` has two rows of 16 (zero behind the CTA's warps), used in turn, so that one barrier a sum is enough
+__device__ __forceinline__ float cta_sum(float v, float (*red)[16], int &turn) {
+  v = warp_sum(v);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  float *at = red[turn];
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const float4 *q = reinterpret_cast<const float4 *>(at);
+  float4 a = q[0], b = q[1];
+  if (warps > 8) {
+    const float4 c = q[2], d = q[3];
+    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+    b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+  }
+  return ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
+}
+
+// One CTA walks over rows; thread i holds the elements 8 (i + blockDim c) .. + 7, c < NC, of each, and of the weights: post_w with a
+// gate per channel and alpha folded in, so that a row costs a dozen operations a value (formed anew for each row, and with the
+// gate's exponential, 57: 16384 rows of 2048 took 106 us, issue slots half full). RING: the next rows travel through a ring of
+// `depth` rows in shared memory, bulk copies on a barrier each; a row ahead in registers was 24 KB under way per SM, too few for
+// HBM (74 us). Without it, one row per CTA straight into registers: bound by the launch and two dependent sums.
+constexpr int kMaxRing = 8;
+template <int NC, bool XW, int Y, bool RING>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
+__global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(const NormParams p, const int depth) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(16) float red[2][16];
+  __shared__ uint64_t bars[kMaxRing];
+  __shared__ volatile int s_fail;
+  int turn = 0;
+  if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
+  __syncthreads();
   grid_dep_wait();
-  const int tid = threadIdx.x, i0 = TPR == 32 ? tid & 31 : tid;
-  const int64_t t = TPR == 32 ? (int64_t)blockIdx.x * 8 + (tid >> 5) : blockIdx.x;
-  if (TPR == 32 && t >= p.T) return;
-  auto row_sum = [&](float v) {
-    if constexpr (TPR == 32) return warp_sum(v);
-    else return block_sum(v, red);
-  };
-  const int H8 = p.H >> 3;
+  const int tid = threadIdx.x, step = blockDim.x, H8 = p.H >> 3;
+  const bool xb = p.x_dtype == KNJ_DT_BF16, yb = p.y_dtype == KNJ_DT_BF16;
   Raw8 xr[NC], yr[NC];
+  const int x_bytes = p.H * (XW ? 4 : 2), y_bytes = Y == 0 ? 0 : p.H * (Y == 2 ? 4 : 2);
+  auto send = [&](int slot, int64_t t) {   // one thread
+    uint8_t *at = ring + (size_t)slot * (x_bytes + y_bytes);
+    mbar_expect_tx(&bars[slot], (uint32_t)(x_bytes + y_bytes));
+    bulk_g2s(at, static_cast<const uint8_t *>(p.x) + t * p.ldx * (XW ? 4 : 2), (uint32_t)x_bytes, &bars[slot]);
+    if (Y != 0) bulk_g2s(at + x_bytes, static_cast<const uint8_t *>(p.y) + t * p.ldy * (Y == 2 ? 4 : 2), (uint32_t)y_bytes, &bars[slot]);
+  };
+  auto fetch = [&](const void *x, const void *y, int64_t xo, int64_t yo) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int i = i0 + TPR * c;
-    if (i < H8) {
-      xr[c] = load_raw8<XW>(p.x, t * p.ldx + 8 * i);
-      if constexpr (Y != 0) yr[c] = load_raw8<Y == 2>(p.y, t * p.ldy + 8 * i);
+    for (int c = 0; c < NC; ++c) {
+      const int i = tid + step * c;
+      if (i < H8) {
+        xr[c] = load_raw8<XW>(x, xo + 8 * i);
+        if constexpr (Y != 0) yr[c] = load_raw8<Y == 2>(y, yo + 8 * i);
+      }
+    }
+  };
+  if constexpr (RING) {
+    if (tid == 0) {
+      for (int r = 0; r < depth; ++r) mbar_init(&bars[r], 1);
+      s_fail = 0;
+      mbar_init_fence();
+      int64_t t = blockIdx.x;
+      for (int r = 0; r < depth && t < p.T; ++r, t += gridDim.x) send(r, t);
+    }
+    __syncthreads();
+  } else {
+    fetch(p.x, p.y, blockIdx.x * p.ldx, blockIdx.x * p.ldy);
+  }
+  // alpha * post_w * gate per channel, and pre_w; kept in registers where they fit, else formed for each row
+  auto post_of = [&](int c, float (&f)[8]) {
+    const int i = tid + step * c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p.alpha;
+    if (Y == 0 || i >= H8) return;
+    float w[8];
+    if (p.post_w) {
+      load8(p.post_w, p.w_dtype, 8 * i, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= w[j];
+    }
+    if (p.gate_kind == KNJ_GATE_CHANNEL) {
+      load8(p.gate, p.gate_dtype, 8 * i, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[j])) : w[j];
+    }
+  };
+  auto pre_of = [&](int c, float (&f)[8]) {
+    const int i = tid + step * c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    if (p.h && i < H8) load8(p.pre_w, p.w_dtype, 8 * i, f);
+  };
+  constexpr bool kKeep = NC <= 2;
+  float post[kKeep ? NC : 1][8], pre[kKeep ? NC : 1][8];
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      post_of(c, post[c]);
+      pre_of(c, pre[c]);
     }
   }
-  float rs = 1.f;
-  if (Y != 0 && p.post_w) {
-    auto squares = [&](float down) {
-      float ss = 0.f;
+  const int groups = (p.H + kFp8Group - 1) / kFp8Group;
+  int slot = 0;
+  uint32_t phase = 0;
+  // where this thread's first run of the row lies in what is written, moved on row by row
+  const int s_esz = p.stream_dtype == KNJ_DT_F32 ? 4 : 2, h_esz = p.h_dtype == KNJ_DT_E4M3 ? 1 : p.h_dtype == KNJ_DT_F32 ? 4 : 2;
+  uint8_t *s_at = static_cast<uint8_t *>(p.stream) + (blockIdx.x * p.ld_stream + 8 * tid) * s_esz;
+  uint8_t *h_at = static_cast<uint8_t *>(p.h) + (blockIdx.x * p.ldh + 8 * tid) * h_esz;
+  const int64_t s_step = gridDim.x * p.ld_stream * s_esz, h_step = gridDim.x * p.ldh * h_esz;
+  for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step) {
+    float s[NC][8], n[NC][8];
+    bool landed = true;
+    if constexpr (RING) {
+      landed = mbar_wait(&bars[slot], phase, &s_fail);
+      const uint8_t *at = ring + (size_t)slot * (x_bytes + y_bytes);
+      fetch(at, at + x_bytes, 0, 0);
+    }
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (i0 + TPR * c < H8) {
-          float v[8];
-          values8<Y == 2>(yr[c], p.y_dtype == KNJ_DT_BF16, v);
+    for (int c = 0; c < NC; ++c) {
+      const bool in = tid + step * c < H8;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ss = fmaf(v[j] * down, v[j] * down, ss);
-        }
+      for (int j = 0; j < 8; ++j) s[c][j] = n[c][j] = 0.f;
+      if (in) values8<XW>(xr[c], xb, s[c]);
+      if (Y != 0 && in) values8<Y == 2>(yr[c], yb, n[c]);
+    }
+    if constexpr (RING) {
+      if (!landed) s[0][0] = __int_as_float(0x7fffffff);   // a wait gave up: the row's outputs are NaN
+      __syncthreads();                                     // every thread has its part of the row
+      if (tid == 0 && t + (int64_t)depth * gridDim.x < p.T) {
+        fence_proxy_async();                               // the slot was read through the generic proxy
+        send(slot, t + (int64_t)depth * gridDim.x);
       }
-      return row_sum(ss);
-    };
-    rs = rms_inverse(squares(1.f), p.H, p.eps, [&] { return squares(kDown); });
-  }
-  float gr = 1.f;
-  if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) gr = gate_value(p, t * p.ldg);
-  float s[NC][8], ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int i = i0 + TPR * c;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[c][j] = 0.f;
-    if (i < H8) {
-      values8<XW>(xr[c], p.x_dtype == KNJ_DT_BF16, s[c]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[c][j] *= p.beta;
-      if constexpr (Y != 0) {
-        float n[8], w[8];
-        values8<Y == 2>(yr[c], p.y_dtype == KNJ_DT_BF16, n);
-        if (p.post_w) {
-          load8(p.post_w, p.w_dtype, 8 * i, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) n[j] *= rs * w[j];
-        }
-        if (p.gate_kind == KNJ_GATE_CHANNEL || p.gate_kind == KNJ_GATE_FULL) {
-          load8(p.gate, p.gate_dtype, (p.gate_kind == KNJ_GATE_FULL ? t * p.ldg : 0) + 8 * i, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) n[j] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[j])) : w[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) n[j] *= gr;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[c][j] = fmaf(p.alpha, n[j], s[c][j]);
+      if (++slot == depth) {
+        slot = 0;
+        phase ^= 1u;
       }
-      if (p.stream) store8(p.stream, p.stream_dtype, t * p.ld_stream + 8 * i, s[c]);
+    }
+    float rs = 1.f;
+    if (Y != 0 && p.post_w) {
+      auto squares = [&](float down) {
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = fmaf(n[c][j] * down, n[c][j] * down, ss);
+        return cta_sum(ss, red, turn);
+      };
+      rs = rms_inverse(squares(1.f), p.inv_h, p.eps, [&] { return squares(kDown); });
+    }
+    if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int i = tid + step * c;
+      if (!kKeep) post_of(c, post[0]);
+      if (i < H8) {
+        if (Y != 0 && p.gate_kind == KNJ_GATE_FULL) {
+          float w[8];
+          load8(p.gate, p.gate_dtype, t * p.ldg + 8 * i, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) n[c][j] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[j])) : w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          s[c][j] *= p.beta;
+          if constexpr (Y != 0) s[c][j] = fmaf(n[c][j] * rs, post[kKeep ? c : 0][j], s[c][j]);
+        }
+        if (p.stream) store8(s_at + 8 * step * c * s_esz, p.stream_dtype, 0, s[c]);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(s[c][j], s[c][j], ss);
     }
-  }
-  if (!p.h) return;
-  const float hs = rms_inverse(row_sum(ss), p.H, p.eps, [&] {
-    float q = 0.f;
+    if (!p.h) continue;
+    const float hs = rms_inverse(cta_sum(ss, red, turn), p.inv_h, p.eps, [&] {
+      float q = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q = fmaf(s[c][j] * kDown, s[c][j] * kDown, q);
-    return row_sum(q);
-  });
+        for (int j = 0; j < 8; ++j) q = fmaf(s[c][j] * kDown, s[c][j] * kDown, q);
+      return cta_sum(q, red, turn);
+    });
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int i = i0 + TPR * c;
-    if (i < H8) {
-      float w[8];
-      load8(p.pre_w, p.w_dtype, 8 * i, w);
+    for (int c = 0; c < NC; ++c) {
+      const int i = tid + step * c;
+      if (!kKeep) pre_of(c, pre[0]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[c][j] *= hs * w[j];
-      if (p.h_dtype != KNJ_DT_E4M3) store8(p.h, p.h_dtype, t * p.ldh + 8 * i, s[c]);
-    }
-    if (p.h_dtype == KNJ_DT_E4M3) {
-      float scale;
-      const uint2 q = codes8(s[c], scale);   // every lane takes part; lanes behind the row hold zeros
-      if (i < H8) *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p.h) + t * p.ldh + 8 * i) = q;
-      if (i < H8 && (i & 15) == 0) p.h_scale[t * ((p.H + kFp8Group - 1) / kFp8Group) + (i >> 4)] = scale;
+      for (int j = 0; j < 8; ++j) s[c][j] *= hs * pre[kKeep ? c : 0][j];   // zeros behind the row
+      if (p.h_dtype != KNJ_DT_E4M3) {
+        if (i < H8) store8(h_at + 8 * step * c * h_esz, p.h_dtype, 0, s[c]);
+      } else {
+        float scale;
+        const uint2 q = codes8(s[c], scale);   // every lane takes part
+        if (i < H8) *reinterpret_cast<uint2 *>(h_at + 8 * step * c) = q;
+        if (i < H8 && (i & 15) == 0) p.h_scale[t * groups + (i >> 4)] = scale;
+      }
     }
   }
 }
 
-template <int TPR, int NC>
-cudaError_t launch_vec(const NormParams &p, cudaStream_t st) {
+template <int NC, bool RING>
+cudaError_t launch_vec(const NormParams &p, int threads, unsigned ctas, int depth, size_t smem, cudaStream_t st) {
   auto go = [&](auto kern) {
-    return launch_chain(kern, dim3((unsigned)(TPR == 32 ? (p.T + 7) / 8 : p.T)), dim3(TPR == 32 ? 256 : TPR), 0, st, p);
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+      if (e != cudaSuccess) return e;
+    }
+    return launch_chain(kern, dim3(ctas), dim3(threads), smem, st, p, depth);
   };
   const bool xw = p.x_dtype == KNJ_DT_F32;
-  if (!p.y) return xw ? go(block_norm_vec_kernel<TPR, NC, true, 0>) : go(block_norm_vec_kernel<TPR, NC, false, 0>);
-  if (p.y_dtype != KNJ_DT_F32) return xw ? go(block_norm_vec_kernel<TPR, NC, true, 1>) : go(block_norm_vec_kernel<TPR, NC, false, 1>);
-  return xw ? go(block_norm_vec_kernel<TPR, NC, true, 2>) : go(block_norm_vec_kernel<TPR, NC, false, 2>);
+  if (!p.y) return xw ? go(block_norm_vec_kernel<NC, true, 0, RING>) : go(block_norm_vec_kernel<NC, false, 0, RING>);
+  if (p.y_dtype != KNJ_DT_F32) return xw ? go(block_norm_vec_kernel<NC, true, 1, RING>) : go(block_norm_vec_kernel<NC, false, 1, RING>);
+  return xw ? go(block_norm_vec_kernel<NC, true, 2, RING>) : go(block_norm_vec_kernel<NC, false, 2, RING>);
+}
+template <int NC>
+cudaError_t launch_vec(const NormParams &p, int threads, cudaStream_t st) {
+  // Rows that one wave of CTAs holds (1024 or 512 threads per SM) take one CTA each; more walk through the ring, as many CTAs as are
+  // resident and their rows under way as fit 160 KB per SM.
+  const int per_sm = (NC == 1 ? 1024 : 512) / threads, cap = sm_count() * per_sm;
+  if (p.T <= cap) return launch_vec<NC, false>(p, threads, (unsigned)p.T, 0, 0, st);
+  const size_t row = (size_t)p.H * ((p.x_dtype == KNJ_DT_F32 ? 4 : 2) + (!p.y ? 0 : p.y_dtype == KNJ_DT_F32 ? 4 : 2));
+  int depth = (int)(160 * 1024 / per_sm / row);
+  int ctas = cap;
+  if (depth < 2) {   // long rows: one CTA per SM
+    depth = (int)(200 * 1024 / row);
+    if (depth < 1) depth = 1;
+    ctas = sm_count();
+  }
+  if (depth > kMaxRing) depth = kMaxRing;
+  return launch_vec<NC, true>(p, threads, (unsigned)ctas, depth, depth * row, st);
 }
 
 // Eight values per lane, sixteen lanes per group; each lane has kUnroll groups' loads under way.
@@ -292,7 +406,7 @@ __global__ void __launch_bounds__(256) block_norm_kernel(const NormParams p) {
       const float v = load_as_f32(p.y, p.y_dtype, t * p.ldy + i);
       ss = fmaf(v, v, ss);
     }
-    rs = rms_inverse(block_sum(ss, red), p.H, p.eps, [&] {
+    rs = rms_inverse(block_sum(ss, red), p.inv_h, p.eps, [&] {
       float q = 0.f;
       for (int i = tid; i < p.H; i += 256) {
         const float v = load_as_f32(p.y, p.y_dtype, t * p.ldy + i) * kDown;
@@ -315,7 +429,7 @@ __global__ void __launch_bounds__(256) block_norm_kernel(const NormParams p) {
     if (p.stream) store_from_f32(p.stream, p.stream_dtype, t * p.ld_stream + i, s);
   }
   if (!p.h) return;
-  const float hs = rms_inverse(block_sum(ss, red), p.H, p.eps, [&] {
+  const float hs = rms_inverse(block_sum(ss, red), p.inv_h, p.eps, [&] {
     float q = 0.f;
     for (int i = tid; i < p.H; i += 256) q = fmaf(row[i] * kDown, row[i] * kDown, q);
     return block_sum(q, red);
@@ -401,7 +515,7 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
   p.h_scale = a->h_scale; p.ldx = a->ldx; p.ldy = a->ldy; p.ldg = a->ldg; p.ld_stream = a->ld_stream; p.ldh = a->ldh;
   p.T = a->n_tokens; p.H = H; p.x_dtype = a->x_dtype; p.y_dtype = a->y_dtype; p.w_dtype = a->w_dtype; p.gate_dtype = a->gate_dtype;
   p.gate_kind = a->gate_kind; p.gate_sigmoid = a->gate_sigmoid; p.stream_dtype = a->stream_dtype; p.h_dtype = a->h_dtype;
-  p.alpha = a->alpha; p.beta = a->beta; p.eps = a->eps;
+  p.alpha = a->alpha; p.beta = a->beta; p.eps = a->eps; p.inv_h = 1.0f / (float)H;
   auto units = [](const void *base, int64_t ld, int dtype) { return aligned16(base) && ld * (dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0; };
   const bool vec = H % 8 == 0 && H <= 16384 && units(p.x, p.ldx, p.x_dtype) && (!p.y || units(p.y, p.ldy, p.y_dtype)) && aligned16(p.post_w) &&
                    aligned16(p.pre_w) && (!p.stream || units(p.stream, p.ld_stream, p.stream_dtype)) &&
@@ -409,17 +523,13 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
                    (p.gate_kind != KNJ_GATE_FULL || units(p.gate, p.ldg, p.gate_dtype)) &&
                    (!p.h || (p.h_dtype == KNJ_DT_E4M3 ? aligned16(p.h) && p.ldh % 8 == 0 : units(p.h, p.ldh, p.h_dtype)));
   if (vec) {
-    // A warp per row where the rows alone fill the GPU (eight warps per SM and more) and fit its registers, else a CTA per row.
-    const char *ev = getenv("KNJ_X");
-    const int x = ev ? atoi(ev) : 0;
-    if (x == 128) KNJ_CUDA((launch_vec<128, 2>(p, as_stream(s))));
-    else if (x == 256) KNJ_CUDA((launch_vec<256, 1>(p, as_stream(s))));
-    else if (x == 64) KNJ_CUDA((launch_vec<64, 4>(p, as_stream(s))));
-    else if (H <= 2048 && p.T >= 8 * sm_count()) KNJ_CUDA(H <= 512 ? (launch_vec<32, 2>(p, as_stream(s))) : (launch_vec<32, 8>(p, as_stream(s))));
-    else if (H <= 2048) KNJ_CUDA((launch_vec<256, 1>(p, as_stream(s))));
-    else if (H <= 4096) KNJ_CUDA((launch_vec<256, 2>(p, as_stream(s))));
-    else if (H <= 8192) KNJ_CUDA((launch_vec<256, 4>(p, as_stream(s))));
-    else KNJ_CUDA((launch_vec<256, 8>(p, as_stream(s))));
+    // one run of eight values per thread up to 1024 values a row, two up to 8192, four up to 16384
+    const int runs = H <= 1024 ? 1 : H <= 8192 ? 2 : 4;
+    int threads = 32;
+    while (threads * 8 * runs < H) threads *= 2;
+    if (runs == 1) KNJ_CUDA((launch_vec<1>(p, threads, as_stream(s))));
+    else if (runs == 2) KNJ_CUDA((launch_vec<2>(p, threads, as_stream(s))));
+    else KNJ_CUDA((launch_vec<4>(p, threads, as_stream(s))));
     return launch_status("block_norm_vec_kernel");
   }
   const size_t smem = (size_t)H * 4;

@@ -84,6 +84,14 @@ NORMS = [
     (2, 32768, F32, F32, BF16, None, False, True, True, E4M3),
     (1, 32001, BF16, F32, BF16, None, False, True, True, F16),
     (600, 512, BF16, F32, BF16, None, False, False, False, None),
+    # more rows than one wave of CTAs: through the ring in shared memory
+    (2500, 512, BF16, F32, BF16, "row", True, True, True, E4M3),
+    (5000, 136, F32, None, F32, None, False, False, True, F16),
+    (701, 2048, BF16, BF16, BF16, "channel", True, True, True, E4M3),
+    (1300, 2048, F32, F16, BF16, "full", False, True, False, None),
+    (413, 4104, BF16, F32, BF16, None, False, True, True, BF16),
+    (163, 8200, BF16, BF16, F32, "channel", False, True, True, E4M3),
+    (150, 16384, F32, F32, BF16, "row", False, True, True, F32),
 ]
 
 
