@@ -267,94 +267,117 @@ def q4k_down_tc(ah, Wd, pair_idx, pair_cnt, P: int, pair_row=None, poison: bool 
 
 
 # ---- experts in bf16, fp16 and e4m3, and what stands between two blocks -------------------------------------------
+# These calls are made once or a few times per layer and decode step, so their host work counts: attributes are read once, outputs
+# come from new_empty / empty_like (1.4 us against torch.empty's 2.4).
 
-def _rows(t: torch.Tensor, what: str, dtypes, shape=None) -> int:
-    """Checks a matrix of rows (dense inside a row, any row stride) on the current device; its row stride in elements."""
-    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+_cur = torch._C._cuda_getDevice
+_OPERAND = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, _E4M3: DT_E4M3}
+_ONLY_F32, _ONLY_I32, _ONLY_E4M3 = {torch.float32: DT_F32}, {torch.int32: 0}, {_E4M3: DT_E4M3}
+
+
+def _refuse(t: torch.Tensor, what: str, cur: int, shape, types):
+    if t.get_device() != cur:
         raise ValueError(f"{what} lives on {t.device}, not on the current CUDA device")
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}" + (f", expected {tuple(shape)}" if shape is not None else ", expected rows"))
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what} is {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
-    n, k = t.shape
-    if k > 1 and t.stride(1) != 1:
-        raise ValueError(f"{what} has rows that are not dense")
-    ld = t.stride(0) if n > 1 else k
-    if ld < k:
-        raise ValueError(f"{what} has overlapping rows (stride {ld} for {k} values)")
-    return ld
+    raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)} with strides {t.stride()}, expected {' / '.join(str(d) for d in types)} "
+                     f"{'rows' if shape is None else tuple(shape)}, dense inside a row and without overlap")
 
 
-def _dense(t: torch.Tensor, what: str, dtypes, shape) -> int:
-    """Checks a contiguous tensor of this shape on the current device; its address."""
-    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
-        raise ValueError(f"{what} lives on {t.device}, not on the current CUDA device")
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.dtype not in dtypes:
-        raise ValueError(f"{what} is {t.dtype} {tuple(t.shape)}, expected contiguous {' / '.join(str(d) for d in dtypes)} {tuple(shape)}")
+def _rows(t: torch.Tensor, what: str, cur: int, shape=None, types=_DT):
+    """A matrix of rows, dense inside a row, any row stride, on the current device: (address, type code, row stride)."""
+    code, s = types.get(t.dtype), t.shape
+    if code is None or len(s) != 2 or t.get_device() != cur or (shape is not None and s != shape):
+        _refuse(t, what, cur, shape, types)
+    n, k = s
+    ld, one = t.stride()
+    if n <= 1:
+        ld = k
+    if (one != 1 and k > 1) or ld < k:
+        _refuse(t, what, cur, shape, types)
+    return t.data_ptr(), code, ld
+
+
+def _dense(t: torch.Tensor, what: str, cur: int, shape, types) -> int:
+    """A contiguous tensor of this shape on the current device: its address."""
+    if t.dtype not in types or t.shape != shape or t.get_device() != cur or not t.is_contiguous():
+        _refuse(t, what, cur, shape, types)
     return t.data_ptr()
 
 
 def fp8_rows(x: torch.Tensor):
     """x [rows][K] (f32 / bf16 / f16) -> (codes float8_e4m3fn [rows][K], scale f32 [rows][ceil(K/128)])."""
-    ld = _rows(x, "x", _DT)
+    ptr, code, ld = _rows(x, "x", _cur())
     n, k = x.shape
-    q = torch.empty((n, k), dtype=_E4M3, device=x.device)
-    scale = torch.empty((n, -(-k // 128)), dtype=torch.float32, device=x.device)
-    check(lib().knj_fp8_rows_launch(x.data_ptr(), _DT[x.dtype], ld, n, k, q.data_ptr(), scale.data_ptr(), _raw_stream()))
+    q = x.new_empty(n, k, dtype=_E4M3)
+    scale = x.new_empty(n, (k + 127) // 128, dtype=torch.float32)
+    check(lib().knj_fp8_rows_launch(ptr, code, ld, n, k, q.data_ptr(), scale.data_ptr(), _raw_stream()))
     return q, scale
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp8_matmul_scratch(m: int, k: int) -> int:
+    return int(lib().knj_fp8_matmul_workspace_bytes(m, k))
 
 
 def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
     """W float8_e4m3fn [n_out][n_in] with W_scale f32 [ceil(n_out/128)][ceil(n_in/128)], x [m][n_in] (f32 / bf16 / f16, turned
     into e4m3 rows as fp8_rows does) -> [m][n_out] in out_dtype."""
-    ld = _rows(x, "x", _DT)
+    cur = _cur()
+    ptr, code, ld = _rows(x, "x", cur)
     m, k = x.shape
-    if W.dim() != 2 or out_dtype not in _DT:
-        raise ValueError(f"W has shape {tuple(W.shape)}, out_dtype is {out_dtype}")
-    n = W.shape[0]
-    w = _dense(W, "W", (_E4M3,), (n, k))
-    ws = _dense(W_scale, "W_scale", (torch.float32,), (-(-n // 128), -(-k // 128)))
-    y = torch.empty((m, n), dtype=out_dtype, device=x.device)
-    L = lib()
-    nbytes = L.knj_fp8_matmul_workspace_bytes(m, k)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    check(L.knj_fp8_matmul_launch(w, ws, k, n, x.data_ptr(), _DT[x.dtype], ld, m, y.data_ptr(), _DT[out_dtype], n, work.data_ptr(), nbytes, None,
-                                  _raw_stream()))
+    n, out_code = W.shape[0], _DT.get(out_dtype)
+    if out_code is None:
+        raise ValueError(f"out_dtype is {out_dtype}")
+    w = _dense(W, "W", cur, (n, k), _ONLY_E4M3)
+    ws = _dense(W_scale, "W_scale", cur, ((n + 127) // 128, (k + 127) // 128), _ONLY_F32)
+    y = x.new_empty(m, n, dtype=out_dtype)
+    nbytes = _fp8_matmul_scratch(m, k)
+    work = x.new_empty(nbytes, dtype=torch.uint8)
+    check(lib().knj_fp8_matmul_launch(w, ws, k, n, ptr, code, ld, m, y.data_ptr(), out_code, n, work.data_ptr(), nbytes, None, _raw_stream()))
     return y
 
 
-def _expert_args(x, x_scale, mats, scales, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale):
-    w = mats[0]
-    if w.dim() != 3 or w.dtype not in (torch.bfloat16, torch.float16, _E4M3):
+def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale):
+    cur = _cur()
+    if w.dim() != 3 or w.dtype not in _OPERAND:
         raise ValueError(f"expert matrices are bf16, f16 or float8_e4m3fn [E][N][K], got {w.dtype} {tuple(w.shape)}")
-    E, N, K = w.shape
-    ptrs = [_dense(m, "an expert matrix", (w.dtype,), (E, N, K)) for m in mats] + [None]
-    sc = [None, None]
+    shape = w.shape
+    E, N, K = shape
+    types = (w.dtype,)
+    w_ptr = _dense(w, "an expert matrix", cur, shape, types)
+    w1_ptr = None if w1 is None else _dense(w1, "an expert matrix", cur, shape, types)
+    xs = s0_ptr = s1_ptr = None
     if w.dtype == _E4M3:
-        if any(s is None for s in scales):
+        if s0 is None or (w1 is not None and s1 is None):
             raise ValueError("e4m3 expert matrices need their scales")
-        sc = [_dense(s, "a matrix's scales", (torch.float32,), (E, -(-N // 128), -(-K // 128))) for s in scales] + [None]
+        sshape = (E, (N + 127) // 128, (K + 127) // 128)
+        s0_ptr = _dense(s0, "a matrix's scales", cur, sshape, _ONLY_F32)
+        if w1 is not None:
+            s1_ptr = _dense(s1, "a matrix's scales", cur, sshape, _ONLY_F32)
         if x.dtype != _E4M3:
+            if x_scale is not None:
+                raise ValueError("x_scale belongs to e4m3 rows")
             x, x_scale = fp8_rows(x)
         elif x_scale is None:
             raise ValueError("e4m3 rows need x_scale")
-    elif any(s is not None for s in scales) or x_scale is not None:
+        xs = _dense(x_scale, "x_scale", cur, (x.shape[0], sshape[2]), _ONLY_F32)
+    elif s0 is not None or s1 is not None or x_scale is not None:
         raise ValueError("scales belong to e4m3 matrices and rows")
-    ld = _rows(x, "x", (w.dtype,))
-    n_rows = x.shape[0]
-    if x.shape[1] != K:
-        raise ValueError(f"x has rows of {x.shape[1]} values, the matrices of {K}")
-    xs = None if x_scale is None else _dense(x_scale, "x_scale", (torch.float32,), (n_rows, -(-K // 128)))
-    stride = pair_idx.shape[1] if pair_idx.dim() == 2 else -1
-    idx = _dense(pair_idx, "pair_idx", (torch.int32,), (E, stride))
-    cnt = _dense(pair_cnt, "pair_cnt", (torch.int32,), (E,))
-    rmap = None if row_map is None else _dense(row_map, "the row map", (torch.int32,), (P,))
+    x_ptr, x_code, ld = _rows(x, "x", cur, (x.shape[0], K), {w.dtype: _OPERAND[w.dtype]})
+    idx_shape = pair_idx.shape
+    if len(idx_shape) != 2:
+        raise ValueError(f"pair_idx has shape {tuple(idx_shape)}")
+    idx = _dense(pair_idx, "pair_idx", cur, (E, idx_shape[1]), _ONLY_I32)
+    cnt = _dense(pair_cnt, "pair_cnt", cur, (E,), _ONLY_I32)
+    rmap = None if row_map is None else _dense(row_map, "the row map", cur, (P,), _ONLY_I32)
     if out is None:
-        out = torch.empty((P, N), dtype=out_dtype, device=x.device)
-    ldo = _rows(out, "out", _DT, (P, N))
-    a = ExpertGemmArgs(x.data_ptr(), xs, ld, ptrs[0], ptrs[1], sc[0], sc[1], idx, cnt, rmap, stride, out.data_ptr(), ldo, None, n_rows, P, N, K, E,
-                       row_div, _DT_ALL[x.dtype], _DT_ALL[w.dtype], _DT[out.dtype], out_scale)
-    return a, out, x, x_scale
+        if out_dtype not in _DT:
+            raise ValueError(f"out_dtype is {out_dtype}")
+        out = x.new_empty(P, N, dtype=out_dtype)
+    out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
+    a = ExpertGemmArgs(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo, None, x.shape[0], P, N, K, E,
+                       row_div, x_code, x_code, out_code, out_scale)
+    check(launch(C.byref(a), _raw_stream()))
+    return out
 
 
 def expert_gateup(x, Wg, Wu, pair_idx, pair_cnt, P: int, top_k: int, pair_tok=None, gate_scale=None, up_scale=None, x_scale=None,
@@ -365,18 +388,15 @@ def expert_gateup(x, Wg, Wu, pair_idx, pair_cnt, P: int, top_k: int, pair_tok=No
     pair p reads row pair_tok[p], or p // top_k. Rows of pairs that no table entry names are left as they were."""
     if out_dtype is None:
         out_dtype = torch.bfloat16 if Wg.dtype == _E4M3 else Wg.dtype
-    a, out, *keep = _expert_args(x, x_scale, (Wg, Wu), (gate_scale, up_scale), pair_idx, pair_cnt, P, pair_tok, top_k, out, out_dtype, out_scale)
-    check(lib().knj_expert_gateup_launch(C.byref(a), _raw_stream()))
-    return out
+    return _expert(lib().knj_expert_gateup_launch, x, x_scale, Wg, Wu, gate_scale, up_scale, pair_idx, pair_cnt, P, pair_tok, top_k, out,
+                   out_dtype, out_scale)
 
 
 def expert_proj(a, W, pair_idx, pair_cnt, P: int, pair_row=None, scale=None, a_scale=None, out_dtype=torch.float32, out=None,
                 out_scale: float = 1.0):
     """a . W[e] * out_scale for every routed pair: [P][N] in out_dtype. a holds one row per pair (row pair_row[p] when given,
     else p); types, scales and unnamed rows as for expert_gateup."""
-    args, out, *keep = _expert_args(a, a_scale, (W,), (scale,), pair_idx, pair_cnt, P, pair_row, 1, out, out_dtype, out_scale)
-    check(lib().knj_expert_proj_launch(C.byref(args), _raw_stream()))
-    return out
+    return _expert(lib().knj_expert_proj_launch, a, a_scale, W, None, scale, None, pair_idx, pair_cnt, P, pair_row, 1, out, out_dtype, out_scale)
 
 
 def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False, alpha: float = 1.0, beta: float = 1.0, pre_w=None,
@@ -386,46 +406,44 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
     gate [H], [T][1] or [T][H] (through a sigmoid with gate_sigmoid). Returns (s, h): s in stream_dtype (default: x's type;
     None without y unless stream_out or stream_dtype asks for it), h in norm_dtype (None without pre_w), for
     torch.float8_e4m3fn as (codes, scale). stream_out may be x or y."""
-    ldx = _rows(x, "x", _DT)
-    T, H = x.shape
-    a = BlockNormArgs(n_tokens=T, hidden=H, x=x.data_ptr(), ldx=ldx, x_dtype=_DT[x.dtype], alpha=alpha, beta=beta, eps=eps,
-                      gate_sigmoid=1 if gate_sigmoid else 0)
+    cur = _cur()
+    x_ptr, x_code, ldx = _rows(x, "x", cur)
+    shape = x.shape
+    T, H = shape
+    y_ptr = gate_ptr = s_ptr = h_ptr = scale_ptr = post = pre = s = h = scale = None
+    y_code = w_code = gate_code = s_code = h_code = ldy = ldg = lds = 0
+    kind = GATE_NONE
     if y is not None:
-        a.ldy, a.y, a.y_dtype = _rows(y, "y", _DT, (T, H)), y.data_ptr(), _DT[y.dtype]
-    for w in (post_w, pre_w):
-        if w is not None:
-            ptr = _dense(w, "a norm weight", _DT, (H,))
-            if post_w is not None and pre_w is not None and post_w.dtype != pre_w.dtype:
-                raise ValueError("post_w and pre_w are of one type")
-            a.w_dtype = _DT[w.dtype]
-            if w is post_w:
-                a.post_w = ptr
-            if w is pre_w:
-                a.pre_w = ptr
+        y_ptr, y_code, ldy = _rows(y, "y", cur, shape)
+    if post_w is not None:
+        post, w_code = _dense(post_w, "post_w", cur, (H,), _DT), _DT[post_w.dtype]
+    if pre_w is not None:
+        pre = _dense(pre_w, "pre_w", cur, (H,), _DT)
+        if post_w is not None and w_code != _DT[pre_w.dtype]:
+            raise ValueError("post_w and pre_w are of one type")
+        w_code = _DT[pre_w.dtype]
+        h_code = _DT_ALL.get(norm_dtype)
+        if h_code is None:
+            raise ValueError(f"norm_dtype is {norm_dtype}")
+        h = torch.empty_like(x, dtype=norm_dtype, memory_format=torch.contiguous_format)
+        h_ptr = h.data_ptr()
+        if h_code == DT_E4M3:
+            scale = x.new_empty(T, (H + 127) // 128, dtype=torch.float32)
+            scale_ptr = scale.data_ptr()
     if gate is not None:
         if gate.dim() == 1:
-            _dense(gate, "gate", _DT, (H,))
-            a.gate_kind = GATE_CHANNEL
-        elif gate.dim() == 2 and gate.shape[1] == 1 and H > 1:
-            a.ldg = max(1, _rows(gate, "gate", _DT, (T, 1)))
-            a.gate_kind = GATE_ROW
+            gate_ptr, gate_code, kind = _dense(gate, "gate", cur, (H,), _DT), _DT[gate.dtype], GATE_CHANNEL
         else:
-            a.ldg = _rows(gate, "gate", _DT, (T, H))
-            a.gate_kind = GATE_FULL
-        a.gate, a.gate_dtype = gate.data_ptr(), _DT[gate.dtype]
-    s = stream_out
-    if s is None and (y is not None or stream_dtype is not None):
-        s = torch.empty((T, H), dtype=stream_dtype or x.dtype, device=x.device)
+            rows_only = gate.shape[1] == 1 and H > 1
+            gate_ptr, gate_code, ldg = _rows(gate, "gate", cur, (T, 1) if rows_only else shape)
+            kind = GATE_ROW if rows_only else GATE_FULL
+    if stream_out is not None:
+        s = stream_out
+    elif y is not None or stream_dtype is not None:
+        s = torch.empty_like(x, dtype=stream_dtype or x.dtype, memory_format=torch.contiguous_format)
     if s is not None:
-        a.ld_stream, a.stream_out, a.stream_dtype = _rows(s, "the stream", _DT, (T, H)), s.data_ptr(), _DT[s.dtype]
-    h = scale = None
-    if pre_w is not None:
-        if norm_dtype not in _DT_ALL:
-            raise ValueError(f"norm_dtype is {norm_dtype}")
-        h = torch.empty((T, H), dtype=norm_dtype, device=x.device)
-        a.h, a.ldh, a.h_dtype = h.data_ptr(), H, _DT_ALL[norm_dtype]
-        if norm_dtype == _E4M3:
-            scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
-            a.h_scale = scale.data_ptr()
+        s_ptr, s_code, lds = _rows(s, "the stream", cur, shape)
+    a = BlockNormArgs(T, H, x_ptr, ldx, y_ptr, ldy, post, pre, gate_ptr, ldg, s_ptr, lds, h_ptr, H, scale_ptr, x_code, y_code, w_code, gate_code,
+                      s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps)
     check(lib().knj_block_norm_launch(C.byref(a), _raw_stream()))
     return s, (h if scale is None else (h, scale))
