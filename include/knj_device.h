@@ -544,7 +544,8 @@ typedef struct knj_expert_gemm_args {
 int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 /* 1 = these products (and the dense e4m3 one) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
- * always on CTA pairs (buckets of up to 256), 0 (default) = by the number of pairs per expert. Process-wide. */
+ * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes.
+ * Process-wide. */
 void knj_expert_tc_form(int form);
 
 /* Dense product with an e4m3 matrix: y[m][n_out] = x[m][n_in] . W^T, W e4m3 [n_out][n_in] with W_scale

@@ -36,7 +36,7 @@ struct GemmParams {
   void *out;
   int *status;
   int64_t ldo, idx_stride;
-  int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles;
+  int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles, parts;   // parts: CTAs that share a tile's K
   uint32_t idesc_format;
   int vec_out;                // bases and strides of the outputs allow 16-byte (lane = row form: 32-byte) stores
   int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
@@ -44,11 +44,18 @@ struct GemmParams {
   CUtensorMap map0, map1, mapx;
 };
 
-template <bool FP8, bool GATEUP, int CG>
+// kSingle: single SMs, two CTAs each, buckets of up to 64 rows. kPair: CTA pairs, buckets of up to 256. kSplit: as kSingle with
+// buckets of up to 32, where the tiles are too few for the GPU: a cluster of CTAs shares each tile's K, and its first CTA adds the
+// parts, in order, out of its shared memory.
+enum Form { kSingle = 0, kPair = 1, kSplit = 2 };
+constexpr int kMaxParts = 6;   // 5 x 16 KB of sums of other CTAs in the first one's idle operand stages
+
+template <bool FP8, bool GATEUP, int FORM>
 struct Shape {
+  static constexpr int CG = FORM == kPair ? 2 : 1;
   // e4m3 in pairs: the MMA's M side is the routed rows and its N side 256 matrix rows (of them 128 of gate and 128 of up)
   static constexpr bool kRowsM = FP8 && CG == 2;
-  static constexpr int kTok = CG == 2 ? 256 : 64;        // routed rows of a bucket
+  static constexpr int kTok = FORM == kPair ? 256 : FORM == kSplit ? 32 : 64;   // routed rows of a bucket
   static constexpr int kTokStep = kRowsM ? 8 : 16 * CG;  // bucket sizes are multiples of this
   static constexpr int kEpiWarps = CG == 2 ? 8 : 4;
   static constexpr int kMmaWarp = kEpiWarps, kMatWarp = kEpiWarps + 1, kScaleWarp = kEpiWarps + 2;
@@ -57,7 +64,7 @@ struct Shape {
   static constexpr int kThreads = 32 * (kRowWarp + kRowWarps);
   static constexpr int kBlocksPerSm = CG == 2 ? 1 : 2;
   static constexpr int kSub = CG == 2 && !FP8 ? 2 : 1;   // slabs of 128 bytes of K per stage
-  static constexpr int kStages = CG == 2 ? 6 / kSub : 4;
+  static constexpr int kStages = FORM == kPair ? 6 / kSub : FORM == kSplit ? 5 : 4;
   static constexpr int kATile = 128 * 128;               // bytes: 128 matrix rows x 128 bytes of K
   static constexpr int kBTile = kTok / CG * 128;
   static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per slab
@@ -136,15 +143,18 @@ __device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&x);
 }
 
-template <bool FP8, bool GATEUP, int CG>
-__global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, GATEUP, CG>::kBlocksPerSm)
+template <bool FP8, bool GATEUP, int FORM>
+__global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8, GATEUP, FORM>::kBlocksPerSm)
     expert_tc_kernel(const __grid_constant__ GemmParams p) {
-  using S = Shape<FP8, GATEUP, CG>;
+  using S = Shape<FP8, GATEUP, FORM>;
+  constexpr int CG = S::CG;
+  constexpr bool SPLIT = FORM == kSplit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = warp_index();
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;                       // in the pair
+  const int part = SPLIT ? (int)cluster_rank() : 0, parts = SPLIT ? p.parts : 1;   // of K
 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kOffBars);
   uint64_t *full = bars;                        // [kStages] operands of both CTAs landed (the even CTA's are used)
@@ -216,7 +226,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
+  if (CG == 2 || SPLIT) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -224,8 +234,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   const int n_tiles = s_pref[kMaxExperts] * p.m_tiles;   // < 2^31: checked on the host
   // As many CTAs (pairs) as take part in whole rounds: of 1536 tiles on 296 CTAs, 256 take six each instead of 56 a sixth; the matrices
   // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
-  const int avail = gridDim.x / CG, rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
-  const int first = (int)(blockIdx.x / CG) < step ? blockIdx.x / CG : n_tiles;
+  const int k_lo = part * nslab / parts, k_hi = (part + 1) * nslab / parts;   // this CTA's slabs
+  const int avail = gridDim.x / (CG * parts), rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
+  const int first = (int)(blockIdx.x / (CG * parts)) < step ? blockIdx.x / (CG * parts) : n_tiles;
       auto tile_at = [&](int t, int &ntok) {
         const int b = t / p.m_tiles, mt = t - b * p.m_tiles;
         int lo = 0;  // the last expert whose first bucket is not behind b
@@ -262,6 +273,23 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     return ok;
   };
 
+  // kSplit: a tile ends for all warps of the cluster together: every sum is formed and the operand stages are idle; the sums of
+  // parts 1, 2, .. are in the first CTA's stages; and, where another tile follows, they are read.
+  auto split_syncs = [&](int t) { return t + step < n_tiles ? 3 : 2; };
+  auto split_end = [&](int t) {   // for the warps that take no part in it
+    if constexpr (SPLIT)
+      for (int i = 0; i < split_syncs(t); ++i) cluster_sync_all();
+  };
+  auto split_give_up = [&](int t, int done) {   // from the tile t on, of whose syncs `done` have been met
+    if constexpr (SPLIT) {
+      if (ok) return;
+      if (lane == 0) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int *>(s_fail), 0)), "r"(1) : "memory");
+      __syncwarp();
+      for (; t < n_tiles; t += step, done = 0)
+        for (int i = done; i < split_syncs(t); ++i) cluster_sync_all();
+    }
+  };
+
   // What a tile is, is found once per CTA, by the matrix warp, and handed on through a ring.
   int tslot = 0;
   uint32_t tpar = 0;
@@ -291,6 +319,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     int buf = S::kRowsM ? group : 0, sg = 0;
     uint32_t par = 0, sg_par = 0;
     int t = first;
+    [[maybe_unused]] int synced = 0;   // syncs of the running tile that are met
     for (; t < n_tiles; t += step, tile_done()) {
       Tile tl;
       if (!tile_take(tl)) break;
@@ -386,18 +415,74 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
           par ^= 1u;
         }
       };
+      // kSplit: this thread's sixteen sums of a step of 16 columns, to the first CTA or out of its stages
+      auto part_at = [&](int from, int c, int i) { return (uint32_t)((((from - 1) * (S::kTok / 16) + c) * 4 + i) * 128 + tid) * 16u; };
+      auto part_send = [&](const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c) {
+        const uint32_t base = cluster_addr(smem, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t *v = i < 2 ? lo + 4 * i : hi + 4 * (i - 2);
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + part_at(part, c, i)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                       : "memory");
+        }
+      };
+      auto part_add = [&](uint32_t (&lo)[8], uint32_t (&hi)[8], int c) {
+        for (int from = 1; from < parts; ++from)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 f = *reinterpret_cast<const float4 *>(smem + part_at(from, c, i));
+            uint32_t *v = i < 2 ? lo + 4 * i : hi + 4 * (i - 2);
+            v[0] = __float_as_uint(__uint_as_float(v[0]) + f.x);
+            v[1] = __float_as_uint(__uint_as_float(v[1]) + f.y);
+            v[2] = __float_as_uint(__uint_as_float(v[2]) + f.z);
+            v[3] = __float_as_uint(__uint_as_float(v[3]) + f.w);
+          }
+      };
+      // every thread of the warp: meets sync `i` of the tile; after the second, whether all parts are there
+      auto part_sync = [&](int i) {
+        fence_proxy_async();   // the stages go over between copies and ordinary accesses
+        cluster_sync_all();
+        synced = i;
+        if (i == 2 && __any_sync(0xffffffffu, *s_fail != 0)) ok = false;
+        return ok;
+      };
       if constexpr (!FP8) {
         if (!wait(&acc_full[buf], par)) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int ch = group; ch * 32 < ncol; ch += kGroups) {
+        if constexpr (SPLIT) {
+          // one chunk of 32 columns
           uint32_t r[4][8];
-          load(r[0], r[1], ch * 32);
-          load(r[2], r[3], ch * 32 + 16);
+          load(r[0], r[1], 0);
+          load(r[2], r[3], 16);
           tmem_ld_wait(r[0], r[1]);
           tmem_ld_wait(r[2], r[3]);
-          finish(r[0], r[1], ch * 32);
-          finish(r[2], r[3], ch * 32 + 16);
+          part_sync(1);
+          if (part != 0) {
+            part_send(r[0], r[1], 0);
+            if (ncol > 16) part_send(r[2], r[3], 1);
+          }
+          if (!part_sync(2)) break;
+          if (part == 0) {
+            part_add(r[0], r[1], 0);
+            finish(r[0], r[1], 0);
+            if (ncol > 16) {
+              part_add(r[2], r[3], 1);
+              finish(r[2], r[3], 16);
+            }
+          }
+          if (split_syncs(t) == 3) part_sync(3);
+          synced = 0;
+        } else {
+#pragma unroll 1
+          for (int ch = group; ch * 32 < ncol; ch += kGroups) {
+            uint32_t r[4][8];
+            load(r[0], r[1], ch * 32);
+            load(r[2], r[3], ch * 32 + 16);
+            tmem_ld_wait(r[0], r[1]);
+            tmem_ld_wait(r[2], r[3]);
+            finish(r[0], r[1], ch * 32);
+            finish(r[2], r[3], ch * 32 + 16);
+          }
         }
         release();
       } else if constexpr (S::kRowsM) {
@@ -510,7 +595,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int j = 0; j < 4; ++j) acc[c][h][j] = 0ull;
-          for (int ks = 0; ks < nslab; ++ks) {
+          for (int ks = 0; ks < k_hi - k_lo; ++ks) {
             if ((ks & 3) == 0) wait(&sc_full[sg], sg_par);
             if (!wait(&acc_full[buf], par)) return;
             tc_fence_after();
@@ -536,7 +621,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
               }
             }
             release();
-            if ((ks & 3) == 3 || ks + 1 == nslab) {
+            if ((ks & 3) == 3 || ks + 1 == k_hi - k_lo) {
               if (lane == 0) mbar_arrive(&sc_empty[sg]);   // behind release()'s __syncwarp
               if (++sg == S::kScaleGroups) {
                 sg = 0;
@@ -544,32 +629,52 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
               }
             }
           }
+          if constexpr (SPLIT) {
+            uint32_t v[kSteps > 0 ? kSteps : 1][2][8];
 #pragma unroll
-          for (int c = 0; c < kSteps; ++c) {
-            uint32_t lo[8], hi[8];
+            for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              lo[2 * j] = (uint32_t)acc[c][0][j];
-              lo[2 * j + 1] = (uint32_t)(acc[c][0][j] >> 32);
-              hi[2 * j] = (uint32_t)acc[c][1][j];
-              hi[2 * j + 1] = (uint32_t)(acc[c][1][j] >> 32);
+              for (int j = 0; j < 8; ++j) {
+                v[c][0][j] = (uint32_t)(acc[c][0][j >> 1] >> (32 * (j & 1)));
+                v[c][1][j] = (uint32_t)(acc[c][1][j >> 1] >> (32 * (j & 1)));
+              }
+            part_sync(1);
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c)
+              if (part != 0 && 16 * c < ncol) part_send(v[c][0], v[c][1], c);
+            if (!part_sync(2)) return;
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c)
+              if (part == 0 && 16 * c < ncol) {
+                part_add(v[c][0], v[c][1], c);
+                finish(v[c][0], v[c][1], 16 * c);
+              }
+            if (split_syncs(t) == 3) part_sync(3);
+            synced = 0;
+          } else {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) {
+              uint32_t lo[8], hi[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                lo[j] = (uint32_t)(acc[c][0][j >> 1] >> (32 * (j & 1)));
+                hi[j] = (uint32_t)(acc[c][1][j >> 1] >> (32 * (j & 1)));
+              }
+              finish(lo, hi, col_of(c));
             }
-            finish(lo, hi, col_of(c));
           }
         };
         const int nc = ((ncol + 31) / 32 - group + kGroups - 1) / kGroups;   // chunks of this group
+        static_assert(kChunks <= 2, "one case for each number of chunks");
         if (nc <= 0) blocks(std::integral_constant<int, 0>{});
         else if (nc == 1) blocks(std::integral_constant<int, 1>{});
-        else if (nc == 2) blocks(std::integral_constant<int, 2>{});
-        else if constexpr (kChunks > 2) {
-          if (nc == 3) blocks(std::integral_constant<int, 3>{});
-          else blocks(std::integral_constant<int, 4>{});
-        }
+        else if constexpr (kChunks > 1) blocks(std::integral_constant<int, 2>{});
         if (!ok) break;
       }
     }
     // a wait gave up: NaN for what this warp has not stored, its tile at that moment and those behind it
-    for (; !ok && t < n_tiles; t += step) {
+    split_give_up(t, synced);
+    for (; !ok && part == 0 && t < n_tiles; t += step) {
       int ntok;
       const Tile tl = tile_at(t, ntok);
       if constexpr (S::kRowsM) {
@@ -593,12 +698,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       const uint64_t a_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffA)), b_desc0 = smem_desc_sw128(smem_u32(smem + S::kOffB));
       int st = 0, buf = 0;
       uint32_t par = 0, acc_par = 1;  // a fresh barrier passes a wait for parity 1
-      for (int t = first; t < n_tiles; t += step, tile_done()) {
+      int t = first;
+      for (; t < n_tiles; tile_done(), split_end(t), t += step) {
         Tile tl;
         if (!tile_take(tl)) break;
         const uint32_t idesc = instr_desc_f16(128 * CG, S::kRowsM ? 128 : tl.ncol) | p.idesc_format;
-        for (int ks = 0; ks < nslab; ks += S::kSub) {
-          if (!S::kRowsM && (FP8 || ks == 0) && !wait(&acc_empty[buf], acc_par)) break;
+        for (int ks = k_lo; ks < k_hi; ks += S::kSub) {
+          if (!S::kRowsM && (FP8 || ks == k_lo) && !wait(&acc_empty[buf], acc_par)) break;
           if (!wait(&full[st], par)) break;
           tc_fence_after();
           const uint64_t mat = a_desc0 + (uint32_t)(st * S::kSub * S::kATile) / 16, rows = b_desc0 + (uint32_t)(st * S::kSub * S::kBTile) / 16;
@@ -625,15 +731,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
             }
             if (!ok) break;
           } else {
-            const bool last = FP8 || ks + S::kSub >= nslab;
+            const bool last = FP8 || ks + S::kSub >= k_hi;
             if (elect_one()) {
 #pragma unroll
               for (int u = 0; u < S::kSub; ++u) {
-                if (u > 0 && ks + u >= nslab) break;
+                if (u > 0 && ks + u >= k_hi) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   tc_mma<FP8, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
-                               (u > 0 || k > 0 || (!FP8 && ks > 0)) ? 1u : 0u);
+                               (u > 0 || k > 0 || (!FP8 && ks > k_lo)) ? 1u : 0u);
               }
               commit(&empty[st]);
               if (last) commit(&acc_full[buf]);
@@ -645,6 +751,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         }
         if (!ok) break;
       }
+      split_give_up(t, 0);
     }
   } else if (warp == S::kMatWarp) {
     // =========================== tiles and matrix rows ===========================
@@ -683,7 +790,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     int st = 0;
     uint32_t par = 1;
     tpar = 1;
-    for (int t = first; t < n_tiles; t += step) {
+    int t = first;
+    for (; t < n_tiles; split_end(t), t += step) {
       const Tile tl = next;
       if (!wait(&tile_empty[tslot], tpar)) break;
 #pragma unroll
@@ -702,14 +810,14 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       // of both CTAs, matrix and rows, per slab
       const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : tl.ncol * 128));
       const bool more = t + step < n_tiles;
-      for (int ks = 0; ks < nslab; ks += S::kSub) {
+      for (int ks = k_lo; ks < k_hi; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
         const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&full[st], bytes * min(S::kSub, nslab - ks));
+          if (rank == 0) mbar_expect_tx(&full[st], bytes * min(S::kSub, k_hi - ks));
 #pragma unroll
           for (int u = 0; u < S::kSub; ++u) {
-            if (u > 0 && ks + u >= nslab) break;
+            if (u > 0 && ks + u >= k_hi) break;
             const uint32_t dst = smem_u32(smem + S::kOffA + (st * S::kSub + u) * S::kATile);
             const int x = (ks + u) * S::kSlab;
             if (S::kRowsM) {
@@ -727,11 +835,12 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         }
         __syncwarp();
         if (++st == S::kStages) { st = 0; par ^= 1u; }
-        if (ks == 0 && more) look(t + step);
+        if (ks == k_lo && more) look(t + step);
       }
       if (!ok) break;
       if (more) resolve();
     }
+    split_give_up(t, 0);
   } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
     // =========================== scales ===========================
     // Asynchronous copies of four bytes, four blocks of K to a group: read into registers, a group had to wait for its loads, and an
@@ -740,7 +849,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
     const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
     int sg = 0;
     uint32_t par = 1;
-    for (int t = first; t < n_tiles; t += step, tile_done()) {
+    int t = first;
+    for (; t < n_tiles; tile_done(), split_end(t), t += step) {
       Tile tl;
       if (!tile_take(tl)) break;
       // scales of block `blk` of matrix 0 and, for two, of matrix 1 or of the next block; behind the last output there is no block:
@@ -755,16 +865,16 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         const int at = S::kRowsM ? (c < n_cta ? (int)rank * n_cta + c : 0) : c;
         xs[j] = p.xs + (int64_t)s_row[tslot * S::kTok + at] * nslab;
       }
-      for (int k0 = 0; k0 < nslab; k0 += 4) {
+      for (int k0 = k_lo; k0 < k_hi; k0 += 4) {
         if (!wait(&sc_empty[sg], par)) break;
         float *dst = reinterpret_cast<float *>(smem + S::kOffScale + sg * S::kScaleGroup);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k0 + i < nslab) {
+          if (k0 + i < k_hi) {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) cp_async4(dst + i * S::kVecRows + c0 + 32 * j, xs[j] + k0 + i);
           }
-        if (warp == S::kScaleWarp && lane < 4 * S::kVecs && k0 + (lane & 3) < nslab) cp_async4(dst + 4 * S::kVecRows + 2 * (lane & 3) + second, ws + k0);
+        if (warp == S::kScaleWarp && lane < 4 * S::kVecs && k0 + (lane & 3) < k_hi) cp_async4(dst + 4 * S::kVecRows + 2 * (lane & 3) + second, ws + k0);
         cp_async_arrive(&sc_full[sg]);
         if (++sg == S::kScaleGroups) {
           sg = 0;
@@ -774,13 +884,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    split_give_up(t, 0);
   } else if (warp >= S::kRowWarp && warp < S::kRowWarp + S::kRowWarps) {
     // =========================== routed rows ===========================
     const int w = warp - S::kRowWarp;
     constexpr int kQuads = S::kTok / CG / (4 * S::kRowWarps);   // copies of four rows per warp and slab
     int st = 0;
     uint32_t par = 1;
-    for (int t = first; t < n_tiles; t += step, tile_done()) {
+    int t = first;
+    for (; t < n_tiles; tile_done(), split_end(t), t += step) {
       Tile tl;
       if (!tile_take(tl)) break;
       const int n_cta = tl.ncol / CG;
@@ -790,13 +902,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
         const int r = 4 * (w + S::kRowWarps * q);
         rows[q] = *reinterpret_cast<const int4 *>(s_row + tslot * S::kTok + (r < n_cta ? (int)rank * n_cta + r : 0));
       }
-      for (int ks = 0; ks < nslab; ks += S::kSub) {
+      for (int ks = k_lo; ks < k_hi; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
         const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
         if (elect_one()) {
 #pragma unroll
           for (int u = 0; u < S::kSub; ++u) {
-            if (u > 0 && ks + u >= nslab) break;
+            if (u > 0 && ks + u >= k_hi) break;
             const uint32_t dst = smem_u32(smem + S::kOffB + (st * S::kSub + u) * S::kBTile);
             const int x = (ks + u) * S::kSlab;
             if (p.dense) {
@@ -815,6 +927,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
       }
       if (!ok) break;
     }
+    split_give_up(t, 0);
+  } else if (SPLIT) {
+    for (int t = first; t < n_tiles; t += step) split_end(t);   // a warp without a part in it
   }
 
   if (!ok) {
@@ -831,7 +946,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, CG>::kThreads, Shape<FP8, G
   if (warp == S::kMmaWarp) tmem_dealloc<CG>(tmem_base, kTmemCols);
 }
 
-int g_form = 0;  // 0 = by the rule below, 1 = single SMs, 2 = pairs (knj_expert_tc_form)
+int g_form = 0;  // 0 = by the rule below, 1 = single SMs, 2 = pairs, 3 = K split over a cluster (knj_expert_tc_form)
 
 struct Operands {
   const void *x, *w0, *w1;
@@ -839,12 +954,20 @@ struct Operands {
   bool fp8;
 };
 
-template <bool FP8, bool GATEUP, int CG>
+// the tiles that these pairs can make; a table that names pairs more than once makes more, which the same grid walks over
+template <class S>
+int64_t most_tiles(const GemmParams &p) {
+  const int64_t rows = S::kOuts * S::CG, buckets = p.dense ? (p.n_pairs + S::kTok - 1) / S::kTok : p.n_pairs / S::kTok + (p.E < p.n_pairs ? p.E : p.n_pairs);
+  return buckets * ((p.N + rows - 1) / rows);
+}
+
+template <bool FP8, bool GATEUP, int FORM>
 int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
-  using S = Shape<FP8, GATEUP, CG>;
+  using S = Shape<FP8, GATEUP, FORM>;
+  constexpr int CG = S::CG;
   int dev = 0;
   KNJ_CUDA(cudaGetDevice(&dev));
-  auto kern = expert_tc_kernel<FP8, GATEUP, CG>;
+  auto kern = expert_tc_kernel<FP8, GATEUP, FORM>;
   static bool opted[64] = {false};
   if (dev >= 0 && dev < 64 && !opted[dev]) {
     KNJ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
@@ -862,17 +985,15 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
   KNJ_REQUIRE(most * p.m_tiles < (1ll << 31) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
-  // the tiles that these pairs can make; a table that names pairs more than once makes more, which the same grid walks over
-  const int64_t tiles = ((int64_t)p.n_pairs / S::kTok + (p.E < p.n_pairs ? p.E : p.n_pairs)) * p.m_tiles;
-  const int64_t cap = (int64_t)sm_count() * S::kBlocksPerSm / CG;
+  const int64_t tiles = most_tiles<S>(p), cap = (int64_t)sm_count() * S::kBlocksPerSm / (CG * p.parts);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * CG));
+  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * CG * p.parts));
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = CG * p.parts;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -883,12 +1004,24 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   return launch_status("expert_tc_kernel");
 }
 
+template <bool FP8, bool GATEUP>
+int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
+  const int experts = p.E < p.n_pairs ? p.E : p.n_pairs;
+  const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
+  int64_t parts = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
+  parts = parts > kMaxParts ? kMaxParts : parts;
+  parts = parts > nslab ? nslab : parts;
+  p.parts = 1;
+  if (g_form == 3 || (g_form == 0 && parts >= 2)) {
+    p.parts = parts < 1 ? 1 : (int)parts;
+    return launch_form<FP8, GATEUP, kSplit>(p, o, st);
+  }
+  const bool pairs = g_form ? g_form == 2 : (int64_t)p.n_pairs > 32ll * experts;
+  return pairs ? launch_form<FP8, GATEUP, kPair>(p, o, st) : launch_form<FP8, GATEUP, kSingle>(p, o, st);
+}
 template <bool GATEUP>
 int launch_gemm(const GemmParams &p, const Operands &o, cudaStream_t st) {
-  const int experts = p.E < p.n_pairs ? p.E : p.n_pairs;
-  const bool pairs = g_form ? g_form == 2 : (int64_t)p.n_pairs > 32ll * experts;
-  if (o.fp8) return pairs ? launch_form<true, GATEUP, 2>(p, o, st) : launch_form<true, GATEUP, 1>(p, o, st);
-  return pairs ? launch_form<false, GATEUP, 2>(p, o, st) : launch_form<false, GATEUP, 1>(p, o, st);
+  return o.fp8 ? launch_rule<true, GATEUP>(p, o, st) : launch_rule<false, GATEUP>(p, o, st);
 }
 
 int check_expert(const knj_expert_gemm_args *a, bool gateup, const char *who) {
@@ -932,7 +1065,7 @@ int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s) { re
 
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s) { return run_expert(a, false, "knj_expert_proj", s); }
 
-void knj_expert_tc_form(int form) { g_form = form == 1 || form == 2 ? form : 0; }
+void knj_expert_tc_form(int form) { g_form = form >= 1 && form <= 3 ? form : 0; }
 
 size_t knj_fp8_matmul_workspace_bytes(int m, int n_in) {
   if (m <= 0 || n_in <= 0) return 0;

@@ -16,9 +16,9 @@ def gen(*key):
     return g
 
 
-@pytest.fixture(params=[1, 2], ids=["single", "pair"])
+@pytest.fixture(params=[1, 2, 3], ids=["single", "pair", "split"])
 def form(request):
-    """Both forms of the products: single SMs with buckets of 64 rows, CTA pairs with buckets of 256."""
+    """The forms of the products: single SMs with buckets of 64 rows, CTA pairs with buckets of 256, K split over a cluster."""
     from kanjoos_b200 import _lib
     _lib.lib().knj_expert_tc_form(request.param)
     yield request.param
