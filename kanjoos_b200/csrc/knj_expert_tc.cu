@@ -48,7 +48,7 @@ struct GemmParams {
 // buckets of up to 32, where the tiles are too few for the GPU: a cluster of CTAs shares each tile's K, and its first CTA adds the
 // parts, in order, out of its shared memory.
 enum Form { kSingle = 0, kPair = 1, kSplit = 2 };
-constexpr int kMaxParts = 6;   // 5 x 16 KB of sums of other CTAs in the first one's idle operand stages
+constexpr int kMaxParts = 4;   // 3 x 16 KB of sums of other CTAs in the first one's idle operand stages
 
 template <bool FP8, bool GATEUP, int FORM>
 struct Shape {
@@ -783,12 +783,43 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         }
       }
     };
-    if (first < n_tiles) {
-      look(first);
-      resolve();
-    }
     int st = 0;
     uint32_t par = 1;
+    // one stage of the matrix, and the announcement of the bytes of both CTAs' copies into it
+    auto issue = [&](const Tile &tl, int ks) {
+      const int y = tl.e * p.N + tl.n0 + (S::kRowsM && !GATEUP ? 128 * (int)rank : 0);
+      const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
+      if (elect_one()) {
+        const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : tl.ncol * 128));
+        if (rank == 0) mbar_expect_tx(&full[st], bytes * min(S::kSub, k_hi - ks));
+#pragma unroll
+        for (int u = 0; u < S::kSub; ++u) {
+          if (u > 0 && ks + u >= k_hi) break;
+          const uint32_t dst = smem_u32(smem + S::kOffA + (st * S::kSub + u) * S::kATile);
+          const int x = (ks + u) * S::kSlab;
+          if (S::kRowsM) {
+            tma_load_box<CG>(dst, GATEUP && rank ? &p.map1 : &p.map0, x, y, bar);
+          } else if (GATEUP) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              tma_load_box<CG>(dst + j * 4096, &p.map0, x, y + 16 * j, bar);
+              tma_load_box<CG>(dst + j * 4096 + 2048, &p.map1, x, y + 16 * j, bar);
+            }
+          } else {
+            tma_load_box<CG>(dst, &p.map0, x, y, bar);
+          }
+        }
+      }
+      __syncwarp();
+      if (++st == S::kStages) { st = 0; par ^= 1u; }
+    };
+    int ahead = k_lo;
+    if (first < n_tiles) {
+      look(first);
+      // the first stages are empty and the matrix depends on no table entry: it travels while those are read
+      for (int i = 0; i < S::kStages && ahead < k_hi; ++i, ahead += S::kSub) issue(next, ahead);
+      resolve();
+    }
     tpar = 1;
     int t = first;
     for (; t < n_tiles; split_end(t), t += step) {
@@ -806,37 +837,13 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         tslot = 0;
         tpar ^= 1u;
       }
-      const int y = tl.e * p.N + tl.n0 + (S::kRowsM && !GATEUP ? 128 * (int)rank : 0);
-      // of both CTAs, matrix and rows, per slab
-      const uint32_t bytes = (uint32_t)(CG * S::kATile + (p.dense ? CG * S::kBTile : tl.ncol * 128));
       const bool more = t + step < n_tiles;
-      for (int ks = k_lo; ks < k_hi; ks += S::kSub) {
+      if (more) look(t + step);
+      for (int ks = ahead; ks < k_hi; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
-        const uint32_t bar = CG == 2 ? cluster_addr(&full[st], 0) : smem_u32(&full[st]);
-        if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&full[st], bytes * min(S::kSub, k_hi - ks));
-#pragma unroll
-          for (int u = 0; u < S::kSub; ++u) {
-            if (u > 0 && ks + u >= k_hi) break;
-            const uint32_t dst = smem_u32(smem + S::kOffA + (st * S::kSub + u) * S::kATile);
-            const int x = (ks + u) * S::kSlab;
-            if (S::kRowsM) {
-              tma_load_box<CG>(dst, GATEUP && rank ? &p.map1 : &p.map0, x, y, bar);
-            } else if (GATEUP) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                tma_load_box<CG>(dst + j * 4096, &p.map0, x, y + 16 * j, bar);
-                tma_load_box<CG>(dst + j * 4096 + 2048, &p.map1, x, y + 16 * j, bar);
-              }
-            } else {
-              tma_load_box<CG>(dst, &p.map0, x, y, bar);
-            }
-          }
-        }
-        __syncwarp();
-        if (++st == S::kStages) { st = 0; par ^= 1u; }
-        if (ks == k_lo && more) look(t + step);
+        issue(tl, ks);
       }
+      ahead = k_lo;
       if (!ok) break;
       if (more) resolve();
     }
@@ -1009,8 +1016,8 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   const int experts = p.E < p.n_pairs ? p.E : p.n_pairs;
   const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
   int64_t parts = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
-  parts = parts > kMaxParts ? kMaxParts : parts;
-  parts = parts > nslab ? nslab : parts;
+  parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;   // powers of two fill a GPC's SMs; clusters of three took two rounds where 96 of them should fit
+  while (parts > nslab) parts /= 2;
   p.parts = 1;
   if (g_form == 3 || (g_form == 0 && parts >= 2)) {
     p.parts = parts < 1 ? 1 : (int)parts;
