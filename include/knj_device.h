@@ -555,6 +555,47 @@ size_t knj_fp8_matmul_workspace_bytes(int m, int n_in);
 int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, int64_t ldx, int m, void *y,
                           int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);
 
+/* A whole MoE block of a residual stream with experts in bf16, fp16 or e4m3 (Model::moe between rmsnorm_rows and the
+ * residual add, src/model/model.cpp:631-652, with what a block may have around it):
+ *   h   = norm(x; pre_w)                           rows in the experts' 16-bit type (bf16 for e4m3 experts, which read their
+ *                                                  e4m3 codes)
+ *   y   = sum over the top_k experts of softmax weight * down(silu(gate(h)) * up(h))
+ *   out = beta * x + alpha * g * norm(y; post_w)   and, for the next block, h_next = norm(out; next_w)
+ * as the launches above chained on one stream: block norm, router and tables, expert products, ordered combine, block norm.
+ * f16 experts: the product of gate and up is held scaled by 2^-6 (up to 4.1e6). hidden a multiple of 256, ffn of 16, at most
+ * 256 experts, top_k <= 8. The struct's norm weights are of one type (w_norm_dtype). Fields left zero are off; alpha and beta
+ * are taken as they are. */
+typedef struct knj_moe_block_args {
+  int32_t n_tokens, hidden, ffn, n_experts, top_k;
+  int32_t x_dtype, out_dtype, w_dtype, w_norm_dtype, gate_dtype, h_next_dtype;
+  int32_t gate_kind, gate_sigmoid;
+  float alpha, beta, eps;
+  const void *x;
+  int64_t ldx;
+  void *out; /* may be x */
+  int64_t ldo;
+  const void *pre_w, *post_w, *next_w; /* [hidden]; pre_w NULL: h = x, post_w NULL: no norm of y, next_w NULL: no h_next */
+  const void *gate;
+  int64_t ldg;
+  const uint16_t *w_router;  /* bf16 [n_experts][hidden] */
+  const float *router_bias;  /* f32 [n_experts] or NULL */
+  const void *w_gate, *w_up; /* [n_experts][ffn][hidden] */
+  const void *w_down;        /* [n_experts][hidden][ffn] */
+  const float *gate_scale, *up_scale, *down_scale; /* e4m3 */
+  void *h_next;
+  int64_t ld_h_next;
+  float *h_next_scale;
+  void *workspace; /* >= knj_moe_block_workspace_bytes(...), 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t *tap_pair_exp; /* optional [T*k] */
+  float *tap_pair_w;
+} knj_moe_block_args;
+size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype);
+int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
+/* Outcome of the last block launch over this argument block: waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a
+ * bounded wait of the expert products gave up. */
+int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s);
+
 /* ======================================================================== */
 /* Device-clock spans for a host profiler                                   */
 /* ======================================================================== */

@@ -52,6 +52,17 @@ class BlockNormArgs(C.Structure):
                 ("gate_sigmoid", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float)]
 
 
+class MoeBlockArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_tokens", "hidden", "ffn", "n_experts", "top_k", "x_dtype", "out_dtype", "w_dtype", "w_norm_dtype",
+                                         "gate_dtype", "h_next_dtype", "gate_kind", "gate_sigmoid")] + \
+               [("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64), ("out", C.c_void_p),
+                ("ldo", C.c_int64), ("pre_w", C.c_void_p), ("post_w", C.c_void_p), ("next_w", C.c_void_p), ("gate", C.c_void_p),
+                ("ldg", C.c_int64), ("w_router", C.c_void_p), ("router_bias", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p),
+                ("w_down", C.c_void_p), ("gate_scale", C.c_void_p), ("up_scale", C.c_void_p), ("down_scale", C.c_void_p),
+                ("h_next", C.c_void_p), ("ld_h_next", C.c_int64), ("h_next_scale", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("tap_pair_exp", C.c_void_p), ("tap_pair_w", C.c_void_p)]
+
+
 class ExpertGemmArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("x_scale", C.c_void_p), ("ldx", C.c_int64), ("w0", C.c_void_p), ("w1", C.c_void_p),
                 ("w0_scale", C.c_void_p), ("w1_scale", C.c_void_p), ("pair_idx", C.c_void_p), ("pair_cnt", C.c_void_p),
@@ -198,6 +209,9 @@ SIGNATURES = {
     "knj_block_norm_launch": (_i, [C.POINTER(BlockNormArgs), _vp]),
     "knj_expert_gateup_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
     "knj_expert_proj_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
+    "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "knj_moe_block_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
+    "knj_moe_block_status": (_i, [C.POINTER(MoeBlockArgs), _vp]),
     "knj_expert_tc_form": (None, [_i]),
     "knj_fp8_matmul_workspace_bytes": (_sz, [_i, _i]),
     "knj_fp8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),

@@ -487,9 +487,8 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const void *x, int dtype,
 
 }  // namespace
 
-extern "C" {
-
-int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
+namespace knj {
+int block_norm_check(const knj_block_norm_args *a) {
   KNJ_REQUIRE(a, "knj_block_norm: null argument block");
   KNJ_REQUIRE(a->n_tokens >= 0 && a->hidden > 0, "knj_block_norm: bad sizes");
   if (a->n_tokens == 0) return KNJ_OK;
@@ -510,6 +509,16 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
   KNJ_REQUIRE(a->ldx >= H && (!a->y || a->ldy >= H) && (!a->stream_out || a->ld_stream >= H) && (!a->h || a->ldh >= H) &&
                   (a->gate_kind != KNJ_GATE_FULL || a->ldg >= H) && (a->gate_kind != KNJ_GATE_ROW || a->ldg >= 1),
               "knj_block_norm: row strides shorter than the rows");
+  return KNJ_OK;
+}
+}  // namespace knj
+
+extern "C" {
+
+int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
+  const int rc = block_norm_check(a);
+  if (rc || a->n_tokens == 0) return rc;
+  const int H = a->hidden;
   NormParams p{};
   p.x = a->x; p.y = a->y; p.post_w = a->post_w; p.gate = a->gate; p.pre_w = a->pre_w; p.stream = a->stream_out; p.h = a->h;
   p.h_scale = a->h_scale; p.ldx = a->ldx; p.ldy = a->ldy; p.ldg = a->ldg; p.ld_stream = a->ld_stream; p.ldh = a->ldh;

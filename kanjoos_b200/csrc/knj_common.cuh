@@ -98,6 +98,9 @@ int make_gather_tensor_map(CUtensorMap *map, const void *base, uint64_t rows, ui
 // zero. With box_rows = 1 the map serves tile::gather4 copies.
 int make_operand_tensor_map(CUtensorMap *map, const void *base, int elem_bytes, uint64_t cols, uint64_t ld, uint64_t rows, uint32_t box_rows);
 
+// What knj_block_norm_launch checks of its arguments.
+int block_norm_check(const knj_block_norm_args *a);
+
 // Limit (SM clock cycles) of the bounded waits of the decode-class kernels, as set by knj_decode_wait_limit.
 long long decode_wait_cycles();
 

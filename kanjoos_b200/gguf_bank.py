@@ -165,6 +165,52 @@ def load_expert_bank(g: GgufFile, layer: int, device="cuda"):
     return bank, a["top_k"]
 
 
+def float_layer_arrays(g: GgufFile, layer: int) -> dict:
+    """Host arrays of one block's MoE-FFN tensors where the experts are not quantised: gate/up [E][F][H] and down [E][H][F] as
+    uint16 bit patterns (`expert_type` "f16" or "bf16", one type for the three), router and norm weights as bf16 bits."""
+    p = g.arch() + "."
+    E = g.meta_int(p + "expert_count")
+    b = f"blk.{layer}."
+    out = {"top_k": g.meta_int(p + "expert_used_count"),
+           "rms_eps": float(g.meta.get(p + "attention.layer_norm_rms_epsilon", 1e-6))}
+    types = set()
+    for key, name in (("gate", "ffn_gate_exps"), ("up", "ffn_up_exps"), ("down", "ffn_down_exps")):
+        info = g.require(b + name + ".weight")
+        if info.ggml_type not in (GGML_F16, GGML_BF16) or len(info.dims) != 3 or info.dims[2] != E:
+            raise ValueError(f"{info.name}: expected an F16 / BF16 tensor [in, out, {E}], got type {info.ggml_type} dims {info.dims}")
+        types.add(info.ggml_type)
+        n_in, n_out, _ = info.dims
+        out[key] = np.asarray(g.payload(info)).view(np.uint16).reshape(E, n_out, n_in)
+    if len(types) != 1:
+        raise ValueError(f"blk.{layer}: gate, up and down experts must be of one type")
+    out["expert_type"] = "f16" if types == {GGML_F16} else "bf16"
+    r = g.require(b + "ffn_gate_inp.weight")
+    out["router"] = _bf16_bits(r, np.asarray(g.payload(r))).reshape(r.dims[1], r.dims[0])
+    out["router_exact"] = r.ggml_type == GGML_BF16
+    for key, name in (("norm", "ffn_norm"), ("post_norm", "post_ffw_norm")):
+        n = g.tensors.get(b + name + ".weight")
+        if n is not None:
+            out[key] = _bf16_bits(n, np.asarray(g.payload(n)))
+            out[key + "_exact"] = n.ggml_type == GGML_BF16
+    return out
+
+
+def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = False):
+    """`FloatExpertBank` of block `layer` (F16 or BF16 experts; e4m3=True turns them into e4m3 blocks) and the block's top-k. A
+    `post_ffw_norm` tensor, where the file has one, becomes the norm behind the block."""
+    import torch
+    from .moe import FloatExpertBank
+    a = float_layer_arrays(g, layer)
+
+    def bits(u16, dtype):
+        return torch.from_numpy(np.ascontiguousarray(u16).view(np.int16).copy()).view(dtype).to(device)
+    kind = torch.float16 if a["expert_type"] == "f16" else torch.bfloat16
+    norm = {k: bits(a[n], torch.bfloat16) if n in a else None for k, n in (("pre_norm", "norm"), ("post_norm", "post_norm"))}
+    bank = FloatExpertBank(gate=bits(a["gate"], kind), up=bits(a["up"], kind), down=bits(a["down"], kind), router=bits(a["router"], torch.bfloat16),
+                           rms_eps=a["rms_eps"], **norm)
+    return (bank.to_e4m3() if e4m3 else bank), a["top_k"]
+
+
 def verify_against_gguf_py(path: str, names=None) -> int:
     """Every tensor this reader located holds the bytes gguf-py hands out for the same name; returns the
     number of tensors compared. Raises on the first mismatch."""

@@ -6,15 +6,17 @@ All arithmetic is done by libknj_device.so."""
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
 
 from . import synth
-from ._lib import DT_BF16, DT_F32, MoeFfnArgs, check, lib
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
+_DT_FLOAT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+_DT_EXPERT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float8_e4m3fn: DT_E4M3}
 
 
 @dataclass
@@ -236,3 +238,162 @@ class FusedMoeStack:
             self.close()
         except Exception:
             pass
+
+
+def e4m3_blocks(w: torch.Tensor):
+    """A matrix [..., N, K] as e4m3 codes and one f32 scale (largest magnitude / 448) for each block of 128 x 128, the form in
+    which ops.fp8_matmul and the expert products take it. Done once, when weights are loaded."""
+    n, k = w.shape[-2:]
+    nb, kb = -(-n // 128), -(-k // 128)
+    v = torch.nn.functional.pad(w.float(), (0, kb * 128 - k, 0, nb * 128 - n)).unflatten(-1, (kb, 128)).unflatten(-3, (nb, 128))
+    scale = v.abs().amax(dim=(-3, -1)) / 448.0
+    q = torch.where(scale[..., :, None, :, None] > 0, v / scale[..., :, None, :, None], torch.zeros_like(v)).clamp_(-448.0, 448.0)
+    return q.flatten(-2).flatten(-3, -2)[..., :n, :k].to(torch.float8_e4m3fn).contiguous(), scale.contiguous()
+
+
+@dataclass
+class FloatExpertBank:
+    """Weights of one MoE block whose experts are bf16, f16 or e4m3, all on one device.
+
+    gate, up [E][F][H]; down [E][H][F]; for e4m3 their scales f32 [E][ceil(rows/128)][ceil(cols/128)]; router bf16 [E][H];
+    router_bias f32 [E] or None; pre_norm, post_norm: norm weights [H] in front of the block and behind it (one type), or None;
+    out_gate [H]: what the block's output is multiplied with (through a sigmoid with gate_sigmoid), or None."""
+    gate: torch.Tensor
+    up: torch.Tensor
+    down: torch.Tensor
+    router: torch.Tensor
+    gate_scale: torch.Tensor | None = None
+    up_scale: torch.Tensor | None = None
+    down_scale: torch.Tensor | None = None
+    router_bias: torch.Tensor | None = None
+    pre_norm: torch.Tensor | None = None
+    post_norm: torch.Tensor | None = None
+    out_gate: torch.Tensor | None = None
+    gate_sigmoid: bool = False
+    alpha: float = 1.0
+    beta: float = 1.0
+    rms_eps: float = synth.RMS_EPS
+
+    @property
+    def n_experts(self) -> int:
+        return self.gate.shape[0]
+
+    @property
+    def ffn(self) -> int:
+        return self.gate.shape[1]
+
+    @property
+    def hidden(self) -> int:
+        return self.gate.shape[2]
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.gate, self.up, self.down))
+
+    def to_e4m3(self) -> "FloatExpertBank":
+        """The same block with its experts as e4m3 codes under block scales."""
+        parts = {}
+        for name in ("gate", "up", "down"):
+            parts[name], parts[name + "_scale"] = e4m3_blocks(getattr(self, name))
+        return replace(self, **parts)
+
+
+class MoeBlock:
+    """One MoE block of a residual stream (knj_moe_block_launch): norm, routing, experts, ordered combine, norm behind the block, gate,
+    scaled residual add and, on request, the norm in front of the next block. Bound to a maximum token count: the workspace is
+    allocated once here."""
+
+    def __init__(self, bank: FloatExpertBank, top_k: int = synth.TOP_K, max_tokens: int = 64, workspace: torch.Tensor | None = None):
+        E, F, H = bank.gate.shape
+        kind = bank.gate.dtype
+        if kind not in _DT_EXPERT or bank.up.dtype != kind or bank.down.dtype != kind:
+            raise ValueError("experts are bf16, f16 or float8_e4m3fn, all three matrices of one type")
+        want = {"gate": (E, F, H), "up": (E, F, H), "down": (E, H, F), "router": (E, H)}
+        if kind == torch.float8_e4m3fn:
+            want.update(gate_scale=(E, -(-F // 128), -(-H // 128)), up_scale=(E, -(-F // 128), -(-H // 128)), down_scale=(E, -(-H // 128), -(-F // 128)))
+        for name, shape in want.items():
+            t = getattr(bank, name)
+            if t is None or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:
+                raise ValueError(f"{name}: expected a contiguous CUDA tensor of shape {shape}")
+        if bank.router.dtype != torch.bfloat16:
+            raise ValueError("the router's weights are bf16")
+        norms = [w for w in (bank.pre_norm, bank.post_norm) if w is not None]
+        if any(tuple(w.shape) != (H,) or w.dtype not in _DT_FLOAT or w.dtype != norms[0].dtype or not w.is_contiguous() for w in norms):
+            raise ValueError(f"norm weights are contiguous [{H}] of one type")
+        if bank.out_gate is not None and (tuple(bank.out_gate.shape) != (H,) or bank.out_gate.dtype not in _DT_FLOAT or not bank.out_gate.is_contiguous()):
+            raise ValueError(f"out_gate is contiguous [{H}]")
+        if bank.router_bias is not None and (tuple(bank.router_bias.shape) != (E,) or bank.router_bias.dtype != torch.float32):
+            raise ValueError(f"router_bias is f32 [{E}]")
+        self.bank, self.top_k, self.max_tokens = bank, top_k, max_tokens
+        need = lib().knj_moe_block_workspace_bytes(max_tokens, H, F, E, top_k, _DT_EXPERT[kind])
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=bank.gate.device)
+        if workspace.numel() < need or workspace.data_ptr() % 256:
+            raise ValueError(f"workspace of {need} bytes, 256-byte aligned, needed")
+        self.workspace = workspace
+
+    def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:
+        b = self.bank
+        T, H = x.shape
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        a = MoeBlockArgs(n_tokens=T, hidden=H, ffn=b.ffn, n_experts=b.n_experts, top_k=self.top_k, x_dtype=_DT_FLOAT[x.dtype],
+                         out_dtype=_DT_FLOAT[out.dtype], w_dtype=_DT_EXPERT[b.gate.dtype], alpha=b.alpha, beta=b.beta, eps=b.rms_eps,
+                         gate_sigmoid=1 if b.gate_sigmoid else 0, x=x.data_ptr(), ldx=x.stride(0) if T > 1 else H, out=out.data_ptr(),
+                         ldo=out.stride(0) if T > 1 else H, pre_w=ptr(b.pre_norm), post_w=ptr(b.post_norm), next_w=ptr(next_norm),
+                         w_router=b.router.data_ptr(), router_bias=ptr(b.router_bias), w_gate=b.gate.data_ptr(), w_up=b.up.data_ptr(),
+                         w_down=b.down.data_ptr(), gate_scale=ptr(b.gate_scale), up_scale=ptr(b.up_scale), down_scale=ptr(b.down_scale),
+                         h_next=ptr(h_next), ld_h_next=H, h_next_scale=ptr(h_scale), workspace=self.workspace.data_ptr(),
+                         workspace_bytes=self.workspace.numel())
+        for w in (b.pre_norm, b.post_norm, next_norm):
+            if w is not None:
+                a.w_norm_dtype = _DT_FLOAT[w.dtype]
+        if gate is not None:
+            a.gate, a.gate_dtype = gate.data_ptr(), _DT_FLOAT[gate.dtype]
+            a.gate_kind = GATE_CHANNEL if gate.dim() == 1 else GATE_ROW if gate.shape[1] == 1 and H > 1 else GATE_FULL
+            a.ldg = 0 if gate.dim() == 1 else gate.stride(0) if T > 1 else gate.shape[1]
+        if h_next is not None:
+            a.h_next_dtype = DT_E4M3 if h_next.dtype == torch.float8_e4m3fn else _DT_FLOAT[h_next.dtype]
+        if taps is not None:
+            a.tap_pair_exp, a.tap_pair_w = taps[0].data_ptr(), taps[1].data_ptr()
+        return a
+
+    def run(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
+        """x [T][H] f32 / bf16 / f16 -> the stream behind the block, in x's type or into `out` (which may be x). gate: the rows' own
+        gate [T][1] or [T][H] in place of the bank's. next_norm [H]: also returns h = norm(out; next_norm) in next_dtype (default:
+        x's type; float8_e4m3fn: (codes, scale)). Returns out, or a tuple (out[, h][, pair_exp, pair_w])."""
+        b = self.bank
+        if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > self.max_tokens or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
+            raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {self.max_tokens}")
+        if x.device != b.gate.device or x.get_device() != torch.cuda.current_device():
+            raise ValueError(f"x lives on {x.device}, the block on {b.gate.device}; the current device is {torch.cuda.current_device()}")
+        T, H = x.shape
+        if out is None:
+            out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype not in _DT_FLOAT or out.device != x.device or out.stride(1) != 1:
+            raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected rows like x")
+        gate = b.out_gate if gate is None else gate
+        if gate is not None and gate.dim() == 2 and (gate.shape[0] != T or gate.shape[1] not in (1, H) or gate.device != x.device or
+                                                     gate.dtype not in _DT_FLOAT or (gate.shape[1] > 1 and gate.stride(1) != 1)):
+            raise ValueError(f"gate is {gate.dtype} {tuple(gate.shape)}, expected [{T}][1] or [{T}][{H}]")
+        if gate is not None and gate.dim() != 2 and gate is not b.out_gate:
+            raise ValueError("a call's gate has a row for each token")
+        h = scale = None
+        if next_norm is not None:
+            norms = [w for w in (b.pre_norm, b.post_norm) if w is not None]
+            if tuple(next_norm.shape) != (H,) or next_norm.dtype not in _DT_FLOAT or any(w.dtype != next_norm.dtype for w in norms) or \
+                    next_norm.device != x.device or not next_norm.is_contiguous():
+                raise ValueError(f"next_norm is {next_norm.dtype} {tuple(next_norm.shape)}, expected [{H}] in the block's norm type")
+            h = torch.empty((T, H), dtype=next_dtype or x.dtype, device=x.device)
+            if h.dtype == torch.float8_e4m3fn:
+                scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
+        taps = None
+        if return_routing:
+            taps = (torch.empty(T * self.top_k, dtype=torch.int32, device=x.device), torch.empty(T * self.top_k, dtype=torch.float32, device=x.device))
+        a = self._args(x, out, gate, next_norm, h, scale, taps)
+        check(lib().knj_moe_block_launch(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        self._last = a
+        result = (out,) + (() if h is None else ((h, scale) if scale is not None else h,)) + (taps or ())
+        return result if len(result) > 1 else out
+
+    def status(self) -> None:
+        """Waits for the stream; raises if a bounded wait of the last run gave up."""
+        check(lib().knj_moe_block_status(C.byref(self._last), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
