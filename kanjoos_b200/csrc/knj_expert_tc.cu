@@ -920,6 +920,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
             const int x = (ks + u) * S::kSlab;
             if (p.dense) {
               if (w == 0) tma_load_box<CG>(dst, &p.mapx, x, tl.tok0 + (int)rank * n_cta, bar);
+            } else if constexpr (S::kRowWarps == 1) {
+              // buckets are multiples of 16 rows: one branch for four copies (with one for each, skipped or not, a stage took this
+              // warp 1000 cycles whatever the bucket)
+#pragma unroll
+              for (int q = 0; q < kQuads; q += 4) {
+                if (4 * q >= n_cta) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tma_gather4<CG>(dst + (q + i) * 512, &p.mapx, x, rows[q + i], bar);
+              }
             } else {
 #pragma unroll
               for (int q = 0; q < kQuads; ++q) {
@@ -1013,17 +1022,27 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
 
 template <bool FP8, bool GATEUP>
 int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
-  const int experts = p.E < p.n_pairs ? p.E : p.n_pairs;
+  const int64_t experts = p.E < p.n_pairs ? p.E : p.n_pairs;
   const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
+  // K is split where even the smallest tiles leave half of the CTAs' places free, into parts of two slabs or more: one row times
+  // 4096 x 4096 e4m3 23.6 -> 17.4 us, 64 rows 31.7 -> 21.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
+  // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two take 16.4).
   int64_t parts = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
-  parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;   // powers of two fill a GPC's SMs; clusters of three took two rounds where 96 of them should fit
-  while (parts > nslab) parts /= 2;
+  parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
+  while (parts > 1 && 2 * parts > nslab) parts /= 2;
   p.parts = 1;
   if (g_form == 3 || (g_form == 0 && parts >= 2)) {
-    p.parts = parts < 1 ? 1 : (int)parts;
+    p.parts = (int)parts;
     return launch_form<FP8, GATEUP, kSplit>(p, o, st);
   }
-  const bool pairs = g_form ? g_form == 2 : (int64_t)p.n_pairs > 32ll * experts;
+  // Pairs or single SMs, us by (rows per expert; experts): 16 bits, gate and up, hidden 2048, ffn 768: 92 single, 90 pair (1; 128),
+  // 162, 141 (32, Zipf; 128), 297, 154 (128; 128); hidden 1024, ffn 512: 18.5, 20.5 (1; 32), 22.6, 22.6 (32; 32), 33, 25 (64; 32) --
+  // pairs where the buckets fill them or the tiles take four rounds of pairs anyway. e4m3, whose pairs always multiply 256 rows and
+  // whose stores no product overlaps: 82, 152 (4; 128), 121, 156 (64; 128), 186, 158 (128; 128), 336, 217 (256; 128), down
+  // products over K = 512 47, 53 (512; 32); 2048 rows x 1000 x 2048 26, 69 (32 tiles of pairs).
+  const int64_t pair_tiles = most_tiles<Shape<FP8, GATEUP, kPair>>(p), round = sm_count() / 2;
+  bool pairs = FP8 ? p.n_pairs >= 128 * experts && nslab >= 6 && pair_tiles >= round : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
+  if (g_form) pairs = g_form == 2;
   return pairs ? launch_form<FP8, GATEUP, kPair>(p, o, st) : launch_form<FP8, GATEUP, kSingle>(p, o, st);
 }
 template <bool GATEUP>
