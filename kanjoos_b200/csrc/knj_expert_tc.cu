@@ -228,32 +228,34 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   __syncthreads();
   if (CG == 2 || SPLIT) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  // what comes out of shared memory and feeds issuing loops goes through a shuffle: the compiler then knows it is the same in all
+  // lanes and keeps it, and what is derived from it, in uniform registers
+  auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+  const uint32_t tmem_base = same(*tmem_slot);
 
   const int nslab = (p.K + S::kSlab - 1) / S::kSlab;
-  const int n_tiles = s_pref[kMaxExperts] * p.m_tiles;   // < 2^31: checked on the host
+  const int n_tiles = same(s_pref[kMaxExperts]) * p.m_tiles;   // < 2^31: checked on the host
   // As many CTAs (pairs) as take part in whole rounds: of 1536 tiles on 296 CTAs, 256 take six each instead of 56 a sixth; the matrices
   // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
   const int k_lo = part * nslab / parts, k_hi = (part + 1) * nslab / parts;   // this CTA's slabs
   const int avail = gridDim.x / (CG * parts), rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
   const int first = (int)(blockIdx.x / (CG * parts)) < step ? blockIdx.x / (CG * parts) : n_tiles;
-      auto tile_at = [&](int t, int &ntok) {
-        const int b = t / p.m_tiles, mt = t - b * p.m_tiles;
-        int lo = 0;  // the last expert whose first bucket is not behind b
-  #pragma unroll
-        for (int h = kMaxExperts / 2; h > 0; h >>= 1)
-          if (s_pref[lo + h] <= b) lo += h;
-        const int nb = s_pref[lo + 1] - s_pref[lo], cnt = s_cnt[lo];
-        // an expert's pairs are spread evenly over its buckets: 256 + 14 pairs would stream the matrix twice for 14
-        const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
-        Tile r;
-        r.e = lo;
-        r.n0 = (mt * CG + (S::kRowsM ? 0 : (int)rank)) * S::kOuts;
-        r.tok0 = (b - s_pref[lo]) * per;
-        ntok = min(per, cnt - r.tok0);
-        r.ncol = (ntok + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
-        return r;
-      };
+  auto tile_at = [&](int t, int &ntok) {   // by a whole warp
+    const int b = t / p.m_tiles, mt = t - b * p.m_tiles;
+    // the last expert whose first bucket is not behind b: of 32 groups of eight experts, then of the eight
+    const int g = 8 * (__popc(__ballot_sync(0xffffffffu, s_pref[8 * lane] <= b)) - 1);
+    const int e = g + __popc(__ballot_sync(0xffffffffu, s_pref[g + (lane & 7)] <= b) & 0xffu) - 1;
+    const int b0 = same(s_pref[e]), nb = same(s_pref[e + 1]) - b0, cnt = same(s_cnt[e]);
+    // an expert's pairs are spread evenly over its buckets: 256 + 14 pairs would stream the matrix twice for 14
+    const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
+    Tile r;
+    r.e = e;
+    r.n0 = (mt * CG + (S::kRowsM ? 0 : (int)rank)) * S::kOuts;
+    r.tok0 = (b - b0) * per;
+    ntok = min(per, cnt - r.tok0);
+    r.ncol = (ntok + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
+    return r;
+  };
   // pair and row of column c of a tile: pair -1: none; pair -2 - p: p's row lies outside x, its output is zero
   auto pair_at = [&](const Tile &tl, int ntok, int c) {
     return c < ntok ? (p.pair_idx ? p.pair_idx[tl.e * p.idx_stride + tl.tok0 + c] : tl.tok0 + c) : -1;
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   auto tile_take = [&](Tile &tl) {
     if (!wait(&tile_full[tslot], tpar)) return false;
     const int4 v = s_tile[tslot];
-    tl = Tile{v.x, v.y, v.z, v.w};
+    tl = Tile{same(v.x), same(v.y), same(v.z), same(v.w)};
     return true;
   };
   auto tile_done = [&] {
@@ -850,8 +852,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     split_give_up(t, 0);
   } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
     // =========================== scales ===========================
-    // Asynchronous copies of four bytes, four blocks of K to a group: read into registers, a group had to wait for its loads, and an
-    // L2 or HBM latency for four blocks set the pace (8192 x 4096 x 4096: 166 us beside SCALES_NOW).
+    // Asynchronous copies of four bytes, four blocks of K to a group: this warp never waits for a load, only for a free group of the
+    // ring. (Loads into registers a group ahead were as fast where HBM or L2 is quiet, 8192 x 4096 x 4096: 166 and 171 us.)
     constexpr int kPer = S::kVecRows / 32 / S::kScaleWarps;   // rows per lane
     const int nb_n = (p.N + 127) / 128, c0 = (warp - S::kScaleWarp) * 32 * kPer + lane;
     int sg = 0;
