@@ -63,67 +63,78 @@ __device__ __forceinline__ Raw8 load_raw8(const void *base, int64_t i) {
   }
   return r;
 }
-__device__ __forceinline__ void unpack16(const uint4 &u, bool bf16, float (&v)[8]) {
+// the branch on the type stands outside the loop: inside, both conversions of every value are formed and one is picked
+__device__ __forceinline__ void unpack16(const uint4 &u, bool bf16, float2 (&v)[4]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (bf16) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (bf16) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
   }
 }
 template <bool WIDE>
-__device__ __forceinline__ void values8(const Raw8 &r, bool bf16, float (&v)[8]) {
+__device__ __forceinline__ void values8(const Raw8 &r, bool bf16, float2 (&v)[4]) {
   if constexpr (WIDE) {
     const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
   } else {
     unpack16(r.a, bf16, v);
   }
 }
-__device__ __forceinline__ void load8(const void *base, int dtype, int64_t i, float (&v)[8]) {
+__device__ __forceinline__ void load8(const void *base, int dtype, int64_t i, float2 (&v)[4]) {
   if (dtype == KNJ_DT_F32) values8<true>(load_raw8<true>(base, i), false, v);
   else values8<false>(load_raw8<false>(base, i), dtype == KNJ_DT_BF16, v);
 }
-__device__ __forceinline__ void store8(void *base, int dtype, int64_t i, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void *base, int dtype, const float2 (&v)[4]) {
   if (dtype == KNJ_DT_F32) {
-    float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(base) + i);
-    q[0] = make_float4(v[0], v[1], v[2], v[3]);
-    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    float4 *q = static_cast<float4 *>(base);
+    q[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    q[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     return;
   }
   uint32_t w[4];
+  if (dtype == KNJ_DT_BF16) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (dtype == KNJ_DT_BF16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 h = __float22bfloat162_rn(v[j]);
       w[j] = *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __float22half2_rn(v[j]);
       w[j] = *reinterpret_cast<const uint32_t *>(&h);
     }
   }
-  *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  *static_cast<uint4 *>(base) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-// sixteen lanes hold a group of 128: the scale, and this lane's eight codes
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float &scale) {
-  float most = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) most = max_nan(most, fabsf(v[j]));
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const Fp8Scale sc = fp8_scale(most);
-  scale = sc.scale;
+__device__ __forceinline__ float2 mul2(float2 a, float b) { return __fmul2_rn(a, make_float2(b, b)); }
+__device__ __forceinline__ float2 sigmoid2(float2 g) {
+  return make_float2(__fdividef(1.0f, 1.0f + expf(-g.x)), __fdividef(1.0f, 1.0f + expf(-g.y)));
+}
+__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], float inverse) {
   uint32_t c[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = e4m3_pair(v[2 * j] * sc.inverse, v[2 * j + 1] * sc.inverse);
+  for (int j = 0; j < 4; ++j) {
+    const float2 q = mul2(v[j], inverse);
+    c[j] = e4m3_pair(q.x, q.y);
+  }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+// scale of a group that LANES lanes in a row hold, RUNS runs of eight values each
+template <int LANES, int RUNS>
+__device__ __forceinline__ Fp8Scale group_scale(const float2 (*v)[4]) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = max3_abs_nan(most, v[r][j].x, v[r][j].y);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  return fp8_scale(most);
 }
 
 // sum over the CTA; `red` has two rows of 16 (zero behind the CTA's warps), used in turn, so that one barrier a sum is enough
@@ -145,14 +156,15 @@ __device__ __forceinline__ float cta_sum(float v, float (*red)[16], int &turn) {
   return ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
 }
 
-// One CTA walks over rows; thread i holds the elements 8 (i + blockDim c) .. + 7, c < NC, of each, and of the weights: post_w with a
-// gate per channel and alpha folded in, so that a row costs a dozen operations a value (formed anew for each row, and with the
-// gate's exponential, 57: 16384 rows of 2048 took 106 us, issue slots half full). RING: the next rows travel through a ring of
+// One CTA walks over rows; a thread holds NC runs of eight values of each, and of the weights: post_w with a gate per channel and
+// alpha folded in, so that a row costs a dozen operations a value (formed anew for each row, and with the gate's exponential, 57:
+// 16384 rows of 2048 took 106 us, issue slots half full). Eight threads in a row hold sixteen runs in turn, a group of e4m3 codes
+// (NC = 1: sixteen threads). RING: the next rows travel through a ring of
 // `depth` rows in shared memory, bulk copies on a barrier each; a row ahead in registers was 24 KB under way per SM, too few for
 // HBM (74 us). Without it, one row per CTA straight into registers: bound by the launch and two dependent sums.
 constexpr int kMaxRing = 8;
 template <int NC, bool XW, int Y, bool RING>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
-__global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(const NormParams p, const int depth) {
+__global__ void __launch_bounds__(NC == 1 ? 256 : 512, NC == 1 ? 4 : 1) block_norm_vec_kernel(const NormParams p, const int depth) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(16) float red[2][16];
   __shared__ uint64_t bars[kMaxRing];
@@ -161,7 +173,8 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
   if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
   __syncthreads();
   grid_dep_wait();
-  const int tid = threadIdx.x, step = blockDim.x, H8 = p.H >> 3;
+  constexpr int kLanes = NC == 1 ? 16 : 8;
+  const int tid = threadIdx.x, H8 = p.H >> 3, first = (tid / kLanes) * (kLanes * NC) + tid % kLanes;   // runs first + kLanes c
   const bool xb = p.x_dtype == KNJ_DT_BF16, yb = p.y_dtype == KNJ_DT_BF16;
   Raw8 xr[NC], yr[NC];
   const int x_bytes = p.H * (XW ? 4 : 2), y_bytes = Y == 0 ? 0 : p.H * (Y == 2 ? 4 : 2);
@@ -174,7 +187,7 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
   auto fetch = [&](const void *x, const void *y, int64_t xo, int64_t yo) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int i = tid + step * c;
+      const int i = first + kLanes * c;
       if (i < H8) {
         xr[c] = load_raw8<XW>(x, xo + 8 * i);
         if constexpr (Y != 0) yr[c] = load_raw8<Y == 2>(y, yo + 8 * i);
@@ -194,31 +207,31 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
     fetch(p.x, p.y, blockIdx.x * p.ldx, blockIdx.x * p.ldy);
   }
   // alpha * post_w * gate per channel, and pre_w; kept in registers where they fit, else formed for each row
-  auto post_of = [&](int c, float (&f)[8]) {
-    const int i = tid + step * c;
+  auto post_of = [&](int c, float2 (&f)[4]) {
+    const int i = first + kLanes * c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = p.alpha;
+    for (int j = 0; j < 4; ++j) f[j] = make_float2(p.alpha, p.alpha);
     if (Y == 0 || i >= H8) return;
-    float w[8];
+    float2 w[4];
     if (p.post_w) {
       load8(p.post_w, p.w_dtype, 8 * i, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= w[j];
+      for (int j = 0; j < 4; ++j) f[j] = __fmul2_rn(f[j], w[j]);
     }
     if (p.gate_kind == KNJ_GATE_CHANNEL) {
       load8(p.gate, p.gate_dtype, 8 * i, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[j])) : w[j];
+      for (int j = 0; j < 4; ++j) f[j] = __fmul2_rn(f[j], p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
     }
   };
-  auto pre_of = [&](int c, float (&f)[8]) {
-    const int i = tid + step * c;
+  auto pre_of = [&](int c, float2 (&f)[4]) {
+    const int i = first + kLanes * c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    for (int j = 0; j < 4; ++j) f[j] = make_float2(0.f, 0.f);
     if (p.h && i < H8) load8(p.pre_w, p.w_dtype, 8 * i, f);
   };
   constexpr bool kKeep = NC <= 2;
-  float post[kKeep ? NC : 1][8], pre[kKeep ? NC : 1][8];
+  float2 post[kKeep ? NC : 1][4], pre[kKeep ? NC : 1][4];
   if constexpr (kKeep) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -226,16 +239,30 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
       pre_of(c, pre[c]);
     }
   }
+  // sum of squares over the row, of values * 2^-64 where `down`
+  auto squares = [&](const float2 (&v)[NC][4], bool down) {
+    float2 a = make_float2(0.f, 0.f), b = a;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float2 x = down ? mul2(v[c][j], kDown) : v[c][j], y = down ? mul2(v[c][j + 1], kDown) : v[c][j + 1];
+        a = __ffma2_rn(x, x, a);
+        b = __ffma2_rn(y, y, b);
+      }
+    a = __fadd2_rn(a, b);
+    return cta_sum(a.x + a.y, red, turn);
+  };
   const int groups = (p.H + kFp8Group - 1) / kFp8Group;
   int slot = 0;
   uint32_t phase = 0;
   // where this thread's first run of the row lies in what is written, moved on row by row
   const int s_esz = p.stream_dtype == KNJ_DT_F32 ? 4 : 2, h_esz = p.h_dtype == KNJ_DT_E4M3 ? 1 : p.h_dtype == KNJ_DT_F32 ? 4 : 2;
-  uint8_t *s_at = static_cast<uint8_t *>(p.stream) + (blockIdx.x * p.ld_stream + 8 * tid) * s_esz;
-  uint8_t *h_at = static_cast<uint8_t *>(p.h) + (blockIdx.x * p.ldh + 8 * tid) * h_esz;
+  uint8_t *s_at = static_cast<uint8_t *>(p.stream) + (blockIdx.x * p.ld_stream + 8 * first) * s_esz;
+  uint8_t *h_at = static_cast<uint8_t *>(p.h) + (blockIdx.x * p.ldh + 8 * first) * h_esz;
   const int64_t s_step = gridDim.x * p.ld_stream * s_esz, h_step = gridDim.x * p.ldh * h_esz;
   for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step) {
-    float s[NC][8], n[NC][8];
+    float2 s[NC][4], n[NC][4];
     bool landed = true;
     if constexpr (RING) {
       landed = mbar_wait(&bars[slot], phase, &s_fail);
@@ -244,14 +271,19 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const bool in = tid + step * c < H8;
+      const bool in = first + kLanes * c < H8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[c][j] = n[c][j] = 0.f;
+      for (int j = 0; j < 4; ++j) s[c][j] = n[c][j] = make_float2(0.f, 0.f);
       if (in) values8<XW>(xr[c], xb, s[c]);
       if (Y != 0 && in) values8<Y == 2>(yr[c], yb, n[c]);
     }
     if constexpr (RING) {
-      if (!landed) s[0][0] = __int_as_float(0x7fffffff);   // a wait gave up: the row's outputs are NaN
+      if (!landed) {   // the wait gave up: NaN is stored
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[c][j].x = s[c][j].y = __int_as_float(0x7fffffff);
+      }
       __syncthreads();                                     // every thread has its part of the row
       if (tid == 0 && t + (int64_t)depth * gridDim.x < p.T) {
         fence_proxy_async();                               // the slot was read through the generic proxy
@@ -263,62 +295,49 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
       }
     }
     float rs = 1.f;
-    if (Y != 0 && p.post_w) {
-      auto squares = [&](float down) {
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss = fmaf(n[c][j] * down, n[c][j] * down, ss);
-        return cta_sum(ss, red, turn);
-      };
-      rs = rms_inverse(squares(1.f), p.inv_h, p.eps, [&] { return squares(kDown); });
-    }
+    if (Y != 0 && p.post_w) rs = rms_inverse(squares(n, false), p.inv_h, p.eps, [&] { return squares(n, true); });
     if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
-    float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int i = tid + step * c;
+      const int i = first + kLanes * c;
       if (!kKeep) post_of(c, post[0]);
       if (i < H8) {
         if (Y != 0 && p.gate_kind == KNJ_GATE_FULL) {
-          float w[8];
+          float2 w[4];
           load8(p.gate, p.gate_dtype, t * p.ldg + 8 * i, w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) n[c][j] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[j])) : w[j];
+          for (int j = 0; j < 4; ++j) n[c][j] = __fmul2_rn(n[c][j], p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          s[c][j] *= p.beta;
-          if constexpr (Y != 0) s[c][j] = fmaf(n[c][j] * rs, post[kKeep ? c : 0][j], s[c][j]);
+        for (int j = 0; j < 4; ++j) {
+          s[c][j] = mul2(s[c][j], p.beta);
+          if constexpr (Y != 0) s[c][j] = __ffma2_rn(mul2(n[c][j], rs), post[kKeep ? c : 0][j], s[c][j]);
         }
-        if (p.stream) store8(s_at + 8 * step * c * s_esz, p.stream_dtype, 0, s[c]);
+        if (p.stream) store8(s_at + 8 * kLanes * c * s_esz, p.stream_dtype, s[c]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(s[c][j], s[c][j], ss);
     }
     if (!p.h) continue;
-    const float hs = rms_inverse(cta_sum(ss, red, turn), p.inv_h, p.eps, [&] {
-      float q = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q = fmaf(s[c][j] * kDown, s[c][j] * kDown, q);
-      return cta_sum(q, red, turn);
-    });
+    const float hs = rms_inverse(squares(s, false), p.inv_h, p.eps, [&] { return squares(s, true); });
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int i = tid + step * c;
       if (!kKeep) pre_of(c, pre[0]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[c][j] *= hs * pre[kKeep ? c : 0][j];   // zeros behind the row
-      if (p.h_dtype != KNJ_DT_E4M3) {
-        if (i < H8) store8(h_at + 8 * step * c * h_esz, p.h_dtype, 0, s[c]);
-      } else {
-        float scale;
-        const uint2 q = codes8(s[c], scale);   // every lane takes part
-        if (i < H8) *reinterpret_cast<uint2 *>(h_at + 8 * step * c) = q;
-        if (i < H8 && (i & 15) == 0) p.h_scale[t * groups + (i >> 4)] = scale;
+      for (int j = 0; j < 4; ++j) s[c][j] = __fmul2_rn(s[c][j], mul2(pre[kKeep ? c : 0][j], hs));   // zeros behind the row
+    }
+    if (p.h_dtype != KNJ_DT_E4M3) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (first + kLanes * c < H8) store8(h_at + 8 * kLanes * c * h_esz, p.h_dtype, s[c]);
+    } else {
+      constexpr int kRuns = 16 / kLanes;   // of a thread in a group
+#pragma unroll
+      for (int c = 0; c < NC; c += kRuns) {
+        const Fp8Scale sc = group_scale<kLanes, kRuns>(&s[c]);   // every lane takes part
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r)
+          if (first + kLanes * (c + r) < H8) *reinterpret_cast<uint2 *>(h_at + 8 * kLanes * (c + r)) = codes8(s[c + r], sc.inverse);
+        const int i = first + kLanes * c;
+        if (i < H8 && (i & 15) == 0) p.h_scale[t * groups + (i >> 4)] = sc.scale;
       }
     }
   }
@@ -327,7 +346,7 @@ __global__ void __launch_bounds__(NC == 1 ? 256 : 512) block_norm_vec_kernel(con
 template <int NC, bool RING>
 cudaError_t launch_vec(const NormParams &p, int threads, unsigned ctas, int depth, size_t smem, cudaStream_t st) {
   auto go = [&](auto kern) {
-    if (smem > 48 * 1024) {
+    if (smem > 40 * 1024) {   // 48 KB less the static part need no opt-in
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
       if (e != cudaSuccess) return e;
     }
@@ -356,37 +375,41 @@ cudaError_t launch_vec(const NormParams &p, int threads, cudaStream_t st) {
   return launch_vec<NC, true>(p, threads, (unsigned)ctas, depth, depth * row, st);
 }
 
-// Eight values per lane, sixteen lanes per group; each lane has kUnroll groups' loads under way.
-constexpr int kRowsUnroll = 4;
+// Eight lanes per group, two runs of eight values each; each lane has kRowsUnroll groups' loads under way.
+constexpr int kRowsUnroll = 2;
 template <bool XW>
 __global__ void __launch_bounds__(256) fp8_rows_vec_kernel(const void *x, int dtype, int64_t ldx, int rows, int K8, int groups, uint8_t *q,
                                                            float *scale) {
   grid_dep_wait();
   if (gridDim.x <= 148u) grid_dep_signal();
-  const int lane16 = threadIdx.x & 15;
-  const int64_t n = (int64_t)rows * groups, stride = (int64_t)gridDim.x * 16;
-  for (int64_t g0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); __any_sync(0xffffffffu, g0 < n); g0 += stride * kRowsUnroll) {
-    Raw8 r[kRowsUnroll];
-    int64_t row[kRowsUnroll];
+  const int lane8 = threadIdx.x & 7;
+  const int64_t n = (int64_t)rows * groups, stride = (int64_t)gridDim.x * 32;
+  for (int64_t g0 = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); __any_sync(0xffffffffu, g0 < n); g0 += stride * kRowsUnroll) {
+    Raw8 r[kRowsUnroll][2];
+    int64_t at[kRowsUnroll];   // first run of the lane, in runs of the codes
     int i[kRowsUnroll];
 #pragma unroll
     for (int u = 0; u < kRowsUnroll; ++u) {
-      const int64_t g = g0 + u * stride;
-      row[u] = n <= 0x7fffffff ? (int64_t)((uint32_t)g / (uint32_t)groups) : g / groups;
-      i[u] = (int)(g - row[u] * groups) * 16 + lane16;
+      const int64_t g = g0 + u * stride, row = n <= 0x7fffffff ? (int64_t)((uint32_t)g / (uint32_t)groups) : g / groups;
+      i[u] = (int)(g - row * groups) * 16 + lane8;
       if (g >= n) i[u] = K8;
-      r[u].a = r[u].b = make_uint4(0, 0, 0, 0);
-      if (i[u] < K8) r[u] = load_raw8<XW>(x, row[u] * ldx + 8 * i[u]);
+      at[u] = row * K8 + i[u];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        r[u][h].a = r[u][h].b = make_uint4(0, 0, 0, 0);
+        if (i[u] + 8 * h < K8) r[u][h] = load_raw8<XW>(x, row * ldx + 8 * (i[u] + 8 * h));
+      }
     }
 #pragma unroll
     for (int u = 0; u < kRowsUnroll; ++u) {
-      float v[8], sc;
-      values8<XW>(r[u], dtype == KNJ_DT_BF16, v);
-      const uint2 c = codes8(v, sc);
-      if (i[u] < K8) {
-        *reinterpret_cast<uint2 *>(q + (row[u] * K8 + i[u]) * 8) = c;
-        if (lane16 == 0) scale[row[u] * groups + (i[u] >> 4)] = sc;
-      }
+      float2 v[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) values8<XW>(r[u][h], dtype == KNJ_DT_BF16, v[h]);
+      const Fp8Scale sc = group_scale<8, 2>(v);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (i[u] + 8 * h < K8) *reinterpret_cast<uint2 *>(q + (at[u] + 8 * h) * 8) = codes8(v[h], sc.inverse);
+      if (lane8 == 0 && i[u] < K8) scale[g0 + u * stride] = sc.scale;
     }
   }
 }
@@ -556,8 +579,8 @@ int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K
   const int groups = (K + kFp8Group - 1) / kFp8Group;
   const int64_t n = (int64_t)rows * groups, cap = (int64_t)sm_count() * 32;
   if (K % 8 == 0 && aligned16(x) && ldx * (x_dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0 && aligned16(q)) {
-    // four groups of sixteen lanes each: as many CTAs as one pass needs, up to eight per SM
-    const int64_t want = (n + 16 * kRowsUnroll - 1) / (16 * kRowsUnroll), few = n < 16ll * sm_count() * kRowsUnroll ? (n + 15) / 16 : want;
+    // 32 groups of a CTA at a time: as many CTAs as one pass needs, up to eight per SM
+    const int64_t want = (n + 32 * kRowsUnroll - 1) / (32 * kRowsUnroll), few = n < 32ll * sm_count() * kRowsUnroll ? (n + 31) / 32 : want;
     const dim3 grid((unsigned)(few < cap / 4 ? few : cap / 4));
     if (x_dtype == KNJ_DT_F32)
       KNJ_CUDA(launch_chain(fp8_rows_vec_kernel<true>, grid, dim3(256), 0, as_stream(s), x, x_dtype, ldx, rows, K / 8, groups, static_cast<uint8_t *>(q), scale));

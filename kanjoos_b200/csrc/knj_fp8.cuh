@@ -19,6 +19,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// max(a, |b|, |c|) of a >= 0 or NaN, one instruction
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // e4m3 codes of (lo, hi) in the low and high byte; magnitudes above 448 saturate, NaN stays NaN
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   uint16_t r;
