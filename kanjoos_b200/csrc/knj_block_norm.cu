@@ -375,42 +375,32 @@ cudaError_t launch_vec(const NormParams &p, int threads, cudaStream_t st) {
   return launch_vec<NC, true>(p, threads, (unsigned)ctas, depth, depth * row, st);
 }
 
-// Eight lanes per group, two runs of eight values each; each lane has kRowsUnroll groups' loads under way.
-constexpr int kRowsUnroll = 2;
+// Eight lanes per group, two runs of eight values each. The loop is short on purpose: 40 registers keep six CTAs on an SM, and their
+// loads cover HBM's latency (8192 x 4096 bf16: 24.6 us with the launch, 101 MB; a group or three more per lane under way: 24.6 and 28.7).
+constexpr int kRowsCtas = 6;
 template <bool XW>
-__global__ void __launch_bounds__(256) fp8_rows_vec_kernel(const void *x, int dtype, int64_t ldx, int rows, int K8, int groups, uint8_t *q,
-                                                           float *scale) {
+__global__ void __launch_bounds__(256, kRowsCtas) fp8_rows_vec_kernel(const void *x, int dtype, int64_t ldx, int rows, int K8, int groups,
+                                                                      uint8_t *q, float *scale) {
   grid_dep_wait();
   if (gridDim.x <= 148u) grid_dep_signal();
   const int lane8 = threadIdx.x & 7;
   const int64_t n = (int64_t)rows * groups, stride = (int64_t)gridDim.x * 32;
-  for (int64_t g0 = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); __any_sync(0xffffffffu, g0 < n); g0 += stride * kRowsUnroll) {
-    Raw8 r[kRowsUnroll][2];
-    int64_t at[kRowsUnroll];   // first run of the lane, in runs of the codes
-    int i[kRowsUnroll];
+  for (int64_t g = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); __any_sync(0xffffffffu, g < n); g += stride) {
+    const int64_t row = n <= 0x7fffffff ? (int64_t)((uint32_t)g / (uint32_t)groups) : g / groups;
+    const int i = g < n ? (int)(g - row * groups) * 16 + lane8 : K8;
+    float2 v[2][4];
 #pragma unroll
-    for (int u = 0; u < kRowsUnroll; ++u) {
-      const int64_t g = g0 + u * stride, row = n <= 0x7fffffff ? (int64_t)((uint32_t)g / (uint32_t)groups) : g / groups;
-      i[u] = (int)(g - row * groups) * 16 + lane8;
-      if (g >= n) i[u] = K8;
-      at[u] = row * K8 + i[u];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        r[u][h].a = r[u][h].b = make_uint4(0, 0, 0, 0);
-        if (i[u] + 8 * h < K8) r[u][h] = load_raw8<XW>(x, row * ldx + 8 * (i[u] + 8 * h));
-      }
+    for (int h = 0; h < 2; ++h) {
+      Raw8 r;
+      r.a = r.b = make_uint4(0, 0, 0, 0);
+      if (i + 8 * h < K8) r = load_raw8<XW>(x, row * ldx + 8 * (i + 8 * h));
+      values8<XW>(r, dtype == KNJ_DT_BF16, v[h]);
     }
+    const Fp8Scale sc = group_scale<8, 2>(v);
 #pragma unroll
-    for (int u = 0; u < kRowsUnroll; ++u) {
-      float2 v[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) values8<XW>(r[u][h], dtype == KNJ_DT_BF16, v[h]);
-      const Fp8Scale sc = group_scale<8, 2>(v);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (i[u] + 8 * h < K8) *reinterpret_cast<uint2 *>(q + (at[u] + 8 * h) * 8) = codes8(v[h], sc.inverse);
-      if (lane8 == 0 && i[u] < K8) scale[g0 + u * stride] = sc.scale;
-    }
+    for (int h = 0; h < 2; ++h)
+      if (i + 8 * h < K8) *reinterpret_cast<uint2 *>(q + (row * K8 + i + 8 * h) * 8) = codes8(v[h], sc.inverse);
+    if (lane8 == 0 && i < K8) scale[g] = sc.scale;
   }
 }
 
@@ -579,9 +569,8 @@ int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K
   const int groups = (K + kFp8Group - 1) / kFp8Group;
   const int64_t n = (int64_t)rows * groups, cap = (int64_t)sm_count() * 32;
   if (K % 8 == 0 && aligned16(x) && ldx * (x_dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0 && aligned16(q)) {
-    // 32 groups of a CTA at a time: as many CTAs as one pass needs, up to eight per SM
-    const int64_t want = (n + 32 * kRowsUnroll - 1) / (32 * kRowsUnroll), few = n < 32ll * sm_count() * kRowsUnroll ? (n + 31) / 32 : want;
-    const dim3 grid((unsigned)(few < cap / 4 ? few : cap / 4));
+    const int64_t want = (n + 31) / 32, most = (int64_t)kRowsCtas * sm_count();
+    const dim3 grid((unsigned)(want < most ? want : most));
     if (x_dtype == KNJ_DT_F32)
       KNJ_CUDA(launch_chain(fp8_rows_vec_kernel<true>, grid, dim3(256), 0, as_stream(s), x, x_dtype, ldx, rows, K / 8, groups, static_cast<uint8_t *>(q), scale));
     else
