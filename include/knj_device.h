@@ -517,14 +517,14 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s);
 
 /* Products of routed rows with expert matrices, grouped by expert, from one pair per expert to all pairs at one
  * (tables as knj_moe_permute_launch makes them; an expert without pairs is not read, rows of out that no table entry
- * names are left as they were):
+ * names are left as they were; one that several experts name holds the product with one of them):
  *   knj_expert_gateup_launch: out[p][n] = out_scale * silu(x[row(p)] . w0[e][n]) * (x[row(p)] . w1[e][n])
  *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
  * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
  * p / row_div. e4m3: x_scale [n_rows][ceil(K/128)], w*_scale [n_experts][ceil(N/128)][ceil(K/128)]; the sum over each 128
  * values of K is scaled and added in f32. N is any number, n_rows >= 1, K and ldx are whole 16-byte units, bases are 16-byte aligned.
  * out f32, bf16 or f16 [n_pairs][N], row stride ldo. Table entries outside [0, n_pairs) are skipped, rows outside
- * [0, n_rows) read as zeros. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
+ * [0, n_rows) read as zeros. out overlaps no operand; n_pairs and idx_stride are at most 2^30. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
  * the outputs it concerns are then NaN. */
 typedef struct knj_expert_gemm_args {
   const void *x;

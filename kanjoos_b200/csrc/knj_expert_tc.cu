@@ -29,6 +29,7 @@ using namespace knj;
 namespace {
 
 constexpr int kMaxExperts = 256;
+constexpr int64_t kMaxPairs = 1 << 30;   // sums of a count and a bucket's size stay in 32 bits
 
 struct GemmParams {
   const float *xs, *ws0, *ws1;
@@ -48,7 +49,7 @@ struct GemmParams {
 // buckets of up to 32, where the tiles are too few for the GPU: a cluster of CTAs shares each tile's K, and its first CTA adds the
 // parts, in order, out of its shared memory.
 enum Form { kSingle = 0, kPair = 1, kSplit = 2 };
-constexpr int kMaxParts = 4;   // 3 x 16 KB of sums of other CTAs in the first one's idle operand stages
+constexpr int kMaxParts = 4;
 
 template <bool FP8, bool GATEUP, int FORM>
 struct Shape {
@@ -88,6 +89,8 @@ struct Shape {
   static constexpr int kOffPref = kOffTile + kTiles * 16;                   // [E + 1] buckets before expert e, [E] pairs of it
   static constexpr int kOffBars = kOffPref + (2 * kMaxExperts + 4) * 4;
   static constexpr int kBytes = kOffBars + 320 + 1024;
+  // the sums of the other CTAs of a split tile wait in the first one's idle operand stages
+  static_assert(FORM != kSplit || (kMaxParts - 1) * kTok * 128 * 4 <= kStages * kSub * kATile, "sums of a split tile");
 };
 
 struct Tile {
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   const uint32_t tmem_base = same(*tmem_slot);
 
   const int nslab = (p.K + S::kSlab - 1) / S::kSlab;
-  const int n_tiles = same(s_pref[kMaxExperts]) * p.m_tiles;   // < 2^31: checked on the host
+  const int n_tiles = same(s_pref[kMaxExperts]) * p.m_tiles;   // at most 2^30: checked on the host
   // As many CTAs (pairs) as take part in whole rounds: of 1536 tiles on 296 CTAs, 256 take six each instead of 56 a sixth; the matrices
   // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
   const int k_lo = part * nslab / parts, k_hi = (part + 1) * nslab / parts;   // this CTA's slabs
@@ -548,8 +551,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         const int n_cta = ncol / CG;
         int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
         if (pr != -1) {
-          const float scale = pr < 0 ? 0.f : p.out_scale;
-          if (pr < 0) pr = -2 - pr;
+          const bool none = pr < 0;
+          if (none) pr = -2 - pr;
           auto value = [&](int c, int j) {   // output 16 c + j of this thread's row
             const unsigned long long w = acc[c][j >> 1];
             return __uint_as_float((uint32_t)((j & 1) ? w >> 32 : w));
@@ -562,7 +565,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
             for (int j = 0; j < 16; ++j) {
               f[j] = value(c, j);
               if constexpr (GATEUP) f[j] = __fdividef(f[j], 1.0f + __expf(-f[j])) * value(c + 4, j);
-              f[j] = scale == 0.f ? 0.f : f[j] * scale;
+              f[j] = none ? 0.f : f[j] * p.out_scale;
             }
             const int n = tl.n0 + group * 64 + (c & 3) * 16 + (c >> 2) * 128;
             if (n >= p.N) continue;
@@ -1001,7 +1004,7 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   const int out_esz = p.out_dtype == KNJ_DT_F32 ? 4 : 2, unit = S::kRowsM ? 32 : 16;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % unit == 0 && p.ldo * out_esz % unit == 0;
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
-  KNJ_REQUIRE(most * p.m_tiles < (1ll << 31) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
+  KNJ_REQUIRE(most * p.m_tiles <= (1ll << 30) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
   const int64_t tiles = most_tiles<S>(p), cap = (int64_t)sm_count() * S::kBlocksPerSm / (CG * p.parts);
   cudaLaunchConfig_t cfg{};
@@ -1030,7 +1033,7 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   // 4096 x 4096 e4m3 23.6 -> 17.4 us, 64 rows 31.7 -> 21.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
   // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two take 16.4).
   int64_t parts = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
-  parts = parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
+  parts = parts >= kMaxParts ? kMaxParts : parts >= 2 ? 2 : 1;
   while (parts > 1 && 2 * parts > nslab) parts /= 2;
   p.parts = 1;
   if (g_form == 3 || (g_form == 0 && parts >= 2)) {
@@ -1056,6 +1059,7 @@ int check_expert(const knj_expert_gemm_args *a, bool gateup, const char *who) {
   KNJ_REQUIRE(a, "%s: null argument block", who);
   KNJ_REQUIRE(a->n_pairs >= 0 && a->n_rows >= 0 && a->N > 0 && a->K > 0 && a->n_experts >= 1 && a->n_experts <= kMaxExperts, "%s: bad sizes", who);
   if (a->n_pairs == 0) return KNJ_OK;
+  KNJ_REQUIRE(a->n_pairs <= kMaxPairs && a->idx_stride <= kMaxPairs, "%s: tables of more than 2^30 pairs", who);
   KNJ_REQUIRE(a->n_rows >= 1, "%s: pairs without a row of x", who);
   KNJ_REQUIRE(a->w_dtype >= KNJ_DT_BF16 && a->w_dtype <= KNJ_DT_E4M3, "%s: expert matrices are bf16, f16 or e4m3", who);
   KNJ_REQUIRE(a->x_dtype == a->w_dtype, "%s: rows (type %d) and matrices (type %d) are of one type", who, a->x_dtype, a->w_dtype);
@@ -1105,6 +1109,7 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
   KNJ_REQUIRE(m >= 0 && n_in > 0 && n_out > 0, "knj_fp8_matmul: bad sizes");
   if (m == 0) return KNJ_OK;
   KNJ_REQUIRE(W && W_scale && x && y, "knj_fp8_matmul: null pointer");
+  KNJ_REQUIRE(m <= kMaxPairs, "knj_fp8_matmul: more than 2^30 rows");
   KNJ_REQUIRE(n_in % 16 == 0, "knj_fp8_matmul: n_in=%d must be a multiple of 16", n_in);
   KNJ_REQUIRE(aligned16(W), "knj_fp8_matmul: the matrix must be 16-byte aligned");
   KNJ_REQUIRE(x_dtype >= KNJ_DT_F32 && x_dtype <= KNJ_DT_F16, "knj_fp8_matmul: rows are f32, bf16 or f16");

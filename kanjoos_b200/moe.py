@@ -314,21 +314,28 @@ class MoeBlock:
             t = getattr(bank, name)
             if t is None or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:
                 raise ValueError(f"{name}: expected a contiguous CUDA tensor of shape {shape}")
+            if name.endswith("_scale") and t.dtype != torch.float32:
+                raise ValueError(f"{name}: scales are f32")
         if bank.router.dtype != torch.bfloat16:
             raise ValueError("the router's weights are bf16")
+        for name in (*want, "pre_norm", "post_norm", "out_gate", "router_bias"):
+            t = getattr(bank, name)
+            if t is not None and t.device != bank.gate.device:
+                raise ValueError(f"{name} lives on {t.device}, the block on {bank.gate.device}")
         norms = [w for w in (bank.pre_norm, bank.post_norm) if w is not None]
         if any(tuple(w.shape) != (H,) or w.dtype not in _DT_FLOAT or w.dtype != norms[0].dtype or not w.is_contiguous() for w in norms):
             raise ValueError(f"norm weights are contiguous [{H}] of one type")
         if bank.out_gate is not None and (tuple(bank.out_gate.shape) != (H,) or bank.out_gate.dtype not in _DT_FLOAT or not bank.out_gate.is_contiguous()):
             raise ValueError(f"out_gate is contiguous [{H}]")
-        if bank.router_bias is not None and (tuple(bank.router_bias.shape) != (E,) or bank.router_bias.dtype != torch.float32):
-            raise ValueError(f"router_bias is f32 [{E}]")
+        if bank.router_bias is not None and (tuple(bank.router_bias.shape) != (E,) or bank.router_bias.dtype != torch.float32 or not bank.router_bias.is_contiguous()):
+            raise ValueError(f"router_bias is contiguous f32 [{E}]")
         self.bank, self.top_k, self.max_tokens = bank, top_k, max_tokens
         need = lib().knj_moe_block_workspace_bytes(max_tokens, H, F, E, top_k, _DT_EXPERT[kind])
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=bank.gate.device)
-        if workspace.numel() < need or workspace.data_ptr() % 256:
-            raise ValueError(f"workspace of {need} bytes, 256-byte aligned, needed")
+        if workspace.dtype != torch.uint8 or workspace.numel() < need or workspace.data_ptr() % 256 or workspace.device != bank.gate.device or \
+                not workspace.is_contiguous():
+            raise ValueError(f"workspace of {need} contiguous uint8 values on the block's device, 256-byte aligned, needed")
         self.workspace = workspace
 
     def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:

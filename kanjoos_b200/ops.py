@@ -405,7 +405,7 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
     x [T][H] the residual stream, y [T][H] the block's output or None, post_w / pre_w [H] norm weights or None (one type),
     gate [H], [T][1] or [T][H] (through a sigmoid with gate_sigmoid). Returns (s, h): s in stream_dtype (default: x's type;
     None without y unless stream_out or stream_dtype asks for it), h in norm_dtype (None without pre_w), for
-    torch.float8_e4m3fn as (codes, scale). stream_out may be x or y."""
+    torch.float8_e4m3fn as (codes, scale). stream_out may be x or y and otherwise overlaps neither."""
     cur = _cur()
     x_ptr, x_code, ldx = _rows(x, "x", cur)
     shape = x.shape

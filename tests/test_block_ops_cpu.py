@@ -117,3 +117,10 @@ def test_python_entry_points_refuse_tensors_off_the_device():
     for call in (lambda: ops.fp8_rows(x), lambda: ops.block_norm(x, x), lambda: ops.fp8_matmul(x.to(torch.float8_e4m3fn), x, x)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+def test_tables_and_rows_beyond_32_bit_counts_are_refused(L):
+    for name in ("knj_expert_gateup_launch", "knj_expert_proj_launch"):
+        refused(L, getattr(L, name)(C.byref(gemm_args(idx_stride=(1 << 30) + 1)), None), "2^30")
+        refused(L, getattr(L, name)(C.byref(gemm_args(idx_stride=1 << 62)), None), "2^30")
+        refused(L, getattr(L, name)(C.byref(gemm_args(n_pairs=(1 << 30) + 1)), None), "2^30")
