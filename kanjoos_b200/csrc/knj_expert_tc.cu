@@ -80,7 +80,8 @@ struct Shape {
   static constexpr int kOffA = 0;
   static constexpr int kOffB = kOffA + kStages * kSub * kATile;
   static constexpr int kOffScale = kOffB + kStages * kSub * kBTile;
-  static constexpr int kStage = kRowsM ? 0 : 16 * 48;    // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16
+  // bytes per epilogue warp: 16 columns x 32 + 16 or 8 x 64 + 16; or 32 rows of 16 f32
+  static constexpr int kStage = kRowsM ? 32 * 17 * 4 : 16 * 48;
   static constexpr int kOffStage = kOffScale + kScaleGroups * kScaleGroup;
   static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [kTiles][kTok] pair of each column
   static constexpr int kTiles = 3;                       // ring of tile descriptions
@@ -144,6 +145,42 @@ __device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {
   }
   const __half2 x = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&x);
+}
+
+// Columns of PER 16-bit outputs from shared memory to rows at any address: a lane per output, so that an instruction touches one run
+// of each row. A function of its own: inlined at each of its dozen places it cost the aligned stores' code 4 us of 29 (2772 x 4096 x 288).
+template <int PER>
+__device__ __noinline__ void store_any(uint16_t *out, int64_t ldo, int n0, int N, const uint8_t *stg, int pitch, const int32_t *pairs) {
+  const int lane = threadIdx.x & 31, j = lane % PER;
+  int pr[8];
+  uint16_t v[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {   // all reads in front of the stores, which the compiler keeps them behind
+    const int col = c * (32 / PER) + lane / PER;
+    pr[c] = pairs[col];
+    v[c] = *reinterpret_cast<const uint16_t *>(stg + col * pitch + 2 * j);
+  }
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    if (pr[c] != -1 && n0 + j < N) out[(pr[c] < 0 ? -2 - pr[c] : pr[c]) * ldo + n0 + j] = pr[c] < 0 ? 0 : v[c];
+}
+
+// The same for 32 rows of 16 f32 values, kRowPitch apart, of which each lane knows its own row's pair.
+constexpr int kRowPitch = 17;
+__device__ __noinline__ void store_rows_any(void *out, int dtype, int64_t ldo, int n, int N, const float *stg, int pr) {
+  const int lane = threadIdx.x & 31, j = lane & 15;
+  int q[16];
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4);
+    q[i] = __shfl_sync(0xffffffffu, pr, r);
+    v[i] = stg[r * kRowPitch + j];
+  }
+  if (n + j >= N) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (q[i] != -1) store_from_f32(out, dtype, (q[i] < 0 ? -2 - q[i] : q[i]) * ldo + n + j, v[i]);
 }
 
 template <bool FP8, bool GATEUP, int FORM>
@@ -374,21 +411,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
                        "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
                        : "memory");
           __syncwarp();
-          const int col = lane / (kRow / 16), part = lane % (kRow / 16);
-          uint4 u = *reinterpret_cast<const uint4 *>(stg + col * kPitch + part * 16);
-          int pr = pairs[c0 + i * kCols + col];
-          if (pr != -1) {
+          uint16_t *out = static_cast<uint16_t *>(p.out);
+          if (p.vec_out && n0 + kRow / 2 <= p.N) {
+            const int col = lane / (kRow / 16), part = lane % (kRow / 16);
+            uint4 u = *reinterpret_cast<const uint4 *>(stg + col * kPitch + part * 16);
+            const int pr = pairs[c0 + i * kCols + col];
             if (pr < 0) u = make_uint4(0, 0, 0, 0);
-            const int n = n0 + 8 * part;
-            uint16_t *at = static_cast<uint16_t *>(p.out) + (pr < 0 ? -2 - pr : pr) * p.ldo + n;
-            if (p.vec_out && n + 8 <= p.N) {
-              *reinterpret_cast<uint4 *>(at) = u;
-            } else {
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (n + j < p.N) at[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-            }
+            if (pr != -1) *reinterpret_cast<uint4 *>(out + (pr < 0 ? -2 - pr : pr) * p.ldo + n0 + 8 * part) = u;
+          } else {
+            store_any<kRow / 2>(out, p.ldo, n0, p.N, stg, kPitch, pairs + c0 + i * kCols);
           }
         }
       };
@@ -549,42 +580,43 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         }
         if (!ok) break;
         const int n_cta = ncol / CG;
-        int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
-        if (pr != -1) {
-          const bool none = pr < 0;
-          if (none) pr = -2 - pr;
-          auto value = [&](int c, int j) {   // output 16 c + j of this thread's row
-            const unsigned long long w = acc[c][j >> 1];
-            return __uint_as_float((uint32_t)((j & 1) ? w >> 32 : w));
-          };
-          constexpr int kOut16 = GATEUP ? 4 : 8;   // runs of 16 outputs
+        const int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
+        const bool none = pr < -1;
+        const int64_t row = (int64_t)(none ? -2 - pr : pr) * p.ldo;
+        auto value = [&](int c, int j) {   // output 16 c + j of this thread's row
+          const unsigned long long w = acc[c][j >> 1];
+          return __uint_as_float((uint32_t)((j & 1) ? w >> 32 : w));
+        };
+        constexpr int kOut16 = GATEUP ? 4 : 8;   // runs of 16 outputs
 #pragma unroll
-          for (int c = 0; c < kOut16; ++c) {
-            float f[16];
+        for (int c = 0; c < kOut16; ++c) {
+          float f[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              f[j] = value(c, j);
-              if constexpr (GATEUP) f[j] = __fdividef(f[j], 1.0f + __expf(-f[j])) * value(c + 4, j);
-              f[j] = none ? 0.f : f[j] * p.out_scale;
-            }
-            const int n = tl.n0 + group * 64 + (c & 3) * 16 + (c >> 2) * 128;
-            if (n >= p.N) continue;
-            const int64_t at = pr * p.ldo + n;
-            if (p.vec_out && n + 16 <= p.N) {
-              if (p.out_dtype == KNJ_DT_F32) {
-                store_sector(static_cast<float *>(p.out) + at, f);
-                store_sector(static_cast<float *>(p.out) + at + 8, f + 8);
-              } else {
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __uint_as_float(pack16(p.out_dtype, f[2 * j], f[2 * j + 1]));
-                store_sector(reinterpret_cast<float *>(static_cast<uint16_t *>(p.out) + at), w);
-              }
+          for (int j = 0; j < 16; ++j) {
+            f[j] = value(c, j);
+            if constexpr (GATEUP) f[j] = __fdividef(f[j], 1.0f + __expf(-f[j])) * value(c + 4, j);
+            f[j] = none ? 0.f : f[j] * p.out_scale;
+          }
+          const int n = tl.n0 + group * 64 + (c & 3) * 16 + (c >> 2) * 128;
+          if (n >= p.N) continue;
+          if (p.vec_out && n + 16 <= p.N) {
+            if (pr == -1) continue;
+            if (p.out_dtype == KNJ_DT_F32) {
+              store_sector(static_cast<float *>(p.out) + row + n, f);
+              store_sector(static_cast<float *>(p.out) + row + n + 8, f + 8);
             } else {
+              float w[8];
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (n + j < p.N) store_from_f32(p.out, p.out_dtype, at + j, f[j]);
+              for (int j = 0; j < 8; ++j) w[j] = __uint_as_float(pack16(p.out_dtype, f[2 * j], f[2 * j + 1]));
+              store_sector(reinterpret_cast<float *>(static_cast<uint16_t *>(p.out) + row + n), w);
             }
+          } else {
+            float *stg = reinterpret_cast<float *>(smem + S::kOffStage + warp * S::kStage);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) stg[lane * kRowPitch + j] = f[j];
+            __syncwarp();
+            store_rows_any(p.out, p.out_dtype, p.ldo, n, p.N, stg, pr);
           }
         }
       } else {
