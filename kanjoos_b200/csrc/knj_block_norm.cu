@@ -406,10 +406,114 @@ __global__ void __launch_bounds__(256, kRowsCtas) fp8_rows_vec_kernel(const void
 
 // ---- any rows ------------------------------------------------------------------------------------------------------
 
-// One CTA per row, the row of s in shared memory.
+// element of a lane's k-th value of a group of 128
+__device__ __forceinline__ int any_at(int group, int lane, int k) { return group * kFp8Group + 32 * k + lane; }
+template <class F>
+__device__ __forceinline__ void of_type(int dtype, F f) {   // f(example of the type): the branch around a run of loads, not inside
+  if (dtype == KNJ_DT_F32) f(float());
+  else if (dtype == KNJ_DT_BF16) f(__nv_bfloat16());
+  else f(__half());
+}
+__device__ __forceinline__ void any_load(const void *base, int dtype, int64_t row, int group, int lane, int n, float (&v)[4]) {
+  of_type(dtype, [&](auto ex) {
+    const decltype(ex) *q = static_cast<const decltype(ex) *>(base) + row;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = any_at(group, lane, k);
+      v[k] = i < n ? (float)q[i] : 0.f;
+    }
+  });
+}
+__device__ __forceinline__ void any_store(void *base, int dtype, int64_t row, int group, int lane, int n, const float (&v)[4]) {
+  of_type(dtype, [&](auto ex) {
+    decltype(ex) *q = static_cast<decltype(ex) *>(base) + row;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = any_at(group, lane, k);
+      if (i < n) q[i] = (decltype(ex))v[k];
+    }
+  });
+}
+// a warp's group as codes; every lane takes part
+__device__ __forceinline__ void any_codes(const float (&v)[4], uint8_t *q, float *scale, int64_t row, int group, int lane, int n) {
+  float most = max3_abs_nan(max3_abs_nan(0.f, v[0], v[1]), v[2], v[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const Fp8Scale sc = fp8_scale(most);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = any_at(group, lane, k);
+    if (i < n) q[row + i] = (uint8_t)e4m3_pair(v[k] * sc.inverse, 0.f);
+  }
+  if (lane == 0) *scale = sc.scale;
+}
+
+// One CTA per row; a warp holds NC groups of 128 values, a lane every 32nd value of each, so that any row's accesses are runs of 32
+// elements.
+template <int NC>
+__global__ void __launch_bounds__(NC == 2 ? 512 : 1024) block_norm_any_kernel(const NormParams p) {
+  __shared__ float red[32];
+  grid_dep_wait();
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, H = p.H;
+  const int groups = (H + kFp8Group - 1) / kFp8Group;
+  float s[NC][4], n[NC][4], w[4];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    any_load(p.x, p.x_dtype, t * p.ldx, warp + warps * c, lane, H, s[c]);
+    if (p.y) any_load(p.y, p.y_dtype, t * p.ldy, warp + warps * c, lane, H, n[c]);
+  }
+  auto squares = [&](const float (&v)[NC][4], float down) {
+    float a = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a = fmaf(v[c][k] * down, v[c][k] * down, a);
+    return block_sum(a, red);
+  };
+  float rs = p.alpha;
+  if (p.y && p.post_w) rs = p.alpha * rms_inverse(squares(n, 1.f), p.inv_h, p.eps, [&] { return squares(n, kDown); });
+  if (p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int g = warp + warps * c;
+    if (g >= groups) break;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[c][k] *= p.beta;
+    if (p.y) {
+      if (p.post_w) {
+        any_load(p.post_w, p.w_dtype, 0, g, lane, H, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n[c][k] *= w[k];
+      }
+      if (p.gate_kind == KNJ_GATE_CHANNEL || p.gate_kind == KNJ_GATE_FULL) {
+        any_load(p.gate, p.gate_dtype, p.gate_kind == KNJ_GATE_FULL ? t * p.ldg : 0, g, lane, H, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n[c][k] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[k])) : w[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[c][k] = any_at(g, lane, k) < H ? fmaf(n[c][k], rs, s[c][k]) : 0.f;
+    }
+    if (p.stream) any_store(p.stream, p.stream_dtype, t * p.ld_stream, g, lane, H, s[c]);
+  }
+  if (!p.h) return;
+  const float hs = rms_inverse(squares(s, 1.f), p.inv_h, p.eps, [&] { return squares(s, kDown); });
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int g = warp + warps * c;
+    if (g >= groups) break;
+    any_load(p.pre_w, p.w_dtype, 0, g, lane, H, w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[c][k] *= hs * w[k];
+    if (p.h_dtype != KNJ_DT_E4M3) any_store(p.h, p.h_dtype, t * p.ldh, g, lane, H, s[c]);
+    else any_codes(s[c], static_cast<uint8_t *>(p.h), p.h_scale + t * groups + g, t * p.ldh, g, lane, H);
+  }
+}
+
+// Rows above 16384 values: one CTA per row, the row of s in shared memory.
 __global__ void __launch_bounds__(256) block_norm_kernel(const NormParams p) {
   extern __shared__ float row[];
-  __shared__ float red[8];
+  __shared__ float red[32];
   const int64_t t = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31;
   float rs = 1.f;
@@ -453,22 +557,12 @@ __global__ void __launch_bounds__(256) block_norm_kernel(const NormParams p) {
   }
   const int groups = (p.H + kFp8Group - 1) / kFp8Group;
   for (int g = tid >> 5; g < groups; g += 8) {
-    float v[4], most = 0.f;
+    float v[4];
+    any_load(p.pre_w, p.w_dtype, 0, g, lane, p.H, v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * kFp8Group + 4 * lane + j;
-      v[j] = i < p.H ? row[i] * hs * load_as_f32(p.pre_w, p.w_dtype, i) : 0.f;
-      most = max_nan(most, fabsf(v[j]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const Fp8Scale sc = fp8_scale(most);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * kFp8Group + 4 * lane + j;
-      if (i < p.H) static_cast<uint8_t *>(p.h)[t * p.ldh + i] = (uint8_t)e4m3_pair(v[j] * sc.inverse, 0.f);
-    }
-    if (lane == 0) p.h_scale[t * groups + g] = sc.scale;
+    for (int k = 0; k < 4; ++k)
+      if (any_at(g, lane, k) < p.H) v[k] *= row[any_at(g, lane, k)] * hs;
+    any_codes(v, static_cast<uint8_t *>(p.h), p.h_scale + t * groups + g, t * p.ldh, g, lane, p.H);
   }
 }
 
@@ -479,22 +573,9 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const void *x, int dtype,
   for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < n_groups; w += (int64_t)gridDim.x * 8) {
     const int64_t t = w / groups;
     const int g = (int)(w - t * groups);
-    float v[4], most = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * kFp8Group + 4 * lane + j;
-      v[j] = i < K ? load_as_f32(x, dtype, t * ldx + i) : 0.f;
-      most = max_nan(most, fabsf(v[j]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const Fp8Scale sc = fp8_scale(most);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * kFp8Group + 4 * lane + j;
-      if (i < K) q[t * K + i] = (uint8_t)e4m3_pair(v[j] * sc.inverse, 0.f);
-    }
-    if (lane == 0) scale[w] = sc.scale;
+    float v[4];
+    any_load(x, dtype, t * ldx, g, lane, K, v);
+    any_codes(v, q, scale + w, t * K, g, lane, K);
   }
 }
 
@@ -553,6 +634,14 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
     else if (runs == 2) KNJ_CUDA((launch_vec<2>(p, threads, as_stream(s))));
     else KNJ_CUDA((launch_vec<4>(p, threads, as_stream(s))));
     return launch_status("block_norm_vec_kernel");
+  }
+  if (H <= 16384) {
+    // two groups of 128 per warp up to 4096 values, four behind that
+    const int groups = (H + kFp8Group - 1) / kFp8Group, nc = H <= 4096 ? 2 : 4;
+    const dim3 grid((unsigned)p.T), block(32 * ((groups + nc - 1) / nc));
+    if (nc == 2) KNJ_CUDA(launch_chain(block_norm_any_kernel<2>, grid, block, 0, as_stream(s), p));
+    else KNJ_CUDA(launch_chain(block_norm_any_kernel<4>, grid, block, 0, as_stream(s), p));
+    return launch_status("block_norm_any_kernel");
   }
   const size_t smem = (size_t)H * 4;
   if (smem > 48 * 1024) KNJ_CUDA(cudaFuncSetAttribute(block_norm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KNJ_BLOCK_NORM_MAX_HIDDEN * 4));
