@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import block_ops_ref as ref
-from test_gpu_block_ops import BF16, E4M3, F32, form, gen  # noqa: F401
+from test_gpu_block_ops import BF16, E4M3, F16, F32, form, gen  # noqa: F401
 from test_gpu_moe_block import bank_of, on_device
 
 pytestmark = pytest.mark.gpu
@@ -194,3 +194,31 @@ def test_operands_that_are_refused():
                torch.empty(1 << 22, dtype=torch.uint8, device="cuda")[1:]):
         with pytest.raises(ValueError):
             MoeBlock(bank, top_k=2, max_tokens=4, workspace=ws)
+
+
+@pytest.mark.parametrize("T,H,st,yt,wt,gate,sig,post,pre,ht", [
+    (3, 129, BF16, F32, BF16, "channel", True, True, True, E4M3), (700, 513, BF16, BF16, F32, "row", True, True, True, E4M3),
+    (2, 4095, F32, BF16, BF16, "full", True, True, True, F16), (2, 4097, BF16, F16, BF16, None, False, True, True, E4M3),
+    (1, 16383, BF16, BF16, BF16, "channel", True, True, True, E4M3), (2, 16385, F16, BF16, BF16, "full", False, True, True, E4M3),
+    (3, 30001, F32, None, F32, None, False, False, True, BF16), (5, 9999, BF16, BF16, BF16, "row", False, False, False, None),
+])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_norms_of_any_width(T, H, st, yt, wt, gate, sig, post, pre, ht, pad):
+    from test_gpu_block_ops import test_block_norm
+    test_block_norm(T, H, st, yt, wt, gate, sig, post, pre, ht, pad)
+
+
+def test_special_rows_of_any_width():
+    """Squares beyond the f32 range, zeros and a NaN, in rows without 16-byte units: each stays in its row."""
+    from kanjoos_b200 import ops
+    for H in (1001, 5003):
+        x = torch.ones((4, H), device="cuda")
+        x[0] *= 1e30
+        x[1] = 0.0
+        x[2, 7] = float("nan")
+        w = torch.ones(H, device="cuda")
+        s, h = ops.block_norm(x, x, post_w=w, pre_w=w, norm_dtype=F32, alpha=2.0)
+        # the mean square is 1e60: n = 1 up to roundings of 2^-24 in the scaled sum, its root and two products
+        assert torch.equal(s[0], x[0]) and (h[0] - 1).abs().max() < 8 * H * 2.0 ** -24
+        assert (s[1] == 0).all() and (h[1] == 0).all() and torch.isnan(h[2]).all()
+        assert (s[3] - 3).abs().max() < 1e-3 and (h[3] - 1).abs().max() < 1e-3
