@@ -32,12 +32,16 @@ constexpr int kMaxExperts = 256;
 constexpr int64_t kMaxPairs = 1 << 30;   // sums of a count and a bucket's size stay in 32 bits
 
 struct GemmParams {
+  const uint8_t *x;
+  int64_t x_row;              // bytes from row to row
   const float *xs, *ws0, *ws1;
   const int32_t *pair_idx, *pair_cnt, *row_map;  // pair_idx null: one expert, pair i is row i
   void *out;
   int *status;
   int64_t ldo, idx_stride;
-  int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles, parts;   // parts: CTAs that share a tile's K
+  int out_dtype, N, K, E, row_div, n_rows, n_pairs, m_tiles;
+  int part_bits;              // 2^part_bits CTAs share a tile's K
+  uint32_t m_inverse;         // floor(2^32 / m_tiles), at most 2^32 - 1
   uint32_t idesc_format;
   int vec_out;                // bases and strides of the outputs allow 16-byte (lane = row form: 32-byte) stores
   int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
@@ -131,6 +135,7 @@ __device__ __forceinline__ void cp_async4(const void *dst_smem, const void *src)
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void l2_line(const void *at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 // 32 bytes, one whole sector
 __device__ __forceinline__ void store_sector(float *at, const float *v) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
@@ -194,7 +199,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = warp_index();
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;                       // in the pair
-  const int part = SPLIT ? (int)cluster_rank() : 0, parts = SPLIT ? p.parts : 1;   // of K
+  const int part = SPLIT ? (int)cluster_rank() : 0, parts = SPLIT ? 1 << p.part_bits : 1;   // of K
 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kOffBars);
   uint64_t *full = bars;                        // [kStages] operands of both CTAs landed (the even CTA's are used)
@@ -212,6 +217,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   int4 *s_tile = reinterpret_cast<int4 *>(smem + S::kOffTile);
   int32_t *s_pref = reinterpret_cast<int32_t *>(smem + S::kOffPref), *s_cnt = s_pref + kMaxExperts + 1;
 
+  if (warp == S::kMatWarp && lane < 3) {   // the maps' first use would wait for them
+    const CUtensorMap *m = lane == 0 ? &p.map0 : lane == 1 ? &p.mapx : &p.map1;
+    if (lane < 2 || GATEUP) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -232,10 +241,20 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     *s_fail = 0;
     mbar_init_fence();
   }
+  __syncwarp();
+  if (CG == 2 || SPLIT) cluster_arrive();
   constexpr uint32_t kTmemCols = S::kAccs * S::kAccCols;
   if (warp == S::kMmaWarp) {
     tmem_alloc<CG>(tmem_slot, kTmemCols);
     tmem_relinquish<CG>();
+  }
+  if constexpr (FORM != kPair) {
+    // The tables' first entries and the first rows start for L2 while the counts are read: found one after the other, they are three
+    // latencies of HBM. A line that an earlier launch still writes is brought there for it.
+    if (tid < 8 && 32 * tid < p.E && p.pair_idx) l2_line(p.pair_cnt + 32 * tid);
+    if (tid < p.E && p.pair_idx) l2_line(p.pair_idx + tid * p.idx_stride);
+    const int per = (p.K * (FP8 ? 1 : 2) + 127) / 128, line = blockIdx.x * S::kThreads + tid, row = line / per;
+    if (row < p.n_rows) l2_line(p.x + row * p.x_row + (line - row * per) * 128);
   }
   grid_dep_wait();  // the tables and the rows come from earlier launches
   if (warp == 0) {
@@ -266,7 +285,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2 || SPLIT) cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
+  if (CG == 2 || SPLIT) cluster_wait();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   // what comes out of shared memory and feeds issuing loops goes through a shuffle: the compiler then knows it is the same in all
   // lanes and keeps it, and what is derived from it, in uniform registers
@@ -277,17 +296,24 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   const int n_tiles = same(s_pref[kMaxExperts]) * p.m_tiles;   // at most 2^30: checked on the host
   // As many CTAs (pairs) as take part in whole rounds: of 1536 tiles on 296 CTAs, 256 take six each instead of 56 a sixth; the matrices
   // stream as fast and no round is left to a few (gate and up of 512 rows, bf16: 172 -> 158 us).
-  const int k_lo = part * nslab / parts, k_hi = (part + 1) * nslab / parts;   // this CTA's slabs
-  const int avail = gridDim.x / (CG * parts), rounds = (n_tiles + avail - 1) / avail, step = rounds ? (n_tiles + rounds - 1) / rounds : 1;
-  const int first = (int)(blockIdx.x / (CG * parts)) < step ? blockIdx.x / (CG * parts) : n_tiles;
+  const int bits = SPLIT ? p.part_bits : 0, k_lo = (part * nslab) >> bits, k_hi = ((part + 1) * nslab) >> bits;   // this CTA's slabs
+  const int avail = (int)(gridDim.x / CG) >> bits, mine = (int)(blockIdx.x / CG) >> bits;
+  int step = max(n_tiles, 1);
+  if (n_tiles > avail) {   // the divisions of a few tiles would be a tenth of the time to the first copy
+    const int rounds = (n_tiles + avail - 1) / avail;
+    step = (n_tiles + rounds - 1) / rounds;
+  }
+  const int first = mine < step ? mine : n_tiles;
   auto tile_at = [&](int t, int &ntok) {   // by a whole warp
-    const int b = t / p.m_tiles, mt = t - b * p.m_tiles;
+    int b = (int)__umulhi((uint32_t)t, p.m_inverse);   // t / m_tiles or one less
+    if (t - b * p.m_tiles >= p.m_tiles) ++b;
+    const int mt = t - b * p.m_tiles;
     // the last expert whose first bucket is not behind b: of 32 groups of eight experts, then of the eight
     const int g = 8 * (__popc(__ballot_sync(0xffffffffu, s_pref[8 * lane] <= b)) - 1);
     const int e = g + __popc(__ballot_sync(0xffffffffu, s_pref[g + (lane & 7)] <= b) & 0xffu) - 1;
     const int b0 = same(s_pref[e]), nb = same(s_pref[e + 1]) - b0, cnt = same(s_cnt[e]);
     // an expert's pairs are spread evenly over its buckets: 256 + 14 pairs would stream the matrix twice for 14
-    const int per = ((cnt + nb - 1) / nb + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
+    const int per = ((nb == 1 ? cnt : (cnt + nb - 1) / nb) + S::kTokStep - 1) / S::kTokStep * S::kTokStep;
     Tile r;
     r.e = e;
     r.n0 = (mt * CG + (S::kRowsM ? 0 : (int)rank)) * S::kOuts;
@@ -1033,20 +1059,21 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   if (!rc) rc = make_operand_tensor_map(&p.mapx, o.x, esz, p.K, o.ldx, p.n_rows, p.dense ? S::kTok / CG : 1);
   if (rc) return rc;
   p.m_tiles = (p.N + S::kOuts * CG - 1) / (S::kOuts * CG);
+  p.m_inverse = (uint32_t)((1ull << 32) / p.m_tiles - (p.m_tiles == 1));
   const int out_esz = p.out_dtype == KNJ_DT_F32 ? 4 : 2, unit = S::kRowsM ? 32 : 16;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % unit == 0 && p.ldo * out_esz % unit == 0;
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
   KNJ_REQUIRE(most * p.m_tiles <= (1ll << 30) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
-  const int64_t tiles = most_tiles<S>(p), cap = (int64_t)sm_count() * S::kBlocksPerSm / (CG * p.parts);
+  const int64_t tiles = most_tiles<S>(p), cap = (int64_t)sm_count() * S::kBlocksPerSm / (CG << p.part_bits);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * CG * p.parts));
+  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * (CG << p.part_bits)));
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG * p.parts;
+  attr[0].val.clusterDim.x = CG << p.part_bits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1064,12 +1091,12 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   // K is split where even the smallest tiles leave half of the CTAs' places free, into parts of two slabs or more: one row times
   // 4096 x 4096 e4m3 23.6 -> 17.4 us, 64 rows 31.7 -> 21.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
   // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two take 16.4).
-  int64_t parts = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
-  parts = parts >= kMaxParts ? kMaxParts : parts >= 2 ? 2 : 1;
-  while (parts > 1 && 2 * parts > nslab) parts /= 2;
-  p.parts = 1;
-  if (g_form == 3 || (g_form == 0 && parts >= 2)) {
-    p.parts = (int)parts;
+  const int64_t places = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
+  int bits = places >= kMaxParts ? 2 : places >= 2 ? 1 : 0;
+  while (bits > 0 && (2 << bits) > nslab) --bits;
+  p.part_bits = 0;
+  if (g_form == 3 || (g_form == 0 && bits > 0)) {
+    p.part_bits = bits;
     return launch_form<FP8, GATEUP, kSplit>(p, o, st);
   }
   // Pairs or single SMs, us by (rows per expert; experts): 16 bits, gate and up, hidden 2048, ffn 768: 92 single, 90 pair (1; 128),
@@ -1115,6 +1142,7 @@ int run_expert(const knj_expert_gemm_args *a, bool gateup, const char *who, knj_
   p.out = a->out; p.status = a->status; p.ldo = a->ldo; p.idx_stride = a->idx_stride; p.out_dtype = a->out_dtype; p.N = a->N; p.K = a->K;
   p.E = a->n_experts; p.row_div = a->row_div > 0 ? a->row_div : 1; p.n_rows = a->n_rows; p.n_pairs = a->n_pairs; p.out_scale = a->out_scale;
   p.idesc_format = a->w_dtype == KNJ_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
+  p.x = static_cast<const uint8_t *>(a->x); p.x_row = a->ldx * (a->w_dtype == KNJ_DT_E4M3 ? 1 : 2);
   const Operands o{a->x, a->w0, a->w1, a->ldx, a->w_dtype == KNJ_DT_E4M3};
   return gateup ? launch_gemm<true>(p, o, as_stream(s)) : launch_gemm<false>(p, o, as_stream(s));
 }
@@ -1158,7 +1186,7 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
   const int rc = knj_fp8_rows_launch(x, x_dtype, ldx, m, n_in, q, qs, s);
   if (rc) return rc;
   GemmParams p{};
-  p.xs = qs; p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
+  p.x = q; p.x_row = n_in; p.xs = qs; p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
   p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f; p.dense = 1;
   return launch_gemm<false>(p, Operands{q, W, nullptr, n_in, true}, as_stream(s));
 }
