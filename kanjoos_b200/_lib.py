@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 # KNJ_DEVICE_LIB points at another build of the same library (e.g. a measurement build); default: the in-tree one
@@ -50,6 +51,13 @@ class BlockNormArgs(C.Structure):
                 ("h_scale", C.c_void_p), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("w_dtype", C.c_int32),
                 ("gate_dtype", C.c_int32), ("stream_dtype", C.c_int32), ("h_dtype", C.c_int32), ("gate_kind", C.c_int32),
                 ("gate_sigmoid", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float)]
+
+
+def packed(cls):
+    """A function from the values of all fields in their order (0 for a null pointer) to the structure's bytes: for calls that are made
+    many times a decode step, 0.25 us where building the structure takes 1.2."""
+    code = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P", C.c_float: "f"}
+    return struct.Struct("".join(code[t] for _, t in cls._fields_) + "0P").pack
 
 
 class MoeBlockArgs(C.Structure):
@@ -206,9 +214,10 @@ SIGNATURES = {
     "knj_q4k_matmul_noalloc_max_scratch": (_sz, []),
     "knj_q4k_matmul_noalloc_launch": (_i, [_vp, _i, _i, _vp, _i, _i64, _i, _vp, _i64, _vp]),
     "knj_fp8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
-    "knj_block_norm_launch": (_i, [C.POINTER(BlockNormArgs), _vp]),
-    "knj_expert_gateup_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
-    "knj_expert_proj_launch": (_i, [C.POINTER(ExpertGemmArgs), _vp]),
+    # a BlockNormArgs or ExpertGemmArgs by reference, or its bytes (packed)
+    "knj_block_norm_launch": (_i, [_vp, _vp]),
+    "knj_expert_gateup_launch": (_i, [_vp, _vp]),
+    "knj_expert_proj_launch": (_i, [_vp, _vp]),
     "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "knj_moe_block_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
     "knj_moe_block_status": (_i, [C.POINTER(MoeBlockArgs), _vp]),

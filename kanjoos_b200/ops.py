@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, check,
-                   lib)
+                   lib, packed)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 _E4M3 = torch.float8_e4m3fn
@@ -272,6 +272,7 @@ def q4k_down_tc(ah, Wd, pair_idx, pair_cnt, P: int, pair_row=None, poison: bool 
 
 _cur = torch._C._cuda_getDevice
 _OPERAND = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, _E4M3: DT_E4M3}
+_norm_args, _expert_args = packed(BlockNormArgs), packed(ExpertGemmArgs)
 _ONLY_F32, _ONLY_I32, _ONLY_E4M3 = {torch.float32: DT_F32}, {torch.int32: 0}, {_E4M3: DT_E4M3}
 
 
@@ -344,8 +345,8 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
     E, N, K = shape
     types = (w.dtype,)
     w_ptr = _dense(w, "an expert matrix", cur, shape, types)
-    w1_ptr = None if w1 is None else _dense(w1, "an expert matrix", cur, shape, types)
-    xs = s0_ptr = s1_ptr = None
+    w1_ptr = 0 if w1 is None else _dense(w1, "an expert matrix", cur, shape, types)
+    xs = s0_ptr = s1_ptr = 0
     if w.dtype == _E4M3:
         if s0 is None or (w1 is not None and s1 is None):
             raise ValueError("e4m3 expert matrices need their scales")
@@ -368,15 +369,15 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
         raise ValueError(f"pair_idx has shape {tuple(idx_shape)}")
     idx = _dense(pair_idx, "pair_idx", cur, (E, idx_shape[1]), _ONLY_I32)
     cnt = _dense(pair_cnt, "pair_cnt", cur, (E,), _ONLY_I32)
-    rmap = None if row_map is None else _dense(row_map, "the row map", cur, (P,), _ONLY_I32)
+    rmap = 0 if row_map is None else _dense(row_map, "the row map", cur, (P,), _ONLY_I32)
     if out is None:
         if out_dtype not in _DT:
             raise ValueError(f"out_dtype is {out_dtype}")
         out = x.new_empty(P, N, dtype=out_dtype)
     out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
-    a = ExpertGemmArgs(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo, None, x.shape[0], P, N, K, E,
-                       row_div, x_code, x_code, out_code, out_scale)
-    check(launch(C.byref(a), _raw_stream()))
+    a = _expert_args(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo, 0, x.shape[0], P, N, K, E,
+                     row_div, x_code, x_code, out_code, out_scale)
+    check(launch(a, _raw_stream()))
     return out
 
 
@@ -410,7 +411,8 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
     x_ptr, x_code, ldx = _rows(x, "x", cur)
     shape = x.shape
     T, H = shape
-    y_ptr = gate_ptr = s_ptr = h_ptr = scale_ptr = post = pre = s = h = scale = None
+    s = h = scale = None
+    y_ptr = gate_ptr = s_ptr = h_ptr = scale_ptr = post = pre = 0
     y_code = w_code = gate_code = s_code = h_code = ldy = ldg = lds = 0
     kind = GATE_NONE
     if y is not None:
@@ -443,7 +445,7 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
         s = torch.empty_like(x, dtype=stream_dtype or x.dtype, memory_format=torch.contiguous_format)
     if s is not None:
         s_ptr, s_code, lds = _rows(s, "the stream", cur, shape)
-    a = BlockNormArgs(T, H, x_ptr, ldx, y_ptr, ldy, post, pre, gate_ptr, ldg, s_ptr, lds, h_ptr, H, scale_ptr, x_code, y_code, w_code, gate_code,
-                      s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps)
-    check(lib().knj_block_norm_launch(C.byref(a), _raw_stream()))
+    a = _norm_args(T, H, x_ptr, ldx, y_ptr, ldy, post, pre, gate_ptr, ldg, s_ptr, lds, h_ptr, H, scale_ptr, x_code, y_code, w_code, gate_code,
+                   s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps)
+    check(lib().knj_block_norm_launch(a, _raw_stream()))
     return s, (h if scale is None else (h, scale))

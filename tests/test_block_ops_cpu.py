@@ -124,3 +124,12 @@ def test_tables_and_rows_beyond_32_bit_counts_are_refused(L):
         refused(L, getattr(L, name)(C.byref(gemm_args(idx_stride=(1 << 30) + 1)), None), "2^30")
         refused(L, getattr(L, name)(C.byref(gemm_args(idx_stride=1 << 62)), None), "2^30")
         refused(L, getattr(L, name)(C.byref(gemm_args(n_pairs=(1 << 30) + 1)), None), "2^30")
+
+
+def test_packed_bytes_are_the_structures():
+    for cls in (_lib.BlockNormArgs, _lib.ExpertGemmArgs):
+        values = list(range(1, len(cls._fields_) + 1))
+        data = _lib.packed(cls)(*values)
+        assert len(data) == C.sizeof(cls)
+        back = cls.from_buffer_copy(data)
+        assert [getattr(back, name) for name, _ in cls._fields_] == values
