@@ -164,7 +164,7 @@ __device__ __forceinline__ float cta_sum(float v, float (*red)[16], int &turn) {
 // HBM (74 us). Without it, one row per CTA straight into registers: bound by the launch and two dependent sums.
 constexpr int kMaxRing = 8;
 template <int NC, bool XW, int Y, bool RING>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
-__global__ void __launch_bounds__(NC == 1 ? 256 : 512, NC == 1 ? 4 : 1) block_norm_vec_kernel(const NormParams p, const int depth) {
+__global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 : 128) block_norm_vec_kernel(const NormParams p, const int depth) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(16) float red[2][16];
   __shared__ uint64_t bars[kMaxRing];
@@ -359,10 +359,10 @@ cudaError_t launch_vec(const NormParams &p, int threads, unsigned ctas, int dept
 }
 template <int NC>
 cudaError_t launch_vec(const NormParams &p, int threads, cudaStream_t st) {
-  // Rows that one wave of CTAs holds (1024 or 512 threads per SM) take one CTA each; more walk through the ring, as many CTAs as are
-  // resident and their rows under way as fit 160 KB per SM.
-  const int per_sm = (NC == 1 ? 1024 : 512) / threads, cap = sm_count() * per_sm;
-  if (p.T <= cap) return launch_vec<NC, false>(p, threads, (unsigned)p.T, 0, 0, st);
+  // Rows that one wave of CTAs holds (512 threads per SM) take one CTA each; more walk through the ring, as many CTAs as are resident
+  // and their rows under way as fit 160 KB per SM.
+  if (p.T <= sm_count() * (512 / threads)) return launch_vec<NC, false>(p, threads, (unsigned)p.T, 0, 0, st);
+  const int resident = NC == 1 ? 1024 : NC == 2 && !p.y ? 768 : 512, per_sm = threads < resident ? resident / threads : 1, cap = sm_count() * per_sm;
   const size_t row = (size_t)p.H * ((p.x_dtype == KNJ_DT_F32 ? 4 : 2) + (!p.y ? 0 : p.y_dtype == KNJ_DT_F32 ? 4 : 2));
   int depth = (int)(160 * 1024 / per_sm / row);
   int ctas = cap;
