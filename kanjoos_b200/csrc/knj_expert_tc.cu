@@ -4,18 +4,21 @@
 //   out[p][n] = out_scale * x[row(p)] . w[e][n]     and     out_scale * silu(x . wg[e][n]) * (x . wu[e][n])
 //   e4m3:  x . w = sum over blocks b of 128 k:  sx[row][b] * sw[n/128][b] * sum_{k in b} qx[k] qw[k]
 //
-// The MMA's M side is matrix rows, its N side a bucket of up to kTok routed rows of one expert, so that a ragged bucket wastes
-// less than 16 (32 in a pair) columns and a single token less than a tile. One CTA (CG = 1) or a pair (CG = 2: tcgen05
-// cta_group::2, 128 matrix rows and half of the bucket's rows each) walks over (bucket, row tile) tiles; consecutive tiles share a
-// bucket, so its rows stay in L2 while the matrices stream through once. Warps:
-//   epilogue   accumulators from tensor memory, scales, SiLU * up, stores. Lane = matrix row, column = routed row.
-//   MMA        one elected thread; accumulators are double-buffered, so a tile's stores overlap the next tile's products
-//   matrix     one elected thread, TMA boxes of 128 bytes of K: 128 rows, or for gate and up eight boxes of 16 rows in turn --
-//              gate and up of one output then lie 16 lanes apart in one warp and meet by a shuffle
-//   rows       tile::gather4 TMA copies of four routed rows each
-//   scales     e4m3: sx * sw of each block of K as vectors in shared memory, a few blocks ahead
+// Few rows are bound by the matrices' bytes: every active expert's matrix is read once (512 rows x 8 of 128 experts, bf16: 806 MB, 136 us,
+// 0.91 of the measured copy rate). Many rows are bound by the tensor core: 16384 rows, bf16, 1.34 PFLOP/s alone, 1.1 in a loop under
+// the power limit. One kernel with three forms (enum Form; launch_rule says when) walks over (bucket, row tile) tiles; a bucket is up
+// to kTok routed rows of one expert, and consecutive tiles share it, so that its rows stay in L2 while the matrices stream through
+// once. Persistent CTAs. In all forms but one the MMA's M side is matrix rows and its N side the bucket, so that a ragged bucket wastes
+// less than 16 (32 in a pair) columns and a single token less than a tile; e4m3 in pairs has it the other way round (see the epilogue).
+// Warps:
+//   epilogue   accumulators from tensor memory, scales, SiLU * up, stores
+//   MMA        tcgen05; accumulators are double-buffered, so a tile's stores overlap the next tile's products
+//   matrix     finds the tiles and their rows in the tables, a tile ahead; TMA boxes of 128 bytes of K: 128 rows, or for gate and up
+//              eight boxes of 16 rows in turn -- gate and up of one output then lie 16 lanes apart in one warp and meet by a shuffle
+//   rows       tile::gather4 TMA copies of four routed rows each; boxes where the rows are all rows in order
+//   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies
 // In 16 bits the tensor core adds over all of K. In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
-// adds to its registers in f32 while the tensor core fills the other.
+// adds to its registers in f32 while the tensor core fills the others.
 //
 // Every wait on an mbarrier is bounded; on give-up the kernel raises a status flag, stores NaN in place of the outputs it did not
 // form, frees its tensor memory and returns.
@@ -1089,8 +1092,8 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   const int64_t experts = p.E < p.n_pairs ? p.E : p.n_pairs;
   const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
   // K is split where even the smallest tiles leave half of the CTAs' places free, into parts of two slabs or more: one row times
-  // 4096 x 4096 e4m3 23.6 -> 17.4 us, 64 rows 31.7 -> 21.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
-  // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two take 16.4).
+  // 4096 x 4096 e4m3 21.5 -> 15.4 us, 64 rows 25.6 -> 19.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
+  // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two took 16.4).
   const int64_t places = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
   int bits = places >= kMaxParts ? 2 : places >= 2 ? 1 : 0;
   while (bits > 0 && (2 << bits) > nslab) --bits;
@@ -1099,13 +1102,14 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
     p.part_bits = bits;
     return launch_form<FP8, GATEUP, kSplit>(p, o, st);
   }
-  // Pairs or single SMs, us by (rows per expert; experts): 16 bits, gate and up, hidden 2048, ffn 768: 92 single, 90 pair (1; 128),
-  // 162, 141 (32, Zipf; 128), 297, 154 (128; 128); hidden 1024, ffn 512: 18.5, 20.5 (1; 32), 22.6, 22.6 (32; 32), 33, 25 (64; 32) --
-  // pairs where the buckets fill them or the tiles take four rounds of pairs anyway. e4m3, whose pairs always multiply 256 rows and
-  // whose stores no product overlaps: 82, 152 (4; 128), 121, 156 (64; 128), 186, 158 (128; 128), 336, 217 (256; 128), down
-  // products over K = 512 47, 53 (512; 32); 2048 rows x 1000 x 2048 26, 69 (32 tiles of pairs).
+  // Single SMs or pairs, us each, by (rows per expert; experts). 16 bits, gate and up, hidden 2048, ffn 768: 86, 86 (1; 128), 131, 133
+  // (32; 128), 136, 135 (32, Zipf; 128), 181, 145 (128; 128), 311, 201 (256; 128); hidden 1024, ffn 512: 18.4, 20.5 (1; 32), 20.5, 22.6
+  // (32; 32), 24.6, 22.6 (64; 32) -- pairs where the buckets fill them or the tiles take four rounds of pairs anyway. e4m3, whose pairs
+  // always multiply 256 rows and whose stores no product overlaps: 53, 96 (1; 128), 81, 141 (32; 128), 102, 141 (64; 128), 158, 143
+  // (128; 128), 282, 205 (256; 128); dense 4096 x 4096 x 4096 157, 103, 1024 x 4096 x 1024 (64 tiles of pairs) 25.6, 21.5,
+  // 1024 x 2048 x 2048 (32 tiles) 23.6, 25.6, 2048 x 4096 x 512 27.6, 25.6, 2772 x 4091 x 288 (rows at any address) 45, 59.
   const int64_t pair_tiles = most_tiles<Shape<FP8, GATEUP, kPair>>(p), round = sm_count() / 2;
-  bool pairs = FP8 ? p.n_pairs >= 128 * experts && nslab >= 6 && pair_tiles >= round : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
+  bool pairs = FP8 ? p.n_pairs >= 128 * experts && nslab >= 4 && 4 * pair_tiles >= 3 * round : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
   if (g_form) pairs = g_form == 2;
   return pairs ? launch_form<FP8, GATEUP, kPair>(p, o, st) : launch_form<FP8, GATEUP, kSingle>(p, o, st);
 }
