@@ -371,10 +371,13 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
     cnt = _dense(pair_cnt, "pair_cnt", cur, (E,), _ONLY_I32)
     rmap = 0 if row_map is None else _dense(row_map, "the row map", cur, (P,), _ONLY_I32)
     if out is None:
-        if out_dtype not in _DT:
+        out_code = _DT.get(out_dtype)
+        if out_code is None:
             raise ValueError(f"out_dtype is {out_dtype}")
         out = x.new_empty(P, N, dtype=out_dtype)
-    out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
+        out_ptr, ldo = out.data_ptr(), N
+    else:
+        out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
     a = _expert_args(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo, 0, x.shape[0], P, N, K, E,
                      row_div, x_code, x_code, out_code, out_scale)
     check(launch(a, _raw_stream()))
@@ -441,10 +444,13 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
             kind = GATE_ROW if rows_only else GATE_FULL
     if stream_out is not None:
         s = stream_out
-    elif y is not None or stream_dtype is not None:
-        s = torch.empty_like(x, dtype=stream_dtype or x.dtype, memory_format=torch.contiguous_format)
-    if s is not None:
         s_ptr, s_code, lds = _rows(s, "the stream", cur, shape)
+    elif y is not None or stream_dtype is not None:
+        s_code = x_code if stream_dtype is None else _DT.get(stream_dtype)
+        if s_code is None:
+            raise ValueError(f"stream_dtype is {stream_dtype}")
+        s = torch.empty_like(x, dtype=stream_dtype, memory_format=torch.contiguous_format)
+        s_ptr, lds = s.data_ptr(), H
     a = _norm_args(T, H, x_ptr, ldx, y_ptr, ldy, post, pre, gate_ptr, ldg, s_ptr, lds, h_ptr, H, scale_ptr, x_code, y_code, w_code, gate_code,
                    s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps)
     check(lib().knj_block_norm_launch(a, _raw_stream()))
