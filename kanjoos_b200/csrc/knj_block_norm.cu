@@ -161,12 +161,12 @@ __device__ __forceinline__ float cta_sum(float v, float (*red)[16], int &turn) {
 // 16384 rows of 2048 took 106 us, issue slots half full). Eight threads in a row hold sixteen runs in turn, a group of e4m3 codes
 // (NC = 1: sixteen threads). RING: the next rows travel through a ring of `depth` rows in shared memory, bulk copies on a barrier
 // each; a row ahead in registers was 24 KB under way per SM, too few for HBM (74 us). 16384 rows of 2048 in bf16 with e4m3 rows out,
-// 235 MB: 57.7 us, 4.07 TB/s (the plain norm in bf16, x only: 4.1); issue slots half full, bound by the two sums over the CTA that wait
-// for one another with four warps per scheduler. Six with the weights in shared memory: 67 us, the rows no longer fit 80 registers.
+// 235 MB: 52.9 us, 4.44 TB/s; bound by the two sums over the CTA that wait for one another, with five warps per scheduler (four, with
+// the block's output unpacked once: 57.7). Six with the weights in shared memory: 67 us, the rows no longer fit 80 registers.
 // Without the ring, one row per CTA straight into registers: bound by the launch and the two sums (one row of 2048: 2.6 us).
 constexpr int kMaxRing = 8;
 template <int NC, bool XW, int Y, bool RING>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
-__global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 : 128) block_norm_vec_kernel(const NormParams p, const int depth) {
+__global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 : XW || Y == 2 ? 128 : 96) block_norm_vec_kernel(const NormParams p, const int depth) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(16) float red[2][16];
   __shared__ uint64_t bars[kMaxRing];
@@ -190,6 +190,7 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int i = first + kLanes * c;
+      xr[c].a = xr[c].b = yr[c].a = yr[c].b = make_uint4(0, 0, 0, 0);
       if (i < H8) {
         xr[c] = load_raw8<XW>(x, xo + 8 * i);
         if constexpr (Y != 0) yr[c] = load_raw8<Y == 2>(y, yo + 8 * i);
@@ -241,17 +242,20 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
       pre_of(c, pre[c]);
     }
   }
-  // sum of squares over the row, of values * 2^-64 where `down`
-  auto squares = [&](const float2 (&v)[NC][4], bool down) {
+  // sum of squares over the row, of values * 2^-64 where `down`; of(c, v): the run's values
+  auto squares = [&](auto of, bool down) {
     float2 a = make_float2(0.f, 0.f), b = a;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
+      float2 v[4];
+      of(c, v);
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
-        const float2 x = down ? mul2(v[c][j], kDown) : v[c][j], y = down ? mul2(v[c][j + 1], kDown) : v[c][j + 1];
+        const float2 x = down ? mul2(v[j], kDown) : v[j], y = down ? mul2(v[j + 1], kDown) : v[j + 1];
         a = __ffma2_rn(x, x, a);
         b = __ffma2_rn(y, y, b);
       }
+    }
     a = __fadd2_rn(a, b);
     return cta_sum(a.x + a.y, red, turn);
   };
@@ -264,28 +268,14 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
   uint8_t *h_at = static_cast<uint8_t *>(p.h) + (blockIdx.x * p.ldh + 8 * first) * h_esz;
   const int64_t s_step = gridDim.x * p.ld_stream * s_esz, h_step = gridDim.x * p.ldh * h_esz;
   for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step) {
-    float2 s[NC][4], n[NC][4];
+    float2 s[NC][4];
     bool landed = true;
     if constexpr (RING) {
       landed = mbar_wait(&bars[slot], phase, &s_fail);
       const uint8_t *at = ring + (size_t)slot * (x_bytes + y_bytes);
       fetch(at, at + x_bytes, 0, 0);
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const bool in = first + kLanes * c < H8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[c][j] = n[c][j] = make_float2(0.f, 0.f);
-      if (in) values8<XW>(xr[c], xb, s[c]);
-      if (Y != 0 && in) values8<Y == 2>(yr[c], yb, n[c]);
-    }
     if constexpr (RING) {
-      if (!landed) {   // the wait gave up: NaN is stored
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[c][j].x = s[c][j].y = __int_as_float(0x7fffffff);
-      }
       __syncthreads();                                     // every thread has its part of the row
       if (tid == 0 && t + (int64_t)depth * gridDim.x < p.T) {
         fence_proxy_async();                               // the slot was read through the generic proxy
@@ -297,29 +287,42 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
       }
     }
     float rs = 1.f;
-    if (Y != 0 && p.post_w) rs = rms_inverse(squares(n, false), p.inv_h, p.eps, [&] { return squares(n, true); });
+    // y is unpacked here and once more below: in the type it came in it takes half of the registers meanwhile
+    auto y_of = [&](int c, float2 (&v)[4]) { values8<Y == 2>(yr[c], yb, v); };
+    if (Y != 0 && p.post_w) rs = rms_inverse(squares(y_of, false), p.inv_h, p.eps, [&] { return squares(y_of, true); });
     if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int i = first + kLanes * c;
       if (!kKeep) post_of(c, post[0]);
+      values8<XW>(xr[c], xb, s[c]);
       if (i < H8) {
+        float2 n[4];
+        if (Y != 0) y_of(c, n);
         if (Y != 0 && p.gate_kind == KNJ_GATE_FULL) {
           float2 w[4];
           load8(p.gate, p.gate_dtype, t * p.ldg + 8 * i, w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) n[c][j] = __fmul2_rn(n[c][j], p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
+          for (int j = 0; j < 4; ++j) n[j] = __fmul2_rn(n[j], p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s[c][j] = mul2(s[c][j], p.beta);
-          if constexpr (Y != 0) s[c][j] = __ffma2_rn(mul2(n[c][j], rs), post[kKeep ? c : 0][j], s[c][j]);
+          if constexpr (Y != 0) s[c][j] = __ffma2_rn(mul2(n[j], rs), post[kKeep ? c : 0][j], s[c][j]);
+        }
+        if (RING && !landed) {   // the wait gave up: NaN is stored
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[c][j].x = s[c][j].y = __int_as_float(0x7fffffff);
         }
         if (p.stream) store8(s_at + 8 * kLanes * c * s_esz, p.stream_dtype, s[c]);
       }
     }
     if (!p.h) continue;
-    const float hs = rms_inverse(squares(s, false), p.inv_h, p.eps, [&] { return squares(s, true); });
+    auto s_of = [&](int c, float2 (&v)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = s[c][j];
+    };
+    const float hs = rms_inverse(squares(s_of, false), p.inv_h, p.eps, [&] { return squares(s_of, true); });
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (!kKeep) pre_of(c, pre[0]);
@@ -364,7 +367,9 @@ cudaError_t launch_vec(const NormParams &p, int threads, cudaStream_t st) {
   // Rows that one wave of CTAs holds (512 threads per SM) take one CTA each; more walk through the ring, as many CTAs as are resident
   // and their rows under way as fit 160 KB per SM.
   if (p.T <= sm_count() * (512 / threads)) return launch_vec<NC, false>(p, threads, (unsigned)p.T, 0, 0, st);
-  const int resident = NC == 1 ? 1024 : NC == 2 && !p.y ? 768 : 512, per_sm = threads < resident ? resident / threads : 1, cap = sm_count() * per_sm;
+  const bool wide = p.x_dtype == KNJ_DT_F32 || p.y_dtype == KNJ_DT_F32;
+  const int resident = NC == 1 ? 1024 : NC == 4 ? 512 : !p.y ? 768 : wide ? 512 : 640, per_sm = threads < resident ? resident / threads : 1;
+  const int cap = sm_count() * per_sm;
   const size_t row = (size_t)p.H * ((p.x_dtype == KNJ_DT_F32 ? 4 : 2) + (!p.y ? 0 : p.y_dtype == KNJ_DT_F32 ? 4 : 2));
   int depth = (int)(160 * 1024 / per_sm / row);
   int ctas = cap;
