@@ -558,7 +558,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         // of up, or of both blocks of 128 outputs. Whole products in two buffers left the tensor core waiting for the hand-offs, which
         // still bound it: 8192 x 4096 x 4096 152 us, tensor pipe 41 % busy (copies and products alone: 101 us). The loads run one step
         // of 16 columns ahead of the sums, across blocks of K too, and whether the next buffer is complete is asked two steps before it
-        // is needed. Sixteen warps with 64 sums a thread and one load under way each took 175 us.
+        // is needed; the next block's scales are read after the first step (4096 tokens gate+up 203 -> 196 us; at the block's start, or
+        // late in it, 203 to 208). Sixteen warps with 64 sums a thread and one load under way each took 175 us.
         constexpr int kSteps = 8;
         auto col_of = [&](int c) { return c * 16; };
         const int local = quad * 32 + lane;
@@ -568,15 +569,29 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         for (int c = 0; c < kSteps; ++c)
 #pragma unroll
           for (int j = 0; j < 8; ++j) acc[c][j] = 0ull;
+        unsigned long long next0 = 0, next1 = 0;
+        auto scales = [&](int ks) {   // of the next block, read while this one's loads are under way
+          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup);
+          const float sx = sc[(ks & 3) * S::kVecRows + local];
+          const float2 sw = *reinterpret_cast<const float2 *>(sc + 4 * S::kVecRows + 2 * (ks & 3));
+          next0 = twice(sx * sw.x);
+          next1 = twice(sx * sw.y);
+        };
+        auto scales_done = [&] {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[sg]);
+          if (++sg == S::kScaleGroups) {
+            sg = 0;
+            sg_par ^= 1u;
+          }
+        };
+        if (!wait(&sc_full[sg], sg_par)) break;
+        scales(0);
         if (!wait(&acc_full[buf], par)) break;
         tc_fence_after();
         tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
         for (int ks = 0; ks < nslab; ++ks) {
-          if ((ks & 3) == 0 && !wait(&sc_full[sg], sg_par)) break;
-          const float *sc = reinterpret_cast<const float *>(smem + S::kOffScale + sg * S::kScaleGroup);
-          const float sx = sc[(ks & 3) * S::kVecRows + local];
-          const float2 sw = *reinterpret_cast<const float2 *>(sc + 4 * S::kVecRows + 2 * (ks & 3));
-          const unsigned long long s0 = twice(sx * sw.x), s1 = twice(sx * sw.y);
+          const unsigned long long s0 = next0, s1 = next1;
           bool ready = false;
 #pragma unroll
           for (int c = 0; c < kSteps; ++c) {
@@ -595,20 +610,20 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
                 tmem_ld_32x16(lanes + buf * S::kAccCols + col_of(0), r[0]);
               }
             }
+            if (c == 1 && ks + 1 < nslab) {
+              if ((ks & 3) == 3) {
+                scales_done();
+                if (!wait(&sc_full[sg], sg_par)) break;
+              }
+              scales(ks + 1);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) fma2(acc[c][j], r[c & 1][2 * j], r[c & 1][2 * j + 1], c >= 4 ? s1 : s0);
           }
           if (!ok) break;
-          if ((ks & 3) == 3 || ks + 1 == nslab) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sc_empty[sg]);
-            if (++sg == S::kScaleGroups) {
-              sg = 0;
-              sg_par ^= 1u;
-            }
-          }
         }
         if (!ok) break;
+        scales_done();
         const int n_cta = ncol / CG;
         const int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
         const bool none = pr < -1;
