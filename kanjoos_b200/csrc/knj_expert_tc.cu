@@ -13,10 +13,11 @@
 // Warps:
 //   epilogue   accumulators from tensor memory, scales, SiLU * up, stores
 //   MMA        tcgen05; accumulators are double-buffered, so a tile's stores overlap the next tile's products
-//   matrix     finds the tiles and their rows in the tables, a tile ahead; TMA boxes of 128 bytes of K: 128 rows, or for gate and up
-//              eight boxes of 16 rows in turn -- gate and up of one output then lie 16 lanes apart in one warp and meet by a shuffle
+//   matrix     TMA boxes of 128 bytes of K: 128 rows, or for gate and up eight boxes of 16 rows in turn -- gate and up of one output
+//              then lie 16 lanes apart in one warp and meet by a shuffle
 //   rows       tile::gather4 TMA copies of four routed rows each; boxes where the rows are all rows in order
-//   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies
+//   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies; 16 bits: finds
+//              the tiles and their rows in the tables, a tile ahead (in e4m3 the matrix warp does)
 // In 16 bits the tensor core adds over all of K. In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
 // adds to its registers in f32 while the tensor core fills the others.
 //
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     }
     for (int i = 0; i < S::kTiles; ++i) {
       mbar_init(&tile_full[i], 1);
-      mbar_init(&tile_empty[i], S::kEpiWarps + S::kRowWarps + (FP8 ? S::kScaleWarps : 0) + (rank == 0 ? 1 : 0));
+      mbar_init(&tile_empty[i], S::kEpiWarps + S::kRowWarps + (FP8 ? S::kScaleWarps : 1) + (rank == 0 ? 1 : 0));
     }
     *s_fail = 0;
     mbar_init_fence();
@@ -361,7 +362,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     }
   };
 
-  // What a tile is, is found once per CTA, by the matrix warp, and handed on through a ring.
+  // What a tile is, is found once per CTA, by one warp (look, publish), and handed on through a ring to all others (tile_take,
+  // tile_done). Finding takes some 2000 cycles a tile. In 16 bits a warp of its own does it, so that the matrix warp leaves no stage
+  // empty meanwhile (4096 tokens gate+up 211 -> 202 us); in e4m3, where the scales take that warp, the matrix
+  // warp does (in front of the scales 1024 tokens gate+up took 108 us instead of 98).
   int tslot = 0;
   uint32_t tpar = 0;
   auto tile_take = [&](Tile &tl) {
@@ -376,6 +380,47 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     if (++tslot == S::kTiles) {
       tslot = 0;
       tpar ^= 1u;
+    }
+  };
+
+  // The tables of a tile are read a tile before it is handed on: behind a full memory queue such a load takes microseconds.
+  constexpr int kPairs = S::kTok / 32;
+  Tile found{};
+  int pr[kPairs], fslot = 0;
+  uint32_t fpar = 1;
+  auto look = [&](int t) {
+    int ntok;
+    found = tile_at(t, ntok);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) pr[j] = pair_at(found, ntok, lane + 32 * j);
+  };
+  auto publish = [&] {
+    int row[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      row[j] = 0;
+      if (pr[j] < 0 || pr[j] >= p.n_pairs) {
+        pr[j] = -1;
+      } else {
+        row[j] = p.row_map ? p.row_map[pr[j]] : p.row_div == 1 ? pr[j] : pr[j] / p.row_div;
+        if (row[j] < 0 || row[j] >= p.n_rows) {
+          pr[j] = -2 - pr[j];
+          row[j] = 0;
+        }
+      }
+    }
+    if (!wait(&tile_empty[fslot], fpar)) return;
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      s_pair[fslot * S::kTok + lane + 32 * j] = pr[j];
+      s_row[fslot * S::kTok + lane + 32 * j] = row[j];
+    }
+    if (lane == 0) s_tile[fslot] = make_int4(found.e, found.n0, found.ncol, found.tok0);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tile_full[fslot]);
+    if (++fslot == S::kTiles) {
+      fslot = 0;
+      fpar ^= 1u;
     }
   };
 
@@ -836,35 +881,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
       split_give_up(t, 0);
     }
   } else if (warp == S::kMatWarp) {
-    // =========================== tiles and matrix rows ===========================
-    constexpr int kPer = S::kTok / 32;
-    // the tables of the next tile are read during this one: behind a full memory queue such a load takes microseconds
-    Tile next{};
-    int pr[kPer], row[kPer];
-    auto look = [&](int t) {
-      int ntok;
-      next = tile_at(t, ntok);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int c = lane + 32 * j;
-        pr[j] = pair_at(next, ntok, c);
-        row[j] = 0;
-      }
-    };
-    auto resolve = [&] {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        if (pr[j] < 0 || pr[j] >= p.n_pairs) {
-          pr[j] = -1;
-        } else {
-          row[j] = p.row_map ? p.row_map[pr[j]] : p.row_div == 1 ? pr[j] : pr[j] / p.row_div;
-          if (row[j] < 0 || row[j] >= p.n_rows) {
-            pr[j] = -2 - pr[j];
-            row[j] = 0;
-          }
-        }
-      }
-    };
+    // =========================== matrix rows (e4m3: and tiles) ===========================
     int st = 0;
     uint32_t par = 1;
     // one stage of the matrix, and the announcement of the bytes of both CTAs' copies into it
@@ -897,37 +914,44 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     };
     int ahead = k_lo;
     if (first < n_tiles) {
-      look(first);
+      int ntok;
+      if constexpr (FP8) look(first);
+      else found = tile_at(first, ntok);
       // the first stages are empty and the matrix depends on no table entry: it travels while those are read
-      for (int i = 0; i < S::kStages && ahead < k_hi; ++i, ahead += S::kSub) issue(next, ahead);
-      resolve();
+      for (int i = 0; i < S::kStages && ahead < k_hi; ++i, ahead += S::kSub) issue(found, ahead);
     }
-    tpar = 1;
     int t = first;
     for (; t < n_tiles; split_end(t), t += step) {
-      const Tile tl = next;
-      if (!wait(&tile_empty[tslot], tpar)) break;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        s_pair[tslot * S::kTok + lane + 32 * j] = pr[j];
-        s_row[tslot * S::kTok + lane + 32 * j] = row[j];
+      Tile tl = found;
+      if constexpr (FP8) {
+        publish();
+        if (!ok) break;
+        if (t + step < n_tiles) look(t + step);
+      } else {
+        if (!tile_take(tl)) break;
       }
-      if (lane == 0) s_tile[tslot] = make_int4(tl.e, tl.n0, tl.ncol, tl.tok0);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tile_full[tslot]);
-      if (++tslot == S::kTiles) {
-        tslot = 0;
-        tpar ^= 1u;
-      }
-      const bool more = t + step < n_tiles;
-      if (more) look(t + step);
       for (int ks = ahead; ks < k_hi; ks += S::kSub) {
         if (!wait(&empty[st], par)) break;
         issue(tl, ks);
       }
       ahead = k_lo;
       if (!ok) break;
-      if (more) resolve();
+      if (!FP8) tile_done();
+    }
+    split_give_up(t, 0);
+  } else if (!FP8 && warp == S::kScaleWarp) {
+    // =========================== tiles ===========================
+    int t = first;
+    if (first < n_tiles) {
+      look(first);
+      publish();
+    }
+    for (; ok && t < n_tiles; split_end(t), t += step) {
+      if (t + step < n_tiles) {
+        look(t + step);
+        publish();
+        if (!ok) break;
+      }
     }
     split_give_up(t, 0);
   } else if (FP8 && warp >= S::kScaleWarp && warp < S::kScaleWarp + S::kScaleWarps) {
@@ -1026,9 +1050,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
       if (!ok) break;
     }
     split_give_up(t, 0);
-  } else if (SPLIT) {
-    for (int t = first; t < n_tiles; t += step) split_end(t);   // a warp without a part in it
   }
+  static_assert(!SPLIT || S::kThreads == 32 * (S::kEpiWarps + 4), "every warp of a split tile meets its syncs");
 
   if (!ok) {
     // a wait gave up: let the copies that are in flight land before this CTA's shared memory is handed on
