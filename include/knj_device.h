@@ -485,6 +485,7 @@ int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K
  *   n = y * rsqrt(mean(y^2) + eps) * post_w   (post_w NULL: n = y)
  *   s = beta * x + alpha * g * n              (y NULL: s = beta * x)
  *   h = s * rsqrt(mean(s^2) + eps) * pre_w    (pre_w and h NULL: not formed)
+ * multiplied from the left to the right, but alpha, post_w and a gate per channel with one another first.
  * stream_out receives s (NULL: not stored), h the rows of the next block; h is formed from s before s is rounded to
  * stream_dtype. The gate g: one value per channel (gate [hidden]), per row (gate[t * ldg]) or per element (row stride
  * ldg); gate_sigmoid = 1 applies 1 / (1 + exp(-g)) first. h_dtype KNJ_DT_E4M3: codes as knj_fp8_rows_launch forms them,

@@ -290,7 +290,9 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
     // y is unpacked here and once more below: in the type it came in it takes half of the registers meanwhile
     auto y_of = [&](int c, float2 (&v)[4]) { values8<Y == 2>(yr[c], yb, v); };
     if (Y != 0 && p.post_w) rs = rms_inverse(squares(y_of, false), p.inv_h, p.eps, [&] { return squares(y_of, true); });
-    if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
+    // The inverse norm meets y before anything else does: y * rs is of order one, y times a gate may be infinite and rs times one denormal.
+    float row_gate = 1.f;
+    if (Y != 0 && p.gate_kind == KNJ_GATE_ROW) row_gate = gate_value(p, t * p.ldg);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int i = first + kLanes * c;
@@ -298,17 +300,24 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
       values8<XW>(xr[c], xb, s[c]);
       if (i < H8) {
         float2 n[4];
-        if (Y != 0) y_of(c, n);
+        if constexpr (Y != 0) y_of(c, n);
         if (Y != 0 && p.gate_kind == KNJ_GATE_FULL) {
           float2 w[4];
           load8(p.gate, p.gate_dtype, t * p.ldg + 8 * i, w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) n[j] = __fmul2_rn(n[j], p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
+          for (int j = 0; j < 4; ++j) n[j] = __fmul2_rn(mul2(n[j], rs), p.gate_sigmoid ? sigmoid2(w[j]) : w[j]);
+        } else if (Y != 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) n[j] = mul2(n[j], rs);
+          if (p.gate_kind == KNJ_GATE_ROW) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) n[j] = mul2(n[j], row_gate);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s[c][j] = mul2(s[c][j], p.beta);
-          if constexpr (Y != 0) s[c][j] = __ffma2_rn(mul2(n[j], rs), post[kKeep ? c : 0][j], s[c][j]);
+          if constexpr (Y != 0) s[c][j] = __ffma2_rn(n[j], post[kKeep ? c : 0][j], s[c][j]);
         }
         if (RING && !landed) {   // the wait gave up: NaN is stored
 #pragma unroll
@@ -327,7 +336,7 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
     for (int c = 0; c < NC; ++c) {
       if (!kKeep) pre_of(c, pre[0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[c][j] = __fmul2_rn(s[c][j], mul2(pre[kKeep ? c : 0][j], hs));   // zeros behind the row
+      for (int j = 0; j < 4; ++j) s[c][j] = __fmul2_rn(mul2(s[c][j], hs), pre[kKeep ? c : 0][j]);   // zeros behind the row
     }
     if (p.h_dtype != KNJ_DT_E4M3) {
 #pragma unroll
@@ -456,9 +465,9 @@ __device__ __forceinline__ void any_codes(const float (&v)[4], uint8_t *q, float
 }
 
 // One CTA per row; a warp holds NC groups of 128 values, a lane every 32nd value of each, so that any row's accesses are runs of 32
-// elements.
+// elements. Two groups a warp: 40 registers, six CTAs of 256 threads (with 48 and five, 16384 x 2047 takes 167 us).
 template <int NC>
-__global__ void __launch_bounds__(NC == 2 ? 512 : 1024) block_norm_any_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NC == 2 ? 512 : 1024, NC == 2 ? 3 : 1) block_norm_any_kernel(const NormParams p) {
   __shared__ float red[32];
   grid_dep_wait();
   const int64_t t = blockIdx.x;
@@ -478,9 +487,15 @@ __global__ void __launch_bounds__(NC == 2 ? 512 : 1024) block_norm_any_kernel(co
       for (int k = 0; k < 4; ++k) a = fmaf(v[c][k] * down, v[c][k] * down, a);
     return block_sum(a, red);
   };
-  float rs = p.alpha;
-  if (p.y && p.post_w) rs = p.alpha * rms_inverse(squares(n, 1.f), p.inv_h, p.eps, [&] { return squares(n, kDown); });
-  if (p.gate_kind == KNJ_GATE_ROW) rs *= gate_value(p, t * p.ldg);
+  // the inverse norm meets y before anything else does: see the 16-byte form
+  auto times = [&](float f) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[c][k] *= f;
+  };
+  if (p.y && p.post_w) times(rms_inverse(squares(n, 1.f), p.inv_h, p.eps, [&] { return squares(n, kDown); }));
+  if (p.gate_kind == KNJ_GATE_ROW) times(gate_value(p, t * p.ldg));
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int g = warp + warps * c;
@@ -499,7 +514,7 @@ __global__ void __launch_bounds__(NC == 2 ? 512 : 1024) block_norm_any_kernel(co
         for (int k = 0; k < 4; ++k) n[c][k] *= p.gate_sigmoid ? __fdividef(1.0f, 1.0f + expf(-w[k])) : w[k];
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[c][k] = any_at(g, lane, k) < H ? fmaf(n[c][k], rs, s[c][k]) : 0.f;
+      for (int k = 0; k < 4; ++k) s[c][k] = any_at(g, lane, k) < H ? fmaf(n[c][k], p.alpha, s[c][k]) : 0.f;
     }
     if (p.stream) any_store(p.stream, p.stream_dtype, t * p.ld_stream, g, lane, H, s[c]);
   }
@@ -511,7 +526,7 @@ __global__ void __launch_bounds__(NC == 2 ? 512 : 1024) block_norm_any_kernel(co
     if (g >= groups) break;
     any_load(p.pre_w, p.w_dtype, 0, g, lane, H, w);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[c][k] *= hs * w[k];
+    for (int k = 0; k < 4; ++k) s[c][k] = s[c][k] * hs * w[k];
     if (p.h_dtype != KNJ_DT_E4M3) any_store(p.h, p.h_dtype, t * p.ldh, g, lane, H, s[c]);
     else any_codes(s[c], static_cast<uint8_t *>(p.h), p.h_scale + t * groups + g, t * p.ldh, g, lane, H);
   }
