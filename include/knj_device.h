@@ -292,8 +292,9 @@ int knj_q4k_proj_launch(const void *A, int a_dtype, int64_t lda, const uint8_t *
                         knj_stream_t s);
 #define knj_q4k_down_launch knj_q4k_proj_launch
 
-/* Limit, in SM clock cycles, of every bounded wait of the decode-class kernels
- * (no reference counterpart; default about one second, <= 0 restores it). A wait
+/* Limit, in SM clock cycles, of every bounded wait of the decode-class kernels and
+ * of knj_block_norm_launch (no reference counterpart; default about one second,
+ * <= 0 restores it). A wait
  * that runs out makes the kernel skip the rest of its work and raise its status
  * word; nothing traps and the context stays usable. */
 void knj_decode_wait_limit(long long cycles);
@@ -490,7 +491,8 @@ int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K
  * stream_dtype. The gate g: one value per channel (gate [hidden]), per row (gate[t * ldg]) or per element (row stride
  * ldg); gate_sigmoid = 1 applies 1 / (1 + exp(-g)) first. h_dtype KNJ_DT_E4M3: codes as knj_fp8_rows_launch forms them,
  * scales in h_scale. stream_out may be x or y itself (same type and stride), h must not overlap an input. Rows whose
- * strides and bases are whole 16-byte units, with hidden a multiple of 8, take 16-byte loads and stores. */
+ * strides and bases are whole 16-byte units, with hidden a multiple of 8, take 16-byte loads and stores. status (optional
+ * device int, zeroed by the caller) is set to 1 when a bounded wait gave up; the rows it concerns are then NaN. */
 #define KNJ_GATE_NONE 0
 #define KNJ_GATE_CHANNEL 1
 #define KNJ_GATE_ROW 2
@@ -513,8 +515,12 @@ typedef struct knj_block_norm_args {
   int32_t x_dtype, y_dtype, w_dtype, gate_dtype, stream_dtype, h_dtype;
   int32_t gate_kind, gate_sigmoid;
   float alpha, beta, eps;
+  int32_t *status;
 } knj_block_norm_args;
 int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s);
+/* Test hook of the calling thread: 1 = in its next norms whose rows travel through shared memory the first row never counts
+ * as landed, so that a wait runs into its limit; 0 = off (default). */
+void knj_block_norm_test_stall(int on);
 
 /* Products of routed rows with expert matrices, grouped by expert, from one pair per expert to all pairs at one
  * (tables as knj_moe_permute_launch makes them; an expert without pairs is not read, rows of out that no table entry
@@ -594,7 +600,7 @@ typedef struct knj_moe_block_args {
 size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype);
 int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
 /* Outcome of the last block launch over this argument block: waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a
- * bounded wait of the expert products gave up. */
+ * bounded wait of its norms or products gave up. */
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s);
 
 /* ======================================================================== */

@@ -50,7 +50,7 @@ class BlockNormArgs(C.Structure):
                 ("stream_out", C.c_void_p), ("ld_stream", C.c_int64), ("h", C.c_void_p), ("ldh", C.c_int64),
                 ("h_scale", C.c_void_p), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("w_dtype", C.c_int32),
                 ("gate_dtype", C.c_int32), ("stream_dtype", C.c_int32), ("h_dtype", C.c_int32), ("gate_kind", C.c_int32),
-                ("gate_sigmoid", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float)]
+                ("gate_sigmoid", C.c_int32), ("alpha", C.c_float), ("beta", C.c_float), ("eps", C.c_float), ("status", C.c_void_p)]
 
 
 def packed(cls):
@@ -216,6 +216,7 @@ SIGNATURES = {
     "knj_fp8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
     # a BlockNormArgs or ExpertGemmArgs by reference, or its bytes (packed)
     "knj_block_norm_launch": (_i, [_vp, _vp]),
+    "knj_block_norm_test_stall": (None, [_i]),
     "knj_expert_gateup_launch": (_i, [_vp, _vp]),
     "knj_expert_proj_launch": (_i, [_vp, _vp]),
     "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),

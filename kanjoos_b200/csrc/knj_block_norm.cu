@@ -18,7 +18,12 @@ struct NormParams {
   int64_t ldx, ldy, ldg, ld_stream, ldh;
   int T, H, x_dtype, y_dtype, w_dtype, gate_dtype, gate_kind, gate_sigmoid, stream_dtype, h_dtype;
   float alpha, beta, eps, inv_h;
+  int *status;
+  long long wait_cycles;  // limit of the ring's waits
+  int stall;              // test hook: the first row of CTA 0 never counts as landed
 };
+
+thread_local int t_stall = 0;   // knj_block_norm_test_stall
 
 __device__ __forceinline__ float gate_value(const NormParams &p, int64_t i) {
   const float g = load_as_f32(p.gate, p.gate_dtype, i);
@@ -156,15 +161,24 @@ __device__ __forceinline__ float cta_sum(float v, float (*red)[16], int &turn) {
   return ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
 }
 
+// The part of a bounded wait that follows its first try, a function of its own: inlined it cost the loop around it 2 us of 53.
+__device__ __noinline__ bool wait_on(uint64_t *bar, uint32_t parity, long long limit, volatile int *fail) {
+  return mbar_wait_for(bar, parity, limit, fail);
+}
+
 // One CTA walks over rows; a thread holds NC runs of eight values of each, and of the weights: post_w with a gate per channel and
 // alpha folded in, so that a row costs a dozen operations a value (formed anew for each row, and with the gate's exponential, 57:
 // 16384 rows of 2048 took 106 us, issue slots half full). Eight threads in a row hold sixteen runs in turn, a group of e4m3 codes
 // (NC = 1: sixteen threads). RING: the next rows travel through a ring of `depth` rows in shared memory, bulk copies on a barrier
 // each; a row ahead in registers was 24 KB under way per SM, too few for HBM (74 us). 16384 rows of 2048 in bf16 with e4m3 rows out,
-// 235 MB: 52.9 us, 4.44 TB/s; bound by the two sums over the CTA that wait for one another, with five warps per scheduler (four, with
+// 235 MB: 51.6 us, 4.55 TB/s; bound by the two sums over the CTA that wait for one another, with five warps per scheduler (four, with
 // the block's output unpacked once: 57.7). Six with the weights in shared memory: 67 us, the rows no longer fit 80 registers.
 // Without the ring, one row per CTA straight into registers: bound by the launch and the two sums (one row of 2048: 2.6 us).
+// A wait of the ring that gives up does so for the whole CTA and for good: from then on it starts no copy and asks no barrier (one
+// whose phase never completed would pass the next lap's wait), every row that it still has is NaN, and its copies under way are given
+// kLinger cycles to land before its shared memory is handed on.
 constexpr int kMaxRing = 8;
+constexpr long long kLinger = 1ll << 20;
 template <int NC, bool XW, int Y, bool RING>  // XW: x is f32; Y: 0 no block output, 1 two-byte, 2 f32
 __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 : XW || Y == 2 ? 128 : 96) block_norm_vec_kernel(const NormParams p, const int depth) {
   extern __shared__ __align__(128) uint8_t ring[];
@@ -199,7 +213,7 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
   };
   if constexpr (RING) {
     if (tid == 0) {
-      for (int r = 0; r < depth; ++r) mbar_init(&bars[r], 1);
+      for (int r = 0; r < depth; ++r) mbar_init(&bars[r], p.stall && blockIdx.x == 0 && r == 0 ? 2 : 1);
       s_fail = 0;
       mbar_init_fence();
       int64_t t = blockIdx.x;
@@ -262,29 +276,30 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
   const int groups = (p.H + kFp8Group - 1) / kFp8Group;
   int slot = 0;
   uint32_t phase = 0;
+  auto advance = [&] {
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  };
   // where this thread's first run of the row lies in what is written, moved on row by row
   const int s_esz = p.stream_dtype == KNJ_DT_F32 ? 4 : 2, h_esz = p.h_dtype == KNJ_DT_E4M3 ? 1 : p.h_dtype == KNJ_DT_F32 ? 4 : 2;
   uint8_t *s_at = static_cast<uint8_t *>(p.stream) + (blockIdx.x * p.ld_stream + 8 * first) * s_esz;
   uint8_t *h_at = static_cast<uint8_t *>(p.h) + (blockIdx.x * p.ldh + 8 * first) * h_esz;
   const int64_t s_step = gridDim.x * p.ld_stream * s_esz, h_step = gridDim.x * p.ldh * h_esz;
-  for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step) {
+  int64_t t = blockIdx.x;
+  for (; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step) {
     float2 s[NC][4];
-    bool landed = true;
     if constexpr (RING) {
-      landed = mbar_wait(&bars[slot], phase, &s_fail);
+      const bool landed = mbar_try_wait(&bars[slot], phase) || wait_on(&bars[slot], phase, p.wait_cycles, &s_fail);
       const uint8_t *at = ring + (size_t)slot * (x_bytes + y_bytes);
       fetch(at, at + x_bytes, 0, 0);
-    }
-    if constexpr (RING) {
-      __syncthreads();                                     // every thread has its part of the row
+      if (__syncthreads_or(!landed)) break;                // every thread has its part of the row
       if (tid == 0 && t + (int64_t)depth * gridDim.x < p.T) {
         fence_proxy_async();                               // the slot was read through the generic proxy
         send(slot, t + (int64_t)depth * gridDim.x);
       }
-      if (++slot == depth) {
-        slot = 0;
-        phase ^= 1u;
-      }
+      advance();
     }
     float rs = 1.f;
     // y is unpacked here and once more below: in the type it came in it takes half of the registers meanwhile
@@ -319,10 +334,6 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
           s[c][j] = mul2(s[c][j], p.beta);
           if constexpr (Y != 0) s[c][j] = __ffma2_rn(n[j], post[kKeep ? c : 0][j], s[c][j]);
         }
-        if (RING && !landed) {   // the wait gave up: NaN is stored
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[c][j].x = s[c][j].y = __int_as_float(0x7fffffff);
-        }
         if (p.stream) store8(s_at + 8 * kLanes * c * s_esz, p.stream_dtype, s[c]);
       }
     }
@@ -354,6 +365,26 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
         if (i < H8 && (i & 15) == 0) p.h_scale[t * groups + (i >> 4)] = sc.scale;
       }
     }
+  }
+  if constexpr (RING) {
+    if (t >= p.T) return;
+    if (tid == 0) {
+      if (p.status) atomicExch(p.status, 1);
+      for (int64_t r = t; r < p.T && r < t + (int64_t)depth * gridDim.x; r += gridDim.x, advance()) mbar_wait_for(&bars[slot], phase, kLinger, nullptr);
+    }
+    const float nan = __int_as_float(0x7fffffff);
+    const float2 v[4] = {{nan, nan}, {nan, nan}, {nan, nan}, {nan, nan}};
+    for (; t < p.T; t += gridDim.x, s_at += s_step, h_at += h_step)
+#pragma unroll 1
+      for (int c = 0; c < NC; ++c) {
+        const int i = first + kLanes * c;
+        if (i >= H8) continue;
+        if (p.stream) store8(s_at + 8 * kLanes * c * s_esz, p.stream_dtype, v);
+        if (!p.h) continue;
+        if (p.h_dtype != KNJ_DT_E4M3) store8(h_at + 8 * kLanes * c * h_esz, p.h_dtype, v);
+        else *reinterpret_cast<uint2 *>(h_at + 8 * kLanes * c) = codes8(v, 1.f);
+        if (p.h_dtype == KNJ_DT_E4M3 && (i & 15) == 0) p.h_scale[t * groups + (i >> 4)] = nan;
+      }
   }
 }
 
@@ -631,6 +662,8 @@ int block_norm_check(const knj_block_norm_args *a) {
 
 extern "C" {
 
+void knj_block_norm_test_stall(int on) { t_stall = on & 1; }
+
 int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
   const int rc = block_norm_check(a);
   if (rc || a->n_tokens == 0) return rc;
@@ -641,6 +674,7 @@ int knj_block_norm_launch(const knj_block_norm_args *a, knj_stream_t s) {
   p.T = a->n_tokens; p.H = H; p.x_dtype = a->x_dtype; p.y_dtype = a->y_dtype; p.w_dtype = a->w_dtype; p.gate_dtype = a->gate_dtype;
   p.gate_kind = a->gate_kind; p.gate_sigmoid = a->gate_sigmoid; p.stream_dtype = a->stream_dtype; p.h_dtype = a->h_dtype;
   p.alpha = a->alpha; p.beta = a->beta; p.eps = a->eps; p.inv_h = 1.0f / (float)H;
+  p.status = a->status; p.wait_cycles = decode_wait_cycles(); p.stall = t_stall;
   auto units = [](const void *base, int64_t ld, int dtype) { return aligned16(base) && ld * (dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0; };
   const bool vec = H % 8 == 0 && H <= 16384 && units(p.x, p.ldx, p.x_dtype) && (!p.y || units(p.y, p.ldy, p.y_dtype)) && aligned16(p.post_w) &&
                    aligned16(p.pre_w) && (!p.stream || units(p.stream, p.ld_stream, p.stream_dtype)) &&

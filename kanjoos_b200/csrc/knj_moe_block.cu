@@ -100,19 +100,19 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   after.pre_w = a->next_w; after.gate = a->gate; after.ldg = a->ldg; after.stream_out = a->out; after.ld_stream = a->ldo; after.h = a->h_next;
   after.ldh = a->ld_h_next; after.h_scale = a->h_next_scale; after.x_dtype = a->x_dtype; after.y_dtype = KNJ_DT_F32; after.w_dtype = a->w_norm_dtype;
   after.gate_dtype = a->gate_dtype; after.stream_dtype = a->out_dtype; after.h_dtype = a->h_next_dtype; after.gate_kind = a->gate_kind;
-  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps;
+  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps; after.status = w.status;
   rc = block_norm_check(&after);
   if (rc) return rc;
   // the rows of x in the experts' 16-bit type, normalised or as they are
   knj_block_norm_args before{};
   before.n_tokens = T; before.hidden = H; before.x = a->x; before.ldx = a->ldx; before.x_dtype = a->x_dtype; before.w_dtype = a->w_norm_dtype;
-  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps;
+  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps; before.status = w.status;
   if (a->pre_w) {
     before.pre_w = a->pre_w; before.h = w.h; before.ldh = H; before.h_dtype = act;
   } else {
     before.stream_out = w.h; before.ld_stream = H; before.stream_dtype = act;
   }
-  KNJ_CUDA(cudaMemsetAsync(w.status, 0, 16, as_stream(s)));  // the products raise it when a bounded wait gives up
+  KNJ_CUDA(cudaMemsetAsync(w.status, 0, 16, as_stream(s)));  // raised when a bounded wait of a norm or a product gives up
   {
     StageSpan sp("moe-router", s);
     rc = knj_block_norm_launch(&before, s);
@@ -162,7 +162,7 @@ int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s) {
   KNJ_CUDA(cudaMemcpyAsync(&word, w.status, sizeof(word), cudaMemcpyDeviceToHost, as_stream(s)));
   KNJ_CUDA(cudaStreamSynchronize(as_stream(s)));
   if (word != 0) {
-    set_error("knj_moe_block: a bounded device wait of the expert products gave up");
+    set_error("knj_moe_block: a bounded device wait of the norms or the expert products gave up");
     return KNJ_E_TIMEOUT;
   }
   return KNJ_OK;

@@ -404,12 +404,13 @@ def expert_proj(a, W, pair_idx, pair_cnt, P: int, pair_row=None, scale=None, a_s
 
 
 def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False, alpha: float = 1.0, beta: float = 1.0, pre_w=None,
-               eps: float = 1e-6, stream_dtype=None, norm_dtype=torch.bfloat16, stream_out=None):
+               eps: float = 1e-6, stream_dtype=None, norm_dtype=torch.bfloat16, stream_out=None, status=None):
     """What stands between two blocks: s = beta * x + alpha * gate * norm(y; post_w), h = norm(s; pre_w).
     x [T][H] the residual stream, y [T][H] the block's output or None, post_w / pre_w [H] norm weights or None (one type),
     gate [H], [T][1] or [T][H] (through a sigmoid with gate_sigmoid). Returns (s, h): s in stream_dtype (default: x's type;
     None without y unless stream_out or stream_dtype asks for it), h in norm_dtype (None without pre_w), for
-    torch.float8_e4m3fn as (codes, scale). stream_out may be x or y and otherwise overlaps neither."""
+    torch.float8_e4m3fn as (codes, scale). stream_out may be x or y and otherwise overlaps neither. status: an i32 tensor of one
+    element that is set to 1 when a bounded wait gave up (rows concerned are NaN), otherwise left as it is."""
     cur = _cur()
     x_ptr, x_code, ldx = _rows(x, "x", cur)
     shape = x.shape
@@ -452,6 +453,6 @@ def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False,
         s = torch.empty_like(x, dtype=stream_dtype, memory_format=torch.contiguous_format)
         s_ptr, lds = s.data_ptr(), H
     a = _norm_args(T, H, x_ptr, ldx, y_ptr, ldy, post, pre, gate_ptr, ldg, s_ptr, lds, h_ptr, H, scale_ptr, x_code, y_code, w_code, gate_code,
-                   s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps)
+                   s_code, h_code, kind, 1 if gate_sigmoid else 0, alpha, beta, eps, 0 if status is None else _dense(status, "status", cur, (1,), _ONLY_I32))
     check(lib().knj_block_norm_launch(a, _raw_stream()))
     return s, (h if scale is None else (h, scale))
