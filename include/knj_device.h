@@ -596,11 +596,12 @@ typedef struct knj_moe_block_args {
   size_t workspace_bytes;
   int32_t *tap_pair_exp; /* optional [T*k] */
   float *tap_pair_w;
+  int32_t *status; /* device word that a launch clears first and sets to 1 when a bounded wait gave up; NULL: the workspace's first */
 } knj_moe_block_args;
 size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype);
 int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
-/* Outcome of the last block launch over this argument block: waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a
- * bounded wait of its norms or products gave up. */
+/* Outcome of the last launch with this argument block's status word (without one: of the last launch over its workspace, whichever
+ * block's that was): waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a bounded wait of its norms or products gave up. */
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s);
 
 /* ======================================================================== */

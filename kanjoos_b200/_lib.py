@@ -68,7 +68,7 @@ class MoeBlockArgs(C.Structure):
                 ("ldg", C.c_int64), ("w_router", C.c_void_p), ("router_bias", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p),
                 ("w_down", C.c_void_p), ("gate_scale", C.c_void_p), ("up_scale", C.c_void_p), ("down_scale", C.c_void_p),
                 ("h_next", C.c_void_p), ("ld_h_next", C.c_int64), ("h_next_scale", C.c_void_p), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_size_t), ("tap_pair_exp", C.c_void_p), ("tap_pair_w", C.c_void_p)]
+                ("workspace_bytes", C.c_size_t), ("tap_pair_exp", C.c_void_p), ("tap_pair_w", C.c_void_p), ("status", C.c_void_p)]
 
 
 class ExpertGemmArgs(C.Structure):

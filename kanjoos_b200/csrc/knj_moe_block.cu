@@ -28,6 +28,7 @@ BlockWs carve(void *base, int T, int H, int F, int E, int k, int w_dtype) {
   };
   const size_t P = (size_t)T * k;
   const bool q = w_dtype == KNJ_DT_E4M3;
+  w.status = reinterpret_cast<int32_t *>(take(16));   // the first word, whatever the sizes
   w.h = take((size_t)T * H * 2);
   w.hq = q ? take((size_t)T * H) : nullptr;
   w.hs = reinterpret_cast<float *>(q ? take((size_t)T * ((H + 127) / 128) * 4) : nullptr);
@@ -36,7 +37,6 @@ BlockWs carve(void *base, int T, int H, int F, int E, int k, int w_dtype) {
   w.pair_w = reinterpret_cast<float *>(take(P * 4));
   w.pair_idx = reinterpret_cast<int32_t *>(take((size_t)E * T * 4));
   w.pair_cnt = reinterpret_cast<int32_t *>(take((size_t)E * 4));
-  w.status = reinterpret_cast<int32_t *>(take(16));
   w.act = take(P * F * 2);
   w.aq = q ? take(P * F) : nullptr;
   w.as = reinterpret_cast<float *>(q ? take(P * ((F + 127) / 128) * 4) : nullptr);
@@ -93,6 +93,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   const BlockWs w = carve(a->workspace, T, H, F, E, k, a->w_dtype);
   int32_t *pair_exp = a->tap_pair_exp ? a->tap_pair_exp : w.pair_exp;
   float *pair_w = a->tap_pair_w ? a->tap_pair_w : w.pair_w;
+  int32_t *status = a->status ? a->status : w.status;
 
   // what the last launch checks is checked before the first runs
   knj_block_norm_args after{};
@@ -100,19 +101,19 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   after.pre_w = a->next_w; after.gate = a->gate; after.ldg = a->ldg; after.stream_out = a->out; after.ld_stream = a->ldo; after.h = a->h_next;
   after.ldh = a->ld_h_next; after.h_scale = a->h_next_scale; after.x_dtype = a->x_dtype; after.y_dtype = KNJ_DT_F32; after.w_dtype = a->w_norm_dtype;
   after.gate_dtype = a->gate_dtype; after.stream_dtype = a->out_dtype; after.h_dtype = a->h_next_dtype; after.gate_kind = a->gate_kind;
-  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps; after.status = w.status;
+  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps; after.status = status;
   rc = block_norm_check(&after);
   if (rc) return rc;
   // the rows of x in the experts' 16-bit type, normalised or as they are
   knj_block_norm_args before{};
   before.n_tokens = T; before.hidden = H; before.x = a->x; before.ldx = a->ldx; before.x_dtype = a->x_dtype; before.w_dtype = a->w_norm_dtype;
-  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps; before.status = w.status;
+  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps; before.status = status;
   if (a->pre_w) {
     before.pre_w = a->pre_w; before.h = w.h; before.ldh = H; before.h_dtype = act;
   } else {
     before.stream_out = w.h; before.ld_stream = H; before.stream_dtype = act;
   }
-  KNJ_CUDA(cudaMemsetAsync(w.status, 0, 16, as_stream(s)));  // raised when a bounded wait of a norm or a product gives up
+  KNJ_CUDA(cudaMemsetAsync(status, 0, 4, as_stream(s)));  // raised when a bounded wait of a norm or a product gives up
   {
     StageSpan sp("moe-router", s);
     rc = knj_block_norm_launch(&before, s);
@@ -130,7 +131,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   }
   knj_expert_gemm_args g{};
   g.pair_idx = w.pair_idx; g.pair_cnt = w.pair_cnt; g.idx_stride = T; g.n_pairs = P; g.n_experts = E; g.x_dtype = g.w_dtype = a->w_dtype;
-  g.status = w.status;
+  g.status = status;
   {
     StageSpan sp("moe-gate", s);
     g.x = q ? w.hq : w.h; g.x_scale = w.hs; g.ldx = H; g.n_rows = T; g.row_div = k; g.w0 = a->w_gate; g.w1 = a->w_up; g.w0_scale = a->gate_scale;
@@ -157,9 +158,9 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s) {
   const int rc = check(a, "knj_moe_block_status");
   if (rc || a->n_tokens == 0) return rc;
-  const BlockWs w = carve(a->workspace, a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
+  const int32_t *status = a->status ? a->status : static_cast<const int32_t *>(a->workspace);
   int32_t word = 0;
-  KNJ_CUDA(cudaMemcpyAsync(&word, w.status, sizeof(word), cudaMemcpyDeviceToHost, as_stream(s)));
+  KNJ_CUDA(cudaMemcpyAsync(&word, status, sizeof(word), cudaMemcpyDeviceToHost, as_stream(s)));
   KNJ_CUDA(cudaStreamSynchronize(as_stream(s)));
   if (word != 0) {
     set_error("knj_moe_block: a bounded device wait of the norms or the expert products gave up");

@@ -337,6 +337,7 @@ class MoeBlock:
                 not workspace.is_contiguous():
             raise ValueError(f"workspace of {need} contiguous uint8 values on the block's device, 256-byte aligned, needed")
         self.workspace = workspace
+        self._status = torch.zeros(1, dtype=torch.int32, device=bank.gate.device)   # this block's own, whoever shares the workspace
 
     def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:
         b = self.bank
@@ -349,7 +350,7 @@ class MoeBlock:
                          w_router=b.router.data_ptr(), router_bias=ptr(b.router_bias), w_gate=b.gate.data_ptr(), w_up=b.up.data_ptr(),
                          w_down=b.down.data_ptr(), gate_scale=ptr(b.gate_scale), up_scale=ptr(b.up_scale), down_scale=ptr(b.down_scale),
                          h_next=ptr(h_next), ld_h_next=H, h_next_scale=ptr(h_scale), workspace=self.workspace.data_ptr(),
-                         workspace_bytes=self.workspace.numel())
+                         workspace_bytes=self.workspace.numel(), status=self._status.data_ptr())
         for w in (b.pre_norm, b.post_norm, next_norm):
             if w is not None:
                 a.w_norm_dtype = _DT_FLOAT[w.dtype]

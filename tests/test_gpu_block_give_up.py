@@ -66,3 +66,35 @@ def test_status_words_that_are_refused():
     for bad in (torch.zeros(1, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32)):
         with pytest.raises(ValueError, match="status"):
             ops.block_norm(x, pre_w=w, status=bad)
+
+
+def test_status_of_blocks_that_share_a_workspace(short_limit):
+    """Each block answers for its own last run, whatever another block of other sizes and weights has run over the workspace since."""
+    from kanjoos_b200._lib import KnjError
+    from kanjoos_b200.moe import MoeBlock
+    from test_gpu_moe_block import bank_of, on_device
+    H = 256
+    banks = [on_device(bank_of(kd, 8, H, 128, 10 + i)) for i, kd in enumerate((BF16, E4M3))]
+    ws = torch.empty(1 << 25, dtype=torch.uint8, device="cuda")
+    first, second = (MoeBlock(b, top_k=2, max_tokens=4000, workspace=ws) for b in banks)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    x = torch.randn((4000, H), device="cuda", generator=g).to(BF16)
+    want = first.run(x[:7]).clone()
+    second.run(x)
+    second.status()
+    first.status()
+    assert int(first._status) == 0 and int(second._status) == 0
+    short_limit.knj_block_norm_test_stall(1)
+    try:
+        out = first.run(x)      # 4000 rows: its norms go through the ring
+    finally:
+        short_limit.knj_block_norm_test_stall(0)
+    second.run(x[:20])
+    second.status()
+    with pytest.raises(KnjError, match="gave up"):
+        first.status()
+    bad = torch.isnan(out.float()).all(1)
+    assert bad[0] and 0 < int(bad.sum()) < 100
+    assert torch.equal(first.run(x[:7]), want)
+    first.status()
