@@ -338,6 +338,7 @@ class MoeBlock:
             raise ValueError(f"workspace of {need} contiguous uint8 values on the block's device, 256-byte aligned, needed")
         self.workspace = workspace
         self._status = torch.zeros(1, dtype=torch.int32, device=bank.gate.device)   # this block's own, whoever shares the workspace
+        self._last = None
 
     def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:
         b = self.bank
@@ -404,4 +405,6 @@ class MoeBlock:
 
     def status(self) -> None:
         """Waits for the stream; raises if a bounded wait of the last run gave up."""
+        if self._last is None:
+            return
         check(lib().knj_moe_block_status(C.byref(self._last), C.c_void_p(torch.cuda.current_stream().cuda_stream)))

@@ -77,6 +77,7 @@ def test_status_of_blocks_that_share_a_workspace(short_limit):
     banks = [on_device(bank_of(kd, 8, H, 128, 10 + i)) for i, kd in enumerate((BF16, E4M3))]
     ws = torch.empty(1 << 25, dtype=torch.uint8, device="cuda")
     first, second = (MoeBlock(b, top_k=2, max_tokens=4000, workspace=ws) for b in banks)
+    first.status()   # nothing has run
     g = torch.Generator(device="cuda")
     g.manual_seed(9)
     x = torch.randn((4000, H), device="cuda", generator=g).to(BF16)
