@@ -100,6 +100,8 @@ int make_operand_tensor_map(CUtensorMap *map, const void *base, int elem_bytes, 
 
 // What knj_block_norm_launch checks of its arguments.
 int block_norm_check(const knj_block_norm_args *a);
+// What knj_expert_gateup_launch and knj_expert_proj_launch check of theirs, but for the number of tiles.
+int expert_product_check(const knj_expert_gemm_args *a, bool gateup, const char *who);
 
 // Limit (SM clock cycles) of the bounded waits of the decode-class kernels, as set by knj_decode_wait_limit.
 long long decode_wait_cycles();

@@ -1157,7 +1157,10 @@ int launch_gemm(const GemmParams &p, const Operands &o, cudaStream_t st) {
   return o.fp8 ? launch_rule<true, GATEUP>(p, o, st) : launch_rule<false, GATEUP>(p, o, st);
 }
 
-int check_expert(const knj_expert_gemm_args *a, bool gateup, const char *who) {
+}  // namespace
+
+namespace knj {
+int expert_product_check(const knj_expert_gemm_args *a, bool gateup, const char *who) {
   KNJ_REQUIRE(a, "%s: null argument block", who);
   KNJ_REQUIRE(a->n_pairs >= 0 && a->n_rows >= 0 && a->N > 0 && a->K > 0 && a->n_experts >= 1 && a->n_experts <= kMaxExperts, "%s: bad sizes", who);
   if (a->n_pairs == 0) return KNJ_OK;
@@ -1176,9 +1179,12 @@ int check_expert(const knj_expert_gemm_args *a, bool gateup, const char *who) {
   KNJ_REQUIRE(a->out_dtype >= KNJ_DT_F32 && a->out_dtype <= KNJ_DT_F16, "%s: outputs are f32, bf16 or f16", who);
   return KNJ_OK;
 }
+}  // namespace knj
+
+namespace {
 
 int run_expert(const knj_expert_gemm_args *a, bool gateup, const char *who, knj_stream_t s) {
-  const int rc = check_expert(a, gateup, who);
+  const int rc = expert_product_check(a, gateup, who);
   if (rc || a->n_pairs == 0) return rc;
   GemmParams p{};
   p.xs = a->x_scale; p.ws0 = a->w0_scale; p.ws1 = a->w1_scale; p.pair_idx = a->pair_idx; p.pair_cnt = a->pair_cnt; p.row_map = a->row_map;

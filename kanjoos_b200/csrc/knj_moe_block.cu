@@ -64,7 +64,8 @@ int check(const knj_moe_block_args *a, const char *who) {
   KNJ_REQUIRE(a->w_dtype >= KNJ_DT_BF16 && a->w_dtype <= KNJ_DT_E4M3, "%s: experts are bf16, f16 or e4m3", who);
   KNJ_REQUIRE(a->x && a->out && a->w_router && a->w_gate && a->w_up && a->w_down, "%s: null tensor pointer", who);
   KNJ_REQUIRE(a->w_dtype != KNJ_DT_E4M3 || (a->gate_scale && a->up_scale && a->down_scale), "%s: e4m3 experts need their scales", who);
-  KNJ_REQUIRE((int64_t)a->n_tokens * a->top_k < (1ll << 31), "%s: too many tokens", who);
+  KNJ_REQUIRE(aligned16(a->w_router), "%s: the router's weights must be 16-byte aligned", who);
+  KNJ_REQUIRE((int64_t)a->n_tokens * a->top_k <= (1ll << 30), "%s: more than 2^30 pairs of a token and an expert", who);
   KNJ_REQUIRE((a->next_w != nullptr) == (a->h_next != nullptr), "%s: next_w and h_next go together", who);
   const size_t need = knj_moe_block_workspace_bytes(a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
   if (!a->workspace || a->workspace_bytes < need) {
@@ -95,7 +96,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   float *pair_w = a->tap_pair_w ? a->tap_pair_w : w.pair_w;
   int32_t *status = a->status ? a->status : w.status;
 
-  // what the last launch checks is checked before the first runs
+  // what the launches check of the caller's operands is checked before the first runs
   knj_block_norm_args after{};
   after.n_tokens = T; after.hidden = H; after.x = a->x; after.ldx = a->ldx; after.y = w.sum; after.ldy = H; after.post_w = a->post_w;
   after.pre_w = a->next_w; after.gate = a->gate; after.ldg = a->ldg; after.stream_out = a->out; after.ld_stream = a->ldo; after.h = a->h_next;
@@ -113,6 +114,19 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   } else {
     before.stream_out = w.h; before.ld_stream = H; before.stream_dtype = act;
   }
+  knj_expert_gemm_args gateup{};
+  gateup.pair_idx = w.pair_idx; gateup.pair_cnt = w.pair_cnt; gateup.idx_stride = T; gateup.n_pairs = P; gateup.n_experts = E;
+  gateup.x_dtype = gateup.w_dtype = a->w_dtype; gateup.status = status;
+  knj_expert_gemm_args down = gateup;
+  gateup.x = q ? w.hq : w.h; gateup.x_scale = w.hs; gateup.ldx = H; gateup.n_rows = T; gateup.row_div = k; gateup.w0 = a->w_gate; gateup.w1 = a->w_up;
+  gateup.w0_scale = a->gate_scale; gateup.w1_scale = a->up_scale; gateup.N = F; gateup.K = H; gateup.out = w.act; gateup.ldo = F; gateup.out_dtype = act;
+  gateup.out_scale = act == KNJ_DT_F16 ? kF16Prescale : 1.0f;
+  down.x = q ? w.aq : w.act; down.x_scale = w.as; down.ldx = F; down.n_rows = P; down.row_div = 1; down.w0 = a->w_down; down.w0_scale = a->down_scale;
+  down.N = H; down.K = F; down.out = w.Y; down.ldo = H; down.out_dtype = KNJ_DT_F32; down.out_scale = act == KNJ_DT_F16 ? 1.0f / kF16Prescale : 1.0f;
+  rc = block_norm_check(&before);
+  if (!rc) rc = expert_product_check(&gateup, true, "knj_moe_block, gate and up");
+  if (!rc) rc = expert_product_check(&down, false, "knj_moe_block, down");
+  if (rc) return rc;
   KNJ_CUDA(cudaMemsetAsync(status, 0, 4, as_stream(s)));  // raised when a bounded wait of a norm or a product gives up
   {
     StageSpan sp("moe-router", s);
@@ -129,24 +143,16 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
     if (q) rc = knj_fp8_rows_launch(w.h, act, H, T, H, w.hq, w.hs, s);
     if (rc) return rc;
   }
-  knj_expert_gemm_args g{};
-  g.pair_idx = w.pair_idx; g.pair_cnt = w.pair_cnt; g.idx_stride = T; g.n_pairs = P; g.n_experts = E; g.x_dtype = g.w_dtype = a->w_dtype;
-  g.status = status;
   {
     StageSpan sp("moe-gate", s);
-    g.x = q ? w.hq : w.h; g.x_scale = w.hs; g.ldx = H; g.n_rows = T; g.row_div = k; g.w0 = a->w_gate; g.w1 = a->w_up; g.w0_scale = a->gate_scale;
-    g.w1_scale = a->up_scale; g.N = F; g.K = H; g.out = w.act; g.ldo = F; g.out_dtype = act; g.out_scale = act == KNJ_DT_F16 ? kF16Prescale : 1.0f;
-    rc = knj_expert_gateup_launch(&g, s);
+    rc = knj_expert_gateup_launch(&gateup, s);
     if (rc) return rc;
   }
   {
     StageSpan sp("moe-down", s);
     if (q) rc = knj_fp8_rows_launch(w.act, act, F, P, F, w.aq, w.as, s);
     if (rc) return rc;
-    g.x = q ? w.aq : w.act; g.x_scale = w.as; g.ldx = F; g.n_rows = P; g.row_div = 1; g.w0 = a->w_down; g.w1 = nullptr; g.w0_scale = a->down_scale;
-    g.w1_scale = nullptr; g.N = H; g.K = F; g.out = w.Y; g.ldo = H; g.out_dtype = KNJ_DT_F32;
-    g.out_scale = act == KNJ_DT_F16 ? 1.0f / kF16Prescale : 1.0f;
-    rc = knj_expert_proj_launch(&g, s);
+    rc = knj_expert_proj_launch(&down, s);
     if (rc) return rc;
   }
   StageSpan sp("moe-scatter", s);
