@@ -123,6 +123,13 @@ def _bf16_bits(info: TensorInfo, raw: np.ndarray) -> np.ndarray:
     return ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
 
 
+def _f32(info: TensorInfo, raw: np.ndarray) -> np.ndarray:
+    """Weights of an unquantised tensor as f32, which holds every f32, f16 and bf16 value."""
+    if info.ggml_type == GGML_BF16:
+        return (raw.view(np.uint16).astype(np.uint32) << 16).view(np.float32)
+    return raw.view(np.float32 if info.ggml_type == GGML_F32 else np.float16).astype(np.float32)
+
+
 def layer_arrays(g: GgufFile, layer: int) -> dict:
     """Host arrays of one block's MoE-FFN tensors: gate/up/down payloads as uint8
     [E][rows][K/256][bytes per block], router and norm weights as bf16 bits."""
@@ -167,7 +174,8 @@ def load_expert_bank(g: GgufFile, layer: int, device="cuda"):
 
 def float_layer_arrays(g: GgufFile, layer: int) -> dict:
     """Host arrays of one block's MoE-FFN tensors where the experts are not quantised: gate/up [E][F][H] and down [E][H][F] as
-    uint16 bit patterns (`expert_type` "f16" or "bf16", one type for the three), router and norm weights as bf16 bits."""
+    uint16 bit patterns (`expert_type` "f16" or "bf16", one type for the three), router as bf16 bits (`router_exact`: whether the file
+    has it so), norm weights as f32."""
     p = g.arch() + "."
     E = g.meta_int(p + "expert_count")
     b = f"blk.{layer}."
@@ -190,14 +198,15 @@ def float_layer_arrays(g: GgufFile, layer: int) -> dict:
     for key, name in (("norm", "ffn_norm"), ("post_norm", "post_ffw_norm")):
         n = g.tensors.get(b + name + ".weight")
         if n is not None:
-            out[key] = _bf16_bits(n, np.asarray(g.payload(n)))
-            out[key + "_exact"] = n.ggml_type == GGML_BF16
+            out[key] = _f32(n, np.asarray(g.payload(n)))
     return out
 
 
 def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = False):
     """`FloatExpertBank` of block `layer` (F16 or BF16 experts; e4m3=True turns them into e4m3 blocks) and the block's top-k. A
-    `post_ffw_norm` tensor, where the file has one, becomes the norm behind the block."""
+    `post_ffw_norm` tensor, where the file has one, becomes the norm behind the block. Norm weights are f32 with the file's values; the
+    router is bf16, and the bank's `router_exact` is False where the file holds more bits: experts whose logits differ by less than
+    that rounding may then be chosen in another order than from the file's values."""
     import torch
     from .moe import FloatExpertBank
     a = float_layer_arrays(g, layer)
@@ -205,9 +214,9 @@ def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = 
     def bits(u16, dtype):
         return torch.from_numpy(np.ascontiguousarray(u16).view(np.int16).copy()).view(dtype).to(device)
     kind = torch.float16 if a["expert_type"] == "f16" else torch.bfloat16
-    norm = {k: bits(a[n], torch.bfloat16) if n in a else None for k, n in (("pre_norm", "norm"), ("post_norm", "post_norm"))}
+    norm = {k: torch.from_numpy(a[n]).to(device) if n in a else None for k, n in (("pre_norm", "norm"), ("post_norm", "post_norm"))}
     bank = FloatExpertBank(gate=bits(a["gate"], kind), up=bits(a["up"], kind), down=bits(a["down"], kind), router=bits(a["router"], torch.bfloat16),
-                           rms_eps=a["rms_eps"], **norm)
+                           router_exact=a["router_exact"], rms_eps=a["rms_eps"], **norm)
     return (bank.to_e4m3() if e4m3 else bank), a["top_k"]
 
 

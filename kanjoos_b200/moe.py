@@ -257,7 +257,8 @@ class FloatExpertBank:
 
     gate, up [E][F][H]; down [E][H][F]; for e4m3 their scales f32 [E][ceil(rows/128)][ceil(cols/128)]; router bf16 [E][H];
     router_bias f32 [E] or None; pre_norm, post_norm: norm weights [H] in front of the block and behind it (one type), or None;
-    out_gate [H]: what the block's output is multiplied with (through a sigmoid with gate_sigmoid), or None."""
+    out_gate [H]: what the block's output is multiplied with (through a sigmoid with gate_sigmoid), or None; router_exact: False where
+    the router's bf16 weights were rounded from a file that holds more bits."""
     gate: torch.Tensor
     up: torch.Tensor
     down: torch.Tensor
@@ -273,6 +274,7 @@ class FloatExpertBank:
     alpha: float = 1.0
     beta: float = 1.0
     rms_eps: float = synth.RMS_EPS
+    router_exact: bool = True
 
     @property
     def n_experts(self) -> int:
@@ -367,8 +369,9 @@ class MoeBlock:
 
     def run(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
         """x [T][H] f32 / bf16 / f16 -> the stream behind the block, in x's type or into `out` (which may be x). gate: the rows' own
-        gate [T][1] or [T][H] in place of the bank's. next_norm [H]: also returns h = norm(out; next_norm) in next_dtype (default:
-        x's type; float8_e4m3fn: (codes, scale)). Returns out, or a tuple (out[, h][, pair_exp, pair_w])."""
+        gate [T][1] or [T][H] in place of the bank's. next_norm [H], in the type of the bank's norms (any float type where those are
+        f32): also returns h = norm(out; next_norm) in next_dtype (default: x's type; float8_e4m3fn: (codes, scale)). Returns out, or
+        a tuple (out[, h][, pair_exp, pair_w])."""
         b = self.bank
         if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > self.max_tokens or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
             raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {self.max_tokens}")
@@ -388,9 +391,11 @@ class MoeBlock:
         h = scale = None
         if next_norm is not None:
             norms = [w for w in (b.pre_norm, b.post_norm) if w is not None]
+            if norms and norms[0].dtype == torch.float32 and next_norm.dtype in _DT_FLOAT:
+                next_norm = next_norm.float()   # the same values
             if tuple(next_norm.shape) != (H,) or next_norm.dtype not in _DT_FLOAT or any(w.dtype != next_norm.dtype for w in norms) or \
                     next_norm.device != x.device or not next_norm.is_contiguous():
-                raise ValueError(f"next_norm is {next_norm.dtype} {tuple(next_norm.shape)}, expected [{H}] in the block's norm type")
+                raise ValueError(f"next_norm is {next_norm.dtype} {tuple(next_norm.shape)}, expected [{H}] in the block's norm type (or narrower than f32 ones)")
             h = torch.empty((T, H), dtype=next_dtype or x.dtype, device=x.device)
             if h.dtype == torch.float8_e4m3fn:
                 scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
