@@ -283,12 +283,19 @@ def _refuse(t: torch.Tensor, what: str, cur: int, shape, types):
                      f"{'rows' if shape is None else tuple(shape)}, dense inside a row and without overlap")
 
 
+def _refuse_count(what: str, shape):
+    """The library counts in 32 bits, and ctypes would hand it a larger number's low word."""
+    raise ValueError(f"{what} is {tuple(shape)}: rows and columns have to stay below 2^31")
+
+
 def _rows(t: torch.Tensor, what: str, cur: int, shape=None, types=_DT):
     """A matrix of rows, dense inside a row, any row stride, on the current device: (address, type code, row stride)."""
     code, s = types.get(t.dtype), t.shape
     if code is None or len(s) != 2 or t.get_device() != cur or (shape is not None and s != shape):
         _refuse(t, what, cur, shape, types)
     n, k = s
+    if (n | k) >> 31:
+        _refuse_count(what, s)
     ld, one = t.stride()
     if n <= 1:
         ld = k
@@ -328,6 +335,8 @@ def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtyp
     n, out_code = W.shape[0], _DT.get(out_dtype)
     if out_code is None:
         raise ValueError(f"out_dtype is {out_dtype}")
+    if n >> 31:
+        _refuse_count("W", W.shape)
     w = _dense(W, "W", cur, (n, k), _ONLY_E4M3)
     ws = _dense(W_scale, "W_scale", cur, ((n + 127) // 128, (k + 127) // 128), _ONLY_F32)
     y = x.new_empty(m, n, dtype=out_dtype)
