@@ -396,6 +396,8 @@ class MoeBlock:
             if tuple(next_norm.shape) != (H,) or next_norm.dtype not in _DT_FLOAT or any(w.dtype != next_norm.dtype for w in norms) or \
                     next_norm.device != x.device or not next_norm.is_contiguous():
                 raise ValueError(f"next_norm is {next_norm.dtype} {tuple(next_norm.shape)}, expected [{H}] in the block's norm type (or narrower than f32 ones)")
+            if next_dtype not in (None, torch.float8_e4m3fn, *_DT_FLOAT):
+                raise ValueError(f"next_dtype is {next_dtype}, expected f32, bf16, f16 or float8_e4m3fn")
             h = torch.empty((T, H), dtype=next_dtype or x.dtype, device=x.device)
             if h.dtype == torch.float8_e4m3fn:
                 scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
