@@ -355,7 +355,9 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   auto split_give_up = [&](int t, int done) {   // from the tile t on, of whose syncs `done` have been met
     if constexpr (SPLIT) {
       if (ok) return;
-      if (lane == 0) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int *>(s_fail), 0)), "r"(1) : "memory");
+      // the first CTA is there as long as a sync is left; without one nobody would read it
+      const bool left = t < n_tiles && (done < split_syncs(t) || t + step < n_tiles);
+      if (left && lane == 0) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int *>(s_fail), 0)), "r"(1) : "memory");
       __syncwarp();
       for (; t < n_tiles; t += step, done = 0)
         for (int i = done; i < split_syncs(t); ++i) cluster_sync_all();
@@ -667,7 +669,10 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
           }
           if (!ok) break;
         }
-        if (!ok) break;
+        if (!ok) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");   // a load may be under way, and tensor memory is freed soon
+          break;
+        }
         scales_done();
         const int n_cta = ncol / CG;
         const int pr = local < n_cta ? pairs[(int)rank * n_cta + local] : -1;
