@@ -292,8 +292,8 @@ int knj_q4k_proj_launch(const void *A, int a_dtype, int64_t lda, const uint8_t *
                         knj_stream_t s);
 #define knj_q4k_down_launch knj_q4k_proj_launch
 
-/* Limit, in SM clock cycles, of every bounded wait of the decode-class kernels and
- * of knj_block_norm_launch (no reference counterpart; default about one second,
+/* Limit, in SM clock cycles, of every bounded wait of the decode-class kernels, of
+ * knj_block_norm_launch and of the products with bf16, f16 and e4m3 matrices (no reference counterpart; default about one second,
  * <= 0 restores it). A wait
  * that runs out makes the kernel skip the rest of its work and raise its status
  * word; nothing traps and the context stays usable. */
@@ -554,10 +554,15 @@ int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
  * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes.
  * Process-wide. */
 void knj_expert_tc_form(int form);
+/* Test hook of the calling thread: in its next products 1 = the first accumulator of the first thread block, 2 = that block's first
+ * operands, 3 = the first accumulator of the last thread block of its pair or cluster never count as complete, so that a wait runs
+ * into its limit; 0 = off (default). */
+void knj_expert_tc_test_stall(int what);
 
 /* Dense product with an e4m3 matrix: y[m][n_out] = x[m][n_in] . W^T, W e4m3 [n_out][n_in] with W_scale
  * [ceil(n_out/128)][ceil(n_in/128)]; the rows of x (f32, bf16 or f16) are turned into e4m3 codes first, as
- * knj_fp8_rows_launch does, in the workspace (256-byte aligned). n_in a multiple of 16. y f32, bf16 or f16. */
+ * knj_fp8_rows_launch does, in the workspace (256-byte aligned). n_in a multiple of 16. y f32, bf16 or f16. status as in
+ * knj_expert_gemm_args. */
 size_t knj_fp8_matmul_workspace_bytes(int m, int n_in);
 int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, int64_t ldx, int m, void *y,
                           int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);

@@ -223,6 +223,7 @@ SIGNATURES = {
     "knj_moe_block_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
     "knj_moe_block_status": (_i, [C.POINTER(MoeBlockArgs), _vp]),
     "knj_expert_tc_form": (None, [_i]),
+    "knj_expert_tc_test_stall": (None, [_i]),
     "knj_fp8_matmul_workspace_bytes": (_sz, [_i, _i]),
     "knj_fp8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),
     "knj_moe_ffn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),

@@ -21,8 +21,9 @@
 // In 16 bits the tensor core adds over all of K. In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
 // adds to its registers in f32 while the tensor core fills the others.
 //
-// Every wait on an mbarrier is bounded; on give-up the kernel raises a status flag, stores NaN in place of the outputs it did not
-// form, frees its tensor memory and returns.
+// Every wait on an mbarrier is bounded (knj_decode_wait_limit); on give-up the kernel raises a status flag, stores NaN in place of the
+// outputs it did not form, frees its tensor memory and returns. Barriers of a CTA or a cluster have no limit of their own: all their
+// warps meet all of them, whichever gave up.
 #include "knj_fp8.cuh"
 #include "knj_tc.cuh"
 
@@ -50,8 +51,11 @@ struct GemmParams {
   int vec_out;                // bases and strides of the outputs allow 16-byte (lane = row form: 32-byte) stores
   int dense;                  // rows 0 .. n_pairs-1 in order: copied as boxes instead of gathered
   float out_scale;
+  int stall;                  // test hook (knj_expert_tc_test_stall)
+  long long wait_cycles;      // limit of the waits on mbarriers
   CUtensorMap map0, map1, mapx;
 };
+thread_local int t_stall = 0;
 
 // kSingle: single SMs, two CTAs each, buckets of up to 64 rows. kPair: CTA pairs, buckets of up to 256. kSplit: as kSingle with
 // buckets of up to 32, where the tiles are too few for the GPU: a cluster of CTAs shares each tile's K, and its first CTA adds the
@@ -226,12 +230,14 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     if (lane < 2 || GATEUP) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   if (tid == 0) {
+    // a barrier that the hook stalls expects an arrival too many
+    const bool first_cta = blockIdx.x == 0, last_of_cluster = (int)blockIdx.x == CG * parts - 1;
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], i == 0 && p.stall == 2 && first_cta ? 2 : 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < S::kAccs; ++i) {
-      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_full[i], i == 0 && ((p.stall == 1 && first_cta) || (p.stall == 3 && last_of_cluster)) ? 2 : 1);
       mbar_init(&acc_empty[i], CG * (S::kRowsM ? S::kEpiWarps / 2 : S::kEpiWarps));
     }
     for (int i = 0; i < S::kScaleGroups; ++i) {
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   // A warp waits, and goes on or gives up, as a whole. The loops of the issuing warps stay warp-uniform around the elected thread's
   // instructions: with the loop inside the elected branch a stage took ~480 cycles to issue, so ~60 and the wait.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (ok && !mbar_wait(bar, parity, s_fail)) ok = false;
+    if (ok && !mbar_wait_for(bar, parity, p.wait_cycles, s_fail)) ok = false;
     ok = __all_sync(0xffffffffu, ok);
     return ok;
   };
@@ -1109,6 +1115,8 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   p.m_inverse = (uint32_t)((1ull << 32) / p.m_tiles - (p.m_tiles == 1));
   const int out_esz = p.out_dtype == KNJ_DT_F32 ? 4 : 2, unit = S::kRowsM ? 32 : 16;
   p.vec_out = reinterpret_cast<uintptr_t>(p.out) % unit == 0 && p.ldo * out_esz % unit == 0;
+  p.stall = t_stall;
+  p.wait_cycles = decode_wait_cycles();
   const int64_t most = p.pair_idx ? p.E * ((p.idx_stride + S::kTok - 1) / S::kTok) : (p.n_pairs + S::kTok - 1) / S::kTok;
   KNJ_REQUIRE(most * p.m_tiles <= (1ll << 30) && (int64_t)w_rows + 256 < (1ll << 31), "expert product: %lld buckets of %d row tiles are too many",
               (long long)most, p.m_tiles);
@@ -1210,6 +1218,8 @@ extern "C" {
 int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s) { return run_expert(a, true, "knj_expert_gateup", s); }
 
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s) { return run_expert(a, false, "knj_expert_proj", s); }
+
+void knj_expert_tc_test_stall(int what) { t_stall = what >= 1 && what <= 3 ? what : 0; }
 
 void knj_expert_tc_form(int form) { g_form = form >= 1 && form <= 3 ? form : 0; }
 

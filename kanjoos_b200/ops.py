@@ -326,9 +326,9 @@ def _fp8_matmul_scratch(m: int, k: int) -> int:
     return int(lib().knj_fp8_matmul_workspace_bytes(m, k))
 
 
-def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
+def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtype=torch.float32, status=None) -> torch.Tensor:
     """W float8_e4m3fn [n_out][n_in] with W_scale f32 [ceil(n_out/128)][ceil(n_in/128)], x [m][n_in] (f32 / bf16 / f16, turned
-    into e4m3 rows as fp8_rows does) -> [m][n_out] in out_dtype."""
+    into e4m3 rows as fp8_rows does) -> [m][n_out] in out_dtype. status as for expert_gateup."""
     cur = _cur()
     ptr, code, ld = _rows(x, "x", cur)
     m, k = x.shape
@@ -342,11 +342,12 @@ def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtyp
     y = x.new_empty(m, n, dtype=out_dtype)
     nbytes = _fp8_matmul_scratch(m, k)
     work = x.new_empty(nbytes, dtype=torch.uint8)
-    check(lib().knj_fp8_matmul_launch(w, ws, k, n, ptr, code, ld, m, y.data_ptr(), out_code, n, work.data_ptr(), nbytes, None, _raw_stream()))
+    check(lib().knj_fp8_matmul_launch(w, ws, k, n, ptr, code, ld, m, y.data_ptr(), out_code, n, work.data_ptr(), nbytes,
+                                      None if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), _raw_stream()))
     return y
 
 
-def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale):
+def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale, status):
     cur = _cur()
     if w.dim() != 3 or w.dtype not in _OPERAND:
         raise ValueError(f"expert matrices are bf16, f16 or float8_e4m3fn [E][N][K], got {w.dtype} {tuple(w.shape)}")
@@ -387,29 +388,32 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
         out_ptr, ldo = out.data_ptr(), N
     else:
         out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
-    a = _expert_args(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo, 0, x.shape[0], P, N, K, E,
+    a = _expert_args(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo,
+                     0 if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), x.shape[0], P, N, K, E,
                      row_div, x_code, x_code, out_code, out_scale)
     check(launch(a, _raw_stream()))
     return out
 
 
 def expert_gateup(x, Wg, Wu, pair_idx, pair_cnt, P: int, top_k: int, pair_tok=None, gate_scale=None, up_scale=None, x_scale=None,
-                  out_dtype=None, out=None, out_scale: float = 1.0):
+                  out_dtype=None, out=None, out_scale: float = 1.0, status=None):
     """silu(x . Wg[e]) * (x . Wu[e]) * out_scale for every routed pair: [P][N] in out_dtype (default: the matrices' type, bf16
     for e4m3 ones). Wg, Wu [E][N][K] bf16 / f16 (x in the same type) or float8_e4m3fn with gate_scale and up_scale f32
     [E][ceil(N/128)][ceil(K/128)] (x e4m3 with x_scale, or f32 / bf16 / f16, which fp8_rows turns into e4m3 rows). x [T][K];
-    pair p reads row pair_tok[p], or p // top_k. Rows of pairs that no table entry names are left as they were."""
+    pair p reads row pair_tok[p], or p // top_k. Rows of pairs that no table entry names are left as they were. status: an i32 tensor of
+    one element that is set to 1 when a bounded wait gave up (outputs concerned are NaN), otherwise left as it is."""
     if out_dtype is None:
         out_dtype = torch.bfloat16 if Wg.dtype == _E4M3 else Wg.dtype
     return _expert(lib().knj_expert_gateup_launch, x, x_scale, Wg, Wu, gate_scale, up_scale, pair_idx, pair_cnt, P, pair_tok, top_k, out,
-                   out_dtype, out_scale)
+                   out_dtype, out_scale, status)
 
 
 def expert_proj(a, W, pair_idx, pair_cnt, P: int, pair_row=None, scale=None, a_scale=None, out_dtype=torch.float32, out=None,
-                out_scale: float = 1.0):
+                out_scale: float = 1.0, status=None):
     """a . W[e] * out_scale for every routed pair: [P][N] in out_dtype. a holds one row per pair (row pair_row[p] when given,
-    else p); types, scales and unnamed rows as for expert_gateup."""
-    return _expert(lib().knj_expert_proj_launch, a, a_scale, W, None, scale, None, pair_idx, pair_cnt, P, pair_row, 1, out, out_dtype, out_scale)
+    else p); types, scales, unnamed rows and status as for expert_gateup."""
+    return _expert(lib().knj_expert_proj_launch, a, a_scale, W, None, scale, None, pair_idx, pair_cnt, P, pair_row, 1, out, out_dtype, out_scale,
+                   status)
 
 
 def block_norm(x, y=None, *, post_w=None, gate=None, gate_sigmoid: bool = False, alpha: float = 1.0, beta: float = 1.0, pre_w=None,
