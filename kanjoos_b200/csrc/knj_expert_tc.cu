@@ -725,8 +725,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         // front of each other's sums.
         auto blocks = [&](auto chunks) {
           constexpr int kSteps = 2 * decltype(chunks)::value;   // of 16 columns
-          auto col_of = [&](int c) { return ((c >> 1) * kGroups + group) * 32 + (c & 1) * 16; };
-          unsigned long long acc[kSteps > 0 ? kSteps : 1][2][4];   // pairs of f32 sums: steps, halves, (8 columns, rows)
+          auto col_of = [&](int c) { return c * 16; };
+          unsigned long long acc[kSteps][2][4];   // pairs of f32 sums: steps, halves, (8 columns, rows)
 #pragma unroll
           for (int c = 0; c < kSteps; ++c)
 #pragma unroll
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
             const float2 sw = *reinterpret_cast<const float2 *>(sg_at + 4 * S::kVecRows + 2 * (ks & 3));
             const unsigned long long w0 = twice(sw.x), w1 = twice(sw.y);
             uint32_t r[2][2][8];
-            if constexpr (kSteps > 0) load(r[0][0], r[0][1], col_of(0));
+            load(r[0][0], r[0][1], col_of(0));
 #pragma unroll
             for (int c = 0; c < kSteps; ++c) {
               tmem_ld_wait(r[c & 1][0], r[c & 1][1]);
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
             }
           }
           if constexpr (SPLIT) {
-            uint32_t v[kSteps > 0 ? kSteps : 1][2][8];
+            uint32_t v[kSteps][2][8];
 #pragma unroll
             for (int c = 0; c < kSteps; ++c)
 #pragma unroll
@@ -802,10 +802,8 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
             }
           }
         };
-        const int nc = ((ncol + 31) / 32 - group + kGroups - 1) / kGroups;   // chunks of this group
-        static_assert(kChunks <= 2, "one case for each number of chunks");
-        if (nc <= 0) blocks(std::integral_constant<int, 0>{});
-        else if (nc == 1) blocks(std::integral_constant<int, 1>{});
+        static_assert(kGroups == 1 && kChunks <= 2, "one case for each number of chunks, and no bucket is empty");
+        if (kChunks == 1 || ncol <= 32) blocks(std::integral_constant<int, 1>{});
         else if constexpr (kChunks > 1) blocks(std::integral_constant<int, 2>{});
         if (!ok) break;
       }

@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import synth
-from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 _DT_FLOAT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
