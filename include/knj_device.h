@@ -529,7 +529,8 @@ void knj_block_norm_test_stall(int on);
  *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
  * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
  * p / row_div. e4m3: x_scale [n_rows][ceil(K/128)], w*_scale [n_experts][ceil(N/128)][ceil(K/128)]; the sum over each 128
- * values of K is scaled and added in f32. N is any number, n_rows >= 1, K and ldx are whole 16-byte units, bases are 16-byte aligned.
+ * values of K is scaled and added in f32. silu takes the fast exponential and division: its relative error reaches
+ * 2^-21 (1 + |gate| / 3), which f32 outputs show, and gates below -87 give 0. N is any number, n_rows >= 1, K and ldx are whole 16-byte units, bases are 16-byte aligned.
  * out f32, bf16 or f16 [n_pairs][N], row stride ldo. Table entries outside [0, n_pairs) are skipped, rows outside
  * [0, n_rows) read as zeros. out overlaps no operand; n_pairs and idx_stride are at most 2^30. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
  * the outputs it concerns are then NaN. */
