@@ -524,7 +524,7 @@ void knj_block_norm_test_stall(int on);
 
 /* Products of routed rows with expert matrices, grouped by expert, from one pair per expert to all pairs at one
  * (tables as knj_moe_permute_launch makes them; an expert without pairs is not read, rows of out that no table entry
- * names are left as they were; one that several experts name holds the product with one of them):
+ * names are left as they were; each value of one that several experts name is the product with one of them):
  *   knj_expert_gateup_launch: out[p][n] = out_scale * silu(x[row(p)] . w0[e][n]) * (x[row(p)] . w1[e][n])
  *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
  * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else

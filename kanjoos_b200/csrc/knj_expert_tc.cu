@@ -4,8 +4,8 @@
 //   out[p][n] = out_scale * x[row(p)] . w[e][n]     and     out_scale * silu(x . wg[e][n]) * (x . wu[e][n])
 //   e4m3:  x . w = sum over blocks b of 128 k:  sx[row][b] * sw[n/128][b] * sum_{k in b} qx[k] qw[k]
 //
-// Few rows are bound by the matrices' bytes: every active expert's matrix is read once (512 rows x 8 of 128 experts, bf16: 806 MB, 136 us,
-// 0.91 of the measured copy rate). Many rows are bound by the tensor core: 16384 rows, bf16, 1.34 PFLOP/s alone, 1.1 in a loop under
+// Few rows are bound by the matrices' bytes: every active expert's matrix is read once (512 rows x 8 of 128 experts, bf16: 806 MB, 131 us,
+// 0.94 of the measured copy rate). Many rows are bound by the tensor core: 16384 rows, bf16, 1.38 PFLOP/s alone, 1.13 in a loop under
 // the power limit. One kernel with three forms (enum Form; launch_rule says when) walks over (bucket, row tile) tiles; a bucket is up
 // to kTok routed rows of one expert, and consecutive tiles share it, so that its rows stay in L2 while the matrices stream through
 // once. Persistent CTAs. In all forms but one the MMA's M side is matrix rows and its N side the bucket, so that a ragged bucket wastes
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         // the 16-lane form, 524 cycles of tensor memory (the products take 512). A product is issued as two of 128 columns, 64 rows
         // of each CTA's matrix tile, into buffers of their own: group g reads the buffers of half g, outputs 64 g .. + 63 of gate and
         // of up, or of both blocks of 128 outputs. Whole products in two buffers left the tensor core waiting for the hand-offs, which
-        // still bound it: 8192 x 4096 x 4096 152 us, tensor pipe 41 % busy (copies and products alone: 101 us). The loads run one step
+        // still bound it: 8192 x 4096 x 4096 154 us, tensor pipe 41 % busy (copies and products alone: 101 us). The loads run one step
         // of 16 columns ahead of the sums, across blocks of K too, and whether the next buffer is complete is asked two steps before it
         // is needed; the next block's scales are read after the first step (4096 tokens gate+up 203 -> 196 us; at the block's start, or
         // late in it, 203 to 208). Sixteen warps with 64 sums a thread and one load under way each took 175 us.
@@ -1142,7 +1142,7 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   const int64_t experts = p.E < p.n_pairs ? p.E : p.n_pairs;
   const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
   // K is split where even the smallest tiles leave half of the CTAs' places free, into parts of two slabs or more: one row times
-  // 4096 x 4096 e4m3 21.5 -> 15.4 us, 64 rows 25.6 -> 19.5 (with parts of one slab, K = 512, 15.4 -> 17.4). Clusters of two and
+  // 4096 x 4096 e4m3, rows in 16 bits, 15.1 -> 9.7 us, 64 rows 19.1 -> 13.0 (parts of one slab, K = 512, cost 2 us more than none). Clusters of two and
   // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two took 16.4).
   const int64_t places = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
   int bits = places >= kMaxParts ? 2 : places >= 2 ? 1 : 0;
@@ -1152,12 +1152,13 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
     p.part_bits = bits;
     return launch_form<FP8, GATEUP, kSplit>(p, o, st);
   }
-  // Single SMs or pairs, us each, by (rows per expert; experts). 16 bits, gate and up, hidden 2048, ffn 768: 86, 86 (1; 128), 131, 133
-  // (32; 128), 136, 135 (32, Zipf; 128), 181, 145 (128; 128), 311, 201 (256; 128); hidden 1024, ffn 512: 18.4, 20.5 (1; 32), 20.5, 22.6
-  // (32; 32), 24.6, 22.6 (64; 32) -- pairs where the buckets fill them or the tiles take four rounds of pairs anyway. e4m3, whose pairs
-  // always multiply 256 rows and whose stores no product overlaps: 53, 96 (1; 128), 81, 141 (32; 128), 102, 141 (64; 128), 158, 143
-  // (128; 128), 282, 205 (256; 128); dense 4096 x 4096 x 4096 157, 103, 1024 x 4096 x 1024 (64 tiles of pairs) 25.6, 21.5,
-  // 1024 x 2048 x 2048 (32 tiles) 23.6, 25.6, 2048 x 4096 x 512 27.6, 25.6, 2772 x 4091 x 288 (rows at any address) 45, 59.
+  // Single SMs or pairs, us each, by (rows per expert; experts), matrices from HBM. 16 bits, gate and up, hidden 2048, ffn 768: 81, 80
+  // (1; 128), 132, 129 (32; 128), 134, 131 (32, Zipf; 128), 187, 146 (128; 128), 336, 205 (256; 128); hidden 1024, ffn 512: 15.3, 15.4
+  // (1; 32), 17.4, 17.6 (32; 32), 19.3, 18.4 (64; 32) -- pairs where the buckets fill them or the tiles take four rounds of pairs anyway.
+  // e4m3, whose pairs always multiply 256 rows and whose stores no product overlaps: 49, 85 (1; 128), 77, 130 (32; 128), 95, 139 (64;
+  // 128), 149, 133 (128; 128), 282, 191 (256; 128), down 104, 97 (128; 128); dense with its rows' quantiser, rows x outputs x K:
+  // 4096 x 4096 x 4096 155, 99, 1024 x 4096 x 1024 (64 tiles of pairs) 18.1, 14.8, 1024 x 2048 x 2048 (32 tiles) 17.5, 18.7,
+  // 2048 x 4096 x 512 21.4, 17.2, 2772 x 4091 x 288 (outputs at any address) 38, 49.
   const int64_t pair_tiles = most_tiles<Shape<FP8, GATEUP, kPair>>(p), round = sm_count() / 2;
   bool pairs = FP8 ? p.n_pairs >= 128 * experts && nslab >= 4 && 4 * pair_tiles >= 3 * round : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
   if (g_form) pairs = g_form == 2;
