@@ -339,7 +339,7 @@ class MoeBlock:
                 not workspace.is_contiguous():
             raise ValueError(f"workspace of {need} contiguous uint8 values on the block's device, 256-byte aligned, needed")
         self.workspace = workspace
-        self._status = torch.zeros(1, dtype=torch.int32, device=bank.gate.device)   # this block's own, whoever shares the workspace
+        self._status = torch.empty(1, dtype=torch.int32, device=bank.gate.device)   # of this block alone; a launch clears it
         self._last = None
 
     def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:
