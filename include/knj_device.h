@@ -75,6 +75,9 @@ extern "C" {
 /* 8-bit codes with f32 scales beside them: rows one scale for each 128 values ([rows][ceil(K/128)]), matrices one for each
  * block of 128 x 128 ([ceil(N/128)][ceil(K/128)]). Where an entry point does not name it, the three above are taken. */
 #define KNJ_DT_E4M3 3
+/* signed 8-bit codes with f32 scales beside them: rows one scale each, matrices one for each output channel ([N]) */
+#define KNJ_DT_I8 5
+#define KNJ_INT8_MAX_K 131072 /* sums of this many products of codes could pass 32 bits */
 
 typedef void *knj_stream_t; /* a cudaStream_t */
 typedef void *knj_event_t;  /* a cudaEvent_t */
@@ -481,6 +484,12 @@ void knj_moe_stack_destroy(knj_moe_stack *st);
  * x [rows][K] f32 / bf16 / f16 with row stride ldx; q dense [rows][K]; scale [rows][ceil(K/128)]. */
 int knj_fp8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K, void *q, float *scale, knj_stream_t s);
 
+/* Rows as int8 codes with one scale each, in f32: scale = most * f32(1/127) with `most` the row's largest magnitude, code = the whole
+ * number nearest to v * (1 / scale), ties to even, in [-127, 127]. A row with most < 2^-100 is stored as zeros under scale 0; a NaN
+ * or an infinity in a row becomes its scale over codes of zero, and products of the row are NaN. x [rows][K] f32 / bf16 / f16 with row
+ * stride ldx; q dense [rows][K]; scale [rows]. */
+int knj_int8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K, void *q, float *scale, knj_stream_t s);
+
 /* What stands between two blocks of a residual stream, in one launch (rmsnorm_rows and the residual add of
  * src/model/model.cpp:258-271, :652 are its simplest cases). Per row, in f32:
  *   n = y * rsqrt(mean(y^2) + eps) * post_w   (post_w NULL: n = y)
@@ -527,9 +536,10 @@ void knj_block_norm_test_stall(int on);
  * names are left as they were; each value of one that several experts name is the product with one of them):
  *   knj_expert_gateup_launch: out[p][n] = out_scale * silu(x[row(p)] . w0[e][n]) * (x[row(p)] . w1[e][n])
  *   knj_expert_proj_launch:   out[p][n] = out_scale * (x[row(p)] . w0[e][n])
- * w0, w1 dense [n_experts][N][K] in bf16, f16 or e4m3 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
+ * w0, w1 dense [n_experts][N][K] in bf16, f16, e4m3 or int8 (w_dtype), x in the same type; row(p) = row_map[p] when given, else
  * p / row_div. e4m3: x_scale [n_rows][ceil(K/128)], w*_scale [n_experts][ceil(N/128)][ceil(K/128)]; the sum over each 128
- * values of K is scaled and added in f32. silu takes the fast exponential and division: its relative error reaches
+ * values of K is scaled and added in f32. int8: x_scale [n_rows], w*_scale [n_experts][N], K below KNJ_INT8_MAX_K; the sum over all
+ * of K is formed in whole numbers and then multiplied, as f32, with (row's scale * channel's scale). silu takes the fast exponential and division: its relative error reaches
  * 2^-21 (1 + |gate| / 3), which f32 outputs show, and gates below -87 give 0. N is any number, n_rows >= 1, K and ldx are whole 16-byte units, bases are 16-byte aligned.
  * out f32, bf16 or f16 [n_pairs][N], row stride ldo. Table entries outside [0, n_pairs) are skipped, rows outside
  * [0, n_rows) read as zeros. out overlaps no operand; n_pairs and idx_stride are at most 2^30. status (optional device int, zeroed by the caller) is set to 1 when a bounded wait gave up;
@@ -551,7 +561,7 @@ typedef struct knj_expert_gemm_args {
 } knj_expert_gemm_args;
 int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
-/* 1 = these products (and the dense e4m3 one) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
+/* 1 = these products (and the dense e4m3 and int8 ones) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
  * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes.
  * Process-wide. */
 void knj_expert_tc_form(int form);
@@ -568,10 +578,19 @@ size_t knj_fp8_matmul_workspace_bytes(int m, int n_in);
 int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, int64_t ldx, int m, void *y,
                           int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);
 
-/* A whole MoE block of a residual stream with experts in bf16, fp16 or e4m3 (Model::moe between rmsnorm_rows and the
+/* Dense product with an int8 matrix: y[m][n_out] = f32(sum_k x[m][k] W[n_out][k]) * (x_scale[m] * W_scale[n_out]), W int8
+ * [n_out][n_in], W_scale f32 [n_out], the sums exact in 32-bit whole numbers. Rows of x in f32, bf16 or f16 (x_scale not read) are
+ * turned into codes first, as knj_int8_rows_launch does, in the workspace (256-byte aligned); int8 rows (16-byte units) come with
+ * their x_scale [m] and need no workspace. n_in a multiple of 16 below KNJ_INT8_MAX_K. y f32, bf16 or f16. status as in
+ * knj_expert_gemm_args. The reference's int8 product (kernels/knj_kernels.hip:132-318 knj_gemm_w4_i8) has 4-bit weights. */
+size_t knj_int8_matmul_workspace_bytes(int m, int n_in);
+int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, const float *x_scale, int64_t ldx,
+                           int m, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);
+
+/* A whole MoE block of a residual stream with experts in bf16, fp16, e4m3 or int8 (Model::moe between rmsnorm_rows and the
  * residual add, src/model/model.cpp:631-652, with what a block may have around it):
- *   h   = norm(x; pre_w)                           rows in the experts' 16-bit type (bf16 for e4m3 experts, which read their
- *                                                  e4m3 codes)
+ *   h   = norm(x; pre_w)                           rows in the experts' 16-bit type (bf16 for e4m3 and int8 experts, which read
+ *                                                  the rows' codes)
  *   y   = sum over the top_k experts of softmax weight * down(silu(gate(h)) * up(h))
  *   out = beta * x + alpha * g * norm(y; post_w)   and, for the next block, h_next = norm(out; next_w)
  * as the launches above chained on one stream: block norm, router and tables, expert products, ordered combine, block norm.
@@ -594,7 +613,7 @@ typedef struct knj_moe_block_args {
   const float *router_bias;  /* f32 [n_experts] or NULL */
   const void *w_gate, *w_up; /* [n_experts][ffn][hidden] */
   const void *w_down;        /* [n_experts][hidden][ffn] */
-  const float *gate_scale, *up_scale, *down_scale; /* e4m3 */
+  const float *gate_scale, *up_scale, *down_scale; /* e4m3: of blocks; int8: [n_experts][rows of the matrix] */
   void *h_next;
   int64_t ld_h_next;
   float *h_next_scale;

@@ -14,7 +14,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 # KNJ_DEVICE_LIB points at another build of the same library (e.g. a measurement build); default: the in-tree one
 LIB_PATH = os.environ.get("KNJ_DEVICE_LIB") or os.path.join(PKG, "libknj_device.so")
 
-DT_F32, DT_BF16, DT_F16, DT_E4M3 = 0, 1, 2, 3
+DT_F32, DT_BF16, DT_F16, DT_E4M3, DT_I8 = 0, 1, 2, 3, 5
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3  # KNJ_GATE_*
 EP_FLAG_WORDS, EP_MAX_CHUNKS = 4096, 8  # KNJ_EP_FLAG_WORDS, KNJ_EP_MAX_CHUNKS
 
@@ -214,6 +214,9 @@ SIGNATURES = {
     "knj_q4k_matmul_noalloc_max_scratch": (_sz, []),
     "knj_q4k_matmul_noalloc_launch": (_i, [_vp, _i, _i, _vp, _i, _i64, _i, _vp, _i64, _vp]),
     "knj_fp8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
+    "knj_int8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
+    "knj_int8_matmul_workspace_bytes": (_sz, [_i, _i]),
+    "knj_int8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),
     # a BlockNormArgs or ExpertGemmArgs by reference, or its bytes (packed)
     "knj_block_norm_launch": (_i, [_vp, _vp]),
     "knj_block_norm_test_stall": (None, [_i]),

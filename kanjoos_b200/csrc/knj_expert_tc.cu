@@ -1,8 +1,10 @@
-// knj_expert_tc.cu -- products of routed rows with expert matrices held in bf16, fp16 or e4m3 (one scale for each block of
-// 128 x 128), grouped by expert, and the dense e4m3 product, which is the same with one expert and all rows.
+// knj_expert_tc.cu -- products of routed rows with expert matrices held in bf16, fp16, e4m3 (one scale for each block of
+// 128 x 128) or int8 (one for each row), grouped by expert, and the dense e4m3 and int8 products, which are the same with one expert
+// and all rows.
 //
 //   out[p][n] = out_scale * x[row(p)] . w[e][n]     and     out_scale * silu(x . wg[e][n]) * (x . wu[e][n])
 //   e4m3:  x . w = sum over blocks b of 128 k:  sx[row][b] * sw[n/128][b] * sum_{k in b} qx[k] qw[k]
+//   int8:  x . w = sx[row] * sw[n] * sum_k qx[k] qw[k], the sum in 32-bit whole numbers: exact, and the same in every order
 //
 // Few rows are bound by the matrices' bytes: every active expert's matrix is read once (512 rows x 8 of 128 experts, bf16: 806 MB, 131 us,
 // 0.94 of the measured copy rate). Many rows are bound by the tensor core: 16384 rows, bf16, 1.38 PFLOP/s alone, 1.13 in a loop under
@@ -16,9 +18,11 @@
 //   matrix     TMA boxes of 128 bytes of K: 128 rows, or for gate and up eight boxes of 16 rows in turn -- gate and up of one output
 //              then lie 16 lanes apart in one warp and meet by a shuffle
 //   rows       tile::gather4 TMA copies of four routed rows each; boxes where the rows are all rows in order
-//   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies; 16 bits: finds
-//              the tiles and their rows in the tables, a tile ahead (in e4m3 the matrix warp does)
-// In 16 bits the tensor core adds over all of K. In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
+//   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies; 16 bits and int8:
+//              finds the tiles and their rows (and the rows' scales) in the tables, a tile ahead (in e4m3 the matrix warp does)
+// In 16 bits and int8 the tensor core adds over all of K. int8 leaves the 16-bit form as it is, but that a slab holds twice the K and
+// the epilogue turns sums into f32 and scales them: 8192 x 4096 x 4096 84 us alone (3.3 P operations a second; the
+// library's product of 8192^3 reaches 2.95). In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
 // adds to its registers in f32 while the tensor core fills the others.
 //
 // Every wait on an mbarrier is bounded (knj_decode_wait_limit); on give-up the kernel raises a status flag, stores NaN in place of the
@@ -63,8 +67,10 @@ thread_local int t_stall = 0;
 enum Form { kSingle = 0, kPair = 1, kSplit = 2 };
 constexpr int kMaxParts = 4;
 
-template <bool FP8, bool GATEUP, int FORM>
+template <Operand KIND, bool GATEUP, int FORM>
 struct Shape {
+  static constexpr bool FP8 = KIND == kE4M3, I8 = KIND == kI8;
+  static constexpr int kElem = KIND == k16 ? 2 : 1;      // bytes of an element
   static constexpr int CG = FORM == kPair ? 2 : 1;
   // e4m3 in pairs: the MMA's M side is the routed rows and its N side 256 matrix rows (of them 128 of gate and 128 of up)
   static constexpr bool kRowsM = FP8 && CG == 2;
@@ -80,7 +86,7 @@ struct Shape {
   static constexpr int kStages = FORM == kPair ? 6 / kSub : FORM == kSplit ? 5 : 4;
   static constexpr int kATile = 128 * 128;               // bytes: 128 matrix rows x 128 bytes of K
   static constexpr int kBTile = kTok / CG * 128;
-  static constexpr int kSlab = FP8 ? 128 : 64;           // elements of K per slab
+  static constexpr int kSlab = 128 / kElem;              // elements of K per slab
   static constexpr int kOuts = GATEUP ? 64 : 128;        // outputs per CTA and tile (of a pair: kOuts * CG)
   static constexpr int kBoxRows = GATEUP && !kRowsM ? 16 : 128;
   static constexpr int kVecs = GATEUP || kRowsM ? 2 : 1; // matrix scales per block of K: gate and up, or two blocks of 128 outputs
@@ -98,7 +104,8 @@ struct Shape {
   static constexpr int kOffPairs = kOffStage + kEpiWarps * kStage;    // [kTiles][kTok] pair of each column
   static constexpr int kTiles = 3;                       // ring of tile descriptions
   static constexpr int kOffRows = kOffPairs + kTiles * kTok * 4;            // [kTiles][kTok] row of each column
-  static constexpr int kOffTile = kOffRows + kTiles * kTok * 4;             // [kTiles] Tile
+  static constexpr int kOffRowScale = kOffRows + kTiles * kTok * 4;         // int8: [kTiles][kTok] scale of each column's row
+  static constexpr int kOffTile = kOffRowScale + (I8 ? kTiles * kTok * 4 : 0);   // [kTiles] Tile
   static constexpr int kOffPref = kOffTile + kTiles * 16;                   // [E + 1] buckets before expert e, [E] pairs of it
   static constexpr int kOffBars = kOffPref + (2 * kMaxExperts + 4) * 4;
   static constexpr int kBytes = kOffBars + 320 + 1024;
@@ -196,11 +203,12 @@ __device__ __noinline__ void store_rows_any(void *out, int dtype, int64_t ldo, i
     if (q[i] != -1) store_from_f32(out, dtype, (q[i] < 0 ? -2 - q[i] : q[i]) * ldo + n + j, v[i]);
 }
 
-template <bool FP8, bool GATEUP, int FORM>
-__global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8, GATEUP, FORM>::kBlocksPerSm)
+template <Operand KIND, bool GATEUP, int FORM>
+__global__ void __launch_bounds__(Shape<KIND, GATEUP, FORM>::kThreads, Shape<KIND, GATEUP, FORM>::kBlocksPerSm)
     expert_tc_kernel(const __grid_constant__ GemmParams p) {
-  using S = Shape<FP8, GATEUP, FORM>;
+  using S = Shape<KIND, GATEUP, FORM>;
   constexpr int CG = S::CG;
+  constexpr bool FP8 = S::FP8, I8 = S::I8;
   constexpr bool SPLIT = FORM == kSplit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -222,6 +230,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
   volatile int *s_fail = reinterpret_cast<volatile int *>(tmem_slot + 1);  // raised by the first wait that gives up
   int32_t *s_pair = reinterpret_cast<int32_t *>(smem + S::kOffPairs);
   int32_t *s_row = reinterpret_cast<int32_t *>(smem + S::kOffRows);
+  [[maybe_unused]] float *s_row_scale = reinterpret_cast<float *>(smem + S::kOffRowScale);
   int4 *s_tile = reinterpret_cast<int4 *>(smem + S::kOffTile);
   int32_t *s_pref = reinterpret_cast<int32_t *>(smem + S::kOffPref), *s_cnt = s_pref + kMaxExperts + 1;
 
@@ -263,7 +272,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
     // latencies of HBM. A line that an earlier launch still writes is brought there for it.
     if (tid < 8 && 32 * tid < p.E && p.pair_idx) l2_line(p.pair_cnt + 32 * tid);
     if (tid < p.E && p.pair_idx) l2_line(p.pair_idx + tid * p.idx_stride);
-    const int per = (p.K * (FP8 ? 1 : 2) + 127) / 128, line = blockIdx.x * S::kThreads + tid, row = line / per;
+    const int per = (p.K * S::kElem + 127) / 128, line = blockIdx.x * S::kThreads + tid, row = line / per;
     if (row < p.n_rows) l2_line(p.x + row * p.x_row + (line - row * per) * 128);
   }
   grid_dep_wait();  // the tables and the rows come from earlier launches
@@ -417,9 +426,15 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         }
       }
     }
+    [[maybe_unused]] float scale[kPairs];
+    if constexpr (I8) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) scale[j] = pr[j] >= 0 ? __ldcg(p.xs + row[j]) : 0.f;
+    }
     if (!wait(&tile_empty[fslot], fpar)) return;
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) {
+      if constexpr (I8) s_row_scale[fslot * S::kTok + lane + 32 * j] = scale[j];
       s_pair[fslot * S::kTok + lane + 32 * j] = pr[j];
       s_row[fslot * S::kTok + lane + 32 * j] = row[j];
     }
@@ -505,11 +520,35 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
           }
         }
       };
+      // int8: scales of the matrix rows whose sums this thread holds -- of each 16 the rows t/4 and t/4 + 8, of gate and of up or of
+      // both halves; read while the products are under way. Behind the last output any will do.
+      [[maybe_unused]] float ws[2][2];
+      if constexpr (I8) {
+        const int64_t at = (int64_t)tl.e * p.N;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr)
+            ws[h][rr] = (GATEUP && h ? p.ws1 : p.ws0)[at + min(n0 + (lane >> 2) + 8 * rr + (GATEUP ? 0 : 16 * h), p.N - 1)];
+      }
       auto finish = [&](const uint32_t (&lo)[8], const uint32_t (&hi)[8], int c0) {
         float v[2][8];
+        [[maybe_unused]] float xs[2][2];   // int8: scales of the columns' rows
+        if constexpr (I8) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 f = *reinterpret_cast<const float2 *>(s_row_scale + tslot * S::kTok + c0 + 8 * i + 2 * (lane & 3));
+            xs[i][0] = f.x;
+            xs[i][1] = f.y;
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float a = __uint_as_float(lo[j]), b = __uint_as_float(hi[j]);
+          float a = __uint_as_float(lo[j]), b = __uint_as_float(hi[j]);
+          if constexpr (I8) {
+            a = __int2float_rn((int)lo[j]) * (xs[j >> 2][j & 1] * ws[0][j >> 1 & 1]);
+            b = __int2float_rn((int)hi[j]) * (xs[j >> 2][j & 1] * ws[1][j >> 1 & 1]);
+          }
           v[0][j] = (GATEUP ? __fdividef(a, 1.0f + __expf(-a)) * b : a) * p.out_scale;
           v[1][j] = b * p.out_scale;
         }
@@ -548,12 +587,11 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
         for (int from = 1; from < parts; ++from)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float4 f = *reinterpret_cast<const float4 *>(smem + part_at(from, c, i));
+            const uint4 f = *reinterpret_cast<const uint4 *>(smem + part_at(from, c, i));
+            const uint32_t add[4] = {f.x, f.y, f.z, f.w};
             uint32_t *v = i < 2 ? lo + 4 * i : hi + 4 * (i - 2);
-            v[0] = __float_as_uint(__uint_as_float(v[0]) + f.x);
-            v[1] = __float_as_uint(__uint_as_float(v[1]) + f.y);
-            v[2] = __float_as_uint(__uint_as_float(v[2]) + f.z);
-            v[3] = __float_as_uint(__uint_as_float(v[3]) + f.w);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = I8 ? v[q] + add[q] : __float_as_uint(__uint_as_float(v[q]) + __uint_as_float(add[q]));
           }
       };
       // every thread of the warp: meets sync `i` of the tile; after the second, whether all parts are there
@@ -838,7 +876,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
       for (; t < n_tiles; tile_done(), split_end(t), t += step) {
         Tile tl;
         if (!tile_take(tl)) break;
-        const uint32_t idesc = instr_desc_f16(128 * CG, S::kRowsM ? 128 : tl.ncol) | p.idesc_format;
+        const uint32_t idesc = I8 ? instr_desc_i8(128 * CG, tl.ncol) : instr_desc_f16(128 * CG, S::kRowsM ? 128 : tl.ncol) | p.idesc_format;
         for (int ks = k_lo; ks < k_hi; ks += S::kSub) {
           if (!S::kRowsM && (FP8 || ks == k_lo) && !wait(&acc_empty[buf], acc_par)) break;
           if (!wait(&full[st], par)) break;
@@ -858,7 +896,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
               tc_fence_after();
               if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma<FP8, CG>(tmem_base + buf * S::kAccCols, rows + 2 * k, mat + h * 512 + 2 * k, idesc, k > 0 ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) tc_mma<KIND, CG>(tmem_base + buf * S::kAccCols, rows + 2 * k, mat + h * 512 + 2 * k, idesc, k > 0 ? 1u : 0u);
                 commit(&acc_full[buf]);
                 if (h == 1) commit(&empty[st]);
               }
@@ -874,7 +912,7 @@ __global__ void __launch_bounds__(Shape<FP8, GATEUP, FORM>::kThreads, Shape<FP8,
                 if (u > 0 && ks + u >= k_hi) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  tc_mma<FP8, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
+                  tc_mma<KIND, CG>(tmem_base + buf * S::kAccCols, mat + u * (S::kATile / 16) + 2 * k, rows + u * (S::kBTile / 16) + 2 * k, idesc,
                                (u > 0 || k > 0 || (!FP8 && ks > k_lo)) ? 1u : 0u);
               }
               commit(&empty[st]);
@@ -1081,7 +1119,7 @@ int g_form = 0;  // 0 = by the rule below, 1 = single SMs, 2 = pairs, 3 = K spli
 struct Operands {
   const void *x, *w0, *w1;
   int64_t ldx;
-  bool fp8;
+  Operand kind;
 };
 
 // the tiles that these pairs can make; a table that names pairs more than once makes more, which the same grid walks over
@@ -1091,19 +1129,19 @@ int64_t most_tiles(const GemmParams &p) {
   return buckets * ((p.N + rows - 1) / rows);
 }
 
-template <bool FP8, bool GATEUP, int FORM>
+template <Operand KIND, bool GATEUP, int FORM>
 int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
-  using S = Shape<FP8, GATEUP, FORM>;
+  using S = Shape<KIND, GATEUP, FORM>;
   constexpr int CG = S::CG;
   int dev = 0;
   KNJ_CUDA(cudaGetDevice(&dev));
-  auto kern = expert_tc_kernel<FP8, GATEUP, FORM>;
+  auto kern = expert_tc_kernel<KIND, GATEUP, FORM>;
   static bool opted[64] = {false};
   if (dev >= 0 && dev < 64 && !opted[dev]) {
     KNJ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     opted[dev] = true;
   }
-  constexpr int esz = FP8 ? 1 : 2;
+  constexpr int esz = S::kElem;
   const uint64_t w_rows = (uint64_t)p.E * p.N;
   int rc = make_operand_tensor_map(&p.map0, o.w0, esz, p.K, p.K, w_rows, S::kBoxRows);
   if (!rc && GATEUP) rc = make_operand_tensor_map(&p.map1, o.w1, esz, p.K, p.K, w_rows, S::kBoxRows);
@@ -1137,20 +1175,21 @@ int launch_form(GemmParams p, const Operands &o, cudaStream_t st) {
   return launch_status("expert_tc_kernel");
 }
 
-template <bool FP8, bool GATEUP>
+template <Operand KIND, bool GATEUP>
 int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   const int64_t experts = p.E < p.n_pairs ? p.E : p.n_pairs;
-  const int nslab = (p.K + Shape<FP8, GATEUP, kSplit>::kSlab - 1) / Shape<FP8, GATEUP, kSplit>::kSlab;
+  constexpr bool FP8 = KIND == kE4M3;
+  const int nslab = (p.K + Shape<KIND, GATEUP, kSplit>::kSlab - 1) / Shape<KIND, GATEUP, kSplit>::kSlab;
   // K is split where even the smallest tiles leave half of the CTAs' places free, into parts of two slabs or more: one row times
   // 4096 x 4096 e4m3, rows in 16 bits, 15.1 -> 9.7 us, 64 rows 19.1 -> 13.0 (parts of one slab, K = 512, cost 2 us more than none). Clusters of two and
   // four fill a GPC's SMs; of clusters of three, 96 did not fit at once (22.6 us where two took 16.4).
-  const int64_t places = 2ll * sm_count() / most_tiles<Shape<FP8, GATEUP, kSplit>>(p);
+  const int64_t places = 2ll * sm_count() / most_tiles<Shape<KIND, GATEUP, kSplit>>(p);
   int bits = places >= kMaxParts ? 2 : places >= 2 ? 1 : 0;
   while (bits > 0 && (2 << bits) > nslab) --bits;
   p.part_bits = 0;
   if (g_form == 3 || (g_form == 0 && bits > 0)) {
     p.part_bits = bits;
-    return launch_form<FP8, GATEUP, kSplit>(p, o, st);
+    return launch_form<KIND, GATEUP, kSplit>(p, o, st);
   }
   // Single SMs or pairs, us each, by (rows per expert; experts), matrices from HBM. 16 bits, gate and up, hidden 2048, ffn 768: 81, 80
   // (1; 128), 132, 129 (32; 128), 134, 131 (32, Zipf; 128), 187, 146 (128; 128), 336, 205 (256; 128); hidden 1024, ffn 512: 15.3, 15.4
@@ -1159,14 +1198,22 @@ int launch_rule(GemmParams p, const Operands &o, cudaStream_t st) {
   // 128), 149, 133 (128; 128), 282, 191 (256; 128), down 104, 97 (128; 128); dense with its rows' quantiser, rows x outputs x K:
   // 4096 x 4096 x 4096 155, 99, 1024 x 4096 x 1024 (64 tiles of pairs) 18.1, 14.8, 1024 x 2048 x 2048 (32 tiles) 17.5, 18.7,
   // 2048 x 4096 x 512 21.4, 17.2, 2772 x 4091 x 288 (outputs at any address) 38, 49.
-  const int64_t pair_tiles = most_tiles<Shape<FP8, GATEUP, kPair>>(p), round = sm_count() / 2;
-  bool pairs = FP8 ? p.n_pairs >= 128 * experts && nslab >= 4 && 4 * pair_tiles >= 3 * round : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
+  // int8 (rows as codes, L2 flushed, events' 5 us included): gate and up 86, 85 (4; 128), 87, 86 (16), 88, 86 (32), 88, 88 (64), 106, 91 (128), 172,
+  // 111 (256); down 54, 61 (4; 128), 53, 54 (16), 54, 54 (32), 60, 57 (64), 77, 72 (128); dense 512 x 4096 x 4096 (32 tiles of pairs) 22.5, 24.7,
+  // 1024 x 4096 x 1024 (64 tiles) 17.2, 16.6, 2048 x 4096 x 512 20.3, 19.5, 4096 x 4096 x 4096 83, 57, 2772 x 4091 x 288 34, 42.
+  const int64_t pair_tiles = most_tiles<Shape<KIND, GATEUP, kPair>>(p), round = sm_count() / 2;
+  bool pairs = KIND != k16 ? p.n_pairs >= (FP8 ? 128 : 64) * experts && nslab >= 4 && 4 * pair_tiles >= 3 * round
+                           : p.n_pairs > 32 * experts || pair_tiles >= 4 * round;
   if (g_form) pairs = g_form == 2;
-  return pairs ? launch_form<FP8, GATEUP, kPair>(p, o, st) : launch_form<FP8, GATEUP, kSingle>(p, o, st);
+  return pairs ? launch_form<KIND, GATEUP, kPair>(p, o, st) : launch_form<KIND, GATEUP, kSingle>(p, o, st);
 }
 template <bool GATEUP>
 int launch_gemm(const GemmParams &p, const Operands &o, cudaStream_t st) {
-  return o.fp8 ? launch_rule<true, GATEUP>(p, o, st) : launch_rule<false, GATEUP>(p, o, st);
+  switch (o.kind) {
+    case kE4M3: return launch_rule<kE4M3, GATEUP>(p, o, st);
+    case kI8: return launch_rule<kI8, GATEUP>(p, o, st);
+    default: return launch_rule<k16, GATEUP>(p, o, st);
+  }
 }
 
 }  // namespace
@@ -1178,11 +1225,13 @@ int expert_product_check(const knj_expert_gemm_args *a, bool gateup, const char 
   if (a->n_pairs == 0) return KNJ_OK;
   KNJ_REQUIRE(a->n_pairs <= kMaxPairs && a->idx_stride <= kMaxPairs, "%s: tables of more than 2^30 pairs", who);
   KNJ_REQUIRE(a->n_rows >= 1, "%s: pairs without a row of x", who);
-  KNJ_REQUIRE(a->w_dtype >= KNJ_DT_BF16 && a->w_dtype <= KNJ_DT_E4M3, "%s: expert matrices are bf16, f16 or e4m3", who);
+  const bool codes = a->w_dtype == KNJ_DT_E4M3 || a->w_dtype == KNJ_DT_I8;
+  KNJ_REQUIRE(codes || a->w_dtype == KNJ_DT_BF16 || a->w_dtype == KNJ_DT_F16, "%s: expert matrices are int8, bf16, f16 or e4m3", who);
   KNJ_REQUIRE(a->x_dtype == a->w_dtype, "%s: rows (type %d) and matrices (type %d) are of one type", who, a->x_dtype, a->w_dtype);
   KNJ_REQUIRE(a->x && a->w0 && (!gateup || a->w1) && a->pair_idx && a->pair_cnt && a->out, "%s: null pointer", who);
-  KNJ_REQUIRE(a->w_dtype != KNJ_DT_E4M3 || (a->x_scale && a->w0_scale && (!gateup || a->w1_scale)), "%s: e4m3 operands need their scales", who);
-  const int64_t esz = a->w_dtype == KNJ_DT_E4M3 ? 1 : 2;
+  KNJ_REQUIRE(!codes || (a->x_scale && a->w0_scale && (!gateup || a->w1_scale)), "%s: e4m3 and int8 operands need their scales", who);
+  KNJ_REQUIRE(a->w_dtype != KNJ_DT_I8 || a->K < KNJ_INT8_MAX_K, "%s: sums of K=%d products of int8 codes may pass 32 bits", who, a->K);
+  const int64_t esz = codes ? 1 : 2;
   KNJ_REQUIRE(a->K * esz % 16 == 0 && a->ldx * esz % 16 == 0, "%s: rows of K=%d and stride %lld are not whole 16-byte units", who, a->K,
               (long long)a->ldx);
   KNJ_REQUIRE(aligned16(a->x) && aligned16(a->w0) && (!gateup || aligned16(a->w1)), "%s: bases must be 16-byte aligned", who);
@@ -1203,8 +1252,9 @@ int run_expert(const knj_expert_gemm_args *a, bool gateup, const char *who, knj_
   p.out = a->out; p.status = a->status; p.ldo = a->ldo; p.idx_stride = a->idx_stride; p.out_dtype = a->out_dtype; p.N = a->N; p.K = a->K;
   p.E = a->n_experts; p.row_div = a->row_div > 0 ? a->row_div : 1; p.n_rows = a->n_rows; p.n_pairs = a->n_pairs; p.out_scale = a->out_scale;
   p.idesc_format = a->w_dtype == KNJ_DT_BF16 ? (1u << 7) | (1u << 10) : 0u;
-  p.x = static_cast<const uint8_t *>(a->x); p.x_row = a->ldx * (a->w_dtype == KNJ_DT_E4M3 ? 1 : 2);
-  const Operands o{a->x, a->w0, a->w1, a->ldx, a->w_dtype == KNJ_DT_E4M3};
+  const Operand kind = a->w_dtype == KNJ_DT_E4M3 ? kE4M3 : a->w_dtype == KNJ_DT_I8 ? kI8 : k16;
+  p.x = static_cast<const uint8_t *>(a->x); p.x_row = a->ldx * (kind == k16 ? 2 : 1);
+  const Operands o{a->x, a->w0, a->w1, a->ldx, kind};
   return gateup ? launch_gemm<true>(p, o, as_stream(s)) : launch_gemm<false>(p, o, as_stream(s));
 }
 
@@ -1251,7 +1301,45 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
   GemmParams p{};
   p.x = q; p.x_row = n_in; p.xs = qs; p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
   p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f; p.dense = 1;
-  return launch_gemm<false>(p, Operands{q, W, nullptr, n_in, true}, as_stream(s));
+  return launch_gemm<false>(p, Operands{q, W, nullptr, n_in, kE4M3}, as_stream(s));
+}
+
+size_t knj_int8_matmul_workspace_bytes(int m, int n_in) {
+  if (m <= 0 || n_in <= 0) return 0;
+  return up256((size_t)m * n_in) + up256((size_t)m * 4);
+}
+
+int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, const float *x_scale, int64_t ldx,
+                           int m, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s) {
+  KNJ_REQUIRE(m >= 0 && n_in > 0 && n_out > 0, "knj_int8_matmul: bad sizes");
+  if (m == 0) return KNJ_OK;
+  const bool codes = x_dtype == KNJ_DT_I8;
+  KNJ_REQUIRE(W && W_scale && x && y && (!codes || x_scale), "knj_int8_matmul: null pointer");
+  KNJ_REQUIRE(m <= kMaxPairs, "knj_int8_matmul: more than 2^30 rows");
+  KNJ_REQUIRE(n_in % 16 == 0 && n_in < KNJ_INT8_MAX_K, "knj_int8_matmul: n_in=%d must be a multiple of 16 below %d", n_in, KNJ_INT8_MAX_K);
+  KNJ_REQUIRE(aligned16(W), "knj_int8_matmul: the matrix must be 16-byte aligned");
+  KNJ_REQUIRE(codes || (x_dtype >= KNJ_DT_F32 && x_dtype <= KNJ_DT_F16), "knj_int8_matmul: rows are f32, bf16, f16 or int8");
+  KNJ_REQUIRE(!codes || (aligned16(x) && ldx % 16 == 0), "knj_int8_matmul: int8 rows and their stride are whole 16-byte units");
+  KNJ_REQUIRE(y_dtype >= KNJ_DT_F32 && y_dtype <= KNJ_DT_F16, "knj_int8_matmul: outputs are f32, bf16 or f16");
+  KNJ_REQUIRE(ldx >= n_in && ldy >= n_out, "knj_int8_matmul: row strides shorter than the rows");
+  GemmParams p{};
+  p.x = static_cast<const uint8_t *>(x); p.x_row = ldx; p.xs = x_scale;
+  if (!codes) {
+    const size_t need = knj_int8_matmul_workspace_bytes(m, n_in);
+    if (!workspace || workspace_bytes < need) {
+      set_error("knj_int8_matmul: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+      return KNJ_E_WORKSPACE;
+    }
+    KNJ_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "knj_int8_matmul: workspace must be 256-byte aligned");
+    uint8_t *q = static_cast<uint8_t *>(workspace);
+    float *qs = reinterpret_cast<float *>(q + up256((size_t)m * n_in));
+    const int rc = knj_int8_rows_launch(x, x_dtype, ldx, m, n_in, q, qs, s);
+    if (rc) return rc;
+    p.x = q; p.x_row = n_in; p.xs = qs;
+  }
+  p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
+  p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f; p.dense = 1;
+  return launch_gemm<false>(p, Operands{p.x, W, nullptr, p.x_row, kI8}, as_stream(s));
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// knj_moe_block.cu -- a whole MoE block with experts in bf16, fp16 or e4m3 as one C-ABI call: the stage sequence of the CPU
+// knj_moe_block.cu -- a whole MoE block with experts in bf16, fp16, e4m3 or int8 as one C-ABI call: the stage sequence of the CPU
 // branch (src/model/model.cpp:631-652) with a norm, a gate and scales around the residual add, every intermediate in a
 // caller-provided workspace.
 #include "knj_common.cuh"
@@ -10,6 +10,12 @@ namespace {
 constexpr float kF16Prescale = 0.015625f;  // 2^-6: room for products of gate and up in fp16
 
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+inline bool has_codes(int w_dtype) { return w_dtype == KNJ_DT_E4M3 || w_dtype == KNJ_DT_I8; }
+// scales of a row of K codes
+inline size_t row_scales(int w_dtype, int K) { return w_dtype == KNJ_DT_E4M3 ? (K + 127) / 128 : 1; }
+int code_rows(int w_dtype, const void *x, int x_dtype, int rows, int K, void *q, float *scale, knj_stream_t s) {
+  return w_dtype == KNJ_DT_E4M3 ? knj_fp8_rows_launch(x, x_dtype, K, rows, K, q, scale, s) : knj_int8_rows_launch(x, x_dtype, K, rows, K, q, scale, s);
+}
 
 struct BlockWs {
   uint8_t *h, *hq, *act, *aq;
@@ -27,11 +33,11 @@ BlockWs carve(void *base, int T, int H, int F, int E, int k, int w_dtype) {
     return r;
   };
   const size_t P = (size_t)T * k;
-  const bool q = w_dtype == KNJ_DT_E4M3;
+  const bool q = has_codes(w_dtype);
   w.status = reinterpret_cast<int32_t *>(take(16));   // the first word, whatever the sizes
   w.h = take((size_t)T * H * 2);
   w.hq = q ? take((size_t)T * H) : nullptr;
-  w.hs = reinterpret_cast<float *>(q ? take((size_t)T * ((H + 127) / 128) * 4) : nullptr);
+  w.hs = reinterpret_cast<float *>(q ? take(T * row_scales(w_dtype, H) * 4) : nullptr);
   w.logits = reinterpret_cast<float *>(take((size_t)T * E * 4));
   w.pair_exp = reinterpret_cast<int32_t *>(take(P * 4));
   w.pair_w = reinterpret_cast<float *>(take(P * 4));
@@ -39,7 +45,7 @@ BlockWs carve(void *base, int T, int H, int F, int E, int k, int w_dtype) {
   w.pair_cnt = reinterpret_cast<int32_t *>(take((size_t)E * 4));
   w.act = take(P * F * 2);
   w.aq = q ? take(P * F) : nullptr;
-  w.as = reinterpret_cast<float *>(q ? take(P * ((F + 127) / 128) * 4) : nullptr);
+  w.as = reinterpret_cast<float *>(q ? take(P * row_scales(w_dtype, F) * 4) : nullptr);
   w.Y = reinterpret_cast<float *>(take(P * H * 4));
   w.sum = reinterpret_cast<float *>(take((size_t)T * H * 4));
   w.bytes = used;
@@ -61,9 +67,9 @@ int check(const knj_moe_block_args *a, const char *who) {
   KNJ_REQUIRE(a->hidden <= KNJ_BLOCK_NORM_MAX_HIDDEN, "%s: hidden=%d above %d", who, a->hidden, KNJ_BLOCK_NORM_MAX_HIDDEN);
   KNJ_REQUIRE(a->n_experts <= 256 && a->top_k >= 1 && a->top_k <= 8 && a->top_k <= a->n_experts, "%s: %d experts, top_k=%d out of range", who,
               a->n_experts, a->top_k);
-  KNJ_REQUIRE(a->w_dtype >= KNJ_DT_BF16 && a->w_dtype <= KNJ_DT_E4M3, "%s: experts are bf16, f16 or e4m3", who);
+  KNJ_REQUIRE(a->w_dtype == KNJ_DT_BF16 || a->w_dtype == KNJ_DT_F16 || has_codes(a->w_dtype), "%s: experts are int8, bf16, f16 or e4m3", who);
   KNJ_REQUIRE(a->x && a->out && a->w_router && a->w_gate && a->w_up && a->w_down, "%s: null tensor pointer", who);
-  KNJ_REQUIRE(a->w_dtype != KNJ_DT_E4M3 || (a->gate_scale && a->up_scale && a->down_scale), "%s: e4m3 experts need their scales", who);
+  KNJ_REQUIRE(!has_codes(a->w_dtype) || (a->gate_scale && a->up_scale && a->down_scale), "%s: e4m3 and int8 experts need their scales", who);
   KNJ_REQUIRE(aligned16(a->w_router), "%s: the router's weights must be 16-byte aligned", who);
   KNJ_REQUIRE((int64_t)a->n_tokens * a->top_k <= (1ll << 30), "%s: more than 2^30 pairs of a token and an expert", who);
   KNJ_REQUIRE((a->next_w != nullptr) == (a->h_next != nullptr), "%s: next_w and h_next go together", who);
@@ -89,7 +95,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   int rc = check(a, "knj_moe_block");
   if (rc || a->n_tokens == 0) return rc;
   const int T = a->n_tokens, H = a->hidden, F = a->ffn, E = a->n_experts, k = a->top_k, P = T * k;
-  const bool q = a->w_dtype == KNJ_DT_E4M3;
+  const bool q = has_codes(a->w_dtype);
   const int act = a->w_dtype == KNJ_DT_F16 ? KNJ_DT_F16 : KNJ_DT_BF16;   // 16-bit rows
   const BlockWs w = carve(a->workspace, T, H, F, E, k, a->w_dtype);
   int32_t *pair_exp = a->tap_pair_exp ? a->tap_pair_exp : w.pair_exp;
@@ -140,7 +146,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
     // long pair lists take the counting-sort form; its scratch is the activation buffer, which is written later
     rc = moe_permute_tables(pair_exp, P, E, T, w.pair_idx, w.pair_cnt, w.act, (size_t)P * F * 2, as_stream(s));
     if (rc) return rc;
-    if (q) rc = knj_fp8_rows_launch(w.h, act, H, T, H, w.hq, w.hs, s);
+    if (q) rc = code_rows(a->w_dtype, w.h, act, T, H, w.hq, w.hs, s);
     if (rc) return rc;
   }
   {
@@ -150,7 +156,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   }
   {
     StageSpan sp("moe-down", s);
-    if (q) rc = knj_fp8_rows_launch(w.act, act, F, P, F, w.aq, w.as, s);
+    if (q) rc = code_rows(a->w_dtype, w.act, act, P, F, w.aq, w.as, s);
     if (rc) return rc;
     rc = knj_expert_proj_launch(&down, s);
     if (rc) return rc;

@@ -177,16 +177,20 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :);
 }
-// D(tmem) (+)= A(smem desc) * B(smem desc), f16 / bf16 (by the instruction descriptor) or e4m3 operands, f32 accumulate, every
-// lane of D written: without the operands of the lane mask, which the issuing thread would have to bring into place each time
-template <bool FP8, int CG>
+// types of a product's operands: f16 / bf16 (by the instruction descriptor), e4m3, int8
+enum Operand { k16 = 0, kE4M3 = 1, kI8 = 2 };
+// D(tmem) (+)= A(smem desc) * B(smem desc), f32 sums (of int8 codes: s32), every lane of D written: without the operands of the
+// lane mask, which the issuing thread would have to bring into place each time
+template <Operand KIND, int CG>
 __device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
 #define KNJ_TC_MMA(GROUP, KIND)                                                                                                       \
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
                ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                                       \
                : "memory")
-  if constexpr (FP8 && CG == 1) KNJ_TC_MMA("1", "f8f6f4");
-  else if constexpr (FP8) KNJ_TC_MMA("2", "f8f6f4");
+  if constexpr (KIND == kE4M3 && CG == 1) KNJ_TC_MMA("1", "f8f6f4");
+  else if constexpr (KIND == kE4M3) KNJ_TC_MMA("2", "f8f6f4");
+  else if constexpr (KIND == kI8 && CG == 1) KNJ_TC_MMA("1", "i8");
+  else if constexpr (KIND == kI8) KNJ_TC_MMA("2", "i8");
   else if constexpr (CG == 1) KNJ_TC_MMA("1", "f16");
   else KNJ_TC_MMA("2", "f16");
 #undef KNJ_TC_MMA
@@ -217,6 +221,10 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr) {
 // fields (bits 7 and 10) are 0 for f16 and, in kind::f8f6f4, for e4m3; 1 for bf16.
 __device__ __forceinline__ uint32_t instr_desc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// kind::i8: D = s32 (2), A and B = signed 8 bits (1); n a multiple of 16, in a pair of 32
+__device__ __forceinline__ uint32_t instr_desc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 #endif

@@ -202,13 +202,16 @@ def float_layer_arrays(g: GgufFile, layer: int) -> dict:
     return out
 
 
-def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = False):
-    """`FloatExpertBank` of block `layer` (F16 or BF16 experts; e4m3=True turns them into e4m3 blocks) and the block's top-k. A
+def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = False, int8: bool = False):
+    """`FloatExpertBank` of block `layer` (F16 or BF16 experts; e4m3=True turns them into e4m3 blocks, int8=True into int8 codes with a
+    scale for each output channel) and the block's top-k. A
     `post_ffw_norm` tensor, where the file has one, becomes the norm behind the block. Norm weights are f32 with the file's values; the
     router is bf16, and the bank's `router_exact` is False where the file holds more bits: experts whose logits differ by less than
     that rounding may then be chosen in another order than from the file's values."""
     import torch
     from .moe import FloatExpertBank
+    if e4m3 and int8:
+        raise ValueError("e4m3 and int8 exclude one another")
     a = float_layer_arrays(g, layer)
 
     def bits(u16, dtype):
@@ -217,7 +220,7 @@ def load_float_expert_bank(g: GgufFile, layer: int, device="cuda", e4m3: bool = 
     norm = {k: torch.from_numpy(a[n]).to(device) if n in a else None for k, n in (("pre_norm", "norm"), ("post_norm", "post_norm"))}
     bank = FloatExpertBank(gate=bits(a["gate"], kind), up=bits(a["up"], kind), down=bits(a["down"], kind), router=bits(a["router"], torch.bfloat16),
                            router_exact=a["router_exact"], rms_eps=a["rms_eps"], **norm)
-    return (bank.to_e4m3() if e4m3 else bank), a["top_k"]
+    return (bank.to_e4m3() if e4m3 else bank.to_int8() if int8 else bank), a["top_k"]
 
 
 def verify_against_gguf_py(path: str, names=None) -> int:

@@ -12,11 +12,11 @@ import numpy as np
 import torch
 
 from . import synth
-from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 _DT_FLOAT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
-_DT_EXPERT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float8_e4m3fn: DT_E4M3}
+_DT_EXPERT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float8_e4m3fn: DT_E4M3, torch.int8: DT_I8}
 
 
 @dataclass
@@ -251,11 +251,20 @@ def e4m3_blocks(w: torch.Tensor):
     return q.flatten(-2).flatten(-3, -2)[..., :n, :k].to(torch.float8_e4m3fn).contiguous(), scale.contiguous()
 
 
+def int8_channels(w: torch.Tensor):
+    """A matrix [..., N, K] as int8 codes and one f32 scale (largest magnitude / 127) for each of its N output channels, the form in
+    which ops.int8_matmul and the expert products take it. Done once, when weights are loaded."""
+    v = w.float()
+    scale = v.abs().amax(-1) / 127.0
+    q = torch.where(scale[..., None] > 0, v / scale[..., None], torch.zeros_like(v)).round_().clamp_(-127.0, 127.0)
+    return q.to(torch.int8).contiguous(), scale.contiguous()
+
+
 @dataclass
 class FloatExpertBank:
-    """Weights of one MoE block whose experts are bf16, f16 or e4m3, all on one device.
+    """Weights of one MoE block whose experts are bf16, f16, e4m3 or int8, all on one device.
 
-    gate, up [E][F][H]; down [E][H][F]; for e4m3 their scales f32 [E][ceil(rows/128)][ceil(cols/128)]; router bf16 [E][H];
+    gate, up [E][F][H]; down [E][H][F]; for e4m3 their scales f32 [E][ceil(rows/128)][ceil(cols/128)], for int8 [E][rows]; router bf16 [E][H];
     router_bias f32 [E] or None; pre_norm, post_norm: norm weights [H] in front of the block and behind it (one type), or None;
     out_gate [H]: what the block's output is multiplied with (through a sigmoid with gate_sigmoid), or None; router_exact: False where
     the router's bf16 weights were rounded from a file that holds more bits."""
@@ -298,6 +307,13 @@ class FloatExpertBank:
             parts[name], parts[name + "_scale"] = e4m3_blocks(getattr(self, name))
         return replace(self, **parts)
 
+    def to_int8(self) -> "FloatExpertBank":
+        """The same block with its experts as int8 codes under a scale for each output channel."""
+        parts = {}
+        for name in ("gate", "up", "down"):
+            parts[name], parts[name + "_scale"] = int8_channels(getattr(self, name))
+        return replace(self, **parts)
+
 
 class MoeBlock:
     """One MoE block of a residual stream (knj_moe_block_launch): norm, routing, experts, ordered combine, norm behind the block, gate,
@@ -308,10 +324,12 @@ class MoeBlock:
         E, F, H = bank.gate.shape
         kind = bank.gate.dtype
         if kind not in _DT_EXPERT or bank.up.dtype != kind or bank.down.dtype != kind:
-            raise ValueError("experts are bf16, f16 or float8_e4m3fn, all three matrices of one type")
+            raise ValueError("experts are bf16, f16, float8_e4m3fn or int8, all three matrices of one type")
         want = {"gate": (E, F, H), "up": (E, F, H), "down": (E, H, F), "router": (E, H)}
         if kind == torch.float8_e4m3fn:
             want.update(gate_scale=(E, -(-F // 128), -(-H // 128)), up_scale=(E, -(-F // 128), -(-H // 128)), down_scale=(E, -(-H // 128), -(-F // 128)))
+        if kind == torch.int8:
+            want.update(gate_scale=(E, F), up_scale=(E, F), down_scale=(E, H))
         for name, shape in want.items():
             t = getattr(bank, name)
             if t is None or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:

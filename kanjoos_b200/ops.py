@@ -9,7 +9,7 @@ import functools
 import torch
 
 from . import _lib
-from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, check,
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, check,
                    lib, packed)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
@@ -266,14 +266,15 @@ def q4k_down_tc(ah, Wd, pair_idx, pair_cnt, P: int, pair_row=None, poison: bool 
     return Y, status
 
 
-# ---- experts in bf16, fp16 and e4m3, and what stands between two blocks -------------------------------------------
+# ---- experts in bf16, fp16, e4m3 and int8, and what stands between two blocks -------------------------------------------
 # These calls are made once or a few times per layer and decode step, so their host work counts: attributes are read once, outputs
 # come from new_empty / empty_like (1.4 us against torch.empty's 2.4).
 
 _cur = torch._C._cuda_getDevice
-_OPERAND = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, _E4M3: DT_E4M3}
+_OPERAND = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, _E4M3: DT_E4M3, torch.int8: DT_I8}
+_DT_OR_I8 = {**_DT, torch.int8: DT_I8}
 _norm_args, _expert_args = packed(BlockNormArgs), packed(ExpertGemmArgs)
-_ONLY_F32, _ONLY_I32, _ONLY_E4M3 = {torch.float32: DT_F32}, {torch.int32: 0}, {_E4M3: DT_E4M3}
+_ONLY_F32, _ONLY_I32, _ONLY_E4M3, _ONLY_I8 = {torch.float32: DT_F32}, {torch.int32: 0}, {_E4M3: DT_E4M3}, {torch.int8: DT_I8}
 
 
 def _refuse(t: torch.Tensor, what: str, cur: int, shape, types):
@@ -347,10 +348,53 @@ def fp8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, out_dtyp
     return y
 
 
+def int8_rows(x: torch.Tensor):
+    """x [rows][K] (f32 / bf16 / f16) -> (codes int8 [rows][K], scale f32 [rows])."""
+    ptr, code, ld = _rows(x, "x", _cur())
+    n, k = x.shape
+    q = x.new_empty(n, k, dtype=torch.int8)
+    scale = x.new_empty(n, dtype=torch.float32)
+    check(lib().knj_int8_rows_launch(ptr, code, ld, n, k, q.data_ptr(), scale.data_ptr(), _raw_stream()))
+    return q, scale
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_matmul_scratch(m: int, k: int) -> int:
+    return int(lib().knj_int8_matmul_workspace_bytes(m, k))
+
+
+def int8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, x_scale=None, out_dtype=torch.float32, status=None) -> torch.Tensor:
+    """W int8 [n_out][n_in] with W_scale f32 [n_out], x [m][n_in] (f32 / bf16 / f16, turned into int8 rows as int8_rows does, or int8
+    with x_scale f32 [m]) -> (x . W^T) * x_scale * W_scale, [m][n_out] in out_dtype. status as for expert_gateup."""
+    cur = _cur()
+    ptr, code, ld = _rows(x, "x", cur, None, _DT_OR_I8)
+    m, k = x.shape
+    n, out_code = W.shape[0], _DT.get(out_dtype)
+    if out_code is None:
+        raise ValueError(f"out_dtype is {out_dtype}")
+    if n >> 31:
+        _refuse_count("W", W.shape)
+    w = _dense(W, "W", cur, (n, k), _ONLY_I8)
+    ws = _dense(W_scale, "W_scale", cur, (n,), _ONLY_F32)
+    if (code == DT_I8) != (x_scale is not None):
+        raise ValueError("x_scale belongs to int8 rows, and they need it")
+    y = x.new_empty(m, n, dtype=out_dtype)
+    xs = work = nbytes = 0
+    if x_scale is not None:
+        xs = _dense(x_scale, "x_scale", cur, (m,), _ONLY_F32)
+    else:
+        nbytes = _int8_matmul_scratch(m, k)
+        scratch = x.new_empty(nbytes, dtype=torch.uint8)
+        work = scratch.data_ptr()
+    check(lib().knj_int8_matmul_launch(w, ws, k, n, ptr, code, xs, ld, m, y.data_ptr(), out_code, n, work, nbytes,
+                                       None if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), _raw_stream()))
+    return y
+
+
 def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, row_div, out, out_dtype, out_scale, status):
     cur = _cur()
     if w.dim() != 3 or w.dtype not in _OPERAND:
-        raise ValueError(f"expert matrices are bf16, f16 or float8_e4m3fn [E][N][K], got {w.dtype} {tuple(w.shape)}")
+        raise ValueError(f"expert matrices are bf16, f16, float8_e4m3fn or int8 [E][N][K], got {w.dtype} {tuple(w.shape)}")
     shape = w.shape
     E, N, K = shape
     types = (w.dtype,)
@@ -371,8 +415,21 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
         elif x_scale is None:
             raise ValueError("e4m3 rows need x_scale")
         xs = _dense(x_scale, "x_scale", cur, (x.shape[0], sshape[2]), _ONLY_F32)
+    elif w.dtype == torch.int8:
+        if s0 is None or (w1 is not None and s1 is None):
+            raise ValueError("int8 expert matrices need their scales")
+        s0_ptr = _dense(s0, "a matrix's scales", cur, (E, N), _ONLY_F32)
+        if w1 is not None:
+            s1_ptr = _dense(s1, "a matrix's scales", cur, (E, N), _ONLY_F32)
+        if x.dtype != torch.int8:
+            if x_scale is not None:
+                raise ValueError("x_scale belongs to int8 rows")
+            x, x_scale = int8_rows(x)
+        elif x_scale is None:
+            raise ValueError("int8 rows need x_scale")
+        xs = _dense(x_scale, "x_scale", cur, (x.shape[0],), _ONLY_F32)
     elif s0 is not None or s1 is not None or x_scale is not None:
-        raise ValueError("scales belong to e4m3 matrices and rows")
+        raise ValueError("scales belong to e4m3 and int8 matrices and rows")
     x_ptr, x_code, ld = _rows(x, "x", cur, (x.shape[0], K), {w.dtype: _OPERAND[w.dtype]})
     idx_shape = pair_idx.shape
     if len(idx_shape) != 2:
@@ -398,12 +455,13 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
 def expert_gateup(x, Wg, Wu, pair_idx, pair_cnt, P: int, top_k: int, pair_tok=None, gate_scale=None, up_scale=None, x_scale=None,
                   out_dtype=None, out=None, out_scale: float = 1.0, status=None):
     """silu(x . Wg[e]) * (x . Wu[e]) * out_scale for every routed pair: [P][N] in out_dtype (default: the matrices' type, bf16
-    for e4m3 ones). Wg, Wu [E][N][K] bf16 / f16 (x in the same type) or float8_e4m3fn with gate_scale and up_scale f32
-    [E][ceil(N/128)][ceil(K/128)] (x e4m3 with x_scale, or f32 / bf16 / f16, which fp8_rows turns into e4m3 rows). x [T][K];
+    for e4m3 and int8 ones). Wg, Wu [E][N][K] bf16 / f16 (x in the same type); float8_e4m3fn with gate_scale and up_scale f32
+    [E][ceil(N/128)][ceil(K/128)] (x e4m3 with x_scale, or f32 / bf16 / f16, which fp8_rows turns into e4m3 rows); or int8 with
+    gate_scale and up_scale f32 [E][N] (x int8 with x_scale [T], or f32 / bf16 / f16, which int8_rows turns into int8 rows). x [T][K];
     pair p reads row pair_tok[p], or p // top_k. Rows of pairs that no table entry names are left as they were. status: an i32 tensor of
     one element that is set to 1 when a bounded wait gave up (outputs concerned are NaN), otherwise left as it is."""
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if Wg.dtype == _E4M3 else Wg.dtype
+        out_dtype = torch.bfloat16 if Wg.dtype in (_E4M3, torch.int8) else Wg.dtype
     return _expert(lib().knj_expert_gateup_launch, x, x_scale, Wg, Wu, gate_scale, up_scale, pair_idx, pair_cnt, P, pair_tok, top_k, out,
                    out_dtype, out_scale, status)
 
