@@ -17,6 +17,7 @@ LIB_PATH = os.environ.get("KNJ_DEVICE_LIB") or os.path.join(PKG, "libknj_device.
 DT_F32, DT_BF16, DT_F16, DT_E4M3, DT_I8 = 0, 1, 2, 3, 5
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3  # KNJ_GATE_*
 EP_FLAG_WORDS, EP_MAX_CHUNKS = 4096, 8  # KNJ_EP_FLAG_WORDS, KNJ_EP_MAX_CHUNKS
+MOE_DECODE_MAX_TOKENS = 16  # KNJ_MOE_DECODE_MAX_TOKENS
 
 
 class KnjError(RuntimeError):
@@ -224,6 +225,8 @@ SIGNATURES = {
     "knj_expert_proj_launch": (_i, [_vp, _vp]),
     "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "knj_moe_block_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
+    "knj_moe_block_decode_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
+    "knj_moe_block_decode_test_stall": (None, [_i]),
     "knj_moe_block_status": (_i, [C.POINTER(MoeBlockArgs), _vp]),
     "knj_expert_tc_form": (None, [_i]),
     "knj_expert_tc_test_stall": (None, [_i]),

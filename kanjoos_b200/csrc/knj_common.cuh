@@ -103,6 +103,10 @@ int block_norm_check(const knj_block_norm_args *a);
 // What knj_expert_gateup_launch and knj_expert_proj_launch check of theirs, but for the number of tiles.
 int expert_product_check(const knj_expert_gemm_args *a, bool gateup, const char *who);
 
+// The MoE block in one launch (knj_moe_decode.cu), its arguments checked but for what concerns this form alone; and its scratch.
+int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t s);
+size_t moe_decode_workspace(int T, int H, int F, int E, int k);
+
 // Limit (SM clock cycles) of the bounded waits of the decode-class kernels, as set by knj_decode_wait_limit.
 long long decode_wait_cycles();
 

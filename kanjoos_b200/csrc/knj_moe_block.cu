@@ -13,6 +13,7 @@ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 inline bool has_codes(int w_dtype) { return w_dtype == KNJ_DT_E4M3 || w_dtype == KNJ_DT_I8; }
 // scales of a row of K codes
 inline size_t row_scales(int w_dtype, int K) { return w_dtype == KNJ_DT_E4M3 ? (K + 127) / 128 : 1; }
+inline int row_type(int w_dtype) { return w_dtype == KNJ_DT_F16 ? KNJ_DT_F16 : KNJ_DT_BF16; }   // 16-bit rows
 int code_rows(int w_dtype, const void *x, int x_dtype, int rows, int K, void *q, float *scale, knj_stream_t s) {
   return w_dtype == KNJ_DT_E4M3 ? knj_fp8_rows_launch(x, x_dtype, K, rows, K, q, scale, s) : knj_int8_rows_launch(x, x_dtype, K, rows, K, q, scale, s);
 }
@@ -59,6 +60,23 @@ struct StageSpan {
   ~StageSpan() { if (h >= 0) knj_span_end(h, s); }
 };
 
+// The norms behind the block and in front of it. The rows of x go on in the experts' 16-bit type, normalised or as they are.
+void norm_args(const knj_moe_block_args *a, const BlockWs &w, int32_t *status, knj_block_norm_args &after, knj_block_norm_args &before) {
+  const int T = a->n_tokens, H = a->hidden, act = row_type(a->w_dtype);
+  after.n_tokens = T; after.hidden = H; after.x = a->x; after.ldx = a->ldx; after.y = w.sum; after.ldy = H; after.post_w = a->post_w;
+  after.pre_w = a->next_w; after.gate = a->gate; after.ldg = a->ldg; after.stream_out = a->out; after.ld_stream = a->ldo; after.h = a->h_next;
+  after.ldh = a->ld_h_next; after.h_scale = a->h_next_scale; after.x_dtype = a->x_dtype; after.y_dtype = KNJ_DT_F32; after.w_dtype = a->w_norm_dtype;
+  after.gate_dtype = a->gate_dtype; after.stream_dtype = a->out_dtype; after.h_dtype = a->h_next_dtype; after.gate_kind = a->gate_kind;
+  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps; after.status = status;
+  before.n_tokens = T; before.hidden = H; before.x = a->x; before.ldx = a->ldx; before.x_dtype = a->x_dtype; before.w_dtype = a->w_norm_dtype;
+  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps; before.status = status;
+  if (a->pre_w) {
+    before.pre_w = a->pre_w; before.h = w.h; before.ldh = H; before.h_dtype = act;
+  } else {
+    before.stream_out = w.h; before.ld_stream = H; before.stream_dtype = act;
+  }
+}
+
 int check(const knj_moe_block_args *a, const char *who) {
   KNJ_REQUIRE(a, "%s: null argument block", who);
   KNJ_REQUIRE(a->n_tokens >= 0 && a->hidden > 0 && a->ffn > 0 && a->n_experts > 0, "%s: bad sizes", who);
@@ -88,7 +106,9 @@ extern "C" {
 
 size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype) {
   if (n_tokens <= 0) return 256;
-  return carve(nullptr, n_tokens, hidden, ffn, n_experts, top_k, w_dtype).bytes;
+  const size_t chain = carve(nullptr, n_tokens, hidden, ffn, n_experts, top_k, w_dtype).bytes;
+  const size_t one = moe_decode_workspace(n_tokens < KNJ_MOE_DECODE_MAX_TOKENS ? n_tokens : KNJ_MOE_DECODE_MAX_TOKENS, hidden, ffn, n_experts, top_k);
+  return chain > one ? chain : one;
 }
 
 int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
@@ -96,30 +116,17 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   if (rc || a->n_tokens == 0) return rc;
   const int T = a->n_tokens, H = a->hidden, F = a->ffn, E = a->n_experts, k = a->top_k, P = T * k;
   const bool q = has_codes(a->w_dtype);
-  const int act = a->w_dtype == KNJ_DT_F16 ? KNJ_DT_F16 : KNJ_DT_BF16;   // 16-bit rows
+  const int act = row_type(a->w_dtype);
   const BlockWs w = carve(a->workspace, T, H, F, E, k, a->w_dtype);
   int32_t *pair_exp = a->tap_pair_exp ? a->tap_pair_exp : w.pair_exp;
   float *pair_w = a->tap_pair_w ? a->tap_pair_w : w.pair_w;
   int32_t *status = a->status ? a->status : w.status;
 
   // what the launches check of the caller's operands is checked before the first runs
-  knj_block_norm_args after{};
-  after.n_tokens = T; after.hidden = H; after.x = a->x; after.ldx = a->ldx; after.y = w.sum; after.ldy = H; after.post_w = a->post_w;
-  after.pre_w = a->next_w; after.gate = a->gate; after.ldg = a->ldg; after.stream_out = a->out; after.ld_stream = a->ldo; after.h = a->h_next;
-  after.ldh = a->ld_h_next; after.h_scale = a->h_next_scale; after.x_dtype = a->x_dtype; after.y_dtype = KNJ_DT_F32; after.w_dtype = a->w_norm_dtype;
-  after.gate_dtype = a->gate_dtype; after.stream_dtype = a->out_dtype; after.h_dtype = a->h_next_dtype; after.gate_kind = a->gate_kind;
-  after.gate_sigmoid = a->gate_sigmoid; after.alpha = a->alpha; after.beta = a->beta; after.eps = a->eps; after.status = status;
+  knj_block_norm_args after{}, before{};
+  norm_args(a, w, status, after, before);
   rc = block_norm_check(&after);
   if (rc) return rc;
-  // the rows of x in the experts' 16-bit type, normalised or as they are
-  knj_block_norm_args before{};
-  before.n_tokens = T; before.hidden = H; before.x = a->x; before.ldx = a->ldx; before.x_dtype = a->x_dtype; before.w_dtype = a->w_norm_dtype;
-  before.beta = 1.0f; before.alpha = 1.0f; before.eps = a->eps; before.status = status;
-  if (a->pre_w) {
-    before.pre_w = a->pre_w; before.h = w.h; before.ldh = H; before.h_dtype = act;
-  } else {
-    before.stream_out = w.h; before.ld_stream = H; before.stream_dtype = act;
-  }
   knj_expert_gemm_args gateup{};
   gateup.pair_idx = w.pair_idx; gateup.pair_cnt = w.pair_cnt; gateup.idx_stride = T; gateup.n_pairs = P; gateup.n_experts = E;
   gateup.x_dtype = gateup.w_dtype = a->w_dtype; gateup.status = status;
@@ -165,6 +172,20 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
   rc = knj_moe_combine_launch(w.Y, nullptr, pair_exp, pair_w, nullptr, 0, 0, w.sum, KNJ_DT_F32, H, T, H, k, s);
   if (rc) return rc;
   return knj_block_norm_launch(&after, s);
+}
+
+int knj_moe_block_decode_launch(const knj_moe_block_args *a, knj_stream_t s) {
+  int rc = check(a, "knj_moe_block_decode");
+  if (rc || a->n_tokens == 0) return rc;
+  const BlockWs w = carve(a->workspace, a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
+  int32_t *status = a->status ? a->status : w.status;
+  knj_block_norm_args after{}, before{};
+  norm_args(a, w, status, after, before);
+  rc = block_norm_check(&after);
+  if (!rc) rc = block_norm_check(&before);
+  if (rc) return rc;
+  KNJ_REQUIRE(aligned16(a->w_gate) && aligned16(a->w_up) && aligned16(a->w_down), "knj_moe_block_decode: the experts' matrices must be 16-byte aligned");
+  return moe_decode_launch(a, status, s);
 }
 
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s) {

@@ -12,7 +12,8 @@ import numpy as np
 import torch
 
 from . import synth
-from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_ROW, MoeBlockArgs, MoeFfnArgs, check, lib)
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_ROW, MOE_DECODE_MAX_TOKENS, MoeBlockArgs, MoeFfnArgs, check,
+                   lib)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 _DT_FLOAT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
@@ -318,7 +319,7 @@ class FloatExpertBank:
 class MoeBlock:
     """One MoE block of a residual stream (knj_moe_block_launch): norm, routing, experts, ordered combine, norm behind the block, gate,
     scaled residual add and, on request, the norm in front of the next block. Bound to a maximum token count: the workspace is
-    allocated once here."""
+    allocated once here. run takes any number of tokens up to it, decode the few of a decode step."""
 
     def __init__(self, bank: FloatExpertBank, top_k: int = synth.TOP_K, max_tokens: int = 64, workspace: torch.Tensor | None = None):
         E, F, H = bank.gate.shape
@@ -390,9 +391,18 @@ class MoeBlock:
         gate [T][1] or [T][H] in place of the bank's. next_norm [H], in the type of the bank's norms (any float type where those are
         f32): also returns h = norm(out; next_norm) in next_dtype (default: x's type; float8_e4m3fn: (codes, scale)). Returns out, or
         a tuple (out[, h][, pair_exp, pair_w])."""
+        return self._call(lib().knj_moe_block_launch, self.max_tokens, x, out, gate, next_norm, next_dtype, return_routing)
+
+    def decode(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
+        """The block for up to MOE_DECODE_MAX_TOKENS tokens in one launch (knj_moe_block_decode_launch): arguments and results as of
+        run, with nothing between x and out rounded to 16 or 8 bits. Needs a device that the process has to itself."""
+        return self._call(lib().knj_moe_block_decode_launch, min(self.max_tokens, MOE_DECODE_MAX_TOKENS), x, out, gate, next_norm, next_dtype,
+                          return_routing)
+
+    def _call(self, launch, most, x, out, gate, next_norm, next_dtype, return_routing):
         b = self.bank
-        if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > self.max_tokens or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
-            raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {self.max_tokens}")
+        if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > most or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
+            raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {most}")
         if x.device != b.gate.device or x.get_device() != torch.cuda.current_device():
             raise ValueError(f"x lives on {x.device}, the block on {b.gate.device}; the current device is {torch.cuda.current_device()}")
         T, H = x.shape
@@ -423,7 +433,7 @@ class MoeBlock:
         if return_routing:
             taps = (torch.empty(T * self.top_k, dtype=torch.int32, device=x.device), torch.empty(T * self.top_k, dtype=torch.float32, device=x.device))
         a = self._args(x, out, gate, next_norm, h, scale, taps)
-        check(lib().knj_moe_block_launch(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        check(launch(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         self._last = a
         result = (out,) + (() if h is None else ((h, scale) if scale is not None else h,)) + (taps or ())
         return result if len(result) > 1 else out
