@@ -5,13 +5,14 @@
 //   out = beta * x + alpha * g * norm(y; post_w),   h_next = norm(out; next_w)
 // What is computed between x and out stays in f32, and so does what the matrices are multiplied with: a row of f32 values goes to the
 // tensor core as two 16-bit planes, hi = round(v) and lo = round(v - hi), which together hold 17 bits of v (bf16 experts, bf16 planes) or 22
-// (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). The planes of eight rows fill the
-// sixteen rows of mma.sync.m16n8k16, so that the second one costs nothing while a step's weights are on their way.
+// (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). In mma.sync.m16n8k16 sixteen matrix rows
+// meet the two planes of four tokens, so that the second plane costs nothing while a step's weights are on their way.
 //
-// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. Weights go
-// straight from HBM to registers (16 bytes a lane, eight loads under way), where they are MMA fragments as they lie: the order of K
-// is free as long as both operands have the same, and a lane takes eight consecutive k of one matrix row for two MMAs.
-// tcgen05 would want them in shared memory first and gives nothing: the tensor work of a token is a fiftieth of the time.
+// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
+// its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
+// multiply. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep HBM
+// busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both operands
+// have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
 //
 // Stages, with a barrier over the grid between them:
 //   1  norm statistics (every CTA, all tokens) and router logits (an expert or two a CTA)
@@ -27,16 +28,35 @@ using namespace knj;
 namespace {
 
 constexpr int kMaxTokens = KNJ_MOE_DECODE_MAX_TOKENS, kMaxK = 8, kMaxExperts = 256;
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kDepth = 4;                      // steps of 64 bytes a matrix row whose loads are under way
-constexpr int kRed = 32 * 1024;                // bytes of the partial sums of a batch of tiles
-constexpr int kPanel = 176 * 1024;             // bytes of the planes of the rows in use
+// Sixteen warps with 128 registers a thread: fifteen that multiply and one that copies. (With sixteen that multiply a thread has 96, and the
+// shared memory that the ring takes leaves no L1 for what then spills: every spilled word came back from L2, 1000 cycles under load.)
+constexpr int kWarps = 15, kThreads = 32 * kWarps, kAll = kThreads + 32;
+// A slot of the ring holds a tile: 64, 32, 16 or 8 matrix rows of up to 512, 1024, 2048 or 4096 bytes as they lie, in one or two copies.
+// (A copy for each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536.) Longer rows
+// come in slices of up to 4096 bytes, eight rows to a slot.
+constexpr int kSlice = 4096;
+constexpr int kSlot = 8 * kSlice;
+constexpr int kMaxSlots = 6;
+constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 64 a tile, warp and token
+constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
 constexpr int kMaxItems = 64;
+constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256,
+                 kCleared = kStatsAt - kSyncAt;   // of the workspace
 constexpr float kDown = 0x1p-64f;
 
 enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
 
+// Of a product: its rows in memory, and how they are cut
+struct Shape {
+  int K, N, row_bytes;
+  int slices, slice;   // of a row, bytes
+  int eight;           // tiles of eight rows, else of 16 a sub-tile
+  int subs;            // sub-tiles of a tile, each of which has 15 / subs warps
+  int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
+};
+
 struct DecodeParams {
+  Shape shape[2];      // gate and up, down
   const void *x, *pre_w, *post_w, *next_w, *gate;
   const uint16_t *router;
   const float *router_bias;
@@ -48,6 +68,8 @@ struct DecodeParams {
   float *tap_w;
   float *logits, *act, *Y;
   unsigned *sync;               // [0] arrivals, [1] raised by a wait that gave up; zero before the launch
+  float2 *stats;                // [tokens] inverse norm, largest magnitude of the normalised row
+  unsigned *row_max;            // [pairs] bits of the largest magnitude of an activation row; zero before the launch
   int32_t *status;
   int64_t ldx, ldo, ldg, ldh;
   int T, H, F, E, k;
@@ -65,22 +87,27 @@ struct Item {
 };
 struct Plan {
   Item item[kMaxItems];
-  int n_items, rounds_k;        // parts of K a tile is split into
+  int n_items, rows;            // rows: most that are in the panel at a time
 };
 
 struct Shared {
-  float part[kWarps][4];
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  int fail;                     // raised by a wait that gave up; read as volatile
+  float part[kAll / 32][4][6];  // of a token: squares, largest, dot products
   float inv[kMaxTokens], mult[kMaxTokens], unmult[kMaxTokens];
   int sel_e[kMaxTokens][kMaxK];
   float sel_w[kMaxTokens][kMaxK];
   unsigned mask[kMaxExperts];
+  uint8_t pair_at[kMaxExperts][kMaxTokens];   // pairs of an expert's tokens in ascending order
   int active[kMaxTokens * kMaxK];
   int n_active, ok;
   Plan plan[2];                 // gate and up, down
-  unsigned row_max[kMaxTokens];
-  float row_mult[kMaxTokens], row_unmult[kMaxTokens];   // of the panel's rows
-  float red[2][kWarps];
+  int row_tok[kMaxTokens], row_pair[kMaxTokens];        // of the panel's rows
+  float row_mult[kMaxTokens], row_unmult[kMaxTokens];
+  float red[4][kAll / 32];
 };
+
+static_assert(kSmem + sizeof(Shared) <= 227 * 1024, "shared memory of a block");
 
 // ---- small pieces -------------------------------------------------------------------------------------------------------
 
@@ -89,54 +116,73 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-// Barrier over the grid, number `n` of the launch. False for all threads of the CTA where it did not complete in time.
-__device__ __forceinline__ bool grid_barrier(const DecodeParams &p, Shared &s, int n) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
+// of the warps that multiply
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+template <int N>
+__device__ __forceinline__ void cta_barrier() {
+  if constexpr (N == kAll) __syncthreads();
+  else meet();
+}
+// Barrier over the grid, number `n` of the launch, in two halves, met by the first N threads of every CTA. A CTA in which a wait has given
+// up never arrives; grid_wait is false for all threads where the barrier did not complete in time.
+template <int N>
+__device__ __forceinline__ void grid_arrive(const DecodeParams &p, Shared &s) {
+  cta_barrier<N>();
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0)
     asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.sync), "r"(1u) : "memory");
+}
+template <int N>
+__device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int n) {
+  if (threadIdx.x == 0) {
+    int ok = *reinterpret_cast<volatile int *>(&s.fail) == 0;
     const unsigned target = gridDim.x * (unsigned)n + (p.stall == n ? 1u : 0u);
     const long long t0 = clock64();
-    int ok = 1;
-    while (ld_acquire(p.sync) < target) {
-      if (ld_acquire(p.sync + 1) != 0u || clock64() - t0 > p.wait_cycles) {
-        atomicExch(p.sync + 1, 1u);
-        atomicExch(p.status, 1);
-        ok = 0;
-        break;
-      }
+    while (ok && ld_acquire(p.sync) < target) {
+      if (ld_acquire(p.sync + 1) != 0u || clock64() - t0 > p.wait_cycles) ok = 0;
     }
     s.ok = ok;
   }
-  __syncthreads();
+  cta_barrier<N>();
   return s.ok != 0;
 }
 
-__device__ __forceinline__ uint4 load_weights(const uint8_t *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// eight consecutive values of a row as they lie in memory, at a 16-byte boundary: without branches, so that many loads go out together
+struct Raw8 {
+  uint4 a, b;
+};
+__device__ __forceinline__ Raw8 load_raw8(const void *base, int dtype, int64_t i) {
+  Raw8 r;
+  const bool wide = dtype == KNJ_DT_F32;
+  const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(base) + i * (wide ? 4 : 2));
+  r.a = q[0];
+  r.b = r.a;
+  if (wide) r.b = q[1];
+  return r;
 }
-
-// eight consecutive values of a row; `vec`: at a 16-byte boundary
+__device__ __forceinline__ void values8(const Raw8 &r, int dtype, float (&v)[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if (dtype == KNJ_DT_BF16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+  } else if (dtype == KNJ_DT_F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+      v[2 * j] = h.x;
+      v[2 * j + 1] = h.y;
+    }
+  }
+}
+// the same of a row at any address
 __device__ __forceinline__ void load8(const void *base, int dtype, int64_t i, bool vec, float (&v)[8]) {
-  if (!vec) {
+  if (vec) {
+    values8(load_raw8(base, dtype, i), dtype, v);
+  } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = load_as_f32(base, dtype, i + j);
-    return;
-  }
-  if (dtype == KNJ_DT_F32) {
-    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i), b = *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + i);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = dtype == KNJ_DT_BF16 ? make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u))
-                                          : __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
   }
 }
 
@@ -192,317 +238,403 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &p0, uint32_t &p1
   }
 }
 
-__device__ __forceinline__ float cta_sum(float v, float *red) {   // red: kWarps words, not in use by an earlier sum
+__device__ __forceinline__ float cta_sum(float v, float *red) {   // by all threads; red: a word for each warp, not in use by an earlier sum
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) t += red[i];
+  for (int i = 0; i < kAll / 32; ++i) t += red[i];
   return t;
 }
 
 template <int KIND>
 struct Geo {
   static constexpr int kElem = KIND <= kF16 ? 2 : 1;
-  // bytes of a plane of K values: whole steps, and rows an odd 64 (of codes: 16) bytes apart, so that the eight lanes that a load of
-  // shared memory serves at a time (two rows, four runs of k) find all banks
+  // bytes of a plane of K values: whole steps, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
   __host__ __device__ static int pitch(int K) { return (2 * K + 127) / 128 * 128 + (kElem == 2 ? 64 : 16); }
-  __host__ __device__ static int cap(int K) { const int c = kPanel / (2 * pitch(K)); return c < kMaxTokens ? c : kMaxTokens; }
+  // rows in the panel at a time: what leaves the ring two slots, or one
+  __host__ __device__ static int cap(int K) {
+    const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
+    return c < 1 ? 1 : c < kMaxTokens ? c : kMaxTokens;
+  }
 };
 
 // ---- products -----------------------------------------------------------------------------------------------------------
 
-// What a warp does in a product: a tile is eight rows of gate and the same eight of up, or sixteen rows of down; `part` of `parts` of
-// its K, and the tiles `group`, `group` + `groups`, .. of each item.
-struct Split {
-  int parts, groups, part, group, s0, s1;   // steps s0 .. s1-1
-};
-
-// The loads of a warp, kDepth steps ahead of its products: they walk over the same tiles and steps in the same order.
-template <int KIND, bool GATEUP>
-struct Feed {
-  uint4 w[kDepth][2];
-  float sc[kDepth][2];         // e4m3: scales of the blocks, for the columns of this lane's sums
-  const uint8_t *p0, *p1;      // this lane's bytes of the tile
-  const float *q0, *q1;        // scales' rows
-  int item, tile, step;        // step: first of the block of kDepth
-  bool row0, row1;             // rows of this item
-};
-
-template <int KIND, bool GATEUP>
-struct Product {
-  static constexpr int kElem = Geo<KIND>::kElem;
-  static constexpr int kRows = GATEUP ? 8 : 16;
-  const DecodeParams &p;
-  const Plan &plan;
-  Split sp;
-  int K, N, row_bytes, lane;
-
-  __device__ __forceinline__ int tiles(const Item &it) const { return (it.r1 - it.r0 + kRows - 1) / kRows; }
-  __device__ __forceinline__ void at_tile(Feed<KIND, GATEUP> &f) const {   // pointers of the feed's tile; steps over items without one for this warp
-    while (f.item < plan.n_items && f.tile >= tiles(plan.item[f.item])) {
-      ++f.item;
-      f.tile = sp.group;
-    }
-    if (f.item >= plan.n_items) return;
-    const Item &it = plan.item[f.item];
-    const int r = it.r0 + f.tile * kRows + (lane >> 2), r2 = GATEUP ? r : r + 8;
-    f.row0 = r < it.r1;
-    f.row1 = r2 < it.r1;
-    const int64_t at = (int64_t)it.expert * N;
-    f.p0 = (GATEUP ? p.w_gate : p.w_down) + (at + r) * row_bytes + (lane & 3) * 16;
-    f.p1 = (GATEUP ? p.w_up : p.w_down) + (at + r2) * row_bytes + (lane & 3) * 16;
-    if constexpr (KIND == kE4) {
-      // sums of columns 2 (lane & 3), + 1: runs start at even rows, so both are in one block
-      const int c = it.r0 + f.tile * kRows + 2 * (lane & 3), c2 = GATEUP ? c : c + 8, kb = (K + 127) / 128, nb = (N + 127) / 128;
-      f.q0 = (GATEUP ? p.s_gate : p.s_down) + ((int64_t)it.expert * nb + min(c / 128, nb - 1)) * kb;
-      f.q1 = (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min(c2 / 128, nb - 1)) * kb;
-    }
-  }
-  __device__ __forceinline__ void start(Feed<KIND, GATEUP> &f) const {
-    f.item = sp.group < sp.groups ? 0 : plan.n_items;
-    f.tile = sp.group;
-    f.step = sp.s0;
-    at_tile(f);
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) issue(f, d);
-    next(f);
-  }
-  __device__ __forceinline__ void issue(Feed<KIND, GATEUP> &f, int d) const {
-    const int s = f.step + d, off = s * 64;
-    const bool any = f.item < plan.n_items && s < sp.s1, in = any && off + (lane & 3) * 16 < row_bytes;
-    f.w[d][0] = in && f.row0 ? load_weights(f.p0 + off) : make_uint4(0, 0, 0, 0);
-    f.w[d][1] = in && f.row1 ? load_weights(f.p1 + off) : make_uint4(0, 0, 0, 0);
-    if constexpr (KIND == kE4) {
-      f.sc[d][0] = any ? __ldg(f.q0 + (s >> 1)) : 0.f;
-      f.sc[d][1] = any ? __ldg(f.q1 + (s >> 1)) : 0.f;
-    }
-  }
-  __device__ __forceinline__ void next(Feed<KIND, GATEUP> &f) const {   // behind the issue of a whole block
-    if (f.item >= plan.n_items) return;
-    f.step += kDepth;
-    if (f.step >= sp.s1) {
-      f.step = sp.s0;
-      f.tile += sp.groups;
-      at_tile(f);
-    }
-  }
-
-  // one step: eight rows' planes (of each GROUPS) times the two row tiles
-  template <int GROUPS>
-  __device__ __forceinline__ void step(const Feed<KIND, GATEUP> &f, int d, int s, const uint8_t *const (&rows)[2], int pitch, float (&acc)[2][2][4]) const {
-#pragma unroll
-    for (int q = 0; q < GROUPS; ++q) {
-      const uint8_t *a = rows[q] + s * (128 / kElem);
-      if constexpr (kElem == 2) {
-        const uint4 h = *reinterpret_cast<const uint4 *>(a), l = *reinterpret_cast<const uint4 *>(a + pitch);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma<KIND>(acc[q][m], h.x, l.x, h.y, l.y, f.w[d][m].x, f.w[d][m].y);
-          mma<KIND>(acc[q][m], h.z, l.z, h.w, l.w, f.w[d][m].z, f.w[d][m].w);
-        }
-      } else {
-        const uint4 h0 = *reinterpret_cast<const uint4 *>(a), h1 = *reinterpret_cast<const uint4 *>(a + 16);
-        const uint4 l0 = *reinterpret_cast<const uint4 *>(a + pitch), l1 = *reinterpret_cast<const uint4 *>(a + pitch + 16);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-          float (&t)[4] = KIND == kE4 ? part : acc[q][m];
-          uint32_t b0, b1;
-          codes_f16<KIND>(f.w[d][m].x, b0, b1);
-          mma<KIND>(t, h0.x, l0.x, h0.y, l0.y, b0, b1);
-          codes_f16<KIND>(f.w[d][m].y, b0, b1);
-          mma<KIND>(t, h0.z, l0.z, h0.w, l0.w, b0, b1);
-          codes_f16<KIND>(f.w[d][m].z, b0, b1);
-          mma<KIND>(t, h1.x, l1.x, h1.y, l1.y, b0, b1);
-          codes_f16<KIND>(f.w[d][m].w, b0, b1);
-          mma<KIND>(t, h1.z, l1.z, h1.w, l1.w, b0, b1);
-          if constexpr (KIND == kE4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[q][m][i] = fmaf(f.sc[d][m], part[i], acc[q][m][i]);
-          }
-        }
-      }
+// place in the ring
+struct Ring {
+  int at, n;
+  uint32_t parity;
+  bool ok;     // of the warps that multiply: no wait has given up
+  __device__ __forceinline__ void next() {
+    if (++at == n) {
+      at = 0;
+      parity ^= 1u;
     }
   }
 };
 
-// slot `i` of an expert: the token of the i-th bit of its mask, and the pair
-__device__ __forceinline__ int slot_token(unsigned mask, int i) {
-  while (i-- > 0) mask &= mask - 1u;
-  return __ffs(mask) - 1;
-}
-__device__ __forceinline__ int slot_pair(const Shared &s, int k, int e, int t) {
-  int at = 0;
-  for (int j = 1; j < k; ++j)
-    if (s.sel_e[t][j] == e) at = j;
-  return t * k + at;
-}
-
-// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y. The first loads may be under way (`feed` started).
-template <int KIND, bool GATEUP>
-__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, const Product<KIND, GATEUP> &pr, Feed<KIND, GATEUP> &feed, uint8_t *panel,
-                                            float4 *red) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  const Plan &plan = pr.plan;
-  const int K = pr.K, pitch = Geo<KIND>::pitch(K), cap = Geo<KIND>::cap(K);
-  const Split sp = pr.sp;
-  int built = 0;   // items whose rows are in the panel
+// The copying warp's side of a product. False after a wait that gave up.
+__device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int product, Ring &ring, uint8_t *slots, int &copied) {
+  const int lane = threadIdx.x & 31;
+  const Shape &sh = p.shape[product];
+  const Plan &plan = s.plan[product];
+  const bool up = product == 0, whole = sh.slices == 1;
   for (int i = 0; i < plan.n_items; ++i) {
     const Item it = plan.item[i];
-    if (i >= built) {
-      // ---- the rows of this and the next items, as many as the panel takes ----
-      int n = 0;
-      for (built = i; built < plan.n_items && n + plan.item[built].n <= cap; ++built) n += plan.item[built].n;
-      __syncthreads();   // the last panel and its powers are read
-      if (!GATEUP && KIND != kBf16) {
-        if (tid < kMaxTokens) s.row_max[tid] = 0u;
-        __syncthreads();
+    for (int first = it.r0; first < it.r1; first += sh.outs) {
+      const int rows = min(sh.outs, it.r1 - first);
+      // lane l copies the rows of matrix l, or row l % rows of matrix l / rows
+      const int second = up && (whole ? lane == 1 : lane >= rows), r = whole ? 0 : lane - second * rows;
+      const bool mine = lane < (whole ? 1 : rows) * (up ? 2 : 1);
+      const uint8_t *src = (up ? (second ? p.w_up : p.w_gate) : p.w_down) + ((int64_t)it.expert * sh.N + first + r) * sh.row_bytes;
+      const int dst = (second * sh.outs + r) * sh.slice;
+      for (int sl = 0; sl < sh.slices; ++sl) {
+        const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - sl * sh.slice);
+        const bool ok = mbar_wait_for(&s.empty[ring.at], ring.parity ^ 1u, p.wait_cycles, &s.fail);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (lane == 0) mbar_expect_tx(&s.full[ring.at], (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
+        __syncwarp();
+        if (mine) bulk_g2s(slots + ring.at * kSlot + dst, src + sl * sh.slice, (uint32_t)bytes, &s.full[ring.at]);
+        ring.next();
+        ++copied;
       }
-      auto row_of = [&](int r, int &e, int &slot) {
-        int j = i;
-        while (r >= plan.item[j].n) r -= plan.item[j++].n;
-        e = plan.item[j].expert;
-        slot = plan.item[j].first + r;
-      };
-      const int chunks = (K + 63) / 64 * 8;   // of eight values: whole steps
-      if (!GATEUP && KIND != kBf16) {
-        for (int r = 0; r < n; ++r) {
-          int e, slot;
-          row_of(r, e, slot);
-          const float *src = p.act + (int64_t)slot_pair(s, p.k, e, slot_token(s.mask[e], slot)) * K;
-          float m = 0.f;
-          for (int c = tid; c < K / 4; c += kThreads) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + c);
-            m = max3_abs_nan(max3_abs_nan(m, v.x, v.y), v.z, v.w);
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (lane == 0) atomicMax(&s.row_max[r], __float_as_uint(m) & 0x7fffffffu);   // magnitudes order as their bits do, a NaN above all
-        }
-        __syncthreads();
-      }
-      for (int idx = tid; idx < n * chunks; idx += kThreads) {
-        const int r = idx / chunks, c = idx - r * chunks;
-        int e, slot;
-        row_of(r, e, slot);
-        const int t = slot_token(s.mask[e], slot);
-        float v[8], mult = 1.f, unmult = 1.f;
-        if (8 * c >= K) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        } else if (GATEUP) {
-          load8(p.x, p.x_dtype, t * p.ldx + 8 * c, p.x_vec, v);
-          if (p.pre_w) {
-            float w[8];
-            load8(p.pre_w, p.norm_dtype, 8 * c, true, w);
-            const float inv = s.inv[t];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * w[j];
-          }
-        } else {
-          const float4 *src = reinterpret_cast<const float4 *>(p.act + (int64_t)slot_pair(s, p.k, e, t) * K) + 2 * c;
-          const float4 a = __ldcg(src), b = __ldcg(src + 1);
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        }
-        if constexpr (KIND != kBf16) {
-          if (GATEUP) {
-            mult = s.mult[t];
-            unmult = s.unmult[t];
-          } else {
-            row_power(__uint_as_float(s.row_max[r]), mult, unmult);
-          }
-        }
-        uint4 hi, lo;
-        planes2<KIND>(v[0] * mult, v[1] * mult, hi.x, lo.x);
-        planes2<KIND>(v[2] * mult, v[3] * mult, hi.y, lo.y);
-        planes2<KIND>(v[4] * mult, v[5] * mult, hi.z, lo.z);
-        planes2<KIND>(v[6] * mult, v[7] * mult, hi.w, lo.w);
-        uint8_t *dst = panel + (2 * r) * pitch + 16 * c;
-        *reinterpret_cast<uint4 *>(dst) = hi;
-        *reinterpret_cast<uint4 *>(dst + pitch) = lo;
-        if (c == 0) s.row_unmult[r] = unmult;
-      }
-      __syncthreads();
     }
-    // ---- the item's tiles ----
-    int base = 0;
-    for (int j = it.panel; j < i; ++j) base += plan.item[j].n;
-    const int tiles = pr.tiles(it), rounds = (tiles + sp.groups - 1) / sp.groups, two = it.n > 8;
-    const int batch = kRed / (kWarps * 512 * (1 + two));   // rounds whose sums fit
-    const uint8_t *rows[2];
+  }
+  return true;
+}
+
+// A lane's part of a run of 128 bytes (two steps of 64): of rows g and g + 8, or of row g of eight, the bytes 16 j .. + 15 of either step.
+struct Weights {
+  uint4 w[2][2];   // [step][row]
+};
+// Rows a multiple of 128 bytes apart lie on the same banks, and a load of shared memory serves two of them at a time: the odd one reads its
+// second step first, and the two change places in registers. left: bytes of the rows from the run's first on; what lies behind is zero.
+template <bool EIGHT>
+__device__ __forceinline__ void load_run(Weights &v, const uint8_t *row0, const uint8_t *row1, bool swap, int left) {
+  const int first = swap ? 64 : 0;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) rows[q] = panel + 2 * (base + min(8 * q + (lane >> 2), it.n - 1)) * pitch + (lane & 3) * (32 / pr.kElem);
-    for (int round = 0; round < rounds; ++round) {
-      const int in_batch = round % batch;
-      if (sp.group < sp.groups && round * sp.groups + sp.group < tiles) {
-        float acc[2][2][4];
+  for (int m = 0; m < 2; ++m) {
+    if (EIGHT && m == 1) {
+      v.w[0][1] = v.w[1][1] = make_uint4(0, 0, 0, 0);
+      break;
+    }
+    const uint8_t *row = m == 0 ? row0 : row1;
+    const uint4 a = *reinterpret_cast<const uint4 *>(row + first), b = *reinterpret_cast<const uint4 *>(row + 64 - first);
+    v.w[0][m] = swap ? b : a;
+    v.w[1][m] = swap ? a : b;
+  }
+  const int at = (threadIdx.x & 3) * 16;
+  if (left < 128) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+    for (int u = 0; u < 2; ++u)
+      if (u * 64 + at >= left) v.w[u][0] = v.w[u][1] = make_uint4(0, 0, 0, 0);
+  }
+}
+// a lane's run of a plane for a step
+template <int KIND>
+struct Acts {
+  uint4 b[KIND <= kF16 ? 1 : 2];
+  __device__ __forceinline__ void load(const uint8_t *at) {
+    b[0] = *reinterpret_cast<const uint4 *>(at);
+    if constexpr (KIND > kF16) b[1] = *reinterpret_cast<const uint4 *>(at + 16);
+  }
+};
+// One step of sixteen rows times the planes of four tokens
+template <int KIND>
+__device__ __forceinline__ void step(const uint4 (&w)[2], const Acts<KIND> &x, float (&acc)[4]) {
+  if constexpr (KIND <= kF16) {
+    mma<KIND>(acc, w[0].x, w[1].x, w[0].y, w[1].y, x.b[0].x, x.b[0].y);
+    mma<KIND>(acc, w[0].z, w[1].z, w[0].w, w[1].w, x.b[0].z, x.b[0].w);
+  } else {
+    const uint32_t r0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, r1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+    const uint32_t b[8] = {x.b[0].x, x.b[0].y, x.b[0].z, x.b[0].w, x.b[1].x, x.b[1].y, x.b[1].z, x.b[1].w};
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[q][m][j] = 0.f;
-        for (int st = sp.s0; st < sp.s1; st += kDepth) {
-#pragma unroll
-          for (int d = 0; d < kDepth; ++d) {
-            if (st + d < sp.s1) {
-              if (two) pr.template step<2>(feed, d, st + d, rows, pitch, acc);
-              else pr.template step<1>(feed, d, st + d, rows, pitch, acc);
-            }
-            pr.issue(feed, d);
-          }
-          pr.next(feed);
-        }
-        float4 *dst = red + ((in_batch * (1 + two)) * kWarps + sp.group * sp.parts + sp.part) * 32 + lane;
-        dst[0] = make_float4(acc[0][0][0] + acc[0][0][2], acc[0][0][1] + acc[0][0][3], acc[0][1][0] + acc[0][1][2], acc[0][1][1] + acc[0][1][3]);
-        if (two)
-          dst[kWarps * 32] = make_float4(acc[1][0][0] + acc[1][0][2], acc[1][0][1] + acc[1][0][3], acc[1][1][0] + acc[1][1][2], acc[1][1][1] + acc[1][1][3]);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a[4];
+      codes_f16<KIND>(r0[i], a[0], a[2]);
+      codes_f16<KIND>(r1[i], a[1], a[3]);
+      mma<KIND>(acc, a[0], a[1], a[2], a[3], b[2 * i], b[2 * i + 1]);
+    }
+  }
+}
+
+// The rows of items i .. in the panel, as many as it takes: their planes, zeros behind K up to whole steps. Returns the item behind them.
+template <int KIND, bool GATEUP>
+__device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, const Plan &plan, int K, uint8_t *panel, int i) {
+  const int tid = threadIdx.x, pitch = Geo<KIND>::pitch(K);
+  int n = 0, built = i;
+  for (; built < plan.n_items && plan.item[built].panel == i; ++built) n += plan.item[built].n;
+  if (tid < n) {
+    int r = tid, j = i;
+    while (r >= plan.item[j].n) r -= plan.item[j++].n;
+    const int pair = s.pair_at[plan.item[j].expert][plan.item[j].first + r], t = pair / p.k;
+    s.row_tok[tid] = t;
+    s.row_pair[tid] = pair;
+    if constexpr (KIND != kBf16) {
+      if (GATEUP) {
+        s.row_mult[tid] = s.mult[t];
+        s.row_unmult[tid] = s.unmult[t];
+      } else {
+        row_power(__uint_as_float(__ldcg(p.row_max + pair)), s.row_mult[tid], s.row_unmult[tid]);
       }
-      if (in_batch != batch - 1 && round != rounds - 1) continue;
-      __syncthreads();
-      // ---- sums over the parts of K, in order ----
-      const int first = (round - in_batch) * sp.groups, here = min(tiles - first, (in_batch + 1) * sp.groups);
-      const int per = it.n * (GATEUP ? 8 : 16);   // outputs of a tile
-      for (int o = tid; o < here * per; o += kThreads) {
-        const int tile = o / per, rest = o - tile * per, tok = rest / (GATEUP ? 8 : 16), r = rest % (GATEUP ? 8 : 16);
-        const int row = it.r0 + (first + tile) * Product<KIND, GATEUP>::kRows + r;
-        if (row >= it.r1) continue;
-        const int rd = tile / sp.groups, gr = tile - rd * sp.groups, q = tok >> 3;
-        const float *src = reinterpret_cast<const float *>(red + ((rd * (1 + two) + q) * kWarps + gr * sp.parts) * 32 + (tok & 7) * 4 + ((r & 7) >> 1)) + (r & 1);
-        float a = 0.f, b = 0.f;
-        for (int part = 0; part < sp.parts; ++part) {
-          a += src[part * 128 + (GATEUP ? 0 : (r >> 3) * 2)];
-          if (GATEUP) b += src[part * 128 + 2];
+    }
+  }
+  meet();
+  const int chunks = (K + 63) / 64 * 8, runs = (chunks + 31) / 32;   // of eight values; of 32 such: a warp's
+#pragma unroll 2
+  for (int u = tid >> 5; u < n * runs; u += kWarps) {
+    const int r = u / runs, c = (u - r * runs) * 32 + (tid & 31);
+    if (c >= chunks) continue;
+    float v[8];
+    if (8 * c >= K) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    } else if (GATEUP) {
+      const int t = s.row_tok[r];
+      load8(p.x, p.x_dtype, t * p.ldx + 8 * c, p.x_vec, v);
+      if (p.pre_w) {
+        float w[8];
+        load8(p.pre_w, p.norm_dtype, 8 * c, true, w);
+        const float inv = s.inv[t];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * w[j];
+      }
+    } else {
+      const float4 *src = reinterpret_cast<const float4 *>(p.act + (int64_t)s.row_pair[r] * K) + 2 * c;
+      const float4 a = __ldcg(src), b = __ldcg(src + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    if constexpr (KIND != kBf16) {
+      const float mult = s.row_mult[r];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= mult;
+    }
+    uint4 hi, lo;
+    planes2<KIND>(v[0], v[1], hi.x, lo.x);
+    planes2<KIND>(v[2], v[3], hi.y, lo.y);
+    planes2<KIND>(v[4], v[5], hi.z, lo.z);
+    planes2<KIND>(v[6], v[7], hi.w, lo.w);
+    uint8_t *dst = panel + (2 * r) * pitch + 16 * c;
+    *reinterpret_cast<uint4 *>(dst) = hi;
+    *reinterpret_cast<uint4 *>(dst + pitch) = lo;
+  }
+  return built;
+}
+
+// The sums over the parts of K of the sub-tiles 0 .. n-1 of a batch, whose first output is `first`: a warp per sub-tile. Parts are added in
+// kShare chains and these in pairs, by as many lanes for a single token, by one for more: in the same order, so that a token's bits do
+// not depend on the others'.
+template <int KIND, bool GATEUP, bool EIGHT>
+__device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, const Item &it, int base, const float *red, int n, int first) {
+  constexpr int kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kShare = GATEUP ? 4 : 2;
+  const int lane = threadIdx.x & 31;
+  const Shape &sh = p.shape[GATEUP ? 0 : 1];
+  const int parts = kWarps / sh.subs, tokens = it.n;
+  const bool one = tokens == 1;
+  for (int u = threadIdx.x >> 5; u < n; u += kWarps)
+    for (int o = lane; o < (tokens * kOuts * (one ? kShare : 1) + 31) / 32 * 32; o += 32) {
+      const int r = o % kOuts, tok = one ? 0 : o / kOuts, chain = one ? o / kOuts : 0, row = first + u * kOuts + r;
+      const bool in = tok < tokens && chain < kShare && row < it.r1;
+      auto sum = [&](int from, float &a, float &b) {
+        a = b = 0.f;
+        if (!in) return;
+        const float *src = red + ((u * parts + from) * tokens + tok) * 16 + r;
+#pragma unroll 4
+        for (int w = from; w < parts; w += kShare, src += kShare * tokens * 16) {
+          a += src[0];
+          if (GATEUP) b += src[kOuts];
         }
+      };
+      float a, b;
+      sum(chain, a, b);
+      if (one) {
+#pragma unroll
+        for (int x = 1; x < kShare; x *= 2) {
+          a += __shfl_xor_sync(0xffffffffu, a, x * kOuts);
+          b += __shfl_xor_sync(0xffffffffu, b, x * kOuts);
+        }
+      } else {
+        float c[2], d[2];
+        sum(1, c[0], d[0]);
+        a += c[0];
+        b += d[0];
+        if constexpr (kShare == 4) {
+          sum(2, c[0], d[0]);
+          sum(3, c[1], d[1]);
+          a += c[0] + c[1];
+          b += d[0] + d[1];
+        }
+      }
+      const int pair = s.row_pair[base + (tok < tokens ? tok : 0)];
+      if (in) {
         const float un = KIND == kBf16 ? 1.0f : s.row_unmult[base + tok];
         a *= un;
         b *= un;
-        const int t = slot_token(s.mask[it.expert], it.first + tok), pair = slot_pair(s, p.k, it.expert, t);
         if constexpr (KIND == kS8) {
-          a *= __ldg((GATEUP ? p.s_gate : p.s_down) + (int64_t)it.expert * pr.N + row);
-          if (GATEUP) b *= __ldg(p.s_up + (int64_t)it.expert * pr.N + row);
+          a *= __ldg((GATEUP ? p.s_gate : p.s_down) + (int64_t)it.expert * sh.N + row);
+          if (GATEUP) b *= __ldg(p.s_up + (int64_t)it.expert * sh.N + row);
         }
-        if (GATEUP) p.act[(int64_t)pair * pr.N + row] = a / (1.0f + expf(-a)) * b;
-        else p.Y[(int64_t)pair * pr.N + row] = a;
+        if (GATEUP) a = a / (1.0f + expf(-a)) * b;
+        if (chain == 0) (GATEUP ? p.act : p.Y)[(int64_t)pair * sh.N + row] = a;
       }
-      __syncthreads();
+      if constexpr (GATEUP && KIND != kBf16) {
+        float m = in ? fabsf(a) : 0.f;
+#pragma unroll
+        for (int x = kOuts / 2; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, x));
+        // magnitudes order as their bits do, a NaN above all
+        if (r == 0 && chain == 0 && in) atomicMax(p.row_max + pair, __float_as_uint(m) & 0x7fffffffu);
+      }
     }
+}
+
+// The tiles of an item. All fifteen warps take part in each: a sub-tile has 15 / subs of them, and a warp every 15 / subs-th run of 128 bytes
+// of a slice of its rows; their sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
+// A warp whose wait gives up raises s.fail, waits no more and frees no slot, but meets every barrier; what it forms then is never used.
+// (Sub-tiles in slots of their own would let the groups of warps drift apart, past what a barrier's two phases tell apart.)
+// Shared memory's bandwidth is what the products would be bound by: 32 KB of weights are 256 cycles of its 128 bytes, in some 1400 that
+// HBM takes to bring them. HOLD: up to four tokens' planes, read once for all tiles, stay in registers where a row is one slice; read
+// from shared memory at each step they cost as much as the weights.
+template <int KIND, bool GATEUP, bool EIGHT, bool HOLD>
+__device__ __forceinline__ void run_tiles(const DecodeParams &p, Shared &s, const Item &it, int base, Ring &ring, const uint8_t *panel, float *red,
+                                          const uint8_t *slots) {
+  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kGroups = HOLD ? 1 : 4;
+  constexpr int kRuns = EIGHT ? 3 : 2;   // most runs of a warp in a slice: 32 of eight rows over fifteen warps; 16, 8 or 4 over 15, 7 or 3
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const Shape &sh = p.shape[GATEUP ? 0 : 1];
+  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = kWarps / subs, sub = warp / parts, part = warp - sub * parts;
+  const int tiles = (it.r1 - it.r0 + sh.outs - 1) / sh.outs, groups = (it.n + 3) / 4, batch = kRed / (64 * 16 * it.n);
+  // this lane's bytes of rows g and g + 8 of its sub-tile in a slot, of gate and up of row g of either; EIGHT: of the slot's row g
+  const bool swap = (g & 1) && (sh.slice & 64) == 0;
+  const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16, row1 = row0 + (GATEUP ? sh.outs : 8) * sh.slice, run_bytes = parts * 128;
+  const uint8_t *rows[kGroups];   // this lane's run of a plane of one of each four tokens
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q)
+    rows[q] = panel + (2 * (base + min(4 * q + (g >> 1), it.n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+  constexpr int kHeld = KIND <= kF16 ? 2 : 1;   // runs whose planes stay in sixteen registers
+  Acts<KIND> held[kHeld][2];
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (part * 128 + r * run_bytes + u * 64 < sh.row_bytes) held[r][u].load(rows[0] + (r * run_bytes + u * 64) * (2 / kElem));
+  }
+  for (int tile = 0, in_batch = 0; tile < tiles; ++tile) {
+    const int first_row = it.r0 + tile * sh.outs + sub * kOuts;
+    const bool mine = sub < subs && first_row < it.r1;   // the last tile may have fewer sub-tiles
+    float acc[kGroups][4];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[q][c] = 0.f;
+    const float *sc0 = nullptr, *sc1 = nullptr;   // e4m3: scales of the blocks of rows g and g + 8, or of row g
+    if constexpr (KIND == kE4) {
+      const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128;
+      const bool up = EIGHT && GATEUP && g >= 4;
+      sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((first_row + g - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
+      sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((first_row + g + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
+    }
+    for (int sl = 0; sl < (HOLD ? 1 : sh.slices); ++sl) {
+      const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
+      float f[kRuns][2];
+      if constexpr (KIND == kE4) {
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) {
+          const int at = sl * (sh.slice / 128) + r * parts;
+          f[r][0] = left > r * run_bytes ? __ldg(sc0 + at) : 0.f;
+          f[r][1] = EIGHT ? 0.f : left > r * run_bytes ? __ldg(sc1 + at) : 0.f;
+        }
+      }
+      if (ring.ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ring.ok = false;
+      ring.ok = __all_sync(0xffffffffu, ring.ok);
+      const uint8_t *slot = slots + ring.at * kSlot;
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        if (left <= r * run_bytes) break;
+        Weights v;
+        load_run<EIGHT>(v, slot + row0 + r * run_bytes, slot + row1 + r * run_bytes, swap, left - r * run_bytes);
+        const bool both = left - r * run_bytes > 64;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+          if (!HOLD && q >= groups) break;
+          float t[4] = {0.f, 0.f, 0.f, 0.f};
+          float (&to)[4] = KIND == kE4 ? t : acc[q];
+          const uint8_t *at = rows[q] + (sl * sh.slice + r * run_bytes) * (2 / kElem);
+          Acts<KIND> x;
+          if (HOLD && r < kHeld) x = held[r < kHeld ? r : 0][0];
+          else x.load(at);
+          step<KIND>(v.w[0], x, to);
+          if (both) {
+            if (HOLD && r < kHeld) x = held[r < kHeld ? r : 0][1];
+            else x.load(at + 64 * (2 / kElem));
+            step<KIND>(v.w[1], x, to);
+          }
+          if constexpr (KIND == kE4) {
+            acc[q][0] = fmaf(f[r][0], t[0], acc[q][0]);
+            acc[q][1] = fmaf(f[r][0], t[1], acc[q][1]);
+            acc[q][2] = fmaf(f[r][1], t[2], acc[q][2]);
+            acc[q][3] = fmaf(f[r][1], t[3], acc[q][3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && ring.ok) mbar_arrive(&s.empty[ring.at]);
+      ring.next();
+    }
+    float *dst = red + (((in_batch * subs + sub) * parts + part) * it.n + j) * 16 + g;
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q)
+      if (mine && 4 * q + j < it.n) {
+        dst[q * 64] = acc[q][0] + acc[q][1];
+        if (!EIGHT) dst[q * 64 + 8] = acc[q][2] + acc[q][3];
+      }
+    if (++in_batch != batch && tile + 1 < tiles) continue;
+    meet();
+    add_parts<KIND, GATEUP, EIGHT>(p, s, it, base, red, in_batch * subs, it.r0 + (tile + 1 - in_batch) * sh.outs);
+    in_batch = 0;
+    meet();
+  }
+}
+
+// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y
+template <int KIND, bool GATEUP>
+__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *red, const uint8_t *slots) {
+  const Plan &plan = s.plan[GATEUP ? 0 : 1];
+  const Shape &sh = p.shape[GATEUP ? 0 : 1];
+  int built = 0, base = 0;
+  for (int i = 0; i < plan.n_items; ++i) {
+    const Item &it = plan.item[i];
+    if (i >= built) {
+      meet();   // the last panel is read
+      built = build_panel<KIND, GATEUP>(p, s, plan, sh.K, panel, i);
+      base = 0;
+      meet();
+    }
+    const bool hold = it.n <= 4 && sh.slices == 1;
+    if (sh.eight) {
+      if (hold) run_tiles<KIND, GATEUP, true, true>(p, s, it, base, ring, panel, red, slots);
+      else run_tiles<KIND, GATEUP, true, false>(p, s, it, base, ring, panel, red, slots);
+    } else if (hold) {
+      run_tiles<KIND, GATEUP, false, true>(p, s, it, base, ring, panel, red, slots);
+    } else {
+      run_tiles<KIND, GATEUP, false, false>(p, s, it, base, ring, panel, red, slots);
+    }
+    base += it.n;
   }
 }
 
 // The rows of a product are dealt to the CTAs in equal numbers, in pairs of rows, over all active experts in a row; an expert's tokens
 // that the panel does not take at once go through in passes.
 __device__ void make_plan(Plan &plan, const Shared &s, int N, int cap) {
-  const int64_t units = (int64_t)s.n_active * (N / 2);
-  int64_t u = units * blockIdx.x / gridDim.x;
-  const int64_t end = units * (blockIdx.x + 1) / gridDim.x;
-  int n = 0, panel = 0, held = 0;
+  const unsigned half = N / 2, units = s.n_active * half;   // at most 128 x 20480, times the CTAs below 2^32
+  unsigned u = units * blockIdx.x / gridDim.x;
+  const unsigned end = units * (blockIdx.x + 1) / gridDim.x;
+  int n = 0, panel = 0, held = 0, most = 0, i = u / half;
   while (u < end) {
-    const int i = (int)(u / (N / 2)), e = s.active[i];
-    const int64_t stop = min(end, (int64_t)(i + 1) * (N / 2));
-    const int r0 = 2 * (int)(u - (int64_t)i * (N / 2)), r1 = r0 + 2 * (int)(stop - u), rows = __popc(s.mask[e]);
+    const unsigned begin = i * half, stop = min(end, begin + half);
+    const int e = s.active[i++], rows = __popc(s.mask[e]);
     for (int f = 0; f < rows && n < kMaxItems; f += cap) {
       const int c = min(cap, rows - f);
       if (held + c > cap) {
@@ -510,196 +642,255 @@ __device__ void make_plan(Plan &plan, const Shared &s, int N, int cap) {
         held = 0;
       }
       held += c;
-      plan.item[n++] = Item{e, r0, r1, f, c, panel};
+      most = max(most, held);
+      plan.item[n++] = Item{e, 2 * (int)(u - begin), 2 * (int)(stop - begin), f, c, panel};
     }
     u = stop;
   }
   plan.n_items = n;
-}
-
-// Parts of K: those that take a warp the fewest steps, of which whole blocks of kDepth count; of equals the fewest parts.
-__device__ __forceinline__ Split make_split(const Plan &plan, int rows_per_tile, int steps) {
-  int tiles = 0;
-  for (int i = 0; i < plan.n_items; ++i) tiles += (plan.item[i].r1 - plan.item[i].r0 + rows_per_tile - 1) / rows_per_tile;
-  Split sp{};
-  int best = 0x7fffffff;
-  constexpr int kParts[7] = {1, 2, 3, 4, 5, 8, 16};
-#pragma unroll
-  for (int j = 0; j < 7; ++j) {
-    const int parts = kParts[j], groups = kWarps / parts;
-    const int cost = ((tiles + groups - 1) / groups) * (((steps + parts - 1) / parts + kDepth - 1) / kDepth);
-    if (cost < best) {
-      best = cost;
-      sp.parts = parts;
-      sp.groups = groups;
-    }
-  }
-  const int warp = threadIdx.x >> 5;
-  sp.group = warp / sp.parts;
-  sp.part = warp - sp.group * sp.parts;
-  sp.s0 = steps * sp.part / sp.parts;
-  sp.s1 = steps * (sp.part + 1) / sp.parts;
-  return sp;
+  plan.rows = most;
 }
 
 // ---- stages 1 and 4 -----------------------------------------------------------------------------------------------------
 
+// four consecutive values; `vec`: at a 16-byte (two-byte types: 8-byte) boundary
+__device__ __forceinline__ float4 load4(const void *base, int dtype, int64_t i, bool vec) {
+  if (!vec) return make_float4(load_as_f32(base, dtype, i), load_as_f32(base, dtype, i + 1), load_as_f32(base, dtype, i + 2), load_as_f32(base, dtype, i + 3));
+  if (dtype == KNJ_DT_F32) return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i);
+  const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(base) + i);
+  if (dtype == KNJ_DT_BF16)
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ bool fours(const void *base, int64_t ld, int dtype) {
+  const int64_t unit = dtype == KNJ_DT_F32 ? 16 : 8;
+  return reinterpret_cast<uintptr_t>(base) % unit == 0 && ld * (dtype == KNJ_DT_F32 ? 4 : 2) % unit == 0;
+}
+__device__ __forceinline__ void store4(void *base, int dtype, int64_t i, bool vec, float4 v) {
+  if (!vec) {
+    store_from_f32(base, dtype, i, v.x);
+    store_from_f32(base, dtype, i + 1, v.y);
+    store_from_f32(base, dtype, i + 2, v.z);
+    store_from_f32(base, dtype, i + 3, v.w);
+    return;
+  }
+  if (dtype == KNJ_DT_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(base) + i) = v;
+    return;
+  }
+  uint2 u;
+  if (dtype == KNJ_DT_BF16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    u = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+  } else {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    u = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+  }
+  *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(base) + i) = u;
+}
+
 __device__ __forceinline__ float inverse_rms(float sum, int H, float eps) { return rsqrtf(fmaf(sum, 1.0f / (float)H, eps)); }
 
-// Statistics of all tokens' rows and the logits of this CTA's experts. A token is shared by 16 / (T rounded up to a power of two) warps.
+// Logits, and with the first experts' the statistics of the tokens' rows. The tokens x experts are dealt to the CTAs in squares of up to
+// four by four, for which 4 + 4 rows are read; a thread takes runs of four channels, so that all its loads go out together (a warp
+// per token over all of x in every CTA: 7 us at sixteen tokens).
+template <int SIDE>
 __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int per = p.T <= 1 ? 16 : p.T <= 2 ? 8 : p.T <= 4 ? 4 : p.T <= 8 ? 2 : 1;   // warps a token
-  const int t = warp / per, w = warp - t * per, e0 = blockIdx.x, e1 = blockIdx.x + gridDim.x;
-  float ss = 0.f, most = 0.f, d0 = 0.f, d1 = 0.f;
-  if (t < p.T) {
-    for (int c = w * 32 + lane; c < p.H / 8; c += per * 32) {
-      float v[8], g[8];
-      load8(p.x, p.x_dtype, t * p.ldx + 8 * c, p.x_vec, v);
-      if (p.pre_w) load8(p.pre_w, p.norm_dtype, 8 * c, true, g);
+  const int token_tiles = (p.T + SIDE - 1) / SIDE, expert_tiles = (p.E + SIDE - 1) / SIDE;
+  const bool x4 = fours(p.x, p.ldx, p.x_dtype);
+  for (int tile = blockIdx.x; tile < token_tiles * expert_tiles; tile += gridDim.x) {
+    const int t0 = tile % token_tiles * SIDE, e0 = tile / token_tiles * SIDE;
+    float ss[SIDE], most[SIDE], dot[SIDE][SIDE];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ss = fmaf(v[j], v[j], ss);
-        if (p.pre_w) v[j] *= g[j];
-        most = max3_abs_nan(most, v[j], 0.f);
-      }
-      if (e0 < p.E) {
-        load8(p.router, KNJ_DT_BF16, (int64_t)e0 * p.H + 8 * c, true, g);
+    for (int i = 0; i < SIDE; ++i) {
+      ss[i] = most[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d0 = fmaf(v[j], g[j], d0);
-      }
-      if (e1 < p.E) {
-        load8(p.router, KNJ_DT_BF16, (int64_t)e1 * p.H + 8 * c, true, g);
+      for (int k = 0; k < SIDE; ++k) dot[i][k] = 0.f;
+    }
+    for (int c = 4 * tid; c < p.H; c += 4 * kAll) {
+      float4 x[SIDE], n = make_float4(1.f, 1.f, 1.f, 1.f);
+      uint2 r[SIDE];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d1 = fmaf(v[j], g[j], d1);
+      for (int k = 0; k < SIDE; ++k) r[k] = *reinterpret_cast<const uint2 *>(p.router + (int64_t)min(e0 + k, p.E - 1) * p.H + c);
+#pragma unroll
+      for (int i = 0; i < SIDE; ++i) x[i] = load4(p.x, p.x_dtype, min(t0 + i, p.T - 1) * p.ldx + c, x4);
+      if (p.pre_w) n = load4(p.pre_w, p.norm_dtype, c, true);
+#pragma unroll
+      for (int i = 0; i < SIDE; ++i) {
+        float4 &v = x[i];
+        ss[i] = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, ss[i]))));
+        v = make_float4(v.x * n.x, v.y * n.y, v.z * n.z, v.w * n.w);
+        most[i] = max3_abs_nan(max3_abs_nan(most[i], v.x, v.y), v.z, v.w);
+#pragma unroll
+        for (int k = 0; k < SIDE; ++k)
+          dot[i][k] = fmaf(v.x, __uint_as_float(r[k].x << 16), fmaf(v.y, __uint_as_float(r[k].x & 0xffff0000u),
+                      fmaf(v.z, __uint_as_float(r[k].y << 16), fmaf(v.w, __uint_as_float(r[k].y & 0xffff0000u), dot[i][k]))));
       }
     }
-  }
-  ss = warp_sum(ss);
-  d0 = warp_sum(d0);
-  d1 = warp_sum(d1);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (lane == 0) {
-    s.part[warp][0] = ss;
-    s.part[warp][1] = most;
-    s.part[warp][2] = d0;
-    s.part[warp][3] = d1;
-  }
-  __syncthreads();
-  if (warp < p.T) {   // a warp per token: a large row's squares are summed once more
-    float tot = 0.f, m = 0.f, a = 0.f, b = 0.f;
-    for (int i = 0; i < per; ++i) {
-      tot += s.part[warp * per + i][0];
-      m = max_nan(m, s.part[warp * per + i][1]);
-      a += s.part[warp * per + i][2];
-      b += s.part[warp * per + i][3];
+    for (int i = 0; i < SIDE; ++i) {
+      ss[i] = warp_sum(ss[i]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most[i] = max_nan(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) dot[i][k] = warp_sum(dot[i][k]);
     }
-    float inv = 1.0f, down = 1.0f;
+    __syncthreads();   // the last tile's sums are read
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < SIDE; ++i) {
+        s.part[warp][i][0] = ss[i];
+        s.part[warp][i][1] = most[i];
+#pragma unroll
+        for (int k = 0; k < SIDE; ++k) s.part[warp][i][2 + k] = dot[i][k];
+      }
+    }
+    __syncthreads();
+    const int i = warp, t = t0 + i;   // a warp per token, lane l the sum of value l
+    if (i >= SIDE || t >= p.T) continue;
+    float v = 0.f;
+    if (lane < 2 + SIDE)
+      for (int w = 0; w < kAll / 32; ++w) v = lane == 1 ? max_nan(v, s.part[w][i][1]) : v + s.part[w][i][lane];
+    const float tot = __shfl_sync(0xffffffffu, v, 0), m = __shfl_sync(0xffffffffu, v, 1);
+    float inv = 1.0f;
     if (p.pre_w) {
       if (tot > 3.402823466e38f) {   // squares of a large row left the range: from values * 2^-64, where eps does not count
         float q = 0.f;
         for (int c = lane; c < p.H; c += 32) {
-          const float v = load_as_f32(p.x, p.x_dtype, warp * p.ldx + c) * kDown;
-          q = fmaf(v, v, q);
+          const float f = load_as_f32(p.x, p.x_dtype, t * p.ldx + c) * kDown;
+          q = fmaf(f, f, q);
         }
         inv = kDown * rsqrtf(warp_sum(q) * (1.0f / (float)p.H));
       } else {
         inv = inverse_rms(tot, p.H, p.eps);
       }
     }
-    if (lane == 0) {
-      s.inv[warp] = inv;
-      row_power(m * inv, s.mult[warp], s.unmult[warp]);
-      if (e0 < p.E) p.logits[warp * p.E + e0] = a * inv + (p.router_bias ? p.router_bias[e0] : 0.f);
-      if (e1 < p.E) p.logits[warp * p.E + e1] = b * inv + (p.router_bias ? p.router_bias[e1] : 0.f);
-    }
+    const int e = e0 + lane - 2;
+    if (lane >= 2 && lane < 2 + SIDE && e < p.E) p.logits[t * p.E + e] = v * inv + (p.router_bias ? p.router_bias[e] : 0.f);
+    if (e0 == 0 && lane == 0) p.stats[t] = make_float2(inv, m * inv);
   }
-}
-
-__device__ __forceinline__ float gate_value(const DecodeParams &p, int t, int i) {
-  if (p.gate_kind == KNJ_GATE_NONE) return 1.0f;
-  const float g = load_as_f32(p.gate, p.gate_dtype, p.gate_kind == KNJ_GATE_CHANNEL ? i : p.gate_kind == KNJ_GATE_ROW ? t * p.ldg : t * p.ldg + i);
-  return p.gate_sigmoid ? 1.0f / (1.0f + expf(-g)) : g;
 }
 
 // sum of squares of the row in shared memory and its inverse norm; a large row once more
-__device__ __forceinline__ float row_inverse(const float *row, int H, float ss, float eps, float (*red)[kWarps]) {
+__device__ __forceinline__ float row_inverse(const float *row, int H, float ss, float eps, float (*red)[kAll / 32]) {
   const float tot = cta_sum(ss, red[0]);
   if (!(tot > 3.402823466e38f)) return inverse_rms(tot, H, eps);
   float q = 0.f;
-  for (int i = threadIdx.x; i < H; i += kThreads) q = fmaf(row[i] * kDown, row[i] * kDown, q);
+  for (int i = threadIdx.x; i < H; i += kAll) q = fmaf(row[i] * kDown, row[i] * kDown, q);
   return kDown * rsqrtf(cta_sum(q, red[1]) * (1.0f / (float)H));
 }
 
-// One token's row: the pairs' rows in ascending order of their experts, then what stands behind the block.
-__device__ __forceinline__ void finish_row(const DecodeParams &p, Shared &s, int t, float *row) {
-  const int tid = threadIdx.x, H = p.H;
-  int order[kMaxK];
+// What stands behind the experts, of one token: a thread holds runs of four channels, the first of them with all that does not depend on
+// the experts read in front of the last barrier (prepare).
+struct Finish {
+  int order[kMaxK];      // pairs in ascending order of their experts
   float weight[kMaxK];
-#pragma unroll
-  for (int i = 0; i < kMaxK; ++i) order[i] = 0, weight[i] = 0.f;
-  for (int j = 0; j < p.k; ++j) {
-    int rank = 0;
-    for (int i = 0; i < p.k; ++i) rank += s.sel_e[t][i] < s.sel_e[t][j];
-#pragma unroll
-    for (int i = 0; i < kMaxK; ++i)
-      if (i == rank) order[i] = j, weight[i] = s.sel_w[t][j];
-  }
-  float ss = 0.f;
-  for (int i = tid; i < H; i += kThreads) {
-    float y = 0.f, v[kMaxK];
-#pragma unroll
-    for (int j = 0; j < kMaxK; ++j) v[j] = j < p.k ? __ldcg(p.Y + ((int64_t)t * p.k + order[j]) * H + i) : 0.f;
-#pragma unroll
-    for (int j = 0; j < kMaxK; ++j)
-      if (j < p.k) y = __fadd_rn(y, __fmul_rn(weight[j], v[j]));
-    row[i] = y;
-    ss = fmaf(y, y, ss);
-  }
-  float inv = 1.0f;
-  if (p.post_w) inv = row_inverse(row, H, ss, p.eps, s.red);
-  __syncthreads();
-  ss = 0.f;
-  for (int i = tid; i < H; i += kThreads) {
-    float n = row[i];
-    if (p.post_w) n = n * inv * load_as_f32(p.post_w, p.norm_dtype, i);
-    const float v = p.beta * load_as_f32(p.x, p.x_dtype, t * p.ldx + i) + p.alpha * gate_value(p, t, i) * n;
-    row[i] = v;
-    ss = fmaf(v, v, ss);
-    store_from_f32(p.out, p.out_dtype, t * p.ldo + i, v);
-  }
-  if (!p.next_w) return;
-  inv = row_inverse(row, H, ss, p.eps, s.red);
-  __syncthreads();
-  if (p.h_dtype != KNJ_DT_E4M3) {
-    for (int i = tid; i < H; i += kThreads) store_from_f32(p.h_next, p.h_dtype, t * p.ldh + i, row[i] * inv * load_as_f32(p.next_w, p.norm_dtype, i));
-    return;
-  }
-  const int lane = tid & 31, groups = H / kFp8Group;
-  for (int g = tid >> 5; g < groups; g += kWarps) {
-    float v[4], most = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = g * kFp8Group + 32 * j + lane;
-      v[j] = row[i] * inv * load_as_f32(p.next_w, p.norm_dtype, i);
-      most = max3_abs_nan(most, v[j], 0.f);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const Fp8Scale sc = fp8_scale(most);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      static_cast<uint8_t *>(p.h_next)[t * p.ldh + g * kFp8Group + 32 * j + lane] = (uint8_t)e4m3_pair(v[j] * sc.inverse, 0.f);
-    if (lane == 0) p.h_next_scale[(int64_t)t * groups + g] = sc.scale;
-  }
-}
+  float4 x, post, gate, next;
 
-// a wait gave up: NaN in the rows that this CTA would have written
-__device__ void give_up(const DecodeParams &p) {
+  __device__ __forceinline__ void load(const DecodeParams &p, int t, int c) {
+    x = load4(p.x, p.x_dtype, t * p.ldx + c, fours(p.x, p.ldx, p.x_dtype));
+    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+    post = p.post_w ? load4(p.post_w, p.norm_dtype, c, fours(p.post_w, 0, p.norm_dtype)) : one;
+    next = p.next_w ? load4(p.next_w, p.norm_dtype, c, fours(p.next_w, 0, p.norm_dtype)) : one;
+    gate = one;
+    if (p.gate_kind == KNJ_GATE_NONE) return;
+    if (p.gate_kind == KNJ_GATE_ROW) {
+      const float g = load_as_f32(p.gate, p.gate_dtype, t * p.ldg);
+      gate = make_float4(g, g, g, g);
+    } else {
+      const bool full = p.gate_kind == KNJ_GATE_FULL;
+      gate = load4(p.gate, p.gate_dtype, full ? t * p.ldg + c : c, fours(p.gate, full ? p.ldg : 0, p.gate_dtype));
+    }
+    if (p.gate_sigmoid)
+      gate = make_float4(1.0f / (1.0f + expf(-gate.x)), 1.0f / (1.0f + expf(-gate.y)), 1.0f / (1.0f + expf(-gate.z)), 1.0f / (1.0f + expf(-gate.w)));
+  }
+  __device__ __forceinline__ void prepare(const DecodeParams &p, const Shared &s, int t) {
+#pragma unroll
+    for (int i = 0; i < kMaxK; ++i) order[i] = 0, weight[i] = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+      int rank = 0;
+      for (int i = 0; i < p.k; ++i) rank += s.sel_e[t][i] < s.sel_e[t][j];
+#pragma unroll
+      for (int i = 0; i < kMaxK; ++i)
+        if (i == rank) order[i] = j, weight[i] = s.sel_w[t][j];
+    }
+    if (4 * threadIdx.x < p.H) load(p, t, 4 * threadIdx.x);
+  }
+  // row: H values in shared memory, of which a thread reads only its own (e4m3 rows: all)
+  __device__ __forceinline__ void run(const DecodeParams &p, Shared &s, int t, float *row) {
+    const int first = 4 * threadIdx.x, H = p.H;
+    constexpr int kStride = 4 * kAll;
+    float ss = 0.f;
+    for (int c = first; c < H; c += kStride) {
+      float4 v[kMaxK], y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kMaxK; ++j)
+        if (j < p.k) v[j] = __ldcg(reinterpret_cast<const float4 *>(p.Y + ((int64_t)t * p.k + order[j]) * H + c));
+#pragma unroll
+      for (int j = 0; j < kMaxK; ++j)
+        if (j < p.k) {
+          y.x = fmaf(weight[j], v[j].x, y.x);
+          y.y = fmaf(weight[j], v[j].y, y.y);
+          y.z = fmaf(weight[j], v[j].z, y.z);
+          y.w = fmaf(weight[j], v[j].w, y.w);
+        }
+      *reinterpret_cast<float4 *>(row + c) = y;
+      ss = fmaf(y.x, y.x, fmaf(y.y, y.y, fmaf(y.z, y.z, fmaf(y.w, y.w, ss))));
+    }
+    const float inv = p.post_w ? row_inverse(row, H, ss, p.eps, s.red) : 1.0f;
+    const bool out4 = fours(p.out, p.ldo, p.out_dtype);
+    ss = 0.f;
+    for (int c = first; c < H; c += kStride) {
+      if (c != first) load(p, t, c);
+      float4 v = *reinterpret_cast<const float4 *>(row + c);
+      v.x = fmaf(p.beta, x.x, p.alpha * gate.x * (v.x * inv * post.x));
+      v.y = fmaf(p.beta, x.y, p.alpha * gate.y * (v.y * inv * post.y));
+      v.z = fmaf(p.beta, x.z, p.alpha * gate.z * (v.z * inv * post.z));
+      v.w = fmaf(p.beta, x.w, p.alpha * gate.w * (v.w * inv * post.w));
+      store4(p.out, p.out_dtype, t * p.ldo + c, out4, v);
+      *reinterpret_cast<float4 *>(row + c) = v;
+      ss = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, ss))));
+    }
+    if (!p.next_w) return;
+    const float inv2 = row_inverse(row, H, ss, p.eps, s.red + 2);
+    const bool codes = p.h_dtype == KNJ_DT_E4M3, h4 = !codes && fours(p.h_next, p.ldh, p.h_dtype);
+    for (int c = first; c < H; c += kStride) {   // 32 threads in a row hold a group of 128 values
+      if (H > kStride) next = load4(p.next_w, p.norm_dtype, c, fours(p.next_w, 0, p.norm_dtype));
+      float4 v = *reinterpret_cast<const float4 *>(row + c);
+      v = make_float4(v.x * inv2 * next.x, v.y * inv2 * next.y, v.z * inv2 * next.z, v.w * inv2 * next.w);
+      if (!codes) {
+        store4(p.h_next, p.h_dtype, t * p.ldh + c, h4, v);
+        continue;
+      }
+      float most = max3_abs_nan(max3_abs_nan(0.f, v.x, v.y), v.z, v.w);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const Fp8Scale sc = fp8_scale(most);
+      const uint32_t lo = e4m3_pair(v.x * sc.inverse, v.y * sc.inverse), hi = e4m3_pair(v.z * sc.inverse, v.w * sc.inverse);
+      uint8_t *at = static_cast<uint8_t *>(p.h_next) + t * p.ldh + c;
+      if ((reinterpret_cast<uintptr_t>(p.h_next) | (uintptr_t)p.ldh) % 4 == 0) {
+        *reinterpret_cast<uint32_t *>(at) = lo | hi << 16;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at[j] = (uint8_t)((lo | hi << 16) >> (8 * j));
+      }
+      if ((threadIdx.x & 31) == 0) p.h_next_scale[(int64_t)t * (H / kFp8Group) + c / kFp8Group] = sc.scale;
+    }
+  }
+};
+
+// A wait gave up: the others are told, and the rows that this CTA would have written are NaN. 
+__device__ void give_up(const DecodeParams &p, Shared &s) {
+  if (threadIdx.x == 0) {
+    *reinterpret_cast<volatile int *>(&s.fail) = 1;
+    atomicExch(p.sync + 1, 1u);
+    atomicExch(p.status, 1);
+  }
   const float nan = __int_as_float(0x7fffffff);
   for (int t = blockIdx.x; t < p.T; t += gridDim.x) {
-    for (int i = threadIdx.x; i < p.H; i += kThreads) {
+    for (int i = threadIdx.x; i < p.H; i += kAll) {
       store_from_f32(p.out, p.out_dtype, t * p.ldo + i, nan);
       if (p.next_w) {
         if (p.h_dtype == KNJ_DT_E4M3) static_cast<uint8_t *>(p.h_next)[t * p.ldh + i] = 0x7f;
@@ -707,25 +898,35 @@ __device__ void give_up(const DecodeParams &p) {
       }
     }
     if (p.next_w && p.h_dtype == KNJ_DT_E4M3)
-      for (int g = threadIdx.x; g < p.H / kFp8Group; g += kThreads) p.h_next_scale[(int64_t)t * (p.H / kFp8Group) + g] = nan;
+      for (int g = threadIdx.x; g < p.H / kFp8Group; g += kAll) p.h_next_scale[(int64_t)t * (p.H / kFp8Group) + g] = nan;
   }
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t *panel = smem;
-  float4 *red = reinterpret_cast<float4 *>(smem + kPanel);
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (blockIdx.x == 0 && tid == 0) *p.status = 0;   // in front of the first barrier, behind which alone it is raised
-  norms_and_logits(p, s);
-  for (int e = tid; e < kMaxExperts; e += kThreads) s.mask[e] = 0u;
-  if (!grid_barrier(p, s, 1)) return give_up(p);
+  if (tid < kMaxExperts) s.mask[tid] = 0u;
+  if (tid == 0) {
+    for (int i = 0; i < kMaxSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], kWarps);
+    }
+    s.fail = 0;
+    mbar_init_fence();
+  }
+  if (p.T == 1) norms_and_logits<1>(p, s);
+  else if (p.T <= 4) norms_and_logits<2>(p, s);
+  else norms_and_logits<4>(p, s);
+  grid_arrive<kAll>(p, s);
+  if (!grid_wait<kAll>(p, s, 1)) return give_up(p, s);
 
   // ---- routing: a warp per token ----
   if (warp < p.T) {
+    const float2 st = __ldcg(p.stats + warp);
     int e;
     float w;
     warp_topk(p.logits + warp * p.E, p.E, p.k, lane, e, w);
@@ -736,8 +937,16 @@ __global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_co
       if (blockIdx.x == 0 && p.tap_exp) p.tap_exp[warp * p.k + lane] = e;
       if (blockIdx.x == 0 && p.tap_w) p.tap_w[warp * p.k + lane] = w;
     }
+    if (lane == 0) {
+      s.inv[warp] = st.x;
+      row_power(st.y, s.mult[warp], s.unmult[warp]);
+    }
   }
   __syncthreads();
+  if (warp < p.T && lane < p.k) {
+    const int e = s.sel_e[warp][lane];
+    s.pair_at[e][__popc(s.mask[e] & ((1u << warp) - 1u))] = (uint8_t)(warp * p.k + lane);
+  }
   if (warp == 0) {
     int n = 0;
     for (int b = 0; b < kMaxExperts; b += 32) {
@@ -752,23 +961,50 @@ __global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_co
   }
   __syncthreads();
 
-  constexpr int kElem = Geo<KIND>::kElem;
-  Product<KIND, true> up{p, s.plan[0], make_split(s.plan[0], 8, (p.H * kElem + 63) / 64), p.H, p.F, p.H * kElem, lane};
-  Feed<KIND, true> feed_up;
-  up.start(feed_up);
-  run_product<KIND, true>(p, s, up, feed_up, panel, red);
-  Product<KIND, false> down{p, s.plan[1], make_split(s.plan[1], 16, (p.F * kElem + 63) / 64), p.F, p.H, p.F * kElem, lane};
-  Feed<KIND, false> feed_down;
-  down.start(feed_down);   // the first weights of the down matrices travel while the grid meets
-  if (!grid_barrier(p, s, 2)) return give_up(p);
-  run_product<KIND, false>(p, s, down, feed_down, panel, red);
-  if (!grid_barrier(p, s, 3)) return give_up(p);
-  for (int t = blockIdx.x; t < p.T; t += gridDim.x) finish_row(p, s, t, reinterpret_cast<float *>(panel));
+  float *red = reinterpret_cast<float *>(smem);
+  uint8_t *panel = smem + kRed;
+  const int held = max(s.plan[0].rows * 2 * Geo<KIND>::pitch(p.H), s.plan[1].rows * 2 * Geo<KIND>::pitch(p.F));
+  const int at = kRed + (held + 127) / 128 * 128;
+  uint8_t *slots = smem + at;
+  Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u, true};
+  const int t = blockIdx.x;
+  Finish end;
+  if (warp == kWarps) {
+    int copied = 0;
+    if (!feed(p, s, 0, ring, slots, copied) || !feed(p, s, 1, ring, slots, copied)) {
+      // the slots filled last may still be written: shared memory is not left before they are
+      if (lane < ring.n && copied > lane) mbar_wait_for(&s.full[lane], (uint32_t)((copied - lane - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
+    }
+    if (t < p.T) end.prepare(p, s, t);
+  } else {
+    run_product<KIND, true>(p, s, ring, panel, red, slots);
+    grid_arrive<kThreads>(p, s);
+    if (grid_wait<kThreads>(p, s, 2)) {
+      run_product<KIND, false>(p, s, ring, panel, red, slots);
+      grid_arrive<kThreads>(p, s);
+      if (t < p.T) end.prepare(p, s, t);
+      grid_wait<kThreads>(p, s, 3);
+    }
+    if (!s.ok && tid == 0) *reinterpret_cast<volatile int *>(&s.fail) = 1;   // ends the copying warp's waits
+  }
+  __syncthreads();
+  if (!s.ok) return give_up(p, s);
+  if (t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
 }
 
 template <int KIND>
 int launch(DecodeParams &p, cudaStream_t st) {
-  constexpr int kSmem = kPanel + kRed;
+  for (int i = 0; i < 2; ++i) {
+    Shape &sh = p.shape[i];
+    sh.K = i == 0 ? p.H : p.F;
+    sh.N = i == 0 ? p.F : p.H;
+    sh.row_bytes = sh.K * Geo<KIND>::kElem;
+    sh.slices = (sh.row_bytes + kSlice - 1) / kSlice;
+    sh.slice = sh.slices == 1 ? sh.row_bytes : ((sh.row_bytes + sh.slices - 1) / sh.slices + 127) / 128 * 128;
+    sh.eight = sh.row_bytes > kSlice / 2;
+    sh.subs = sh.row_bytes <= kSlice / 8 ? 4 : sh.row_bytes <= kSlice / 4 ? 2 : 1;
+    sh.outs = (i == 0 ? 8 : 16) * sh.subs / (sh.eight ? 2 : 1);
+  }
   int dev = 0;
   KNJ_CUDA(cudaGetDevice(&dev));
   auto kern = moe_decode_kernel<KIND>;
@@ -777,9 +1013,9 @@ int launch(DecodeParams &p, cudaStream_t st) {
     KNJ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     opted[dev] = true;
   }
-  KNJ_CUDA(cudaMemsetAsync(p.sync, 0, 8, st));
+  KNJ_CUDA(cudaMemsetAsync(p.sync, 0, kCleared, st));
   void *args[] = {&p};
-  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kThreads), args, kSmem, st));
+  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kAll), args, kSmem, st));
   return launch_status("moe_decode_kernel");
 }
 
@@ -789,7 +1025,7 @@ namespace knj {
 size_t moe_decode_workspace(int T, int H, int F, int E, int k) {
   auto up256 = [](size_t n) { return (n + 255) & ~(size_t)255; };
   const size_t P = (size_t)T * k;
-  return 256 + up256((size_t)T * E * 4) + up256(P * F * 4) + up256(P * H * 4);
+  return kHead + up256((size_t)T * E * 4) + up256(P * F * 4) + up256(P * H * 4);
 }
 
 int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t stream) {
@@ -805,8 +1041,10 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   p.s_gate = a->gate_scale; p.s_up = a->up_scale; p.s_down = a->down_scale; p.out = a->out; p.h_next = a->h_next; p.h_next_scale = a->h_next_scale;
   p.tap_exp = a->tap_pair_exp; p.tap_w = a->tap_pair_w;
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
-  p.sync = reinterpret_cast<unsigned *>(ws + 128);   // behind the status word of the whole block
-  ws += 256;
+  p.sync = reinterpret_cast<unsigned *>(ws + kSyncAt);   // behind the status word of the whole block
+  p.row_max = reinterpret_cast<unsigned *>(ws + kMaxAt);
+  p.stats = reinterpret_cast<float2 *>(ws + kStatsAt);
+  ws += kHead;
   p.logits = reinterpret_cast<float *>(ws);
   ws += up256((size_t)T * E * 4);
   p.act = reinterpret_cast<float *>(ws);
