@@ -8,11 +8,11 @@
 // (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). In mma.sync.m16n8k16 sixteen matrix rows
 // meet the two planes of four tokens, so that the second plane costs nothing while a step's weights are on their way.
 //
-// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
-// its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
-// multiply. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep HBM
-// busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both operands
-// have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
+// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. This CTA's
+// matrix rows, of gate and up and behind them of down, stream through a ring in shared memory, which one of the sixteen warps fills between
+// its products. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep
+// HBM busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both
+// operands have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
 //
 // Stages, with a barrier over the grid between them:
 //   1  norm statistics (every CTA, all tokens) and router logits (an expert or two a CTA)
@@ -20,6 +20,8 @@
 //   3  down, likewise
 //   4  weighted sum, norm, gate, residual, next norm: a CTA for each token
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
+#include <type_traits>
+
 #include "knj_fp8.cuh"
 #include "knj_topk.cuh"
 
@@ -27,17 +29,18 @@ using namespace knj;
 
 namespace {
 
+constexpr int kMaxRows = 8;   // of activations in the panel at a time: two groups of four
 constexpr int kMaxTokens = KNJ_MOE_DECODE_MAX_TOKENS, kMaxK = 8, kMaxExperts = 256;
-// Sixteen warps with 128 registers a thread: fifteen that multiply and one that copies. (With sixteen that multiply a thread has 96, and the
-// shared memory that the ring takes leaves no L1 for what then spills: every spilled word came back from L2, 1000 cycles under load.)
-constexpr int kWarps = 15, kThreads = 32 * kWarps, kAll = kThreads + 32;
+// 128 registers a thread. (With a seventeenth warp that copies a thread has 96, and the shared memory that the ring takes leaves no L1 for
+// what then spills: every spilled word came back from L2, 1000 cycles under load.)
+constexpr int kThreads = 512, kWarps = kThreads / 32, kFiller = kWarps - 1;   // kFiller: the warp that fills the ring
 // A slot of the ring holds a tile: 64, 32, 16 or 8 matrix rows of up to 512, 1024, 2048 or 4096 bytes as they lie, in one or two copies.
 // (A copy for each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536.) Longer rows
 // come in slices of up to 4096 bytes, eight rows to a slot.
 constexpr int kSlice = 4096;
 constexpr int kSlot = 8 * kSlice;
 constexpr int kMaxSlots = 6;
-constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 64 a tile, warp and token
+constexpr int kRed = 8 * 1024;                // bytes of the sums of a batch of tiles: 1 KB a tile and token; there are two, in turn
 constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
 constexpr int kMaxItems = 64;
 constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256,
@@ -51,7 +54,7 @@ struct Shape {
   int K, N, row_bytes;
   int slices, slice;   // of a row, bytes
   int eight;           // tiles of eight rows, else of 16 a sub-tile
-  int subs;            // sub-tiles of a tile, each of which has 15 / subs warps
+  int subs;            // sub-tiles of a tile, each of which has 16 / subs warps
   int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
 };
 
@@ -74,6 +77,7 @@ struct DecodeParams {
   int64_t ldx, ldo, ldg, ldh;
   int T, H, F, E, k;
   int x_dtype, out_dtype, norm_dtype, gate_dtype, h_dtype, gate_kind, gate_sigmoid;
+  unsigned grid_inverse;        // 2^32 / CTAs, rounded down
   int x_vec;                    // rows of x are whole 16-byte units
   float alpha, beta, eps;
   long long wait_cycles;
@@ -90,10 +94,18 @@ struct Plan {
   int n_items, rows;            // rows: most that are in the panel at a time
 };
 
+// the next tile (or slice of one) to copy
+struct Cursor {
+  int product, item, row, slice;
+  int slot, copied;   // copied: slots filled so far
+  uint32_t parity;    // of the slot's barrier once it is read
+};
+
 struct Shared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
+  Cursor next;                  // of the warp that fills the ring
   int fail;                     // raised by a wait that gave up; read as volatile
-  float part[kAll / 32][4][6];  // of a token: squares, largest, dot products
+  float part[kWarps][4][6];  // of a token: squares, largest, dot products
   float inv[kMaxTokens], mult[kMaxTokens], unmult[kMaxTokens];
   int sel_e[kMaxTokens][kMaxK];
   float sel_w[kMaxTokens][kMaxK];
@@ -104,7 +116,7 @@ struct Shared {
   Plan plan[2];                 // gate and up, down
   int row_tok[kMaxTokens], row_pair[kMaxTokens];        // of the panel's rows
   float row_mult[kMaxTokens], row_unmult[kMaxTokens];
-  float red[4][kAll / 32];
+  float red[4][kWarps];
 };
 
 static_assert(kSmem + sizeof(Shared) <= 227 * 1024, "shared memory of a block");
@@ -116,22 +128,13 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-// of the warps that multiply
-__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-template <int N>
-__device__ __forceinline__ void cta_barrier() {
-  if constexpr (N == kAll) __syncthreads();
-  else meet();
-}
-// Barrier over the grid, number `n` of the launch, in two halves, met by the first N threads of every CTA. A CTA in which a wait has given
-// up never arrives; grid_wait is false for all threads where the barrier did not complete in time.
-template <int N>
+// Barrier over the grid, number `n` of the launch, in two halves. A CTA in which a wait has given up never arrives; grid_wait is false for
+// all threads where the barrier did not complete in time.
 __device__ __forceinline__ void grid_arrive(const DecodeParams &p, Shared &s) {
-  cta_barrier<N>();
+  __syncthreads();
   if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0)
     asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.sync), "r"(1u) : "memory");
 }
-template <int N>
 __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int n) {
   if (threadIdx.x == 0) {
     int ok = *reinterpret_cast<volatile int *>(&s.fail) == 0;
@@ -142,7 +145,7 @@ __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int 
     }
     s.ok = ok;
   }
-  cta_barrier<N>();
+  __syncthreads();
   return s.ok != 0;
 }
 
@@ -244,7 +247,7 @@ __device__ __forceinline__ float cta_sum(float v, float *red) {   // by all thre
   __syncthreads();
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kAll / 32; ++i) t += red[i];
+  for (int i = 0; i < kWarps; ++i) t += red[i];
   return t;
 }
 
@@ -255,8 +258,8 @@ struct Geo {
   __host__ __device__ static int pitch(int K) { return (2 * K + 127) / 128 * 128 + (kElem == 2 ? 64 : 16); }
   // rows in the panel at a time: what leaves the ring two slots, or one
   __host__ __device__ static int cap(int K) {
-    const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
-    return c < 1 ? 1 : c < kMaxTokens ? c : kMaxTokens;
+    const int c = (kSmem - 2 * kRed - 2 * kSlot) / (2 * pitch(K));
+    return c < 1 ? 1 : c < kMaxRows ? c : kMaxRows;
   }
 };
 
@@ -266,8 +269,11 @@ struct Geo {
 struct Ring {
   int at, n;
   uint32_t parity;
-  bool ok;     // of the warps that multiply: no wait has given up
+  int read;    // slots read so far
+  int turn;    // of the two places for sums
+  bool ok;     // no wait has given up
   __device__ __forceinline__ void next() {
+    ++read;
     if (++at == n) {
       at = 0;
       parity ^= 1u;
@@ -275,34 +281,60 @@ struct Ring {
   }
 };
 
-// The copying warp's side of a product. False after a wait that gave up.
-__device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int product, Ring &ring, uint8_t *slots, int &copied) {
+// By the warp that fills the ring: copies tiles into its free slots; with `must`, waits until at least `must` slots in all have been filled.
+// False after a wait that gave up.
+__device__ __forceinline__ bool fill(const DecodeParams &p, Shared &s, uint8_t *slots, int n_slots, int must) {
   const int lane = threadIdx.x & 31;
-  const Shape &sh = p.shape[product];
-  const Plan &plan = s.plan[product];
-  const bool up = product == 0, whole = sh.slices == 1;
-  for (int i = 0; i < plan.n_items; ++i) {
-    const Item it = plan.item[i];
-    for (int first = it.r0; first < it.r1; first += sh.outs) {
-      const int rows = min(sh.outs, it.r1 - first);
-      // lane l copies the rows of matrix l, or row l % rows of matrix l / rows
-      const int second = up && (whole ? lane == 1 : lane >= rows), r = whole ? 0 : lane - second * rows;
-      const bool mine = lane < (whole ? 1 : rows) * (up ? 2 : 1);
-      const uint8_t *src = (up ? (second ? p.w_up : p.w_gate) : p.w_down) + ((int64_t)it.expert * sh.N + first + r) * sh.row_bytes;
-      const int dst = (second * sh.outs + r) * sh.slice;
-      for (int sl = 0; sl < sh.slices; ++sl) {
-        const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - sl * sh.slice);
-        const bool ok = mbar_wait_for(&s.empty[ring.at], ring.parity ^ 1u, p.wait_cycles, &s.fail);
-        if (!__all_sync(0xffffffffu, ok)) return false;
-        if (lane == 0) mbar_expect_tx(&s.full[ring.at], (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
-        __syncwarp();
-        if (mine) bulk_g2s(slots + ring.at * kSlot + dst, src + sl * sh.slice, (uint32_t)bytes, &s.full[ring.at]);
-        ring.next();
-        ++copied;
+  Cursor c = s.next;
+  bool ok = true;
+  while (c.product < 2) {
+    uint64_t *free = &s.empty[c.slot];
+    bool there = mbar_try_wait(free, c.parity ^ 1u);
+    if (!__all_sync(0xffffffffu, there)) {
+      if (c.copied >= must) break;
+      there = mbar_wait_for(free, c.parity ^ 1u, p.wait_cycles, &s.fail);
+      if (!__all_sync(0xffffffffu, there)) {
+        ok = false;
+        break;
+      }
+    }
+    const bool up = c.product == 0;
+    const Shape &sh = p.shape[c.product];
+    const Plan &plan = s.plan[c.product];
+    const Item &it = plan.item[c.item];
+    const int rows = min(sh.outs, it.r1 - c.row);
+    // lane l copies the rows of matrix l, or row l % rows of matrix l / rows
+    const bool whole = sh.slices == 1;
+    const int second = up && (whole ? lane == 1 : lane >= rows), r = whole ? 0 : lane - second * rows;
+    const uint8_t *w = up ? (second ? p.w_up : p.w_gate) : p.w_down;
+    const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - c.slice * sh.slice);
+    uint64_t *bar = &s.full[c.slot];
+    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
+    __syncwarp();
+    if (lane < (whole ? 1 : rows) * (up ? 2 : 1))
+      bulk_g2s(slots + c.slot * kSlot + (second * sh.outs + r) * sh.slice, w + ((int64_t)it.expert * sh.N + c.row + r) * sh.row_bytes + c.slice * sh.slice,
+               (uint32_t)bytes, bar);
+    ++c.copied;
+    if (++c.slot == n_slots) {
+      c.slot = 0;
+      c.parity ^= 1u;
+    }
+    if (++c.slice == sh.slices) {
+      c.slice = 0;
+      c.row += sh.outs;
+      if (c.row >= it.r1) {
+        if (++c.item == plan.n_items) {
+          c.item = 0;
+          c.product = up && s.plan[1].n_items > 0 ? 1 : 2;
+        }
+        if (c.product < 2) c.row = s.plan[c.product].item[c.item].r0;
       }
     }
   }
-  return true;
+  __syncwarp();
+  if (lane == 0) s.next = c;
+  __syncwarp();
+  return ok;
 }
 
 // A lane's part of a run of 128 bytes (two steps of 64): of rows g and g + 8, or of row g of eight, the bytes 16 j .. + 15 of either step.
@@ -340,25 +372,40 @@ struct Acts {
     b[0] = *reinterpret_cast<const uint4 *>(at);
     if constexpr (KIND > kF16) b[1] = *reinterpret_cast<const uint4 *>(at + 16);
   }
+  __device__ __forceinline__ void clear() {
+    b[0] = make_uint4(0, 0, 0, 0);
+    if constexpr (KIND > kF16) b[1] = b[0];
+  }
 };
-// One step of sixteen rows times the planes of four tokens
+// One step of sixteen rows as MMA operands, and its products with the planes of four tokens
 template <int KIND>
-__device__ __forceinline__ void step(const uint4 (&w)[2], const Acts<KIND> &x, float (&acc)[4]) {
-  if constexpr (KIND <= kF16) {
-    mma<KIND>(acc, w[0].x, w[1].x, w[0].y, w[1].y, x.b[0].x, x.b[0].y);
-    mma<KIND>(acc, w[0].z, w[1].z, w[0].w, w[1].w, x.b[0].z, x.b[0].w);
-  } else {
-    const uint32_t r0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, r1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
-    const uint32_t b[8] = {x.b[0].x, x.b[0].y, x.b[0].z, x.b[0].w, x.b[1].x, x.b[1].y, x.b[1].z, x.b[1].w};
+struct Step {
+  uint32_t a[KIND <= kF16 ? 2 : 4][4];
+  __device__ __forceinline__ explicit Step(const uint4 (&w)[2]) {
+    if constexpr (KIND <= kF16) {
+      a[0][0] = w[0].x; a[0][1] = w[1].x; a[0][2] = w[0].y; a[0][3] = w[1].y;
+      a[1][0] = w[0].z; a[1][1] = w[1].z; a[1][2] = w[0].w; a[1][3] = w[1].w;
+    } else {
+      const uint32_t r0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, r1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t a[4];
-      codes_f16<KIND>(r0[i], a[0], a[2]);
-      codes_f16<KIND>(r1[i], a[1], a[3]);
-      mma<KIND>(acc, a[0], a[1], a[2], a[3], b[2 * i], b[2 * i + 1]);
+      for (int i = 0; i < 4; ++i) {
+        codes_f16<KIND>(r0[i], a[i][0], a[i][2]);
+        codes_f16<KIND>(r1[i], a[i][1], a[i][3]);
+      }
     }
   }
-}
+  __device__ __forceinline__ void times(const Acts<KIND> &x, float (&acc)[4]) const {
+    if constexpr (KIND <= kF16) {
+      mma<KIND>(acc, a[0][0], a[0][1], a[0][2], a[0][3], x.b[0].x, x.b[0].y);
+      mma<KIND>(acc, a[1][0], a[1][1], a[1][2], a[1][3], x.b[0].z, x.b[0].w);
+    } else {
+      mma<KIND>(acc, a[0][0], a[0][1], a[0][2], a[0][3], x.b[0].x, x.b[0].y);
+      mma<KIND>(acc, a[1][0], a[1][1], a[1][2], a[1][3], x.b[0].z, x.b[0].w);
+      mma<KIND>(acc, a[2][0], a[2][1], a[2][2], a[2][3], x.b[1].x, x.b[1].y);
+      mma<KIND>(acc, a[3][0], a[3][1], a[3][2], a[3][3], x.b[1].z, x.b[1].w);
+    }
+  }
+};
 
 // The rows of items i .. in the panel, as many as it takes: their planes, zeros behind K up to whole steps. Returns the item behind them.
 template <int KIND, bool GATEUP>
@@ -381,7 +428,7 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
       }
     }
   }
-  meet();
+  __syncthreads();
   const int chunks = (K + 63) / 64 * 8, runs = (chunks + 31) / 32;   // of eight values; of 32 such: a warp's
 #pragma unroll 2
   for (int u = tid >> 5; u < n * runs; u += kWarps) {
@@ -489,46 +536,50 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
     }
 }
 
-// The tiles of an item. All fifteen warps take part in each: a sub-tile has 15 / subs of them, and a warp every 15 / subs-th run of 128 bytes
-// of a slice of its rows; their sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
+// The tiles of an item of up to 4 GROUPS tokens. All sixteen warps take part in each: a sub-tile has 16 / subs of them, and a warp one or
+// (EIGHT) two runs of 128 bytes of a slice of its rows; their sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
 // A warp whose wait gives up raises s.fail, waits no more and frees no slot, but meets every barrier; what it forms then is never used.
 // (Sub-tiles in slots of their own would let the groups of warps drift apart, past what a barrier's two phases tell apart.)
 // Shared memory's bandwidth is what the products would be bound by: 32 KB of weights are 256 cycles of its 128 bytes, in some 1400 that
-// HBM takes to bring them. HOLD: up to four tokens' planes, read once for all tiles, stay in registers where a row is one slice; read
-// from shared memory at each step they cost as much as the weights.
-template <int KIND, bool GATEUP, bool EIGHT, bool HOLD>
-__device__ __forceinline__ void run_tiles(const DecodeParams &p, Shared &s, const Item &it, int base, Ring &ring, const uint8_t *panel, float *red,
-                                          const uint8_t *slots) {
-  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kGroups = HOLD ? 1 : 4;
-  constexpr int kRuns = EIGHT ? 3 : 2;   // most runs of a warp in a slice: 32 of eight rows over fifteen warps; 16, 8 or 4 over 15, 7 or 3
+// HBM takes to bring them. HOLD: the planes of the tokens, read once for all tiles, stay in registers where a row is one slice; read
+// from shared memory at each step those of four tokens cost as much as the weights.
+template <int KIND, bool GATEUP, bool EIGHT, int GROUPS, bool HOLD>
+__device__ __forceinline__ void run_tiles(const DecodeParams &p, Shared &s, const Item &it, int base, Ring &ring, const uint8_t *panel, float *sums,
+                                          uint8_t *slots) {
+  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kRuns = EIGHT ? 2 : 1, kRunBytes = kWarps * 128;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = kWarps / subs, sub = warp / parts, part = warp - sub * parts;
-  const int tiles = (it.r1 - it.r0 + sh.outs - 1) / sh.outs, groups = (it.n + 3) / 4, batch = kRed / (64 * 16 * it.n);
+  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = kWarps / subs, sub = warp & (subs - 1), part = warp / subs;
+  const int tiles = (it.r1 - it.r0 + sh.outs - 1) / sh.outs, batch = kRed / (64 * kWarps * it.n);
   // this lane's bytes of rows g and g + 8 of its sub-tile in a slot, of gate and up of row g of either; EIGHT: of the slot's row g
   const bool swap = (g & 1) && (sh.slice & 64) == 0;
-  const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16, row1 = row0 + (GATEUP ? sh.outs : 8) * sh.slice, run_bytes = parts * 128;
-  const uint8_t *rows[kGroups];   // this lane's run of a plane of one of each four tokens
+  const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16, row1 = row0 + (GATEUP ? sh.outs : 8) * sh.slice;
+  const uint8_t *rows[GROUPS];   // this lane's run of a plane of one of each four tokens
 #pragma unroll
-  for (int q = 0; q < kGroups; ++q)
+  for (int q = 0; q < GROUPS; ++q)
     rows[q] = panel + (2 * (base + min(4 * q + (g >> 1), it.n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
-  constexpr int kHeld = KIND <= kF16 ? 2 : 1;   // runs whose planes stay in sixteen registers
-  Acts<KIND> held[kHeld][2];
+  Acts<KIND> held[HOLD ? kRuns : 1][2][GROUPS];
   if constexpr (HOLD) {
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r)
+    for (int r = 0; r < kRuns; ++r)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (part * 128 + r * run_bytes + u * 64 < sh.row_bytes) held[r][u].load(rows[0] + (r * run_bytes + u * 64) * (2 / kElem));
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q)
+          if (part * 128 + r * kRunBytes + u * 64 < sh.row_bytes) held[r][u][q].load(rows[q] + (r * kRunBytes + u * 64) * (2 / kElem));
+          else held[r][u][q].clear();
   }
   for (int tile = 0, in_batch = 0; tile < tiles; ++tile) {
     const int first_row = it.r0 + tile * sh.outs + sub * kOuts;
-    const bool mine = sub < subs && first_row < it.r1;   // the last tile may have fewer sub-tiles
-    float acc[kGroups][4];
+    const bool mine = first_row < it.r1;   // the last tile may have fewer sub-tiles
+    constexpr int kChains = GROUPS == 1 ? 2 : 1;
+    float acc[GROUPS][kChains][4];
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q)
+    for (int q = 0; q < GROUPS; ++q)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[q][c] = 0.f;
+      for (int u = 0; u < kChains; ++u)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[q][u][c] = 0.f;
     const float *sc0 = nullptr, *sc1 = nullptr;   // e4m3: scales of the blocks of rows g and g + 8, or of row g
     if constexpr (KIND == kE4) {
       const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128;
@@ -542,96 +593,102 @@ __device__ __forceinline__ void run_tiles(const DecodeParams &p, Shared &s, cons
       if constexpr (KIND == kE4) {
 #pragma unroll
         for (int r = 0; r < kRuns; ++r) {
-          const int at = sl * (sh.slice / 128) + r * parts;
-          f[r][0] = left > r * run_bytes ? __ldg(sc0 + at) : 0.f;
-          f[r][1] = EIGHT ? 0.f : left > r * run_bytes ? __ldg(sc1 + at) : 0.f;
+          const int at = sl * (sh.slice / 128) + r * kWarps;
+          f[r][0] = left > r * kRunBytes ? __ldg(sc0 + at) : 0.f;
+          f[r][1] = EIGHT ? 0.f : left > r * kRunBytes ? __ldg(sc1 + at) : 0.f;
         }
       }
+      if (warp == kFiller && ring.ok && !fill(p, s, slots, ring.n, ring.read + 1)) ring.ok = false;
       if (ring.ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ring.ok = false;
       ring.ok = __all_sync(0xffffffffu, ring.ok);
       const uint8_t *slot = slots + ring.at * kSlot;
+      Weights v[kRuns];
 #pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        if (left <= r * run_bytes) break;
-        Weights v;
-        load_run<EIGHT>(v, slot + row0 + r * run_bytes, slot + row1 + r * run_bytes, swap, left - r * run_bytes);
-        const bool both = left - r * run_bytes > 64;
-#pragma unroll
-        for (int q = 0; q < kGroups; ++q) {
-          if (!HOLD && q >= groups) break;
-          float t[4] = {0.f, 0.f, 0.f, 0.f};
-          float (&to)[4] = KIND == kE4 ? t : acc[q];
-          const uint8_t *at = rows[q] + (sl * sh.slice + r * run_bytes) * (2 / kElem);
-          Acts<KIND> x;
-          if (HOLD && r < kHeld) x = held[r < kHeld ? r : 0][0];
-          else x.load(at);
-          step<KIND>(v.w[0], x, to);
-          if (both) {
-            if (HOLD && r < kHeld) x = held[r < kHeld ? r : 0][1];
-            else x.load(at + 64 * (2 / kElem));
-            step<KIND>(v.w[1], x, to);
-          }
-          if constexpr (KIND == kE4) {
-            acc[q][0] = fmaf(f[r][0], t[0], acc[q][0]);
-            acc[q][1] = fmaf(f[r][0], t[1], acc[q][1]);
-            acc[q][2] = fmaf(f[r][1], t[2], acc[q][2]);
-            acc[q][3] = fmaf(f[r][1], t[3], acc[q][3]);
-          }
-        }
-      }
+      for (int r = 0; r < kRuns; ++r)
+        if (left > r * kRunBytes) load_run<EIGHT>(v[r], slot + row0 + r * kRunBytes, slot + row1 + r * kRunBytes, swap, left - r * kRunBytes);
       __syncwarp();
       if (lane == 0 && ring.ok) mbar_arrive(&s.empty[ring.at]);
       ring.next();
-    }
-    float *dst = red + (((in_batch * subs + sub) * parts + part) * it.n + j) * 16 + g;
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q)
+      for (int r = 0; r < kRuns; ++r) {
+        if (left <= r * kRunBytes) break;
+        // The steps' sums are chains of their own where there is one group, and under e4m3's scales of the run's block everywhere.
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (!HOLD && left - r * kRunBytes <= u * 64) break;
+          const Step<KIND> w(v[r].w[u]);
+#pragma unroll
+          for (int q = 0; q < GROUPS; ++q) {
+            Acts<KIND> x;
+            if constexpr (HOLD) x = held[r][u][q];
+            else x.load(rows[q] + (sl * sh.slice + r * kRunBytes + u * 64) * (2 / kElem));
+            if constexpr (KIND == kE4) {
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              w.times(x, t);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[q][u % kChains][c] = fmaf(f[r][c >> 1], t[c], acc[q][u % kChains][c]);
+            } else {
+              w.times(x, acc[q][u % kChains]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (kChains == 2) acc[q][0][c] += acc[q][kChains - 1][c];
+    float *red = sums + ring.turn * (kRed / 4), *dst = red + (((in_batch * subs + sub) * parts + part) * it.n + j) * 16 + g;
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q)
       if (mine && 4 * q + j < it.n) {
-        dst[q * 64] = acc[q][0] + acc[q][1];
-        if (!EIGHT) dst[q * 64 + 8] = acc[q][2] + acc[q][3];
+        dst[q * 64] = acc[q][0][0] + acc[q][0][1];
+        if (!EIGHT) dst[q * 64 + 8] = acc[q][0][2] + acc[q][0][3];
       }
     if (++in_batch != batch && tile + 1 < tiles) continue;
-    meet();
+    __syncthreads();
     add_parts<KIND, GATEUP, EIGHT>(p, s, it, base, red, in_batch * subs, it.r0 + (tile + 1 - in_batch) * sh.outs);
     in_batch = 0;
-    meet();
+    ring.turn ^= 1;   // who still adds is met at the next barrier
   }
 }
 
 // One product over this CTA's items: gate, up and silu into p.act, or down into p.Y
 template <int KIND, bool GATEUP>
-__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *red, const uint8_t *slots) {
+__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *red, uint8_t *slots) {
   const Plan &plan = s.plan[GATEUP ? 0 : 1];
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
   int built = 0, base = 0;
   for (int i = 0; i < plan.n_items; ++i) {
     const Item &it = plan.item[i];
     if (i >= built) {
-      meet();   // the last panel is read
+      __syncthreads();   // the last panel is read
       built = build_panel<KIND, GATEUP>(p, s, plan, sh.K, panel, i);
       base = 0;
-      meet();
+      __syncthreads();
     }
-    const bool hold = it.n <= 4 && sh.slices == 1;
-    if (sh.eight) {
-      if (hold) run_tiles<KIND, GATEUP, true, true>(p, s, it, base, ring, panel, red, slots);
-      else run_tiles<KIND, GATEUP, true, false>(p, s, it, base, ring, panel, red, slots);
-    } else if (hold) {
-      run_tiles<KIND, GATEUP, false, true>(p, s, it, base, ring, panel, red, slots);
-    } else {
-      run_tiles<KIND, GATEUP, false, false>(p, s, it, base, ring, panel, red, slots);
-    }
+    auto go = [&](auto eight) {
+      constexpr bool kEight = decltype(eight)::value;
+      if (it.n <= 4 && sh.slices == 1) run_tiles<KIND, GATEUP, kEight, 1, true>(p, s, it, base, ring, panel, red, slots);
+      else run_tiles<KIND, GATEUP, kEight, 2, false>(p, s, it, base, ring, panel, red, slots);
+    };
+    if (sh.eight) go(std::true_type());
+    else go(std::false_type());
     base += it.n;
   }
 }
 
 // The rows of a product are dealt to the CTAs in equal numbers, in pairs of rows, over all active experts in a row; an expert's tokens
 // that the panel does not take at once go through in passes.
-__device__ void make_plan(Plan &plan, const Shared &s, int N, int cap) {
+__device__ __forceinline__ void make_plan(const DecodeParams &p, Plan &plan, const Shared &s, int N, int cap) {
   const unsigned half = N / 2, units = s.n_active * half;   // at most 128 x 20480, times the CTAs below 2^32
-  unsigned u = units * blockIdx.x / gridDim.x;
-  const unsigned end = units * (blockIdx.x + 1) / gridDim.x;
-  int n = 0, panel = 0, held = 0, most = 0, i = u / half;
+  auto border = [&](unsigned b) { return b == gridDim.x ? units : __umulhi(units * b, p.grid_inverse); };   // about units * b / grid, growing with b
+  unsigned u = border(blockIdx.x);
+  const unsigned end = border(blockIdx.x + 1);
+  int n = 0, panel = 0, held = 0, most = 0, i = (int)__fdividef((float)u, (float)half);
+  if (i * half > u) --i;   // the quotient of numbers below 2^24 may be off by one
+  if ((i + 1) * half <= u) ++i;
   while (u < end) {
     const unsigned begin = i * half, stop = min(end, begin + half);
     const int e = s.active[i++], rows = __popc(s.mask[e]);
@@ -709,7 +766,7 @@ __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &
 #pragma unroll
       for (int k = 0; k < SIDE; ++k) dot[i][k] = 0.f;
     }
-    for (int c = 4 * tid; c < p.H; c += 4 * kAll) {
+    for (int c = 4 * tid; c < p.H; c += 4 * kThreads) {
       float4 x[SIDE], n = make_float4(1.f, 1.f, 1.f, 1.f);
       uint2 r[SIDE];
 #pragma unroll
@@ -752,7 +809,7 @@ __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &
     if (i >= SIDE || t >= p.T) continue;
     float v = 0.f;
     if (lane < 2 + SIDE)
-      for (int w = 0; w < kAll / 32; ++w) v = lane == 1 ? max_nan(v, s.part[w][i][1]) : v + s.part[w][i][lane];
+      for (int w = 0; w < kWarps; ++w) v = lane == 1 ? max_nan(v, s.part[w][i][1]) : v + s.part[w][i][lane];
     const float tot = __shfl_sync(0xffffffffu, v, 0), m = __shfl_sync(0xffffffffu, v, 1);
     float inv = 1.0f;
     if (p.pre_w) {
@@ -774,11 +831,11 @@ __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &
 }
 
 // sum of squares of the row in shared memory and its inverse norm; a large row once more
-__device__ __forceinline__ float row_inverse(const float *row, int H, float ss, float eps, float (*red)[kAll / 32]) {
+__device__ __forceinline__ float row_inverse(const float *row, int H, float ss, float eps, float (*red)[kWarps]) {
   const float tot = cta_sum(ss, red[0]);
   if (!(tot > 3.402823466e38f)) return inverse_rms(tot, H, eps);
   float q = 0.f;
-  for (int i = threadIdx.x; i < H; i += kAll) q = fmaf(row[i] * kDown, row[i] * kDown, q);
+  for (int i = threadIdx.x; i < H; i += kThreads) q = fmaf(row[i] * kDown, row[i] * kDown, q);
   return kDown * rsqrtf(cta_sum(q, red[1]) * (1.0f / (float)H));
 }
 
@@ -821,7 +878,7 @@ struct Finish {
   // row: H values in shared memory, of which a thread reads only its own (e4m3 rows: all)
   __device__ __forceinline__ void run(const DecodeParams &p, Shared &s, int t, float *row) {
     const int first = 4 * threadIdx.x, H = p.H;
-    constexpr int kStride = 4 * kAll;
+    constexpr int kStride = 4 * kThreads;
     float ss = 0.f;
     for (int c = first; c < H; c += kStride) {
       float4 v[kMaxK], y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -890,7 +947,7 @@ __device__ void give_up(const DecodeParams &p, Shared &s) {
   }
   const float nan = __int_as_float(0x7fffffff);
   for (int t = blockIdx.x; t < p.T; t += gridDim.x) {
-    for (int i = threadIdx.x; i < p.H; i += kAll) {
+    for (int i = threadIdx.x; i < p.H; i += kThreads) {
       store_from_f32(p.out, p.out_dtype, t * p.ldo + i, nan);
       if (p.next_w) {
         if (p.h_dtype == KNJ_DT_E4M3) static_cast<uint8_t *>(p.h_next)[t * p.ldh + i] = 0x7f;
@@ -898,12 +955,12 @@ __device__ void give_up(const DecodeParams &p, Shared &s) {
       }
     }
     if (p.next_w && p.h_dtype == KNJ_DT_E4M3)
-      for (int g = threadIdx.x; g < p.H / kFp8Group; g += kAll) p.h_next_scale[(int64_t)t * (p.H / kFp8Group) + g] = nan;
+      for (int g = threadIdx.x; g < p.H / kFp8Group; g += kThreads) p.h_next_scale[(int64_t)t * (p.H / kFp8Group) + g] = nan;
   }
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -921,8 +978,8 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   if (p.T == 1) norms_and_logits<1>(p, s);
   else if (p.T <= 4) norms_and_logits<2>(p, s);
   else norms_and_logits<4>(p, s);
-  grid_arrive<kAll>(p, s);
-  if (!grid_wait<kAll>(p, s, 1)) return give_up(p, s);
+  grid_arrive(p, s);
+  if (!grid_wait(p, s, 1)) return give_up(p, s);
 
   // ---- routing: a warp per token ----
   if (warp < p.T) {
@@ -957,39 +1014,39 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     }
     if (lane == 0) s.n_active = n;
     __syncwarp();
-    if (lane < 2) make_plan(s.plan[lane], s, lane == 0 ? p.F : p.H, Geo<KIND>::cap(lane == 0 ? p.H : p.F));
+    if (lane < 2) make_plan(p, s.plan[lane], s, lane == 0 ? p.F : p.H, Geo<KIND>::cap(lane == 0 ? p.H : p.F));
+    __syncwarp();
+    if (lane == 0) {
+      const int first = s.plan[0].n_items > 0 ? 0 : s.plan[1].n_items > 0 ? 1 : 2;
+      s.next = Cursor{first, 0, first < 2 ? s.plan[first].item[0].r0 : 0, 0, 0, 0, 0u};
+    }
   }
   __syncthreads();
 
   float *red = reinterpret_cast<float *>(smem);
-  uint8_t *panel = smem + kRed;
+  uint8_t *panel = smem + 2 * kRed;
   const int held = max(s.plan[0].rows * 2 * Geo<KIND>::pitch(p.H), s.plan[1].rows * 2 * Geo<KIND>::pitch(p.F));
-  const int at = kRed + (held + 127) / 128 * 128;
+  const int at = 2 * kRed + (held + 127) / 128 * 128;
   uint8_t *slots = smem + at;
-  Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u, true};
+  Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u, 0, 0, true};
+  if (warp == kFiller) ring.ok = fill(p, s, slots, ring.n, 0);
+  run_product<KIND, true>(p, s, ring, panel, red, slots);
+  grid_arrive(p, s);
+  if (warp == kFiller && ring.ok) ring.ok = fill(p, s, slots, ring.n, 0);   // down's rows travel while the grid meets
   const int t = blockIdx.x;
-  Finish end;
-  if (warp == kWarps) {
-    int copied = 0;
-    if (!feed(p, s, 0, ring, slots, copied) || !feed(p, s, 1, ring, slots, copied)) {
-      // the slots filled last may still be written: shared memory is not left before they are
-      if (lane < ring.n && copied > lane) mbar_wait_for(&s.full[lane], (uint32_t)((copied - lane - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
-    }
+  bool ok = grid_wait(p, s, 2);
+  if (ok) {
+    run_product<KIND, false>(p, s, ring, panel, red, slots);
+    grid_arrive(p, s);
+    Finish end;
     if (t < p.T) end.prepare(p, s, t);
-  } else {
-    run_product<KIND, true>(p, s, ring, panel, red, slots);
-    grid_arrive<kThreads>(p, s);
-    if (grid_wait<kThreads>(p, s, 2)) {
-      run_product<KIND, false>(p, s, ring, panel, red, slots);
-      grid_arrive<kThreads>(p, s);
-      if (t < p.T) end.prepare(p, s, t);
-      grid_wait<kThreads>(p, s, 3);
-    }
-    if (!s.ok && tid == 0) *reinterpret_cast<volatile int *>(&s.fail) = 1;   // ends the copying warp's waits
+    ok = grid_wait(p, s, 3);
+    if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
   }
-  __syncthreads();
-  if (!s.ok) return give_up(p, s);
-  if (t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
+  if (ok) return;
+  give_up(p, s);
+  // the slots filled last may still be written: shared memory is not left before they are
+  if (tid < ring.n && s.next.copied > tid) mbar_wait_for(&s.full[tid], (uint32_t)((s.next.copied - tid - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
 }
 
 template <int KIND>
@@ -1015,7 +1072,7 @@ int launch(DecodeParams &p, cudaStream_t st) {
   }
   KNJ_CUDA(cudaMemsetAsync(p.sync, 0, kCleared, st));
   void *args[] = {&p};
-  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kAll), args, kSmem, st));
+  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kThreads), args, kSmem, st));
   return launch_status("moe_decode_kernel");
 }
 
@@ -1056,7 +1113,7 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   p.gate_kind = a->gate_kind; p.gate_sigmoid = a->gate_sigmoid;
   p.x_vec = aligned16(a->x) && a->ldx * (a->x_dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0;
   p.alpha = a->alpha; p.beta = a->beta; p.eps = a->eps;
-  p.wait_cycles = decode_wait_cycles(); p.stall = t_stall;
+  p.wait_cycles = decode_wait_cycles(); p.stall = t_stall; p.grid_inverse = (unsigned)((1ull << 32) / sm_count());
   const cudaStream_t st = as_stream(stream);
   switch (a->w_dtype) {
     case KNJ_DT_BF16: return launch<kBf16>(p, st);
