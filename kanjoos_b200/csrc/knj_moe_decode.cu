@@ -8,11 +8,11 @@
 // (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). In mma.sync.m16n8k16 sixteen matrix rows
 // meet the two planes of four tokens, so that the second plane costs nothing while a step's weights are on their way.
 //
-// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. This CTA's
-// matrix rows, of gate and up and behind them of down, stream through a ring in shared memory, which one of the sixteen warps fills between
-// its products. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep
-// HBM busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both
-// operands have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
+// Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
+// its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
+// multiply. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep HBM
+// busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both operands
+// have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
 //
 // Stages, with a barrier over the grid between them:
 //   1  norm statistics (every CTA, all tokens) and router logits (an expert or two a CTA)
@@ -20,8 +20,6 @@
 //   3  down, likewise
 //   4  weighted sum, norm, gate, residual, next norm: a CTA for each token
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
-#include <type_traits>
-
 #include "knj_fp8.cuh"
 #include "knj_topk.cuh"
 
@@ -31,16 +29,18 @@ namespace {
 
 constexpr int kMaxRows = 8;   // of activations in the panel at a time: two groups of four
 constexpr int kMaxTokens = KNJ_MOE_DECODE_MAX_TOKENS, kMaxK = 8, kMaxExperts = 256;
-// 128 registers a thread. (With a seventeenth warp that copies a thread has 96, and the shared memory that the ring takes leaves no L1 for
-// what then spills: every spilled word came back from L2, 1000 cycles under load.)
-constexpr int kThreads = 512, kWarps = kThreads / 32, kFiller = kWarps - 1;   // kFiller: the warp that fills the ring
-// A slot of the ring holds a tile: 64, 32, 16 or 8 matrix rows of up to 512, 1024, 2048 or 4096 bytes as they lie, in one or two copies.
-// (A copy for each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536.) Longer rows
-// come in slices of up to 4096 bytes, eight rows to a slot.
-constexpr int kSlice = 4096;
-constexpr int kSlot = 8 * kSlice;
+// Seventeen warps leave 96 registers a thread, and the shared memory that the ring takes leaves no L1 for what does not fit: a spilled word
+// comes back from L2, 1000 cycles under load. So the products' loops are kept small: forms with the planes of the tokens in registers
+// spilled, and took three times as long.
+constexpr int kThreads = 512, kWarps = kThreads / 32;   // that multiply; behind them the warp that copies
+constexpr int kAll = kThreads + 32;
+// A slot of the ring holds a tile: 64, 32 or 16 matrix rows of up to 512, 1024 or 2048 bytes as they lie, in one or two copies. (A copy for
+// each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536.) Longer rows come in slices
+// of up to 2048 bytes, sixteen rows to a slot.
+constexpr int kSlice = 2048;
+constexpr int kSlot = 16 * kSlice;
 constexpr int kMaxSlots = 6;
-constexpr int kRed = 8 * 1024;                // bytes of the sums of a batch of tiles: 1 KB a tile and token; there are two, in turn
+constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 256 a tile and token
 constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
 constexpr int kMaxItems = 64;
 constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256,
@@ -53,8 +53,7 @@ enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
 struct Shape {
   int K, N, row_bytes;
   int slices, slice;   // of a row, bytes
-  int eight;           // tiles of eight rows, else of 16 a sub-tile
-  int subs;            // sub-tiles of a tile, each of which has 16 / subs warps
+  int subs;            // sub-tiles of 16 rows of a tile, each of which has 4 / subs warps
   int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
 };
 
@@ -94,16 +93,8 @@ struct Plan {
   int n_items, rows;            // rows: most that are in the panel at a time
 };
 
-// the next tile (or slice of one) to copy
-struct Cursor {
-  int product, item, row, slice;
-  int slot, copied;   // copied: slots filled so far
-  uint32_t parity;    // of the slot's barrier once it is read
-};
-
 struct Shared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
-  Cursor next;                  // of the warp that fills the ring
   int fail;                     // raised by a wait that gave up; read as volatile
   float part[kWarps][4][6];  // of a token: squares, largest, dot products
   float inv[kMaxTokens], mult[kMaxTokens], unmult[kMaxTokens];
@@ -128,13 +119,22 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-// Barrier over the grid, number `n` of the launch, in two halves. A CTA in which a wait has given up never arrives; grid_wait is false for
-// all threads where the barrier did not complete in time.
+// of the warps that multiply
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+template <int N>
+__device__ __forceinline__ void cta_barrier() {
+  if constexpr (N == kAll) __syncthreads();
+  else meet();
+}
+// Barrier over the grid, number `n` of the launch, in two halves, met by the first N threads of every CTA. A CTA in which a wait has given
+// up never arrives; grid_wait is false for all threads where the barrier did not complete in time.
+template <int N>
 __device__ __forceinline__ void grid_arrive(const DecodeParams &p, Shared &s) {
-  __syncthreads();
+  cta_barrier<N>();
   if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0)
     asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.sync), "r"(1u) : "memory");
 }
+template <int N>
 __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int n) {
   if (threadIdx.x == 0) {
     int ok = *reinterpret_cast<volatile int *>(&s.fail) == 0;
@@ -145,7 +145,7 @@ __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int 
     }
     s.ok = ok;
   }
-  __syncthreads();
+  cta_barrier<N>();
   return s.ok != 0;
 }
 
@@ -244,7 +244,7 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &p0, uint32_t &p1
 __device__ __forceinline__ float cta_sum(float v, float *red) {   // by all threads; red: a word for each warp, not in use by an earlier sum
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
+  meet();
   float t = 0.f;
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) t += red[i];
@@ -258,7 +258,7 @@ struct Geo {
   __host__ __device__ static int pitch(int K) { return (2 * K + 127) / 128 * 128 + (kElem == 2 ? 64 : 16); }
   // rows in the panel at a time: what leaves the ring two slots, or one
   __host__ __device__ static int cap(int K) {
-    const int c = (kSmem - 2 * kRed - 2 * kSlot) / (2 * pitch(K));
+    const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
     return c < 1 ? 1 : c < kMaxRows ? c : kMaxRows;
   }
 };
@@ -269,11 +269,7 @@ struct Geo {
 struct Ring {
   int at, n;
   uint32_t parity;
-  int read;    // slots read so far
-  int turn;    // of the two places for sums
-  bool ok;     // no wait has given up
   __device__ __forceinline__ void next() {
-    ++read;
     if (++at == n) {
       at = 0;
       parity ^= 1u;
@@ -281,84 +277,53 @@ struct Ring {
   }
 };
 
-// By the warp that fills the ring: copies tiles into its free slots; with `must`, waits until at least `must` slots in all have been filled.
-// False after a wait that gave up.
-__device__ __forceinline__ bool fill(const DecodeParams &p, Shared &s, uint8_t *slots, int n_slots, int must) {
+// The copying warp's side of a product. False after a wait that gave up.
+__device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int product, Ring &ring, uint8_t *slots, int &copied) {
   const int lane = threadIdx.x & 31;
-  Cursor c = s.next;
-  bool ok = true;
-  while (c.product < 2) {
-    uint64_t *free = &s.empty[c.slot];
-    bool there = mbar_try_wait(free, c.parity ^ 1u);
-    if (!__all_sync(0xffffffffu, there)) {
-      if (c.copied >= must) break;
-      there = mbar_wait_for(free, c.parity ^ 1u, p.wait_cycles, &s.fail);
-      if (!__all_sync(0xffffffffu, there)) {
-        ok = false;
-        break;
-      }
-    }
-    const bool up = c.product == 0;
-    const Shape &sh = p.shape[c.product];
-    const Plan &plan = s.plan[c.product];
-    const Item &it = plan.item[c.item];
-    const int rows = min(sh.outs, it.r1 - c.row);
-    // lane l copies the rows of matrix l, or row l % rows of matrix l / rows
-    const bool whole = sh.slices == 1;
-    const int second = up && (whole ? lane == 1 : lane >= rows), r = whole ? 0 : lane - second * rows;
-    const uint8_t *w = up ? (second ? p.w_up : p.w_gate) : p.w_down;
-    const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - c.slice * sh.slice);
-    uint64_t *bar = &s.full[c.slot];
-    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
-    __syncwarp();
-    if (lane < (whole ? 1 : rows) * (up ? 2 : 1))
-      bulk_g2s(slots + c.slot * kSlot + (second * sh.outs + r) * sh.slice, w + ((int64_t)it.expert * sh.N + c.row + r) * sh.row_bytes + c.slice * sh.slice,
-               (uint32_t)bytes, bar);
-    ++c.copied;
-    if (++c.slot == n_slots) {
-      c.slot = 0;
-      c.parity ^= 1u;
-    }
-    if (++c.slice == sh.slices) {
-      c.slice = 0;
-      c.row += sh.outs;
-      if (c.row >= it.r1) {
-        if (++c.item == plan.n_items) {
-          c.item = 0;
-          c.product = up && s.plan[1].n_items > 0 ? 1 : 2;
-        }
-        if (c.product < 2) c.row = s.plan[c.product].item[c.item].r0;
+  const Shape &sh = p.shape[product];
+  const Plan &plan = s.plan[product];
+  const bool up = product == 0, whole = sh.slices == 1;
+  for (int i = 0; i < plan.n_items; ++i) {
+    const Item it = plan.item[i];
+    for (int first = it.r0; first < it.r1; first += sh.outs) {
+      const int rows = min(sh.outs, it.r1 - first);
+      // lane l copies the rows of matrix l, or row l % rows of matrix l / rows
+      const int second = up && (whole ? lane == 1 : lane >= rows), r = whole ? 0 : lane - second * rows;
+      const bool mine = lane < (whole ? 1 : rows) * (up ? 2 : 1);
+      const uint8_t *src = (up ? (second ? p.w_up : p.w_gate) : p.w_down) + ((int64_t)it.expert * sh.N + first + r) * sh.row_bytes;
+      const int dst = (second * sh.outs + r) * sh.slice;
+      for (int sl = 0; sl < sh.slices; ++sl) {
+        const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - sl * sh.slice);
+        const bool ok = mbar_wait_for(&s.empty[ring.at], ring.parity ^ 1u, p.wait_cycles, &s.fail);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (lane == 0) mbar_expect_tx(&s.full[ring.at], (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
+        __syncwarp();
+        if (mine) bulk_g2s(slots + ring.at * kSlot + dst, src + sl * sh.slice, (uint32_t)bytes, &s.full[ring.at]);
+        ring.next();
+        ++copied;
       }
     }
   }
-  __syncwarp();
-  if (lane == 0) s.next = c;
-  __syncwarp();
-  return ok;
+  return true;
 }
 
-// A lane's part of a run of 128 bytes (two steps of 64): of rows g and g + 8, or of row g of eight, the bytes 16 j .. + 15 of either step.
+// A lane's part of a run of 128 bytes (two steps of 64) of sixteen rows: of rows g and g + 8 the bytes 16 j .. + 15 of either step.
 struct Weights {
   uint4 w[2][2];   // [step][row]
 };
 // Rows a multiple of 128 bytes apart lie on the same banks, and a load of shared memory serves two of them at a time: the odd one reads its
 // second step first, and the two change places in registers. left: bytes of the rows from the run's first on; what lies behind is zero.
-template <bool EIGHT>
 __device__ __forceinline__ void load_run(Weights &v, const uint8_t *row0, const uint8_t *row1, bool swap, int left) {
   const int first = swap ? 64 : 0;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (EIGHT && m == 1) {
-      v.w[0][1] = v.w[1][1] = make_uint4(0, 0, 0, 0);
-      break;
-    }
     const uint8_t *row = m == 0 ? row0 : row1;
     const uint4 a = *reinterpret_cast<const uint4 *>(row + first), b = *reinterpret_cast<const uint4 *>(row + 64 - first);
     v.w[0][m] = swap ? b : a;
     v.w[1][m] = swap ? a : b;
   }
-  const int at = (threadIdx.x & 3) * 16;
   if (left < 128) {
+    const int at = (threadIdx.x & 3) * 16;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       if (u * 64 + at >= left) v.w[u][0] = v.w[u][1] = make_uint4(0, 0, 0, 0);
@@ -371,10 +336,6 @@ struct Acts {
   __device__ __forceinline__ void load(const uint8_t *at) {
     b[0] = *reinterpret_cast<const uint4 *>(at);
     if constexpr (KIND > kF16) b[1] = *reinterpret_cast<const uint4 *>(at + 16);
-  }
-  __device__ __forceinline__ void clear() {
-    b[0] = make_uint4(0, 0, 0, 0);
-    if constexpr (KIND > kF16) b[1] = b[0];
   }
 };
 // One step of sixteen rows as MMA operands, and its products with the planes of four tokens
@@ -428,7 +389,7 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
       }
     }
   }
-  __syncthreads();
+  meet();
   const int chunks = (K + 63) / 64 * 8, runs = (chunks + 31) / 32;   // of eight values; of 32 such: a warp's
 #pragma unroll 2
   for (int u = tid >> 5; u < n * runs; u += kWarps) {
@@ -470,52 +431,26 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
   return built;
 }
 
-// The sums over the parts of K of the sub-tiles 0 .. n-1 of a batch, whose first output is `first`: a warp per sub-tile. Parts are added in
-// kShare chains and these in pairs, by as many lanes for a single token, by one for more: in the same order, so that a token's bits do
-// not depend on the others'.
-template <int KIND, bool GATEUP, bool EIGHT>
+// The sums over the parts of K of the sub-tiles 0 .. n-1 of a batch, whose first output is `first`, and what becomes of them: a warp per
+// sub-tile, lanes over tokens and outputs.
+template <int KIND, bool GATEUP>
 __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, const Item &it, int base, const float *red, int n, int first) {
-  constexpr int kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kShare = GATEUP ? 4 : 2;
-  const int lane = threadIdx.x & 31;
+  constexpr int kOuts = GATEUP ? 8 : 16;
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  const int parts = kWarps / sh.subs, tokens = it.n;
-  const bool one = tokens == 1;
+  const int parts = 4 / sh.subs, tokens = it.n;
   for (int u = threadIdx.x >> 5; u < n; u += kWarps)
-    for (int o = lane; o < (tokens * kOuts * (one ? kShare : 1) + 31) / 32 * 32; o += 32) {
-      const int r = o % kOuts, tok = one ? 0 : o / kOuts, chain = one ? o / kOuts : 0, row = first + u * kOuts + r;
-      const bool in = tok < tokens && chain < kShare && row < it.r1;
-      auto sum = [&](int from, float &a, float &b) {
-        a = b = 0.f;
-        if (!in) return;
-        const float *src = red + ((u * parts + from) * tokens + tok) * 16 + r;
-#pragma unroll 4
-        for (int w = from; w < parts; w += kShare, src += kShare * tokens * 16) {
-          a += src[0];
-          if (GATEUP) b += src[kOuts];
-        }
-      };
-      float a, b;
-      sum(chain, a, b);
-      if (one) {
-#pragma unroll
-        for (int x = 1; x < kShare; x *= 2) {
-          a += __shfl_xor_sync(0xffffffffu, a, x * kOuts);
-          b += __shfl_xor_sync(0xffffffffu, b, x * kOuts);
-        }
-      } else {
-        float c[2], d[2];
-        sum(1, c[0], d[0]);
-        a += c[0];
-        b += d[0];
-        if constexpr (kShare == 4) {
-          sum(2, c[0], d[0]);
-          sum(3, c[1], d[1]);
-          a += c[0] + c[1];
-          b += d[0] + d[1];
-        }
-      }
-      const int pair = s.row_pair[base + (tok < tokens ? tok : 0)];
+    for (int o = threadIdx.x & 31; o < (tokens * kOuts + 31) / 32 * 32; o += 32) {
+      const int r = o % kOuts, tok = o / kOuts, row = first + u * kOuts + r;
+      const bool in = tok < tokens && row < it.r1;
+      float a = 0.f, b = 0.f;
       if (in) {
+        const float *src = red + (u * parts * tokens + tok) * 16 + r;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (w >= parts) break;
+          a += src[w * tokens * 16];
+          if (GATEUP) b += src[w * tokens * 16 + 8];
+        }
         const float un = KIND == kBf16 ? 1.0f : s.row_unmult[base + tok];
         a *= un;
         b *= un;
@@ -524,158 +459,122 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
           if (GATEUP) b *= __ldg(p.s_up + (int64_t)it.expert * sh.N + row);
         }
         if (GATEUP) a = a / (1.0f + expf(-a)) * b;
-        if (chain == 0) (GATEUP ? p.act : p.Y)[(int64_t)pair * sh.N + row] = a;
+        (GATEUP ? p.act : p.Y)[(int64_t)s.row_pair[base + tok] * sh.N + row] = a;
       }
       if constexpr (GATEUP && KIND != kBf16) {
         float m = in ? fabsf(a) : 0.f;
 #pragma unroll
         for (int x = kOuts / 2; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, x));
         // magnitudes order as their bits do, a NaN above all
-        if (r == 0 && chain == 0 && in) atomicMax(p.row_max + pair, __float_as_uint(m) & 0x7fffffffu);
+        if (r == 0 && in) atomicMax(p.row_max + s.row_pair[base + tok], __float_as_uint(m) & 0x7fffffffu);
       }
     }
 }
 
-// The tiles of an item of up to 4 GROUPS tokens. All sixteen warps take part in each: a sub-tile has 16 / subs of them, and a warp one or
-// (EIGHT) two runs of 128 bytes of a slice of its rows; their sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
+// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y. The sixteen warps are four groups of four, which take the
+// tiles in turn, so that a tile's chain of waits, loads and MMAs runs beside three others (all warps at one tile took three times as long as
+// HBM needs to bring it). Of a group a sub-tile has 4 / subs warps, each with every 4 / subs-th run of 128 bytes of its rows, about four; the
+// sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
+// Every warp waits for every slot and releases it, in order, whether it reads it or not: a group that ran ahead or behind by the ring's
+// length would take one phase of a barrier for another.
 // A warp whose wait gives up raises s.fail, waits no more and frees no slot, but meets every barrier; what it forms then is never used.
-// (Sub-tiles in slots of their own would let the groups of warps drift apart, past what a barrier's two phases tell apart.)
-// Shared memory's bandwidth is what the products would be bound by: 32 KB of weights are 256 cycles of its 128 bytes, in some 1400 that
-// HBM takes to bring them. HOLD: the planes of the tokens, read once for all tiles, stay in registers where a row is one slice; read
-// from shared memory at each step those of four tokens cost as much as the weights.
-template <int KIND, bool GATEUP, bool EIGHT, int GROUPS, bool HOLD>
-__device__ __forceinline__ void run_tiles(const DecodeParams &p, Shared &s, const Item &it, int base, Ring &ring, const uint8_t *panel, float *sums,
-                                          uint8_t *slots) {
-  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kRuns = EIGHT ? 2 : 1, kRunBytes = kWarps * 128;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-  const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = kWarps / subs, sub = warp & (subs - 1), part = warp / subs;
-  const int tiles = (it.r1 - it.r0 + sh.outs - 1) / sh.outs, batch = kRed / (64 * kWarps * it.n);
-  // this lane's bytes of rows g and g + 8 of its sub-tile in a slot, of gate and up of row g of either; EIGHT: of the slot's row g
-  const bool swap = (g & 1) && (sh.slice & 64) == 0;
-  const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16, row1 = row0 + (GATEUP ? sh.outs : 8) * sh.slice;
-  const uint8_t *rows[GROUPS];   // this lane's run of a plane of one of each four tokens
-#pragma unroll
-  for (int q = 0; q < GROUPS; ++q)
-    rows[q] = panel + (2 * (base + min(4 * q + (g >> 1), it.n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
-  Acts<KIND> held[HOLD ? kRuns : 1][2][GROUPS];
-  if constexpr (HOLD) {
-#pragma unroll
-    for (int r = 0; r < kRuns; ++r)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int q = 0; q < GROUPS; ++q)
-          if (part * 128 + r * kRunBytes + u * 64 < sh.row_bytes) held[r][u][q].load(rows[q] + (r * kRunBytes + u * 64) * (2 / kElem));
-          else held[r][u][q].clear();
-  }
-  for (int tile = 0, in_batch = 0; tile < tiles; ++tile) {
-    const int first_row = it.r0 + tile * sh.outs + sub * kOuts;
-    const bool mine = first_row < it.r1;   // the last tile may have fewer sub-tiles
-    constexpr int kChains = GROUPS == 1 ? 2 : 1;
-    float acc[GROUPS][kChains][4];
-#pragma unroll
-    for (int q = 0; q < GROUPS; ++q)
-#pragma unroll
-      for (int u = 0; u < kChains; ++u)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[q][u][c] = 0.f;
-    const float *sc0 = nullptr, *sc1 = nullptr;   // e4m3: scales of the blocks of rows g and g + 8, or of row g
-    if constexpr (KIND == kE4) {
-      const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128;
-      const bool up = EIGHT && GATEUP && g >= 4;
-      sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((first_row + g - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
-      sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((first_row + g + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
-    }
-    for (int sl = 0; sl < (HOLD ? 1 : sh.slices); ++sl) {
-      const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
-      float f[kRuns][2];
-      if constexpr (KIND == kE4) {
-#pragma unroll
-        for (int r = 0; r < kRuns; ++r) {
-          const int at = sl * (sh.slice / 128) + r * kWarps;
-          f[r][0] = left > r * kRunBytes ? __ldg(sc0 + at) : 0.f;
-          f[r][1] = EIGHT ? 0.f : left > r * kRunBytes ? __ldg(sc1 + at) : 0.f;
-        }
-      }
-      if (warp == kFiller && ring.ok && !fill(p, s, slots, ring.n, ring.read + 1)) ring.ok = false;
-      if (ring.ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ring.ok = false;
-      ring.ok = __all_sync(0xffffffffu, ring.ok);
-      const uint8_t *slot = slots + ring.at * kSlot;
-      Weights v[kRuns];
-#pragma unroll
-      for (int r = 0; r < kRuns; ++r)
-        if (left > r * kRunBytes) load_run<EIGHT>(v[r], slot + row0 + r * kRunBytes, slot + row1 + r * kRunBytes, swap, left - r * kRunBytes);
-      __syncwarp();
-      if (lane == 0 && ring.ok) mbar_arrive(&s.empty[ring.at]);
-      ring.next();
-#pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        if (left <= r * kRunBytes) break;
-        // The steps' sums are chains of their own where there is one group, and under e4m3's scales of the run's block everywhere.
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (!HOLD && left - r * kRunBytes <= u * 64) break;
-          const Step<KIND> w(v[r].w[u]);
-#pragma unroll
-          for (int q = 0; q < GROUPS; ++q) {
-            Acts<KIND> x;
-            if constexpr (HOLD) x = held[r][u][q];
-            else x.load(rows[q] + (sl * sh.slice + r * kRunBytes + u * 64) * (2 / kElem));
-            if constexpr (KIND == kE4) {
-              float t[4] = {0.f, 0.f, 0.f, 0.f};
-              w.times(x, t);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) acc[q][u % kChains][c] = fmaf(f[r][c >> 1], t[c], acc[q][u % kChains][c]);
-            } else {
-              w.times(x, acc[q][u % kChains]);
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < GROUPS; ++q)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (kChains == 2) acc[q][0][c] += acc[q][kChains - 1][c];
-    float *red = sums + ring.turn * (kRed / 4), *dst = red + (((in_batch * subs + sub) * parts + part) * it.n + j) * 16 + g;
-#pragma unroll
-    for (int q = 0; q < GROUPS; ++q)
-      if (mine && 4 * q + j < it.n) {
-        dst[q * 64] = acc[q][0][0] + acc[q][0][1];
-        if (!EIGHT) dst[q * 64 + 8] = acc[q][0][2] + acc[q][0][3];
-      }
-    if (++in_batch != batch && tile + 1 < tiles) continue;
-    __syncthreads();
-    add_parts<KIND, GATEUP, EIGHT>(p, s, it, base, red, in_batch * subs, it.r0 + (tile + 1 - in_batch) * sh.outs);
-    in_batch = 0;
-    ring.turn ^= 1;   // who still adds is met at the next barrier
-  }
-}
-
-// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y
 template <int KIND, bool GATEUP>
-__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *red, uint8_t *slots) {
+__device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *sums, const uint8_t *slots) {
+  constexpr int kElem = Geo<KIND>::kElem, kOuts = GATEUP ? 8 : 16;   // of a sub-tile
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
   const Plan &plan = s.plan[GATEUP ? 0 : 1];
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  int built = 0, base = 0;
+  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = 4 / subs, group = warp >> 2, sub = warp & (subs - 1), part = (warp & 3) / subs;
+  // this lane's bytes of rows g and g + 8 of its sub-tile in a slot; of gate and up these are row g of either
+  const bool swap = (g & 1) && (sh.slice & 64) == 0;
+  const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16;
+  int built = 0, base = 0, turn = 0;   // turn: whose tile it is
+  bool ok = true;
   for (int i = 0; i < plan.n_items; ++i) {
     const Item &it = plan.item[i];
     if (i >= built) {
-      __syncthreads();   // the last panel is read
+      meet();   // the last panel is read
       built = build_panel<KIND, GATEUP>(p, s, plan, sh.K, panel, i);
       base = 0;
-      __syncthreads();
+      meet();
     }
-    auto go = [&](auto eight) {
-      constexpr bool kEight = decltype(eight)::value;
-      if (it.n <= 4 && sh.slices == 1) run_tiles<KIND, GATEUP, kEight, 1, true>(p, s, it, base, ring, panel, red, slots);
-      else run_tiles<KIND, GATEUP, kEight, 2, false>(p, s, it, base, ring, panel, red, slots);
-    };
-    if (sh.eight) go(std::true_type());
-    else go(std::false_type());
-    base += it.n;
+    const int n = it.n, last = it.r1, batch = kRed / (64 * 4 * n);   // tiles whose sums fit
+    // this lane's run of a plane of one of the first four tokens, and of the others
+    const uint8_t *x0 = panel + (2 * (base + min(g >> 1, n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+    const uint8_t *x1 = panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+    int in_batch = 0;
+    for (int first = it.r0; first < last; first += sh.outs) {
+      const bool mine = turn == group && first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
+      turn = (turn + 1) & 3;
+      float acc[2][4] = {};
+      const float *sc0 = nullptr, *sc1 = nullptr;   // e4m3: scales of the blocks of rows g and g + 8
+      if constexpr (KIND == kE4)
+        if (mine) {
+          const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128, row = first + sub * kOuts + g;
+          sc0 = (GATEUP ? p.s_gate : p.s_down) + ((int64_t)it.expert * nb + min(row / 128, nb - 1)) * kb + part;
+          sc1 = (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
+        }
+      for (int sl = 0; sl < sh.slices; ++sl) {
+        const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
+        float f[4][2];
+        if constexpr (KIND == kE4) {   // of the up to four runs, ahead of the wait
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = sl * (sh.slice / 128) + r * parts;
+            f[r][0] = left > r * parts * 128 ? __ldg(sc0 + at) : 0.f;
+            f[r][1] = left > r * parts * 128 ? __ldg(sc1 + at) : 0.f;
+          }
+        }
+        if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        const uint8_t *slot = slots + ring.at * kSlot + row0;
+        const int at = sl * sh.slice * (2 / kElem);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int rest = left - r * parts * 128;
+          if (rest <= 0) break;
+          Weights v;
+          load_run(v, slot + r * parts * 128, slot + r * parts * 128 + (GATEUP ? sh.outs : 8) * sh.slice, swap, rest);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (rest <= u * 64) break;
+            const Step<KIND> w(v.w[u]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              if (q == 1 && n <= 4) break;
+              Acts<KIND> x;
+              x.load((q == 0 ? x0 : x1) + at + (r * parts * 128 + u * 64) * (2 / kElem));
+              if constexpr (KIND == kE4) {
+                float t[4] = {};
+                w.times(x, t);
+                acc[q][0] = fmaf(f[r][0], t[0], acc[q][0]);
+                acc[q][1] = fmaf(f[r][0], t[1], acc[q][1]);
+                acc[q][2] = fmaf(f[r][1], t[2], acc[q][2]);
+                acc[q][3] = fmaf(f[r][1], t[3], acc[q][3]);
+              } else {
+                w.times(x, acc[q]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
+        ring.next();
+      }
+      float *dst = sums + (((in_batch * subs + sub) * parts + part) * n + j) * 16 + g;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (mine && 4 * q + j < n) {
+          dst[q * 64] = acc[q][0] + acc[q][1];
+          dst[q * 64 + 8] = acc[q][2] + acc[q][3];
+        }
+      if (++in_batch != batch && first + sh.outs < last) continue;
+      meet();
+      add_parts<KIND, GATEUP>(p, s, it, base, sums, in_batch * subs, first - (in_batch - 1) * sh.outs);
+      in_batch = 0;
+      meet();
+    }
+    base += n;
   }
 }
 
@@ -794,7 +693,7 @@ __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &
 #pragma unroll
       for (int k = 0; k < SIDE; ++k) dot[i][k] = warp_sum(dot[i][k]);
     }
-    __syncthreads();   // the last tile's sums are read
+    meet();   // the last tile's sums are read
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < SIDE; ++i) {
@@ -804,7 +703,7 @@ __device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &
         for (int k = 0; k < SIDE; ++k) s.part[warp][i][2 + k] = dot[i][k];
       }
     }
-    __syncthreads();
+    meet();
     const int i = warp, t = t0 + i;   // a warp per token, lane l the sum of value l
     if (i >= SIDE || t >= p.T) continue;
     float v = 0.f;
@@ -960,7 +859,7 @@ __device__ void give_up(const DecodeParams &p, Shared &s) {
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -975,11 +874,13 @@ __global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_co
     s.fail = 0;
     mbar_init_fence();
   }
-  if (p.T == 1) norms_and_logits<1>(p, s);
-  else if (p.T <= 4) norms_and_logits<2>(p, s);
-  else norms_and_logits<4>(p, s);
-  grid_arrive(p, s);
-  if (!grid_wait(p, s, 1)) return give_up(p, s);
+  if (warp < kWarps) {
+    if (p.T == 1) norms_and_logits<1>(p, s);
+    else if (p.T <= 4) norms_and_logits<2>(p, s);
+    else norms_and_logits<4>(p, s);
+  }
+  grid_arrive<kAll>(p, s);
+  if (!grid_wait<kAll>(p, s, 1)) return give_up(p, s);
 
   // ---- routing: a warp per token ----
   if (warp < p.T) {
@@ -1015,38 +916,36 @@ __global__ void __launch_bounds__(kThreads, 1) moe_decode_kernel(const __grid_co
     if (lane == 0) s.n_active = n;
     __syncwarp();
     if (lane < 2) make_plan(p, s.plan[lane], s, lane == 0 ? p.F : p.H, Geo<KIND>::cap(lane == 0 ? p.H : p.F));
-    __syncwarp();
-    if (lane == 0) {
-      const int first = s.plan[0].n_items > 0 ? 0 : s.plan[1].n_items > 0 ? 1 : 2;
-      s.next = Cursor{first, 0, first < 2 ? s.plan[first].item[0].r0 : 0, 0, 0, 0, 0u};
-    }
   }
   __syncthreads();
 
-  float *red = reinterpret_cast<float *>(smem);
-  uint8_t *panel = smem + 2 * kRed;
+  float *sums = reinterpret_cast<float *>(smem);
+  uint8_t *panel = smem + kRed;
   const int held = max(s.plan[0].rows * 2 * Geo<KIND>::pitch(p.H), s.plan[1].rows * 2 * Geo<KIND>::pitch(p.F));
-  const int at = 2 * kRed + (held + 127) / 128 * 128;
+  const int at = kRed + (held + 127) / 128 * 128;
   uint8_t *slots = smem + at;
-  Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u, 0, 0, true};
-  if (warp == kFiller) ring.ok = fill(p, s, slots, ring.n, 0);
-  run_product<KIND, true>(p, s, ring, panel, red, slots);
-  grid_arrive(p, s);
-  if (warp == kFiller && ring.ok) ring.ok = fill(p, s, slots, ring.n, 0);   // down's rows travel while the grid meets
+  Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u};
+  if (warp == kWarps) {
+    int copied = 0;
+    if (!feed(p, s, 0, ring, slots, copied) || !feed(p, s, 1, ring, slots, copied)) {
+      // the slots filled last may still be written: shared memory is not left before they are
+      if (lane < ring.n && copied > lane) mbar_wait_for(&s.full[lane], (uint32_t)((copied - lane - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
+    }
+    return;
+  }
+  run_product<KIND, true>(p, s, ring, panel, sums, slots);
+  grid_arrive<kThreads>(p, s);
   const int t = blockIdx.x;
-  bool ok = grid_wait(p, s, 2);
+  bool ok = grid_wait<kThreads>(p, s, 2);
   if (ok) {
-    run_product<KIND, false>(p, s, ring, panel, red, slots);
-    grid_arrive(p, s);
+    run_product<KIND, false>(p, s, ring, panel, sums, slots);
+    grid_arrive<kThreads>(p, s);
     Finish end;
     if (t < p.T) end.prepare(p, s, t);
-    ok = grid_wait(p, s, 3);
+    ok = grid_wait<kThreads>(p, s, 3);
     if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
   }
-  if (ok) return;
-  give_up(p, s);
-  // the slots filled last may still be written: shared memory is not left before they are
-  if (tid < ring.n && s.next.copied > tid) mbar_wait_for(&s.full[tid], (uint32_t)((s.next.copied - tid - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
+  if (!ok) give_up(p, s);   // ends the copying warp's waits, too
 }
 
 template <int KIND>
@@ -1058,9 +957,8 @@ int launch(DecodeParams &p, cudaStream_t st) {
     sh.row_bytes = sh.K * Geo<KIND>::kElem;
     sh.slices = (sh.row_bytes + kSlice - 1) / kSlice;
     sh.slice = sh.slices == 1 ? sh.row_bytes : ((sh.row_bytes + sh.slices - 1) / sh.slices + 127) / 128 * 128;
-    sh.eight = sh.row_bytes > kSlice / 2;
-    sh.subs = sh.row_bytes <= kSlice / 8 ? 4 : sh.row_bytes <= kSlice / 4 ? 2 : 1;
-    sh.outs = (i == 0 ? 8 : 16) * sh.subs / (sh.eight ? 2 : 1);
+    sh.subs = sh.row_bytes <= kSlice / 4 ? 4 : sh.row_bytes <= kSlice / 2 ? 2 : 1;
+    sh.outs = (i == 0 ? 8 : 16) * sh.subs;
   }
   int dev = 0;
   KNJ_CUDA(cudaGetDevice(&dev));
@@ -1072,7 +970,7 @@ int launch(DecodeParams &p, cudaStream_t st) {
   }
   KNJ_CUDA(cudaMemsetAsync(p.sync, 0, kCleared, st));
   void *args[] = {&p};
-  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kThreads), args, kSmem, st));
+  KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kAll), args, kSmem, st));
   return launch_status("moe_decode_kernel");
 }
 
