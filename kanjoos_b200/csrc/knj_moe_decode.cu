@@ -20,8 +20,9 @@
 //   3  down, likewise
 //   4  weighted sum, norm, gate, residual, next norm: a CTA for each token
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
+#include <type_traits>
+
 #include "knj_fp8.cuh"
-#include "knj_topk.cuh"
 
 using namespace knj;
 
@@ -100,6 +101,7 @@ struct Shared {
   float inv[kMaxTokens], mult[kMaxTokens], unmult[kMaxTokens];
   int sel_e[kMaxTokens][kMaxK];
   float sel_w[kMaxTokens][kMaxK];
+  int order[kMaxTokens][kMaxK];   // a token's choices by ascending expert
   unsigned mask[kMaxExperts];
   uint8_t pair_at[kMaxExperts][kMaxTokens];   // pairs of an expert's tokens in ascending order
   int active[kMaxTokens * kMaxK];
@@ -254,8 +256,8 @@ __device__ __forceinline__ float cta_sum(float v, float *red) {   // by all thre
 template <int KIND>
 struct Geo {
   static constexpr int kElem = KIND <= kF16 ? 2 : 1;
-  // bytes of a plane of K values: whole steps, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
-  __host__ __device__ static int pitch(int K) { return (2 * K + 127) / 128 * 128 + (kElem == 2 ? 64 : 16); }
+  // bytes of a plane of K values: whole runs of 128 bytes of weights, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
+  __host__ __device__ static int pitch(int K) { return (K * kElem + 127) / 128 * (256 / kElem) + (kElem == 2 ? 64 : 16); }
   // rows in the panel at a time: what leaves the ring two slots, or one
   __host__ __device__ static int cap(int K) {
     const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
@@ -307,28 +309,26 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
   return true;
 }
 
-// A lane's part of a run of 128 bytes (two steps of 64) of sixteen rows: of rows g and g + 8 the bytes 16 j .. + 15 of either step.
+// A lane's part of a run of 128 bytes (two steps of 64) of sixteen rows: of rows g and g + 8 the bytes 16 j .. + 15 of either step. (Rows a
+// multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. Letting odd rows read their second step first and
+// swapping in registers avoids that and costs sixteen instructions a run, which are dearer.) left: bytes of the rows from the run's first
+// on; what lies behind is zero.
 struct Weights {
   uint4 w[2][2];   // [step][row]
+  __device__ __forceinline__ void load(const uint8_t *row0, const uint8_t *row1, int left) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      w[u][0] = *reinterpret_cast<const uint4 *>(row0 + 64 * u);
+      w[u][1] = *reinterpret_cast<const uint4 *>(row1 + 64 * u);
+    }
+    if (left < 128) {
+      const int at = (threadIdx.x & 3) * 16;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u * 64 + at >= left) w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+    }
+  }
 };
-// Rows a multiple of 128 bytes apart lie on the same banks, and a load of shared memory serves two of them at a time: the odd one reads its
-// second step first, and the two change places in registers. left: bytes of the rows from the run's first on; what lies behind is zero.
-__device__ __forceinline__ void load_run(Weights &v, const uint8_t *row0, const uint8_t *row1, bool swap, int left) {
-  const int first = swap ? 64 : 0;
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const uint8_t *row = m == 0 ? row0 : row1;
-    const uint4 a = *reinterpret_cast<const uint4 *>(row + first), b = *reinterpret_cast<const uint4 *>(row + 64 - first);
-    v.w[0][m] = swap ? b : a;
-    v.w[1][m] = swap ? a : b;
-  }
-  if (left < 128) {
-    const int at = (threadIdx.x & 3) * 16;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (u * 64 + at >= left) v.w[u][0] = v.w[u][1] = make_uint4(0, 0, 0, 0);
-  }
-}
 // a lane's run of a plane for a step
 template <int KIND>
 struct Acts {
@@ -338,37 +338,35 @@ struct Acts {
     if constexpr (KIND > kF16) b[1] = *reinterpret_cast<const uint4 *>(at + 16);
   }
 };
-// One step of sixteen rows as MMA operands, and its products with the planes of four tokens
-template <int KIND>
-struct Step {
-  uint32_t a[KIND <= kF16 ? 2 : 4][4];
-  __device__ __forceinline__ explicit Step(const uint4 (&w)[2]) {
-    if constexpr (KIND <= kF16) {
-      a[0][0] = w[0].x; a[0][1] = w[1].x; a[0][2] = w[0].y; a[0][3] = w[1].y;
-      a[1][0] = w[0].z; a[1][1] = w[1].z; a[1][2] = w[0].w; a[1][3] = w[1].w;
-    } else {
-      const uint32_t r0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, r1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+// One step of sixteen rows times the planes of four tokens, or (TWO) of eight
+template <int KIND, bool TWO>
+__device__ __forceinline__ void step(const uint4 (&w)[2], const uint8_t *x0, const uint8_t *x1, float (&acc0)[4], float (&acc1)[4]) {
+  Acts<KIND> a, b;
+  a.load(x0);
+  if constexpr (TWO) b.load(x1);
+  if constexpr (KIND <= kF16) {
+    mma<KIND>(acc0, w[0].x, w[1].x, w[0].y, w[1].y, a.b[0].x, a.b[0].y);
+    if constexpr (TWO) mma<KIND>(acc1, w[0].x, w[1].x, w[0].y, w[1].y, b.b[0].x, b.b[0].y);
+    mma<KIND>(acc0, w[0].z, w[1].z, w[0].w, w[1].w, a.b[0].z, a.b[0].w);
+    if constexpr (TWO) mma<KIND>(acc1, w[0].z, w[1].z, w[0].w, w[1].w, b.b[0].z, b.b[0].w);
+  } else {
+    const uint32_t r0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, r1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        codes_f16<KIND>(r0[i], a[i][0], a[i][2]);
-        codes_f16<KIND>(r1[i], a[i][1], a[i][3]);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t c[4];
+      codes_f16<KIND>(r0[i], c[0], c[2]);
+      codes_f16<KIND>(r1[i], c[1], c[3]);
+      const uint4 &p = a.b[i >> 1];
+      mma<KIND>(acc0, c[0], c[1], c[2], c[3], i & 1 ? p.z : p.x, i & 1 ? p.w : p.y);
+      if constexpr (TWO) {
+        const uint4 &q = b.b[i >> 1];
+        mma<KIND>(acc1, c[0], c[1], c[2], c[3], i & 1 ? q.z : q.x, i & 1 ? q.w : q.y);
       }
     }
   }
-  __device__ __forceinline__ void times(const Acts<KIND> &x, float (&acc)[4]) const {
-    if constexpr (KIND <= kF16) {
-      mma<KIND>(acc, a[0][0], a[0][1], a[0][2], a[0][3], x.b[0].x, x.b[0].y);
-      mma<KIND>(acc, a[1][0], a[1][1], a[1][2], a[1][3], x.b[0].z, x.b[0].w);
-    } else {
-      mma<KIND>(acc, a[0][0], a[0][1], a[0][2], a[0][3], x.b[0].x, x.b[0].y);
-      mma<KIND>(acc, a[1][0], a[1][1], a[1][2], a[1][3], x.b[0].z, x.b[0].w);
-      mma<KIND>(acc, a[2][0], a[2][1], a[2][2], a[2][3], x.b[1].x, x.b[1].y);
-      mma<KIND>(acc, a[3][0], a[3][1], a[3][2], a[3][3], x.b[1].z, x.b[1].w);
-    }
-  }
-};
+}
 
-// The rows of items i .. in the panel, as many as it takes: their planes, zeros behind K up to whole steps. Returns the item behind them.
+// The rows of items i .. in the panel, as many as it takes: their planes, zeros behind K up to whole runs. Returns the item behind them.
 template <int KIND, bool GATEUP>
 __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, const Plan &plan, int K, uint8_t *panel, int i) {
   const int tid = threadIdx.x, pitch = Geo<KIND>::pitch(K);
@@ -390,7 +388,9 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
     }
   }
   meet();
-  const int chunks = (K + 63) / 64 * 8, runs = (chunks + 31) / 32;   // of eight values; of 32 such: a warp's
+  // of eight values, up to the end of a run of 128 bytes of weights; and of 32 such: a warp's
+  constexpr int kRun = 128 / Geo<KIND>::kElem;
+  const int chunks = (K + kRun - 1) / kRun * (kRun / 8), runs = (chunks + 31) / 32;
 #pragma unroll 2
   for (int u = tid >> 5; u < n * runs; u += kWarps) {
     const int r = u / runs, c = (u - r * runs) * 32 + (tid & 31);
@@ -486,7 +486,6 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
   const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = 4 / subs, group = warp >> 2, sub = warp & (subs - 1), part = (warp & 3) / subs;
   // this lane's bytes of rows g and g + 8 of its sub-tile in a slot; of gate and up these are row g of either
-  const bool swap = (g & 1) && (sh.slice & 64) == 0;
   const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16;
   int built = 0, base = 0, turn = 0;   // turn: whose tile it is
   bool ok = true;
@@ -504,70 +503,81 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
     const uint8_t *x1 = panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
     int in_batch = 0;
     for (int first = it.r0; first < last; first += sh.outs) {
-      const bool mine = turn == group && first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
-      turn = (turn + 1) & 3;
-      float acc[2][4] = {};
-      const float *sc0 = nullptr, *sc1 = nullptr;   // e4m3: scales of the blocks of rows g and g + 8
-      if constexpr (KIND == kE4)
-        if (mine) {
+      if (turn != group) {
+        for (int sl = 0; sl < sh.slices; ++sl) {
+          if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
+          ring.next();
+        }
+      } else {
+        const bool mine = first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
+        float acc[3][4] = {};                           // tokens 0 .. 3, even and odd steps; 4 .. 7
+        const float *sc0 = nullptr, *sc1 = nullptr;     // e4m3: scales of the blocks of rows g and g + 8
+        if constexpr (KIND == kE4) {
           const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128, row = first + sub * kOuts + g;
           sc0 = (GATEUP ? p.s_gate : p.s_down) + ((int64_t)it.expert * nb + min(row / 128, nb - 1)) * kb + part;
           sc1 = (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
         }
-      for (int sl = 0; sl < sh.slices; ++sl) {
-        const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
-        float f[4][2];
-        if constexpr (KIND == kE4) {   // of the up to four runs, ahead of the wait
+        for (int sl = 0; sl < sh.slices; ++sl) {
+          const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
+          float f[4][2];
+          if constexpr (KIND == kE4) {   // of the up to four runs, ahead of the wait
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int at = sl * (sh.slice / 128) + r * parts;
-            f[r][0] = left > r * parts * 128 ? __ldg(sc0 + at) : 0.f;
-            f[r][1] = left > r * parts * 128 ? __ldg(sc1 + at) : 0.f;
-          }
-        }
-        if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        const uint8_t *slot = slots + ring.at * kSlot + row0;
-        const int at = sl * sh.slice * (2 / kElem);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int rest = left - r * parts * 128;
-          if (rest <= 0) break;
-          Weights v;
-          load_run(v, slot + r * parts * 128, slot + r * parts * 128 + (GATEUP ? sh.outs : 8) * sh.slice, swap, rest);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (rest <= u * 64) break;
-            const Step<KIND> w(v.w[u]);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              if (q == 1 && n <= 4) break;
-              Acts<KIND> x;
-              x.load((q == 0 ? x0 : x1) + at + (r * parts * 128 + u * 64) * (2 / kElem));
-              if constexpr (KIND == kE4) {
-                float t[4] = {};
-                w.times(x, t);
-                acc[q][0] = fmaf(f[r][0], t[0], acc[q][0]);
-                acc[q][1] = fmaf(f[r][0], t[1], acc[q][1]);
-                acc[q][2] = fmaf(f[r][1], t[2], acc[q][2]);
-                acc[q][3] = fmaf(f[r][1], t[3], acc[q][3]);
-              } else {
-                w.times(x, acc[q]);
-              }
+            for (int r = 0; r < 4; ++r) {
+              const int at = sl * (sh.slice / 128) + r * parts;
+              f[r][0] = left > r * parts * 128 ? __ldg(sc0 + at) : 0.f;
+              f[r][1] = left > r * parts * 128 ? __ldg(sc1 + at) : 0.f;
             }
           }
-        }
-        __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
-        ring.next();
-      }
-      float *dst = sums + (((in_batch * subs + sub) * parts + part) * n + j) * 16 + g;
+          if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          const uint8_t *slot = slots + ring.at * kSlot + row0, *slot1 = slot + (GATEUP ? sh.outs : 8) * sh.slice;
+          const int at = sl * sh.slice * (2 / kElem), run = parts * 128;
+          auto runs = [&](auto two) {
+            constexpr bool kTwo = decltype(two)::value;
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (mine && 4 * q + j < n) {
-          dst[q * 64] = acc[q][0] + acc[q][1];
-          dst[q * 64 + 8] = acc[q][2] + acc[q][3];
+            for (int r = 0; r < 4; ++r) {
+              const int rest = left - r * run;
+              if (rest <= 0) break;
+              Weights v;
+              v.load(slot + r * run, slot1 + r * run, rest);
+              // the second step may lie behind the row's end: its weights are zeros then, and the planes reach to the end of a run
+              float t[2][4] = {};
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int here = at + (r * run + u * 64) * (2 / kElem);
+                if constexpr (KIND == kE4) step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, t[0], t[1]);
+                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, acc[u], acc[2]);
+              }
+              if constexpr (KIND == kE4) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  acc[0][c] = fmaf(f[r][c >> 1], t[0][c], acc[0][c]);
+                  if (kTwo) acc[2][c] = fmaf(f[r][c >> 1], t[1][c], acc[2][c]);
+                }
+              }
+            }
+          };
+          if (n <= 4) runs(std::false_type());
+          else runs(std::true_type());
+          __syncwarp();
+          if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
+          ring.next();
         }
+        if (mine) {
+          float *dst = sums + (((in_batch * subs + sub) * parts + part) * n + j) * 16 + g;
+          if (j < n) {
+            dst[0] = (acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1]);
+            dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
+          }
+          if (4 + j < n) {
+            dst[64] = acc[2][0] + acc[2][1];
+            dst[72] = acc[2][2] + acc[2][3];
+          }
+        }
+      }
+      turn = (turn + 1) & 3;
       if (++in_batch != batch && first + sh.outs < last) continue;
       meet();
       add_parts<KIND, GATEUP>(p, s, it, base, sums, in_batch * subs, first - (in_batch - 1) * sh.outs);
@@ -576,6 +586,57 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
     }
     base += n;
   }
+}
+
+// A token's experts and weights, by one warp: top-k of the logits by (value descending, expert ascending), a softmax over the chosen ones (the
+// others' part of the softmax over all falls out where the weights are renormalised). Lane l's experts are 32 i + l; every lane sorts its own
+// (stable), and a round then takes the largest of the lanes' heads. -inf is the least of all values: with fewer than k others such experts
+// follow, weight 0; of a row of -inf alone all weights are 0.
+template <int EPL>
+__device__ __forceinline__ void choose(const float *logits, int E, int k, int lane, int *sel_e, float *sel_w) {
+  unsigned key[EPL];
+  int id[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    // order-preserving: larger float <=> larger unsigned key; 0 only past the last expert
+    const unsigned u = i * 32 + lane < E ? __float_as_uint(__ldcg(logits + i * 32 + lane)) : 0u;
+    key[i] = i * 32 + lane < E ? max(1u, (u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;
+    id[i] = i * 32 + lane;
+  }
+#pragma unroll
+  for (int r = 0; r < EPL - 1; ++r)
+#pragma unroll
+    for (int i = EPL - 1; i > r; --i)
+      if (key[i] > key[i - 1]) {
+        const unsigned t = key[i]; key[i] = key[i - 1]; key[i - 1] = t;
+        const int d = id[i]; id[i] = id[i - 1]; id[i - 1] = d;
+      }
+  unsigned mine = 0u;   // lane s < k: key of the s-th choice
+#pragma unroll 1
+  for (int s = 0; s < k; ++s) {
+    const unsigned top = __reduce_max_sync(0xffffffffu, key[0]);
+    const unsigned holders = __ballot_sync(0xffffffffu, key[0] == top);
+    int src = __ffs(holders) - 1;
+    if (holders & (holders - 1u))   // equal logits: the smallest id among the lanes that hold one
+      src = __reduce_min_sync(0xffffffffu, key[0] == top ? id[0] : 0x7fffffff) & 31;
+    if (lane == s) mine = top;
+    if (lane == src) {
+      sel_e[s] = id[0];
+#pragma unroll
+      for (int i = 0; i + 1 < EPL; ++i) {
+        key[i] = key[i + 1];
+        id[i] = id[i + 1];
+      }
+      key[EPL - 1] = 0u;
+    }
+  }
+  const float v = __uint_as_float((mine & 0x80000000u) ? mine & 0x7fffffffu : ~mine), most = __shfl_sync(0xffffffffu, v, 0);
+  const float e = lane < k && v != -INFINITY ? expf(v - most) : 0.f;
+  float sum = e;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane < k) sel_w[lane] = sum == 0.f ? 0.f : e / sum;
+  __syncwarp();
 }
 
 // The rows of a product are dealt to the CTAs in equal numbers, in pairs of rows, over all active experts in a row; an expert's tokens
@@ -741,8 +802,6 @@ __device__ __forceinline__ float row_inverse(const float *row, int H, float ss, 
 // What stands behind the experts, of one token: a thread holds runs of four channels, the first of them with all that does not depend on
 // the experts read in front of the last barrier (prepare).
 struct Finish {
-  int order[kMaxK];      // pairs in ascending order of their experts
-  float weight[kMaxK];
   float4 x, post, gate, next;
 
   __device__ __forceinline__ void load(const DecodeParams &p, int t, int c) {
@@ -762,16 +821,7 @@ struct Finish {
     if (p.gate_sigmoid)
       gate = make_float4(1.0f / (1.0f + expf(-gate.x)), 1.0f / (1.0f + expf(-gate.y)), 1.0f / (1.0f + expf(-gate.z)), 1.0f / (1.0f + expf(-gate.w)));
   }
-  __device__ __forceinline__ void prepare(const DecodeParams &p, const Shared &s, int t) {
-#pragma unroll
-    for (int i = 0; i < kMaxK; ++i) order[i] = 0, weight[i] = 0.f;
-    for (int j = 0; j < p.k; ++j) {
-      int rank = 0;
-      for (int i = 0; i < p.k; ++i) rank += s.sel_e[t][i] < s.sel_e[t][j];
-#pragma unroll
-      for (int i = 0; i < kMaxK; ++i)
-        if (i == rank) order[i] = j, weight[i] = s.sel_w[t][j];
-    }
+  __device__ __forceinline__ void prepare(const DecodeParams &p, int t) {
     if (4 * threadIdx.x < p.H) load(p, t, 4 * threadIdx.x);
   }
   // row: H values in shared memory, of which a thread reads only its own (e4m3 rows: all)
@@ -783,14 +833,15 @@ struct Finish {
       float4 v[kMaxK], y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < kMaxK; ++j)
-        if (j < p.k) v[j] = __ldcg(reinterpret_cast<const float4 *>(p.Y + ((int64_t)t * p.k + order[j]) * H + c));
+        if (j < p.k) v[j] = __ldcg(reinterpret_cast<const float4 *>(p.Y + ((int64_t)t * p.k + s.order[t][j]) * H + c));
 #pragma unroll
       for (int j = 0; j < kMaxK; ++j)
         if (j < p.k) {
-          y.x = fmaf(weight[j], v[j].x, y.x);
-          y.y = fmaf(weight[j], v[j].y, y.y);
-          y.z = fmaf(weight[j], v[j].z, y.z);
-          y.w = fmaf(weight[j], v[j].w, y.w);
+          const float weight = s.sel_w[t][s.order[t][j]];
+          y.x = fmaf(weight, v[j].x, y.x);
+          y.y = fmaf(weight, v[j].y, y.y);
+          y.z = fmaf(weight, v[j].z, y.z);
+          y.w = fmaf(weight, v[j].w, y.w);
         }
       *reinterpret_cast<float4 *>(row + c) = y;
       ss = fmaf(y.x, y.x, fmaf(y.y, y.y, fmaf(y.z, y.z, fmaf(y.w, y.w, ss))));
@@ -885,15 +936,17 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   // ---- routing: a warp per token ----
   if (warp < p.T) {
     const float2 st = __ldcg(p.stats + warp);
-    int e;
-    float w;
-    warp_topk(p.logits + warp * p.E, p.E, p.k, lane, e, w);
+    if (p.E <= 128) choose<4>(p.logits + warp * p.E, p.E, p.k, lane, s.sel_e[warp], s.sel_w[warp]);
+    else choose<8>(p.logits + warp * p.E, p.E, p.k, lane, s.sel_e[warp], s.sel_w[warp]);
     if (lane < p.k) {
-      s.sel_e[warp][lane] = e;
-      s.sel_w[warp][lane] = w;
+      const int e = s.sel_e[warp][lane];
       atomicOr(&s.mask[e], 1u << warp);
       if (blockIdx.x == 0 && p.tap_exp) p.tap_exp[warp * p.k + lane] = e;
-      if (blockIdx.x == 0 && p.tap_w) p.tap_w[warp * p.k + lane] = w;
+      if (blockIdx.x == 0 && p.tap_w) p.tap_w[warp * p.k + lane] = s.sel_w[warp][lane];
+      // in ascending order of the experts, in which their rows are added
+      int rank = 0;
+      for (int i = 0; i < p.k; ++i) rank += s.sel_e[warp][i] < e;
+      s.order[warp][rank] = lane;
     }
     if (lane == 0) {
       s.inv[warp] = st.x;
@@ -906,14 +959,18 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     s.pair_at[e][__popc(s.mask[e] & ((1u << warp) - 1u))] = (uint8_t)(warp * p.k + lane);
   }
   if (warp == 0) {
-    int n = 0;
-    for (int b = 0; b < kMaxExperts; b += 32) {
-      const bool on = s.mask[b + lane] != 0u;
-      const unsigned all = __ballot_sync(0xffffffffu, on);
-      if (on) s.active[n + __popc(all & ((1u << lane) - 1u))] = b + lane;
-      n += __popc(all);
+    unsigned on = 0u;   // which of this lane's eight experts are active
+#pragma unroll
+    for (int i = 0; i < 8; ++i) on |= (s.mask[8 * lane + i] != 0u ? 1u : 0u) << i;
+    int at = __popc(on);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
     }
-    if (lane == 0) s.n_active = n;
+    if (lane == 31) s.n_active = at;
+    at -= __popc(on);
+    for (; on; on &= on - 1u) s.active[at++] = 8 * lane + __ffs(on) - 1;
     __syncwarp();
     if (lane < 2) make_plan(p, s.plan[lane], s, lane == 0 ? p.F : p.H, Geo<KIND>::cap(lane == 0 ? p.H : p.F));
   }
@@ -941,7 +998,7 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     run_product<KIND, false>(p, s, ring, panel, sums, slots);
     grid_arrive<kThreads>(p, s);
     Finish end;
-    if (t < p.T) end.prepare(p, s, t);
+    if (t < p.T) end.prepare(p, t);
     ok = grid_wait<kThreads>(p, s, 3);
     if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
   }
