@@ -35,11 +35,11 @@ constexpr int kMaxTokens = KNJ_MOE_DECODE_MAX_TOKENS, kMaxK = 8, kMaxExperts = 2
 // spilled, and took three times as long.
 constexpr int kThreads = 512, kWarps = kThreads / 32;   // that multiply; behind them the warp that copies
 constexpr int kAll = kThreads + 32;
-// A slot of the ring holds a tile: 64, 32 or 16 matrix rows of up to 512, 1024 or 2048 bytes as they lie, in one or two copies. (A copy for
-// each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536.) Longer rows come in slices
-// of up to 2048 bytes, sixteen rows to a slot.
-constexpr int kSlice = 2048;
-constexpr int kSlot = 16 * kSlice;
+// A slot of the ring holds a tile: 64, 32, 16 or 8 matrix rows of up to 512, 1024, 2048 or 4096 bytes as they lie, in one or two copies.
+// (A copy for each row passes the copy unit in some 100 cycles whatever its length: 768 bytes a row took as long as 1536, and rows of
+// 2048 bytes more than HBM needs to bring them.) Longer rows come in slices of up to 4096 bytes, eight rows to a slot.
+constexpr int kSlice = 4096;
+constexpr int kSlot = 8 * kSlice;
 constexpr int kMaxSlots = 6;
 constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 256 a tile and token
 constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
@@ -54,7 +54,8 @@ enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
 struct Shape {
   int K, N, row_bytes;
   int slices, slice;   // of a row, bytes
-  int subs;            // sub-tiles of 16 rows of a tile, each of which has 4 / subs warps
+  int eight;           // tiles of eight rows, else sub-tiles of sixteen
+  int subs;            // sub-tiles of a tile, each of which has 4 / subs warps
   int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
 };
 
@@ -313,13 +314,14 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
 // multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. Letting odd rows read their second step first and
 // swapping in registers avoids that and costs sixteen instructions a run, which are dearer.) left: bytes of the rows from the run's first
 // on; what lies behind is zero.
+template <bool EIGHT>
 struct Weights {
-  uint4 w[2][2];   // [step][row]
+  uint4 w[2][2];   // [step][row]; EIGHT: of row g alone
   __device__ __forceinline__ void load(const uint8_t *row0, const uint8_t *row1, int left) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       w[u][0] = *reinterpret_cast<const uint4 *>(row0 + 64 * u);
-      w[u][1] = *reinterpret_cast<const uint4 *>(row1 + 64 * u);
+      w[u][1] = EIGHT ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(row1 + 64 * u);
     }
     if (left < 128) {
       const int at = (threadIdx.x & 3) * 16;
@@ -433,9 +435,9 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
 
 // The sums over the parts of K of the sub-tiles 0 .. n-1 of a batch, whose first output is `first`, and what becomes of them: a warp per
 // sub-tile, lanes over tokens and outputs.
-template <int KIND, bool GATEUP>
+template <int KIND, bool GATEUP, bool EIGHT>
 __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, const Item &it, int base, const float *red, int n, int first) {
-  constexpr int kOuts = GATEUP ? 8 : 16;
+  constexpr int kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1);
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
   const int parts = 4 / sh.subs, tokens = it.n;
   for (int u = threadIdx.x >> 5; u < n; u += kWarps)
@@ -449,7 +451,7 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
         for (int w = 0; w < 4; ++w) {
           if (w >= parts) break;
           a += src[w * tokens * 16];
-          if (GATEUP) b += src[w * tokens * 16 + 8];
+          if (GATEUP) b += src[w * tokens * 16 + kOuts];
         }
         const float un = KIND == kBf16 ? 1.0f : s.row_unmult[base + tok];
         a *= un;
@@ -478,14 +480,14 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
 // Every warp waits for every slot and releases it, in order, whether it reads it or not: a group that ran ahead or behind by the ring's
 // length would take one phase of a barrier for another.
 // A warp whose wait gives up raises s.fail, waits no more and frees no slot, but meets every barrier; what it forms then is never used.
-template <int KIND, bool GATEUP>
+template <int KIND, bool GATEUP, bool EIGHT>
 __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *sums, const uint8_t *slots) {
-  constexpr int kElem = Geo<KIND>::kElem, kOuts = GATEUP ? 8 : 16;   // of a sub-tile
+  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kRuns = EIGHT ? 8 : 4;   // of a sub-tile; of a warp in a slice, at most
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
   const Plan &plan = s.plan[GATEUP ? 0 : 1];
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
   const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = 4 / subs, group = warp >> 2, sub = warp & (subs - 1), part = (warp & 3) / subs;
-  // this lane's bytes of rows g and g + 8 of its sub-tile in a slot; of gate and up these are row g of either
+  // this lane's bytes of row g of its sub-tile in a slot; row g + 8 is 8 rows behind it, or of gate and up row g of up. EIGHT: rows of gate, then of up
   const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16;
   int built = 0, base = 0, turn = 0;   // turn: whose tile it is
   bool ok = true;
@@ -516,18 +518,19 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
         const float *sc0 = nullptr, *sc1 = nullptr;     // e4m3: scales of the blocks of rows g and g + 8
         if constexpr (KIND == kE4) {
           const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128, row = first + sub * kOuts + g;
-          sc0 = (GATEUP ? p.s_gate : p.s_down) + ((int64_t)it.expert * nb + min(row / 128, nb - 1)) * kb + part;
-          sc1 = (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
+          const bool up = EIGHT && GATEUP && g >= 4;
+          sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((row - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
+          sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
         }
         for (int sl = 0; sl < sh.slices; ++sl) {
           const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
-          float f[4][2];
-          if constexpr (KIND == kE4) {   // of the up to four runs, ahead of the wait
+          float f[kRuns][2];
+          if constexpr (KIND == kE4) {   // of all runs, ahead of the wait
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < kRuns; ++r) {
               const int at = sl * (sh.slice / 128) + r * parts;
               f[r][0] = left > r * parts * 128 ? __ldg(sc0 + at) : 0.f;
-              f[r][1] = left > r * parts * 128 ? __ldg(sc1 + at) : 0.f;
+              f[r][1] = EIGHT ? 0.f : left > r * parts * 128 ? __ldg(sc1 + at) : 0.f;
             }
           }
           if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
@@ -537,10 +540,10 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           auto runs = [&](auto two) {
             constexpr bool kTwo = decltype(two)::value;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < kRuns; ++r) {
               const int rest = left - r * run;
               if (rest <= 0) break;
-              Weights v;
+              Weights<EIGHT> v;
               v.load(slot + r * run, slot1 + r * run, rest);
               // the second step may lie behind the row's end: its weights are zeros then, and the planes reach to the end of a run
               float t[2][4] = {};
@@ -569,18 +572,18 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           float *dst = sums + (((in_batch * subs + sub) * parts + part) * n + j) * 16 + g;
           if (j < n) {
             dst[0] = (acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1]);
-            dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
+            if (!EIGHT) dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
           }
           if (4 + j < n) {
             dst[64] = acc[2][0] + acc[2][1];
-            dst[72] = acc[2][2] + acc[2][3];
+            if (!EIGHT) dst[72] = acc[2][2] + acc[2][3];
           }
         }
       }
       turn = (turn + 1) & 3;
       if (++in_batch != batch && first + sh.outs < last) continue;
       meet();
-      add_parts<KIND, GATEUP>(p, s, it, base, sums, in_batch * subs, first - (in_batch - 1) * sh.outs);
+      add_parts<KIND, GATEUP, EIGHT>(p, s, it, base, sums, in_batch * subs, first - (in_batch - 1) * sh.outs);
       in_batch = 0;
       meet();
     }
@@ -990,12 +993,14 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     }
     return;
   }
-  run_product<KIND, true>(p, s, ring, panel, sums, slots);
+  if (p.shape[0].eight) run_product<KIND, true, true>(p, s, ring, panel, sums, slots);
+  else run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
   grid_arrive<kThreads>(p, s);
   const int t = blockIdx.x;
   bool ok = grid_wait<kThreads>(p, s, 2);
   if (ok) {
-    run_product<KIND, false>(p, s, ring, panel, sums, slots);
+    if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
+    else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
     grid_arrive<kThreads>(p, s);
     Finish end;
     if (t < p.T) end.prepare(p, t);
@@ -1014,8 +1019,9 @@ int launch(DecodeParams &p, cudaStream_t st) {
     sh.row_bytes = sh.K * Geo<KIND>::kElem;
     sh.slices = (sh.row_bytes + kSlice - 1) / kSlice;
     sh.slice = sh.slices == 1 ? sh.row_bytes : ((sh.row_bytes + sh.slices - 1) / sh.slices + 127) / 128 * 128;
-    sh.subs = sh.row_bytes <= kSlice / 4 ? 4 : sh.row_bytes <= kSlice / 2 ? 2 : 1;
-    sh.outs = (i == 0 ? 8 : 16) * sh.subs;
+    sh.eight = sh.row_bytes > kSlice / 2;
+    sh.subs = sh.row_bytes <= kSlice / 8 ? 4 : sh.row_bytes <= kSlice / 4 ? 2 : 1;
+    sh.outs = (i == 0 ? 8 : 16) * sh.subs / (sh.eight ? 2 : 1);
   }
   int dev = 0;
   KNJ_CUDA(cudaGetDevice(&dev));
