@@ -1,4 +1,4 @@
-// knj_moe_decode.cu -- a whole MoE block of a residual stream for up to sixteen tokens in one cooperative launch, experts in bf16,
+// knj_moe_decode.cu -- a whole MoE block of a residual stream for up to sixteen tokens in two kernels, experts in bf16,
 // fp16, e4m3 (one scale for each block of 128 x 128) or int8 (one for each output channel):
 //   h   = norm(x; pre_w)
 //   y   = sum over the top_k experts of softmax weight * down(silu(gate(h)) * up(h))
@@ -6,7 +6,7 @@
 // What is computed between x and out stays in f32, and so does what the matrices are multiplied with: a row of f32 values goes to the
 // tensor core as two 16-bit planes, hi = round(v) and lo = round(v - hi), which together hold 17 bits of v (bf16 experts, bf16 planes) or 22
 // (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). In mma.sync.m16n8k16 sixteen matrix rows
-// meet the two planes of four tokens, so that the second plane costs nothing while a step's weights are on their way.
+// meet the two planes of four tokens, or eight rows those of eight, so that the second plane costs nothing while weights are on their way.
 //
 // Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
 // its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
@@ -14,11 +14,11 @@
 // busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both operands
 // have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
 //
-// Stages, with a barrier over the grid between them:
-//   1  norm statistics (every CTA, all tokens) and router logits (an expert or two a CTA)
-//   2  top-k (every CTA for itself); gate, up, silu: every CTA has the same number of matrix rows, of all active experts in a row
-//   3  down, likewise
-//   4  weighted sum, norm, gate, residual, next norm: a CTA for each token
+// The first kernel forms norm statistics and router logits. The second, cooperative, has a CTA for each SM and two barriers over the grid:
+//   1  top-k (every CTA for itself); gate, up, silu: every CTA has the same number of matrix rows, of all active experts in a row
+//   2  down, likewise
+//   3  weighted sum, norm, gate, residual, next norm: a CTA for each token
+// (The first stage inside the cooperative kernel needed a third barrier and a fill that cleared its counter in front of the launch.)
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
 #include <type_traits>
 
@@ -44,8 +44,7 @@ constexpr int kMaxSlots = 6;
 constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 256 a tile and token
 constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
 constexpr int kMaxItems = 64;
-constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256,
-                 kCleared = kStatsAt - kSyncAt;   // of the workspace
+constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256;   // of the workspace
 constexpr float kDown = 0x1p-64f;
 
 enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
@@ -71,9 +70,9 @@ struct DecodeParams {
   int32_t *tap_exp;
   float *tap_w;
   float *logits, *act, *Y;
-  unsigned *sync;               // [0] arrivals, [1] raised by a wait that gave up; zero before the launch
+  unsigned *sync;               // [0] arrivals, [1] raised by a wait that gave up; cleared by the first kernel
   float2 *stats;                // [tokens] inverse norm, largest magnitude of the normalised row
-  unsigned *row_max;            // [pairs] bits of the largest magnitude of an activation row; zero before the launch
+  unsigned *row_max;            // [pairs] bits of the largest magnitude of an activation row; cleared by the first kernel
   int32_t *status;
   int64_t ldx, ldo, ldg, ldh;
   int T, H, F, E, k;
@@ -98,7 +97,6 @@ struct Plan {
 struct Shared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   int fail;                     // raised by a wait that gave up; read as volatile
-  float part[kWarps][4][6];  // of a token: squares, largest, dot products
   float inv[kMaxTokens], mult[kMaxTokens], unmult[kMaxTokens];
   int sel_e[kMaxTokens][kMaxK];
   float sel_w[kMaxTokens][kMaxK];
@@ -124,20 +122,13 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
 }
 // of the warps that multiply
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-template <int N>
-__device__ __forceinline__ void cta_barrier() {
-  if constexpr (N == kAll) __syncthreads();
-  else meet();
-}
-// Barrier over the grid, number `n` of the launch, in two halves, met by the first N threads of every CTA. A CTA in which a wait has given
-// up never arrives; grid_wait is false for all threads where the barrier did not complete in time.
-template <int N>
+// Barrier over the grid, number `n` of the launch, in two halves, met by the warps that multiply. A CTA in which a wait has given up never
+// arrives; grid_wait is false for all threads where the barrier did not complete in time.
 __device__ __forceinline__ void grid_arrive(const DecodeParams &p, Shared &s) {
-  cta_barrier<N>();
+  meet();
   if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0)
     asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.sync), "r"(1u) : "memory");
 }
-template <int N>
 __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int n) {
   if (threadIdx.x == 0) {
     int ok = *reinterpret_cast<volatile int *>(&s.fail) == 0;
@@ -148,7 +139,7 @@ __device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int 
     }
     s.ok = ok;
   }
-  cta_barrier<N>();
+  meet();
   return s.ok != 0;
 }
 
@@ -314,20 +305,20 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
 // multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. Letting odd rows read their second step first and
 // swapping in registers avoids that and costs sixteen instructions a run, which are dearer.) left: bytes of the rows from the run's first
 // on; what lies behind is zero.
-template <bool EIGHT>
+template <int ROWS>   // two, or of tiles of eight rows one
 struct Weights {
-  uint4 w[2][2];   // [step][row]; EIGHT: of row g alone
+  uint4 w[2][ROWS];   // [step][row]
   __device__ __forceinline__ void load(const uint8_t *row0, const uint8_t *row1, int left) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       w[u][0] = *reinterpret_cast<const uint4 *>(row0 + 64 * u);
-      w[u][1] = EIGHT ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(row1 + 64 * u);
+      if (ROWS == 2) w[u][ROWS - 1] = *reinterpret_cast<const uint4 *>(row1 + 64 * u);
     }
     if (left < 128) {
       const int at = (threadIdx.x & 3) * 16;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (u * 64 + at >= left) w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+        if (u * 64 + at >= left) w[u][0] = w[u][ROWS - 1] = make_uint4(0, 0, 0, 0);
     }
   }
 };
@@ -364,6 +355,27 @@ __device__ __forceinline__ void step(const uint4 (&w)[2], const uint8_t *x0, con
         const uint4 &q = b.b[i >> 1];
         mma<KIND>(acc1, c[0], c[1], c[2], c[3], i & 1 ? q.z : q.x, i & 1 ? q.w : q.y);
       }
+    }
+  }
+}
+
+// One step of eight rows times the planes of eight tokens, which are the MMA's sixteen rows here
+template <int KIND>
+__device__ __forceinline__ void step(const uint4 (&w)[1], const uint8_t *hi, const uint8_t *lo, float (&acc)[4]) {
+  Acts<KIND> h, l;
+  h.load(hi);
+  l.load(lo);
+  if constexpr (KIND <= kF16) {
+    mma<KIND>(acc, h.b[0].x, l.b[0].x, h.b[0].y, l.b[0].y, w[0].x, w[0].y);
+    mma<KIND>(acc, h.b[0].z, l.b[0].z, h.b[0].w, l.b[0].w, w[0].z, w[0].w);
+  } else {
+    const uint32_t r[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t b0, b1;
+      codes_f16<KIND>(r[i], b0, b1);
+      const uint4 &p = h.b[i >> 1], &q = l.b[i >> 1];
+      mma<KIND>(acc, i & 1 ? p.z : p.x, i & 1 ? q.z : q.x, i & 1 ? p.w : p.y, i & 1 ? q.w : q.y, b0, b1);
     }
   }
 }
@@ -500,9 +512,9 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
       meet();
     }
     const int n = it.n, last = it.r1, batch = kRed / (64 * 4 * n);   // tiles whose sums fit
-    // this lane's run of a plane of one of the first four tokens, and of the others
-    const uint8_t *x0 = panel + (2 * (base + min(g >> 1, n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
-    const uint8_t *x1 = panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+    // this lane's run of a plane of one of the first four tokens, and of the others; EIGHT: of both planes of one of eight
+    const uint8_t *x0 = panel + (EIGHT ? 2 * (base + min(g, n - 1)) : 2 * (base + min(g >> 1, n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+    const uint8_t *x1 = EIGHT ? x0 + pitch : panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
     int in_batch = 0;
     for (int first = it.r0; first < last; first += sh.outs) {
       if (turn != group) {
@@ -514,11 +526,12 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
         }
       } else {
         const bool mine = first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
-        float acc[3][4] = {};                           // tokens 0 .. 3, even and odd steps; 4 .. 7
-        const float *sc0 = nullptr, *sc1 = nullptr;     // e4m3: scales of the blocks of rows g and g + 8
+        float acc[3][4] = {};   // tokens 0 .. 3 (EIGHT: all), even and odd steps; 4 .. 7
+        // e4m3: scales of the blocks of rows g and g + 8; EIGHT: of rows 2 j and 2 j + 1, which are in one, runs starting at even rows
+        const float *sc0 = nullptr, *sc1 = nullptr;
         if constexpr (KIND == kE4) {
-          const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128, row = first + sub * kOuts + g;
-          const bool up = EIGHT && GATEUP && g >= 4;
+          const int kb = (sh.K + 127) / 128, nb = (sh.N + 127) / 128, row = first + sub * kOuts + (EIGHT ? 2 * j : g);
+          const bool up = EIGHT && GATEUP && j >= 2;
           sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((row - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
           sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
         }
@@ -543,40 +556,45 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
             for (int r = 0; r < kRuns; ++r) {
               const int rest = left - r * run;
               if (rest <= 0) break;
-              Weights<EIGHT> v;
+              Weights<EIGHT ? 1 : 2> v;
               v.load(slot + r * run, slot1 + r * run, rest);
               // the second step may lie behind the row's end: its weights are zeros then, and the planes reach to the end of a run
               float t[2][4] = {};
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 const int here = at + (r * run + u * 64) * (2 / kElem);
-                if constexpr (KIND == kE4) step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, t[0], t[1]);
-                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, acc[u], acc[2]);
+                if constexpr (EIGHT) step<KIND>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[u]);
+                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[u], KIND == kE4 ? t[1] : acc[2]);
               }
               if constexpr (KIND == kE4) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                  acc[0][c] = fmaf(f[r][c >> 1], t[0][c], acc[0][c]);
+                  acc[0][c] = fmaf(f[r][EIGHT ? 0 : c >> 1], t[0][c], acc[0][c]);
                   if (kTwo) acc[2][c] = fmaf(f[r][c >> 1], t[1][c], acc[2][c]);
                 }
               }
             }
           };
-          if (n <= 4) runs(std::false_type());
+          if (EIGHT || n <= 4) runs(std::false_type());
           else runs(std::true_type());
           __syncwarp();
           if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
           ring.next();
         }
         if (mine) {
-          float *dst = sums + (((in_batch * subs + sub) * parts + part) * n + j) * 16 + g;
-          if (j < n) {
-            dst[0] = (acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1]);
-            if (!EIGHT) dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
-          }
-          if (4 + j < n) {
-            dst[64] = acc[2][0] + acc[2][1];
-            if (!EIGHT) dst[72] = acc[2][2] + acc[2][3];
+          float *dst = sums + ((in_batch * subs + sub) * parts + part) * n * 16;
+          if constexpr (EIGHT) {
+            if (g < n) *reinterpret_cast<float2 *>(dst + g * 16 + 2 * j) = make_float2((acc[0][0] + acc[1][0]) + (acc[0][2] + acc[1][2]), (acc[0][1] + acc[1][1]) + (acc[0][3] + acc[1][3]));
+          } else {
+            dst += j * 16 + g;
+            if (j < n) {
+              dst[0] = (acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1]);
+              dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
+            }
+            if (4 + j < n) {
+              dst[64] = acc[2][0] + acc[2][1];
+              dst[72] = acc[2][2] + acc[2][3];
+            }
           }
         }
       }
@@ -712,87 +730,6 @@ __device__ __forceinline__ void store4(void *base, int dtype, int64_t i, bool ve
 
 __device__ __forceinline__ float inverse_rms(float sum, int H, float eps) { return rsqrtf(fmaf(sum, 1.0f / (float)H, eps)); }
 
-// Logits, and with the first experts' the statistics of the tokens' rows. The tokens x experts are dealt to the CTAs in squares of up to
-// four by four, for which 4 + 4 rows are read; a thread takes runs of four channels, so that all its loads go out together (a warp
-// per token over all of x in every CTA: 7 us at sixteen tokens).
-template <int SIDE>
-__device__ __forceinline__ void norms_and_logits(const DecodeParams &p, Shared &s) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int token_tiles = (p.T + SIDE - 1) / SIDE, expert_tiles = (p.E + SIDE - 1) / SIDE;
-  const bool x4 = fours(p.x, p.ldx, p.x_dtype);
-  for (int tile = blockIdx.x; tile < token_tiles * expert_tiles; tile += gridDim.x) {
-    const int t0 = tile % token_tiles * SIDE, e0 = tile / token_tiles * SIDE;
-    float ss[SIDE], most[SIDE], dot[SIDE][SIDE];
-#pragma unroll
-    for (int i = 0; i < SIDE; ++i) {
-      ss[i] = most[i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < SIDE; ++k) dot[i][k] = 0.f;
-    }
-    for (int c = 4 * tid; c < p.H; c += 4 * kThreads) {
-      float4 x[SIDE], n = make_float4(1.f, 1.f, 1.f, 1.f);
-      uint2 r[SIDE];
-#pragma unroll
-      for (int k = 0; k < SIDE; ++k) r[k] = *reinterpret_cast<const uint2 *>(p.router + (int64_t)min(e0 + k, p.E - 1) * p.H + c);
-#pragma unroll
-      for (int i = 0; i < SIDE; ++i) x[i] = load4(p.x, p.x_dtype, min(t0 + i, p.T - 1) * p.ldx + c, x4);
-      if (p.pre_w) n = load4(p.pre_w, p.norm_dtype, c, true);
-#pragma unroll
-      for (int i = 0; i < SIDE; ++i) {
-        float4 &v = x[i];
-        ss[i] = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, ss[i]))));
-        v = make_float4(v.x * n.x, v.y * n.y, v.z * n.z, v.w * n.w);
-        most[i] = max3_abs_nan(max3_abs_nan(most[i], v.x, v.y), v.z, v.w);
-#pragma unroll
-        for (int k = 0; k < SIDE; ++k)
-          dot[i][k] = fmaf(v.x, __uint_as_float(r[k].x << 16), fmaf(v.y, __uint_as_float(r[k].x & 0xffff0000u),
-                      fmaf(v.z, __uint_as_float(r[k].y << 16), fmaf(v.w, __uint_as_float(r[k].y & 0xffff0000u), dot[i][k]))));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < SIDE; ++i) {
-      ss[i] = warp_sum(ss[i]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most[i] = max_nan(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
-#pragma unroll
-      for (int k = 0; k < SIDE; ++k) dot[i][k] = warp_sum(dot[i][k]);
-    }
-    meet();   // the last tile's sums are read
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < SIDE; ++i) {
-        s.part[warp][i][0] = ss[i];
-        s.part[warp][i][1] = most[i];
-#pragma unroll
-        for (int k = 0; k < SIDE; ++k) s.part[warp][i][2 + k] = dot[i][k];
-      }
-    }
-    meet();
-    const int i = warp, t = t0 + i;   // a warp per token, lane l the sum of value l
-    if (i >= SIDE || t >= p.T) continue;
-    float v = 0.f;
-    if (lane < 2 + SIDE)
-      for (int w = 0; w < kWarps; ++w) v = lane == 1 ? max_nan(v, s.part[w][i][1]) : v + s.part[w][i][lane];
-    const float tot = __shfl_sync(0xffffffffu, v, 0), m = __shfl_sync(0xffffffffu, v, 1);
-    float inv = 1.0f;
-    if (p.pre_w) {
-      if (tot > 3.402823466e38f) {   // squares of a large row left the range: from values * 2^-64, where eps does not count
-        float q = 0.f;
-        for (int c = lane; c < p.H; c += 32) {
-          const float f = load_as_f32(p.x, p.x_dtype, t * p.ldx + c) * kDown;
-          q = fmaf(f, f, q);
-        }
-        inv = kDown * rsqrtf(warp_sum(q) * (1.0f / (float)p.H));
-      } else {
-        inv = inverse_rms(tot, p.H, p.eps);
-      }
-    }
-    const int e = e0 + lane - 2;
-    if (lane >= 2 && lane < 2 + SIDE && e < p.E) p.logits[t * p.E + e] = v * inv + (p.router_bias ? p.router_bias[e] : 0.f);
-    if (e0 == 0 && lane == 0) p.stats[t] = make_float2(inv, m * inv);
-  }
-}
-
 // sum of squares of the row in shared memory and its inverse norm; a large row once more
 __device__ __forceinline__ float row_inverse(const float *row, int H, float ss, float eps, float (*red)[kWarps]) {
   const float tot = cta_sum(ss, red[0]);
@@ -912,13 +849,97 @@ __device__ void give_up(const DecodeParams &p, Shared &s) {
   }
 }
 
+// Logits, and with the first experts' the statistics of the tokens' rows. The tokens x experts are dealt to the CTAs in squares of up to
+// four by four, for which 4 + 4 rows are read; a thread takes runs of four channels, so that all its loads go out together (a warp
+// per token over all of x in every CTA: 7 us at sixteen tokens).
+template <int SIDE>
+__global__ void __launch_bounds__(kThreads) moe_decode_front_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ float part[kWarps][SIDE][2 + SIDE];   // of a token: squares, largest, dot products
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int token_tiles = (p.T + SIDE - 1) / SIDE;
+  const bool x4 = fours(p.x, p.ldx, p.x_dtype);
+  const int t0 = blockIdx.x % token_tiles * SIDE, e0 = blockIdx.x / token_tiles * SIDE;
+  grid_dep_wait();   // x comes from an earlier launch, which may still use the workspace
+  if (blockIdx.x == 0) {
+    if (tid < 2) p.sync[tid] = 0u;
+    if (tid == 2) *p.status = 0;
+    if (tid < kMaxTokens * kMaxK) p.row_max[tid] = 0u;
+  }
+  float ss[SIDE], most[SIDE], dot[SIDE][SIDE];
+#pragma unroll
+  for (int i = 0; i < SIDE; ++i) {
+    ss[i] = most[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) dot[i][k] = 0.f;
+  }
+  for (int c = 4 * tid; c < p.H; c += 4 * kThreads) {
+    float4 x[SIDE], n = make_float4(1.f, 1.f, 1.f, 1.f);
+    uint2 r[SIDE];
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) r[k] = *reinterpret_cast<const uint2 *>(p.router + (int64_t)min(e0 + k, p.E - 1) * p.H + c);
+#pragma unroll
+    for (int i = 0; i < SIDE; ++i) x[i] = load4(p.x, p.x_dtype, min(t0 + i, p.T - 1) * p.ldx + c, x4);
+    if (p.pre_w) n = load4(p.pre_w, p.norm_dtype, c, true);
+#pragma unroll
+    for (int i = 0; i < SIDE; ++i) {
+      float4 &v = x[i];
+      ss[i] = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, ss[i]))));
+      v = make_float4(v.x * n.x, v.y * n.y, v.z * n.z, v.w * n.w);
+      most[i] = max3_abs_nan(max3_abs_nan(most[i], v.x, v.y), v.z, v.w);
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k)
+        dot[i][k] = fmaf(v.x, __uint_as_float(r[k].x << 16), fmaf(v.y, __uint_as_float(r[k].x & 0xffff0000u),
+                    fmaf(v.z, __uint_as_float(r[k].y << 16), fmaf(v.w, __uint_as_float(r[k].y & 0xffff0000u), dot[i][k]))));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < SIDE; ++i) {
+    ss[i] = warp_sum(ss[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most[i] = max_nan(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) dot[i][k] = warp_sum(dot[i][k]);
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < SIDE; ++i) {
+      part[warp][i][0] = ss[i];
+      part[warp][i][1] = most[i];
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) part[warp][i][2 + k] = dot[i][k];
+    }
+  }
+  __syncthreads();
+  const int i = warp, t = t0 + i;   // a warp per token, lane l the sum of value l
+  if (i >= SIDE || t >= p.T) return;
+  float v = 0.f;
+  if (lane < 2 + SIDE)
+    for (int w = 0; w < kWarps; ++w) v = lane == 1 ? max_nan(v, part[w][i][1]) : v + part[w][i][lane];
+  const float tot = __shfl_sync(0xffffffffu, v, 0), m = __shfl_sync(0xffffffffu, v, 1);
+  float inv = 1.0f;
+  if (p.pre_w) {
+    if (tot > 3.402823466e38f) {   // squares of a large row left the range: from values * 2^-64, where eps does not count
+      float q = 0.f;
+      for (int c = lane; c < p.H; c += 32) {
+        const float f = load_as_f32(p.x, p.x_dtype, t * p.ldx + c) * kDown;
+        q = fmaf(f, f, q);
+      }
+      inv = kDown * rsqrtf(warp_sum(q) * (1.0f / (float)p.H));
+    } else {
+      inv = inverse_rms(tot, p.H, p.eps);
+    }
+  }
+  const int e = e0 + lane - 2;
+  if (lane >= 2 && lane < 2 + SIDE && e < p.E) p.logits[t * p.E + e] = v * inv + (p.router_bias ? p.router_bias[e] : 0.f);
+  if (e0 == 0 && lane == 0) p.stats[t] = make_float2(inv, m * inv);
+}
+
 template <int KIND>
 __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (blockIdx.x == 0 && tid == 0) *p.status = 0;   // in front of the first barrier, behind which alone it is raised
   if (tid < kMaxExperts) s.mask[tid] = 0u;
   if (tid == 0) {
     for (int i = 0; i < kMaxSlots; ++i) {
@@ -928,13 +949,7 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     s.fail = 0;
     mbar_init_fence();
   }
-  if (warp < kWarps) {
-    if (p.T == 1) norms_and_logits<1>(p, s);
-    else if (p.T <= 4) norms_and_logits<2>(p, s);
-    else norms_and_logits<4>(p, s);
-  }
-  grid_arrive<kAll>(p, s);
-  if (!grid_wait<kAll>(p, s, 1)) return give_up(p, s);
+  __syncthreads();
 
   // ---- routing: a warp per token ----
   if (warp < p.T) {
@@ -995,16 +1010,16 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   }
   if (p.shape[0].eight) run_product<KIND, true, true>(p, s, ring, panel, sums, slots);
   else run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
-  grid_arrive<kThreads>(p, s);
+  grid_arrive(p, s);
   const int t = blockIdx.x;
-  bool ok = grid_wait<kThreads>(p, s, 2);
+  bool ok = grid_wait(p, s, 1);
   if (ok) {
     if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
     else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
-    grid_arrive<kThreads>(p, s);
+    grid_arrive(p, s);
     Finish end;
     if (t < p.T) end.prepare(p, t);
-    ok = grid_wait<kThreads>(p, s, 3);
+    ok = grid_wait(p, s, 2);
     if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
   }
   if (!ok) give_up(p, s);   // ends the copying warp's waits, too
@@ -1031,7 +1046,13 @@ int launch(DecodeParams &p, cudaStream_t st) {
     KNJ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     opted[dev] = true;
   }
-  KNJ_CUDA(cudaMemsetAsync(p.sync, 0, kCleared, st));
+  const int side = p.T == 1 ? 1 : p.T <= 4 ? 2 : 4;
+  const dim3 front((unsigned)(((p.T + side - 1) / side) * ((p.E + side - 1) / side)));
+  if (side == 1) KNJ_CUDA(launch_chain(moe_decode_front_kernel<1>, front, dim3(kThreads), 0, st, p));
+  else if (side == 2) KNJ_CUDA(launch_chain(moe_decode_front_kernel<2>, front, dim3(kThreads), 0, st, p));
+  else KNJ_CUDA(launch_chain(moe_decode_front_kernel<4>, front, dim3(kThreads), 0, st, p));
+  const int rc = launch_status("moe_decode_front_kernel");
+  if (rc) return rc;
   void *args[] = {&p};
   KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kAll), args, kSmem, st));
   return launch_status("moe_decode_kernel");
@@ -1085,4 +1106,4 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
 }
 }  // namespace knj
 
-extern "C" void knj_moe_block_decode_test_stall(int barrier) { t_stall = barrier >= 1 && barrier <= 3 ? barrier : 0; }
+extern "C" void knj_moe_block_decode_test_stall(int barrier) { t_stall = barrier >= 1 && barrier <= 2 ? barrier : 0; }

@@ -220,7 +220,7 @@ def test_two_launches_at_once():
         blk.status()
 
 
-@pytest.mark.parametrize("barrier", [1, 2, 3])
+@pytest.mark.parametrize("barrier", [1, 2])
 def test_a_barrier_that_gives_up(barrier):
     from kanjoos_b200 import _lib
     from kanjoos_b200.moe import MoeBlock
