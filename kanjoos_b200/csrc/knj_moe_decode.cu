@@ -28,7 +28,7 @@ using namespace knj;
 
 namespace {
 
-constexpr int kMaxRows = 8;   // of activations in the panel at a time: two groups of four
+constexpr int kMaxRows = 8;   // of activations that go through a matrix row at a time
 constexpr int kMaxTokens = KNJ_MOE_DECODE_MAX_TOKENS, kMaxK = 8, kMaxExperts = 256;
 // Seventeen warps leave 96 registers a thread, and the shared memory that the ring takes leaves no L1 for what does not fit: a spilled word
 // comes back from L2, 1000 cycles under load. So the products' loops are kept small: forms with the planes of the tokens in registers
@@ -104,6 +104,7 @@ struct Shared {
   unsigned mask[kMaxExperts];
   uint8_t pair_at[kMaxExperts][kMaxTokens];   // pairs of an expert's tokens in ascending order
   int active[kMaxTokens * kMaxK];
+  unsigned cost[kMaxTokens * kMaxK + 1];   // of the active experts in front
   int n_active, ok;
   Plan plan[2];                 // gate and up, down
   int row_tok[kMaxTokens], row_pair[kMaxTokens];        // of the panel's rows
@@ -250,10 +251,15 @@ struct Geo {
   static constexpr int kElem = KIND <= kF16 ? 2 : 1;
   // bytes of a plane of K values: whole runs of 128 bytes of weights, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
   __host__ __device__ static int pitch(int K) { return (K * kElem + 127) / 128 * (256 / kElem) + (kElem == 2 ? 64 : 16); }
-  // rows in the panel at a time: what leaves the ring two slots, or one
-  __host__ __device__ static int cap(int K) {
+  // rows of a pass: what leaves the ring two slots, or one
+  __host__ __device__ static int pass(int K) {
     const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
     return c < 1 ? 1 : c < kMaxRows ? c : kMaxRows;
+  }
+  // rows in the panel at a time: what leaves it four slots, or those of a pass
+  __host__ __device__ static int cap(int K) {
+    const int c = (kSmem - kRed - 4 * kSlot) / (2 * pitch(K));
+    return c < pass(K) ? pass(K) : c < kMaxTokens ? c : kMaxTokens;
   }
 };
 
@@ -302,17 +308,21 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
 }
 
 // A lane's part of a run of 128 bytes (two steps of 64) of sixteen rows: of rows g and g + 8 the bytes 16 j .. + 15 of either step. (Rows a
-// multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. Letting odd rows read their second step first and
-// swapping in registers avoids that and costs sixteen instructions a run, which are dearer.) left: bytes of the rows from the run's first
+// multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. SWAP: odd rows read their second step first, and the
+// two change places in registers. Of bf16 and fp16 experts that pays, 16 tokens 162 -> 155 us; of codes the instructions are dearer.) left: bytes of the rows from the run's first
 // on; what lies behind is zero.
 template <int ROWS>   // two, or of tiles of eight rows one
 struct Weights {
   uint4 w[2][ROWS];   // [step][row]
-  __device__ __forceinline__ void load(const uint8_t *row0, const uint8_t *row1, int left) {
+  template <bool SWAP>
+  __device__ __forceinline__ void load(const uint8_t *row0, const uint8_t *row1, bool odd, int left) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      w[u][0] = *reinterpret_cast<const uint4 *>(row0 + 64 * u);
-      if (ROWS == 2) w[u][ROWS - 1] = *reinterpret_cast<const uint4 *>(row1 + 64 * u);
+    for (int r = 0; r < ROWS; ++r) {
+      const uint8_t *row = r == 0 ? row0 : row1;
+      const int first = SWAP && odd ? 64 : 0;
+      const uint4 a = *reinterpret_cast<const uint4 *>(row + first), b = *reinterpret_cast<const uint4 *>(row + 64 - first);
+      w[0][r] = SWAP && odd ? b : a;
+      w[1][r] = SWAP && odd ? a : b;
     }
     if (left < 128) {
       const int at = (threadIdx.x & 3) * 16;
@@ -501,6 +511,8 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
   const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = 4 / subs, group = warp >> 2, sub = warp & (subs - 1), part = (warp & 3) / subs;
   // this lane's bytes of row g of its sub-tile in a slot; row g + 8 is 8 rows behind it, or of gate and up row g of up. EIGHT: rows of gate, then of up
   const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16;
+  constexpr bool kSwap = KIND <= kF16;
+  const bool odd = (g & 1) && (sh.slice & 64) == 0;
   int built = 0, base = 0, turn = 0;   // turn: whose tile it is
   bool ok = true;
   for (int i = 0; i < plan.n_items; ++i) {
@@ -557,7 +569,7 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
               const int rest = left - r * run;
               if (rest <= 0) break;
               Weights<EIGHT ? 1 : 2> v;
-              v.load(slot + r * run, slot1 + r * run, rest);
+              v.template load<kSwap>(slot + r * run, slot1 + r * run, odd, rest);
               // the second step may lie behind the row's end: its weights are zeros then, and the planes reach to the end of a run
               float t[2][4] = {};
 #pragma unroll
@@ -660,30 +672,50 @@ __device__ __forceinline__ void choose(const float *logits, int E, int k, int la
   __syncwarp();
 }
 
-// The rows of a product are dealt to the CTAs in equal numbers, in pairs of rows, over all active experts in a row; an expert's tokens
-// that the panel does not take at once go through in passes.
-__device__ __forceinline__ void make_plan(const DecodeParams &p, Plan &plan, const Shared &s, int N, int cap) {
-  const unsigned half = N / 2, units = s.n_active * half;   // at most 128 x 20480, times the CTAs below 2^32
-  auto border = [&](unsigned b) { return b == gridDim.x ? units : __umulhi(units * b, p.grid_inverse); };   // about units * b / grid, growing with b
-  unsigned u = border(blockIdx.x);
-  const unsigned end = border(blockIdx.x + 1);
-  int n = 0, panel = 0, held = 0, most = 0, i = (int)__fdividef((float)u, (float)half);
-  if (i * half > u) --i;   // the quotient of numbers below 2^24 may be off by one
-  if ((i + 1) * half <= u) ++i;
-  while (u < end) {
-    const unsigned begin = i * half, stop = min(end, begin + half);
-    const int e = s.active[i++], rows = __popc(s.mask[e]);
-    for (int f = 0; f < rows && n < kMaxItems; f += cap) {
-      const int c = min(cap, rows - f);
+// What a matrix row costs where n tokens go through it, in sixteenths of the cheapest: more tokens read more of the panel at each step.
+// (Gate and up of 16 tokens, time of the CTAs whose fullest expert has 1, 2, 3, 4, 5 tokens: bf16 80, 86, 90, 97, 100 us, int8 53, 54, 56, 56, 68.)
+template <int KIND>
+__device__ __forceinline__ int row_cost(int n) {
+  const int last = n & 7, full = n >> 3;
+  auto pass = [](int m) { return KIND <= kF16 ? 15 + m : m <= 4 ? 16 : 20; };
+  return full * pass(8) + (last ? pass(last) : 0);
+}
+// The matrix rows of a product, of all active experts in a row, are dealt to the CTAs by their cost, in pairs of rows. Where CTA b's begin:
+// position `at` of the active list, pair `unit` of its `half`. By a whole warp; every CTA forms the same borders.
+struct Border {
+  int at;
+  unsigned unit;
+};
+__device__ __forceinline__ Border border(const DecodeParams &p, const Shared &s, unsigned half, unsigned b) {
+  const int lane = threadIdx.x & 31;
+  if (b == gridDim.x) return Border{s.n_active, 0u};
+  const unsigned total = s.cost[s.n_active] * half;   // below 128 x 46 x 20480
+  const unsigned pos = (unsigned)((unsigned long long)total * b * p.grid_inverse >> 32);
+  int at = -1;
+#pragma unroll
+  for (int i = 0; i < kMaxTokens * kMaxK / 32; ++i) {
+    const int j = 32 * i + lane;
+    at += __popc(__ballot_sync(0xffffffffu, j < s.n_active && s.cost[j] * half <= pos));
+  }
+  const unsigned unit = (unsigned)__fdividef((float)(pos - s.cost[at] * half), (float)(s.cost[at + 1] - s.cost[at]));
+  return Border{at, min(unit, half)};
+}
+// This CTA's items between two borders; an expert's tokens go through in passes of up to kMaxRows.
+__device__ __forceinline__ void make_plan(Plan &plan, const Shared &s, int N, int pass, int cap, Border from, Border to) {
+  int n = 0, panel = 0, held = 0, most = 0;
+  for (int i = from.at; i <= to.at && i < s.n_active; ++i) {
+    const unsigned begin = i == from.at ? from.unit : 0u, end = i == to.at ? to.unit : N / 2;
+    const int e = s.active[i], rows = __popc(s.mask[e]);
+    for (int f = 0; begin < end && f < rows && n < kMaxItems; f += pass) {
+      const int c = min(pass, rows - f);
       if (held + c > cap) {
         panel = n;
         held = 0;
       }
       held += c;
       most = max(most, held);
-      plan.item[n++] = Item{e, 2 * (int)(u - begin), 2 * (int)(stop - begin), f, c, panel};
+      plan.item[n++] = Item{e, 2 * (int)begin, 2 * (int)end, f, c, panel};
     }
-    u = stop;
   }
   plan.n_items = n;
   plan.rows = most;
@@ -977,20 +1009,38 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     s.pair_at[e][__popc(s.mask[e] & ((1u << warp) - 1u))] = (uint8_t)(warp * p.k + lane);
   }
   if (warp == 0) {
-    unsigned on = 0u;   // which of this lane's eight experts are active
+    // this lane's eight experts: which are active, and in one word their number and, from bit 8 on, their cost
+    unsigned on = 0u, sum = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) on |= (s.mask[8 * lane + i] != 0u ? 1u : 0u) << i;
-    int at = __popc(on);
+    for (int i = 0; i < 8; ++i) {
+      const unsigned m = s.mask[8 * lane + i];
+      if (m == 0u) continue;
+      on |= 1u << i;
+      sum += 1u + ((unsigned)row_cost<KIND>(__popc(m)) << 8);
+    }
+    unsigned before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, at, o);
-      if (lane >= o) at += v;
+      const unsigned v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
     }
-    if (lane == 31) s.n_active = at;
-    at -= __popc(on);
-    for (; on; on &= on - 1u) s.active[at++] = 8 * lane + __ffs(on) - 1;
-    __syncwarp();
-    if (lane < 2) make_plan(p, s.plan[lane], s, lane == 0 ? p.F : p.H, Geo<KIND>::cap(lane == 0 ? p.H : p.F));
+    if (lane == 31) {
+      s.n_active = before & 255u;
+      s.cost[before & 255u] = before >> 8;
+    }
+    before -= sum;
+    for (; on; on &= on - 1u) {
+      const int e = 8 * lane + __ffs(on) - 1;
+      s.active[before & 255u] = e;
+      s.cost[before & 255u] = before >> 8;
+      before += 1u + ((unsigned)row_cost<KIND>(__popc(s.mask[e])) << 8);
+    }
+  }
+  __syncthreads();
+  if (warp < 2) {   // a warp for each product
+    const int N = warp == 0 ? p.F : p.H, K = warp == 0 ? p.H : p.F;
+    const Border from = border(p, s, N / 2, blockIdx.x), to = border(p, s, N / 2, blockIdx.x + 1);
+    if (lane == 0) make_plan(s.plan[warp], s, N, Geo<KIND>::pass(K), Geo<KIND>::cap(K), from, to);
   }
   __syncthreads();
 
