@@ -54,7 +54,7 @@ struct Shape {
   int K, N, row_bytes;
   int slices, slice;   // of a row, bytes
   int eight;           // tiles of eight rows, else sub-tiles of sixteen
-  int subs;            // sub-tiles of a tile, each of which has 4 / subs warps
+  int subs;            // sub-tiles of a tile, among which a group's warps are split
   int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
 };
 
@@ -249,6 +249,9 @@ __device__ __forceinline__ float cta_sum(float v, float *red) {   // by all thre
 template <int KIND>
 struct Geo {
   static constexpr int kElem = KIND <= kF16 ? 2 : 1;
+  // Groups of warps that take the tiles in turn, and warps of one: so that a warp has about four runs of a slot, of rows of 2048 x 2 bytes eight.
+  // (Of 4 and 2 groups, us: bf16 1 token 31.8, 33.4, 4 tokens 64.5, 67.4, 16 tokens 147, 150; e4m3 5 tokens 62.8, 59.8; int8 8 tokens 78.5, 77.0, 16 tokens 107, 109.)
+  static constexpr int kGroups = KIND <= kF16 ? 4 : 2, kTeam = kWarps / kGroups;
   // bytes of a plane of K values: whole runs of 128 bytes of weights, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
   __host__ __device__ static int pitch(int K) { return (K * kElem + 127) / 128 * (256 / kElem) + (kElem == 2 ? 64 : 16); }
   // rows of a pass: what leaves the ring two slots, or one
@@ -461,7 +464,8 @@ template <int KIND, bool GATEUP, bool EIGHT>
 __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, const Item &it, int base, const float *red, int n, int first) {
   constexpr int kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1);
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  const int parts = 4 / sh.subs, tokens = it.n;
+  constexpr int kTeam = Geo<KIND>::kTeam;
+  const int parts = kTeam / sh.subs, tokens = it.n;
   for (int u = threadIdx.x >> 5; u < n; u += kWarps)
     for (int o = threadIdx.x & 31; o < (tokens * kOuts + 31) / 32 * 32; o += 32) {
       const int r = o % kOuts, tok = o / kOuts, row = first + u * kOuts + r;
@@ -470,7 +474,7 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
       if (in) {
         const float *src = red + (u * parts * tokens + tok) * 16 + r;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < kTeam; ++w) {
           if (w >= parts) break;
           a += src[w * tokens * 16];
           if (GATEUP) b += src[w * tokens * 16 + kOuts];
@@ -478,10 +482,6 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
         const float un = KIND == kBf16 ? 1.0f : s.row_unmult[base + tok];
         a *= un;
         b *= un;
-        if constexpr (KIND == kS8) {
-          a *= __ldg((GATEUP ? p.s_gate : p.s_down) + (int64_t)it.expert * sh.N + row);
-          if (GATEUP) b *= __ldg(p.s_up + (int64_t)it.expert * sh.N + row);
-        }
         if (GATEUP) a = a / (1.0f + expf(-a)) * b;
         (GATEUP ? p.act : p.Y)[(int64_t)s.row_pair[base + tok] * sh.N + row] = a;
       }
@@ -495,20 +495,21 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
     }
 }
 
-// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y. The sixteen warps are four groups of four, which take the
-// tiles in turn, so that a tile's chain of waits, loads and MMAs runs beside three others (all warps at one tile took three times as long as
-// HBM needs to bring it). Of a group a sub-tile has 4 / subs warps, each with every 4 / subs-th run of 128 bytes of its rows, about four; the
-// sums meet in shared memory, [tile of the batch][sub-tile][part][token][row of 16].
+// One product over this CTA's items: gate, up and silu into p.act, or down into p.Y. The sixteen warps are groups, which take the tiles in
+// turn, so that a tile's chain of waits, loads and MMAs runs beside others (all warps at one tile took three times as long as HBM needs to
+// bring it). A group's warps are split among the sub-tiles, and a warp takes every parts-th run of 128 bytes of its rows; the sums meet in
+// shared memory, [tile of the batch][sub-tile][part][token][row of 16].
 // Every warp waits for every slot and releases it, in order, whether it reads it or not: a group that ran ahead or behind by the ring's
 // length would take one phase of a barrier for another.
 // A warp whose wait gives up raises s.fail, waits no more and frees no slot, but meets every barrier; what it forms then is never used.
 template <int KIND, bool GATEUP, bool EIGHT>
 __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ring &ring, uint8_t *panel, float *sums, const uint8_t *slots) {
-  constexpr int kElem = Geo<KIND>::kElem, kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kRuns = EIGHT ? 8 : 4;   // of a sub-tile; of a warp in a slice, at most
+  constexpr int kElem = Geo<KIND>::kElem, kGroups = Geo<KIND>::kGroups, kTeam = Geo<KIND>::kTeam;
+  constexpr int kOuts = (GATEUP ? 8 : 16) / (EIGHT ? 2 : 1), kRuns = (EIGHT ? 32 : 16) / kTeam;   // of a sub-tile; of a warp in a slice, at most
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
   const Plan &plan = s.plan[GATEUP ? 0 : 1];
   const Shape &sh = p.shape[GATEUP ? 0 : 1];
-  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = 4 / subs, group = warp >> 2, sub = warp & (subs - 1), part = (warp & 3) / subs;
+  const int pitch = Geo<KIND>::pitch(sh.K), subs = sh.subs, parts = kTeam / subs, group = warp / kTeam, sub = warp & (subs - 1), part = (warp % kTeam) / subs;
   // this lane's bytes of row g of its sub-tile in a slot; row g + 8 is 8 rows behind it, or of gate and up row g of up. EIGHT: rows of gate, then of up
   const int row0 = (sub * kOuts + g) * sh.slice + part * 128 + j * 16;
   constexpr bool kSwap = KIND <= kF16;
@@ -523,7 +524,7 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
       base = 0;
       meet();
     }
-    const int n = it.n, last = it.r1, batch = kRed / (64 * 4 * n);   // tiles whose sums fit
+    const int n = it.n, last = it.r1, batch = kRed / (64 * kTeam * n);   // tiles whose sums fit
     // this lane's run of a plane of one of the first four tokens, and of the others; EIGHT: of both planes of one of eight
     const uint8_t *x0 = panel + (EIGHT ? 2 * (base + min(g, n - 1)) : 2 * (base + min(g >> 1, n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
     const uint8_t *x1 = EIGHT ? x0 + pitch : panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
@@ -547,6 +548,16 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((row - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
           sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
         }
+        // int8: scales of the rows whose sums this lane will hold, g and g + 8 or 2 j and 2 j + 1; read here, in front of the waits
+        float row_scale[2] = {1.f, 1.f};
+        if constexpr (KIND == kS8)
+          if (mine) {
+            const bool up = EIGHT && GATEUP && j >= 2;
+            const int row = first + sub * kOuts + (EIGHT ? 2 * j - (up ? 4 : 0) : g);
+            const float *a = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + (int64_t)it.expert * sh.N, *b = GATEUP && !EIGHT ? p.s_up + (int64_t)it.expert * sh.N : a;
+            row_scale[0] = __ldg(a + min(row, sh.N - 1));
+            row_scale[1] = __ldg(b + min(row + (EIGHT ? 1 : GATEUP ? 0 : 8), sh.N - 1));
+          }
         for (int sl = 0; sl < sh.slices; ++sl) {
           const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
           float f[kRuns][2];
@@ -596,21 +607,23 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
         if (mine) {
           float *dst = sums + ((in_batch * subs + sub) * parts + part) * n * 16;
           if constexpr (EIGHT) {
-            if (g < n) *reinterpret_cast<float2 *>(dst + g * 16 + 2 * j) = make_float2((acc[0][0] + acc[1][0]) + (acc[0][2] + acc[1][2]), (acc[0][1] + acc[1][1]) + (acc[0][3] + acc[1][3]));
+            if (g < n)
+              *reinterpret_cast<float2 *>(dst + g * 16 + 2 * j) = make_float2(((acc[0][0] + acc[1][0]) + (acc[0][2] + acc[1][2])) * row_scale[0],
+                                                                              ((acc[0][1] + acc[1][1]) + (acc[0][3] + acc[1][3])) * row_scale[1]);
           } else {
             dst += j * 16 + g;
             if (j < n) {
-              dst[0] = (acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1]);
-              dst[8] = (acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3]);
+              dst[0] = ((acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1])) * row_scale[0];
+              dst[8] = ((acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3])) * row_scale[1];
             }
             if (4 + j < n) {
-              dst[64] = acc[2][0] + acc[2][1];
-              dst[72] = acc[2][2] + acc[2][3];
+              dst[64] = (acc[2][0] + acc[2][1]) * row_scale[0];
+              dst[72] = (acc[2][2] + acc[2][3]) * row_scale[1];
             }
           }
         }
       }
-      turn = (turn + 1) & 3;
+      turn = (turn + 1) % kGroups;
       if (++in_batch != batch && first + sh.outs < last) continue;
       meet();
       add_parts<KIND, GATEUP, EIGHT>(p, s, it, base, sums, in_batch * subs, first - (in_batch - 1) * sh.outs);
@@ -1122,8 +1135,9 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   const int T = a->n_tokens, H = a->hidden, F = a->ffn, E = a->n_experts, k = a->top_k;
   KNJ_REQUIRE(T <= kMaxTokens, "knj_moe_block_decode: %d tokens, at most %d", T, kMaxTokens);
   KNJ_REQUIRE(F <= KNJ_MOE_DECODE_MAX_FFN, "knj_moe_block_decode: ffn=%d above %d", F, KNJ_MOE_DECODE_MAX_FFN);
-  KNJ_REQUIRE(sm_count() >= kMaxExperts / 2, "knj_moe_block_decode: a device of %d SMs or more needed", kMaxExperts / 2);
   KNJ_REQUIRE(aligned16(a->pre_w), "knj_moe_block_decode: pre_w must be 16-byte aligned");
+  // a CTA's items: its share of the cost and two experts at its borders, sixteen passes each, stay far below kMaxItems then
+  KNJ_REQUIRE(sm_count() >= KNJ_MOE_DECODE_MIN_SMS, "knj_moe_block_decode: a device of %d SMs or more needed", KNJ_MOE_DECODE_MIN_SMS);
   DecodeParams p{};
   p.x = a->x; p.pre_w = a->pre_w; p.post_w = a->post_w; p.next_w = a->next_w; p.gate = a->gate; p.router = a->w_router; p.router_bias = a->router_bias;
   p.w_gate = static_cast<const uint8_t *>(a->w_gate); p.w_up = static_cast<const uint8_t *>(a->w_up); p.w_down = static_cast<const uint8_t *>(a->w_down);

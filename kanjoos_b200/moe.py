@@ -391,15 +391,15 @@ class MoeBlock:
         gate [T][1] or [T][H] in place of the bank's. next_norm [H], in the type of the bank's norms (any float type where those are
         f32): also returns h = norm(out; next_norm) in next_dtype (default: x's type; float8_e4m3fn: (codes, scale)). Returns out, or
         a tuple (out[, h][, pair_exp, pair_w])."""
-        return self._call(lib().knj_moe_block_launch, self.max_tokens, x, out, gate, next_norm, next_dtype, return_routing)
+        return self._call("knj_moe_block_launch", self.max_tokens, x, out, gate, next_norm, next_dtype, return_routing)
 
     def decode(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
         """The block for up to MOE_DECODE_MAX_TOKENS tokens in one launch (knj_moe_block_decode_launch): arguments and results as of
         run, with nothing between x and out rounded to 16 or 8 bits. Needs a device that the process has to itself."""
-        return self._call(lib().knj_moe_block_decode_launch, min(self.max_tokens, MOE_DECODE_MAX_TOKENS), x, out, gate, next_norm, next_dtype,
+        return self._call("knj_moe_block_decode_launch", min(self.max_tokens, MOE_DECODE_MAX_TOKENS), x, out, gate, next_norm, next_dtype,
                           return_routing)
 
-    def _call(self, launch, most, x, out, gate, next_norm, next_dtype, return_routing):
+    def _call(self, entry, most, x, out, gate, next_norm, next_dtype, return_routing):
         b = self.bank
         if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > most or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
             raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {most}")
@@ -433,7 +433,7 @@ class MoeBlock:
         if return_routing:
             taps = (torch.empty(T * self.top_k, dtype=torch.int32, device=x.device), torch.empty(T * self.top_k, dtype=torch.float32, device=x.device))
         a = self._args(x, out, gate, next_norm, h, scale, taps)
-        check(launch(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        check(getattr(lib(), entry)(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         self._last = a
         result = (out,) + (() if h is None else ((h, scale) if scale is not None else h,)) + (taps or ())
         return result if len(result) > 1 else out

@@ -264,6 +264,57 @@ def test_run_and_decode_agree():
     ref.check(r, s2, es2 + ref.held(s2, F32), "run")
 
 
+@pytest.mark.parametrize("kind", [BF16, I8])
+def test_experts_rows_and_outputs_beyond_32_bits(kind):
+    """The last experts' matrices and the last rows lie more than 2^31 elements behind the first."""
+    from kanjoos_b200.moe import FloatExpertBank, MoeBlock
+    from test_gpu_block_ops_use import far
+    E, H, F, T, ld = 132, 4096, 4096, 3, 1 << 30
+    assert (E - 3) * H * F > 1 << 31 and (T - 1) * ld >= 1 << 31
+    few = bank(kind, 3, H, F, 31)
+    full = {}
+    for n in ("gate", "up", "down"):
+        m = getattr(few, n)
+        full[n] = torch.empty((E, *m.shape[1:]), dtype=m.dtype, device="cuda")
+        full[n][E - 3:] = m.cuda()
+        sc = getattr(few, n + "_scale")
+        if sc is not None:
+            full[n + "_scale"] = torch.zeros((E, *sc.shape[1:]), device="cuda")
+            full[n + "_scale"][E - 3:] = sc.cuda()
+    router = torch.zeros((E, H), dtype=BF16)
+    router[E - 3:] = few.router
+    bias = torch.full((E,), float("-inf"))
+    bias[E - 3:] = 0.0
+    big = FloatExpertBank(**full, router=router.cuda(), router_bias=bias.cuda(), pre_norm=few.pre_norm.cuda())
+    x = rows(T, H, 90, BF16)
+    wide, out = far(T, H, ld, BF16), far(T, H, ld, F32)
+    wide.copy_(x)
+    blk = MoeBlock(big, top_k=2)
+    got, pe, pw = blk.decode(wide, out=out, return_routing=True)
+    blk.status()
+    assert got is out and (pe >= E - 3).all()
+    small = replace(few, router_bias=torch.zeros(3), post_norm=None, out_gate=None, alpha=1.0, beta=1.0)
+    compare(small, x, 2, (got, pe - (E - 3), pw))
+
+
+def test_status_word_and_workspace_of_ones_own():
+    """Nothing in the workspace or the status word has to be cleared before the first launch, nor after a launch of another block."""
+    from kanjoos_b200.moe import MoeBlock
+    H, k = 256, 2
+    a, b = (MoeBlock(on_device(bank(kind, 8, H, 64, 33)), top_k=k) for kind in (BF16, E4M3))
+    need = max(a.workspace.numel(), b.workspace.numel())
+    a, b = (MoeBlock(m.bank, top_k=k, max_tokens=64, workspace=torch.full((8 * need,), 0xA5, dtype=torch.uint8, device="cuda")) for m in (a, b))
+    shared = [MoeBlock(m.bank, top_k=k, workspace=a.workspace) for m in (a, b)]
+    x = rows(3, H, 91).cuda()
+    want = [a.decode(x), b.decode(x)]
+    for _ in range(3):
+        for m, w in zip(shared, want):
+            m._status.fill_(77)
+            assert torch.equal(m.decode(x), w)
+            m.status()
+            m.run(x)
+
+
 def test_refusals():
     from kanjoos_b200.moe import MoeBlock
     blk = MoeBlock(on_device(bank(BF16, 8, 256, 64, 29)), top_k=2, max_tokens=32)
