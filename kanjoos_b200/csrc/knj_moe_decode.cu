@@ -41,8 +41,10 @@ constexpr int kAll = kThreads + 32;
 constexpr int kSlice = 4096;
 constexpr int kSlot = 8 * kSlice;
 constexpr int kMaxSlots = 6;
-constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles: 256 a tile and token
-constexpr int kSmem = 214 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
+constexpr int kRed = 16 * 1024;                // bytes of the sums of a batch of tiles, 256 or 512 a tile and token
+constexpr int kSmem = 213 * 1024;              // sums, planes of the rows in use, and the ring in what they leave
+// int8: the scales of a slot's rows, up to 32 of gate and of up or 64 of down, in whole 16-byte units
+constexpr int kScales = 80;
 constexpr int kMaxItems = 64;
 constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256;   // of the workspace
 constexpr float kDown = 0x1p-64f;
@@ -110,6 +112,7 @@ struct Shared {
   int row_tok[kMaxTokens], row_pair[kMaxTokens];        // of the panel's rows
   float row_mult[kMaxTokens], row_unmult[kMaxTokens];
   float red[4][kWarps];
+  alignas(16) float scale[kMaxSlots][kScales];   // int8: of a slot's rows
 };
 
 static_assert(kSmem + sizeof(Shared) <= 227 * 1024, "shared memory of a block");
@@ -281,6 +284,7 @@ struct Ring {
 };
 
 // The copying warp's side of a product. False after a wait that gave up.
+template <int KIND>
 __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int product, Ring &ring, uint8_t *slots, int &copied) {
   const int lane = threadIdx.x & 31;
   const Shape &sh = p.shape[product];
@@ -295,13 +299,18 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
       const bool mine = lane < (whole ? 1 : rows) * (up ? 2 : 1);
       const uint8_t *src = (up ? (second ? p.w_up : p.w_gate) : p.w_down) + ((int64_t)it.expert * sh.N + first + r) * sh.row_bytes;
       const int dst = (second * sh.outs + r) * sh.slice;
+      // int8: the rows' scales, in units of four (N is a multiple of 16), come with the first slice (a read past L1 ahead of each tile: one token 30.3 us, so 29.6)
+      const int scale0 = first & ~3, scale_bytes = KIND == kS8 ? (((first + rows + 3) & ~3) - scale0) * 4 : 0;
       for (int sl = 0; sl < sh.slices; ++sl) {
         const int bytes = whole ? rows * sh.row_bytes : min(sh.slice, sh.row_bytes - sl * sh.slice);
         const bool ok = mbar_wait_for(&s.empty[ring.at], ring.parity ^ 1u, p.wait_cycles, &s.fail);
         if (!__all_sync(0xffffffffu, ok)) return false;
-        if (lane == 0) mbar_expect_tx(&s.full[ring.at], (uint32_t)(bytes * (whole ? 1 : rows) * (up ? 2 : 1)));
+        if (lane == 0) mbar_expect_tx(&s.full[ring.at], (uint32_t)((bytes * (whole ? 1 : rows) + (sl == 0 ? scale_bytes : 0)) * (up ? 2 : 1)));
         __syncwarp();
         if (mine) bulk_g2s(slots + ring.at * kSlot + dst, src + sl * sh.slice, (uint32_t)bytes, &s.full[ring.at]);
+        if (KIND == kS8 && sl == 0 && lane >= (up ? 30 : 31))
+          bulk_g2s(&s.scale[ring.at][lane == 30 ? kScales / 2 : 0], (up ? (lane == 30 ? p.s_up : p.s_gate) : p.s_down) + (int64_t)it.expert * sh.N + scale0,
+                   (uint32_t)scale_bytes, &s.full[ring.at]);
         ring.next();
         ++copied;
       }
@@ -548,16 +557,7 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           sc0 = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + ((int64_t)it.expert * nb + min((row - (up ? 4 : 0)) / 128, nb - 1)) * kb + part;
           sc1 = EIGHT ? sc0 : (GATEUP ? p.s_up : p.s_down) + ((int64_t)it.expert * nb + min((row + (GATEUP ? 0 : 8)) / 128, nb - 1)) * kb + part;
         }
-        // int8: scales of the rows whose sums this lane will hold, g and g + 8 or 2 j and 2 j + 1; read here, in front of the waits
-        float row_scale[2] = {1.f, 1.f};
-        if constexpr (KIND == kS8)
-          if (mine) {
-            const bool up = EIGHT && GATEUP && j >= 2;
-            const int row = first + sub * kOuts + (EIGHT ? 2 * j - (up ? 4 : 0) : g);
-            const float *a = (GATEUP ? (up ? p.s_up : p.s_gate) : p.s_down) + (int64_t)it.expert * sh.N, *b = GATEUP && !EIGHT ? p.s_up + (int64_t)it.expert * sh.N : a;
-            row_scale[0] = __ldg(a + min(row, sh.N - 1));
-            row_scale[1] = __ldg(b + min(row + (EIGHT ? 1 : GATEUP ? 0 : 8), sh.N - 1));
-          }
+        float row_scale[2] = {1.f, 1.f};   // int8: of the rows whose sums this lane will hold, g and g + 8 or 2 j and 2 j + 1
         for (int sl = 0; sl < sh.slices; ++sl) {
           const int left = mine ? min(sh.slice, sh.row_bytes - sl * sh.slice) - part * 128 : 0;   // bytes from this warp's first run on
           float f[kRuns][2];
@@ -571,14 +571,17 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           }
           if (ok && !mbar_wait_for(&s.full[ring.at], ring.parity, p.wait_cycles, &s.fail)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
+          if (KIND == kS8 && sl == 0) {   // row_scale's rows may lie behind the last copied one: what is read then is never used
+            const float *a = s.scale[ring.at] + (first & 3) + sub * kOuts + (EIGHT ? 2 * j - (GATEUP && j >= 2 ? 4 : 0) : g);
+            const int up = kScales / 2;
+            row_scale[0] = a[EIGHT && GATEUP && j >= 2 ? up : 0];
+            row_scale[1] = a[(EIGHT && GATEUP && j >= 2 ? up : 0) + (EIGHT ? 1 : GATEUP ? up : 8)];
+          }
           const uint8_t *slot = slots + ring.at * kSlot + row0, *slot1 = slot + (GATEUP ? sh.outs : 8) * sh.slice;
           const int at = sl * sh.slice * (2 / kElem), run = parts * 128;
           auto runs = [&](auto two) {
             constexpr bool kTwo = decltype(two)::value;
-#pragma unroll
-            for (int r = 0; r < kRuns; ++r) {
-              const int rest = left - r * run;
-              if (rest <= 0) break;
+            auto one = [&](int r, int rest) {
               Weights<EIGHT ? 1 : 2> v;
               v.template load<kSwap>(slot + r * run, slot1 + r * run, odd, rest);
               // the second step may lie behind the row's end: its weights are zeros then, and the planes reach to the end of a run
@@ -594,6 +597,27 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
                 for (int c = 0; c < 4; ++c) {
                   acc[0][c] = fmaf(f[r][EIGHT ? 0 : c >> 1], t[0][c], acc[0][c]);
                   if (kTwo) acc[2][c] = fmaf(f[r][c >> 1], t[1][c], acc[2][c]);
+                }
+              }
+            };
+            if constexpr (KIND <= kF16) {
+#pragma unroll
+              for (int r = 0; r < kRuns; ++r) {
+                const int rest = left - r * run;
+                if (rest <= 0) break;
+                one(r, rest);
+              }
+            } else {   // two whole runs without a branch between them: the second's loads go ahead of the first's MMAs (e4m3 4 tokens 56 -> 54 us, 16 tokens
+                       // 110 -> 107; bf16, whose runs are shorter, lost 5 to 10 % by it)
+#pragma unroll
+              for (int r = 0; r < kRuns; r += 2) {
+                if (left >= (r + 1) * run + 128) {
+                  one(r, 128);
+                  one(r + 1, 128);
+                } else {
+                  if (left > r * run) one(r, left - r * run);
+                  if (left > (r + 1) * run) one(r + 1, left - (r + 1) * run);
+                  break;
                 }
               }
             }
@@ -1065,7 +1089,7 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u};
   if (warp == kWarps) {
     int copied = 0;
-    if (!feed(p, s, 0, ring, slots, copied) || !feed(p, s, 1, ring, slots, copied)) {
+    if (!feed<KIND>(p, s, 0, ring, slots, copied) || !feed<KIND>(p, s, 1, ring, slots, copied)) {
       // the slots filled last may still be written: shared memory is not left before they are
       if (lane < ring.n && copied > lane) mbar_wait_for(&s.full[lane], (uint32_t)((copied - lane - 1) / ring.n) & 1u, p.wait_cycles, nullptr);
     }
@@ -1136,6 +1160,8 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   KNJ_REQUIRE(T <= kMaxTokens, "knj_moe_block_decode: %d tokens, at most %d", T, kMaxTokens);
   KNJ_REQUIRE(F <= KNJ_MOE_DECODE_MAX_FFN, "knj_moe_block_decode: ffn=%d above %d", F, KNJ_MOE_DECODE_MAX_FFN);
   KNJ_REQUIRE(aligned16(a->pre_w), "knj_moe_block_decode: pre_w must be 16-byte aligned");
+  KNJ_REQUIRE(a->w_dtype != KNJ_DT_I8 || (aligned16(a->gate_scale) && aligned16(a->up_scale) && aligned16(a->down_scale)),
+              "knj_moe_block_decode: the scales of int8 matrices must be 16-byte aligned");
   // a CTA's items: its share of the cost and two experts at its borders, sixteen passes each, stay far below kMaxItems then
   KNJ_REQUIRE(sm_count() >= KNJ_MOE_DECODE_MIN_SMS, "knj_moe_block_decode: a device of %d SMs or more needed", KNJ_MOE_DECODE_MIN_SMS);
   DecodeParams p{};

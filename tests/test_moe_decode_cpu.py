@@ -17,7 +17,7 @@ CODES = dict(w_dtype=5, gate_scale=A, up_scale=A, down_scale=A)
     (dict(gate_kind=1), "gate", -1), (dict(ldo=255), "stride", -1), (dict(ldx=255), "stride", -1), (dict(x_dtype=3), "f32, bf16 or f16", -1),
     (dict(out_dtype=5), "f32, bf16 or f16", -1), (dict(w_norm_dtype=3), "weights", -1), (dict(next_w=A, h_next=A, ld_h_next=256, h_next_dtype=5), "h_dtype", -1),
     (dict(w_gate=A + 8), "aligned", -1), (dict(w_up=A + 4), "aligned", -1), (dict(w_down=A + 8), "aligned", -1), (dict(pre_w=A + 2), "aligned", -1),
-    (dict(w_router=A + 8), "aligned", -1), (dict(n_tokens=17), "at most 16", -1), (dict(ffn=40976, workspace_bytes=1 << 40), "40960", -1),
+    ({**CODES, "up_scale": A + 8}, "aligned", -1), (dict(w_router=A + 8), "aligned", -1), (dict(n_tokens=17), "at most 16", -1), (dict(ffn=40976, workspace_bytes=1 << 40), "40960", -1),
 ])
 def test_refusals(L, change, word, code):
     refused(L, L.knj_moe_block_decode_launch(C.byref(block_args(L, **change)), None), word, code)
