@@ -1305,7 +1305,7 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
 }
 
 size_t knj_int8_matmul_workspace_bytes(int m, int n_in) {
-  if (m <= 0 || n_in <= 0) return 0;
+  if (m <= 0 || n_in <= 0 || int8_few(m, n_in)) return 0;
   return up256((size_t)m * n_in) + up256((size_t)m * 4);
 }
 
@@ -1324,6 +1324,7 @@ int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_
   KNJ_REQUIRE(ldx >= n_in && ldy >= n_out, "knj_int8_matmul: row strides shorter than the rows");
   GemmParams p{};
   p.x = static_cast<const uint8_t *>(x); p.x_row = ldx; p.xs = x_scale;
+  if (!codes && int8_few(m, n_in)) return int8_few_launch(W, W_scale, n_in, n_out, x, x_dtype, ldx, m, y, y_dtype, ldy, as_stream(s));
   if (!codes) {
     const size_t need = knj_int8_matmul_workspace_bytes(m, n_in);
     if (!workspace || workspace_bytes < need) {

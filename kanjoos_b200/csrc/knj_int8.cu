@@ -1,5 +1,5 @@
 // knj_int8.cu -- rows as signed 8-bit codes with one f32 scale each, the form in which the int8 products (knj_expert_tc.cu) take
-// their rows:
+// their rows, and the product of few rows:
 //   scale = most * f32(1/127), most = the row's largest magnitude;  code = the whole number nearest to v * (1 / scale), ties to even
 // in f32, so that any program with IEEE arithmetic forms the same bits. |v| <= most keeps the product within 127 (1 + 2^-22), so a code
 // never passes 127. A row whose `most` is below 2^-100 is zeros under a zero scale: there the scale or its inverse would leave the
@@ -113,7 +113,119 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const void *x, int dtype
   if (threadIdx.x == 0) scale[row] = s.scale;
 }
 
+// Few rows times a matrix: y[r][n] = f32(sum over k of codes[r][k] W[n][k]) * (scale[r] * ws[n]), the rows' codes formed by every CTA for
+// itself in shared memory. One launch and no workspace, where rows and product on the tensor cores are two launches. Bound by the matrix,
+// read once: a warp takes pairs of matrix rows, a lane 16 bytes of either at a time, which meet the codes in dp4a; the sums are whole
+// numbers, so the bits are those of the other form whatever their order.
+// us in a graph, this form and the two launches, for 1, 2, 4 rows: 2048 x 2048 3.3, 3.9, 4.2 and 7.3, 7.4, 8.2; 16384 x 4096 (10.2 at HBM's
+// rate) 12.9, 13.8, 17.2 and 18.6, 18.5, 19.0. Of 8 rows every 16 bytes of the matrix meet eight reads of shared memory: 27 us against 18,
+// so that more than four rows take the other. (Host time of a call with one row: 9.1 us, so 13.7.)
+constexpr int kFewRows = 4, kFewBytes = 40 * 1024;   // rows; bytes of codes, which need no opting in
+
+template <int M>
+__global__ void __launch_bounds__(256, 4) int8_few_kernel(const int8_t *W, const float *ws, int K, int N, const void *x, int dtype, int64_t ldx, int vec,
+                                                          int m, void *y, int y_dtype, int64_t ldy) {
+  extern __shared__ __align__(16) uint8_t codes[];   // [M][K]
+  __shared__ float part[8], scale[M];
+  constexpr int kWpr = 8 / M;   // warps of a row
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, units = K / 16, pairs = N / 2 + (N & 1);
+  grid_dep_wait();
+  int pair = blockIdx.x * 8 + warp;
+  uint4 w[2][4];
+  auto load = [&](int at, int from) {
+    const int8_t *a = W + (int64_t)(2 * at) * K, *b = W + (int64_t)min(2 * at + 1, N - 1) * K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = from + lane + 32 * i;
+      if (u < units) {
+        w[0][i] = __ldg(reinterpret_cast<const uint4 *>(a) + u);
+        w[1][i] = __ldg(reinterpret_cast<const uint4 *>(b) + u);
+      }
+    }
+  };
+  if (pair < pairs) load(pair, 0);   // on its way while the codes are formed
+  const int row = warp / kWpr, first = warp % kWpr * 32 + lane;
+  auto value8 = [&](int i, float2 (&v)[4]) {
+    if (vec) {
+      load8(x, dtype, row * ldx + 8 * i, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = make_float2(load_as_f32(x, dtype, row * ldx + 8 * i + 2 * j), load_as_f32(x, dtype, row * ldx + 8 * i + 2 * j + 1));
+    }
+  };
+  float most = 0.f;
+  if (row < m)
+    for (int i = first; i < K / 8; i += 32 * kWpr) {
+      float2 v[4];
+      value8(i, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = max3_abs_nan(most, v[j].x, v[j].y);
+    }
+  most = warp_max_nan(most);
+  if (lane == 0) part[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWpr; ++i) most = max_nan(most, part[row * kWpr + i]);
+  const RowScale s = row_scale(most);
+  for (int i = first; i < K / 8; i += 32 * kWpr) {   // zeros of rows behind the last
+    float2 v[4];
+    if (row < m) value8(i, v);
+    else v[0] = v[1] = v[2] = v[3] = make_float2(0.f, 0.f);
+    *reinterpret_cast<uint2 *>(codes + row * K + 8 * i) = make_uint2(codes4(v[0], v[1], s), codes4(v[2], v[3], s));
+  }
+  if (warp % kWpr == 0 && lane == 0) scale[row] = s.scale;
+  __syncthreads();
+  for (; pair < pairs; pair += gridDim.x * 8) {
+    int acc[2][M] = {};
+    for (int from = 0; from < units; from += 128) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int u = from + lane + 32 * i;
+        if (u >= units) continue;
+#pragma unroll
+        for (int r = 0; r < M; ++r) {
+          const uint4 c = *reinterpret_cast<const uint4 *>(codes + r * K + 16 * u);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            acc[h][r] = __dp4a((int)w[h][i].x, (int)c.x, __dp4a((int)w[h][i].y, (int)c.y, __dp4a((int)w[h][i].z, (int)c.z, __dp4a((int)w[h][i].w, (int)c.w, acc[h][r]))));
+        }
+      }
+      const bool more = from + 128 < units;
+      const int next = more ? pair : pair + gridDim.x * 8;
+      if (next < pairs) load(next, more ? from + 128 : 0);
+    }
+    int mine = 0;   // lane 2 r + h: of row r and the pair's row h
+#pragma unroll
+    for (int r = 0; r < M; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[h][r]);
+        if (lane == 2 * r + h) mine = sum;
+      }
+    const int r = lane >> 1, n = 2 * pair + (lane & 1);
+    if (r < m && n < N) store_from_f32(y, y_dtype, r * ldy + n, __int2float_rn(mine) * (scale[r < M ? r : 0] * __ldg(ws + n)));
+  }
+}
+
 }  // namespace
+
+namespace knj {
+static int few_rows(int m) { return m <= 2 ? m : kFewRows; }   // that a kernel is built for
+bool int8_few(int m, int K) { return m <= kFewRows && few_rows(m) * (int64_t)K <= kFewBytes; }
+
+int int8_few_launch(const void *W, const float *ws, int K, int N, const void *x, int dtype, int64_t ldx, int m, void *y, int y_dtype, int64_t ldy, cudaStream_t st) {
+  const int vec = aligned16(x) && (m == 1 || ldx * (dtype == KNJ_DT_F32 ? 4 : 2) % 16 == 0);
+  const int blocks = (N - 1) / 16 + 1, most = 4 * sm_count(), M = few_rows(m);
+  const dim3 grid(blocks < most ? blocks : most), block(256);
+  const size_t smem = (size_t)M * K;
+  const int8_t *w = static_cast<const int8_t *>(W);
+  if (M == 1) KNJ_CUDA(launch_chain(int8_few_kernel<1>, grid, block, smem, st, w, ws, K, N, x, dtype, ldx, vec, m, y, y_dtype, ldy));
+  else if (M == 2) KNJ_CUDA(launch_chain(int8_few_kernel<2>, grid, block, smem, st, w, ws, K, N, x, dtype, ldx, vec, m, y, y_dtype, ldy));
+  else KNJ_CUDA(launch_chain(int8_few_kernel<kFewRows>, grid, block, smem, st, w, ws, K, N, x, dtype, ldx, vec, m, y, y_dtype, ldy));
+  return launch_status("int8_few_kernel");
+}
+}  // namespace knj
 
 extern "C" int knj_int8_rows_launch(const void *x, int x_dtype, int64_t ldx, int rows, int K, void *q, float *scale, knj_stream_t s) {
   KNJ_REQUIRE(rows >= 0 && K > 0, "knj_int8_rows: bad sizes");

@@ -384,8 +384,9 @@ def int8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, x_scale
         xs = _dense(x_scale, "x_scale", cur, (m,), _ONLY_F32)
     else:
         nbytes = _int8_matmul_scratch(m, k)
-        scratch = x.new_empty(nbytes, dtype=torch.uint8)
-        work = scratch.data_ptr()
+        if nbytes:
+            scratch = x.new_empty(nbytes, dtype=torch.uint8)
+            work = scratch.data_ptr()
     check(lib().knj_int8_matmul_launch(w, ws, k, n, ptr, code, xs, ld, m, y.data_ptr(), out_code, n, work, nbytes,
                                        None if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), _raw_stream()))
     return y

@@ -71,6 +71,70 @@ def test_int8_matmul(m, n, k, dtype, out, pad, form):
         assert torch.equal(got, ops.int8_matmul(w.cuda(), s.cuda(), rows, qs, out_dtype=out)), "of rows in codes"
 
 
+@pytest.mark.parametrize("n,k,pad", [(1, 16, 0), (7, 160, 3), (2048, 2048, 0), (1000, 4096, 8), (20011, 512, 1), (33, 5120, 0), (64, 5136, 0), (5, 20480, 5)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_few_rows_have_the_bits_of_many(n, k, pad, dtype):
+    """Each number of rows that a kernel is built for and those between, strided and at odd addresses, outputs of every type; a row's result
+    does not depend on the rows around it."""
+    from kanjoos_b200 import ops
+    g = gen("few8", n, k, dtype)
+    w, s = i8.matrix((n, k), g)
+    w, s = w.cuda(), s.cuda()
+    x = torch.randn((9, k), generator=g).to(dtype)
+    x[2] = 0.0
+    x[4, k // 2] = 1e4
+    x = strided(x.cuda(), pad) if pad else x.cuda()
+    q, qs = ops.int8_rows(x)
+    for out in (F32, BF16, F16):
+        want = ops.int8_matmul(w, s, q, qs, out_dtype=out)
+        for m in (1, 2, 3, 4, 5, 7, 8, 9):
+            assert torch.equal(ops.int8_matmul(w, s, x[:m], out_dtype=out), want[:m]), m
+        for at in (1, 3):
+            assert torch.equal(ops.int8_matmul(w, s, x[at:at + 5], out_dtype=out), want[at:at + 5])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_that_are_not_finite(dtype):
+    from kanjoos_b200 import ops
+    g = gen("few nan8")
+    w, s = i8.matrix((100, 304), g)
+    x = torch.randn((8, 304), generator=g).to(dtype)
+    clean = ops.int8_matmul(w.cuda(), s.cuda(), x.cuda()).cpu()
+    x[1, 303], x[3, 0], x[6, 5] = float("nan"), float("inf"), float("-inf")
+    got = ops.int8_matmul(w.cuda(), s.cuda(), x.cuda()).cpu()
+    bad = [1, 3, 6]
+    keep = [i for i in range(8) if i not in bad]
+    assert torch.isnan(got[bad]).all() and torch.equal(got[keep], clean[keep])
+
+
+def test_few_rows_write_their_rows_alone():
+    """An output with a row stride of its own through the entry point: nothing between and behind the rows is written."""
+    from kanjoos_b200 import _lib
+    g = gen("few ld8")
+    w, s = (t.cuda() for t in i8.matrix((37, 64), g))
+    x = torch.randn((3, 64), generator=g).cuda()
+    y = torch.full((6, 50), -77.0, device="cuda")
+    _lib.check(_lib.lib().knj_int8_matmul_launch(w.data_ptr(), s.data_ptr(), 64, 37, x.data_ptr(), 0, None, 64, 3, y.data_ptr(), 0, 50, None, 0, None,
+                                                 torch.cuda.current_stream().cuda_stream))
+    from kanjoos_b200 import ops
+    assert torch.equal(y[:3, :37], ops.int8_matmul(w, s, x))
+    assert (y[3:] == -77.0).all() and (y[:, 37:] == -77.0).all()
+
+
+def test_few_rows_of_a_matrix_beyond_32_bits():
+    from kanjoos_b200 import ops
+    n, k = 525000, 4096
+    assert (n - 3) * k > 1 << 31
+    g = gen("few far8")
+    few, s3 = i8.matrix((3, k), g)
+    w = torch.zeros((n, k), dtype=I8, device="cuda")
+    s = torch.ones(n, device="cuda")
+    w[-3:], s[-3:] = few.cuda(), s3.cuda()
+    x = torch.randn((2, k), generator=g).cuda()
+    got = ops.int8_matmul(w, s, x)
+    assert torch.equal(got[:, -3:], ops.int8_matmul(few.cuda(), s3.cuda(), x)) and (got[:, :-3] == 0).all()
+
+
 def test_sums_of_the_largest_codes(form):
     """Sums next to the end of 32 bits: every product 16384 or -16256, as many as the entry points take."""
     from kanjoos_b200 import ops

@@ -13,7 +13,13 @@ from test_moe_block_cpu import block_args, write_float_file
 def test_empty_calls_and_workspaces(L):
     assert L.knj_int8_rows_launch(None, 0, 0, 0, 64, None, None, None) == 0
     assert L.knj_int8_matmul_launch(None, None, 64, 64, None, 0, None, 64, 0, None, 0, 64, None, 0, None, None) == 0
-    assert L.knj_int8_matmul_workspace_bytes(0, 64) == 0 and L.knj_int8_matmul_workspace_bytes(3, 130) == 512 + 256
+    assert L.knj_int8_matmul_workspace_bytes(0, 64) == 0 and L.knj_int8_matmul_workspace_bytes(9, 130) == 1280 + 256
+
+
+def test_few_rows_need_no_workspace(L):
+    for m, k, few in ((1, 40960, True), (1, 40976, False), (2, 20480, True), (3, 10240, True), (3, 10256, False), (4, 10240, True),
+                      (5, 16, False)):
+        assert (L.knj_int8_matmul_workspace_bytes(m, k) == 0) == few, (m, k)
 
 
 @pytest.mark.parametrize("args,word", [
@@ -30,11 +36,11 @@ def test_rows_refusals(L, args, word):
     (dict(x=None), "null", -1), (dict(y=None), "null", -1), (dict(n_in=72, ldx=72), "multiple of 16", -1), (dict(W=A + 8), "aligned", -1),
     (dict(n_in=131072, ldx=131072), "131072", -1), (dict(dt=3), "f32, bf16, f16 or int8", -1), (dict(dt=4), "f32, bf16, f16 or int8", -1),
     (dict(yt=5), "f32, bf16 or f16", -1), (dict(ldx=63), "stride", -1), (dict(ldy=7), "stride", -1), (dict(ws=None), "workspace", -4),
-    (dict(nb=511), "workspace", -4), (dict(ws=A + 16), "256-byte", -1), (dict(dt=5), "null", -1), (dict(dt=5, XS=A, ldx=72), "16-byte", -1),
+    (dict(nb=1023), "workspace", -4), (dict(ws=A + 16), "256-byte", -1), (dict(dt=5), "null", -1), (dict(dt=5, XS=A, ldx=72), "16-byte", -1),
     (dict(dt=5, XS=A, x=A + 4), "16-byte", -1), (dict(m=(1 << 30) + 1), "2^30", -1),
 ])
 def test_matmul_refusals(L, change, word, code):
-    v = dict(W=A, S=A, n_in=64, n_out=8, x=A, dt=0, XS=None, ldx=64, m=2, y=A, yt=0, ldy=8, ws=A, nb=512)
+    v = dict(W=A, S=A, n_in=64, n_out=8, x=A, dt=0, XS=None, ldx=64, m=9, y=A, yt=0, ldy=8, ws=A, nb=1024)
     v.update(change)
     rc = L.knj_int8_matmul_launch(v["W"], v["S"], v["n_in"], v["n_out"], v["x"], v["dt"], v["XS"], v["ldx"], v["m"], v["y"], v["yt"], v["ldy"],
                                   v["ws"], v["nb"], None, None)
