@@ -580,9 +580,10 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
 
 /* Dense product with an int8 matrix: y[m][n_out] = f32(sum_k x[m][k] W[n_out][k]) * (x_scale[m] * W_scale[n_out]), W int8
  * [n_out][n_in], W_scale f32 [n_out], the sums exact in 32-bit whole numbers. Rows of x in f32, bf16 or f16 (x_scale not read) are
- * turned into codes first, as knj_int8_rows_launch does, in the workspace (256-byte aligned; knj_int8_matmul_workspace_bytes is 0 for
- * few rows, whose codes the product's kernel forms itself); int8 rows (16-byte units) come with their x_scale [m] and need no workspace. n_in a multiple of 16 below KNJ_INT8_MAX_K. y f32, bf16 or f16. status as in
- * knj_expert_gemm_args. The reference's int8 product (kernels/knj_kernels.hip:132-318 knj_gemm_w4_i8) has 4-bit weights. */
+ * turned into codes first, as knj_int8_rows_launch does, in the workspace (256-byte aligned; knj_int8_matmul_workspace_bytes is 0 for up
+ * to four rows, whose codes the product's kernel forms itself); int8 rows (16-byte units) come with their x_scale [m] and need no
+ * workspace. n_in a multiple of 16 below KNJ_INT8_MAX_K. y f32, bf16 or f16. status as in knj_expert_gemm_args. The reference's int8
+ * product (kernels/knj_kernels.hip:132-318 knj_gemm_w4_i8) has 4-bit weights. */
 size_t knj_int8_matmul_workspace_bytes(int m, int n_in);
 int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, const float *x_scale, int64_t ldx,
                            int m, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);

@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(256, 4) int8_few_kernel(const int8_t *W, const
     for (int i = 0; i < 4; ++i) {
       const int u = from + lane + 32 * i;
       if (u < units) {
-        w[0][i] = __ldg(reinterpret_cast<const uint4 *>(a) + u);
-        w[1][i] = __ldg(reinterpret_cast<const uint4 *>(b) + u);
+        w[0][i] = __ldcg(reinterpret_cast<const uint4 *>(a) + u);
+        w[1][i] = __ldcg(reinterpret_cast<const uint4 *>(b) + u);
       }
     }
   };
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(256, 4) int8_few_kernel(const int8_t *W, const
         if (lane == 2 * r + h) mine = sum;
       }
     const int r = lane >> 1, n = 2 * pair + (lane & 1);
-    if (r < m && n < N) store_from_f32(y, y_dtype, r * ldy + n, __int2float_rn(mine) * (scale[r < M ? r : 0] * __ldg(ws + n)));
+    if (r < m && n < N) store_from_f32(y, y_dtype, r * ldy + n, __int2float_rn(mine) * (scale[r < M ? r : 0] * __ldcg(ws + n)));
   }
 }
 
