@@ -562,8 +562,8 @@ typedef struct knj_expert_gemm_args {
 int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 /* 1 = these products (and the dense e4m3 and int8 ones) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
- * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes.
- * Process-wide. */
+ * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes. (The
+ * int8 product of up to four rows that are not codes yet is none of these, whatever is set.) Process-wide. */
 void knj_expert_tc_form(int form);
 /* Test hook of the calling thread: in its next products 1 = the first accumulator of the first thread block, 2 = that block's first
  * operands, 3 = the first accumulator of the last thread block of its pair or cluster never count as complete, so that a wait runs

@@ -303,6 +303,8 @@ class FloatExpertBank:
 
     def to_e4m3(self) -> "FloatExpertBank":
         """The same block with its experts as e4m3 codes under block scales."""
+        if self.gate.dtype == torch.int8:
+            raise ValueError("these experts are int8 codes already")
         parts = {}
         for name in ("gate", "up", "down"):
             parts[name], parts[name + "_scale"] = e4m3_blocks(getattr(self, name))
@@ -310,6 +312,8 @@ class FloatExpertBank:
 
     def to_int8(self) -> "FloatExpertBank":
         """The same block with its experts as int8 codes under a scale for each output channel."""
+        if self.gate_scale is not None:
+            raise ValueError("these experts are codes already")
         parts = {}
         for name in ("gate", "up", "down"):
             parts[name], parts[name + "_scale"] = int8_channels(getattr(self, name))
@@ -394,7 +398,7 @@ class MoeBlock:
         return self._call("knj_moe_block_launch", self.max_tokens, x, out, gate, next_norm, next_dtype, return_routing)
 
     def decode(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
-        """The block for up to MOE_DECODE_MAX_TOKENS tokens in one launch (knj_moe_block_decode_launch): arguments and results as of
+        """The block for up to MOE_DECODE_MAX_TOKENS tokens in two kernels (knj_moe_block_decode_launch): arguments and results as of
         run, with nothing between x and out rounded to 16 or 8 bits. Needs a device that the process has to itself."""
         return self._call("knj_moe_block_decode_launch", min(self.max_tokens, MOE_DECODE_MAX_TOKENS), x, out, gate, next_norm, next_dtype,
                           return_routing)

@@ -99,3 +99,15 @@ def test_gguf_experts_as_int8(tmp_path):
         assert ((q * s[..., None] - w).abs() <= 0.5001 * s[..., None]).all()
     with pytest.raises(ValueError, match="exclude"):
         gguf_bank.load_float_expert_bank(g, 0, device="cpu", e4m3=True, int8=True)
+
+
+def test_codes_are_not_turned_into_codes_again():
+    from kanjoos_b200.moe import FloatExpertBank
+    g = torch.Generator().manual_seed(3)
+    bank = FloatExpertBank(gate=torch.randn((2, 16, 256), generator=g).bfloat16(), up=torch.randn((2, 16, 256), generator=g).bfloat16(),
+                           down=torch.randn((2, 256, 16), generator=g).bfloat16(), router=torch.randn((2, 256), generator=g).bfloat16())
+    for codes in (bank.to_int8(), bank.to_e4m3()):
+        with pytest.raises(ValueError, match="already"):
+            codes.to_int8()
+    with pytest.raises(ValueError, match="already"):
+        bank.to_int8().to_e4m3()
