@@ -402,6 +402,7 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
     w_ptr = _dense(w, "an expert matrix", cur, shape, types)
     w1_ptr = 0 if w1 is None else _dense(w1, "an expert matrix", cur, shape, types)
     xs = s0_ptr = s1_ptr = 0
+    x_ptr = None
     if w.dtype == _E4M3:
         if s0 is None or (w1 is not None and s1 is None):
             raise ValueError("e4m3 expert matrices need their scales")
@@ -425,13 +426,21 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
         if x.dtype != torch.int8:
             if x_scale is not None:
                 raise ValueError("x_scale belongs to int8 rows")
-            x, x_scale = int8_rows(x)
+            ptr, code, ld = _rows(x, "x", cur, (x.shape[0], K))
+            n = x.shape[0]
+            at = (n * K + 255) & ~255
+            rows = x.new_empty(at + 4 * n, dtype=torch.uint8)   # codes, and behind them the scales
+            x_ptr = rows.data_ptr()
+            xs, x_code, ld_rows = x_ptr + at, DT_I8, K
+            check(lib().knj_int8_rows_launch(ptr, code, ld, n, K, x_ptr, xs, _raw_stream()))
         elif x_scale is None:
             raise ValueError("int8 rows need x_scale")
-        xs = _dense(x_scale, "x_scale", cur, (x.shape[0],), _ONLY_F32)
+        else:
+            xs = _dense(x_scale, "x_scale", cur, (x.shape[0],), _ONLY_F32)
     elif s0 is not None or s1 is not None or x_scale is not None:
         raise ValueError("scales belong to e4m3 and int8 matrices and rows")
-    x_ptr, x_code, ld = _rows(x, "x", cur, (x.shape[0], K), {w.dtype: _OPERAND[w.dtype]})
+    if x_ptr is None:
+        x_ptr, x_code, ld_rows = _rows(x, "x", cur, (x.shape[0], K), {w.dtype: _OPERAND[w.dtype]})
     idx_shape = pair_idx.shape
     if len(idx_shape) != 2:
         raise ValueError(f"pair_idx has shape {tuple(idx_shape)}")
@@ -446,7 +455,7 @@ def _expert(launch, x, x_scale, w, w1, s0, s1, pair_idx, pair_cnt, P, row_map, r
         out_ptr, ldo = out.data_ptr(), N
     else:
         out_ptr, out_code, ldo = _rows(out, "out", cur, (P, N))
-    a = _expert_args(x_ptr, xs, ld, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo,
+    a = _expert_args(x_ptr, xs, ld_rows, w_ptr, w1_ptr, s0_ptr, s1_ptr, idx, cnt, rmap, idx_shape[1], out_ptr, ldo,
                      0 if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), x.shape[0], P, N, K, E,
                      row_div, x_code, x_code, out_code, out_scale)
     check(launch(a, _raw_stream()))
