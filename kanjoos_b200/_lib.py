@@ -57,7 +57,7 @@ class BlockNormArgs(C.Structure):
 def packed(cls):
     """A function from the values of all fields in their order (0 for a null pointer) to the structure's bytes: for calls that are made
     many times a decode step, 0.25 us where building the structure takes 1.2."""
-    code = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P", C.c_float: "f"}
+    code = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P", C.c_float: "f", C.c_size_t: "N"}
     return struct.Struct("".join(code[t] for _, t in cls._fields_) + "0P").pack
 
 
@@ -218,16 +218,16 @@ SIGNATURES = {
     "knj_int8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
     "knj_int8_matmul_workspace_bytes": (_sz, [_i, _i]),
     "knj_int8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),
-    # a BlockNormArgs or ExpertGemmArgs by reference, or its bytes (packed)
+    # a BlockNormArgs, ExpertGemmArgs or MoeBlockArgs by reference, or its bytes (packed)
     "knj_block_norm_launch": (_i, [_vp, _vp]),
     "knj_block_norm_test_stall": (None, [_i]),
     "knj_expert_gateup_launch": (_i, [_vp, _vp]),
     "knj_expert_proj_launch": (_i, [_vp, _vp]),
     "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
-    "knj_moe_block_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
-    "knj_moe_block_decode_launch": (_i, [C.POINTER(MoeBlockArgs), _vp]),
+    "knj_moe_block_launch": (_i, [_vp, _vp]),
+    "knj_moe_block_decode_launch": (_i, [_vp, _vp]),
     "knj_moe_block_decode_test_stall": (None, [_i]),
-    "knj_moe_block_status": (_i, [C.POINTER(MoeBlockArgs), _vp]),
+    "knj_moe_block_status": (_i, [_vp, _vp]),
     "knj_expert_tc_form": (None, [_i]),
     "knj_expert_tc_test_stall": (None, [_i]),
     "knj_fp8_matmul_workspace_bytes": (_sz, [_i, _i]),

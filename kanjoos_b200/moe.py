@@ -13,10 +13,12 @@ import torch
 
 from . import synth
 from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_ROW, MOE_DECODE_MAX_TOKENS, MoeBlockArgs, MoeFfnArgs, check,
-                   lib)
+                   lib, packed)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 _DT_FLOAT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+_DT_ROWS = {**_DT_FLOAT, torch.float8_e4m3fn: DT_E4M3}
+_block_args = packed(MoeBlockArgs)
 _DT_EXPERT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float8_e4m3fn: DT_E4M3, torch.int8: DT_I8}
 
 
@@ -261,6 +263,10 @@ def int8_channels(w: torch.Tensor):
     return q.to(torch.int8).contiguous(), scale.contiguous()
 
 
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 @dataclass
 class FloatExpertBank:
     """Weights of one MoE block whose experts are bf16, f16, e4m3 or int8, all on one device.
@@ -365,30 +371,26 @@ class MoeBlock:
         self._status = torch.empty(1, dtype=torch.int32, device=bank.gate.device)   # of this block alone; a launch clears it
         self._last = None
 
-    def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> MoeBlockArgs:
+    def _args(self, x, out, gate, next_norm, h_next, h_scale, taps) -> bytes:
+        """The fields of MoeBlockArgs in their order."""
         b = self.bank
         T, H = x.shape
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        a = MoeBlockArgs(n_tokens=T, hidden=H, ffn=b.ffn, n_experts=b.n_experts, top_k=self.top_k, x_dtype=_DT_FLOAT[x.dtype],
-                         out_dtype=_DT_FLOAT[out.dtype], w_dtype=_DT_EXPERT[b.gate.dtype], alpha=b.alpha, beta=b.beta, eps=b.rms_eps,
-                         gate_sigmoid=1 if b.gate_sigmoid else 0, x=x.data_ptr(), ldx=x.stride(0) if T > 1 else H, out=out.data_ptr(),
-                         ldo=out.stride(0) if T > 1 else H, pre_w=ptr(b.pre_norm), post_w=ptr(b.post_norm), next_w=ptr(next_norm),
-                         w_router=b.router.data_ptr(), router_bias=ptr(b.router_bias), w_gate=b.gate.data_ptr(), w_up=b.up.data_ptr(),
-                         w_down=b.down.data_ptr(), gate_scale=ptr(b.gate_scale), up_scale=ptr(b.up_scale), down_scale=ptr(b.down_scale),
-                         h_next=ptr(h_next), ld_h_next=H, h_next_scale=ptr(h_scale), workspace=self.workspace.data_ptr(),
-                         workspace_bytes=self.workspace.numel(), status=self._status.data_ptr())
-        for w in (b.pre_norm, b.post_norm, next_norm):
-            if w is not None:
-                a.w_norm_dtype = _DT_FLOAT[w.dtype]
+        norm = next_norm if next_norm is not None else b.post_norm if b.post_norm is not None else b.pre_norm
+        gate_ptr = gate_dtype = gate_kind = ldg = 0
         if gate is not None:
-            a.gate, a.gate_dtype = gate.data_ptr(), _DT_FLOAT[gate.dtype]
-            a.gate_kind = GATE_CHANNEL if gate.dim() == 1 else GATE_ROW if gate.shape[1] == 1 and H > 1 else GATE_FULL
-            a.ldg = 0 if gate.dim() == 1 else gate.stride(0) if T > 1 else gate.shape[1]
-        if h_next is not None:
-            a.h_next_dtype = DT_E4M3 if h_next.dtype == torch.float8_e4m3fn else _DT_FLOAT[h_next.dtype]
-        if taps is not None:
-            a.tap_pair_exp, a.tap_pair_w = taps[0].data_ptr(), taps[1].data_ptr()
-        return a
+            gate_ptr, gate_dtype = gate.data_ptr(), _DT_FLOAT[gate.dtype]
+            if gate.dim() == 1:
+                gate_kind = GATE_CHANNEL
+            else:
+                gate_kind = GATE_ROW if gate.shape[1] == 1 and H > 1 else GATE_FULL
+                ldg = gate.stride(0) if T > 1 else gate.shape[1]
+        return _block_args(T, H, b.ffn, b.n_experts, self.top_k, _DT_FLOAT[x.dtype], _DT_FLOAT[out.dtype], _DT_EXPERT[b.gate.dtype],
+                           0 if norm is None else _DT_FLOAT[norm.dtype], gate_dtype, 0 if h_next is None else _DT_ROWS[h_next.dtype], gate_kind,
+                           1 if b.gate_sigmoid else 0, b.alpha, b.beta, b.rms_eps, x.data_ptr(), x.stride(0) if T > 1 else H, out.data_ptr(),
+                           out.stride(0) if T > 1 else H, _ptr(b.pre_norm), _ptr(b.post_norm), _ptr(next_norm), gate_ptr, ldg, b.router.data_ptr(),
+                           _ptr(b.router_bias), b.gate.data_ptr(), b.up.data_ptr(), b.down.data_ptr(), _ptr(b.gate_scale), _ptr(b.up_scale),
+                           _ptr(b.down_scale), _ptr(h_next), H, _ptr(h_scale), self.workspace.data_ptr(), self.workspace.numel(),
+                           0 if taps is None else taps[0].data_ptr(), 0 if taps is None else taps[1].data_ptr(), self._status.data_ptr())
 
     def run(self, x, out=None, gate=None, next_norm=None, next_dtype=None, return_routing=False):
         """x [T][H] f32 / bf16 / f16 -> the stream behind the block, in x's type or into `out` (which may be x). gate: the rows' own
@@ -407,11 +409,12 @@ class MoeBlock:
         b = self.bank
         if x.dim() != 2 or x.shape[1] != b.hidden or x.shape[0] > most or x.dtype not in _DT_FLOAT or x.stride(1) != 1:
             raise ValueError(f"x is {x.dtype} {tuple(x.shape)}, expected rows of {b.hidden} values, at most {most}")
-        if x.device != b.gate.device or x.get_device() != torch.cuda.current_device():
+        device = x.get_device()
+        if device != b.gate.get_device() or device != torch.cuda.current_device():
             raise ValueError(f"x lives on {x.device}, the block on {b.gate.device}; the current device is {torch.cuda.current_device()}")
         T, H = x.shape
         if out is None:
-            out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+            out = x.new_empty(T, H)
         elif out.shape != x.shape or out.dtype not in _DT_FLOAT or out.device != x.device or out.stride(1) != 1:
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, expected rows like x")
         gate = b.out_gate if gate is None else gate
@@ -428,16 +431,16 @@ class MoeBlock:
             if tuple(next_norm.shape) != (H,) or next_norm.dtype not in _DT_FLOAT or any(w.dtype != next_norm.dtype for w in norms) or \
                     next_norm.device != x.device or not next_norm.is_contiguous():
                 raise ValueError(f"next_norm is {next_norm.dtype} {tuple(next_norm.shape)}, expected [{H}] in the block's norm type (or narrower than f32 ones)")
-            if next_dtype not in (None, torch.float8_e4m3fn, *_DT_FLOAT):
+            if next_dtype is not None and next_dtype not in _DT_ROWS:
                 raise ValueError(f"next_dtype is {next_dtype}, expected f32, bf16, f16 or float8_e4m3fn")
-            h = torch.empty((T, H), dtype=next_dtype or x.dtype, device=x.device)
+            h = x.new_empty(T, H, dtype=next_dtype)
             if h.dtype == torch.float8_e4m3fn:
                 scale = torch.empty((T, -(-H // 128)), dtype=torch.float32, device=x.device)
         taps = None
         if return_routing:
             taps = (torch.empty(T * self.top_k, dtype=torch.int32, device=x.device), torch.empty(T * self.top_k, dtype=torch.float32, device=x.device))
         a = self._args(x, out, gate, next_norm, h, scale, taps)
-        check(getattr(lib(), entry)(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        check(getattr(lib(), entry)(a, torch._C._cuda_getCurrentRawStream(device)))
         self._last = a
         result = (out,) + (() if h is None else ((h, scale) if scale is not None else h,)) + (taps or ())
         return result if len(result) > 1 else out
@@ -446,4 +449,4 @@ class MoeBlock:
         """Waits for the stream; raises if a bounded wait of the last run gave up."""
         if self._last is None:
             return
-        check(lib().knj_moe_block_status(C.byref(self._last), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        check(lib().knj_moe_block_status(self._last, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
