@@ -584,9 +584,21 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
  * to four rows, whose codes the product's kernel forms itself); int8 rows (16-byte units) come with their x_scale [m] and need no
  * workspace. n_in a multiple of 16 below KNJ_INT8_MAX_K. y f32, bf16 or f16. status as in knj_expert_gemm_args. The reference's int8
  * product (kernels/knj_kernels.hip:132-318 knj_gemm_w4_i8) has 4-bit weights. */
+typedef struct {
+  const void *w;
+  const float *w_scale;
+  const void *x;
+  const float *x_scale;
+  int64_t ldx;
+  void *y;
+  int64_t ldy;
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t *status;
+  int32_t n_in, n_out, m, x_dtype, y_dtype;
+} knj_int8_matmul_args;
 size_t knj_int8_matmul_workspace_bytes(int m, int n_in);
-int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, const float *x_scale, int64_t ldx,
-                           int m, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s);
+int knj_int8_matmul_launch(const knj_int8_matmul_args *a, knj_stream_t s);
 
 /* A whole MoE block of a residual stream with experts in bf16, fp16, e4m3 or int8 (Model::moe between rmsnorm_rows and the
  * residual add, src/model/model.cpp:631-652, with what a block may have around it):

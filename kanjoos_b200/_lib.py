@@ -81,6 +81,12 @@ class ExpertGemmArgs(C.Structure):
                 ("out_dtype", C.c_int32), ("out_scale", C.c_float)]
 
 
+class Int8MatmulArgs(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("w_scale", C.c_void_p), ("x", C.c_void_p), ("x_scale", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p), ("n_in", C.c_int32),
+                ("n_out", C.c_int32), ("m", C.c_int32), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32)]
+
+
 class EpDescC(C.Structure):
     _fields_ = [("world", C.c_int32), ("rank", C.c_int32), ("n_tokens_local", C.c_int32), ("hidden", C.c_int32),
                 ("ffn", C.c_int32), ("n_experts", C.c_int32), ("top_k", C.c_int32), ("n_chunks", C.c_int32),
@@ -217,8 +223,8 @@ SIGNATURES = {
     "knj_fp8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
     "knj_int8_rows_launch": (_i, [_vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
     "knj_int8_matmul_workspace_bytes": (_sz, [_i, _i]),
-    "knj_int8_matmul_launch": (_i, [_vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i, _vp, _i, _i64, _vp, _sz, _vp, _vp]),
-    # a BlockNormArgs, ExpertGemmArgs or MoeBlockArgs by reference, or its bytes (packed)
+    # an Int8MatmulArgs, BlockNormArgs, ExpertGemmArgs or MoeBlockArgs by reference, or its bytes (packed)
+    "knj_int8_matmul_launch": (_i, [_vp, _vp]),
     "knj_block_norm_launch": (_i, [_vp, _vp]),
     "knj_block_norm_test_stall": (None, [_i]),
     "knj_expert_gateup_launch": (_i, [_vp, _vp]),

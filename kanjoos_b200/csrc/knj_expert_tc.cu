@@ -1309,8 +1309,14 @@ size_t knj_int8_matmul_workspace_bytes(int m, int n_in) {
   return up256((size_t)m * n_in) + up256((size_t)m * 4);
 }
 
-int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_out, const void *x, int x_dtype, const float *x_scale, int64_t ldx,
-                           int m, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, int *status, knj_stream_t s) {
+int knj_int8_matmul_launch(const knj_int8_matmul_args *a, knj_stream_t s) {
+  KNJ_REQUIRE(a, "knj_int8_matmul: null argument block");
+  const void *W = a->w, *x = a->x;
+  const float *W_scale = a->w_scale, *x_scale = a->x_scale;
+  const int n_in = a->n_in, n_out = a->n_out, m = a->m, x_dtype = a->x_dtype, y_dtype = a->y_dtype;
+  const int64_t ldx = a->ldx, ldy = a->ldy;
+  void *y = a->y, *workspace = a->workspace;
+  const size_t workspace_bytes = a->workspace_bytes;
   KNJ_REQUIRE(m >= 0 && n_in > 0 && n_out > 0, "knj_int8_matmul: bad sizes");
   if (m == 0) return KNJ_OK;
   const bool codes = x_dtype == KNJ_DT_I8;
@@ -1338,7 +1344,7 @@ int knj_int8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_
     if (rc) return rc;
     p.x = q; p.x_row = n_in; p.xs = qs;
   }
-  p.ws0 = W_scale; p.out = y; p.status = status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
+  p.ws0 = W_scale; p.out = y; p.status = a->status; p.ldo = ldy; p.out_dtype = y_dtype; p.N = n_out; p.K = n_in; p.E = 1;
   p.row_div = 1; p.n_rows = m; p.n_pairs = m; p.out_scale = 1.0f; p.dense = 1;
   return launch_gemm<false>(p, Operands{p.x, W, nullptr, p.x_row, kI8}, as_stream(s));
 }

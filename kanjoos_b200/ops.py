@@ -9,7 +9,7 @@ import functools
 import torch
 
 from . import _lib
-from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, check,
+from ._lib import (DT_BF16, DT_E4M3, DT_F16, DT_F32, DT_I8, GATE_CHANNEL, GATE_FULL, GATE_NONE, GATE_ROW, BlockNormArgs, ExpertGemmArgs, Int8MatmulArgs, check,
                    lib, packed)
 
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
@@ -273,7 +273,7 @@ def q4k_down_tc(ah, Wd, pair_idx, pair_cnt, P: int, pair_row=None, poison: bool 
 _cur = torch._C._cuda_getDevice
 _OPERAND = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, _E4M3: DT_E4M3, torch.int8: DT_I8}
 _DT_OR_I8 = {**_DT, torch.int8: DT_I8}
-_norm_args, _expert_args = packed(BlockNormArgs), packed(ExpertGemmArgs)
+_norm_args, _expert_args, _int8_args = packed(BlockNormArgs), packed(ExpertGemmArgs), packed(Int8MatmulArgs)
 _ONLY_F32, _ONLY_I32, _ONLY_E4M3, _ONLY_I8 = {torch.float32: DT_F32}, {torch.int32: 0}, {_E4M3: DT_E4M3}, {torch.int8: DT_I8}
 
 
@@ -387,8 +387,9 @@ def int8_matmul(W: torch.Tensor, W_scale: torch.Tensor, x: torch.Tensor, x_scale
         if nbytes:
             scratch = x.new_empty(nbytes, dtype=torch.uint8)
             work = scratch.data_ptr()
-    check(lib().knj_int8_matmul_launch(w, ws, k, n, ptr, code, xs, ld, m, y.data_ptr(), out_code, n, work, nbytes,
-                                       None if status is None else _dense(status, "status", cur, (1,), _ONLY_I32), _raw_stream()))
+    a = _int8_args(w, ws, ptr, xs, ld, y.data_ptr(), n, work, nbytes, 0 if status is None else _dense(status, "status", cur, (1,), _ONLY_I32),
+                   k, n, m, code, out_code)
+    check(lib().knj_int8_matmul_launch(a, _raw_stream()))
     return y
 
 

@@ -1,4 +1,6 @@
 """int8 rows, the dense int8 product and the products grouped by expert, against their definitions in 64 bits."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -114,8 +116,8 @@ def test_few_rows_write_their_rows_alone():
     w, s = (t.cuda() for t in i8.matrix((37, 64), g))
     x = torch.randn((3, 64), generator=g).cuda()
     y = torch.full((6, 50), -77.0, device="cuda")
-    _lib.check(_lib.lib().knj_int8_matmul_launch(w.data_ptr(), s.data_ptr(), 64, 37, x.data_ptr(), 0, None, 64, 3, y.data_ptr(), 0, 50, None, 0, None,
-                                                 torch.cuda.current_stream().cuda_stream))
+    a = _lib.Int8MatmulArgs(w=w.data_ptr(), w_scale=s.data_ptr(), n_in=64, n_out=37, x=x.data_ptr(), ldx=64, m=3, y=y.data_ptr(), ldy=50)
+    _lib.check(_lib.lib().knj_int8_matmul_launch(C.byref(a), torch.cuda.current_stream().cuda_stream))
     from kanjoos_b200 import ops
     assert torch.equal(y[:3, :37], ops.int8_matmul(w, s, x))
     assert (y[3:] == -77.0).all() and (y[:, 37:] == -77.0).all()

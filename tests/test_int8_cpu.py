@@ -12,7 +12,8 @@ from test_moe_block_cpu import block_args, write_float_file
 
 def test_empty_calls_and_workspaces(L):
     assert L.knj_int8_rows_launch(None, 0, 0, 0, 64, None, None, None) == 0
-    assert L.knj_int8_matmul_launch(None, None, 64, 64, None, 0, None, 64, 0, None, 0, 64, None, 0, None, None) == 0
+    assert L.knj_int8_matmul_launch(C.byref(_lib.Int8MatmulArgs(n_in=64, n_out=64, m=0)), None) == 0
+    refused(L, L.knj_int8_matmul_launch(None, None), "null")
     assert L.knj_int8_matmul_workspace_bytes(0, 64) == 0 and L.knj_int8_matmul_workspace_bytes(9, 130) == 1280 + 256
 
 
@@ -42,8 +43,9 @@ def test_rows_refusals(L, args, word):
 def test_matmul_refusals(L, change, word, code):
     v = dict(W=A, S=A, n_in=64, n_out=8, x=A, dt=0, XS=None, ldx=64, m=9, y=A, yt=0, ldy=8, ws=A, nb=1024)
     v.update(change)
-    rc = L.knj_int8_matmul_launch(v["W"], v["S"], v["n_in"], v["n_out"], v["x"], v["dt"], v["XS"], v["ldx"], v["m"], v["y"], v["yt"], v["ldy"],
-                                  v["ws"], v["nb"], None, None)
+    a = _lib.Int8MatmulArgs(w=v["W"], w_scale=v["S"], n_in=v["n_in"], n_out=v["n_out"], x=v["x"], x_dtype=v["dt"], x_scale=v["XS"], ldx=v["ldx"], m=v["m"],
+                            y=v["y"], y_dtype=v["yt"], ldy=v["ldy"], workspace=v["ws"], workspace_bytes=v["nb"])
+    rc = L.knj_int8_matmul_launch(C.byref(a), None)
     refused(L, rc, word, code)
 
 
