@@ -649,9 +649,9 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
 #define KNJ_MOE_DECODE_MAX_FFN 40960
 #define KNJ_MOE_DECODE_MIN_SMS 64
 int knj_moe_block_decode_launch(const knj_moe_block_args *a, knj_stream_t s);
-/* Test hook of the calling thread: in its next decode launches the 1st or 2nd barrier over the grid is never complete, so that the wait
- * runs into its limit; 0 = off (default). */
-void knj_moe_block_decode_test_stall(int barrier);
+/* Test hook of the calling thread: in its next decode launches 1 = the activations of no expert, 2 = the barrier over the grid is never
+ * complete, so that a wait runs into its limit; 0 = off (default). */
+void knj_moe_block_decode_test_stall(int what);
 /* Outcome of the last launch with this argument block's status word (without one: of the last launch over its workspace, whichever
  * block's that was): waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a bounded wait of its norms or products gave up. */
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s);

@@ -10,15 +10,17 @@
 //
 // Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
 // its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
-// multiply. So the down matrices are on their way while the grid still meets behind gate and up, and the ring's 130 KB and more keep HBM
+// multiply. So the down matrices are on their way while other SMs are still at gate and up, and the ring's 130 KB and more keep HBM
 // busy. A lane takes its weights as 16 bytes of a row, which are MMA fragments as they lie: the order of K is free as long as both operands
 // have the same. tcgen05 gives nothing here: the tensor work of a token is a fiftieth of the time.
 //
-// The first kernel forms norm statistics and router logits. The second, cooperative, has a CTA for each SM and two barriers over the grid:
-//   1  top-k (every CTA for itself); gate, up, silu: every CTA has the same number of matrix rows, of all active experts in a row
-//   2  down, likewise
-//   3  weighted sum, norm, gate, residual, next norm: a CTA for each token
-// (The first stage inside the cooperative kernel needed a third barrier and a fill that cleared its counter in front of the launch.)
+// The first kernel forms norm statistics and router logits. The second, cooperative, has a CTA for each SM:
+//   1  top-k (every CTA for itself); gate, up, silu: every CTA has matrix rows of the same cost, of all active experts in a row
+//   2  down, likewise, as soon as gate and up of the CTA's own experts are done everywhere (a count of rows for each expert; a barrier over
+//      the grid in its place waits for the slowest SM of all: 16 tokens bf16 150 us, so 146, int8 4 tokens 53.6, so 52.2)
+//   3  behind a barrier over the grid: weighted sum, norm, gate, residual, next norm, a CTA for each token
+// (The first stage inside the cooperative kernel needed one barrier more and a fill that cleared its counter in front of the launch.)
+// A block of 128 experts of 2048 x 768, top 8, takes 32 us for one token in bf16 and 146 for sixteen (5.1 TB/s over its whole length).
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
 #include <type_traits>
 
@@ -46,7 +48,8 @@ constexpr int kSmem = 213 * 1024;              // sums, planes of the rows in us
 // int8: the scales of a slot's rows, up to 32 of gate and of up or 64 of down, in whole 16-byte units
 constexpr int kScales = 80;
 constexpr int kMaxItems = 64;
-constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4, kHead = kStatsAt + 256;   // of the workspace
+constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4,
+                 kReadyAt = kStatsAt + 256, kHead = kReadyAt + kMaxExperts * 4;   // of the workspace
 constexpr float kDown = 0x1p-64f;
 
 enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
@@ -74,6 +77,7 @@ struct DecodeParams {
   float *logits, *act, *Y;
   unsigned *sync;               // [0] arrivals, [1] raised by a wait that gave up; cleared by the first kernel
   float2 *stats;                // [tokens] inverse norm, largest magnitude of the normalised row
+  unsigned *ready;              // [experts] matrix rows of gate and up whose outputs are written; cleared by the first kernel
   unsigned *row_max;            // [pairs] bits of the largest magnitude of an activation row; cleared by the first kernel
   int32_t *status;
   int64_t ldx, ldo, ldg, ldh;
@@ -83,7 +87,7 @@ struct DecodeParams {
   int x_vec;                    // rows of x are whole 16-byte units
   float alpha, beta, eps;
   long long wait_cycles;
-  int stall;                    // test hook: this barrier's target is out of reach
+  int stall;                    // test hook: 1 = no expert's rows are ever ready, 2 = the barrier's target is out of reach
 };
 thread_local int t_stall = 0;
 
@@ -126,23 +130,22 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
 }
 // of the warps that multiply
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-// Barrier over the grid, number `n` of the launch, in two halves, met by the warps that multiply. A CTA in which a wait has given up never
-// arrives; grid_wait is false for all threads where the barrier did not complete in time.
+// Waits of thread 0 (of an expert's rows: of any thread) for a word that other CTAs add to: false where it did not come to `target` in time.
+__device__ __forceinline__ bool reaches(const DecodeParams &p, const Shared &s, const unsigned *word, unsigned target) {
+  const long long t0 = clock64();
+  while (ld_acquire(word) < target)
+    if (*reinterpret_cast<const volatile int *>(&s.fail) != 0 || ld_acquire(p.sync + 1) != 0u || clock64() - t0 > p.wait_cycles) return false;
+  return true;
+}
+__device__ __forceinline__ void add_release(unsigned *word, unsigned n) { asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(word), "r"(n) : "memory"); }
+// Barrier over the grid, in two halves, met by the warps that multiply. A CTA in which a wait has given up never arrives; grid_wait is
+// false for all threads where the barrier did not complete in time.
 __device__ __forceinline__ void grid_arrive(const DecodeParams &p, Shared &s) {
   meet();
-  if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0)
-    asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(p.sync), "r"(1u) : "memory");
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0) add_release(p.sync, 1u);
 }
-__device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s, int n) {
-  if (threadIdx.x == 0) {
-    int ok = *reinterpret_cast<volatile int *>(&s.fail) == 0;
-    const unsigned target = gridDim.x * (unsigned)n + (p.stall == n ? 1u : 0u);
-    const long long t0 = clock64();
-    while (ok && ld_acquire(p.sync) < target) {
-      if (ld_acquire(p.sync + 1) != 0u || clock64() - t0 > p.wait_cycles) ok = 0;
-    }
-    s.ok = ok;
-  }
+__device__ __forceinline__ bool grid_wait(const DecodeParams &p, Shared &s) {
+  if (threadIdx.x == 0) s.ok = *reinterpret_cast<volatile int *>(&s.fail) == 0 && reaches(p, s, p.sync, gridDim.x + (p.stall == 2 ? 1u : 0u));
   meet();
   return s.ok != 0;
 }
@@ -408,6 +411,14 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
   const int tid = threadIdx.x, pitch = Geo<KIND>::pitch(K);
   int n = 0, built = i;
   for (; built < plan.n_items && plan.item[built].panel == i; ++built) n += plan.item[built].n;
+  if (!GATEUP) {   // the experts' rows of activations, from the CTAs that gate and up were dealt to
+    if (tid < built - i) {
+      const int e = plan.item[i + tid].expert, pass = Geo<KIND>::pass(p.H);
+      const unsigned whole = (unsigned)p.F * ((__popc(s.mask[e]) + pass - 1) / pass);
+      if (!reaches(p, s, p.ready + e, whole + (p.stall == 1 ? 1u : 0u))) *reinterpret_cast<volatile int *>(&s.fail) = 1;
+    }
+    meet();
+  }
   if (tid < n) {
     int r = tid, j = i;
     while (r >= plan.item[j].n) r -= plan.item[j++].n;
@@ -654,6 +665,7 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
       in_batch = 0;
       meet();
     }
+    if (GATEUP && threadIdx.x == 0 && *reinterpret_cast<volatile int *>(&s.fail) == 0) add_release(p.ready + it.expert, (unsigned)(last - it.r0));
     base += n;
   }
 }
@@ -933,6 +945,7 @@ __global__ void __launch_bounds__(kThreads) moe_decode_front_kernel(const __grid
     if (tid < 2) p.sync[tid] = 0u;
     if (tid == 2) *p.status = 0;
     if (tid < kMaxTokens * kMaxK) p.row_max[tid] = 0u;
+    if (tid < kMaxExperts) p.ready[tid] = 0u;
   }
   float ss[SIDE], most[SIDE], dot[SIDE][SIDE];
 #pragma unroll
@@ -1097,18 +1110,14 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   }
   if (p.shape[0].eight) run_product<KIND, true, true>(p, s, ring, panel, sums, slots);
   else run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
+  if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
+  else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
   grid_arrive(p, s);
   const int t = blockIdx.x;
-  bool ok = grid_wait(p, s, 1);
-  if (ok) {
-    if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
-    else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
-    grid_arrive(p, s);
-    Finish end;
-    if (t < p.T) end.prepare(p, t);
-    ok = grid_wait(p, s, 2);
-    if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
-  }
+  Finish end;
+  if (t < p.T) end.prepare(p, t);
+  const bool ok = grid_wait(p, s);
+  if (ok && t < p.T) end.run(p, s, t, reinterpret_cast<float *>(panel));
   if (!ok) give_up(p, s);   // ends the copying warp's waits, too
 }
 
@@ -1173,6 +1182,7 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   p.sync = reinterpret_cast<unsigned *>(ws + kSyncAt);   // behind the status word of the whole block
   p.row_max = reinterpret_cast<unsigned *>(ws + kMaxAt);
   p.stats = reinterpret_cast<float2 *>(ws + kStatsAt);
+  p.ready = reinterpret_cast<unsigned *>(ws + kReadyAt);
   ws += kHead;
   p.logits = reinterpret_cast<float *>(ws);
   ws += up256((size_t)T * E * 4);
@@ -1196,4 +1206,4 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
 }
 }  // namespace knj
 
-extern "C" void knj_moe_block_decode_test_stall(int barrier) { t_stall = barrier >= 1 && barrier <= 2 ? barrier : 0; }
+extern "C" void knj_moe_block_decode_test_stall(int what) { t_stall = what == 1 || what == 2 ? what : 0; }
