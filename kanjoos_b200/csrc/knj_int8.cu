@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(256, 4) int8_few_kernel(const int8_t *W, const
           const uint4 c = *reinterpret_cast<const uint4 *>(codes + r * K + 16 * u);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            acc[h][r] = __dp4a((int)w[h][i].x, (int)c.x, __dp4a((int)w[h][i].y, (int)c.y, __dp4a((int)w[h][i].z, (int)c.z, __dp4a((int)w[h][i].w, (int)c.w, acc[h][r]))));
+            acc[h][r] = __dp4a((int)w[h][i].x, (int)c.x, __dp4a((int)w[h][i].y, (int)c.y,
+                        __dp4a((int)w[h][i].z, (int)c.z, __dp4a((int)w[h][i].w, (int)c.w, acc[h][r]))));
         }
       }
       const bool more = from + 128 < units;

@@ -20,7 +20,7 @@
 //      the grid in its place waits for the slowest SM of all: 16 tokens bf16 150 us, so 146, int8 4 tokens 53.6, so 52.2)
 //   3  behind a barrier over the grid: weighted sum, norm, gate, residual, next norm, a CTA for each token
 // (The first stage inside the cooperative kernel needed one barrier more and a fill that cleared its counter in front of the launch.)
-// A block of 128 experts of 2048 x 768, top 8, takes 32 us for one token in bf16 and 146 for sixteen (5.1 TB/s over its whole length).
+// A block of 128 experts of 2048 x 768, top 8, takes 32 us for one token in bf16 and 146 for sixteen (5.3 TB/s over both kernels).
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
 #include <type_traits>
 
@@ -256,7 +256,8 @@ template <int KIND>
 struct Geo {
   static constexpr int kElem = KIND <= kF16 ? 2 : 1;
   // Groups of warps that take the tiles in turn, and warps of one: so that a warp has about four runs of a slot, of rows of 2048 x 2 bytes eight.
-  // (Of 4 and 2 groups, us: bf16 1 token 31.8, 33.4, 4 tokens 64.5, 67.4, 16 tokens 147, 150; e4m3 5 tokens 62.8, 59.8; int8 8 tokens 78.5, 77.0, 16 tokens 107, 109.)
+  // (Of 4 and 2 groups, us: bf16 1 token 31.8, 33.4, 4 tokens 64.5, 67.4, 16 tokens 147, 150; e4m3 5 tokens 62.8, 59.8; int8 8 tokens 78.5,
+  // 77.0, 16 tokens 107, 109.)
   static constexpr int kGroups = KIND <= kF16 ? 4 : 2, kTeam = kWarps / kGroups;
   // bytes of a plane of K values: whole runs of 128 bytes of weights, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
   __host__ __device__ static int pitch(int K) { return (K * kElem + 127) / 128 * (256 / kElem) + (kElem == 2 ? 64 : 16); }
@@ -324,8 +325,8 @@ __device__ __forceinline__ bool feed(const DecodeParams &p, Shared &s, int produ
 
 // A lane's part of a run of 128 bytes (two steps of 64) of sixteen rows: of rows g and g + 8 the bytes 16 j .. + 15 of either step. (Rows a
 // multiple of 128 bytes apart lie on the same banks, and such a load takes two turns. SWAP: odd rows read their second step first, and the
-// two change places in registers. Of bf16 and fp16 experts that pays, 16 tokens 162 -> 155 us; of codes the instructions are dearer.) left: bytes of the rows from the run's first
-// on; what lies behind is zero.
+// two change places in registers. Of bf16 and fp16 experts that pays, 16 tokens 162 -> 155 us; of codes the instructions are dearer.)
+// left: bytes of the rows from the run's first on; what lies behind is zero.
 template <int ROWS>   // two, or of tiles of eight rows one
 struct Weights {
   uint4 w[2][ROWS];   // [step][row]
@@ -559,7 +560,9 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
         }
       } else {
         const bool mine = first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
-        float acc[3][4] = {};   // tokens 0 .. 3 (EIGHT: all), even and odd steps; 4 .. 7
+        // tokens 0 .. 3, 4 .. 7 (EIGHT: all, even and odd steps): no sum's order depends on a token's place. (Two accumulators for either four
+        // tokens take registers that are not there: int8 16 tokens 110 us, so 100.)
+        float acc[2][4] = {};
         // e4m3: scales of the blocks of rows g and g + 8; EIGHT: of rows 2 j and 2 j + 1, which are in one, runs starting at even rows
         const float *sc0 = nullptr, *sc1 = nullptr;
         if constexpr (KIND == kE4) {
@@ -601,13 +604,13 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
               for (int u = 0; u < 2; ++u) {
                 const int here = at + (r * run + u * 64) * (2 / kElem);
                 if constexpr (EIGHT) step<KIND>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[u]);
-                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[u], KIND == kE4 ? t[1] : acc[2]);
+                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[0], KIND == kE4 ? t[1] : acc[1]);
               }
               if constexpr (KIND == kE4) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                   acc[0][c] = fmaf(f[r][EIGHT ? 0 : c >> 1], t[0][c], acc[0][c]);
-                  if (kTwo) acc[2][c] = fmaf(f[r][c >> 1], t[1][c], acc[2][c]);
+                  if (kTwo) acc[1][c] = fmaf(f[r][c >> 1], t[1][c], acc[1][c]);
                 }
               }
             };
@@ -648,12 +651,12 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           } else {
             dst += j * 16 + g;
             if (j < n) {
-              dst[0] = ((acc[0][0] + acc[1][0]) + (acc[0][1] + acc[1][1])) * row_scale[0];
-              dst[8] = ((acc[0][2] + acc[1][2]) + (acc[0][3] + acc[1][3])) * row_scale[1];
+              dst[0] = (acc[0][0] + acc[0][1]) * row_scale[0];
+              dst[8] = (acc[0][2] + acc[0][3]) * row_scale[1];
             }
             if (4 + j < n) {
-              dst[64] = (acc[2][0] + acc[2][1]) * row_scale[0];
-              dst[72] = (acc[2][2] + acc[2][3]) * row_scale[1];
+              dst[64] = (acc[1][0] + acc[1][1]) * row_scale[0];
+              dst[72] = (acc[1][2] + acc[1][3]) * row_scale[1];
             }
           }
         }

@@ -169,6 +169,24 @@ def test_rows_stand_for_themselves(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("H,F", [(512, 208), (1024, 1040), (2304, 48), (256, 4160)])
+def test_a_token_has_the_same_bits_at_any_place(kind, H, F):
+    """Up to sixteen tokens of an expert, in tiles of sixteen rows and of eight: alone, in front of or behind others."""
+    from kanjoos_b200.moe import MoeBlock
+    T, k = 16, 2
+    blk = MoeBlock(on_device(bank(kind, 3, H, F, 34)), top_k=k, max_tokens=T)
+    x = rows(T, H, 92).cuda()
+    want, pe, pw = blk.decode(x, return_routing=True)
+    assert pe.bincount().max() > 8
+    for a, b in [(i, i + 1) for i in range(T)] + [(0, 5), (3, 12), (9, 16), (5, 14)]:
+        out, e, w = blk.decode(x[a:b], return_routing=True)
+        assert torch.equal(e, pe[a * k:b * k]) and torch.equal(w, pw[a * k:b * k])
+        assert torch.equal(out, want[a:b]), (a, b)
+    turned = blk.decode(x.flip(0))
+    assert torch.equal(turned.flip(0), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_same_bits_again_in_place_captured_and_on_another_stream(kind):
     from kanjoos_b200.moe import MoeBlock
     T, H, k = 12, 512, 4
