@@ -641,10 +641,11 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
 /* The same block for 1 to KNJ_MOE_DECODE_MAX_TOKENS tokens in two kernels, the second a cooperative launch (one thread block per SM: it
  * needs a device of KNJ_MOE_DECODE_MIN_SMS SMs or more that the process has to itself, as the whole-stack launch does), bound by the
  * bytes of the experts in use. Between x and out nothing is rounded to 16 or 8 bits: rows reach the experts' products as the f32 values
- * that the norm forms (to 17 bits with bf16 experts, to 22 with the others), and e4m3 and int8 experts multiply them with the values
- * that their codes stand for. Results are therefore nearer to the formulas than knj_moe_block_launch's and differ from them by its
- * roundings; a pair of experts whose logits are that close may be chosen the other way. ffn at most KNJ_MOE_DECODE_MAX_FFN; pre_w and
- * the scales of int8 experts 16-byte aligned; other fields, workspace and status as for knj_moe_block_launch. */
+ * that the norm forms (all 24 bits of them with bf16 experts, but 17 in rows of more than 22656 values; 22 bits with the others), and
+ * e4m3 and int8 experts multiply them with the values that their codes stand for. Results are therefore nearer to the formulas than
+ * knj_moe_block_launch's and differ from them by its roundings; a pair of experts whose logits are that close may be chosen the other
+ * way. ffn at most KNJ_MOE_DECODE_MAX_FFN; pre_w and the scales of int8 experts 16-byte aligned; other fields, workspace and status as
+ * for knj_moe_block_launch. */
 #define KNJ_MOE_DECODE_MAX_TOKENS 16
 #define KNJ_MOE_DECODE_MAX_FFN 40960
 #define KNJ_MOE_DECODE_MIN_SMS 64

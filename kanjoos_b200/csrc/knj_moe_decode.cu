@@ -4,9 +4,13 @@
 //   y   = sum over the top_k experts of softmax weight * down(silu(gate(h)) * up(h))
 //   out = beta * x + alpha * g * norm(y; post_w),   h_next = norm(out; next_w)
 // What is computed between x and out stays in f32, and so does what the matrices are multiplied with: a row of f32 values goes to the
-// tensor core as two 16-bit planes, hi = round(v) and lo = round(v - hi), which together hold 17 bits of v (bf16 experts, bf16 planes) or 22
-// (fp16 planes under a power of two for each row, for the others: their codes are exact in fp16). In mma.sync.m16n8k16 sixteen matrix rows
-// meet the two planes of four tokens, or eight rows those of eight, so that the second plane costs nothing while weights are on their way.
+// tensor core as 16-bit planes, each the rounded rest that the ones in front of it leave. bf16 experts meet three bf16 planes, which hold
+// all 24 bits of a value; the others two fp16 planes under a power of two for each row, which hold 22 (their codes are exact in fp16). In
+// mma.sync.m16n8k16 sixteen matrix rows meet the eight planes of two (two planes: four) tokens, or eight rows the sixteen of five (eight),
+// so that further planes cost little while weights are on their way. (Two planes in bf16, 17 bits, left the block's part off by 4e-6 of its
+// norm, which an f32 stream shows. us with two planes and three: 128 experts of 2048 x 768, 1, 4, 16 tokens 32, 64, 145 and 33.5, 66, 148; 32
+// of 1024 x 512, 16 tokens 36 and 40; 8 of 8192 x 2048, top 2, 16 tokens, whose planes take twice the passes, 319 and 376.) Rows so long
+// that three planes of one leave the ring less than two slots, above 22656 values, stay with two.
 //
 // Bound by the bytes of the experts that the tokens use, each read once: one token, 8 experts of 2048 x 768 in bf16, 75.5 MB. A warp of
 // its own streams this CTA's matrix rows, of gate and up and behind them of down, through a ring in shared memory; sixteen warps
@@ -20,7 +24,7 @@
 //      the grid in its place waits for the slowest SM of all: 16 tokens bf16 150 us, so 146, int8 4 tokens 53.6, so 52.2)
 //   3  behind a barrier over the grid: weighted sum, norm, gate, residual, next norm, a CTA for each token
 // (The first stage inside the cooperative kernel needed one barrier more and a fill that cleared its counter in front of the launch.)
-// A block of 128 experts of 2048 x 768, top 8, takes 32 us for one token in bf16 and 146 for sixteen (5.3 TB/s over both kernels).
+// A block of 128 experts of 2048 x 768, top 8, takes 33.5 us for one token in bf16 and 148 for sixteen (5.2 TB/s over both kernels), in a graph.
 // Every wait is bounded (knj_decode_wait_limit): on give-up the status word is raised and the outputs are NaN.
 #include <type_traits>
 
@@ -52,7 +56,7 @@ constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * k
                  kReadyAt = kStatsAt + 256, kHead = kReadyAt + kMaxExperts * 4;   // of the workspace
 constexpr float kDown = 0x1p-64f;
 
-enum Kind { kBf16 = 0, kF16 = 1, kE4 = 2, kS8 = 3 };
+enum Kind { kBf16 = 0, kBf16Many = 1, kF16 = 2, kE4 = 3, kS8 = 4 };   // kBf16Many: see launch_bf16
 
 // Of a product: its rows in memory, and how they are cut
 struct Shape {
@@ -60,6 +64,7 @@ struct Shape {
   int slices, slice;   // of a row, bytes
   int eight;           // tiles of eight rows, else sub-tiles of sixteen
   int subs;            // sub-tiles of a tile, among which a group's warps are split
+  int planes;          // of a row of activations
   int outs;            // outputs of a tile: its matrix rows, of which of gate and up the first half is gate's
 };
 
@@ -198,26 +203,28 @@ __device__ __forceinline__ void row_power(float m, float &mult, float &unmult) {
   unmult = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 }
 
+// a plane of two values, in which what it leaves out stays
 template <int KIND>
-__device__ __forceinline__ void planes2(float a, float b, uint32_t &hi, uint32_t &lo) {
-  if constexpr (KIND == kBf16) {
+__device__ __forceinline__ uint32_t plane2(float &a, float &b) {
+  uint32_t bits;
+  float2 f;
+  if constexpr (KIND <= kBf16Many) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const float2 f = __bfloat1622float2(h);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+    f = __bfloat1622float2(h);
+    bits = *reinterpret_cast<const uint32_t *>(&h);
   } else {
     const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+    f = __half22float2(h);
+    bits = *reinterpret_cast<const uint32_t *>(&h);
   }
+  a -= f.x;
+  b -= f.y;
+  return bits;
 }
 
 template <int KIND>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (KIND == kBf16)
+  if constexpr (KIND <= kBf16Many)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -261,15 +268,20 @@ struct Geo {
   static constexpr int kGroups = KIND <= kF16 ? 4 : 2, kTeam = kWarps / kGroups;
   // bytes of a plane of K values: whole runs of 128 bytes of weights, and rows an odd 64 (of codes: 16) bytes apart, for the banks as in the ring
   __host__ __device__ static int pitch(int K) { return (K * kElem + 127) / 128 * (256 / kElem) + (kElem == 2 ? 64 : 16); }
+  __host__ __device__ static int planes(int K) { return KIND <= kBf16Many && 3 * pitch(K) <= kSmem - kRed - 2 * kSlot ? 3 : 2; }
+  // Most rows of a pass. bf16: the planes of five are the sixteen rows or columns of two MMAs. (A form of up to eight besides, us: tiles of eight
+  // rows, 1 token 35.9, so 33.6, 16 tokens 157, so 148; tiles of sixteen, 1 token 34.1, 16 tokens 151.)
+  static constexpr int kMost = KIND == kBf16 ? 5 : kMaxRows;
   // rows of a pass: what leaves the ring two slots, or one
   __host__ __device__ static int pass(int K) {
-    const int c = (kSmem - kRed - 2 * kSlot) / (2 * pitch(K));
-    return c < 1 ? 1 : c < kMaxRows ? c : kMaxRows;
+    const int c = (kSmem - kRed - 2 * kSlot) / (planes(K) * pitch(K));
+    return c < 1 ? 1 : c < kMost ? c : kMost;
   }
-  // rows in the panel at a time: what leaves it four slots, or those of a pass
+  // Rows in the panel at a time: what leaves it four slots, or those of a pass. (bf16: a pass of more rows is alone there.)
   __host__ __device__ static int cap(int K) {
-    const int c = (kSmem - kRed - 4 * kSlot) / (2 * pitch(K));
-    return c < pass(K) ? pass(K) : c < kMaxTokens ? c : kMaxTokens;
+    const int c = (kSmem - kRed - 4 * kSlot) / (planes(K) * pitch(K));
+    if (KIND > kBf16Many && c < pass(K)) return pass(K);
+    return c < 1 ? 1 : c < kMaxTokens ? c : kMaxTokens;
   }
 };
 
@@ -357,9 +369,12 @@ struct Acts {
     if constexpr (KIND > kF16) b[1] = *reinterpret_cast<const uint4 *>(at + 16);
   }
 };
-// One step of sixteen rows times the planes of four tokens, or (TWO) of eight
-template <int KIND, bool TWO>
-__device__ __forceinline__ void step(const uint4 (&w)[2], const uint8_t *x0, const uint8_t *x1, float (&acc0)[4], float (&acc1)[4]) {
+// One step of sixteen rows times SETS sets of eight planes, in the order that run_product gives them
+template <int KIND, int SETS>
+__device__ __forceinline__ void step(const uint4 (&w)[2], const uint8_t *x0, const uint8_t *x1, const uint8_t *x2, float (&acc0)[4], float (&acc1)[4],
+                                     float (&acc2)[4]) {
+  constexpr bool TWO = SETS >= 2;
+  if constexpr (SETS == 3) step<KIND, 1>(w, x2, x2, x2, acc2, acc2, acc2);
   Acts<KIND> a, b;
   a.load(x0);
   if constexpr (TWO) b.load(x1);
@@ -385,12 +400,12 @@ __device__ __forceinline__ void step(const uint4 (&w)[2], const uint8_t *x0, con
   }
 }
 
-// One step of eight rows times the planes of eight tokens, which are the MMA's sixteen rows here
+// One step of eight rows times sixteen planes, which are the MMA's rows here
 template <int KIND>
-__device__ __forceinline__ void step(const uint4 (&w)[1], const uint8_t *hi, const uint8_t *lo, float (&acc)[4]) {
+__device__ __forceinline__ void step(const uint4 (&w)[1], const uint8_t *x0, const uint8_t *x1, float (&acc)[4]) {
   Acts<KIND> h, l;
-  h.load(hi);
-  l.load(lo);
+  h.load(x0);
+  l.load(x1);
   if constexpr (KIND <= kF16) {
     mma<KIND>(acc, h.b[0].x, l.b[0].x, h.b[0].y, l.b[0].y, w[0].x, w[0].y);
     mma<KIND>(acc, h.b[0].z, l.b[0].z, h.b[0].w, l.b[0].w, w[0].z, w[0].w);
@@ -409,7 +424,7 @@ __device__ __forceinline__ void step(const uint4 (&w)[1], const uint8_t *hi, con
 // The rows of items i .. in the panel, as many as it takes: their planes, zeros behind K up to whole runs. Returns the item behind them.
 template <int KIND, bool GATEUP>
 __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, const Plan &plan, int K, uint8_t *panel, int i) {
-  const int tid = threadIdx.x, pitch = Geo<KIND>::pitch(K);
+  const int tid = threadIdx.x, pitch = Geo<KIND>::pitch(K), planes = Geo<KIND>::planes(K);
   int n = 0, built = i;
   for (; built < plan.n_items && plan.item[built].panel == i; ++built) n += plan.item[built].n;
   if (!GATEUP) {   // the experts' rows of activations, from the CTAs that gate and up were dealt to
@@ -426,7 +441,7 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
     const int pair = s.pair_at[plan.item[j].expert][plan.item[j].first + r], t = pair / p.k;
     s.row_tok[tid] = t;
     s.row_pair[tid] = pair;
-    if constexpr (KIND != kBf16) {
+    if constexpr (KIND > kBf16Many) {
       if (GATEUP) {
         s.row_mult[tid] = s.mult[t];
         s.row_unmult[tid] = s.unmult[t];
@@ -462,19 +477,22 @@ __device__ __forceinline__ int build_panel(const DecodeParams &p, Shared &s, con
       const float4 a = __ldcg(src), b = __ldcg(src + 1);
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
-    if constexpr (KIND != kBf16) {
+    if constexpr (KIND > kBf16Many) {
       const float mult = s.row_mult[r];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= mult;
     }
-    uint4 hi, lo;
-    planes2<KIND>(v[0], v[1], hi.x, lo.x);
-    planes2<KIND>(v[2], v[3], hi.y, lo.y);
-    planes2<KIND>(v[4], v[5], hi.z, lo.z);
-    planes2<KIND>(v[6], v[7], hi.w, lo.w);
-    uint8_t *dst = panel + (2 * r) * pitch + 16 * c;
-    *reinterpret_cast<uint4 *>(dst) = hi;
-    *reinterpret_cast<uint4 *>(dst + pitch) = lo;
+    uint8_t *dst = panel + (planes * r) * pitch + 16 * c;
+#pragma unroll
+    for (int i = 0; i < (KIND <= kBf16Many ? 3 : 2); ++i) {
+      if (i == planes) break;
+      uint4 q;
+      q.x = plane2<KIND>(v[0], v[1]);
+      q.y = plane2<KIND>(v[2], v[3]);
+      q.z = plane2<KIND>(v[4], v[5]);
+      q.w = plane2<KIND>(v[6], v[7]);
+      *reinterpret_cast<uint4 *>(dst + i * pitch) = q;
+    }
   }
   return built;
 }
@@ -500,13 +518,13 @@ __device__ __forceinline__ void add_parts(const DecodeParams &p, Shared &s, cons
           a += src[w * tokens * 16];
           if (GATEUP) b += src[w * tokens * 16 + kOuts];
         }
-        const float un = KIND == kBf16 ? 1.0f : s.row_unmult[base + tok];
+        const float un = KIND <= kBf16Many ? 1.0f : s.row_unmult[base + tok];
         a *= un;
         b *= un;
         if (GATEUP) a = a / (1.0f + expf(-a)) * b;
         (GATEUP ? p.act : p.Y)[(int64_t)s.row_pair[base + tok] * sh.N + row] = a;
       }
-      if constexpr (GATEUP && KIND != kBf16) {
+      if constexpr (GATEUP && KIND > kBf16Many) {
         float m = in ? fabsf(a) : 0.f;
 #pragma unroll
         for (int x = kOuts / 2; x > 0; x >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, x));
@@ -546,9 +564,30 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
       meet();
     }
     const int n = it.n, last = it.r1, batch = kRed / (64 * kTeam * n);   // tiles whose sums fit
-    // this lane's run of a plane of one of the first four tokens, and of the others; EIGHT: of both planes of one of eight
-    const uint8_t *x0 = panel + (EIGHT ? 2 * (base + min(g, n - 1)) : 2 * (base + min(g >> 1, n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
-    const uint8_t *x1 = EIGHT ? x0 + pitch : panel + (2 * (base + min(4 + (g >> 1), n - 1)) + (g & 1)) * pitch + (part * 128 + j * 16) * (2 / kElem);
+    // This lane's runs of the planes that are the MMAs' columns g, 8 + g and 16 + g (EIGHT: rows). Two planes: both of the first four tokens, then of
+    // the others; EIGHT: the first plane of eight tokens, then the second. Three planes of
+    //   up to two tokens   each plane of either
+    //   up to five         the first two planes of tokens 0 .. 3; their third and between them the planes of token 4
+    //   kBf16Many          the first two planes of tokens 0 .. 3; the third of 0, 4, 1, 5 ..; the first two of tokens 4 .. 7
+    //   EIGHT              the first plane of five tokens and the third of 0, 1, 2; the second plane of five and the third of 3, 4
+    auto run_of = [&](int token, int plane) { return panel + (sh.planes * (base + min(token, n - 1)) + plane) * pitch + (part * 128 + j * 16) * (2 / kElem); };
+    const uint8_t *x0, *x1;
+    const uint8_t *x2 = panel;   // kBf16Many
+    if constexpr (KIND <= kBf16Many && EIGHT) {
+      x0 = g < 5 ? run_of(g, 0) : run_of(g - 5, sh.planes - 1);
+      x1 = g < 5 ? run_of(g, 1) : run_of(g - 2, sh.planes - 1);
+    } else if constexpr (KIND <= kBf16Many) {
+      x0 = n <= 2 ? run_of(g & 1, min(g >> 1, 2)) : run_of(g >> 1, g & 1);
+      if constexpr (KIND == kBf16) {
+        x1 = g & 1 ? run_of(4, min(g >> 1, 2)) : run_of(g >> 1, 2);
+      } else {
+        x1 = run_of((g >> 1) + 4 * (g & 1), 2);
+        x2 = run_of(4 + (g >> 1), g & 1);
+      }
+    } else {
+      x0 = EIGHT ? run_of(g, 0) : run_of(g >> 1, g & 1);
+      x1 = EIGHT ? run_of(g, 1) : run_of(4 + (g >> 1), g & 1);
+    }
     int in_batch = 0;
     for (int first = it.r0; first < last; first += sh.outs) {
       if (turn != group) {
@@ -560,9 +599,10 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
         }
       } else {
         const bool mine = first + sub * kOuts < last;   // the last tile may have fewer sub-tiles
-        // tokens 0 .. 3, 4 .. 7 (EIGHT: all, even and odd steps): no sum's order depends on a token's place. (Two accumulators for either four
+        // columns 0 .. 7, 8 .. 15, 16 .. (EIGHT: rows 0 .. 15, even and odd steps, 16 ..): no sum's order depends on a token's place. (Two accumulators for either four
         // tokens take registers that are not there: int8 16 tokens 110 us, so 100.)
-        float acc[2][4] = {};
+        constexpr int kSets = KIND == kBf16Many ? 3 : 2, kLast = kSets - 1;
+        float acc[kSets][4] = {};
         // e4m3: scales of the blocks of rows g and g + 8; EIGHT: of rows 2 j and 2 j + 1, which are in one, runs starting at even rows
         const float *sc0 = nullptr, *sc1 = nullptr;
         if constexpr (KIND == kE4) {
@@ -593,8 +633,7 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
           }
           const uint8_t *slot = slots + ring.at * kSlot + row0, *slot1 = slot + (GATEUP ? sh.outs : 8) * sh.slice;
           const int at = sl * sh.slice * (2 / kElem), run = parts * 128;
-          auto runs = [&](auto two) {
-            constexpr bool kTwo = decltype(two)::value;
+          auto runs = [&](auto sets) {
             auto one = [&](int r, int rest) {
               Weights<EIGHT ? 1 : 2> v;
               v.template load<kSwap>(slot + r * run, slot1 + r * run, odd, rest);
@@ -604,13 +643,13 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
               for (int u = 0; u < 2; ++u) {
                 const int here = at + (r * run + u * 64) * (2 / kElem);
                 if constexpr (EIGHT) step<KIND>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[u]);
-                else step<KIND, kTwo>(v.w[u], x0 + here, x1 + here, KIND == kE4 ? t[0] : acc[0], KIND == kE4 ? t[1] : acc[1]);
+                else step<KIND, decltype(sets)::value>(v.w[u], x0 + here, x1 + here, x2 + here, KIND == kE4 ? t[0] : acc[0], KIND == kE4 ? t[1] : acc[1], acc[kLast]);
               }
               if constexpr (KIND == kE4) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                   acc[0][c] = fmaf(f[r][EIGHT ? 0 : c >> 1], t[0][c], acc[0][c]);
-                  if (kTwo) acc[1][c] = fmaf(f[r][c >> 1], t[1][c], acc[1][c]);
+                  if (decltype(sets)::value == 2) acc[1][c] = fmaf(f[r][c >> 1], t[1][c], acc[1][c]);
                 }
               }
             };
@@ -636,15 +675,54 @@ __device__ __forceinline__ void run_product(const DecodeParams &p, Shared &s, Ri
               }
             }
           };
-          if (EIGHT || n <= 4) runs(std::false_type());
-          else runs(std::true_type());
+          if (EIGHT || n <= (KIND <= kBf16Many ? 2 : 4)) runs(std::integral_constant<int, 1>());
+          else runs(std::integral_constant<int, kSets>());
           __syncwarp();
           if (lane == 0 && ok) mbar_arrive(&s.empty[ring.at]);
           ring.next();
         }
         if (mine) {
           float *dst = sums + ((in_batch * subs + sub) * parts + part) * n * 16;
-          if constexpr (EIGHT) {
+          if constexpr (KIND <= kBf16Many && EIGHT) {
+            float v[4], third[2];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = acc[0][c] + acc[1][c];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int from = (g < 3 ? 5 + g : 2 + g) * 4 + j;
+              const float a = __shfl_sync(0xffffffffu, v[c], from), b = __shfl_sync(0xffffffffu, v[2 + c], from);
+              third[c] = sh.planes == 2 ? 0.f : g < 3 ? a : b;
+            }
+            if (g < n) *reinterpret_cast<float2 *>(dst + g * 16 + 2 * j) = make_float2(v[0] + (v[2] + third[0]), v[1] + (v[3] + third[1]));
+          } else if constexpr (KIND <= kBf16Many) {
+            auto of_lane = [&](float v, int i) { return __shfl_sync(0xffffffffu, v, (lane & ~3) + i); };
+            auto join = [&](float v) { return of_lane(v, 0) + (of_lane(v, 1) + of_lane(v, 2)); };   // a token's planes in three lanes
+            dst += j * 16 + g;
+            if (n <= 2) {
+              const float a0 = join(acc[0][0]), b0 = join(acc[0][1]), a8 = join(acc[0][2]), b8 = join(acc[0][3]);
+              if (j < n) {
+                dst[0] = j == 0 ? a0 : b0;
+                dst[8] = j == 0 ? a8 : b8;
+              }
+            } else {
+              if (j < n) {
+                dst[0] = acc[0][0] + (acc[0][1] + acc[1][0]);
+                dst[8] = acc[0][2] + (acc[0][3] + acc[1][2]);
+              }
+              float e0, e8;
+              if constexpr (KIND == kBf16) {
+                e0 = join(acc[1][1]);
+                e8 = join(acc[1][3]);
+              } else {
+                e0 = acc[kLast][0] + (acc[kLast][1] + acc[1][1]);
+                e8 = acc[kLast][2] + (acc[kLast][3] + acc[1][3]);
+              }
+              if (4 + j < n) {
+                dst[64] = e0;
+                dst[72] = e8;
+              }
+            }
+          } else if constexpr (EIGHT) {
             if (g < n)
               *reinterpret_cast<float2 *>(dst + g * 16 + 2 * j) = make_float2(((acc[0][0] + acc[1][0]) + (acc[0][2] + acc[1][2])) * row_scale[0],
                                                                               ((acc[0][1] + acc[1][1]) + (acc[0][3] + acc[1][3])) * row_scale[1]);
@@ -728,9 +806,10 @@ __device__ __forceinline__ void choose(const float *logits, int E, int k, int la
 // (Gate and up of 16 tokens, time of the CTAs whose fullest expert has 1, 2, 3, 4, 5 tokens: bf16 80, 86, 90, 97, 100 us, int8 53, 54, 56, 56, 68.)
 template <int KIND>
 __device__ __forceinline__ int row_cost(int n) {
-  const int last = n & 7, full = n >> 3;
+  constexpr int kMost = Geo<KIND>::kMost;
+  const int full = n / kMost, last = n - full * kMost;
   auto pass = [](int m) { return KIND <= kF16 ? 15 + m : m <= 4 ? 16 : 20; };
-  return full * pass(8) + (last ? pass(last) : 0);
+  return full * pass(kMost) + (last ? pass(last) : 0);
 }
 // The matrix rows of a product, of all active experts in a row, are dealt to the CTAs by their cost, in pairs of rows. Where CTA b's begin:
 // position `at` of the active list, pair `unit` of its `half`. By a whole warp; every CTA forms the same borders.
@@ -1099,7 +1178,7 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
 
   float *sums = reinterpret_cast<float *>(smem);
   uint8_t *panel = smem + kRed;
-  const int held = max(s.plan[0].rows * 2 * Geo<KIND>::pitch(p.H), s.plan[1].rows * 2 * Geo<KIND>::pitch(p.F));
+  const int held = max(s.plan[0].rows * p.shape[0].planes * Geo<KIND>::pitch(p.H), s.plan[1].rows * p.shape[1].planes * Geo<KIND>::pitch(p.F));
   const int at = kRed + (held + 127) / 128 * 128;
   uint8_t *slots = smem + at;
   Ring ring{0, min(kMaxSlots, (kSmem - at) / kSlot), 0u};
@@ -1111,10 +1190,15 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
     }
     return;
   }
-  if (p.shape[0].eight) run_product<KIND, true, true>(p, s, ring, panel, sums, slots);
-  else run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
-  if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
-  else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
+  if constexpr (KIND == kBf16Many) {   // rows of few bytes alone
+    run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
+    run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
+  } else {
+    if (p.shape[0].eight) run_product<KIND, true, true>(p, s, ring, panel, sums, slots);
+    else run_product<KIND, true, false>(p, s, ring, panel, sums, slots);
+    if (p.shape[1].eight) run_product<KIND, false, true>(p, s, ring, panel, sums, slots);
+    else run_product<KIND, false, false>(p, s, ring, panel, sums, slots);
+  }
   grid_arrive(p, s);
   const int t = blockIdx.x;
   Finish end;
@@ -1131,6 +1215,7 @@ int launch(DecodeParams &p, cudaStream_t st) {
     sh.K = i == 0 ? p.H : p.F;
     sh.N = i == 0 ? p.F : p.H;
     sh.row_bytes = sh.K * Geo<KIND>::kElem;
+    sh.planes = Geo<KIND>::planes(sh.K);
     sh.slices = (sh.row_bytes + kSlice - 1) / kSlice;
     sh.slice = sh.slices == 1 ? sh.row_bytes : ((sh.row_bytes + sh.slices - 1) / sh.slices + 127) / 128 * 128;
     sh.eight = sh.row_bytes > kSlice / 2;
@@ -1155,6 +1240,14 @@ int launch(DecodeParams &p, cudaStream_t st) {
   void *args[] = {&p};
   KNJ_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(kern), dim3(sm_count()), dim3(kAll), args, kSmem, st));
   return launch_status("moe_decode_kernel");
+}
+
+// bf16: passes of up to five tokens, or where experts have three and more on average and no row is in tiles of eight, of up to eight. us, by
+// (experts, hidden, ffn, top_k, tokens), five and eight: (32, 1024, 512, 8, 12) 41.0, 37.8, (.., 16) 46.6, 40.0; (20, 512, 208, 8, 8) 28.3, 25.6,
+// (.., 16) 37.8, 33.3; (8, 1024, 512, 2, 16) 33.3, 28.7. Fewer tokens an expert lose by it: (128, 1024, 512, 8, 16) 65.0, 69.7.
+int launch_bf16(DecodeParams &p, cudaStream_t st) {
+  const int longest = p.H > p.F ? p.H : p.F;
+  return 2 * longest <= kSlice / 2 && p.T * p.k >= 3 * p.E ? launch<kBf16Many>(p, st) : launch<kBf16>(p, st);
 }
 
 }  // namespace
@@ -1201,7 +1294,7 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
   p.wait_cycles = decode_wait_cycles(); p.stall = t_stall; p.grid_inverse = (unsigned)((1ull << 32) / sm_count());
   const cudaStream_t st = as_stream(stream);
   switch (a->w_dtype) {
-    case KNJ_DT_BF16: return launch<kBf16>(p, st);
+    case KNJ_DT_BF16: return launch_bf16(p, st);
     case KNJ_DT_F16: return launch<kF16>(p, st);
     case KNJ_DT_E4M3: return launch<kE4>(p, st);
     default: return launch<kS8>(p, st);
