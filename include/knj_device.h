@@ -630,13 +630,16 @@ typedef struct knj_moe_block_args {
   void *h_next;
   int64_t ld_h_next;
   float *h_next_scale;
-  void *workspace; /* >= knj_moe_block_workspace_bytes(...), 256-byte aligned */
+  void *workspace; /* of knj_moe_block_workspace_bytes(...), 256-byte aligned */
   size_t workspace_bytes;
   int32_t *tap_pair_exp; /* optional [T*k] */
   float *tap_pair_w;
   int32_t *status; /* device word that a launch clears first and sets to 1 when a bounded wait gave up; NULL: the workspace's first */
 } knj_moe_block_args;
+/* Room for either launch below with up to n_tokens tokens; and for knj_moe_block_launch alone, which up to KNJ_MOE_DECODE_MAX_TOKENS tokens may
+ * need less. Each launch checks its own need. */
 size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype);
+size_t knj_moe_block_launch_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype);
 int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
 /* The same block for 1 to KNJ_MOE_DECODE_MAX_TOKENS tokens in two kernels, the second a cooperative launch (one thread block per SM: it
  * needs a device of KNJ_MOE_DECODE_MIN_SMS SMs or more that the process has to itself, as the whole-stack launch does), bound by the

@@ -230,6 +230,7 @@ SIGNATURES = {
     "knj_expert_gateup_launch": (_i, [_vp, _vp]),
     "knj_expert_proj_launch": (_i, [_vp, _vp]),
     "knj_moe_block_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "knj_moe_block_launch_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "knj_moe_block_launch": (_i, [_vp, _vp]),
     "knj_moe_block_decode_launch": (_i, [_vp, _vp]),
     "knj_moe_block_decode_test_stall": (None, [_i]),

@@ -77,7 +77,14 @@ void norm_args(const knj_moe_block_args *a, const BlockWs &w, int32_t *status, k
   }
 }
 
-int check(const knj_moe_block_args *a, const char *who) {
+// what either form needs of the workspace for up to this many tokens
+size_t chain_bytes(int T, int H, int F, int E, int k, int w_dtype) { return carve(nullptr, T, H, F, E, k, w_dtype).bytes; }
+size_t decode_bytes(int T, int H, int F, int E, int k) {
+  return moe_decode_workspace(T < KNJ_MOE_DECODE_MAX_TOKENS ? T : KNJ_MOE_DECODE_MAX_TOKENS, H, F, E, k);
+}
+enum Form { kChain, kDecode, kEither };
+
+int check(const knj_moe_block_args *a, const char *who, Form form) {
   KNJ_REQUIRE(a, "%s: null argument block", who);
   KNJ_REQUIRE(a->n_tokens >= 0 && a->hidden > 0 && a->ffn > 0 && a->n_experts > 0, "%s: bad sizes", who);
   if (a->n_tokens == 0) return KNJ_OK;
@@ -91,7 +98,9 @@ int check(const knj_moe_block_args *a, const char *who) {
   KNJ_REQUIRE(aligned16(a->w_router), "%s: the router's weights must be 16-byte aligned", who);
   KNJ_REQUIRE((int64_t)a->n_tokens * a->top_k <= (1ll << 30), "%s: more than 2^30 pairs of a token and an expert", who);
   KNJ_REQUIRE((a->next_w != nullptr) == (a->h_next != nullptr), "%s: next_w and h_next go together", who);
-  const size_t need = knj_moe_block_workspace_bytes(a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
+  const size_t chain = chain_bytes(a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
+  const size_t one = decode_bytes(a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k);
+  const size_t need = form == kChain ? chain : form == kDecode ? one : chain < one ? chain : one;
   if (!a->workspace || a->workspace_bytes < need) {
     set_error("%s: workspace of %zu bytes needed, %zu given", who, need, a->workspace_bytes);
     return KNJ_E_WORKSPACE;
@@ -106,13 +115,16 @@ extern "C" {
 
 size_t knj_moe_block_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype) {
   if (n_tokens <= 0) return 256;
-  const size_t chain = carve(nullptr, n_tokens, hidden, ffn, n_experts, top_k, w_dtype).bytes;
-  const size_t one = moe_decode_workspace(n_tokens < KNJ_MOE_DECODE_MAX_TOKENS ? n_tokens : KNJ_MOE_DECODE_MAX_TOKENS, hidden, ffn, n_experts, top_k);
+  const size_t chain = chain_bytes(n_tokens, hidden, ffn, n_experts, top_k, w_dtype), one = decode_bytes(n_tokens, hidden, ffn, n_experts, top_k);
   return chain > one ? chain : one;
 }
 
+size_t knj_moe_block_launch_workspace_bytes(int n_tokens, int hidden, int ffn, int n_experts, int top_k, int w_dtype) {
+  return n_tokens <= 0 ? 256 : chain_bytes(n_tokens, hidden, ffn, n_experts, top_k, w_dtype);
+}
+
 int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
-  int rc = check(a, "knj_moe_block");
+  int rc = check(a, "knj_moe_block", kChain);
   if (rc || a->n_tokens == 0) return rc;
   const int T = a->n_tokens, H = a->hidden, F = a->ffn, E = a->n_experts, k = a->top_k, P = T * k;
   const bool q = has_codes(a->w_dtype);
@@ -175,7 +187,7 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s) {
 }
 
 int knj_moe_block_decode_launch(const knj_moe_block_args *a, knj_stream_t s) {
-  int rc = check(a, "knj_moe_block_decode");
+  int rc = check(a, "knj_moe_block_decode", kDecode);
   if (rc || a->n_tokens == 0) return rc;
   const BlockWs w = carve(a->workspace, a->n_tokens, a->hidden, a->ffn, a->n_experts, a->top_k, a->w_dtype);
   int32_t *status = a->status ? a->status : w.status;
@@ -189,7 +201,7 @@ int knj_moe_block_decode_launch(const knj_moe_block_args *a, knj_stream_t s) {
 }
 
 int knj_moe_block_status(const knj_moe_block_args *a, knj_stream_t s) {
-  const int rc = check(a, "knj_moe_block_status");
+  const int rc = check(a, "knj_moe_block_status", kEither);
   if (rc || a->n_tokens == 0) return rc;
   const int32_t *status = a->status ? a->status : static_cast<const int32_t *>(a->workspace);
   int32_t word = 0;

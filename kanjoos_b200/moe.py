@@ -329,7 +329,8 @@ class FloatExpertBank:
 class MoeBlock:
     """One MoE block of a residual stream (knj_moe_block_launch): norm, routing, experts, ordered combine, norm behind the block, gate,
     scaled residual add and, on request, the norm in front of the next block. Bound to a maximum token count: the workspace is
-    allocated once here. run takes any number of tokens up to it, decode the few of a decode step."""
+    allocated once here. run takes any number of tokens up to it, decode the few of a decode step. A workspace that the caller gives may be
+    as small as run alone needs; decode refuses it then."""
 
     def __init__(self, bank: FloatExpertBank, top_k: int = synth.TOP_K, max_tokens: int = 64, workspace: torch.Tensor | None = None):
         E, F, H = bank.gate.shape
@@ -361,9 +362,12 @@ class MoeBlock:
         if bank.router_bias is not None and (tuple(bank.router_bias.shape) != (E,) or bank.router_bias.dtype != torch.float32 or not bank.router_bias.is_contiguous()):
             raise ValueError(f"router_bias is contiguous f32 [{E}]")
         self.bank, self.top_k, self.max_tokens = bank, top_k, max_tokens
-        need = lib().knj_moe_block_workspace_bytes(max_tokens, H, F, E, top_k, _DT_EXPERT[kind])
+        sizes = max_tokens, H, F, E, top_k, _DT_EXPERT[kind]
+        need = lib().knj_moe_block_workspace_bytes(*sizes)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=bank.gate.device)
+        elif workspace.numel() < need:
+            need = lib().knj_moe_block_launch_workspace_bytes(*sizes)   # for run alone: decode checks its own need
         if workspace.dtype != torch.uint8 or workspace.numel() < need or workspace.data_ptr() % 256 or workspace.device != bank.gate.device or \
                 not workspace.is_contiguous():
             raise ValueError(f"workspace of {need} contiguous uint8 values on the block's device, 256-byte aligned, needed")
