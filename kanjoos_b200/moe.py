@@ -307,10 +307,15 @@ class FloatExpertBank:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.gate, self.up, self.down))
 
+    def _refuse_codes(self):
+        """Codes taken for values would lose their scales."""
+        for name in ("gate", "up", "down"):
+            if getattr(self, name).element_size() == 1 or getattr(self, name + "_scale") is not None:
+                raise ValueError(f"these experts ({name}) are codes already")
+
     def to_e4m3(self) -> "FloatExpertBank":
         """The same block with its experts as e4m3 codes under block scales."""
-        if self.gate.dtype == torch.int8:
-            raise ValueError("these experts are int8 codes already")
+        self._refuse_codes()
         parts = {}
         for name in ("gate", "up", "down"):
             parts[name], parts[name + "_scale"] = e4m3_blocks(getattr(self, name))
@@ -318,8 +323,7 @@ class FloatExpertBank:
 
     def to_int8(self) -> "FloatExpertBank":
         """The same block with its experts as int8 codes under a scale for each output channel."""
-        if self.gate_scale is not None:
-            raise ValueError("these experts are codes already")
+        self._refuse_codes()
         parts = {}
         for name in ("gate", "up", "down"):
             parts[name], parts[name + "_scale"] = int8_channels(getattr(self, name))
