@@ -54,7 +54,7 @@ constexpr int kScales = 80;
 constexpr int kMaxItems = 64;
 constexpr size_t kSyncAt = 128, kMaxAt = 256, kStatsAt = kMaxAt + kMaxTokens * kMaxK * 4,
                  kReadyAt = kStatsAt + 256, kHead = kReadyAt + kMaxExperts * 4;   // of the workspace
-constexpr float kDown = 0x1p-64f;
+constexpr float kDown = 0x1p-80f;   // of rows whose squares leave the range: those of 2^128 and their sum are in it then, those of the smallest such row (2^56) too
 
 enum Kind { kBf16 = 0, kBf16Many = 1, kF16 = 2, kE4 = 3, kS8 = 4 };   // kBf16Many: see launch_bf16
 
@@ -1079,23 +1079,38 @@ __global__ void __launch_bounds__(kThreads) moe_decode_front_kernel(const __grid
   float v = 0.f;
   if (lane < 2 + SIDE)
     for (int w = 0; w < kWarps; ++w) v = lane == 1 ? max_nan(v, part[w][i][1]) : v + part[w][i][lane];
-  const float tot = __shfl_sync(0xffffffffu, v, 0), m = __shfl_sync(0xffffffffu, v, 1);
-  float inv = 1.0f;
+  const float tot = __shfl_sync(0xffffffffu, v, 0);
+  float inv = 1.0f, scale = 1.0f;   // of the row's values; of the sums over it
   if (p.pre_w) {
-    if (tot > 3.402823466e38f) {   // squares of a large row left the range: from values * 2^-64, where eps does not count
-      float q = 0.f;
+    if (tot > 3.402823466e38f) {   // squares of a large row left the range, other sums may have: all from values * 2^-80, where eps does not count
+      float q = 0.f, d[SIDE], far = 0.f;
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) d[k] = 0.f;
       for (int c = lane; c < p.H; c += 32) {
-        const float f = load_as_f32(p.x, p.x_dtype, t * p.ldx + c) * kDown;
+        const float f = load_as_f32(p.x, p.x_dtype, t * p.ldx + c) * kDown, g = f * load_as_f32(p.pre_w, p.norm_dtype, c);
         q = fmaf(f, f, q);
+        far = max3_abs_nan(far, g, 0.f);
+#pragma unroll
+        for (int k = 0; k < SIDE; ++k) d[k] = fmaf(g, __uint_as_float((uint32_t)p.router[(int64_t)min(e0 + k, p.E - 1) * p.H + c] << 16), d[k]);
       }
-      inv = kDown * rsqrtf(warp_sum(q) * (1.0f / (float)p.H));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) far = max_nan(far, __shfl_xor_sync(0xffffffffu, far, o));
+      v = far;
+#pragma unroll
+      for (int k = 0; k < SIDE; ++k) {
+        const float sum = warp_sum(d[k]);
+        if (lane == 2 + k) v = sum;
+      }
+      scale = rsqrtf(warp_sum(q) * (1.0f / (float)p.H));
+      inv = kDown * scale;
     } else {
-      inv = inverse_rms(tot, p.H, p.eps);
+      inv = scale = inverse_rms(tot, p.H, p.eps);
     }
   }
+  const float m = __shfl_sync(0xffffffffu, v, 1);
   const int e = e0 + lane - 2;
-  if (lane >= 2 && lane < 2 + SIDE && e < p.E) p.logits[t * p.E + e] = v * inv + (p.router_bias ? p.router_bias[e] : 0.f);
-  if (e0 == 0 && lane == 0) p.stats[t] = make_float2(inv, m * inv);
+  if (lane >= 2 && lane < 2 + SIDE && e < p.E) p.logits[t * p.E + e] = v * scale + (p.router_bias ? p.router_bias[e] : 0.f);
+  if (e0 == 0 && lane == 0) p.stats[t] = make_float2(inv, m * scale);
 }
 
 template <int KIND>
