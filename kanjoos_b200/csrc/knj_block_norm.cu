@@ -41,8 +41,9 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 }
 
 // 1 / sqrt(mean square + eps) of a row whose sum of squares is `tot`. Where the squares of a large row leave the f32 range
-// they are summed once more from values * 2^-64 (`again`); eps does not count there.
-constexpr float kDown = 0x1p-64f;
+// they are summed once more from values * 2^-80 (`again`), of which the largest and the smallest such row's squares are in it; eps does not
+// count there.
+constexpr float kDown = 0x1p-80f;
 // rsqrtf is off by 2 units in the last place; an IEEE root and two divisions are a hundred instructions of every thread and row.
 template <class Again>
 __device__ __forceinline__ float rms_inverse(float tot, float inv_h, float eps, Again again) {
@@ -256,7 +257,7 @@ __global__ void __maxnreg__(!RING || NC == 4 ? 128 : NC == 1 ? 64 : Y == 0 ? 80 
       pre_of(c, pre[c]);
     }
   }
-  // sum of squares over the row, of values * 2^-64 where `down`; of(c, v): the run's values
+  // sum of squares over the row, of values * kDown where `down`; of(c, v): the run's values
   auto squares = [&](auto of, bool down) {
     float2 a = make_float2(0.f, 0.f), b = a;
 #pragma unroll
