@@ -129,7 +129,7 @@ void small_stack_destroy(SmallStack *st);
 // Blocks until the grids this launch depends on have completed and their writes are visible. A no-op for a plain launch.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next launch of the chain take its places while this grid still runs (once every block has called this or
-// exited). Only the decode layer's front and projection kernels do, grids of one block per SM or less. After a larger
+// exited). Only the decode layer's front and projection kernels, grids of one block per SM or less, and the int8 rows do. After a larger
 // grid the next one's blocks take what places are left and run worse from there than launched at its end: signalled by
 // the row normalisation, the router made a layer of 512 tokens 284 us long, not signalled 247; signalled by the down
 // GEMM, the combine cost 4 us at 100 tokens and 45 at 16384 (hidden 2048, 128 experts; hidden 1024, 32 experts at 16384
