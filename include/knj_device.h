@@ -654,7 +654,8 @@ int knj_moe_block_launch(const knj_moe_block_args *a, knj_stream_t s);
 #define KNJ_MOE_DECODE_MIN_SMS 64
 int knj_moe_block_decode_launch(const knj_moe_block_args *a, knj_stream_t s);
 /* Test hook of the calling thread: in its next decode launches 1 = the activations of no expert, 2 = the barrier over the grid is never
- * complete, so that a wait runs into its limit; 0 = off (default). */
+ * complete, so that a wait runs into its limit, 3 = a thread block has room for one expert's matrix rows in its plan, so that it gives up
+ * where it has two; 0 = off (default). */
 void knj_moe_block_decode_test_stall(int what);
 /* Outcome of the last launch with this argument block's status word (without one: of the last launch over its workspace, whichever
  * block's that was): waits for the stream, then KNJ_OK, or KNJ_E_TIMEOUT when a bounded wait of its norms or products gave up. */

@@ -92,7 +92,7 @@ struct DecodeParams {
   int x_vec;                    // rows of x are whole 16-byte units
   float alpha, beta, eps;
   long long wait_cycles;
-  int stall;                    // test hook: 1 = no expert's rows are ever ready, 2 = the barrier's target is out of reach
+  int stall;                    // test hook: 1 = no expert's rows are ever ready, 2 = the barrier's target is out of reach, 3 = plans have room for one item
 };
 thread_local int t_stall = 0;
 
@@ -831,13 +831,19 @@ __device__ __forceinline__ Border border(const DecodeParams &p, const Shared &s,
   const unsigned unit = (unsigned)__fdividef((float)(pos - s.cost[at] * half), (float)(s.cost[at + 1] - s.cost[at]));
   return Border{at, min(unit, half)};
 }
-// This CTA's items between two borders; an expert's tokens go through in passes of up to kMaxRows.
-__device__ __forceinline__ void make_plan(Plan &plan, const Shared &s, int N, int pass, int cap, Border from, Border to) {
+// This CTA's items between two borders; an expert's tokens go through in passes of up to kMaxRows. False where there are more items than room
+// for them (a device of KNJ_MOE_DECODE_MIN_SMS SMs comes to 32 of kMaxItems: a share of the cost and two experts at its borders).
+__device__ __forceinline__ bool make_plan(Plan &plan, const Shared &s, int N, int pass, int cap, Border from, Border to, int most_items) {
+  bool fits = true;
   int n = 0, panel = 0, held = 0, most = 0;
   for (int i = from.at; i <= to.at && i < s.n_active; ++i) {
     const unsigned begin = i == from.at ? from.unit : 0u, end = i == to.at ? to.unit : N / 2;
     const int e = s.active[i], rows = __popc(s.mask[e]);
-    for (int f = 0; begin < end && f < rows && n < kMaxItems; f += pass) {
+    for (int f = 0; begin < end && f < rows; f += pass) {
+      if (n == most_items) {
+        fits = false;
+        break;
+      }
       const int c = min(pass, rows - f);
       if (held + c > cap) {
         panel = n;
@@ -850,6 +856,7 @@ __device__ __forceinline__ void make_plan(Plan &plan, const Shared &s, int N, in
   }
   plan.n_items = n;
   plan.rows = most;
+  return fits;
 }
 
 // ---- stages 1 and 4 -----------------------------------------------------------------------------------------------------
@@ -1187,7 +1194,9 @@ __global__ void __launch_bounds__(kAll, 1) moe_decode_kernel(const __grid_consta
   if (warp < 2) {   // a warp for each product
     const int N = warp == 0 ? p.F : p.H, K = warp == 0 ? p.H : p.F;
     const Border from = border(p, s, N / 2, blockIdx.x), to = border(p, s, N / 2, blockIdx.x + 1);
-    if (lane == 0) make_plan(s.plan[warp], s, N, Geo<KIND>::pass(K), Geo<KIND>::cap(K), from, to);
+    // a plan that is not whole is a wait that gave up
+    if (lane == 0 && !make_plan(s.plan[warp], s, N, Geo<KIND>::pass(K), Geo<KIND>::cap(K), from, to, p.stall == 3 ? 1 : kMaxItems))
+      *reinterpret_cast<volatile int *>(&s.fail) = 1;
   }
   __syncthreads();
 
@@ -1317,4 +1326,4 @@ int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t
 }
 }  // namespace knj
 
-extern "C" void knj_moe_block_decode_test_stall(int what) { t_stall = what == 1 || what == 2 ? what : 0; }
+extern "C" void knj_moe_block_decode_test_stall(int what) { t_stall = what >= 1 && what <= 3 ? what : 0; }
