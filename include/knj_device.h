@@ -563,7 +563,8 @@ int knj_expert_gateup_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 int knj_expert_proj_launch(const knj_expert_gemm_args *a, knj_stream_t s);
 /* 1 = these products (and the dense e4m3 and int8 ones) always on single SMs (tcgen05 cta_group::1, buckets of up to 64 rows), 2 =
  * always on CTA pairs (buckets of up to 256), 3 = always with K split over the CTAs of a cluster, 0 (default) = by the sizes. (The
- * int8 product of up to four rows that are not codes yet is none of these, whatever is set.) Process-wide. */
+ * int8 product of few rows that are not codes yet, those for which knj_int8_matmul_workspace_bytes is 0, is none of these, whatever is
+ * set.) Process-wide. */
 void knj_expert_tc_form(int form);
 /* Test hook of the calling thread: in its next products 1 = the first accumulator of the first thread block, 2 = that block's first
  * operands, 3 = the first accumulator of the last thread block of its pair or cluster never count as complete, so that a wait runs
@@ -580,8 +581,8 @@ int knj_fp8_matmul_launch(const void *W, const float *W_scale, int n_in, int n_o
 
 /* Dense product with an int8 matrix: y[m][n_out] = f32(sum_k x[m][k] W[n_out][k]) * (x_scale[m] * W_scale[n_out]), W int8
  * [n_out][n_in], W_scale f32 [n_out], the sums exact in 32-bit whole numbers. Rows of x in f32, bf16 or f16 (x_scale not read) are
- * turned into codes first, as knj_int8_rows_launch does, in the workspace (256-byte aligned; knj_int8_matmul_workspace_bytes is 0 for up
- * to four rows, whose codes the product's kernel forms itself); int8 rows (16-byte units) come with their x_scale [m] and need no
+ * turned into codes first, as knj_int8_rows_launch does, in the workspace (256-byte aligned; knj_int8_matmul_workspace_bytes says how much:
+ * none for one row of up to 40960 values, two of 20480, three or four of 10240, whose codes the product's kernel forms itself); int8 rows (16-byte units) come with their x_scale [m] and need no
  * workspace. n_in a multiple of 16 below KNJ_INT8_MAX_K. y f32, bf16 or f16. status as in knj_expert_gemm_args. The reference's int8
  * product (kernels/knj_kernels.hip:132-318 knj_gemm_w4_i8) has 4-bit weights. */
 typedef struct {

@@ -103,11 +103,11 @@ int block_norm_check(const knj_block_norm_args *a);
 // What knj_expert_gateup_launch and knj_expert_proj_launch check of theirs, but for the number of tiles.
 int expert_product_check(const knj_expert_gemm_args *a, bool gateup, const char *who);
 
-// The MoE block in one launch (knj_moe_decode.cu), its arguments checked but for what concerns this form alone; and its scratch.
 // The int8 product of few rows (knj_int8.cu), and whether m rows of K values are that
 bool int8_few(int m, int K);
 int int8_few_launch(const void *W, const float *ws, int K, int N, const void *x, int dtype, int64_t ldx, int m, void *y, int y_dtype, int64_t ldy,
                     cudaStream_t st);
+// The MoE block of a decode step in two kernels (knj_moe_decode.cu), its arguments checked but for what concerns this form alone; and its scratch.
 int moe_decode_launch(const knj_moe_block_args *a, int32_t *status, knj_stream_t s);
 size_t moe_decode_workspace(int T, int H, int F, int E, int k);
 

@@ -21,8 +21,8 @@
 //   scales     e4m3: the rows' and the matrix blocks' scales, four blocks of K to a group, by asynchronous copies; 16 bits and int8:
 //              finds the tiles and their rows (and the rows' scales) in the tables, a tile ahead (in e4m3 the matrix warp does)
 // In 16 bits and int8 the tensor core adds over all of K. int8 leaves the 16-bit form as it is, but that a slab holds twice the K and
-// the epilogue turns sums into f32 and scales them: 8192 x 4096 x 4096 84 us alone (3.3 P operations a second; the
-// library's product of 8192^3 reaches 2.95). In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
+// the epilogue turns sums into f32 and scales them: 8192 x 4096 x 4096 88 us by itself (3.13 P operations a second), 94 ten in a row, 103
+// in a loop under the power limit (the library's product of 8192^3 reached 2.95 P). In e4m3 each block of K is one accumulator buffer, which the epilogue scales and
 // adds to its registers in f32 while the tensor core fills the others.
 //
 // Every wait on an mbarrier is bounded (knj_decode_wait_limit); on give-up the kernel raises a status flag, stores NaN in place of the
